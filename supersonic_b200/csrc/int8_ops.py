@@ -10,7 +10,7 @@ The modelled project's 8-bit lanes: an int8/int4 tiered cache (kernels/certified
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Tuple
 
 import torch
@@ -29,7 +29,8 @@ _SIGNATURES = {
     "ssb_int8_attention_plain": ("int8_attention", [_P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I,
                                                     _I, _I, _I, _I, _I, _F, _P]),
     "ssb_int8_quantize_rows": ("int8_linear", [_P, _I, _I, _P, _I, _P, _I, _I, _P]),
-    "ssb_int8_product": ("int8_linear", [_P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "ssb_int8_linear": ("int8_linear", [_P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "ssb_int8_linear_scratch": ("int8_linear", [_I, _I, _I]),
 }
 _functions = {}
 
@@ -41,7 +42,7 @@ def _fn(name: str):
     if f is None:
         library, types = _SIGNATURES[name]
         f = getattr(load_library(library), name)
-        f.restype, f.argtypes = c_int, types
+        f.restype, f.argtypes = c_longlong if name.endswith("_scratch") else c_int, types
         _functions[name] = f
     return f
 
@@ -233,9 +234,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, ou
         raise KernelError("linear: results are added in float32 only")
     if rows == 0 or n == 0:
         return
-    scratch = torch.empty(rows * (k + 4), dtype=torch.int8, device=x.device)          # codes, then a float32 scale a row
-    codes, scales = scratch.data_ptr(), scratch.data_ptr() + rows * k
-    stream = _stream()
-    _check(_fn("ssb_int8_quantize_rows")(x_at, ldx, _CODES[x.dtype], codes, k, scales, rows, k, stream), "int8_quantize_rows")
-    _check(_fn("ssb_int8_product")(codes, k, scales, weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), o_at, ldo,
-                                   _CODES[out.dtype], rows, n, k, 1 if accumulate else 0, stream), "int8_product")
+    scratch = torch.empty(_fn("ssb_int8_linear_scratch")(rows, n, k), dtype=torch.int8, device=x.device)
+    ops.note_bounded_wait_launches(1)
+    _check(_fn("ssb_int8_linear")(x_at, ldx, _CODES[x.dtype], weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), o_at, ldo,
+                                  _CODES[out.dtype], rows, n, k, 1 if accumulate else 0, scratch.data_ptr(),
+                                  ops.tc_error_word(x.device).data_ptr(), _stream()), "int8_linear")

@@ -389,3 +389,20 @@ def test_linear_is_the_same_in_every_run_and_batch():
         part = torch.zeros((rows, 384), device=DEV)
         int8_ops.linear(x[:rows], w, sw, part)
         assert torch.equal(part, whole[:rows]), rows
+
+
+@pytest.mark.parametrize("rows", [2, 100, 2000])
+def test_linear_on_a_side_stream_and_no_wait_runs_out(rows):
+    from supersonic_b200.csrc import int8_ops, ops
+    x, w = torch.randn((rows, 640), device=DEV), torch.randint(-127, 128, (2064, 640), dtype=torch.int8, device=DEV)
+    sw = torch.rand(2064, device=DEV)
+    want, got = torch.zeros((rows, 2064), device=DEV), torch.zeros((rows, 2064), device=DEV)
+    int8_ops.linear(x, w, sw, want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            int8_ops.linear(x, w, sw, got)
+    side.synchronize()
+    ops.check_device_errors()
+    assert torch.equal(got, want)
