@@ -4,7 +4,11 @@
 // with codes kc, vc and their blocks' scales ks, vs.  The rows that keep account add exp(s_ij - lse_i), summed over the query
 // heads of a kv head, to the weight of key j.
 #include "common.cuh"
+#include "tc_helpers.cuh"
+#include <cuda_fp16.h>
 #include <math.h>
+#include <algorithm>
+#include <type_traits>
 
 typedef __nv_bfloat16 bf16;
 
@@ -27,6 +31,7 @@ struct IaArgs {
     float scale;
 };
 
+// ---- head sizes other than 64 and 128, and more than 32 query heads a kv head -------------------------------------------
 // Any head size that is a multiple of 16 up to 256: a warp a row and query head, words of four codes over its lanes.
 template <typename T>
 __global__ void __launch_bounds__(128)
@@ -126,27 +131,853 @@ int8_weigh_plain_kernel(const IaArgs a) {
     }
 }
 
-SSB_API int ssb_int8_attention_plain(const void* q, int ldq, int dtype, void* out, int ldo, float* lse, const void* k, const void* v,
-                                     const float* k_scale, const float* v_scale, float* weight, const int* page_table, int n_slots,
-                                     int max_pages, int n_pages, const int* cu_new, const int* seq_start, const int* seq_slot,
-                                     int n_seqs, int rows, int n_q, int n_kv, int head_dim, int block, int window, int weigh_last,
-                                     float scale, cudaStream_t stream) {
+// ---- tensor cores, a page at a time ---------------------------------------------------------------------------------
+// Rows of a step that share a kv head (the query heads of its group, and up to ``tt`` neighbouring tokens) are the columns of
+// m16n8k16 products of float16: S^T = K Q^T with the 16 keys of a warp as rows, O^T = V^T P^T.  Codes are whole numbers up to 127,
+// so float16 holds them exactly; a query's column is taken times the power of two that brings its largest element to 256 .. 512,
+// which loses nothing of a bfloat16, and a float32 one goes in two halves of 11 bits each (WIDE), as do its probabilities.  The
+// scales stay outside the products: a key's goes onto the score; a value's, f * 2^x, into the exponent (x) and onto the
+// probability (f), with the running maximum taken over score + x, so that float16 holds what is summed whatever the scales are.
+// The maximum is rounded up to a whole number, in the log2 domain: taking x and it off a score then costs no bits.
+//
+// Codes become float16 in registers: 1024 + (code + 128) is a float16 whose low byte is the code with its sign bit turned, so four
+// codes take one exclusive-or, two byte permutations and two subtractions.  Which key is which row of the products, and which
+// dims its k-steps, is free as long as both operands agree: chosen so that every lane reads whole 16-byte pieces of a row, keys
+// {0, 4, 1, 5, 2, 6, 3, 7} on rows 0 .. 7, with no two lanes of a quarter-warp in one bank (head size 128).
+//
+// The launch's work is its pages: tiles of rows x pages that they see, dealt out evenly over the blocks wherever a tile ends (a
+// block finds its range from the batch's integers alone).  A tile that lies in one block's range is finished there; pieces of
+// others go to scratch, and int8_finish_kernel puts them together in the order of the keys.  Nothing is left from one launch
+// to the next.
+constexpr int IR_THREADS = 128, IR_WARPS = 4, IR_SEQS = 1024, IR_STAGES = 4;
+constexpr int IR_SIDE = 12;                  // beside a stage's page: its scales of keys and of values, and its id
+constexpr int IR_LEAST_X = -80, IR_MOST_X = 120;
+
+struct IrSeq { int row0, n_new, start, slot; };
+
+// What the dealing needs: tokens a tile (1 << tts), the window, and the batch with the units before each sequence.
+struct IrBatch {
+    const IrSeq* seqs;
+    const long long* cum;                // [n_seqs + 1]
+    int n_seqs, n_kv, tts, window;
+    bool one_tile;                       // a sequence's rows are one tile, however many
+
+    // sum over i < t of floor(max(0, a + i * 2^tts) / 64)
+    __device__ long long floors(long long t, long long a) const {
+        if (a < 0) {
+            const long long skip = min(t, (-a + (1 << tts) - 1) >> tts);
+            t -= skip;
+            a += skip << tts;
+            if (a < 0) return 0;
+        }
+        const int gs = 6 - tts;
+        auto ramp = [&](long long m) { const long long q = m >> gs; return (q * (q - 1) / 2 << gs) + q * (m & ((1 << gs) - 1)); };
+        const long long r0 = (a & 63) >> tts;
+        return (a >> 6) * t + ramp(r0 + t) - ramp(r0);
+    }
+    __device__ int tiles(const IrSeq& s) const { return s.slot < 0 || s.n_new <= 0 ? 0 : one_tile ? 1 : (s.n_new + (1 << tts) - 1) >> tts; }
+    // pages that the first t tiles of a sequence see, tile by tile
+    __device__ long long pages_before(const IrSeq& s, long long t) const {
+        if (one_tile) return t * (((s.start + s.n_new - 1) >> 6) - first_page(s, 0) + 1);
+        return t + floors(t, (long long)s.start + (1 << tts) - 1) - (window > 0 ? floors(t, (long long)s.start - window + 1) : 0);
+    }
+    __device__ int first_page(const IrSeq& s, int tile) const {
+        const long long lo = (long long)s.start + ((long long)tile << tts) - window + 1;
+        return window > 0 && lo > 0 ? (int)(lo >> 6) : 0;
+    }
+};
+
+// A run of pages of one tile and kv head: what of it lies in a block's range.
+struct IrSegment {
+    int b, kvh, tile, page, n;           // pages page .. page + n - 1 of the sequence
+    long long first, units;              // the tile's units
+    __device__ bool whole() const { return n == units; }
+};
+
+__device__ __forceinline__ IrSegment ir_locate(const IrBatch& B, long long u, long long end) {
+    int lo = 0, hi = B.n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (B.cum[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    const IrSeq s = B.seqs[lo];
+    IrSegment g;
+    g.b = lo;
+    const int tiles = B.tiles(s);
+    const long long per = (B.cum[lo + 1] - B.cum[lo]) / B.n_kv;
+    long long r = u - B.cum[lo];
+    g.kvh = (int)(r / per);
+    r -= g.kvh * per;
+    int t0 = 0, t1 = tiles - 1;          // the last tile that begins at or before the unit
+    while (t0 < t1) {
+        const int mid = (t0 + t1 + 1) >> 1;
+        if (B.pages_before(s, mid) <= r) t0 = mid; else t1 = mid - 1;
+    }
+    const long long before = B.pages_before(s, t0);
+    g.tile = t0;
+    g.units = B.pages_before(s, t0 + 1) - before;
+    g.first = u - (r - before);
+    g.page = B.first_page(s, t0) + (int)(r - before);
+    g.n = (int)min(g.first + g.units - u, end - u);
+    return g;
+}
+
+// Reads the batch and sums its units up; every thread of the block gets the total.
+__device__ __forceinline__ long long ir_read_batch(const IaArgs& a, int s0, int n_seqs, IrBatch& B, IrSeq* seqs, long long* cum,
+                                                   long long* warp_total, int last = 0) {
+    for (int b = threadIdx.x; b < n_seqs; b += IR_THREADS) {
+        const int row0 = a.cu_new[s0 + b], slot = a.seq_slot[s0 + b];
+        const int n_new = a.cu_new[s0 + b + 1] - row0, start = a.seq_start[s0 + b];
+        const int skip = last > 0 && n_new > last ? n_new - last : 0;        // with ``last``, that many last rows only
+        seqs[b] = IrSeq{row0 + skip, n_new - skip, start + skip, slot < a.n_slots && start >= 0 ? slot : -1};
+    }
+    __syncthreads();
+    const int per = (n_seqs + IR_THREADS - 1) / IR_THREADS, b0 = (int)threadIdx.x * per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto units_of = [&](int b) { return b < n_seqs ? B.pages_before(seqs[b], B.tiles(seqs[b])) * B.n_kv : 0LL; };
+    long long local = 0;
+    for (int i = 0; i < per; ++i) local += units_of(b0 + i);
+    long long incl = local;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_total[warp] = incl;
+    __syncthreads();
+    long long base = 0, total = 0;
+    for (int w = 0; w < IR_WARPS; ++w) {
+        if (w < warp) base += warp_total[w];
+        total += warp_total[w];
+    }
+    long long running = base + incl - local;
+    for (int i = 0; i < per; ++i)
+        if (b0 + i < n_seqs) { cum[b0 + i] = running; running += units_of(b0 + i); }
+    if (threadIdx.x == 0) cum[n_seqs] = total;
+    __syncthreads();
+    B.seqs = seqs;
+    B.cum = cum;
+    B.n_seqs = n_seqs;
+    return total;
+}
+// Where block c's units begin; no more blocks are dealt to than there are units, so that none of those is left without.
+__device__ __forceinline__ long long ir_begin(long long total, int c, int blocks) { return total * min(c, blocks) / blocks; }
+__device__ __forceinline__ int ir_dealt(long long total) { return (int)max(1LL, min((long long)gridDim.x, total)); }
+__device__ __forceinline__ int ir_owner(long long unit, long long total, int blocks) { return (int)(((unit + 1) * blocks - 1) / total); }
+
+__device__ __forceinline__ float ir_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ir_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t ir_transpose8(uint32_t v) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+__device__ __forceinline__ uint32_t ir_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The bytes of ``w`` that ``sel`` puts into the low byte of each half (codes with their sign bit turned), as float16 codes.
+__device__ __forceinline__ uint32_t ir_codes(uint32_t w, uint32_t sel) {
+    const uint32_t v = __byte_perm(w, 0x64646464u, sel);
+    const uint32_t bias = 0x64806480u;                            // 1024 + 128
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Byte offset of 16-byte piece c of row r of a page tile as the TMA unit leaves it (rows of 128 or 64 bytes with the swizzle of
+// that width).
+template <int HD> __device__ __forceinline__ uint32_t ir_at(int r, int c) {
+    return HD == 128 ? (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)) : (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ int ir_key_of(int g) { return (g >> 1) + 4 * (g & 1); }       // row g's key; row g + 8's is 8 further
+
+// S^T of a warp's 16 keys: rows ir_key_of(g) (+ 8), columns 2 t, 2 t + 1 of every tile of 8.
+template <int HD, int NT, bool WIDE>
+__device__ __forceinline__ void ir_scores(const unsigned char* keys, const uint32_t* qs, int warp, int lane, float (&s)[NT][4]) {
+    const int g = lane >> 2, t = lane & 3, r0 = 16 * warp + ir_key_of(g), r1 = r0 + 8;
+    constexpr int STEPS = HD / 16;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+#pragma unroll
+    for (int h = 0; h < HD / 64; ++h) {
+        const uint4 k0 = *reinterpret_cast<const uint4*>(keys + ir_at<HD>(r0, 4 * h + t));
+        const uint4 k1 = *reinterpret_cast<const uint4*>(keys + ir_at<HD>(r1, 4 * h + t));
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t u0 = w0[e] ^ 0x80808080u, u1 = w1[e] ^ 0x80808080u;
+            const uint32_t a0 = ir_codes(u0, 0x4140), a2 = ir_codes(u0, 0x4342), a1 = ir_codes(u1, 0x4140), a3 = ir_codes(u1, 0x4342);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int at = (i * STEPS + 4 * h + e) * 32 + lane;
+                if (WIDE) {
+                    const uint4 q = reinterpret_cast<const uint4*>(qs)[at];
+                    ir_mma(s[i], a0, a1, a2, a3, q.z, q.w);      // the low halves first
+                    ir_mma(s[i], a0, a1, a2, a3, q.x, q.y);
+                } else {
+                    const uint2 q = reinterpret_cast<const uint2*>(qs)[at];
+                    ir_mma(s[i], a0, a1, a2, a3, q.x, q.y);
+                }
+            }
+        }
+    }
+}
+
+// Query columns c0 .. c0 + 8 NT - 1 of a (sequence, kv head) as fragments of the products' B operand, and each column's factor
+// (scale * log2 e over its power of two).  Column c: token c / group of the tile, head c % group.
+template <int HD, int NT, bool WIDE>
+__device__ __forceinline__ void ir_queries(const IaArgs& a, int row0, int n_tokens, int kvh, int c0, uint32_t* qs, float* qf) {
+    using T = typename std::conditional<WIDE, float, bf16>::type;
+    constexpr int LANES = HD / 8, STEPS = HD / 16;               // lanes a column, 8 elements each
+    const int group = a.n_q / a.n_kv, l = threadIdx.x % LANES;
+#pragma unroll
+    for (int pass = 0; pass < (8 * NT * LANES + IR_THREADS - 1) / IR_THREADS; ++pass) {
+        const int col = pass * (IR_THREADS / LANES) + threadIdx.x / LANES, c = c0 + col, token = c / group;
+        float x[8] = {};
+        if (col < 8 * NT && token < n_tokens) {
+            const T* src = (const T*)a.q + (size_t)(row0 + token) * a.ldq + (size_t)(kvh * group + c % group) * HD + 8 * l;
+            if constexpr (WIDE) {
+                const float4 u = reinterpret_cast<const float4*>(src)[0], v = reinterpret_cast<const float4*>(src)[1];
+                x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+            } else {
+                const uint4 v = *reinterpret_cast<const uint4*>(src);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+            }
+        }
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // 2^up brings the largest element to 256 .. 512
+        const int up = most > 0.f ? min(8 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
+        const float times = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
+        if (col < 8 * NT) {
+            const int piece = l >> 1, lane = (col & 7) * 4 + (piece & 3);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {                        // four elements: one k-step of this lane
+                const int step = 4 * (piece >> 2) + 2 * (l & 1) + w, at = ((col >> 3) * STEPS + step) * 32 + lane;
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = x[4 * w + i] * times;
+                const uint32_t h0 = ir_half2(y[0], y[1]), h1 = ir_half2(y[2], y[3]);
+                if constexpr (WIDE) {
+                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                    reinterpret_cast<uint4*>(qs)[at] = make_uint4(h0, h1, ir_half2(y[0] - f0.x, y[1] - f0.y), ir_half2(y[2] - f1.x, y[3] - f1.y));
+                } else {
+                    reinterpret_cast<uint2*>(qs)[at] = make_uint2(h0, h1);
+                }
+            }
+            if (l == 0) qf[col] = a.scale * 1.4426950408889634f * back;
+        }
+    }
+}
+
+// Pages on their way into the ring: warp 0 asks for them, up to IR_STAGES - 1 ahead of the warps that work.
+template <int HD, bool VALUES> constexpr int ir_stage_bytes() { return (VALUES ? 2 : 1) * 64 * HD; }
+
+struct IrFeed {
+    IrSegment seg;
+    long long next, end;                 // the unit to be asked for next
+    int left, ids, ids_from, issued;     // pages of the segment not yet asked for; page ids of 32 pages, one a lane
+};
+
+template <int HD, bool VALUES>
+__device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFeed& f, unsigned char* stages, float* scales, uint32_t full0,
+                                        uint32_t empty0, const CUtensorMap& map_k, const CUtensorMap& map_v, volatile int* abort_flag) {
+    const int lane = threadIdx.x & 31, per = 64 / a.block;
+    if (f.left == 0) {
+        f.seg = ir_locate(B, f.next, f.end);
+        f.left = f.seg.n;
+        f.ids_from = -1;
+    }
+    const IrSeq s = B.seqs[f.seg.b];
+    const int i = f.seg.n - f.left;
+    if (f.ids_from < 0 || i - f.ids_from >= 32) {
+        // a tile that is not full may count a page behind the sequence's last: the last again, which no row of it sees
+        const int page = min(min(f.seg.page + i + lane, (s.start + s.n_new - 1) >> 6), a.max_pages - 1);
+        f.ids = min(max(a.page_table[(size_t)s.slot * a.max_pages + page], 0), a.n_pages - 1);
+        f.ids_from = i;
+    }
+    const int id = __shfl_sync(0xffffffffu, f.ids, i - f.ids_from);
+    const int st = f.issued % IR_STAGES;
+    bool ok = true;
+    if (lane == 0) ok = mbar_wait(empty0 + 8 * st, ((f.issued / IR_STAGES) & 1) ^ 1, abort_flag);
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    if (!ok) return false;
+    const size_t head = (size_t)id * a.n_kv + f.seg.kvh;
+    if (lane < 2 * per) {
+        const float* src = (lane < per ? a.k_scale : a.v_scale) + head * per + lane % per;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(scales + IR_SIDE * st + lane)), "l"(src) : "memory");
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full0 + 8 * st) : "memory");
+    if (lane == 0) {
+        scales[IR_SIDE * st + 8] = __int_as_float(id);            // before this lane's arrival at the barrier, below
+        const uint32_t dst = smem_u32(stages + st * ir_stage_bytes<HD, VALUES>());
+        mbar_expect_tx(full0 + 8 * st, ir_stage_bytes<HD, VALUES>());
+        tma_load_2d(dst, &map_k, full0 + 8 * st, 0, (int)(head * 64));
+        if (VALUES) tma_load_2d(dst + 64 * HD, &map_v, full0 + 8 * st, 0, (int)(head * 64));
+    }
+    ++f.issued;
+    ++f.next;
+    --f.left;
+    return true;
+}
+
+template <int HD, int NT> constexpr int ir_acc_ld() { return HD + 4; }
+template <int HD, int NT, bool WIDE> constexpr size_t ir_smem(int n_seqs) {
+    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, true>() + IR_WARPS * 8 * NT * ir_acc_ld<HD, NT>() * 4 +
+           (size_t)NT * (HD / 16) * 32 * (WIDE ? 16 : 8) + IR_STAGES * 48 + 2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IrSeq) + 8) + 8;
+}
+// floats of a piece: a column's sums, its maximum and its sum of weights
+template <int HD, int NT> constexpr int ir_piece() { return 8 * NT * (HD + 2); }
+
+template <typename T> __device__ __forceinline__ void ir_store4(T* p, float4 v);
+template <> __device__ __forceinline__ void ir_store4<float>(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+template <> __device__ __forceinline__ void ir_store4<bf16>(bf16* p, float4 v) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+// What a column's result is written as.
+template <int HD, bool WIDE>
+__device__ __forceinline__ void ir_put(const IaArgs& a, const IrSeq& s, int tile, int tts, int kvh, int col, int d, float4 o, float m, float l, float offset) {
+    using T = typename std::conditional<WIDE, float, bf16>::type;
+    const int group = a.n_q / a.n_kv, token = (tile << tts) + col / group, head = kvh * group + col % group;
+    if (col / group >= (1 << tts) || token >= s.n_new) return;
+    const size_t row = (size_t)(s.row0 + token);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    ir_store4<T>((T*)a.out + row * a.ldo + (size_t)head * HD + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (d == 0 && a.lse) a.lse[row * a.n_q + head] = l > 0.f ? (m - offset + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <int HD, int NT, bool WIDE>
+__global__ void __launch_bounds__(IR_THREADS)
+int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict__ pieces, int* __restrict__ error_word,
+                 const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    // probabilities are summed times 2^OFFSET and may exceed that by 2^LAZY before the reference maximum is moved; with f below 2
+    // and both in float16, 2^(OFFSET + LAZY + 1) stays below 2^16
+    constexpr float OFFSET = WIDE ? 13.f : 6.f, LAZY = WIDE ? 1.f : 8.f;
+    constexpr int C = 8 * NT, ACC_LD = ir_acc_ld<HD, NT>(), TILES = HD / 16;
+    using T = typename std::conditional<WIDE, float, bf16>::type;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* stages = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* acc = (float*)(stages + IR_STAGES * ir_stage_bytes<HD, true>());       // [warp][column][ACC_LD]
+    uint32_t* qs = (uint32_t*)(acc + IR_WARPS * C * ACC_LD);
+    float* scales = (float*)(qs + NT * (HD / 16) * 32 * (WIDE ? 4 : 2));          // [stage][keys' | values' | page id]
+    uint64_t* bars = (uint64_t*)(scales + IR_STAGES * IR_SIDE);                         // full, empty
+    long long* cum = (long long*)(bars + 2 * IR_STAGES);
+    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    __shared__ float warp_m[IR_WARPS][C], warp_l[IR_WARPS][C], qf[C];
+    __shared__ long long warp_total[IR_WARPS];
+    __shared__ int sm_abort[2];
+    volatile int* abort_flag = sm_abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + IR_STAGES);
+    ssb_pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < IR_STAGES; ++i) { mbar_init(full0 + 8 * i, 33); mbar_init(empty0 + 8 * i, IR_WARPS); }
+        abort_flag[0] = 0;
+        abort_flag[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false};
+    const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
+    const int blocks = ir_dealt(total);
+    const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
+    const int group = a.n_q / a.n_kv;
+
+    // sequences without a slot: zeros
+    for (int b = blockIdx.x; b < n_seqs; b += gridDim.x)
+        if (seqs[b].slot < 0)
+            for (int e = threadIdx.x; e < seqs[b].n_new * a.n_q * (HD / 4); e += IR_THREADS) {
+                const int d = e % (HD / 4) * 4, head = e / (HD / 4) % a.n_q;
+                const size_t row = (size_t)(seqs[b].row0 + e / (HD / 4) / a.n_q);
+                ir_store4<T>((T*)a.out + row * a.ldo + (size_t)head * HD + d, make_float4(0.f, 0.f, 0.f, 0.f));
+                if (d == 0 && a.lse) a.lse[row * a.n_q + head] = -INFINITY;
+            }
+
+    IrFeed feed{};
+    feed.next = begin;
+    feed.end = end;
+    bool ok = true;
+    if (warp == 0)
+        while (ok && feed.next < end && feed.issued < IR_STAGES - 1)
+            ok = ir_feed<HD, true>(a, B, feed, stages, scales, full0, empty0, map_k, map_v, abort_flag);
+    int done = 0;                                                  // pages worked on
+    for (long long u = begin; u < end;) {
+        const IrSegment seg = ir_locate(B, u, end);
+        const IrSeq s = seqs[seg.b];
+        const int token0 = seg.tile << tts, n_tokens = min(1 << tts, s.n_new - token0);
+        ir_queries<HD, NT, WIDE>(a, s.row0 + token0, n_tokens, seg.kvh, 0, qs, qf);
+        __syncthreads();
+        // a column's last and first visible key, and those that all columns see
+        int hi[NT][2], lo[NT][2];
+        float m[NT][2], l[NT][2], factor[NT][2], o[TILES][NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = 8 * i + 2 * t + e, token = c / group;
+                hi[i][e] = token < n_tokens ? s.start + token0 + token : -1;
+                lo[i][e] = a.window > 0 ? hi[i][e] - a.window + 1 : 0;
+                m[i][e] = -INFINITY;
+                l[i][e] = 0.f;
+                factor[i][e] = qf[c];
+            }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
+        const int all_hi = s.start + token0, all_lo = a.window > 0 ? s.start + token0 + n_tokens - a.window : 0;
+        for (int p = 0; p < seg.n; ++p, ++done) {
+            if (warp == 0 && ok && feed.next < end)
+                ok = ir_feed<HD, true>(a, B, feed, stages, scales, full0, empty0, map_k, map_v, abort_flag);
+            const int st = done % IR_STAGES;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * st, (done / IR_STAGES) & 1, abort_flag));
+            if (!ok) {                                             // give up, but meet the others at the segment's end
+                if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
+                continue;
+            }
+            const unsigned char* keys = stages + st * ir_stage_bytes<HD, true>();
+            const unsigned char* values = keys + 64 * HD;
+            const int key0 = (seg.page + p) * 64 + 16 * warp, per = 64 / a.block;
+            const float ks = scales[IR_SIDE * st + 16 * warp / a.block], vs = scales[IR_SIDE * st + per + 16 * warp / a.block];
+            float sc[NT][4];
+            ir_scores<HD, NT, WIDE>(keys, qs, warp, lane, sc);
+            // vs = f 2^x; what is no scale belongs to keys that nobody sees
+            const int x = min(max((int)(__float_as_uint(vs) >> 23 & 255) - 127, IR_LEAST_X), IR_MOST_X);
+            const float fx = (float)x, down = __uint_as_float((uint32_t)(127 - x) << 23), f = fabsf(vs) < 3e38f ? vs * down : 0.f;
+            const bool inside = key0 >= all_lo && key0 + 15 <= all_hi;
+            float worst = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = key0 + ir_key_of(g) + (e >> 1) * 8;
+                    sc[i][e] *= factor[i][e & 1] * ks;
+                    if (!inside && (key > hi[i][e & 1] || key < lo[i][e & 1])) sc[i][e] = -INFINITY;
+                    worst = fmaxf(worst, sc[i][e] - (m[i][e & 1] - fx));     // -inf - -inf: no number, which fmaxf passes over
+                }
+            if (__any_sync(0xffffffffu, worst > LAZY)) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(sc[i][e], sc[i][e + 2]) + fx;
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const float now = fmaxf(m[i][e], ceilf(top)), alpha = m[i][e] == -INFINITY ? 0.f : ir_ex2(m[i][e] - now);
+                        m[i][e] = now;
+                        l[i][e] *= alpha;
+#pragma unroll
+                        for (int k = 0; k < TILES; ++k) { o[k][i][e] *= alpha; o[k][i][e + 2] *= alpha; }
+                    }
+            }
+            uint32_t p_hi[NT][2], p_lo[NT][2];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float ref = m[i][e & 1] == -INFINITY ? 0.f : m[i][e & 1] - fx - OFFSET;
+                    v[e] = ir_ex2(sc[i][e] - ref);
+                }
+                l[i][0] = fmaf(v[0] + v[2], down, l[i][0]);
+                l[i][1] = fmaf(v[1] + v[3], down, l[i][1]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float v0 = v[2 * h] * f, v1 = v[2 * h + 1] * f;
+                    const uint32_t top = ir_half2(v0, v1);
+                    p_hi[i][h] = ir_transpose8(top);
+                    if (WIDE) {
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&top));
+                        p_lo[i][h] = ir_transpose8(ir_half2(v0 - r.x, v1 - r.y));
+                    }
+                }
+            }
+            // values of keys t, t + 4, t + 8, t + 12 of the warp: HD / 8 dims of this lane each
+            constexpr int WORDS = HD / 32;
+            uint32_t vw[4][WORDS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 16 * warp + t + 4 * j;
+                if (HD == 128) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(values + ir_at<HD>(r, g));
+                    vw[j][0] = c.x; vw[j][1] = c.y; vw[j][WORDS - 2] = c.z; vw[j][WORDS - 1] = c.w;
+                } else {
+                    const uint2 c = *reinterpret_cast<const uint2*>(values + ir_at<HD>(r, g >> 1) + 8 * (g & 1));
+                    vw[j][0] = c.x; vw[j][1] = c.y;
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+                const uint32_t u0 = vw[0][w] ^ 0x80808080u, u1 = vw[1][w] ^ 0x80808080u, u2 = vw[2][w] ^ 0x80808080u, u3 = vw[3][w] ^ 0x80808080u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {                      // two of the word's four dims: one tile of the products
+                    const uint32_t lo2 = __byte_perm(u0, u1, h ? 0x7362 : 0x5140), hi2 = __byte_perm(u2, u3, h ? 0x7362 : 0x5140);
+                    const uint32_t a0 = ir_codes(lo2, 0x4140), a1 = ir_codes(lo2, 0x4342), a2 = ir_codes(hi2, 0x4140), a3 = ir_codes(hi2, 0x4342);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        if (WIDE) ir_mma(o[2 * w + h][i], a0, a1, a2, a3, p_lo[i][0], p_lo[i][1]);
+                        ir_mma(o[2 * w + h][i], a0, a1, a2, a3, p_hi[i][0], p_hi[i][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty0 + 8 * st) : "memory");
+        }
+        // the warps' parts: a column's sums, maximum and sum of weights
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], d);
+                const int c = 8 * i + 2 * t + e;
+                if (g == 0) { warp_m[warp][c] = m[i][e]; warp_l[warp][c] = l[i][e]; }
+#pragma unroll
+                for (int k = 0; k < TILES; ++k)                    // dims 16 g + 2 k, + 1 (head size 64: 8 g + 2 k, + 1)
+                    *reinterpret_cast<float2*>(acc + (warp * C + c) * ACC_LD + (HD / 8) * g + 2 * k) = make_float2(o[k][i][e], o[k][i][e + 2]);
+            }
+        __syncthreads();
+        const bool whole = seg.whole();
+        float* piece = pieces + (size_t)(2 * blockIdx.x + (seg.first >= begin)) * ir_piece<HD, NT>();
+        for (int e = threadIdx.x; e < C * (HD / 4); e += IR_THREADS) {
+            const int c = e / (HD / 4), d = e % (HD / 4) * 4;
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < IR_WARPS; ++w) top = fmaxf(top, warp_m[w][c]);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < IR_WARPS; ++w) {
+                const float by = warp_m[w][c] == -INFINITY ? 0.f : ir_ex2(warp_m[w][c] - top);
+                const float4 y = *reinterpret_cast<const float4*>(acc + (w * C + c) * ACC_LD + d);
+                v.x = fmaf(y.x, by, v.x); v.y = fmaf(y.y, by, v.y); v.z = fmaf(y.z, by, v.z); v.w = fmaf(y.w, by, v.w);
+                sum = fmaf(warp_l[w][c], by, sum);
+            }
+            if (whole) {
+                ir_put<HD, WIDE>(a, s, seg.tile, tts, seg.kvh, c, d, v, top, sum, OFFSET);
+            } else {
+                *reinterpret_cast<float4*>(piece + c * HD + d) = v;
+                if (d == 0) { piece[C * HD + c] = top; piece[C * HD + C + c] = sum; }
+            }
+        }
+        u += seg.n;
+    }
+    if (!ok && warp == 0)                                          // let issued copies land before the block ends
+        for (int i = max(0, feed.issued - IR_STAGES); i < feed.issued; ++i)
+            mbar_wait(full0 + 8 * (i % IR_STAGES), (i / IR_STAGES) & 1, abort_flag + 1);
+}
+
+// Tiles whose pages lay in several blocks' ranges: block c takes the one that began in c's range and went on behind it.
+template <int HD, int NT, bool WIDE>
+__global__ void __launch_bounds__(IR_THREADS)
+int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __restrict__ pieces) {
+    constexpr float OFFSET = WIDE ? 13.f : 6.f;
+    constexpr int C = 8 * NT;
+    extern __shared__ unsigned char smem_raw[];
+    long long* cum = (long long*)smem_raw;
+    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    __shared__ long long warp_total[IR_WARPS];
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false};
+    ssb_pdl_launch_dependents();
+    const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
+    ssb_pdl_wait();
+    const int blocks = ir_dealt(total), c0 = blockIdx.x;
+    const long long begin = ir_begin(total, c0, blocks), end = ir_begin(total, c0 + 1, blocks);
+    if (begin >= end) return;
+    const IrSegment seg = ir_locate(B, end - 1, end);
+    if (seg.first < begin || seg.first + seg.units <= end) return;
+    const int c1 = ir_owner(seg.first + seg.units - 1, total, blocks);
+    auto piece = [&](int c) { return pieces + (size_t)(2 * c + (c == c0)) * ir_piece<HD, NT>(); };
+    for (int e = threadIdx.x; e < C * (HD / 4); e += IR_THREADS) {
+        const int col = e / (HD / 4), d = e % (HD / 4) * 4;
+        float top = -INFINITY, sum = 0.f;
+        for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(piece(c) + C * HD + col));
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = c0; c <= c1; ++c) {
+            const float* p = piece(c);
+            const float mc = __ldcg(p + C * HD + col), by = mc == -INFINITY ? 0.f : ir_ex2(mc - top);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(p + col * HD + d));
+            v.x = fmaf(y.x, by, v.x); v.y = fmaf(y.y, by, v.y); v.z = fmaf(y.z, by, v.z); v.w = fmaf(y.w, by, v.w);
+            sum = fmaf(__ldcg(p + C * HD + C + col), by, sum);
+        }
+        ir_put<HD, WIDE>(a, seqs[seg.b], seg.tile, tts, seg.kvh, col, d, v, top, sum, OFFSET);
+    }
+}
+
+// What the last rows of every sequence attend to, from their lse: the keys once more, 8 NT of the (row, head) columns at a time, QB
+// such batches beside each page.  A key belongs to one block, which adds its columns' probabilities up in one order and then to the
+// key's weight.
+template <int HD, int NT, int QB, bool WIDE> constexpr size_t ir_weigh_smem(int n_seqs) {
+    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, false>() + (size_t)QB * NT * (HD / 16) * 32 * (WIDE ? 16 : 8) + IR_STAGES * 48 +
+           2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IrSeq) + 8) + 8;
+}
+template <int HD, int NT, int QB, bool WIDE>
+__global__ void __launch_bounds__(IR_THREADS)
+int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restrict__ error_word, const __grid_constant__ CUtensorMap map_k) {
+    constexpr int C = 8 * NT, Q_WORDS = NT * (HD / 16) * 32 * (WIDE ? 4 : 2);
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* stages = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint32_t* qs = (uint32_t*)(stages + IR_STAGES * ir_stage_bytes<HD, false>());
+    float* scales = (float*)(qs + QB * Q_WORDS);
+    uint64_t* bars = (uint64_t*)(scales + IR_STAGES * IR_SIDE);
+    long long* cum = (long long*)(bars + 2 * IR_STAGES);
+    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    __shared__ float qf[QB * C], lse2[QB * C];
+    __shared__ long long warp_total[IR_WARPS];
+    __shared__ int sm_abort[2];
+    volatile int* abort_flag = sm_abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.n_q / a.n_kv;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + IR_STAGES);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < IR_STAGES; ++i) { mbar_init(full0 + 8 * i, 33); mbar_init(empty0 + 8 * i, IR_WARPS); }
+        abort_flag[0] = 0;
+        abort_flag[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, true};
+    const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total, a.weigh_last);
+    const int blocks = ir_dealt(total);
+    const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
+    IrFeed feed{};
+    feed.next = begin;
+    feed.end = end;
+    bool ok = true;
+    if (warp == 0)
+        while (ok && feed.next < end && feed.issued < IR_STAGES - 1)
+            ok = ir_feed<HD, false>(a, B, feed, stages, scales, full0, empty0, map_k, map_k, abort_flag);
+    ssb_pdl_wait();                                                // the rows' lse
+    int done = 0;
+    for (long long u = begin; u < end;) {
+        const IrSegment seg = ir_locate(B, u, end);
+        const IrSeq s = seqs[seg.b];
+        __syncthreads();                                           // the segment before is done with its queries
+        const int batches = min(QB, (s.n_new * group - column0 + C - 1) / C);      // may be none
+        for (int q = 0; q < batches; ++q)
+            ir_queries<HD, NT, WIDE>(a, s.row0, s.n_new, seg.kvh, column0 + q * C, qs + q * Q_WORDS, qf + q * C);
+        for (int c = threadIdx.x; c < batches * C; c += IR_THREADS) {
+            const int token = (column0 + c) / group;
+            lse2[c] = token < s.n_new ? a.lse[(size_t)(s.row0 + token) * a.n_q + seg.kvh * group + (column0 + c) % group] * 1.4426950408889634f : INFINITY;
+        }
+        __syncthreads();
+        for (int p = 0; p < seg.n; ++p, ++done) {
+            if (warp == 0 && ok && feed.next < end)
+                ok = ir_feed<HD, false>(a, B, feed, stages, scales, full0, empty0, map_k, map_k, abort_flag);
+            const int st = done % IR_STAGES;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * st, (done / IR_STAGES) & 1, abort_flag));
+            if (!ok) {
+                if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
+                continue;
+            }
+            const unsigned char* keys = stages + st * ir_stage_bytes<HD, false>();
+            const int key0 = (seg.page + p) * 64 + 16 * warp;
+            const float ks = scales[IR_SIDE * st + 16 * warp / a.block];
+            const bool inside = key0 + 15 <= s.start + column0 / group && (a.window <= 0 || key0 > s.start + s.n_new - 1 - a.window);
+            float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+            for (int q = 0; q < batches; ++q) {
+                float sc[NT][4];
+                ir_scores<HD, NT, WIDE>(keys, qs + q * Q_WORDS, warp, lane, sc);
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = q * C + 8 * i + 2 * t + (e & 1);
+                        const float v = ir_ex2(sc[i][e] * (qf[c] * ks) - lse2[c]);
+                        if (inside) {
+                            sum[e >> 1] += v;
+                        } else {
+                            const int key = key0 + ir_key_of(g) + (e >> 1) * 8, at = s.start + (column0 + c) / group;
+                            if (key <= at && (a.window <= 0 || key > at - a.window)) sum[e >> 1] += v;
+                        }
+                    }
+            }
+            const int id = __float_as_int(scales[IR_SIDE * st + 8]);
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty0 + 8 * st) : "memory");
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+                const int key = key0 + ir_key_of(g) + 8 * h;
+                if (t == 0 && key < s.start + s.n_new && sum[h] > 0.f)
+                    atomicAdd(a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + (key & 63), sum[h]);
+            }
+        }
+        u += seg.n;
+    }
+    if (!ok && warp == 0)
+        for (int i = max(0, feed.issued - IR_STAGES); i < feed.issued; ++i)
+            mbar_wait(full0 + 8 * (i % IR_STAGES), (i / IR_STAGES) & 1, abort_flag + 1);
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+static int ir_map(CUtensorMap* map, const void* codes, long long rows, int head_dim) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return SSB_ERR_UNSUPPORTED;
+    if (rows > 0x7fffffffLL) return SSB_ERR_BAD_SIZE;
+    cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)head_dim};
+    cuuint32_t box[2] = {(cuuint32_t)head_dim, 64};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : SSB_ERR_BAD_SIZE;
+}
+
+// Blocks of a kernel that the device holds at once, at ``smem`` bytes a block.
+template <typename K> static int ir_resident(K kernel, size_t smem) {
+    int each = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, IR_THREADS, smem) != cudaSuccess || each < 1) each = 1;
+    return each * ssb_sm_count();
+}
+template <typename K> static int ir_configure(K kernel, size_t smem) {
+    return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+}
+
+struct IrPlan { int nt, tts, blocks; size_t piece; };
+
+template <int HD, int NT, bool WIDE> static int ir_blocks(int n_seqs) {
+    static int blocks = 0;
+    static size_t at = 0;
+    const size_t smem = ir_smem<HD, NT, WIDE>(n_seqs);
+    if (blocks == 0 || at != smem) {
+        if (ir_configure(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT, WIDE>(IR_SEQS)) != 0) { cudaGetLastError(); return -1; }
+        blocks = ir_resident(int8_rows_kernel<HD, NT, WIDE>, smem);
+        at = smem;
+    }
+    return blocks;
+}
+#define IR_EACH(HD_, NT_, WIDE_, WHAT_) \
+    do { \
+        if (HD_ == 64) { \
+            if (WIDE_) { if (NT_ == 1) { WHAT_(64, 1, true); } else if (NT_ == 2) { WHAT_(64, 2, true); } else { WHAT_(64, 4, true); } } \
+            else { if (NT_ == 1) { WHAT_(64, 1, false); } else if (NT_ == 2) { WHAT_(64, 2, false); } else { WHAT_(64, 4, false); } } \
+        } else { \
+            if (WIDE_) { if (NT_ == 1) { WHAT_(128, 1, true); } else if (NT_ == 2) { WHAT_(128, 2, true); } else { WHAT_(128, 4, true); } } \
+            else { if (NT_ == 1) { WHAT_(128, 1, false); } else if (NT_ == 2) { WHAT_(128, 2, false); } else { WHAT_(128, 4, false); } } \
+        } \
+    } while (0)
+
+static bool ir_takes(int n_q, int n_kv, int head_dim) { return (head_dim == 64 || head_dim == 128) && n_q / n_kv <= 32; }
+
+static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim) {
+    IrPlan p{};
+    const int group = n_q / n_kv;
+    const long long most = (long long)max_new * group;
+    p.nt = most <= 8 ? 1 : most <= 16 ? 2 : 4;
+    while (p.tts < 6 && (2 << p.tts) * group <= 8 * p.nt) ++p.tts;
+    const int n = std::min(n_seqs, IR_SEQS);
+#define IR_BLOCKS(H_, N_, W_) { p.blocks = ir_blocks<H_, N_, W_>(n); p.piece = ir_piece<H_, N_>(); }
+    IR_EACH(head_dim, p.nt, wide, IR_BLOCKS);
+#undef IR_BLOCKS
+    const long long units = ((long long)(rows >> p.tts) + n_seqs) * n_kv * max_pages;
+    p.blocks = (int)std::min<long long>(p.blocks, std::max(1LL, units));
+    return p;
+}
+
+// float32 elements of scratch that the launch needs.
+SSB_API long long ssb_int8_attention_scratch(int dtype, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim) {
+    if (n_seqs <= 0 || rows <= 0 || n_kv <= 0 || !ir_takes(n_q, n_kv, head_dim)) return 0;
+    const IrPlan p = ir_plan(dtype == SSB_F32, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
+    return p.blocks < 0 ? 0 : 2LL * p.blocks * (long long)p.piece;
+}
+
+template <int HD, int NT, bool WIDE>
+static int ir_rows(const IaArgs& a, const IrPlan& p, float* pieces, int* error_word, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+    for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
+        const int n = std::min(IR_SEQS, a.n_seqs - s0);
+        int8_rows_kernel<HD, NT, WIDE><<<p.blocks, IR_THREADS, ir_smem<HD, NT, WIDE>(n), stream>>>(a, s0, n, p.tts, pieces, error_word, mk, mv);
+        int rc = ssb_launch_status();
+        if (rc) return rc;
+        rc = ssb_launch(int8_finish_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IrSeq) + 8) + 8, stream, true,
+                        a, s0, n, p.tts, (const float*)pieces);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+template <int HD, int NT, int QB, bool WIDE>
+static int ir_weigh(const IaArgs& a, int max_new, int* error_word, const CUtensorMap& mk, bool chained, cudaStream_t stream) {
+    static int blocks = 0;
+    if (blocks == 0) {
+        const int rc = ir_configure(int8_weigh_kernel<HD, NT, QB, WIDE>, ir_weigh_smem<HD, NT, QB, WIDE>(IR_SEQS));
+        if (rc) return rc;
+        blocks = ir_resident(int8_weigh_kernel<HD, NT, QB, WIDE>, ir_weigh_smem<HD, NT, QB, WIDE>(64));
+    }
+    const long long columns = (long long)std::min(a.weigh_last, max_new) * (a.n_q / a.n_kv);
+    for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
+        const int n = std::min(IR_SEQS, a.n_seqs - s0);
+        const int grid = (int)std::min<long long>(blocks, (long long)n * a.n_kv * a.max_pages);
+        for (long long c = 0; c < columns; c += 8 * NT * QB) {
+            const int rc = ssb_launch(int8_weigh_kernel<HD, NT, QB, WIDE>, dim3(grid), dim3(IR_THREADS), ir_weigh_smem<HD, NT, QB, WIDE>(n),
+                                      stream, chained && s0 == 0 && c == 0, a, s0, n, (int)c, error_word, mk);
+            if (rc) return rc;
+        }
+    }
+    return 0;
+}
+
+SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int ldo, float* lse, const void* k, const void* v,
+                               const float* k_scale, const float* v_scale, float* weight, const int* page_table, int n_slots,
+                               int max_pages, int n_pages, const int* cu_new, const int* seq_start, const int* seq_slot,
+                               int n_seqs, int rows, int max_new, int n_q, int n_kv, int head_dim, int block, int window, int weigh_last,
+                               float scale, float* scratch, int* error_word, cudaStream_t stream) {
     if (n_seqs <= 0 || rows <= 0) return 0;
     if (head_dim % 16 || head_dim <= 0 || head_dim > 256 || n_kv <= 0 || n_q % n_kv || (block != 16 && block != 32 && block != 64) ||
-        (n_q + 3) / 4 > 65535 || n_kv > 65535)
+        (n_q + 3) / 4 > 65535 || n_kv > 65535 || max_new <= 0 || max_pages <= 0 || n_pages <= 0 || !error_word)
         return SSB_ERR_BAD_SIZE;
-    if (weigh_last > 0 && (!weight || !lse || n_seqs > 65535)) return SSB_ERR_BAD_SIZE;
+    if (weigh_last > 0 && (!weight || !lse)) return SSB_ERR_BAD_SIZE;
+    if (dtype != SSB_BF16 && dtype != SSB_F32) return SSB_ERR_BAD_DTYPE;
     const IaArgs a{q, out, lse, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, weight, page_table, cu_new, seq_start, seq_slot,
                    ldq, ldo, rows, n_seqs, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, block, window, weigh_last, scale};
-    const dim3 grid(rows, (n_q + 3) / 4), wgrid(min((max_pages * IA_PAGE + 3) / 4, 512), n_kv, n_seqs);
-    if (dtype == SSB_BF16) {
-        int8_attention_plain_kernel<bf16><<<grid, 128, 0, stream>>>(a);
-        if (weigh_last > 0) int8_weigh_plain_kernel<bf16><<<wgrid, 128, 0, stream>>>(a);
-    } else if (dtype == SSB_F32) {
-        int8_attention_plain_kernel<float><<<grid, 128, 0, stream>>>(a);
-        if (weigh_last > 0) int8_weigh_plain_kernel<float><<<wgrid, 128, 0, stream>>>(a);
-    } else {
-        return SSB_ERR_BAD_DTYPE;
+    if (!ir_takes(n_q, n_kv, head_dim)) {
+        if (weigh_last > 0 && n_seqs > 65535) return SSB_ERR_BAD_SIZE;
+        const dim3 grid(rows, (n_q + 3) / 4), wgrid(std::min((max_pages * IA_PAGE + 3) / 4, 512), n_kv, n_seqs);
+        if (dtype == SSB_BF16) {
+            int8_attention_plain_kernel<bf16><<<grid, 128, 0, stream>>>(a);
+            if (weigh_last > 0) int8_weigh_plain_kernel<bf16><<<wgrid, 128, 0, stream>>>(a);
+        } else {
+            int8_attention_plain_kernel<float><<<grid, 128, 0, stream>>>(a);
+            if (weigh_last > 0) int8_weigh_plain_kernel<float><<<wgrid, 128, 0, stream>>>(a);
+        }
+        return ssb_launch_status();
     }
-    return ssb_launch_status();
+    const bool wide = dtype == SSB_F32;
+    CUtensorMap mk, mv;
+    int rc = ir_map(&mk, k, (long long)n_pages * n_kv * 64, head_dim);
+    if (rc) return rc;
+    rc = ir_map(&mv, v, (long long)n_pages * n_kv * 64, head_dim);
+    if (rc) return rc;
+    if (!scratch) return SSB_ERR_BAD_SIZE;
+    const IrPlan p = ir_plan(wide, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
+    if (p.blocks < 0) return SSB_ERR_UNSUPPORTED;
+#define IR_ROWS(H_, N_, W_) rc = ir_rows<H_, N_, W_>(a, p, scratch, error_word, mk, mv, stream)
+    IR_EACH(head_dim, p.nt, wide, IR_ROWS);
+#undef IR_ROWS
+    if (rc || weigh_last <= 0) return rc;
+    const long long columns = (long long)std::min(weigh_last, max_new) * (n_q / n_kv);
+#define IR_WEIGH(N_, B_) \
+    rc = head_dim == 64 ? (wide ? ir_weigh<64, N_, B_, true>(a, max_new, error_word, mk, true, stream) : ir_weigh<64, N_, B_, false>(a, max_new, error_word, mk, true, stream)) \
+                        : (wide ? ir_weigh<128, N_, B_, true>(a, max_new, error_word, mk, true, stream) : ir_weigh<128, N_, B_, false>(a, max_new, error_word, mk, true, stream))
+    if (columns <= 8) IR_WEIGH(1, 1);
+    else IR_WEIGH(4, 4);
+#undef IR_WEIGH
+    return rc;
 }

@@ -26,8 +26,9 @@ _SIGNATURES = {
                                        _I, _I, _P]),
     "ssb_int8_read": ("int8_cache", [_P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P]),
     "ssb_int8_evict": ("int8_cache", [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
-    "ssb_int8_attention_plain": ("int8_attention", [_P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I,
-                                                    _I, _I, _I, _I, _I, _F, _P]),
+    "ssb_int8_attention": ("int8_attention", [_P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I,
+                                              _I, _I, _I, _I, _F, _P, _P, _P]),
+    "ssb_int8_attention_scratch": ("int8_attention", [_I] * 8),
     "ssb_int8_quantize_rows": ("int8_linear", [_P, _I, _I, _P, _I, _P, _I, _I, _P]),
     "ssb_int8_linear": ("int8_linear", [_P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
     "ssb_int8_linear_scratch": ("int8_linear", [_I, _I, _I]),
@@ -186,12 +187,17 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
         lse = torch.empty((rows, n_q), dtype=torch.float32, device=q.device)
     if rows == 0 or B == 0:
         return
-    _check(_fn("ssb_int8_attention_plain")(
-        q_at, ldq, _CODES[q.dtype], o_at, ldo, 0 if lse is None else lse.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(),
+    if max_new <= 0:
+        raise KernelError(f"attention: max_new {max_new} new tokens")
+    code, width = _CODES[q.dtype], page_table.shape[1]
+    scratch = torch.empty(_fn("ssb_int8_attention_scratch")(code, B, rows, max_new, width, n_q, n_kv, dim), dtype=torch.float32, device=q.device)
+    ops.note_bounded_wait_launches(1)
+    _check(_fn("ssb_int8_attention")(
+        q_at, ldq, code, o_at, ldo, 0 if lse is None else lse.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(),
         pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), 0 if pages.weight is None else pages.weight.data_ptr(),
-        page_table.data_ptr(), page_table.shape[0], page_table.shape[1], n_pages, _ints(cu_new, "cu_new", B + 1),
-        _ints(seq_start, "seq_start", B), _ints(seq_slot, "seq_slot", B), B, rows, n_q, n_kv, dim, block, int(window or 0), weigh_last,
-        scale, _stream()), "int8_attention")
+        page_table.data_ptr(), page_table.shape[0], width, n_pages, _ints(cu_new, "cu_new", B + 1),
+        _ints(seq_start, "seq_start", B), _ints(seq_slot, "seq_slot", B), B, rows, max_new, n_q, n_kv, dim, block, int(window or 0),
+        weigh_last, scale, scratch.data_ptr(), ops.tc_error_word(q.device).data_ptr(), _stream()), "int8_attention")
 
 
 # ---- matrix products ------------------------------------------------------------------------------------------------
