@@ -27,7 +27,7 @@ struct IaArgs {
     const int* cu_new;
     const int* seq_start;
     const int* seq_slot;
-    int ldq, ldo, rows, n_seqs, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, block, window, weigh_last;
+    int ldq, ldo, rows, n_seqs, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, shift, window, weigh_last;    // 1 << shift tokens a scale
     float scale;
 };
 
@@ -70,11 +70,11 @@ int8_attention_plain_kernel(const IaArgs a) {
             }
 #pragma unroll
         for (int x = 16; x; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-        d *= a.scale * a.k_scale[r / a.block];
+        d *= a.scale * a.k_scale[r >> a.shift];
         const float m_new = fmaxf(m, d), keep = m == -INFINITY ? 0.f : expf(m - m_new), p = expf(d - m_new);
         l = l * keep + p;
         m = m_new;
-        const float pv = p * a.v_scale[r / a.block];
+        const float pv = p * a.v_scale[r >> a.shift];
 #pragma unroll
         for (int w = 0; w < 2; ++w)
             if (lane + 32 * w < words) {
@@ -109,7 +109,7 @@ int8_weigh_plain_kernel(const IaArgs a) {
         const int page = a.page_table[(size_t)s * a.max_pages + (j >> 6)];
         if (page < 0 || page >= a.n_pages) continue;
         const size_t r = ((size_t)page * a.n_kv + kvh) * IA_PAGE + (j & 63);
-        const float ks = a.scale * a.k_scale[r / a.block];
+        const float ks = a.scale * a.k_scale[r >> a.shift];
         float sum = 0.f;
         for (int i = max(i0, j - start); i < n_new; ++i) {
             if (a.window > 0 && j <= start + i - a.window) break;
@@ -132,24 +132,29 @@ int8_weigh_plain_kernel(const IaArgs a) {
 }
 
 // ---- tensor cores, a page at a time ---------------------------------------------------------------------------------
-// Rows of a step that share a kv head (the query heads of its group, and up to ``tt`` neighbouring tokens) are the columns of
-// m16n8k16 products of float16: S^T = K Q^T with the 16 keys of a warp as rows, O^T = V^T P^T.  Codes are whole numbers up to 127,
-// so float16 holds them exactly; a query's column is taken times the power of two that brings its largest element to 256 .. 512,
-// which loses nothing of a bfloat16, and a float32 one goes in two halves of 11 bits each (WIDE), as do its probabilities.  The
-// scales stay outside the products: a key's goes onto the score; a value's, f * 2^x, into the exponent (x) and onto the
+// Rows of a step that share a kv head (the query heads of its group, and up to 2^tts neighbouring tokens) are the columns, the 16
+// keys of a warp what is summed over.  Scores take the codes as they are, in products of 8-bit integers (m16n8k32): a query goes
+// times the power of two that brings its largest element to 2^29 .. 2^30, is rounded to a whole number (which keeps all of a
+// float32 and more), and its four bytes, as digits -128 .. 127, are rows of the A operand, 8 columns' two digits an instruction; K
+// is the B operand as it lies in memory.  The sums are exact and are put together in float32.  O^T = V^T P^T is in float16
+// (m16n8k16): codes are whole numbers up to 127, which float16 holds exactly; probabilities are rounded to its 11 bits, or (WIDE,
+// float32 rows) go in two halves.  The scores' registers are the B operand's, so nothing moves between lanes.
+// The scales stay outside the products: a key's goes onto the score; a value's, f * 2^x, into the exponent (x) and onto the
 // probability (f), with the running maximum taken over score + x, so that float16 holds what is summed whatever the scales are.
 // The maximum is rounded up to a whole number, in the log2 domain: taking x and it off a score then costs no bits.
 //
-// Codes become float16 in registers: 1024 + (code + 128) is a float16 whose low byte is the code with its sign bit turned, so four
-// codes take one exclusive-or, two byte permutations and two subtractions.  Which key is which row of the products, and which
-// dims its k-steps, is free as long as both operands agree: chosen so that every lane reads whole 16-byte pieces of a row, keys
-// {0, 4, 1, 5, 2, 6, 3, 7} on rows 0 .. 7, with no two lanes of a quarter-warp in one bank (head size 128).
+// Value codes become float16 in registers: 1024 + (code + 128) is a float16 whose low byte is the code with its sign bit turned, so
+// two keys' four codes take two exclusive-ors, six byte permutations and four subtractions.  Which key is which column or k of
+// the products, and which dims its k-steps, is free as long as both operands agree: chosen so that every lane reads whole 16-byte
+// pieces of a row, a quarter-warp from 8 banks' groups (head size 128).
 //
 // The launch's work is its pages: tiles of rows x pages that they see, dealt out evenly over the blocks wherever a tile ends (a
 // block finds its range from the batch's integers alone).  A tile that lies in one block's range is finished there; pieces of
 // others go to scratch, and int8_finish_kernel puts them together in the order of the keys.  Nothing is left from one launch
 // to the next.
-constexpr int IR_THREADS = 128, IR_WARPS = 4, IR_SEQS = 1024, IR_STAGES = 4;
+constexpr int IR_THREADS = 128, IR_WARPS = 4, IR_SEQS = 1024, IR_STAGES = 3;
+constexpr int IR_EXTRA = 3;
+constexpr float IR_NONE = -1e30f;               // a maximum over no key: finite, so that nothing below needs to ask for it
 constexpr int IR_SIDE = 12;                  // beside a stage's page: its scales of keys and of values, and its id
 constexpr int IR_LEAST_X = -80, IR_MOST_X = 120;
 
@@ -161,6 +166,7 @@ struct IrBatch {
     const long long* cum;                // [n_seqs + 1]
     int n_seqs, n_kv, tts, window;
     bool one_tile;                       // a sequence's rows are one tile, however many
+    int extra;                           // what beginning and ending a tile costs, in pages: units without a page before its first
 
     // sum over i < t of floor(max(0, a + i * 2^tts) / 64)
     __device__ long long floors(long long t, long long a) const {
@@ -176,10 +182,10 @@ struct IrBatch {
         return (a >> 6) * t + ramp(r0 + t) - ramp(r0);
     }
     __device__ int tiles(const IrSeq& s) const { return s.slot < 0 || s.n_new <= 0 ? 0 : one_tile ? 1 : (s.n_new + (1 << tts) - 1) >> tts; }
-    // pages that the first t tiles of a sequence see, tile by tile
-    __device__ long long pages_before(const IrSeq& s, long long t) const {
-        if (one_tile) return t * (((s.start + s.n_new - 1) >> 6) - first_page(s, 0) + 1);
-        return t + floors(t, (long long)s.start + (1 << tts) - 1) - (window > 0 ? floors(t, (long long)s.start - window + 1) : 0);
+    // units of the first t tiles of a sequence: the pages that each sees, and the extra ones
+    __device__ long long units_before(const IrSeq& s, long long t) const {
+        if (one_tile) return t * (((s.start + s.n_new - 1) >> 6) - first_page(s, 0) + 1 + extra);
+        return t * (1 + extra) + floors(t, (long long)s.start + (1 << tts) - 1) - (window > 0 ? floors(t, (long long)s.start - window + 1) : 0);
     }
     __device__ int first_page(const IrSeq& s, int tile) const {
         const long long lo = (long long)s.start + ((long long)tile << tts) - window + 1;
@@ -189,9 +195,9 @@ struct IrBatch {
 
 // A run of pages of one tile and kv head: what of it lies in a block's range.
 struct IrSegment {
-    int b, kvh, tile, page, n;           // pages page .. page + n - 1 of the sequence
-    long long first, units;              // the tile's units
-    __device__ bool whole() const { return n == units; }
+    int b, kvh, tile, page, n;           // pages page .. page + n - 1 of the sequence (n may be 0)
+    long long first, last, next;         // the units of the tile's first and last page, and the one behind the segment
+    bool begins, whole;                  // has the tile's first page; all of them
 };
 
 __device__ __forceinline__ IrSegment ir_locate(const IrBatch& B, long long u, long long end) {
@@ -204,21 +210,29 @@ __device__ __forceinline__ IrSegment ir_locate(const IrBatch& B, long long u, lo
     IrSegment g;
     g.b = lo;
     const int tiles = B.tiles(s);
-    const long long per = (B.cum[lo + 1] - B.cum[lo]) / B.n_kv;
+    const long long per = tiles == 1 ? B.units_before(s, 1) : (B.cum[lo + 1] - B.cum[lo]) / B.n_kv;
     long long r = u - B.cum[lo];
-    g.kvh = (int)(r / per);
-    r -= g.kvh * per;
+    // r / per, below n_kv: by float32, and put right
+    int h = (int)((float)r / (float)per);
+    while (h > 0 && h * per > r) --h;
+    while ((h + 1) * per <= r) ++h;
+    g.kvh = h;
+    r -= h * per;
     int t0 = 0, t1 = tiles - 1;          // the last tile that begins at or before the unit
     while (t0 < t1) {
         const int mid = (t0 + t1 + 1) >> 1;
-        if (B.pages_before(s, mid) <= r) t0 = mid; else t1 = mid - 1;
+        if (B.units_before(s, mid) <= r) t0 = mid; else t1 = mid - 1;
     }
-    const long long before = B.pages_before(s, t0);
+    const long long before = t0 ? B.units_before(s, t0) : 0, units = (tiles == 1 ? per : B.units_before(s, t0 + 1)) - before;
     g.tile = t0;
-    g.units = B.pages_before(s, t0 + 1) - before;
-    g.first = u - (r - before);
-    g.page = B.first_page(s, t0) + (int)(r - before);
-    g.n = (int)min(g.first + g.units - u, end - u);
+    g.first = u - (r - before) + B.extra;
+    g.last = g.first + units - B.extra - 1;
+    const long long from = max(u, g.first);
+    g.next = min(g.last + 1, end);
+    g.n = (int)max(0LL, g.next - from);
+    g.page = B.first_page(s, t0) + (int)(from - g.first);
+    g.begins = from == g.first;
+    g.whole = g.begins && g.next == g.last + 1;
     return g;
 }
 
@@ -233,7 +247,7 @@ __device__ __forceinline__ long long ir_read_batch(const IaArgs& a, int s0, int 
     }
     __syncthreads();
     const int per = (n_seqs + IR_THREADS - 1) / IR_THREADS, b0 = (int)threadIdx.x * per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto units_of = [&](int b) { return b < n_seqs ? B.pages_before(seqs[b], B.tiles(seqs[b])) * B.n_kv : 0LL; };
+    auto units_of = [&](int b) { return b < n_seqs ? B.units_before(seqs[b], B.tiles(seqs[b])) * B.n_kv : 0LL; };
     long long local = 0;
     for (int i = 0; i < per; ++i) local += units_of(b0 + i);
     long long incl = local;
@@ -273,10 +287,13 @@ __device__ __forceinline__ void ir_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t ir_transpose8(uint32_t v) {
-    uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
-    return d;
+__device__ __forceinline__ void ir_mma8(int (&c)[4], const uint4& a, uint32_t b0, uint32_t b1, bool first) {
+    if (first)
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(0));
+    else
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t ir_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -295,48 +312,51 @@ __device__ __forceinline__ uint32_t ir_codes(uint32_t w, uint32_t sel) {
 template <int HD> __device__ __forceinline__ uint32_t ir_at(int r, int c) {
     return HD == 128 ? (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)) : (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
-__device__ __forceinline__ int ir_key_of(int g) { return (g >> 1) + 4 * (g & 1); }       // row g's key; row g + 8's is 8 further
+// Column g of eight keys is key ir_key_of(g) of them: a lane's columns 2 t, 2 t + 1 are keys t and t + 4.
+__device__ __forceinline__ int ir_key_of(int g) { return (g >> 1) + 4 * (g & 1); }
 
-// S^T of a warp's 16 keys: rows ir_key_of(g) (+ 8), columns 2 t, 2 t + 1 of every tile of 8.
-template <int HD, int NT, bool WIDE>
+// Words of a column tile's queries: for each 64 dims and half of 16-byte pieces two pairs of digits, four words a lane.
+template <int HD> constexpr int ir_q_words() { return HD / 64 * 2 * 2 * 32 * 4; }
+
+// Scores of a warp's 16 keys: of column 8 i + g with keys t, t + 4, t + 8, t + 12.
+template <int HD, int NT>
 __device__ __forceinline__ void ir_scores(const unsigned char* keys, const uint32_t* qs, int warp, int lane, float (&s)[NT][4]) {
-    const int g = lane >> 2, t = lane & 3, r0 = 16 * warp + ir_key_of(g), r1 = r0 + 8;
-    constexpr int STEPS = HD / 16;
+    const int g = lane >> 2, t = lane & 3, r0 = 16 * warp + ir_key_of(g);
+    constexpr int H = HD / 64;
+    uint4 k[2][H];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+        for (int j = 0; j < 2; ++j) k[j][h] = *reinterpret_cast<const uint4*>(keys + ir_at<HD>(r0 + 8 * j, 4 * h + t));
 #pragma unroll
-    for (int h = 0; h < HD / 64; ++h) {
-        const uint4 k0 = *reinterpret_cast<const uint4*>(keys + ir_at<HD>(r0, 4 * h + t));
-        const uint4 k1 = *reinterpret_cast<const uint4*>(keys + ir_at<HD>(r1, 4 * h + t));
-        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+    for (int i = 0; i < NT; ++i) {
+        int sum[2][2][4];                                        // [pair of digits][eight keys]
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const uint4 q = reinterpret_cast<const uint4*>(qs)[(((i * H + h) * 2 + half) * 2 + d) * 32 + lane];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        ir_mma8(sum[d][j], q, half ? k[j][h].z : k[j][h].x, half ? k[j][h].w : k[j][h].y, h == 0 && half == 0);
+                }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t u0 = w0[e] ^ 0x80808080u, u1 = w1[e] ^ 0x80808080u;
-            const uint32_t a0 = ir_codes(u0, 0x4140), a2 = ir_codes(u0, 0x4342), a1 = ir_codes(u1, 0x4140), a3 = ir_codes(u1, 0x4342);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int at = (i * STEPS + 4 * h + e) * 32 + lane;
-                if (WIDE) {
-                    const uint4 q = reinterpret_cast<const uint4*>(qs)[at];
-                    ir_mma(s[i], a0, a1, a2, a3, q.z, q.w);      // the low halves first
-                    ir_mma(s[i], a0, a1, a2, a3, q.x, q.y);
-                } else {
-                    const uint2 q = reinterpret_cast<const uint2*>(qs)[at];
-                    ir_mma(s[i], a0, a1, a2, a3, q.x, q.y);
-                }
-            }
+            const int j = e >> 1, c = e & 1;
+            s[i][e] = fmaf((float)(sum[0][j][c] * 256 + sum[0][j][c + 2]), 65536.f, (float)(sum[1][j][c] * 256 + sum[1][j][c + 2]));
         }
     }
 }
 
-// Query columns c0 .. c0 + 8 NT - 1 of a (sequence, kv head) as fragments of the products' B operand, and each column's factor
-// (scale * log2 e over its power of two).  Column c: token c / group of the tile, head c % group.
+// Query columns c0 .. c0 + 8 NT - 1 of a (sequence, kv head) as digits of the products' A operand, and each column's factor (scale *
+// log2 e over its power of two; no number for a column that holds one that is not finite).  Column c: token c / group of the
+// tile, head c % group.
 template <int HD, int NT, bool WIDE>
 __device__ __forceinline__ void ir_queries(const IaArgs& a, int row0, int n_tokens, int kvh, int c0, uint32_t* qs, float* qf) {
     using T = typename std::conditional<WIDE, float, bf16>::type;
-    constexpr int LANES = HD / 8, STEPS = HD / 16;               // lanes a column, 8 elements each
+    constexpr int LANES = HD / 8;                                // lanes a column, 8 elements each
     const int group = a.n_q / a.n_kv, l = threadIdx.x % LANES;
 #pragma unroll
     for (int pass = 0; pass < (8 * NT * LANES + IR_THREADS - 1) / IR_THREADS; ++pass) {
@@ -354,33 +374,39 @@ __device__ __forceinline__ void ir_queries(const IaArgs& a, int row0, int n_toke
                 for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
             }
         }
-        float most = 0.f;
+        uint32_t most = 0;                                       // magnitudes in the order of their bits: no number is above infinity
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        // 2^up brings the largest element to 256 .. 512
-        const int up = most > 0.f ? min(8 - ((int)(__float_as_uint(most) >> 23) - 127), 100) : 0;
+        for (int o = LANES / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const int up = most ? min(29 - ((int)(most >> 23) - 127), 126) : 0;
         const float times = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
         if (col < 8 * NT) {
             const int piece = l >> 1, lane = (col & 7) * 4 + (piece & 3);
+            uint32_t n[8], w[4][2];                              // digit, four elements
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {                        // four elements: one k-step of this lane
-                const int step = 4 * (piece >> 2) + 2 * (l & 1) + w, at = ((col >> 3) * STEPS + step) * 32 + lane;
-                float y[4];
+            for (int i = 0; i < 8; ++i) n[i] = ((uint32_t)__float2int_rn(x[i] * times) + 0x00808080u) ^ 0x00808080u;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = x[4 * w + i] * times;
-                const uint32_t h0 = ir_half2(y[0], y[1]), h1 = ir_half2(y[2], y[3]);
-                if constexpr (WIDE) {
-                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                    reinterpret_cast<uint4*>(qs)[at] = make_uint4(h0, h1, ir_half2(y[0] - f0.x, y[1] - f0.y), ir_half2(y[2] - f1.x, y[3] - f1.y));
-                } else {
-                    reinterpret_cast<uint2*>(qs)[at] = make_uint2(h0, h1);
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t sel = 0x0040u + 0x11u * d;     // byte d of two words
+                    w[d][i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], sel), __byte_perm(n[4 * i + 2], n[4 * i + 3], sel), 0x5410);
                 }
-            }
-            if (l == 0) qf[col] = a.scale * 1.4426950408889634f * back;
+            uint4* at = reinterpret_cast<uint4*>(qs) + ((((col >> 3) * (HD / 64) + (piece >> 2)) * 2 + (l & 1)) * 2) * 32 + lane;
+            at[0] = make_uint4(w[3][0], w[2][0], w[3][1], w[2][1]);
+            at[32] = make_uint4(w[1][0], w[0][0], w[1][1], w[0][1]);
+            if (l == 0) qf[col] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * 1.4426950408889634f * back;
         }
     }
+}
+
+// mbar_wait, asking once before the clock is read.
+__device__ __forceinline__ bool ir_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred P1;\nmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\nselp.b32 %0, 1, 0, P1;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok || mbar_wait(bar, parity, abort_flag);
 }
 
 // Pages on their way into the ring: warp 0 asks for them, up to IR_STAGES - 1 ahead of the warps that work.
@@ -388,16 +414,19 @@ template <int HD, bool VALUES> constexpr int ir_stage_bytes() { return (VALUES ?
 
 struct IrFeed {
     IrSegment seg;
-    long long next, end;                 // the unit to be asked for next
+    long long next, end;                 // the unit behind the segment
     int left, ids, ids_from, issued;     // pages of the segment not yet asked for; page ids of 32 pages, one a lane
+    int stage, lap;                      // where the next page goes
 };
 
 template <int HD, bool VALUES>
 __device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFeed& f, unsigned char* stages, float* scales, uint32_t full0,
                                         uint32_t empty0, const CUtensorMap& map_k, const CUtensorMap& map_v, volatile int* abort_flag) {
-    const int lane = threadIdx.x & 31, per = 64 / a.block;
-    if (f.left == 0) {
+    const int lane = threadIdx.x & 31, per = 64 >> a.shift;
+    while (f.left == 0) {
+        if (f.next >= f.end) return true;
         f.seg = ir_locate(B, f.next, f.end);
+        f.next = f.seg.next;
         f.left = f.seg.n;
         f.ids_from = -1;
     }
@@ -410,14 +439,14 @@ __device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFee
         f.ids_from = i;
     }
     const int id = __shfl_sync(0xffffffffu, f.ids, i - f.ids_from);
-    const int st = f.issued % IR_STAGES;
+    const int st = f.stage;
     bool ok = true;
-    if (lane == 0) ok = mbar_wait(empty0 + 8 * st, ((f.issued / IR_STAGES) & 1) ^ 1, abort_flag);
+    if (lane == 0) ok = ir_wait(empty0 + 8 * st, f.lap ^ 1, abort_flag);
     ok = __shfl_sync(0xffffffffu, ok, 0);
     if (!ok) return false;
     const size_t head = (size_t)id * a.n_kv + f.seg.kvh;
     if (lane < 2 * per) {
-        const float* src = (lane < per ? a.k_scale : a.v_scale) + head * per + lane % per;
+        const float* src = (lane < per ? a.k_scale : a.v_scale) + head * per + (lane & (per - 1));
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(scales + IR_SIDE * st + lane)), "l"(src) : "memory");
     }
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full0 + 8 * st) : "memory");
@@ -428,16 +457,18 @@ __device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFee
         tma_load_2d(dst, &map_k, full0 + 8 * st, 0, (int)(head * 64));
         if (VALUES) tma_load_2d(dst + 64 * HD, &map_v, full0 + 8 * st, 0, (int)(head * 64));
     }
+    if (++f.stage == IR_STAGES) { f.stage = 0; f.lap ^= 1; }
     ++f.issued;
-    ++f.next;
     --f.left;
     return true;
 }
 
-template <int HD, int NT> constexpr int ir_acc_ld() { return HD + 4; }
-template <int HD, int NT, bool WIDE> constexpr size_t ir_smem(int n_seqs) {
-    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, true>() + IR_WARPS * 8 * NT * ir_acc_ld<HD, NT>() * 4 +
-           (size_t)NT * (HD / 16) * 32 * (WIDE ? 16 : 8) + IR_STAGES * 48 + 2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IrSeq) + 8) + 8;
+template <int HD> constexpr int ir_acc_ld() { return HD + 4; }
+template <int HD, int NT> constexpr int ir_work_words() {
+    return 8 * NT * ir_acc_ld<HD>() > NT * ir_q_words<HD>() ? 8 * NT * ir_acc_ld<HD>() : NT * ir_q_words<HD>();
+}
+template <int HD, int NT> constexpr size_t ir_smem(int n_seqs) {
+    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, true>() + (size_t)ir_work_words<HD, NT>() * 4 + IR_STAGES * IR_SIDE * 4 + 2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IrSeq) + 8) + 8;
 }
 // floats of a piece: a column's sums, its maximum and its sum of weights
 template <int HD, int NT> constexpr int ir_piece() { return 8 * NT * (HD + 2); }
@@ -455,25 +486,26 @@ __device__ __forceinline__ void ir_put(const IaArgs& a, const IrSeq& s, int tile
     const int group = a.n_q / a.n_kv, token = (tile << tts) + col / group, head = kvh * group + col % group;
     if (col / group >= (1 << tts) || token >= s.n_new) return;
     const size_t row = (size_t)(s.row0 + token);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     ir_store4<T>((T*)a.out + row * a.ldo + (size_t)head * HD + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-    if (d == 0 && a.lse) a.lse[row * a.n_q + head] = l > 0.f ? (m - offset + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    if (d == 0 && a.lse) a.lse[row * a.n_q + head] = l == 0.f ? -INFINITY : (m - offset + log2f(l)) * 0.6931471805599453f;
 }
 
 template <int HD, int NT, bool WIDE>
-__global__ void __launch_bounds__(IR_THREADS)
+__global__ void __launch_bounds__(IR_THREADS, NT == 1 ? 4 : 2)
 int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict__ pieces, int* __restrict__ error_word,
                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     // probabilities are summed times 2^OFFSET and may exceed that by 2^LAZY before the reference maximum is moved; with f below 2
     // and both in float16, 2^(OFFSET + LAZY + 1) stays below 2^16
     constexpr float OFFSET = WIDE ? 13.f : 6.f, LAZY = WIDE ? 1.f : 8.f;
-    constexpr int C = 8 * NT, ACC_LD = ir_acc_ld<HD, NT>(), TILES = HD / 16;
+    constexpr int C = 8 * NT, ACC_LD = ir_acc_ld<HD>(), TILES = HD / 16;
     using T = typename std::conditional<WIDE, float, bf16>::type;
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* stages = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* acc = (float*)(stages + IR_STAGES * ir_stage_bytes<HD, true>());       // [warp][column][ACC_LD]
-    uint32_t* qs = (uint32_t*)(acc + IR_WARPS * C * ACC_LD);
-    float* scales = (float*)(qs + NT * (HD / 16) * 32 * (WIDE ? 4 : 2));          // [stage][keys' | values' | page id]
+    unsigned char* stages = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    // a segment's queries, and when all its pages are worked on its sums [column][ACC_LD]
+    float* acc = (float*)(stages + IR_STAGES * ir_stage_bytes<HD, true>());
+    uint32_t* qs = (uint32_t*)acc;
+    float* scales = acc + ir_work_words<HD, NT>();                                // [stage][keys' | values' | page id]
     uint64_t* bars = (uint64_t*)(scales + IR_STAGES * IR_SIDE);                         // full, empty
     long long* cum = (long long*)(bars + 2 * IR_STAGES);
     IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
@@ -483,6 +515,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
     volatile int* abort_flag = sm_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + IR_STAGES);
+    const int block_at = (16 * warp) >> a.shift;                   // the warp's keys have one scale
     ssb_pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < IR_STAGES; ++i) { mbar_init(full0 + 8 * i, 33); mbar_init(empty0 + 8 * i, IR_WARPS); }
@@ -491,7 +524,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     const int blocks = ir_dealt(total);
     const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
@@ -512,29 +545,28 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
     feed.end = end;
     bool ok = true;
     if (warp == 0)
-        while (ok && feed.next < end && feed.issued < IR_STAGES - 1)
+        for (int i = 0; ok && i < IR_STAGES - 1; ++i)
             ok = ir_feed<HD, true>(a, B, feed, stages, scales, full0, empty0, map_k, map_v, abort_flag);
-    int done = 0;                                                  // pages worked on
+    int st = 0, lap = 0;                                           // the stage of the page that comes next
     for (long long u = begin; u < end;) {
         const IrSegment seg = ir_locate(B, u, end);
+        if (seg.n == 0) { u = seg.next; continue; }
         const IrSeq s = seqs[seg.b];
         const int token0 = seg.tile << tts, n_tokens = min(1 << tts, s.n_new - token0);
         ir_queries<HD, NT, WIDE>(a, s.row0 + token0, n_tokens, seg.kvh, 0, qs, qf);
         __syncthreads();
         // a column's last and first visible key, and those that all columns see
-        int hi[NT][2], lo[NT][2];
-        float m[NT][2], l[NT][2], factor[NT][2], o[TILES][NT][4];
+        int hi[NT], lo[NT];
+        float m[NT], l[NT], factor[NT], o[TILES][NT][4];
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = 8 * i + 2 * t + e, token = c / group;
-                hi[i][e] = token < n_tokens ? s.start + token0 + token : -1;
-                lo[i][e] = a.window > 0 ? hi[i][e] - a.window + 1 : 0;
-                m[i][e] = -INFINITY;
-                l[i][e] = 0.f;
-                factor[i][e] = qf[c];
-            }
+        for (int i = 0; i < NT; ++i) {
+            const int token = (8 * i + g) / group;
+            hi[i] = token < n_tokens ? s.start + token0 + token : -1;
+            lo[i] = a.window > 0 ? hi[i] - a.window + 1 : 0;
+            m[i] = IR_NONE;
+            l[i] = 0.f;
+            factor[i] = qf[8 * i + g];
+        }
 #pragma unroll
         for (int i = 0; i < TILES; ++i)
 #pragma unroll
@@ -542,69 +574,66 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
         const int all_hi = s.start + token0, all_lo = a.window > 0 ? s.start + token0 + n_tokens - a.window : 0;
-        for (int p = 0; p < seg.n; ++p, ++done) {
-            if (warp == 0 && ok && feed.next < end)
+        for (int p = 0; p < seg.n; ++p, lap ^= st == IR_STAGES - 1, st = st == IR_STAGES - 1 ? 0 : st + 1) {
+            if (warp == 0 && ok)
                 ok = ir_feed<HD, true>(a, B, feed, stages, scales, full0, empty0, map_k, map_v, abort_flag);
-            const int st = done % IR_STAGES;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * st, (done / IR_STAGES) & 1, abort_flag));
+            if (ok) ok = __all_sync(0xffffffffu, ir_wait(full0 + 8 * st, lap, abort_flag));
             if (!ok) {                                             // give up, but meet the others at the segment's end
                 if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
                 continue;
             }
             const unsigned char* keys = stages + st * ir_stage_bytes<HD, true>();
             const unsigned char* values = keys + 64 * HD;
-            const int key0 = (seg.page + p) * 64 + 16 * warp, per = 64 / a.block;
-            const float ks = scales[IR_SIDE * st + 16 * warp / a.block], vs = scales[IR_SIDE * st + per + 16 * warp / a.block];
+            const int key0 = (seg.page + p) * 64 + 16 * warp;
+            const float ks = scales[IR_SIDE * st + block_at], vs = scales[IR_SIDE * st + (64 >> a.shift) + block_at];
             float sc[NT][4];
-            ir_scores<HD, NT, WIDE>(keys, qs, warp, lane, sc);
+            ir_scores<HD, NT>(keys, qs, warp, lane, sc);
             // vs = f 2^x; what is no scale belongs to keys that nobody sees
             const int x = min(max((int)(__float_as_uint(vs) >> 23 & 255) - 127, IR_LEAST_X), IR_MOST_X);
             const float fx = (float)x, down = __uint_as_float((uint32_t)(127 - x) << 23), f = fabsf(vs) < 3e38f ? vs * down : 0.f;
             const bool inside = key0 >= all_lo && key0 + 15 <= all_hi;
             float worst = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int i = 0; i < NT; ++i) {
+                const float by = factor[i] * ks;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = key0 + ir_key_of(g) + (e >> 1) * 8;
-                    sc[i][e] *= factor[i][e & 1] * ks;
-                    if (!inside && (key > hi[i][e & 1] || key < lo[i][e & 1])) sc[i][e] = -INFINITY;
-                    worst = fmaxf(worst, sc[i][e] - (m[i][e & 1] - fx));     // -inf - -inf: no number, which fmaxf passes over
+                for (int e = 0; e < 4; ++e) sc[i][e] *= by;
+                if (!inside) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (key0 + t + 4 * e > hi[i] || key0 + t + 4 * e < lo[i]) sc[i][e] = -INFINITY;
                 }
+                worst = fmaxf(worst, fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])) - (m[i] - fx));
+            }
             if (__any_sync(0xffffffffu, worst > LAZY)) {
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int i = 0; i < NT; ++i) {
+                    float top = fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])) + fx;
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const float now = fmaxf(m[i], ceilf(top)), alpha = ir_ex2(m[i] - now);
+                    m[i] = now;
+                    l[i] *= alpha;
+                    const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);    // columns 2 t, 2 t + 1
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(sc[i][e], sc[i][e + 2]) + fx;
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float now = fmaxf(m[i][e], ceilf(top)), alpha = m[i][e] == -INFINITY ? 0.f : ir_ex2(m[i][e] - now);
-                        m[i][e] = now;
-                        l[i][e] *= alpha;
-#pragma unroll
-                        for (int k = 0; k < TILES; ++k) { o[k][i][e] *= alpha; o[k][i][e + 2] *= alpha; }
-                    }
+                    for (int k = 0; k < TILES; ++k) { o[k][i][0] *= a0; o[k][i][1] *= a1; o[k][i][2] *= a0; o[k][i][3] *= a1; }
+                }
             }
             uint32_t p_hi[NT][2], p_lo[NT][2];
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
+                const float ref = m[i] - fx - OFFSET;
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float ref = m[i][e & 1] == -INFINITY ? 0.f : m[i][e & 1] - fx - OFFSET;
-                    v[e] = ir_ex2(sc[i][e] - ref);
-                }
-                l[i][0] = fmaf(v[0] + v[2], down, l[i][0]);
-                l[i][1] = fmaf(v[1] + v[3], down, l[i][1]);
+                for (int e = 0; e < 4; ++e) v[e] = ir_ex2(sc[i][e] - ref);
+                l[i] = fmaf((v[0] + v[1]) + (v[2] + v[3]), down, l[i]);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < 2; ++h) {                      // keys t, t + 4, then t + 8, t + 12
                     const float v0 = v[2 * h] * f, v1 = v[2 * h + 1] * f;
-                    const uint32_t top = ir_half2(v0, v1);
-                    p_hi[i][h] = ir_transpose8(top);
+                    p_hi[i][h] = ir_half2(v0, v1);
                     if (WIDE) {
-                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&top));
-                        p_lo[i][h] = ir_transpose8(ir_half2(v0 - r.x, v1 - r.y));
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&p_hi[i][h]));
+                        p_lo[i][h] = ir_half2(v0 - r.x, v1 - r.y);
                     }
                 }
             }
@@ -639,43 +668,53 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty0 + 8 * st) : "memory");
         }
-        // the warps' parts: a column's sums, maximum and sum of weights
+        // the warps' parts: a column's maximum and sum of weights, then its sums, warp after warp; dims (HD / 8) g + 2 k, + 1 of
+        // the head lie at 16 k + 2 g
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], d);
-                const int c = 8 * i + 2 * t + e;
-                if (g == 0) { warp_m[warp][c] = m[i][e]; warp_l[warp][c] = l[i][e]; }
-#pragma unroll
-                for (int k = 0; k < TILES; ++k)                    // dims 16 g + 2 k, + 1 (head size 64: 8 g + 2 k, + 1)
-                    *reinterpret_cast<float2*>(acc + (warp * C + c) * ACC_LD + (HD / 8) * g + 2 * k) = make_float2(o[k][i][e], o[k][i][e + 2]);
-            }
+        for (int i = 0; i < NT; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (t == 0) { warp_m[warp][8 * i + g] = m[i]; warp_l[warp][8 * i + g] = l[i]; }
+        }
         __syncthreads();
-        const bool whole = seg.whole();
-        float* piece = pieces + (size_t)(2 * blockIdx.x + (seg.first >= begin)) * ir_piece<HD, NT>();
+#pragma unroll 1
+        for (int w = 0; w < IR_WARPS; ++w) {
+            if (warp == w) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int c = 8 * i + 2 * t + e;
+                        const float by = ir_ex2(warp_m[w][c] - fmaxf(fmaxf(warp_m[0][c], warp_m[1][c]), fmaxf(warp_m[2][c], warp_m[3][c])));
+#pragma unroll
+                        for (int k = 0; k < TILES; ++k) {
+                            float2* at = reinterpret_cast<float2*>(acc + c * ACC_LD + 16 * k + 2 * g);
+                            const float2 was = w ? *at : make_float2(0.f, 0.f);
+                            *at = make_float2(fmaf(o[k][i][e], by, was.x), fmaf(o[k][i][e + 2], by, was.y));
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        float* piece = pieces + (size_t)(2 * blockIdx.x + seg.begins) * ir_piece<HD, NT>();
         for (int e = threadIdx.x; e < C * (HD / 4); e += IR_THREADS) {
             const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-            float top = -INFINITY, sum = 0.f;
+            const float top = fmaxf(fmaxf(warp_m[0][c], warp_m[1][c]), fmaxf(warp_m[2][c], warp_m[3][c]));
+            float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < IR_WARPS; ++w) top = fmaxf(top, warp_m[w][c]);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < IR_WARPS; ++w) {
-                const float by = warp_m[w][c] == -INFINITY ? 0.f : ir_ex2(warp_m[w][c] - top);
-                const float4 y = *reinterpret_cast<const float4*>(acc + (w * C + c) * ACC_LD + d);
-                v.x = fmaf(y.x, by, v.x); v.y = fmaf(y.y, by, v.y); v.z = fmaf(y.z, by, v.z); v.w = fmaf(y.w, by, v.w);
-                sum = fmaf(warp_l[w][c], by, sum);
-            }
-            if (whole) {
+            for (int w = 0; w < IR_WARPS; ++w) sum = fmaf(warp_l[w][c], ir_ex2(warp_m[w][c] - top), sum);
+            const float* at = acc + c * ACC_LD + 16 * (d % (HD / 8) / 2) + 2 * (d / (HD / 8));
+            const float2 x = *reinterpret_cast<const float2*>(at), y = *reinterpret_cast<const float2*>(at + 16);
+            const float4 v = make_float4(x.x, x.y, y.x, y.y);
+            if (seg.whole) {
                 ir_put<HD, WIDE>(a, s, seg.tile, tts, seg.kvh, c, d, v, top, sum, OFFSET);
             } else {
                 *reinterpret_cast<float4*>(piece + c * HD + d) = v;
                 if (d == 0) { piece[C * HD + c] = top; piece[C * HD + C + c] = sum; }
             }
         }
-        u += seg.n;
+        __syncthreads();                                           // the queries of the next segment go where the sums were
+        u = seg.next;
     }
     if (!ok && warp == 0)                                          // let issued copies land before the block ends
         for (int i = max(0, feed.issued - IR_STAGES); i < feed.issued; ++i)
@@ -692,25 +731,26 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     long long* cum = (long long*)smem_raw;
     IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
     __shared__ long long warp_total[IR_WARPS];
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
     ssb_pdl_launch_dependents();
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     ssb_pdl_wait();
     const int blocks = ir_dealt(total), c0 = blockIdx.x;
     const long long begin = ir_begin(total, c0, blocks), end = ir_begin(total, c0 + 1, blocks);
     if (begin >= end) return;
+    // the tile whose unit is the range's last: its first page may be here or (the range ends among its extra units) elsewhere
     const IrSegment seg = ir_locate(B, end - 1, end);
-    if (seg.first < begin || seg.first + seg.units <= end) return;
-    const int c1 = ir_owner(seg.first + seg.units - 1, total, blocks);
+    if (seg.first < begin || seg.first >= end || seg.last < end) return;
+    const int c1 = ir_owner(seg.last, total, blocks);
     auto piece = [&](int c) { return pieces + (size_t)(2 * c + (c == c0)) * ir_piece<HD, NT>(); };
     for (int e = threadIdx.x; e < C * (HD / 4); e += IR_THREADS) {
         const int col = e / (HD / 4), d = e % (HD / 4) * 4;
-        float top = -INFINITY, sum = 0.f;
+        float top = IR_NONE, sum = 0.f;
         for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(piece(c) + C * HD + col));
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int c = c0; c <= c1; ++c) {
             const float* p = piece(c);
-            const float mc = __ldcg(p + C * HD + col), by = mc == -INFINITY ? 0.f : ir_ex2(mc - top);
+            const float mc = __ldcg(p + C * HD + col), by = ir_ex2(mc - top);
             const float4 y = __ldcg(reinterpret_cast<const float4*>(p + col * HD + d));
             v.x = fmaf(y.x, by, v.x); v.y = fmaf(y.y, by, v.y); v.z = fmaf(y.z, by, v.z); v.w = fmaf(y.w, by, v.w);
             sum = fmaf(__ldcg(p + C * HD + C + col), by, sum);
@@ -722,16 +762,16 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
 // What the last rows of every sequence attend to, from their lse: the keys once more, 8 NT of the (row, head) columns at a time, QB
 // such batches beside each page.  A key belongs to one block, which adds its columns' probabilities up in one order and then to the
 // key's weight.
-template <int HD, int NT, int QB, bool WIDE> constexpr size_t ir_weigh_smem(int n_seqs) {
-    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, false>() + (size_t)QB * NT * (HD / 16) * 32 * (WIDE ? 16 : 8) + IR_STAGES * 48 +
+template <int HD, int NT, int QB> constexpr size_t ir_weigh_smem(int n_seqs) {
+    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, false>() + (size_t)QB * NT * ir_q_words<HD>() * 4 + IR_STAGES * IR_SIDE * 4 +
            2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IrSeq) + 8) + 8;
 }
 template <int HD, int NT, int QB, bool WIDE>
 __global__ void __launch_bounds__(IR_THREADS)
 int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restrict__ error_word, const __grid_constant__ CUtensorMap map_k) {
-    constexpr int C = 8 * NT, Q_WORDS = NT * (HD / 16) * 32 * (WIDE ? 4 : 2);
+    constexpr int C = 8 * NT, Q_WORDS = NT * ir_q_words<HD>();
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* stages = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* stages = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint32_t* qs = (uint32_t*)(stages + IR_STAGES * ir_stage_bytes<HD, false>());
     float* scales = (float*)(qs + QB * Q_WORDS);
     uint64_t* bars = (uint64_t*)(scales + IR_STAGES * IR_SIDE);
@@ -743,6 +783,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
     volatile int* abort_flag = sm_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.n_q / a.n_kv;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + IR_STAGES);
+    const int block_at = (16 * warp) >> a.shift;                   // the warp's keys have one scale
     if (threadIdx.x == 0) {
         for (int i = 0; i < IR_STAGES; ++i) { mbar_init(full0 + 8 * i, 33); mbar_init(empty0 + 8 * i, IR_WARPS); }
         abort_flag[0] = 0;
@@ -750,7 +791,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, true};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, true, IR_EXTRA};
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total, a.weigh_last);
     const int blocks = ir_dealt(total);
     const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
@@ -759,12 +800,13 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
     feed.end = end;
     bool ok = true;
     if (warp == 0)
-        while (ok && feed.next < end && feed.issued < IR_STAGES - 1)
+        for (int i = 0; ok && i < IR_STAGES - 1; ++i)
             ok = ir_feed<HD, false>(a, B, feed, stages, scales, full0, empty0, map_k, map_k, abort_flag);
     ssb_pdl_wait();                                                // the rows' lse
-    int done = 0;
+    int st = 0, lap = 0;
     for (long long u = begin; u < end;) {
         const IrSegment seg = ir_locate(B, u, end);
+        if (seg.n == 0) { u = seg.next; continue; }
         const IrSeq s = seqs[seg.b];
         __syncthreads();                                           // the segment before is done with its queries
         const int batches = min(QB, (s.n_new * group - column0 + C - 1) / C);      // may be none
@@ -775,51 +817,51 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
             lse2[c] = token < s.n_new ? a.lse[(size_t)(s.row0 + token) * a.n_q + seg.kvh * group + (column0 + c) % group] * 1.4426950408889634f : INFINITY;
         }
         __syncthreads();
-        for (int p = 0; p < seg.n; ++p, ++done) {
-            if (warp == 0 && ok && feed.next < end)
+        for (int p = 0; p < seg.n; ++p, lap ^= st == IR_STAGES - 1, st = st == IR_STAGES - 1 ? 0 : st + 1) {
+            if (warp == 0 && ok)
                 ok = ir_feed<HD, false>(a, B, feed, stages, scales, full0, empty0, map_k, map_k, abort_flag);
-            const int st = done % IR_STAGES;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * st, (done / IR_STAGES) & 1, abort_flag));
+            if (ok) ok = __all_sync(0xffffffffu, ir_wait(full0 + 8 * st, lap, abort_flag));
             if (!ok) {
                 if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
                 continue;
             }
             const unsigned char* keys = stages + st * ir_stage_bytes<HD, false>();
             const int key0 = (seg.page + p) * 64 + 16 * warp;
-            const float ks = scales[IR_SIDE * st + 16 * warp / a.block];
+            const float ks = scales[IR_SIDE * st + block_at];
             const bool inside = key0 + 15 <= s.start + column0 / group && (a.window <= 0 || key0 > s.start + s.n_new - 1 - a.window);
-            float sum[2] = {0.f, 0.f};
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};                   // keys t, t + 4, t + 8, t + 12
 #pragma unroll 1
             for (int q = 0; q < batches; ++q) {
                 float sc[NT][4];
-                ir_scores<HD, NT, WIDE>(keys, qs + q * Q_WORDS, warp, lane, sc);
+                ir_scores<HD, NT>(keys, qs + q * Q_WORDS, warp, lane, sc);
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int i = 0; i < NT; ++i) {
+                    const int c = q * C + 8 * i + g, at = s.start + (column0 + c) / group;
+                    const float by = qf[c] * ks, ref = lse2[c];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int c = q * C + 8 * i + 2 * t + (e & 1);
-                        const float v = ir_ex2(sc[i][e] * (qf[c] * ks) - lse2[c]);
-                        if (inside) {
-                            sum[e >> 1] += v;
-                        } else {
-                            const int key = key0 + ir_key_of(g) + (e >> 1) * 8, at = s.start + (column0 + c) / group;
-                            if (key <= at && (a.window <= 0 || key > at - a.window)) sum[e >> 1] += v;
-                        }
+                        const float v = ir_ex2(sc[i][e] * by - ref);
+                        const int key = key0 + t + 4 * e;
+                        if (inside || (key <= at && (a.window <= 0 || key > at - a.window))) sum[e] += v;
                     }
+                }
             }
             const int id = __float_as_int(scales[IR_SIDE * st + 8]);
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty0 + 8 * st) : "memory");
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-                const int key = key0 + ir_key_of(g) + 8 * h;
-                if (t == 0 && key < s.start + s.n_new && sum[h] > 0.f)
-                    atomicAdd(a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + (key & 63), sum[h]);
-            }
+            // over the columns: eight lanes' four sums, two of them handed over at each of the first two steps
+            const bool up2 = lane & 16, up1 = lane & 8;
+            float x0 = up2 ? sum[2] : sum[0], x1 = up2 ? sum[3] : sum[1];
+            x0 += __shfl_xor_sync(0xffffffffu, up2 ? sum[0] : sum[2], 16);
+            x1 += __shfl_xor_sync(0xffffffffu, up2 ? sum[1] : sum[3], 16);
+            float x = up1 ? x1 : x0;
+            x += __shfl_xor_sync(0xffffffffu, up1 ? x0 : x1, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            const int key = key0 + t + 4 * (2 * up2 + up1);
+            if (!(lane & 4) && key < s.start + s.n_new && x > 0.f)
+                atomicAdd(a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + (key & 63), x);
         }
-        u += seg.n;
+        u = seg.next;
     }
     if (!ok && warp == 0)
         for (int i = max(0, feed.issued - IR_STAGES); i < feed.issued; ++i)
@@ -856,9 +898,9 @@ struct IrPlan { int nt, tts, blocks; size_t piece; };
 template <int HD, int NT, bool WIDE> static int ir_blocks(int n_seqs) {
     static int blocks = 0;
     static size_t at = 0;
-    const size_t smem = ir_smem<HD, NT, WIDE>(n_seqs);
+    const size_t smem = ir_smem<HD, NT>(n_seqs);
     if (blocks == 0 || at != smem) {
-        if (ir_configure(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT, WIDE>(IR_SEQS)) != 0) { cudaGetLastError(); return -1; }
+        if (ir_configure(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(IR_SEQS)) != 0) { cudaGetLastError(); return -1; }
         blocks = ir_resident(int8_rows_kernel<HD, NT, WIDE>, smem);
         at = smem;
     }
@@ -903,7 +945,7 @@ template <int HD, int NT, bool WIDE>
 static int ir_rows(const IaArgs& a, const IrPlan& p, float* pieces, int* error_word, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
     for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
         const int n = std::min(IR_SEQS, a.n_seqs - s0);
-        int8_rows_kernel<HD, NT, WIDE><<<p.blocks, IR_THREADS, ir_smem<HD, NT, WIDE>(n), stream>>>(a, s0, n, p.tts, pieces, error_word, mk, mv);
+        int8_rows_kernel<HD, NT, WIDE><<<p.blocks, IR_THREADS, ir_smem<HD, NT>(n), stream>>>(a, s0, n, p.tts, pieces, error_word, mk, mv);
         int rc = ssb_launch_status();
         if (rc) return rc;
         rc = ssb_launch(int8_finish_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IrSeq) + 8) + 8, stream, true,
@@ -917,16 +959,16 @@ template <int HD, int NT, int QB, bool WIDE>
 static int ir_weigh(const IaArgs& a, int max_new, int* error_word, const CUtensorMap& mk, bool chained, cudaStream_t stream) {
     static int blocks = 0;
     if (blocks == 0) {
-        const int rc = ir_configure(int8_weigh_kernel<HD, NT, QB, WIDE>, ir_weigh_smem<HD, NT, QB, WIDE>(IR_SEQS));
+        const int rc = ir_configure(int8_weigh_kernel<HD, NT, QB, WIDE>, ir_weigh_smem<HD, NT, QB>(IR_SEQS));
         if (rc) return rc;
-        blocks = ir_resident(int8_weigh_kernel<HD, NT, QB, WIDE>, ir_weigh_smem<HD, NT, QB, WIDE>(64));
+        blocks = ir_resident(int8_weigh_kernel<HD, NT, QB, WIDE>, ir_weigh_smem<HD, NT, QB>(64));
     }
     const long long columns = (long long)std::min(a.weigh_last, max_new) * (a.n_q / a.n_kv);
     for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
         const int n = std::min(IR_SEQS, a.n_seqs - s0);
         const int grid = (int)std::min<long long>(blocks, (long long)n * a.n_kv * a.max_pages);
         for (long long c = 0; c < columns; c += 8 * NT * QB) {
-            const int rc = ssb_launch(int8_weigh_kernel<HD, NT, QB, WIDE>, dim3(grid), dim3(IR_THREADS), ir_weigh_smem<HD, NT, QB, WIDE>(n),
+            const int rc = ssb_launch(int8_weigh_kernel<HD, NT, QB, WIDE>, dim3(grid), dim3(IR_THREADS), ir_weigh_smem<HD, NT, QB>(n),
                                       stream, chained && s0 == 0 && c == 0, a, s0, n, (int)c, error_word, mk);
             if (rc) return rc;
         }
@@ -946,7 +988,7 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
     if (weigh_last > 0 && (!weight || !lse)) return SSB_ERR_BAD_SIZE;
     if (dtype != SSB_BF16 && dtype != SSB_F32) return SSB_ERR_BAD_DTYPE;
     const IaArgs a{q, out, lse, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, weight, page_table, cu_new, seq_start, seq_slot,
-                   ldq, ldo, rows, n_seqs, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, block, window, weigh_last, scale};
+                   ldq, ldo, rows, n_seqs, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, block == 16 ? 4 : block == 32 ? 5 : 6, window, weigh_last, scale};
     if (!ir_takes(n_q, n_kv, head_dim)) {
         if (weigh_last > 0 && n_seqs > 65535) return SSB_ERR_BAD_SIZE;
         const dim3 grid(rows, (n_q + 3) / 4), wgrid(std::min((max_pages * IA_PAGE + 3) / 4, 512), n_kv, n_seqs);
