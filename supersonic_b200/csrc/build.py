@@ -57,7 +57,7 @@ LIBRARIES: Dict[str, Dict[str, List[str]]] = {
     "stream_ops": {"sources": ["stream_ops.cu"], "flags": [], "link": []},
     "step_inputs": {"sources": ["step_inputs.cu"], "flags": [], "link": []},
     "int8_cache": {"sources": ["int8_cache.cu"], "flags": [], "link": []},
-    "int8_attention": {"sources": ["int8_attention.cu"], "flags": [], "link": []},
+    "int8_attention": {"sources": ["int8_attention.cu", "int8_attention_tc.cu"], "flags": [], "link": []},
     "int8_linear": {"sources": ["int8_linear.cu"], "flags": [], "link": []},
     "random_fill": {"sources": ["random_fill.cu"], "flags": [], "link": []},
     # the host side's native core: no CUDA in it, so it is compiled by the C++ compiler alone

@@ -3,7 +3,7 @@
 //   s_ij = scale * ks_j * (q_i . kc_j),   o_i = sum_j softmax_j(s_ij) * vs_j * vc_j,   lse_i = ln sum_j exp(s_ij)
 // with codes kc, vc and their blocks' scales ks, vs.  The rows that keep account add exp(s_ij - lse_i), summed over the query
 // heads of a kv head, to the weight of key j.
-#include "common.cuh"
+#include "int8_attention.cuh"
 #include "tc_helpers.cuh"
 #include <cuda_fp16.h>
 #include <math.h>
@@ -11,25 +11,6 @@
 #include <type_traits>
 
 typedef __nv_bfloat16 bf16;
-
-constexpr int IA_PAGE = 64;
-
-struct IaArgs {
-    const void* q;                // [rows, ldq]
-    void* out;                    // [rows, ldo]
-    float* lse;                   // [rows, n_q]
-    const int8_t* k;
-    const int8_t* v;
-    const float* k_scale;
-    const float* v_scale;
-    float* weight;
-    const int* page_table;
-    const int* cu_new;
-    const int* seq_start;
-    const int* seq_slot;
-    int ldq, ldo, rows, n_seqs, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, shift, window, weigh_last;    // 1 << shift tokens a scale
-    float scale;
-};
 
 // ---- head sizes other than 64 and 128, and more than 32 query heads a kv head -------------------------------------------
 // Any head size that is a multiple of 16 up to 256: a warp a row and query head, words of four codes over its lanes.
@@ -976,6 +957,16 @@ static int ir_weigh(const IaArgs& a, int max_new, int* error_word, const CUtenso
     return 0;
 }
 
+static int ia_weigh(const IaArgs& a, bool wide, int max_new, int* error_word, const CUtensorMap& mk, cudaStream_t stream) {
+    const long long columns = (long long)std::min(a.weigh_last, max_new) * (a.n_q / a.n_kv);
+#define IR_WEIGH(N_, B_) \
+    return a.head_dim == 64 ? (wide ? ir_weigh<64, N_, B_, true>(a, max_new, error_word, mk, true, stream) : ir_weigh<64, N_, B_, false>(a, max_new, error_word, mk, true, stream)) \
+                            : (wide ? ir_weigh<128, N_, B_, true>(a, max_new, error_word, mk, true, stream) : ir_weigh<128, N_, B_, false>(a, max_new, error_word, mk, true, stream))
+    if (columns <= 8) IR_WEIGH(1, 1);
+    IR_WEIGH(4, 4);
+#undef IR_WEIGH
+}
+
 SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int ldo, float* lse, const void* k, const void* v,
                                const float* k_scale, const float* v_scale, float* weight, const int* page_table, int n_slots,
                                int max_pages, int n_pages, const int* cu_new, const int* seq_start, const int* seq_slot,
@@ -1001,10 +992,15 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
         }
         return ssb_launch_status();
     }
-    const bool wide = dtype == SSB_F32;
+    const bool wide = dtype == SSB_F32, prompt = ia_tc_takes(a, dtype, max_new);
     CUtensorMap mk, mv;
-    int rc = ir_map(&mk, k, (long long)n_pages * n_kv * 64, head_dim);
+    int rc = prompt && weigh_last <= 0 ? 0 : ir_map(&mk, k, (long long)n_pages * n_kv * 64, head_dim);
     if (rc) return rc;
+    if (prompt) {
+        rc = ia_tc_launch(a, max_new, error_word, stream);
+        if (rc || weigh_last <= 0) return rc;
+        return ia_weigh(a, wide, max_new, error_word, mk, stream);
+    }
     rc = ir_map(&mv, v, (long long)n_pages * n_kv * 64, head_dim);
     if (rc) return rc;
     if (!scratch) return SSB_ERR_BAD_SIZE;
@@ -1013,13 +1009,5 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
 #define IR_ROWS(H_, N_, W_) rc = ir_rows<H_, N_, W_>(a, p, scratch, error_word, mk, mv, stream)
     IR_EACH(head_dim, p.nt, wide, IR_ROWS);
 #undef IR_ROWS
-    if (rc || weigh_last <= 0) return rc;
-    const long long columns = (long long)std::min(weigh_last, max_new) * (n_q / n_kv);
-#define IR_WEIGH(N_, B_) \
-    rc = head_dim == 64 ? (wide ? ir_weigh<64, N_, B_, true>(a, max_new, error_word, mk, true, stream) : ir_weigh<64, N_, B_, false>(a, max_new, error_word, mk, true, stream)) \
-                        : (wide ? ir_weigh<128, N_, B_, true>(a, max_new, error_word, mk, true, stream) : ir_weigh<128, N_, B_, false>(a, max_new, error_word, mk, true, stream))
-    if (columns <= 8) IR_WEIGH(1, 1);
-    else IR_WEIGH(4, 4);
-#undef IR_WEIGH
-    return rc;
+    return rc || weigh_last <= 0 ? rc : ia_weigh(a, wide, max_new, error_word, mk, stream);
 }
