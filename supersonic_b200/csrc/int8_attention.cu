@@ -478,7 +478,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     // probabilities are summed times 2^OFFSET and may exceed that by 2^LAZY before the reference maximum is moved; with f below 2
     // and both in float16, 2^(OFFSET + LAZY + 1) stays below 2^16
-    constexpr float OFFSET = WIDE ? 13.f : 6.f, LAZY = WIDE ? 1.f : 8.f;
+    constexpr float OFFSET = WIDE ? 13.f : 2.f, LAZY = WIDE ? 1.f : 12.f;
     constexpr int C = 8 * NT, ACC_LD = ir_acc_ld<HD>(), TILES = HD / 16;
     using T = typename std::conditional<WIDE, float, bf16>::type;
     extern __shared__ unsigned char smem_raw[];
@@ -706,7 +706,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
 template <int HD, int NT, bool WIDE>
 __global__ void __launch_bounds__(IR_THREADS)
 int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __restrict__ pieces) {
-    constexpr float OFFSET = WIDE ? 13.f : 6.f;
+    constexpr float OFFSET = WIDE ? 13.f : 2.f;
     constexpr int C = 8 * NT;
     extern __shared__ unsigned char smem_raw[];
     long long* cum = (long long*)smem_raw;

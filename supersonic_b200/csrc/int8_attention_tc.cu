@@ -15,8 +15,8 @@
 //   scale, at no instruction more than the probability alone; a group's sum is divided by vs once before it counts in the
 //   denominator.  The maximum m is over s ks + log2 vs, so float16 holds what is summed whatever the scales are.
 //
-// The maximum is looked for only in a tile's first turn and when a turn's sum exceeds 2^14 (probabilities are held times 2^6, so
-// that is 2^8 times what a maximum of one would give); only then is O rescaled.  Every mbarrier wait is bounded.
+// A row's reference moves only when a maximum is 2^12 above it (float16 holds up to 2^16), and only then is O rescaled; what lies
+// 2^-14 below the reference is rounded to 2^-25 of it, and a sum is at least 2^-12 of the largest.  Every mbarrier wait is bounded.
 #include "int8_attention.cuh"
 #include "tc_helpers.cuh"
 #include <cuda_fp16.h>
@@ -28,7 +28,7 @@ typedef __nv_bfloat16 bf16;
 constexpr int IT_BM = 128, IT_BN = 128;    // query rows a tile, keys a turn
 constexpr int IT_SEQS = 512;               // sequences a launch: their table lies in shared memory
 constexpr int IT_SCALES = 4;               // turns whose scales are kept
-constexpr float IT_OFFSET = 6.f, IT_LAZY = 16384.f;
+constexpr float IT_LAZY = 12.f;            // how far, in the log2 domain, a maximum may rise above its row's reference
 constexpr float IT_LEAST = 7.888609052210118e-31f;
 struct ItSeq { int row0, n_new, start, slot; };
 struct ItTile { int row, head, p0, rows, turns; };
@@ -40,7 +40,7 @@ __host__ __device__ constexpr size_t it_smem(int tiles, int hd) {
            IT_BARS * 8 + 32 + 1024;
 }
 // Registers a thread of the three kinds of warps: 4 that control, 4 that convert, 4 a tile that take the softmax.
-constexpr int IT_REGS_CONTROL = 40, IT_REGS_CONVERT = 104;
+constexpr int IT_REGS_CONTROL = 48, IT_REGS_CONVERT = 96;
 __host__ __device__ constexpr int it_regs_softmax(int tiles) { return tiles == 2 ? 184 : 232; }
 
 __device__ __forceinline__ void it_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
@@ -77,6 +77,12 @@ __device__ __forceinline__ void it_st32(uint32_t taddr, const uint32_t* r) {
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                  : "memory");
 }
+__device__ __forceinline__ void it_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 __device__ __forceinline__ void it_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float it_ex2(float x) {
     float y;
@@ -86,6 +92,12 @@ __device__ __forceinline__ float it_ex2(float x) {
 // MN-major operand (values: [key][dim], dim contiguous) in 64-column boxes 8 KB apart, rows of 128 bytes with the 128-byte swizzle.
 __device__ __forceinline__ uint64_t it_desc_mn(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | (512ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// Codes pass through a block once: not by way of its L1, which is what shared memory leaves of it.
+__device__ __forceinline__ uint4 it_load_once(const int8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
 }
 // Two codes of a word as bfloat16 or float16.
 __device__ __forceinline__ uint32_t it_bf16(uint32_t w, uint32_t sel) {
@@ -350,7 +362,7 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {               // the first half of the pieces is the first page's
                     const int pg = i / (PIECES / 2), row = (i % (PIECES / 2)) * ROWS + row_of;
-                    r[i] = *reinterpret_cast<const uint4*>(codes + (((size_t)p[pg] * a.n_kv + kvh) * 64 + row) * HD + 16 * c);
+                    r[i] = it_load_once(codes + (((size_t)p[pg] * a.n_kv + kvh) * 64 + row) * HD + 16 * c);
                 }
             };
             auto fetch_scales = [&](const int (&p)[2]) {
@@ -452,71 +464,41 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                 const bool edge = key0 + IT_BN - 1 > p0 || window > 0;   // on the diagonal or at a window's edge
                 const int hi = pos - key0;                       // keys 0..hi of the turn are seen
                 const int lo = window > 0 ? hi - window + 1 : 0;
-                uint32_t raw[IT_BN];
+                // Two rounds over the scores, 32 at a time from tensor memory: their maximum, then their probabilities, written over
+                // scores that both rounds are done with.  Both are loops: unrolled, the warps' roles together outgrew the
+                // instruction cache, and times moved by a quarter with any change to the code.
+                auto scores = [&](int q, uint32_t (&v)[32]) {
+                    it_ld32(t_s + q * 32, v);
+                    it_ld_wait();
+                    if (edge) {
+                        const int top = hi - q * 32, bottom = lo - q * 32;
 #pragma unroll
-                for (int i = 0; i < IT_BN / 32; ++i) it_ld32(t_s + i * 32, raw + i * 32);
-                it_ld_wait();
-                if (edge) {
-#pragma unroll
-                    for (int i = 0; i < IT_BN; ++i)
-                        if (i > hi || i < lo) raw[i] = 0xff800000u;
-                }
-                // probabilities times their values' scale, as float16 over the scores in tensor memory; their sum, and beside
-                // it that of the probabilities
-                float denominator;
-                auto probabilities = [&](float ref) -> float {
-                    float total = 0.f;
-                    denominator = 0.f;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t packed[32];
-#pragma unroll
-                        for (int gr = 0; gr < 4; ++gr) {
-                            const float4 f = sc[half * 4 + gr];
-                            const float at = f.y - ref;
-                            float sum[2] = {0.f, 0.f};
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const float pa = it_ex2(fmaf(__uint_as_float(raw[half * 64 + gr * 16 + i]), f.x, at));
-                                const float pb = it_ex2(fmaf(__uint_as_float(raw[half * 64 + gr * 16 + i + 1]), f.x, at));
-                                sum[0] += pa;
-                                sum[1] += pb;
-                                const __half2 v = __floats2half2_rn(pa, pb);
-                                packed[gr * 8 + i / 2] = *reinterpret_cast<const uint32_t*>(&v);
-                            }
-                            const float both = sum[0] + sum[1];
-                            total += both;
-                            denominator = fmaf(both, f.z, denominator);
-                        }
-                        it_st32(t_s + half * 32, packed);
+                        for (int i = 0; i < 32; ++i)
+                            if (i > top || i < bottom) v[i] = 0xff800000u;
                     }
-                    return total;
                 };
-                // After a row's first turn the probabilities are taken against the reference as it stands, without looking for
-                // the turn's maximum first; a probability that exceeds what float16 has room for makes the sum exceed it too,
-                // and only then (or while a row has seen no key) is the maximum found, the output rescaled and the turn done again.
-                bool find_max = j == 0;
-                if (!find_max) {
-                    const float total = probabilities((m_ref == -INFINITY ? 0.f : m_ref) - IT_OFFSET);
-                    find_max = __any_sync(0xffffffffu, !(total <= IT_LAZY) || m_ref == -INFINITY);
-                }
-                if (find_max) {
-                    float m_new = m_ref;
+                float m_new = m_ref;
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t v[32];
+                    scores(q, v);
 #pragma unroll
-                    for (int gr = 0; gr < 8; ++gr) {
-                        const float4 f = sc[gr];
-                        float mx[2] = {-INFINITY, -INFINITY};
+                    for (int gr = 0; gr < 2; ++gr) {
+                        const float4 f = sc[q * 2 + gr];
+                        float mx = __uint_as_float(v[gr * 16]);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(raw[gr * 16 + i]));
-                        m_new = fmaxf(m_new, fmaf(fmaxf(mx[0], mx[1]), f.x, f.y));
+                        for (int i = 1; i < 15; i += 2) mx = fmaxf(fmaxf(mx, __uint_as_float(v[gr * 16 + i])), __uint_as_float(v[gr * 16 + i + 1]));
+                        mx = fmaxf(mx, __uint_as_float(v[gr * 16 + 15]));
+                        m_new = fmaxf(m_new, fmaf(mx, f.x, f.y));
                     }
-                    if (j > 0 && __any_sync(0xffffffffu, m_new > m_ref)) {
-                        // rescale what this warp's rows have summed so far to their new maxima
-                        bool wo = mbar_wait(o_full, (turn - 1) & 1, abort_flag);
-                        wo = __all_sync(0xffffffffu, wo);
-                        if (!wo) { ok = false; break; }
+                }
+                // The reference moves when a maximum is 2^12 above it, in the warp's 32 rows together; what was summed follows
+                if (__any_sync(0xffffffffu, m_new > m_ref + IT_LAZY)) {
+                    if (j > 0) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(o_full, (turn - 1) & 1, abort_flag));
+                        if (!ok) break;
                         tc_fence_after();
-                        const float alpha = (m_new == -INFINITY) ? 1.f : it_ex2(m_ref - m_new);
+                        const float alpha = m_new == -INFINITY ? 1.f : it_ex2(m_ref - m_new);
 #pragma unroll 1
                         for (int i = 0; i < HD / 32; ++i) {
                             uint32_t o[32];
@@ -529,14 +511,34 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                         l_run *= alpha;
                     }
                     m_ref = m_new;
-                    it_st_wait();                                // what was written against the old reference has landed
-                    probabilities((m_ref == -INFINITY ? 0.f : m_ref) - IT_OFFSET);
+                }
+                const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t v[32], packed[16];
+                    scores(q, v);
+#pragma unroll
+                    for (int gr = 0; gr < 2; ++gr) {
+                        const float4 f = sc[q * 2 + gr];
+                        const float at = f.y - ref;
+                        float sum[2] = {0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const float pa = it_ex2(fmaf(__uint_as_float(v[gr * 16 + i]), f.x, at));
+                            const float pb = it_ex2(fmaf(__uint_as_float(v[gr * 16 + i + 1]), f.x, at));
+                            sum[0] += pa;
+                            sum[1] += pb;
+                            const __half2 p = __floats2half2_rn(pa, pb);
+                            packed[gr * 8 + i / 2] = *reinterpret_cast<const uint32_t*>(&p);
+                        }
+                        l_run = fmaf(sum[0] + sum[1], f.z, l_run);
+                    }
+                    it_st16(t_s + q * 16, packed);
                 }
                 it_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) it_arrive(p_full);
-                l_run += denominator;
             }
             if (ok) {
                 bool w = mbar_wait(o_full, (turn - 1) & 1, abort_flag);
@@ -568,7 +570,7 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                     }
                 }
                 if (a.lse && r < tile.rows)
-                    a.lse[row * a.n_q + tile.head] = l_run == 0.f ? -INFINITY : (m_ref - IT_OFFSET + log2f(l_run)) * 0.6931471805599453f;
+                    a.lse[row * a.n_q + tile.head] = l_run == 0.f ? -INFINITY : (m_ref + log2f(l_run)) * 0.6931471805599453f;
             }
         }
     }
