@@ -18,6 +18,7 @@
 // A row's reference moves only when a maximum is 2^12 above it (float16 holds up to 2^16), and only then is O rescaled; what lies
 // 2^-14 below the reference is rounded to 2^-25 of it, and a sum is at least 2^-12 of the largest.  Every mbarrier wait is bounded.
 #include "int8_attention.cuh"
+#include "packed_f32.cuh"
 #include "tc_helpers.cuh"
 #include <cuda_fp16.h>
 #include <math.h>
@@ -520,18 +521,17 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
 #pragma unroll
                     for (int gr = 0; gr < 2; ++gr) {
                         const float4 f = sc[q * 2 + gr];
-                        const float at = f.y - ref;
-                        float sum[2] = {0.f, 0.f};
+                        const unsigned long long by = f2_twice(f.x), at = f2_twice(f.y - ref);
+                        unsigned long long sum = 0;
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            const float pa = it_ex2(fmaf(__uint_as_float(v[gr * 16 + i]), f.x, at));
-                            const float pb = it_ex2(fmaf(__uint_as_float(v[gr * 16 + i + 1]), f.x, at));
-                            sum[0] += pa;
-                            sum[1] += pb;
+                            const unsigned long long e = f2_fma(f2_pair(__uint_as_float(v[gr * 16 + i]), __uint_as_float(v[gr * 16 + i + 1])), by, at);
+                            const float pa = it_ex2(f2_lo(e)), pb = it_ex2(f2_hi(e));
+                            sum = f2_add(sum, f2_pair(pa, pb));
                             const __half2 p = __floats2half2_rn(pa, pb);
                             packed[gr * 8 + i / 2] = *reinterpret_cast<const uint32_t*>(&p);
                         }
-                        l_run = fmaf(sum[0] + sum[1], f.z, l_run);
+                        l_run = fmaf(f2_lo(sum) + f2_hi(sum), f.z, l_run);
                     }
                     it_st16(t_s + q * 16, packed);
                 }
