@@ -497,7 +497,6 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + IR_STAGES);
     const int block_at = (16 * warp) >> a.shift;                   // the warp's keys have one scale
-    ssb_pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < IR_STAGES; ++i) { mbar_init(full0 + 8 * i, 33); mbar_init(empty0 + 8 * i, IR_WARPS); }
         abort_flag[0] = 0;
@@ -506,6 +505,9 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
+    // dependents may start once all that came before this launch is done: they read the batch and the pages ahead of their own wait
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     const int blocks = ir_dealt(total);
     const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
@@ -727,14 +729,27 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     for (int e = threadIdx.x; e < C * (HD / 4); e += IR_THREADS) {
         const int col = e / (HD / 4), d = e % (HD / 4) * 4;
         float top = IR_NONE, sum = 0.f;
-        for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(piece(c) + C * HD + col));
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = c0; c <= c1; ++c) {
-            const float* p = piece(c);
-            const float mc = __ldcg(p + C * HD + col), by = ir_ex2(mc - top);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(p + col * HD + d));
-            v.x = fmaf(y.x, by, v.x); v.y = fmaf(y.y, by, v.y); v.z = fmaf(y.z, by, v.z); v.w = fmaf(y.w, by, v.w);
-            sum = fmaf(__ldcg(p + C * HD + C + col), by, sum);
+        constexpr int AT_ONCE = 4;                                 // pieces asked for together
+        for (int c = c0; c <= c1; c += AT_ONCE) {
+            float pm[AT_ONCE], pl[AT_ONCE];
+            float4 pv[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const float* p = piece(min(c + i, c1));
+                pm[i] = c + i <= c1 ? __ldcg(p + C * HD + col) : IR_NONE;
+                pl[i] = __ldcg(p + C * HD + C + col);
+                pv[i] = __ldcg(reinterpret_cast<const float4*>(p + col * HD + d));
+            }
+            const float now = fmaxf(top, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), keep = ir_ex2(top - now);
+            v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep; sum *= keep;
+            top = now;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const float by = c + i <= c1 ? ir_ex2(pm[i] - now) : 0.f;
+                v.x = fmaf(pv[i].x, by, v.x); v.y = fmaf(pv[i].y, by, v.y); v.z = fmaf(pv[i].z, by, v.z); v.w = fmaf(pv[i].w, by, v.w);
+                sum = fmaf(pl[i], by, sum);
+            }
         }
         ir_put<HD, WIDE>(a, seqs[seg.b], seg.tile, tts, seg.kvh, col, d, v, top, sum, OFFSET);
     }
@@ -926,8 +941,10 @@ template <int HD, int NT, bool WIDE>
 static int ir_rows(const IaArgs& a, const IrPlan& p, float* pieces, int* error_word, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
     for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
         const int n = std::min(IR_SEQS, a.n_seqs - s0);
-        int8_rows_kernel<HD, NT, WIDE><<<p.blocks, IR_THREADS, ir_smem<HD, NT>(n), stream>>>(a, s0, n, p.tts, pieces, error_word, mk, mv);
-        int rc = ssb_launch_status();
+        // not as a dependent of what came before: blocks that wait beside another launch's are dealt to SMs unevenly (64 sequences of
+        // 1 to 8,192 tokens, one call behind another: 111 us, 162 as dependents)
+        int rc = ssb_launch(int8_rows_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), ir_smem<HD, NT>(n), stream, false, a, s0, n, p.tts,
+                            pieces, error_word, mk, mv);
         if (rc) return rc;
         rc = ssb_launch(int8_finish_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IrSeq) + 8) + 8, stream, true,
                         a, s0, n, p.tts, (const float*)pieces);

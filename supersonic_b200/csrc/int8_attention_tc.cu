@@ -142,6 +142,8 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
     const int group = a.n_q / a.n_kv, window = a.window;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();                                 // dependents read the batch and the pages ahead of their own wait
     for (int b = threadIdx.x; b < n_seqs; b += it_threads(TILES)) {
         const int row0 = a.cu_new[s0 + b], n_new = a.cu_new[s0 + b + 1] - row0, start = a.seq_start[s0 + b];
         int slot = a.seq_slot[s0 + b];
@@ -173,7 +175,6 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    ssb_pdl_launch_dependents();
 
     // sequences without a slot: zeros
     for (int b = blockIdx.x; b < n_seqs; b += gridDim.x)
@@ -601,8 +602,8 @@ static int it_launch(const IaArgs& a, const CUtensorMap& mq, int s0, int n, int 
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
-    int8_attention_tc_kernel<HD, TILES><<<(unsigned)grid, it_threads(TILES), smem, stream>>>(a, mq, s0, n, levels, error_word);
-    return ssb_launch_status();
+    return ssb_launch(int8_attention_tc_kernel<HD, TILES>, dim3((unsigned)grid), dim3(it_threads(TILES)), smem, stream, true, a, mq, s0, n, levels,
+                      error_word);
 }
 
 int ia_tc_launch(const IaArgs& a, int max_new, int* error_word, cudaStream_t stream) {

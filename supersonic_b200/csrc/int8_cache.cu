@@ -10,6 +10,7 @@
 // The reference keeps keys in int8 and values in int4 for one of its lanes, a scale per block of tokens and channel
 // (kernels/certified_kv_bridge_cuda.cu:32-420); this cache has one scale per block of tokens and head, and both in int8.
 #include "common.cuh"
+#include <algorithm>
 
 typedef __nv_bfloat16 bf16;
 
@@ -42,12 +43,17 @@ __device__ __forceinline__ void i8_store8(float* p, const float (&x)[8]) {
 }
 // What of a number a code can stand for: NaN counts as zero, an infinity as 2^127 of its sign.
 __device__ __forceinline__ float i8_finite(float x) { return x != x ? 0.f : fminf(fmaxf(x, -I8_MOST), I8_MOST); }
-// Eight codes of eight numbers, and the values that the codes stand for.
-__device__ __forceinline__ uint2 i8_encode8(float (&x)[8], float scale) {
+// Eight codes of eight numbers, rint(x / scale), and the values that the codes stand for.  The division is correctly rounded: x
+// times the reciprocal is within 2e-5 of it (127 times two roundings), so only where that lies about half-way between two codes is
+// there anything to divide for.
+__device__ __forceinline__ uint2 i8_encode8(float (&x)[8], float scale, float inverse) {
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -127.f), 127.f);
+        const float y = x[i] * inverse;
+        float c = rintf(y);
+        if (fabsf(fabsf(y - c) - 0.5f) < 1e-4f) c = rintf(__fdiv_rn(x[i], scale));
+        c = fminf(fmaxf(c, -127.f), 127.f);
         w[i >> 2] |= (uint32_t)(uint8_t)(int8_t)(int)c << (8 * (i & 3));
         x[i] = __fmul_rn(c, scale);
     }
@@ -73,126 +79,157 @@ struct I8Append {
     int8_t* codes[2];             // keys, values
     float* scale[2];
     float* weight;                // or null
-    int ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block, span;
+    int ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block, chunk, kv_warps;
 };
 
-constexpr int I8_APPEND_THREADS = 128;
+constexpr int I8_APPEND_WARPS = 4, I8_Q_HEADS = 8;
 
-// A block of the grid takes ``span`` rows of one head.  16 numbers of a head are a lane's: 8 of its pairs' first and 8 of their
-// second members (or 16 that are not rotated), so a head of 128 is 8 lanes and the block works on 16 rows at a time.  A row that
-// begins a run (of consecutive places in one scale block) has the whole run quantised by its block: the numbers stay in
-// registers between the run's maximum and its codes, PASSES rows a lane.
-template <typename T, int PASSES>
-__global__ void __launch_bounds__(I8_APPEND_THREADS)
+// 16 numbers of a head are a lane's: 8 of its pairs' first and 8 of their second members (or 16 that are not rotated), so a head of
+// 128 is 8 lanes and a warp works on ROWS = 4 rows at a time.  Two kinds of warps:
+//  * keys and values: ``chunk`` rows of one head.  A row that begins a run (consecutive places in one scale block) has the whole run
+//    quantised by the warp that owns it, up to 4 ROWS rows in registers between their maximum and their codes, so nothing but the
+//    warp's own reduction stands between (a block a run spent its time in barriers and in asking 16 rows one after another
+//    whether they begin one: 18,000 rows of 48 heads 153 us).
+//  * queries: ROWS rows of up to 8 heads, the rotation tables' rows read once for all of them.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(32 * I8_APPEND_WARPS)
 int8_append_kernel(const I8Append a) {
-    const int head = blockIdx.y, hd = a.head_dim, lanes = hd / 16, at_once = I8_APPEND_THREADS / lanes;
-    const int l = threadIdx.x % lanes, r_of = threadIdx.x / lanes, half = a.rot / 2;
-    const bool turns = a.cos_t != nullptr && l < a.rot / 16 && head < a.n_q + a.n_kv;
+    constexpr int ROWS = 32 / LANES, KEEP = 4, HD = 16 * LANES;
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, l = lane % LANES, r_of = lane / LANES, half = a.rot / 2;
+    const bool turned = a.cos_t != nullptr && l < a.rot / 16;
     const int e0 = l < a.rot / 16 ? 8 * l : a.rot + 16 * (l - a.rot / 16), e1 = l < a.rot / 16 ? half + 8 * l : e0 + 8;
-    const int row0 = blockIdx.x * a.span;
-    const bool is_q = head < a.n_q;
-    const int which = head >= a.n_q + a.n_kv, kvh = head - a.n_q - which * a.n_kv;
-    __shared__ int run_len;
-    __shared__ float warp_max[I8_APPEND_THREADS / 32];
+    int w = blockIdx.x * I8_APPEND_WARPS + (threadIdx.x >> 5);
 
-    auto page_of = [&](int row) -> int {                      // or -1: a row without a place
-        const int s = a.slot[row], p = a.place[row];
+    auto page_of = [&](int s, int p) -> int {                 // or -1: no place
         if (s < 0 || s >= a.n_slots || p < 0 || (p >> 6) >= a.max_pages) return -1;
         const int page = a.page_table[(size_t)s * a.max_pages + (p >> 6)];
         return page < a.n_pages ? page : -1;
     };
-    auto load = [&](int row, float (&x)[8], float (&y)[8]) {
-        const T* src = (const T*)a.qkv + (size_t)row * a.ldq + (size_t)head * hd;
-        i8_load8(src + e0, x);
-        i8_load8(src + e1, y);
-        if (turns) {
-            const int p = a.pos[row];
-            if (p >= 0 && p < a.positions) {
-                float c[8], s[8];
-                i8_load8(a.cos_t + (size_t)p * half + e0, c);
-                i8_load8(a.sin_t + (size_t)p * half + e0, s);
+    auto tables = [&](int row, float (&c)[8], float (&s)[8]) -> bool {
+        const int p = turned ? a.pos[row] : -1;
+        if (p < 0 || p >= a.positions) return false;
+        i8_load8(a.cos_t + (size_t)p * half + e0, c);
+        i8_load8(a.sin_t + (size_t)p * half + e0, s);
+        return true;
+    };
+    auto turn = [&](float (&x)[8], float (&y)[8], const float (&c)[8], const float (&s)[8]) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float u = x[i], v = y[i];
-                    x[i] = __fsub_rn(__fmul_rn(u, c[i]), __fmul_rn(v, s[i]));
-                    y[i] = __fadd_rn(__fmul_rn(u, s[i]), __fmul_rn(v, c[i]));
-                }
-            }
+        for (int i = 0; i < 8; ++i) {
+            const float u = x[i], v = y[i];
+            x[i] = __fsub_rn(__fmul_rn(u, c[i]), __fmul_rn(v, s[i]));
+            y[i] = __fadd_rn(__fmul_rn(u, s[i]), __fmul_rn(v, c[i]));
         }
     };
-    auto store = [&](int row, const float (&x)[8], const float (&y)[8]) {
-        T* dst = (T*)a.out + (size_t)row * a.ldo + (size_t)head * hd;
-        i8_store8(dst + e0, x);
-        i8_store8(dst + e1, y);
-    };
-    if (is_q) {
-        for (int r = r_of; r < a.span && row0 + r < a.T; r += at_once) {
-            if (page_of(row0 + r) < 0) continue;
+    if (w >= a.kv_warps) {                                     // queries
+        w -= a.kv_warps;
+        const int blocks = (a.n_q + I8_Q_HEADS - 1) / I8_Q_HEADS, head0 = w % blocks * I8_Q_HEADS, row = w / blocks * ROWS + r_of;
+        if (row >= a.T || page_of(a.slot[row], a.place[row]) < 0) return;
+        float c[8], s[8];
+        const bool turns = tables(row, c, s);
+        const T* src = (const T*)a.qkv + (size_t)row * a.ldq;
+        T* dst = (T*)a.out + (size_t)row * a.ldo;
+#pragma unroll 4
+        for (int h = head0; h < min(head0 + I8_Q_HEADS, a.n_q); ++h) {
             float x[8], y[8];
-            load(row0 + r, x, y);
-            store(row0 + r, x, y);
+            i8_load8(src + h * HD + e0, x);
+            i8_load8(src + h * HD + e1, y);
+            if (turns) turn(x, y, c, s);
+            i8_store8(dst + h * HD + e0, x);
+            i8_store8(dst + h * HD + e1, y);
         }
         return;
     }
-    for (int r = 0; r < a.span && row0 + r < a.T; ++r) {
-        const int lead = row0 + r, page = page_of(lead);       // the same for the whole block
+    const int kv_heads = 2 * a.n_kv, which = w % kv_heads / a.n_kv, kvh = w % a.n_kv, head = a.n_q + which * a.n_kv + kvh;
+    const int row0 = w / kv_heads * a.chunk;
+    if (row0 >= a.T) return;
+    // which of the chunk's rows begin a run
+    unsigned leads;
+    {
+        const int row = row0 + lane;
+        bool lead = false;
+        if (lane < a.chunk && row < a.T) {
+            const int s = a.slot[row], p = a.place[row];
+            lead = s >= 0 && ((p & (a.block - 1)) == 0 || row == 0 || a.slot[row - 1] != s || a.place[row - 1] != p - 1);
+        }
+        leads = __ballot_sync(0xffffffffu, lead);
+    }
+    for (; leads; leads &= leads - 1) {
+        const int lead = row0 + __ffs(leads) - 1, s0 = a.slot[lead], p0 = a.place[lead], page = page_of(s0, p0);
         if (page < 0) continue;
-        const int p0 = a.place[lead], s0 = a.slot[lead], in_block = p0 & (a.block - 1);
-        if (in_block != 0 && lead > 0 && a.slot[lead - 1] == s0 && a.place[lead - 1] == p0 - 1) continue;    // inside a run
-        __syncthreads();
-        if (threadIdx.x == 0) run_len = a.block - in_block;
-        __syncthreads();
-        if ((int)threadIdx.x < a.block - in_block) {
-            const int row = lead + (int)threadIdx.x;
-            if (row >= a.T || a.slot[row] != s0 || a.place[row] != p0 + (int)threadIdx.x) atomicMin(&run_len, (int)threadIdx.x);
+        const int in_block = p0 & (a.block - 1), in_page = p0 & (I8_PAGE - 1), most_n = a.block - in_block;
+        int n = 0;
+        for (int i0 = 0; i0 < most_n; i0 += 32) {
+            const int i = i0 + lane, row = lead + i;
+            const unsigned on = __ballot_sync(0xffffffffu, i < most_n && row < a.T && a.slot[min(row, a.T - 1)] == s0 && a.place[min(row, a.T - 1)] == p0 + i);
+            n = i0 + (on == 0xffffffffu ? 32 : __ffs(~on) - 1);
+            if (on != 0xffffffffu) break;
         }
-        __syncthreads();
-        const int n = run_len;
-        float x[PASSES][8], y[PASSES][8], most = 0.f;
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int row = i * at_once + r_of;
-            if (row < n) {
-                load(lead + row, x[i], y[i]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[i][e] = i8_finite(x[i][e]);
-                    y[i][e] = i8_finite(y[i][e]);
-                    most = fmaxf(most, fmaxf(fabsf(x[i][e]), fabsf(y[i][e])));
-                }
-            }
-        }
-        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));      // not negative: the order of its bits
-        if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = most;
         const size_t head_at = (size_t)page * a.n_kv + kvh;
-        const int per = I8_PAGE / a.block, in_page = p0 & (I8_PAGE - 1);
+        const int per = I8_PAGE / a.block;
         float* scale_at = a.scale[which] + head_at * per + in_page / a.block;
         const float old = in_block ? *scale_at : 0.f;
-        __syncthreads();                                       // and the old scale has been read
+        float x[KEEP][8], y[KEEP][8], most = 0.f;
+        auto load = [&](int first) {                           // rows first .. first + KEEP ROWS - 1 of the run
 #pragma unroll
-        for (int w = 0; w < I8_APPEND_THREADS / 32; ++w) most = fmaxf(most, warp_max[w]);
-        const float now = fmaxf(fmaxf(old, __fmul_rn(most, 1.f / 127.f)), I8_LEAST_SCALE);
-        int8_t* codes = a.codes[which] + (head_at * I8_PAGE + in_page) * hd;
+            for (int i = 0; i < KEEP; ++i) {
+                const int row = first + i * ROWS + r_of;
+                if (row < n) {
+                    const T* src = (const T*)a.qkv + (size_t)(lead + row) * a.ldq + (size_t)head * HD;
+                    i8_load8(src + e0, x[i]);
+                    i8_load8(src + e1, y[i]);
+                }
+            }
+            if (!which) {
+#pragma unroll
+                for (int i = 0; i < KEEP; ++i) {
+                    const int row = first + i * ROWS + r_of;
+                    float c[8], s[8];
+                    if (row < n && tables(lead + row, c, s)) turn(x[i], y[i], c, s);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i)
+                if (first + i * ROWS + r_of < n)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[i][e] = i8_finite(x[i][e]);
+                        y[i][e] = i8_finite(y[i][e]);
+                        most = fmaxf(most, fmaxf(fabsf(x[i][e]), fabsf(y[i][e])));
+                    }
+        };
+        const int last = (n - 1) / (KEEP * ROWS) * (KEEP * ROWS);
+        for (int first = 0; first <= last; first += KEEP * ROWS) load(first);
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));      // not negative: the order of its bits
+        const float now = fmaxf(fmaxf(old, __fmul_rn(most, 1.f / 127.f)), I8_LEAST_SCALE), inverse = 1.f / now;
+        int8_t* codes = a.codes[which] + (head_at * I8_PAGE + in_page) * HD;
         if (in_block && now > old) {                           // the block's earlier codes under the larger scale
             const float ratio = __fdiv_rn(old, now);
-            for (int e = threadIdx.x; e < in_block * lanes; e += I8_APPEND_THREADS) {
-                uint4* at = reinterpret_cast<uint4*>(codes - (size_t)in_block * hd) + e;
+            for (int e = lane; e < in_block * LANES; e += 32) {
+                uint4* at = reinterpret_cast<uint4*>(codes - (size_t)in_block * HD) + e;
                 uint4 v = *at;
                 v.x = i8_rescale4(v.x, ratio); v.y = i8_rescale4(v.y, ratio); v.z = i8_rescale4(v.z, ratio); v.w = i8_rescale4(v.w, ratio);
                 *at = v;
             }
         }
+        for (int first = last; first >= 0; first -= KEEP * ROWS) {       // the last rows are still in registers
+            if (first != last) load(first);
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int row = i * at_once + r_of;
-            if (row < n) {
-                *reinterpret_cast<uint2*>(codes + (size_t)row * hd + e0) = i8_encode8(x[i], now);
-                *reinterpret_cast<uint2*>(codes + (size_t)row * hd + e1) = i8_encode8(y[i], now);
-                store(lead + row, x[i], y[i]);
+            for (int i = 0; i < KEEP; ++i) {
+                const int row = first + i * ROWS + r_of;
+                if (row < n) {
+                    *reinterpret_cast<uint2*>(codes + (size_t)row * HD + e0) = i8_encode8(x[i], now, inverse);
+                    *reinterpret_cast<uint2*>(codes + (size_t)row * HD + e1) = i8_encode8(y[i], now, inverse);
+                    T* dst = (T*)a.out + (size_t)(lead + row) * a.ldo + (size_t)head * HD;
+                    i8_store8(dst + e0, x[i]);
+                    i8_store8(dst + e1, y[i]);
+                }
             }
         }
-        if (threadIdx.x == 0) *scale_at = now;
-        if (a.weight && !which && (int)threadIdx.x < n) a.weight[head_at * I8_PAGE + in_page + threadIdx.x] = 0.f;
+        if (lane == 0) *scale_at = now;
+        if (a.weight && !which)
+            for (int i = lane; i < n; i += 32) a.weight[head_at * I8_PAGE + in_page + i] = 0.f;
     }
 }
 
@@ -201,28 +238,30 @@ SSB_API int ssb_int8_append(const void* qkv, int ldq, int dtype, void* out, int 
                             const int* page_table, int n_slots, int max_pages, void* k, void* v, float* k_scale, float* v_scale,
                             float* weight, int n_pages, int n_q, int n_kv, int head_dim, int block, cudaStream_t stream) {
     if (T <= 0) return 0;
-    const int lanes = head_dim / 16;
-    if (head_dim % 16 || lanes < 1 || lanes > 16 || (lanes & (lanes - 1)) || rot % 16 || rot > head_dim || n_kv <= 0 || n_q < 0 ||
-        (block != 16 && block != 32 && block != 64) || n_q + 2 * n_kv > 65535)
-        return SSB_ERR_BAD_SIZE;
+    if (rot % 16 || rot > head_dim || n_kv <= 0 || n_q < 0 || (block != 16 && block != 32 && block != 64)) return SSB_ERR_BAD_SIZE;
     I8Append a{qkv, out, cos_t, sin_t, pos, place, slot, page_table, {(int8_t*)k, (int8_t*)v}, {k_scale, v_scale}, weight,
-               ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block, 1};
-    // a block a row while there are few; else as many rows as a scale block has, so that hardly a block finds nothing to do
-    a.span = T <= 256 ? 1 : block;
-    const int passes = (block * lanes + I8_APPEND_THREADS - 1) / I8_APPEND_THREADS;
-    const dim3 grid((T + a.span - 1) / a.span, n_q + 2 * n_kv);
-#define I8_APPEND(P_) \
-    do { \
-        if (dtype == SSB_BF16) int8_append_kernel<bf16, P_><<<grid, I8_APPEND_THREADS, 0, stream>>>(a); \
-        else if (dtype == SSB_F32) int8_append_kernel<float, P_><<<grid, I8_APPEND_THREADS, 0, stream>>>(a); \
-        else return SSB_ERR_BAD_DTYPE; \
-    } while (0)
-    if (passes <= 1) I8_APPEND(1);
-    else if (passes <= 2) I8_APPEND(2);
-    else if (passes <= 4) I8_APPEND(4);
-    else I8_APPEND(8);
+               ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block};
+    // a warp a row while there are few; else a chunk of rows, of which two or so begin a run
+    a.chunk = T <= 256 ? 1 : 32;
+    const int rows = 32 / std::max(1, head_dim / 16);
+    const long long kv = (long long)((T + a.chunk - 1) / a.chunk) * 2 * n_kv;
+    const long long q = (long long)((T + rows - 1) / std::max(1, rows)) * ((n_q + I8_Q_HEADS - 1) / I8_Q_HEADS);
+    const long long blocks = (kv + q + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS;
+    if (blocks > 0x7fffffffLL || kv > 0x7fffffffLL) return SSB_ERR_BAD_SIZE;
+    a.kv_warps = (int)kv;
+    const dim3 grid((unsigned)blocks), threads(32 * I8_APPEND_WARPS);
+#define I8_APPEND(L_) \
+    return dtype == SSB_BF16 ? ssb_launch(int8_append_kernel<bf16, L_>, grid, threads, 0, stream, true, a) \
+         : dtype == SSB_F32 ? ssb_launch(int8_append_kernel<float, L_>, grid, threads, 0, stream, true, a) : (int)SSB_ERR_BAD_DTYPE
+    switch (head_dim) {
+        case 16: I8_APPEND(1);
+        case 32: I8_APPEND(2);
+        case 64: I8_APPEND(4);
+        case 128: I8_APPEND(8);
+        case 256: I8_APPEND(16);
+    }
 #undef I8_APPEND
-    return ssb_launch_status();
+    return SSB_ERR_BAD_SIZE;
 }
 
 // ---- values back ----------------------------------------------------------------------------------------------------
@@ -233,6 +272,8 @@ int8_read_kernel(const int8_t* __restrict__ k, const int8_t* __restrict__ v, con
                  const float* __restrict__ v_scale, const int* __restrict__ page_table, int n_slots, int max_pages, int n_pages,
                  const int* __restrict__ seq_slot, const int* __restrict__ lengths, T* __restrict__ k_out, T* __restrict__ v_out,
                  int most, int n_kv, int head_dim, int block) {
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
     const int lanes = head_dim / 16, b = blockIdx.y, which = blockIdx.z;
     const long long at = (long long)blockIdx.x * 256 + threadIdx.x;           // of the sequence's tokens, heads and lanes
     const int l = (int)(at % lanes), head = (int)(at / lanes % n_kv), i = (int)(at / lanes / n_kv);
@@ -263,13 +304,12 @@ SSB_API int ssb_int8_read(const void* k, const void* v, const float* k_scale, co
     if (blocks > 0x7fffffffLL || n_seqs > 65535) return SSB_ERR_BAD_SIZE;
     const dim3 grid((unsigned)blocks, n_seqs, 2);
 #define I8_READ(T_) \
-    int8_read_kernel<T_><<<grid, 256, 0, stream>>>((const int8_t*)k, (const int8_t*)v, k_scale, v_scale, page_table, n_slots, max_pages, \
-                                                   n_pages, seq_slot, lengths, (T_*)k_out, (T_*)v_out, most, n_kv, head_dim, block)
+    return ssb_launch(int8_read_kernel<T_>, grid, dim3(256), 0, stream, true, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, \
+                      page_table, n_slots, max_pages, n_pages, seq_slot, lengths, (T_*)k_out, (T_*)v_out, most, n_kv, head_dim, block)
     if (dtype == SSB_BF16) I8_READ(bf16);
-    else if (dtype == SSB_F32) I8_READ(float);
-    else return SSB_ERR_BAD_DTYPE;
+    if (dtype == SSB_F32) I8_READ(float);
 #undef I8_READ
-    return ssb_launch_status();
+    return SSB_ERR_BAD_DTYPE;
 }
 
 // ---- eviction -------------------------------------------------------------------------------------------------------
@@ -280,82 +320,135 @@ __device__ __forceinline__ uint32_t i8_rank(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int I8_SELECT_THREADS = 1024;
+constexpr int I8_SELECT_THREADS = 1024, I8_BINS = 2048;
+constexpr int I8_SELECT_KEYS = 32768;      // ranks a block keeps in shared memory; further ones are read again
+
+__device__ __forceinline__ int i8_cluster_int(const int* mine, unsigned rank) {
+    return __float_as_int(ssb_cluster_f32(reinterpret_cast<const float*>(mine), rank));
+}
 
 // kept[b, head] = the places that stay, in order: the first ``first``, the last ``recent``, and of the others the heaviest, equal
-// ones by their place; -1 behind them.  One block a (sequence, kv head): the rank of the last one that stays is found from its
-// highest byte to its lowest by counting, then one more pass writes places in order.
+// ones by their place; -1 behind them.  A cluster of 1, 4 or 8 blocks a (sequence, kv head), each with a run of whole pages of the
+// sequence: the rank of the last one that stays is found 11, 11 and 10 bits at a time, by counting (each block its own ranks, from
+// shared memory; every block adds the cluster's counts up for itself), then every block writes its places behind those of the
+// blocks before it.
 __global__ void __launch_bounds__(I8_SELECT_THREADS)
 int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ page_table, int n_slots, int max_pages, int n_pages,
                    const int* __restrict__ seq_slot, const int* __restrict__ lengths, int n_kv, int keep, int first, int recent,
-                   int* __restrict__ kept) {
-    const int b = blockIdx.x, head = blockIdx.y, s = seq_slot[b];
+                   int cluster, int held, int* __restrict__ kept) {
+    extern __shared__ uint32_t ranks[];
+    __shared__ int count[I8_BINS];
+    __shared__ int warp_sum[2][32];
+    __shared__ int chosen, still;
+    __shared__ int mine[2];                                    // this block's ties and sure ones
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
+    const int rank_in = cluster > 1 ? (int)ssb_cluster_rank() : 0, pair = blockIdx.x / cluster, b = pair / n_kv, head = pair % n_kv;
+    const int s = seq_slot[b], warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n = s < 0 || s >= n_slots ? 0 : min(lengths[b], max_pages * I8_PAGE);
     int* dst = kept + ((size_t)b * n_kv + head) * keep;
-    if (n <= keep) {
-        for (int i = threadIdx.x; i < keep; i += I8_SELECT_THREADS) dst[i] = i < n ? i : -1;
+    if (n <= keep) {                                           // the same for the whole cluster
+        for (int i = rank_in * I8_SELECT_THREADS + threadIdx.x; i < keep; i += cluster * I8_SELECT_THREADS) dst[i] = i < n ? i : -1;
         return;
     }
     const int* pt = page_table + (size_t)s * max_pages;
-    auto rank_of = [&](int j) {
+    const int pages = (n + I8_PAGE - 1) / I8_PAGE, share = (pages + cluster - 1) / cluster * I8_PAGE;
+    const int j0 = min(rank_in * share, n), j1 = min(j0 + share, n);        // this block's places
+    const int lo = first, hi = n - recent;                     // places that have to be chosen from
+    auto fetch = [&](int j) -> uint32_t {
         const int page = pt[j >> 6];
         return page < 0 || page >= n_pages ? 0u : i8_rank(weight[((size_t)page * n_kv + head) * I8_PAGE + (j & 63)]);
     };
-    __shared__ int count[256];
-    __shared__ int chosen_digit, still;
-    __shared__ int warp_sum[2][32];
-    const int lo = first, hi = n - recent, want = keep - first - recent;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t prefix = 0;
-    int left = want;                                           // of those with the prefix, how many stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (threadIdx.x < 256) count[threadIdx.x] = 0;
-        __syncthreads();
-        for (int j = lo + (int)threadIdx.x; j < hi; j += I8_SELECT_THREADS) {
+    for (int i = threadIdx.x; i < I8_BINS; i += I8_SELECT_THREADS) count[i] = 0;
+#pragma unroll 4
+    for (int j = j0 + (int)threadIdx.x; j < min(j1, j0 + held); j += I8_SELECT_THREADS) ranks[j - j0] = fetch(j);
+    __syncthreads();
+    auto rank_of = [&](int j) -> uint32_t { return j - j0 < held ? ranks[j - j0] : fetch(j); };
+
+    uint32_t prefix = 0;                                       // the bits found so far
+    int left = keep - first - recent;                          // of those with the prefix, how many stay
+    for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
+        const int bits = shift == 0 ? 10 : 11;
+        const uint32_t above = shift == 21 ? 0u : ~0u << (shift + bits);
+        for (int j = max(j0, lo) + (int)threadIdx.x; j < min(j1, hi); j += I8_SELECT_THREADS) {
             const uint32_t r = rank_of(j);
-            if (shift == 24 || (r >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&count[(r >> shift) & 255], 1);
+            if (((r ^ prefix) & above) == 0) atomicAdd(&count[(r >> shift) & ((1 << bits) - 1)], 1);
         }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int above = 0, d = 255;
-            for (; d > 0 && above + count[d] < left; --d) above += count[d];
-            chosen_digit = d;
-            still = left - above;
+        if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
+        // two bins a thread, the highest first: how many lie above them
+        const int top = I8_BINS - 1 - 2 * (int)threadIdx.x;
+        int c0 = count[top], c1 = count[top - 1];
+        if (cluster > 1) {
+            c0 = c1 = 0;
+            for (int r = 0; r < cluster; ++r) { c0 += i8_cluster_int(count + top, r); c1 += i8_cluster_int(count + top - 1, r); }
         }
+        int incl = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) warp_sum[0][warp] = incl;
         __syncthreads();
-        prefix |= (uint32_t)chosen_digit << shift;
-        left = still;
+        if (warp == 0) {
+            int v = warp_sum[0][lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            warp_sum[1][lane] = v;
+        }
+        if (threadIdx.x == 0) { chosen = 0; still = 0; }
         __syncthreads();
+        const int over = (warp ? warp_sum[1][warp - 1] : 0) + incl - c0 - c1;       // in the bins above these two
+        if (over < left && over + c0 >= left) { chosen = top; still = left - over; }
+        else if (over + c0 < left && over + c0 + c1 >= left) { chosen = top - 1; still = left - over - c0; }
+        if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
+        if (left > 0) { prefix |= (uint32_t)chosen << shift; left = still; }
+        else prefix = 0xffffffffu;                             // none of them stays
+        for (int i = threadIdx.x; i < I8_BINS; i += I8_SELECT_THREADS) count[i] = 0;
+        if (left <= 0) break;
+        if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
     }
-    // want 0: the loop above ends at the largest rank with none of it to take
-    int done = 0, equal = 0;                                   // places written, equal ones met
-    for (int j0 = 0; j0 < n; j0 += I8_SELECT_THREADS) {
-        const int j = j0 + (int)threadIdx.x;
-        const bool sure = j < n && (j < lo || j >= hi);
-        const uint32_t r = j < n && !sure ? rank_of(j) : 0u;
-        const bool tie = j < n && !sure && r == prefix;
-        const unsigned ties = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) warp_sum[0][warp] = __popc(ties);
-        __syncthreads();
-        int before = equal;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) before += warp_sum[0][w];
-            equal += warp_sum[0][w];
-        }
-        before += __popc(ties & ((1u << lane) - 1));
-        const bool stays = sure || (j < n && !sure && r > prefix) || (tie && before < left);
-        const unsigned all = __ballot_sync(0xffffffffu, stays);
-        if (lane == 0) warp_sum[1][warp] = __popc(all);
-        __syncthreads();
-        int at = done;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) at += warp_sum[1][w];
-            done += warp_sum[1][w];
-        }
-        at += __popc(all & ((1u << lane) - 1));
-        if (stays && at < keep) dst[at] = j;
-        __syncthreads();
+    // a warp a run of whole 32 places of the block: how many tie, how many stay for sure; then those before this block and warp
+    const int per_warp = ((j1 - j0 + 31) / 32 + 31) / 32 * 32, w0 = j0 + warp * per_warp, w1 = min(w0 + per_warp, j1);
+    auto look = [&](int j, bool& sure, bool& tie) {
+        const bool in = j < w1, free = in && j >= lo && j < hi;
+        const uint32_t r = free ? rank_of(j) : 0u;
+        tie = free && r == prefix && left > 0;
+        sure = in && (!free || r > prefix);
+    };
+    int ties = 0, sures = 0;
+    for (int j = w0; j < w1; j += 32) {
+        bool sure, tie;
+        look(j + lane, sure, tie);
+        ties += __popc(__ballot_sync(0xffffffffu, tie));
+        sures += __popc(__ballot_sync(0xffffffffu, sure));
     }
+    __syncthreads();
+    if (lane == 0) { warp_sum[0][warp] = ties; warp_sum[1][warp] = sures; }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        int sum = 0;
+        for (int w = 0; w < 32; ++w) sum += warp_sum[threadIdx.x][w];
+        mine[threadIdx.x] = sum;
+    }
+    if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
+    int ties_before = 0, sures_before = 0;
+    for (int r = 0; r < rank_in; ++r) { ties_before += i8_cluster_int(mine, r); sures_before += i8_cluster_int(mine + 1, r); }
+    for (int w = 0; w < warp; ++w) { ties_before += warp_sum[0][w]; sures_before += warp_sum[1][w]; }
+    for (int j = w0; j < w1; j += 32) {
+        bool sure, tie;
+        look(j + lane, sure, tie);
+        const unsigned t = __ballot_sync(0xffffffffu, tie), u = __ballot_sync(0xffffffffu, sure), below = (1u << lane) - 1;
+        const int tie_at = ties_before + __popc(t & below);
+        const int at = sures_before + __popc(u & below) + min(tie_at, left);
+        if ((sure || (tie && tie_at < left)) && at < keep) dst[at] = j + lane;
+        ties_before += __popc(t);
+        sures_before += __popc(u);
+    }
+    if (cluster > 1) ssb_cluster_sync();                       // no block leaves while another may read its counts
 }
 
 constexpr int I8_MOVE_THREADS = 256;
@@ -366,6 +459,8 @@ int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restri
                  float* __restrict__ weight, const int* __restrict__ page_table, int n_slots, int max_pages, int n_pages,
                  const int* __restrict__ seq_slot, const int* __restrict__ new_table, int new_pages, int n_kv, int head_dim, int block,
                  int keep, const int* __restrict__ kept) {
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
     const int to = blockIdx.x, head = blockIdx.y, b = blockIdx.z, s = seq_slot[b];
     if (s < 0 || s >= n_slots) return;
     const int target = new_table[(size_t)b * new_pages + to];
@@ -418,12 +513,22 @@ SSB_API int ssb_int8_evict(void* k, void* v, float* k_scale, float* v_scale, flo
     if (head_dim % 16 || head_dim <= 0 || n_kv <= 0 || (block != 16 && block != 32 && block != 64) || keep <= 0 || first < 0 ||
         recent < 0 || (long long)first + recent > keep || (long long)new_pages * I8_PAGE < keep || n_seqs > 65535 || n_kv > 65535)
         return SSB_ERR_BAD_SIZE;
-    int8_select_kernel<<<dim3(n_seqs, n_kv), I8_SELECT_THREADS, 0, stream>>>(weight, page_table, n_slots, max_pages, n_pages, seq_slot,
-                                                                             lengths, n_kv, keep, first, recent, kept);
-    int rc = ssb_launch_status();
+    // blocks a (sequence, kv head) by the longest sequence there can be
+    const long long longest = (long long)max_pages * I8_PAGE;
+    const int cluster = longest <= 8192 ? 1 : longest <= 32768 ? 4 : 8;
+    const int held = (int)std::min<long long>(I8_SELECT_KEYS, ((long long)max_pages + cluster - 1) / cluster * I8_PAGE);
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(int8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I8_SELECT_KEYS * 4);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    if ((long long)n_seqs * n_kv * cluster > 0x7fffffffLL) return SSB_ERR_BAD_SIZE;
+    int rc = ssb_launch_cluster(int8_select_kernel, dim3(n_seqs * n_kv * cluster), dim3(I8_SELECT_THREADS), (size_t)held * 4, stream, true, cluster,
+                                (const float*)weight, page_table, n_slots, max_pages, n_pages, seq_slot, lengths, n_kv, keep, first, recent, cluster,
+                                held, kept);
     if (rc) return rc;
-    int8_move_kernel<<<dim3((keep + I8_PAGE - 1) / I8_PAGE, n_kv, n_seqs), I8_MOVE_THREADS, 0, stream>>>(
-        (int8_t*)k, (int8_t*)v, k_scale, v_scale, weight, page_table, n_slots, max_pages, n_pages, seq_slot, new_table, new_pages,
-        n_kv, head_dim, block, keep, kept);
-    return ssb_launch_status();
+    return ssb_launch(int8_move_kernel, dim3((keep + I8_PAGE - 1) / I8_PAGE, n_kv, n_seqs), dim3(I8_MOVE_THREADS), 0, stream, true,
+                      (int8_t*)k, (int8_t*)v, k_scale, v_scale, weight, page_table, n_slots, max_pages, n_pages, seq_slot, new_table, new_pages,
+                      n_kv, head_dim, block, keep, (const int*)kept);
 }

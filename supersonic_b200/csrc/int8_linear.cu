@@ -58,7 +58,8 @@ __global__ void __launch_bounds__(1024)
 int8_quantize_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ codes, int ldc, float* __restrict__ scale, int K,
                      int* __restrict__ clear, int n_clear) {
     __shared__ float warp_max[32];
-    ssb_pdl_launch_dependents();
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
     const int row = blockIdx.x;
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n_clear; i += gridDim.x * blockDim.x) clear[i] = 0;
     float v[NV][8], most = 0.f;
@@ -92,7 +93,8 @@ __global__ void __launch_bounds__(256)
 int8_quantize_any_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ codes, int ldc, float* __restrict__ scale, int K,
                          int* __restrict__ clear, int n_clear) {
     __shared__ float warp_max[32];
-    ssb_pdl_launch_dependents();
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
     const T* src = x + (size_t)blockIdx.x * ldx;
     for (int i = blockIdx.x * 256 + threadIdx.x; i < n_clear; i += gridDim.x * 256) clear[i] = 0;
     float most = 0.f;
@@ -109,17 +111,15 @@ static int quantize_rows(const T* x, int ldx, int8_t* codes, int ldc, float* sca
     const bool whole = K % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)codes & 7) == 0 && ((size_t)ldx * sizeof(T)) % 16 == 0 &&
                        ((uintptr_t)x & 15) == 0 && K <= 8 * 4 * 1024;
     if (!whole) {
-        int8_quantize_any_kernel<T><<<rows, 256, 0, stream>>>(x, ldx, codes, ldc, scale, K, clear, n_clear);
-        return ssb_launch_status();
+        return ssb_launch(int8_quantize_any_kernel<T>, dim3(rows), dim3(256), 0, stream, true, x, ldx, codes, ldc, scale, K, clear, n_clear);
     }
     const int vectors = K / 8;
     // few rows: as many threads as there are vectors, for the shortest way through; many: two vectors a thread
     const int threads = std::min(1024, std::max(32, ((rows > 256 ? (vectors + 1) / 2 : vectors) + 31) / 32 * 32));
     const int nv = (vectors + threads - 1) / threads;
-    if (nv == 1) int8_quantize_kernel<T, 1><<<rows, threads, 0, stream>>>(x, ldx, codes, ldc, scale, K, clear, n_clear);
-    else if (nv == 2) int8_quantize_kernel<T, 2><<<rows, threads, 0, stream>>>(x, ldx, codes, ldc, scale, K, clear, n_clear);
-    else int8_quantize_kernel<T, 4><<<rows, threads, 0, stream>>>(x, ldx, codes, ldc, scale, K, clear, n_clear);
-    return ssb_launch_status();
+    if (nv == 1) return ssb_launch(int8_quantize_kernel<T, 1>, dim3(rows), dim3(threads), 0, stream, true, x, ldx, codes, ldc, scale, K, clear, n_clear);
+    if (nv == 2) return ssb_launch(int8_quantize_kernel<T, 2>, dim3(rows), dim3(threads), 0, stream, true, x, ldx, codes, ldc, scale, K, clear, n_clear);
+    return ssb_launch(int8_quantize_kernel<T, 4>, dim3(rows), dim3(threads), 0, stream, true, x, ldx, codes, ldc, scale, K, clear, n_clear);
 }
 
 SSB_API int ssb_int8_quantize_rows(const void* x, int ldx, int dtype, void* codes, int ldc, float* scale, int rows, int K,
