@@ -9,56 +9,13 @@
 //
 // The reference keeps keys in int8 and values in int4 for one of its lanes, a scale per block of tokens and channel
 // (kernels/certified_kv_bridge_cuda.cu:32-420); this cache has one scale per block of tokens and head, and both in int8.
-#include "common.cuh"
+#include "int8_codes.cuh"
 #include <algorithm>
 
 typedef __nv_bfloat16 bf16;
 
-constexpr float I8_LEAST_SCALE = 7.888609052210118e-31f;        // 2^-100: a block of zeros has a scale too
-constexpr float I8_MOST = 1.7014118346046923e38f;               // 2^127: its largest code still stands for a finite number
 constexpr int I8_PAGE = 64;
 
-__device__ __forceinline__ void i8_load8(const bf16* p, float (&x)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ void i8_load8(const float* p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void i8_store8(bf16* p, const float (&x)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void i8_store8(float* p, const float (&x)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-// What of a number a code can stand for: NaN counts as zero, an infinity as 2^127 of its sign.
-__device__ __forceinline__ float i8_finite(float x) { return x != x ? 0.f : fminf(fmaxf(x, -I8_MOST), I8_MOST); }
-// Eight codes of eight numbers, rint(x / scale), and the values that the codes stand for.  The division is correctly rounded: x
-// times the reciprocal is within 2e-5 of it (127 times two roundings), so only where that lies about half-way between two codes is
-// there anything to divide for.
-__device__ __forceinline__ uint2 i8_encode8(float (&x)[8], float scale, float inverse) {
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = x[i] * inverse;
-        float c = rintf(y);
-        if (fabsf(fabsf(y - c) - 0.5f) < 1e-4f) c = rintf(__fdiv_rn(x[i], scale));
-        c = fminf(fmaxf(c, -127.f), 127.f);
-        w[i >> 2] |= (uint32_t)(uint8_t)(int8_t)(int)c << (8 * (i & 3));
-        x[i] = __fmul_rn(c, scale);
-    }
-    return make_uint2(w[0], w[1]);
-}
 __device__ __forceinline__ int i8_code(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
 __device__ __forceinline__ uint32_t i8_rescale4(uint32_t w, float ratio) {
     uint32_t r = 0;
@@ -91,8 +48,9 @@ constexpr int I8_APPEND_WARPS = 4, I8_Q_HEADS = 8;
 //    warp's own reduction stands between (a block a run spent its time in barriers and in asking 16 rows one after another
 //    whether they begin one: 18,000 rows of 48 heads 153 us).
 //  * queries: ROWS rows of up to 8 heads, the rotation tables' rows read once for all of them.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(32 * I8_APPEND_WARPS)
+// KV, Q: which kinds of warps the launch has; where there are many rows each kind has a launch of its own, and its own number of registers.
+template <typename T, int LANES, bool KV, bool Q>
+__global__ void __launch_bounds__(32 * I8_APPEND_WARPS, KV ? 4 : 8)
 int8_append_kernel(const I8Append a) {
     constexpr int ROWS = 32 / LANES, KEEP = 4, HD = 16 * LANES;
     ssb_pdl_wait();
@@ -107,9 +65,8 @@ int8_append_kernel(const I8Append a) {
         const int page = a.page_table[(size_t)s * a.max_pages + (p >> 6)];
         return page < a.n_pages ? page : -1;
     };
-    auto tables = [&](int row, float (&c)[8], float (&s)[8]) -> bool {
-        const int p = turned ? a.pos[row] : -1;
-        if (p < 0 || p >= a.positions) return false;
+    auto tables = [&](int p, float (&c)[8], float (&s)[8]) -> bool {
+        if (!turned || p < 0 || p >= a.positions) return false;
         i8_load8(a.cos_t + (size_t)p * half + e0, c);
         i8_load8(a.sin_t + (size_t)p * half + e0, s);
         return true;
@@ -122,14 +79,16 @@ int8_append_kernel(const I8Append a) {
             y[i] = __fadd_rn(__fmul_rn(u, s[i]), __fmul_rn(v, c[i]));
         }
     };
-    if (w >= a.kv_warps) {                                     // queries
-        w -= a.kv_warps;
+    if (Q && (!KV || w >= a.kv_warps)) {                       // queries
+        if (KV) w -= a.kv_warps;
         const int blocks = (a.n_q + I8_Q_HEADS - 1) / I8_Q_HEADS, head0 = w % blocks * I8_Q_HEADS, row = w / blocks * ROWS + r_of;
-        if (row >= a.T || page_of(a.slot[row], a.place[row]) < 0) return;
+        if (row >= a.T) return;
+        const int sl = a.slot[row], pl = a.place[row];
         float c[8], s[8];
-        const bool turns = tables(row, c, s);
+        const bool turns = tables(turned ? a.pos[row] : -1, c, s);
         const T* src = (const T*)a.qkv + (size_t)row * a.ldq;
         T* dst = (T*)a.out + (size_t)row * a.ldo;
+        if (sl < 0 || sl >= a.n_slots || pl < 0 || (pl >> 6) >= a.max_pages) return;
 #pragma unroll 4
         for (int h = head0; h < min(head0 + I8_Q_HEADS, a.n_q); ++h) {
             float x[8], y[8];
@@ -141,36 +100,52 @@ int8_append_kernel(const I8Append a) {
         }
         return;
     }
+    if (!KV) return;
     const int kv_heads = 2 * a.n_kv, which = w % kv_heads / a.n_kv, kvh = w % a.n_kv, head = a.n_q + which * a.n_kv + kvh;
     const int row0 = w / kv_heads * a.chunk;
     if (row0 >= a.T) return;
-    // which of the chunk's rows begin a run
-    unsigned leads;
+    // a row a lane: its place, and whether it goes on from the row before it or begins a run
+    int my_slot = -1, my_place = -1, my_pos = -1, my_page = -1;
+    unsigned leads, goes_on;
     {
         const int row = row0 + lane;
-        bool lead = false;
+        bool lead = false, on = false;
         if (lane < a.chunk && row < a.T) {
-            const int s = a.slot[row], p = a.place[row];
-            lead = s >= 0 && ((p & (a.block - 1)) == 0 || row == 0 || a.slot[row - 1] != s || a.place[row - 1] != p - 1);
+            my_slot = a.slot[row];
+            my_place = a.place[row];
+            my_pos = a.cos_t != nullptr && !which ? a.pos[row] : -1;
+            on = row > 0 && (my_place & (a.block - 1)) != 0 && a.slot[row - 1] == my_slot && a.place[row - 1] == my_place - 1;
+            lead = my_slot >= 0 && !on;
+            my_page = page_of(my_slot, my_place);
         }
         leads = __ballot_sync(0xffffffffu, lead);
+        goes_on = __ballot_sync(0xffffffffu, on);
     }
     for (; leads; leads &= leads - 1) {
-        const int lead = row0 + __ffs(leads) - 1, s0 = a.slot[lead], p0 = a.place[lead], page = page_of(s0, p0);
+        const int at = __ffs(leads) - 1, lead = row0 + at;
+        const int s0 = __shfl_sync(0xffffffffu, my_slot, at), p0 = __shfl_sync(0xffffffffu, my_place, at), page = __shfl_sync(0xffffffffu, my_page, at);
         if (page < 0) continue;
         const int in_block = p0 & (a.block - 1), in_page = p0 & (I8_PAGE - 1), most_n = a.block - in_block;
-        int n = 0;
-        for (int i0 = 0; i0 < most_n; i0 += 32) {
-            const int i = i0 + lane, row = lead + i;
-            const unsigned on = __ballot_sync(0xffffffffu, i < most_n && row < a.T && a.slot[min(row, a.T - 1)] == s0 && a.place[min(row, a.T - 1)] == p0 + i);
-            n = i0 + (on == 0xffffffffu ? 32 : __ffs(~on) - 1);
-            if (on != 0xffffffffu) break;
+        // rows that go on from the first: in the chunk by its lanes, behind it (a run may cross its end) by asking
+        const unsigned after = at == 31 ? 0u : goes_on >> (at + 1);
+        int n = 1 + (~after ? __ffs(~after) - 1 : 32);
+        if (at + n >= a.chunk) {
+            n = a.chunk - at;
+            for (bool more = n < most_n; more;) {
+                const int i = n + lane, row = lead + i;
+                const unsigned on = __ballot_sync(0xffffffffu, i < most_n && row < a.T && a.slot[min(row, a.T - 1)] == s0 && a.place[min(row, a.T - 1)] == p0 + i);
+                const int got = on == 0xffffffffu ? 32 : __ffs(~on) - 1;
+                n += got;
+                more = got == 32 && n < most_n;
+            }
         }
         const size_t head_at = (size_t)page * a.n_kv + kvh;
         const int per = I8_PAGE / a.block;
         float* scale_at = a.scale[which] + head_at * per + in_page / a.block;
         const float old = in_block ? *scale_at : 0.f;
-        float x[KEEP][8], y[KEEP][8], most = 0.f;
+        float x[KEEP][8], y[KEEP][8];
+        uint32_t top = 0;
+        bool wild = false;                                     // a number of the run is none, or too large
         auto load = [&](int first) {                           // rows first .. first + KEEP ROWS - 1 of the run
 #pragma unroll
             for (int i = 0; i < KEEP; ++i) {
@@ -184,24 +159,31 @@ int8_append_kernel(const I8Append a) {
             if (!which) {
 #pragma unroll
                 for (int i = 0; i < KEEP; ++i) {
-                    const int row = first + i * ROWS + r_of;
+                    const int row = first + i * ROWS + r_of, known = __shfl_sync(0xffffffffu, my_pos, (at + row) & 31);
                     float c[8], s[8];
-                    if (row < n && tables(lead + row, c, s)) turn(x[i], y[i], c, s);
+                    if (row < n && tables(at + row < a.chunk ? known : turned ? a.pos[lead + row] : -1, c, s)) turn(x[i], y[i], c, s);
                 }
             }
 #pragma unroll
             for (int i = 0; i < KEEP; ++i)
-                if (first + i * ROWS + r_of < n)
+                if (first + i * ROWS + r_of < n) {
+                    if (wild) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[i][e] = i8_finite(x[i][e]);
-                        y[i][e] = i8_finite(y[i][e]);
-                        most = fmaxf(most, fmaxf(fabsf(x[i][e]), fabsf(y[i][e])));
+                        for (int e = 0; e < 8; ++e) { x[i][e] = i8_finite(x[i][e]); y[i][e] = i8_finite(y[i][e]); }
                     }
+                    top = max(top, max(i8_magnitude(x[i]), i8_magnitude(y[i])));
+                }
         };
         const int last = (n - 1) / (KEEP * ROWS) * (KEEP * ROWS);
         for (int first = 0; first <= last; first += KEEP * ROWS) load(first);
-        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));      // not negative: the order of its bits
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (top >= I8_WILD) {
+            wild = true;
+            top = 0;
+            for (int first = 0; first <= last; first += KEEP * ROWS) load(first);
+            top = __reduce_max_sync(0xffffffffu, top);
+        }
+        const float most = __uint_as_float(top);
         const float now = fmaxf(fmaxf(old, __fmul_rn(most, 1.f / 127.f)), I8_LEAST_SCALE), inverse = 1.f / now;
         int8_t* codes = a.codes[which] + (head_at * I8_PAGE + in_page) * HD;
         if (in_block && now > old) {                           // the block's earlier codes under the larger scale
@@ -242,17 +224,25 @@ SSB_API int ssb_int8_append(const void* qkv, int ldq, int dtype, void* out, int 
     I8Append a{qkv, out, cos_t, sin_t, pos, place, slot, page_table, {(int8_t*)k, (int8_t*)v}, {k_scale, v_scale}, weight,
                ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block};
     // a warp a row while there are few; else a chunk of rows, of which two or so begin a run
-    a.chunk = T <= 256 ? 1 : 32;
+    const bool many = T > 256;
+    a.chunk = many ? std::min(block, 32) : 1;
     const int rows = 32 / std::max(1, head_dim / 16);
     const long long kv = (long long)((T + a.chunk - 1) / a.chunk) * 2 * n_kv;
     const long long q = (long long)((T + rows - 1) / std::max(1, rows)) * ((n_q + I8_Q_HEADS - 1) / I8_Q_HEADS);
     const long long blocks = (kv + q + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS;
     if (blocks > 0x7fffffffLL || kv > 0x7fffffffLL) return SSB_ERR_BAD_SIZE;
     a.kv_warps = (int)kv;
-    const dim3 grid((unsigned)blocks), threads(32 * I8_APPEND_WARPS);
+    const dim3 threads(32 * I8_APPEND_WARPS), kv_grid((unsigned)((kv + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS)),
+        q_grid((unsigned)((q + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS));
+    int rc = 0;
+#define I8_LAUNCH(T_, L_) \
+    if (!many) return ssb_launch(int8_append_kernel<T_, L_, true, true>, dim3((unsigned)blocks), threads, 0, stream, true, a); \
+    rc = ssb_launch(int8_append_kernel<T_, L_, true, false>, kv_grid, threads, 0, stream, true, a); \
+    return rc || q == 0 ? rc : ssb_launch(int8_append_kernel<T_, L_, false, true>, q_grid, threads, 0, stream, true, a)
 #define I8_APPEND(L_) \
-    return dtype == SSB_BF16 ? ssb_launch(int8_append_kernel<bf16, L_>, grid, threads, 0, stream, true, a) \
-         : dtype == SSB_F32 ? ssb_launch(int8_append_kernel<float, L_>, grid, threads, 0, stream, true, a) : (int)SSB_ERR_BAD_DTYPE
+    if (dtype == SSB_BF16) { I8_LAUNCH(bf16, L_); } \
+    if (dtype == SSB_F32) { I8_LAUNCH(float, L_); } \
+    return SSB_ERR_BAD_DTYPE
     switch (head_dim) {
         case 16: I8_APPEND(1);
         case 32: I8_APPEND(2);
@@ -261,6 +251,7 @@ SSB_API int ssb_int8_append(const void* qkv, int ldq, int dtype, void* out, int 
         case 256: I8_APPEND(16);
     }
 #undef I8_APPEND
+#undef I8_LAUNCH
     return SSB_ERR_BAD_SIZE;
 }
 
@@ -274,7 +265,7 @@ int8_read_kernel(const int8_t* __restrict__ k, const int8_t* __restrict__ v, con
                  int most, int n_kv, int head_dim, int block) {
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
-    const int lanes = head_dim / 16, b = blockIdx.y, which = blockIdx.z;
+    const int lanes = head_dim / 16, b = blockIdx.y;
     const long long at = (long long)blockIdx.x * 256 + threadIdx.x;           // of the sequence's tokens, heads and lanes
     const int l = (int)(at % lanes), head = (int)(at / lanes % n_kv), i = (int)(at / lanes / n_kv);
     const int s = seq_slot[b], n = min(min(lengths[b], most), max_pages * I8_PAGE);
@@ -282,16 +273,19 @@ int8_read_kernel(const int8_t* __restrict__ k, const int8_t* __restrict__ v, con
     const int page = page_table[(size_t)s * max_pages + (i >> 6)];
     if (page < 0 || page >= n_pages) return;
     const size_t row = ((size_t)page * n_kv + head) * I8_PAGE + (i & 63);
-    const float scale = (which ? v_scale : k_scale)[row / block];
-    const uint4 c = reinterpret_cast<const uint4*>((which ? v : k) + row * head_dim)[l];
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    T* dst = (which ? v_out : k_out) + (((size_t)b * most + i) * n_kv + head) * head_dim + 16 * l;
+    const uint4 c[2] = {reinterpret_cast<const uint4*>(k + row * head_dim)[l], reinterpret_cast<const uint4*>(v + row * head_dim)[l]};
+    const float scale[2] = {k_scale[row / block], v_scale[row / block]};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float x[8];
+    for (int which = 0; which < 2; ++which) {
+        const uint32_t w[4] = {c[which].x, c[which].y, c[which].z, c[which].w};
+        T* dst = (which ? v_out : k_out) + (((size_t)b * most + i) * n_kv + head) * head_dim + 16 * l;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)i8_code(w[2 * h + (e >> 2)], e & 3), scale);
-        i8_store8(dst + 8 * h, x);
+        for (int h = 0; h < 2; ++h) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)i8_code(w[2 * h + (e >> 2)], e & 3), scale[which]);
+            i8_store8(dst + 8 * h, x);
+        }
     }
 }
 
@@ -302,7 +296,7 @@ SSB_API int ssb_int8_read(const void* k, const void* v, const float* k_scale, co
     if (head_dim % 16 || head_dim <= 0 || n_kv <= 0 || (block != 16 && block != 32 && block != 64)) return SSB_ERR_BAD_SIZE;
     const long long blocks = ((long long)most * n_kv * (head_dim / 16) + 255) / 256;
     if (blocks > 0x7fffffffLL || n_seqs > 65535) return SSB_ERR_BAD_SIZE;
-    const dim3 grid((unsigned)blocks, n_seqs, 2);
+    const dim3 grid((unsigned)blocks, n_seqs);
 #define I8_READ(T_) \
     return ssb_launch(int8_read_kernel<T_>, grid, dim3(256), 0, stream, true, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, \
                       page_table, n_slots, max_pages, n_pages, seq_slot, lengths, (T_*)k_out, (T_*)v_out, most, n_kv, head_dim, block)
@@ -320,24 +314,32 @@ __device__ __forceinline__ uint32_t i8_rank(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int I8_SELECT_THREADS = 1024, I8_BINS = 2048;
-constexpr int I8_SELECT_KEYS = 32768;      // ranks a block keeps in shared memory; further ones are read again
+constexpr int I8_SELECT_THREADS = 512, I8_SELECT_WARPS = I8_SELECT_THREADS / 32, I8_BINS = 2048;
+constexpr int I8_SELECT_KEEP = 16384;      // ranks a block keeps in shared memory; further ones are read again
 
+__device__ __forceinline__ int4 i8_cluster_int4(const int* mine, unsigned rank) {
+    uint32_t remote;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote) : "memory");
+    return v;
+}
 __device__ __forceinline__ int i8_cluster_int(const int* mine, unsigned rank) {
     return __float_as_int(ssb_cluster_f32(reinterpret_cast<const float*>(mine), rank));
 }
 
 // kept[b, head] = the places that stay, in order: the first ``first``, the last ``recent``, and of the others the heaviest, equal
 // ones by their place; -1 behind them.  A cluster of 1, 4 or 8 blocks a (sequence, kv head), each with a run of whole pages of the
-// sequence: the rank of the last one that stays is found 11, 11 and 10 bits at a time, by counting (each block its own ranks, from
-// shared memory; every block adds the cluster's counts up for itself), then every block writes its places behind those of the
-// blocks before it.
-__global__ void __launch_bounds__(I8_SELECT_THREADS)
+// sequence and each warp with a run of whole 32 places of its block's: the rank of the last one that stays is found 11, 11 and 10 bits
+// at a time, by counting (every block adds the cluster's counts up for itself), then every warp writes its places behind those of the
+// warps and blocks before it.  Ranks lie in shared memory and the loops over them stay loops: 32 ranks a thread in registers, every
+// loop unrolled, is code that runs once, and took longer to fetch than to run (sequences of 700 tokens 9 us and 32).
+__global__ void __launch_bounds__(I8_SELECT_THREADS, 2)
 int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ page_table, int n_slots, int max_pages, int n_pages,
                    const int* __restrict__ seq_slot, const int* __restrict__ lengths, int n_kv, int keep, int first, int recent,
                    int cluster, int held, int* __restrict__ kept) {
     extern __shared__ uint32_t ranks[];
-    __shared__ int count[I8_BINS];
+    __shared__ __align__(16) int count[I8_BINS], total[I8_BINS];
     __shared__ int warp_sum[2][32];
     __shared__ int chosen, still;
     __shared__ int mine[2];                                    // this block's ties and sure ones
@@ -359,30 +361,49 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
         const int page = pt[j >> 6];
         return page < 0 || page >= n_pages ? 0u : i8_rank(weight[((size_t)page * n_kv + head) * I8_PAGE + (j & 63)]);
     };
+    const int per_warp = ((j1 - j0 + I8_SELECT_WARPS - 1) / I8_SELECT_WARPS + 31) / 32 * 32, w0 = min(j0 + warp * per_warp, j1), w1 = min(w0 + per_warp, j1);
     for (int i = threadIdx.x; i < I8_BINS; i += I8_SELECT_THREADS) count[i] = 0;
-#pragma unroll 4
-    for (int j = j0 + (int)threadIdx.x; j < min(j1, j0 + held); j += I8_SELECT_THREADS) ranks[j - j0] = fetch(j);
+    const int kept_in = min(held / I8_SELECT_WARPS / 32 * 32, per_warp);     // of the warp's places, in shared memory
+    uint32_t* own = ranks + warp * kept_in;
+#pragma unroll 8
+    for (int j = w0 + lane; j < min(w0 + kept_in, w1); j += 32) own[j - w0] = fetch(j);
     __syncthreads();
-    auto rank_of = [&](int j) -> uint32_t { return j - j0 < held ? ranks[j - j0] : fetch(j); };
+    // f(place, rank) for each of the warp's places, 32 at a time
+    auto each = [&](auto&& f) {
+        for (int j = w0 + lane; j - lane < w1; j += 32) f(j, j >= w1 ? 0u : j - w0 < kept_in ? own[j - w0] : fetch(j));
+    };
 
     uint32_t prefix = 0;                                       // the bits found so far
     int left = keep - first - recent;                          // of those with the prefix, how many stay
     for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
         const int bits = shift == 0 ? 10 : 11;
         const uint32_t above = shift == 21 ? 0u : ~0u << (shift + bits);
-        for (int j = max(j0, lo) + (int)threadIdx.x; j < min(j1, hi); j += I8_SELECT_THREADS) {
-            const uint32_t r = rank_of(j);
-            if (((r ^ prefix) & above) == 0) atomicAdd(&count[(r >> shift) & ((1 << bits) - 1)], 1);
-        }
+        each([&](int j, uint32_t r) {
+            if (((r ^ prefix) & above) == 0 && j >= lo && j < min(w1, hi)) atomicAdd(&count[(r >> shift) & ((1 << bits) - 1)], 1);
+        });
         if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
-        // two bins a thread, the highest first: how many lie above them
-        const int top = I8_BINS - 1 - 2 * (int)threadIdx.x;
-        int c0 = count[top], c1 = count[top - 1];
+        // four bins a thread, the highest first: how many lie above them.  In a cluster every block adds up its share of the bins over
+        // the blocks and fetches the other shares' totals (each adding all of them up for itself moved 64 KB a block and pass through
+        // the cluster: 24 us of a pass over 131,000 places)
+        constexpr int EACH = I8_BINS / I8_SELECT_THREADS;
+        static_assert(EACH == 4, "a 16-byte load a thread");
+        const int top = I8_BINS - 1 - EACH * (int)threadIdx.x, share_bins = I8_BINS / cluster;
+        int4 four = *reinterpret_cast<const int4*>(count + top - 3);
         if (cluster > 1) {
-            c0 = c1 = 0;
-            for (int r = 0; r < cluster; ++r) { c0 += i8_cluster_int(count + top, r); c1 += i8_cluster_int(count + top - 1, r); }
+            if ((int)threadIdx.x * 4 < share_bins) {
+                const int at = rank_in * share_bins + 4 * (int)threadIdx.x;
+                int4 sum = make_int4(0, 0, 0, 0);
+                for (int r = 0; r < cluster; ++r) {
+                    const int4 v = i8_cluster_int4(count + at, r);
+                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                }
+                *reinterpret_cast<int4*>(total + at) = sum;
+            }
+            ssb_cluster_sync();
+            four = i8_cluster_int4(total + top - 3, (top - 3) / share_bins);
         }
-        int incl = c0 + c1;
+        const int c[EACH] = {four.w, four.z, four.y, four.x}, mine_sum = four.x + four.y + four.z + four.w;
+        int incl = mine_sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -391,7 +412,7 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
         if (lane == 31) warp_sum[0][warp] = incl;
         __syncthreads();
         if (warp == 0) {
-            int v = warp_sum[0][lane];
+            int v = lane < I8_SELECT_WARPS ? warp_sum[0][lane] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -401,73 +422,78 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
         }
         if (threadIdx.x == 0) { chosen = 0; still = 0; }
         __syncthreads();
-        const int over = (warp ? warp_sum[1][warp - 1] : 0) + incl - c0 - c1;       // in the bins above these two
-        if (over < left && over + c0 >= left) { chosen = top; still = left - over; }
-        else if (over + c0 < left && over + c0 + c1 >= left) { chosen = top - 1; still = left - over - c0; }
-        if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
+        int over = (warp ? warp_sum[1][warp - 1] : 0) + incl - mine_sum;        // in the bins above these
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (over < left && over + c[i] >= left) { chosen = top - i; still = left - over; }
+            over += c[i];
+        }
+        __syncthreads();
         if (left > 0) { prefix |= (uint32_t)chosen << shift; left = still; }
         else prefix = 0xffffffffu;                             // none of them stays
-        for (int i = threadIdx.x; i < I8_BINS; i += I8_SELECT_THREADS) count[i] = 0;
         if (left <= 0) break;
-        if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
+        for (int i = threadIdx.x; i < I8_BINS; i += I8_SELECT_THREADS) count[i] = 0;        // nobody reads them any more
+        __syncthreads();
     }
-    // a warp a run of whole 32 places of the block: how many tie, how many stay for sure; then those before this block and warp
-    const int per_warp = ((j1 - j0 + 31) / 32 + 31) / 32 * 32, w0 = j0 + warp * per_warp, w1 = min(w0 + per_warp, j1);
-    auto look = [&](int j, bool& sure, bool& tie) {
+    // how many tie and how many stay for sure; then those before this block and warp
+    auto look = [&](int j, uint32_t r, bool& sure, bool& tie) {
         const bool in = j < w1, free = in && j >= lo && j < hi;
-        const uint32_t r = free ? rank_of(j) : 0u;
         tie = free && r == prefix && left > 0;
         sure = in && (!free || r > prefix);
     };
     int ties = 0, sures = 0;
-    for (int j = w0; j < w1; j += 32) {
+    each([&](int j, uint32_t r) {
         bool sure, tie;
-        look(j + lane, sure, tie);
+        look(j, r, sure, tie);
         ties += __popc(__ballot_sync(0xffffffffu, tie));
         sures += __popc(__ballot_sync(0xffffffffu, sure));
-    }
+    });
     __syncthreads();
     if (lane == 0) { warp_sum[0][warp] = ties; warp_sum[1][warp] = sures; }
     __syncthreads();
     if (threadIdx.x < 2) {
         int sum = 0;
-        for (int w = 0; w < 32; ++w) sum += warp_sum[threadIdx.x][w];
+        for (int w = 0; w < I8_SELECT_WARPS; ++w) sum += warp_sum[threadIdx.x][w];
         mine[threadIdx.x] = sum;
     }
     if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
     int ties_before = 0, sures_before = 0;
     for (int r = 0; r < rank_in; ++r) { ties_before += i8_cluster_int(mine, r); sures_before += i8_cluster_int(mine + 1, r); }
     for (int w = 0; w < warp; ++w) { ties_before += warp_sum[0][w]; sures_before += warp_sum[1][w]; }
-    for (int j = w0; j < w1; j += 32) {
+    each([&](int j, uint32_t r) {
         bool sure, tie;
-        look(j + lane, sure, tie);
+        look(j, r, sure, tie);
         const unsigned t = __ballot_sync(0xffffffffu, tie), u = __ballot_sync(0xffffffffu, sure), below = (1u << lane) - 1;
         const int tie_at = ties_before + __popc(t & below);
         const int at = sures_before + __popc(u & below) + min(tie_at, left);
-        if ((sure || (tie && tie_at < left)) && at < keep) dst[at] = j + lane;
+        if ((sure || (tie && tie_at < left)) && at < keep) dst[at] = j;
         ties_before += __popc(t);
         sures_before += __popc(u);
-    }
+    });
     if (cluster > 1) ssb_cluster_sync();                       // no block leaves while another may read its counts
 }
 
 constexpr int I8_MOVE_THREADS = 256;
 
-// The kept tokens of one destination page and kv head: codes under the largest scale of their new block, weights beside them.
+// The kept tokens of one destination page and kv head: codes under the largest scale of their new block, weights beside them.  A
+// thread's pieces of codes are on their way while the block's scales are compared.
+template <int LANES>
 __global__ void __launch_bounds__(I8_MOVE_THREADS)
 int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restrict__ k_scale, float* __restrict__ v_scale,
                  float* __restrict__ weight, const int* __restrict__ page_table, int n_slots, int max_pages, int n_pages,
-                 const int* __restrict__ seq_slot, const int* __restrict__ new_table, int new_pages, int n_kv, int head_dim, int block,
-                 int keep, const int* __restrict__ kept) {
+                 const int* __restrict__ seq_slot, const int* __restrict__ new_table, int new_pages, int n_kv, int block, int keep,
+                 const int* __restrict__ kept) {
+    constexpr int PIECES = (2 * I8_PAGE * LANES + I8_MOVE_THREADS - 1) / I8_MOVE_THREADS;
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
     const int to = blockIdx.x, head = blockIdx.y, b = blockIdx.z, s = seq_slot[b];
     if (s < 0 || s >= n_slots) return;
     const int target = new_table[(size_t)b * new_pages + to];
     if (target < 0 || target >= n_pages) return;
-    const int lanes = head_dim / 16, per = I8_PAGE / block;
+    const int per = I8_PAGE / block;
     __shared__ long long from[I8_PAGE];                        // the row's place among all rows, or -1
-    __shared__ float scale[2][I8_PAGE], now[2][4];
+    __shared__ float scale[2][I8_PAGE];
+    const size_t head_at = (size_t)target * n_kv + head;
     if (threadIdx.x < I8_PAGE) {
         const int i = to * I8_PAGE + (int)threadIdx.x, j = i < keep ? kept[((size_t)b * n_kv + head) * keep + i] : -1;
         long long row = -1;
@@ -476,32 +502,39 @@ int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restri
             if (page >= 0 && page < n_pages) row = ((long long)page * n_kv + head) * I8_PAGE + (j & 63);
         }
         from[threadIdx.x] = row;
-        scale[0][threadIdx.x] = row >= 0 ? k_scale[row / block] : 0.f;
-        scale[1][threadIdx.x] = row >= 0 ? v_scale[row / block] : 0.f;
+        if (weight && row >= 0) weight[head_at * I8_PAGE + threadIdx.x] = weight[row];
     }
     __syncthreads();
-    const size_t head_at = (size_t)target * n_kv + head;
-    if ((int)threadIdx.x < 2 * per) {
-        const int which = threadIdx.x / per, blk = threadIdx.x % per;
+    uint4 c[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int e = threadIdx.x + i * I8_MOVE_THREADS, which = e / (I8_PAGE * LANES), row = e / LANES % I8_PAGE;
+        if (e < 2 * I8_PAGE * LANES && from[row] >= 0)
+            c[i] = reinterpret_cast<const uint4*>((which ? v : k) + (size_t)from[row] * (16 * LANES))[e % LANES];
+    }
+    if (threadIdx.x < 2 * I8_PAGE) {                           // four warps: 32 rows of keys or values each, whose maxima blocks of 16 share
+        const int which = threadIdx.x / I8_PAGE, row = threadIdx.x % I8_PAGE;
+        const float mine = from[row] >= 0 ? (which ? v_scale : k_scale)[from[row] / block] : 0.f;
+        scale[which][row] = mine;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int e = threadIdx.x + i * I8_MOVE_THREADS, which = e / (I8_PAGE * LANES), row = e / LANES % I8_PAGE;
+        if (e >= 2 * I8_PAGE * LANES || from[row] < 0) continue;
+        const int first = row / block * block;
         float m = 0.f;
-        bool any = false;
-        for (int i = blk * block; i < (blk + 1) * block; ++i) { m = fmaxf(m, scale[which][i]); any |= from[i] >= 0; }
-        now[which][blk] = m;
-        if (any) (which ? v_scale : k_scale)[head_at * per + blk] = m;
-    }
-    if (weight && threadIdx.x < I8_PAGE && from[threadIdx.x] >= 0) weight[head_at * I8_PAGE + threadIdx.x] = weight[from[threadIdx.x]];
-    __syncthreads();
-    for (int e = threadIdx.x; e < 2 * I8_PAGE * lanes; e += I8_MOVE_THREADS) {
-        const int which = e / (I8_PAGE * lanes), row = e / lanes % I8_PAGE, l = e % lanes;
-        if (from[row] < 0) continue;
-        int8_t* codes = which ? v : k;
-        uint4 c = reinterpret_cast<const uint4*>(codes + (size_t)from[row] * head_dim)[l];
-        const float m = now[which][row / block];
+        for (int r = first; r < first + block; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(&scale[which][r]);
+            m = fmaxf(fmaxf(m, fmaxf(f.x, f.y)), fmaxf(f.z, f.w));
+        }
+        if (e % LANES == 0 && row == first) (which ? v_scale : k_scale)[head_at * per + row / block] = m;        // the block's first row is kept if any is
         if (scale[which][row] != m) {
             const float ratio = __fdiv_rn(scale[which][row], m);
-            c.x = i8_rescale4(c.x, ratio); c.y = i8_rescale4(c.y, ratio); c.z = i8_rescale4(c.z, ratio); c.w = i8_rescale4(c.w, ratio);
+            c[i].x = i8_rescale4(c[i].x, ratio); c[i].y = i8_rescale4(c[i].y, ratio);
+            c[i].z = i8_rescale4(c[i].z, ratio); c[i].w = i8_rescale4(c[i].w, ratio);
         }
-        reinterpret_cast<uint4*>(codes + (head_at * I8_PAGE + row) * head_dim)[l] = c;
+        reinterpret_cast<uint4*>((which ? v : k) + (head_at * I8_PAGE + row) * (16 * LANES))[e % LANES] = c[i];
     }
 }
 
@@ -516,10 +549,12 @@ SSB_API int ssb_int8_evict(void* k, void* v, float* k_scale, float* v_scale, flo
     // blocks a (sequence, kv head) by the longest sequence there can be
     const long long longest = (long long)max_pages * I8_PAGE;
     const int cluster = longest <= 8192 ? 1 : longest <= 32768 ? 4 : 8;
-    const int held = (int)std::min<long long>(I8_SELECT_KEYS, ((long long)max_pages + cluster - 1) / cluster * I8_PAGE);
+    // a warp's share of a block's places, in whole 32, as the kernel has it for the longest
+    const long long block_most = ((long long)max_pages + cluster - 1) / cluster * I8_PAGE, warp_most = ((block_most + I8_SELECT_WARPS - 1) / I8_SELECT_WARPS + 31) / 32 * 32;
+    const int held = (int)std::min<long long>(I8_SELECT_KEEP, warp_most * I8_SELECT_WARPS);
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(int8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I8_SELECT_KEYS * 4);
+        const cudaError_t e = cudaFuncSetAttribute(int8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, I8_SELECT_KEEP * 4);
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
@@ -528,7 +563,17 @@ SSB_API int ssb_int8_evict(void* k, void* v, float* k_scale, float* v_scale, flo
                                 (const float*)weight, page_table, n_slots, max_pages, n_pages, seq_slot, lengths, n_kv, keep, first, recent, cluster,
                                 held, kept);
     if (rc) return rc;
-    return ssb_launch(int8_move_kernel, dim3((keep + I8_PAGE - 1) / I8_PAGE, n_kv, n_seqs), dim3(I8_MOVE_THREADS), 0, stream, true,
-                      (int8_t*)k, (int8_t*)v, k_scale, v_scale, weight, page_table, n_slots, max_pages, n_pages, seq_slot, new_table, new_pages,
-                      n_kv, head_dim, block, keep, (const int*)kept);
+#define I8_MOVE(L_) \
+    return ssb_launch(int8_move_kernel<L_>, dim3((keep + I8_PAGE - 1) / I8_PAGE, n_kv, n_seqs), dim3(I8_MOVE_THREADS), 0, stream, true, \
+                      (int8_t*)k, (int8_t*)v, k_scale, v_scale, weight, page_table, n_slots, max_pages, n_pages, seq_slot, new_table, \
+                      new_pages, n_kv, block, keep, (const int*)kept)
+    switch (head_dim) {
+        case 16: I8_MOVE(1);
+        case 32: I8_MOVE(2);
+        case 64: I8_MOVE(4);
+        case 128: I8_MOVE(8);
+        case 256: I8_MOVE(16);
+    }
+#undef I8_MOVE
+    return SSB_ERR_BAD_SIZE;
 }

@@ -11,44 +11,29 @@
 //
 // The reference's 8-bit lane of this architecture multiplies int8 weights by activations of the model's type
 // (crates/runner/src/llama31_engine.rs:289-430).
-#include "common.cuh"
+#include "int8_codes.cuh"
 #include "tc_helpers.cuh"
 #include "tc_rows.cuh"
 #include <algorithm>
 
 typedef __nv_bfloat16 bf16;
 
-constexpr float IL_LEAST_SCALE = 7.888609052210118e-31f;        // 2^-100: a row of zeros has a scale too
-constexpr float IL_MOST = 1.7014118346046923e38f;               // 2^127: what an infinity counts as
 constexpr int IL_MOST_K = 133136;
 
 // ---- rows to codes ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void il_load8(const bf16* p, float (&x)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ void il_load8(const float* p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ float il_finite(float x) { return x != x ? 0.f : fminf(fmaxf(x, -IL_MOST), IL_MOST); }
-// rint(x / s), the division correctly rounded.  x times the reciprocal is within 2e-5 of it (127 times two roundings), so only
-// where that lies about half-way between two codes is there anything to divide for.
+// rint(x / s), the division correctly rounded (as in i8_encode8).
 __device__ __forceinline__ int il_code(float x, float s, float inverse) {
     const float y = x * inverse;
     float c = rintf(y);
     if (fabsf(fabsf(y - c) - 0.5f) < 1e-4f) c = rintf(__fdiv_rn(x, s));
-    return (int)fminf(fmaxf(c, -127.f), 127.f);
+    return (int)c;
 }
-// The maximum of non-negative numbers over a block (their bits have their order).
-__device__ __forceinline__ float il_block_max(float m, float* warp_max) {
-    m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+__device__ __forceinline__ uint32_t il_block_max(uint32_t m, uint32_t* warp_max) {
+    m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
     __syncthreads();
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    return __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(warp_max[lane]) : 0u));
+    return __reduce_max_sync(0xffffffffu, lane < warps ? warp_max[lane] : 0u);
 }
 
 // A block a row, 8 numbers a thread and turn, all of them in registers between the row's maximum and its codes (NV turns).
@@ -57,32 +42,38 @@ template <typename T, int NV>
 __global__ void __launch_bounds__(1024)
 int8_quantize_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ codes, int ldc, float* __restrict__ scale, int K,
                      int* __restrict__ clear, int n_clear) {
-    __shared__ float warp_max[32];
+    __shared__ uint32_t warp_max[2][32];
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
     const int row = blockIdx.x;
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n_clear; i += gridDim.x * blockDim.x) clear[i] = 0;
-    float v[NV][8], most = 0.f;
+    float v[NV][8];
+    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int k = 8 * (threadIdx.x + j * blockDim.x);
-        if (k < K) il_load8(x + (size_t)row * ldx + k, v[j]);
+        if (k < K) i8_load8(x + (size_t)row * ldx + k, v[j]);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-        if (8 * (int)(threadIdx.x + j * blockDim.x) < K)
+        if (8 * (int)(threadIdx.x + j * blockDim.x) < K) top = max(top, i8_magnitude(v[j]));
+    top = il_block_max(top, warp_max[0]);
+    if (top >= I8_WILD) {                                      // the same for the whole block
+        top = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { v[j][e] = il_finite(v[j][e]); most = fmaxf(most, fabsf(v[j][e])); }
-    const float s = fmaxf(__fmul_rn(il_block_max(most, warp_max), 1.f / 127.f), IL_LEAST_SCALE), inverse = 1.f / s;
+        for (int j = 0; j < NV; ++j)
+            if (8 * (int)(threadIdx.x + j * blockDim.x) < K) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = i8_finite(v[j][e]);
+                top = max(top, i8_magnitude(v[j]));
+            }
+        top = il_block_max(top, warp_max[1]);
+    }
+    const float s = fmaxf(__fmul_rn(__uint_as_float(top), 1.f / 127.f), I8_LEAST_SCALE), inverse = 1.f / s;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int k = 8 * (threadIdx.x + j * blockDim.x);
-        if (k < K) {
-            uint32_t w[2] = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(uint8_t)(int8_t)il_code(v[j][e], s, inverse) << (8 * (e & 3));
-            *reinterpret_cast<uint2*>(codes + (size_t)row * ldc + k) = make_uint2(w[0], w[1]);
-        }
+        if (k < K) *reinterpret_cast<uint2*>(codes + (size_t)row * ldc + k) = i8_encode8(v[j], s, inverse);
     }
     if (threadIdx.x == 0) scale[row] = s;
 }
@@ -92,16 +83,16 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 int8_quantize_any_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ codes, int ldc, float* __restrict__ scale, int K,
                          int* __restrict__ clear, int n_clear) {
-    __shared__ float warp_max[32];
+    __shared__ uint32_t warp_max[2][32];
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
     const T* src = x + (size_t)blockIdx.x * ldx;
     for (int i = blockIdx.x * 256 + threadIdx.x; i < n_clear; i += gridDim.x * 256) clear[i] = 0;
-    float most = 0.f;
-    for (int k = threadIdx.x; k < K; k += 256) most = fmaxf(most, fabsf(il_finite(ssb_to_float(src[k]))));
-    const float s = fmaxf(__fmul_rn(il_block_max(most, warp_max), 1.f / 127.f), IL_LEAST_SCALE), inverse = 1.f / s;
+    uint32_t top = 0;
+    for (int k = threadIdx.x; k < K; k += 256) top = max(top, __float_as_uint(fabsf(i8_finite(ssb_to_float(src[k])))));
+    const float s = fmaxf(__fmul_rn(__uint_as_float(il_block_max(top, warp_max[0])), 1.f / 127.f), I8_LEAST_SCALE), inverse = 1.f / s;
     for (int k = threadIdx.x; k < K; k += 256)
-        codes[(size_t)blockIdx.x * ldc + k] = (int8_t)il_code(il_finite(ssb_to_float(src[k])), s, inverse);
+        codes[(size_t)blockIdx.x * ldc + k] = (int8_t)il_code(i8_finite(ssb_to_float(src[k])), s, inverse);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
 }
 
@@ -245,27 +236,33 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (warp == 0) {
         if (lane == 0) {
             // the first stages' weights are nobody's output: they come while the rows are still being quantised
-            const long long ahead = min((long long)STAGES, range.end - range.begin);
-            for (int s = 0; s < ahead; ++s) {
-                const long long u = range.begin + s;
-                const int tile = (int)(u / k_blocks), kb = (int)(u - (long long)tile * k_blocks);
+            const int all = (int)(range.end - range.begin), ahead = min(STAGES, all);
+            // a unit's place: channels of W, rows of x, k; the next one's
+            const int tile0 = (int)(range.begin / k_blocks), m_first = tile0 % m_tiles, n_first = tile0 / m_tiles;
+            const int kb_first = (int)(range.begin - (long long)tile0 * k_blocks);
+            auto next = [&](int& kb, int& m, int& n) {
+                if (++kb == k_blocks) { kb = 0; if (++m == m_tiles) { m = 0; ++n; } }
+            };
+            int kb = kb_first, m = m_first, n = n_first;
+            for (int s = 0; s < ahead; ++s, next(kb, m, n)) {
                 mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
-                tma_load_2d(smem_u32(smem + s * STAGE_BYTES), &map_w, full0 + 8 * s, kb * IL_BK, tile / m_tiles * IL_BM);
+                tma_load_2d(smem_u32(smem + s * STAGE_BYTES), &map_w, full0 + 8 * s, kb * IL_BK, n * IL_BM);
             }
             ssb_pdl_wait();
-            int c = 0;
-            for (long long u = range.begin; u < range.end; ++u, ++c) {
-                const int s = c % STAGES;
-                const int tile = (int)(u / k_blocks), kb = (int)(u - (long long)tile * k_blocks);
+            kb = kb_first; m = m_first; n = n_first;
+            int c = 0, s = 0;
+            uint32_t lap = 1;
+            for (; c < all; ++c, next(kb, m, n)) {
                 const uint32_t w_dst = smem_u32(smem + s * STAGE_BYTES);
                 if (c >= ahead) {
-                    if (!mbar_wait(empty0 + 8 * s, ((c / STAGES) & 1) ^ 1, abort_flag)) {
+                    if (!mbar_wait(empty0 + 8 * s, lap, abort_flag)) {
                         *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_PRODUCER); break;
                     }
                     mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
-                    tma_load_2d(w_dst, &map_w, full0 + 8 * s, kb * IL_BK, tile / m_tiles * IL_BM);
+                    tma_load_2d(w_dst, &map_w, full0 + 8 * s, kb * IL_BK, n * IL_BM);
                 }
-                tma_load_2d(w_dst + W_BYTES, &map_x, full0 + 8 * s, kb * IL_BK, tile % m_tiles * BN);
+                tma_load_2d(w_dst + W_BYTES, &map_x, full0 + 8 * s, kb * IL_BK, m * BN);
+                if (++s == STAGES) { s = 0; lap ^= 1; }
             }
             if (*abort_flag)                                       // let copies that were issued land before the block ends
                 for (int i = max(0, c - STAGES); i < c; ++i)
@@ -276,7 +273,8 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (lane == 0) {
             constexpr uint32_t idesc = il_idesc(IL_BM, BN);
             bool ok = true;
-            int c = 0, i = 0;
+            int i = 0, s = 0;
+            uint32_t lap = 0;
             for (long long u = range.begin; u < range.end && ok; ++i) {
                 const int kb0 = (int)(u % k_blocks), n = (int)min((long long)(k_blocks - kb0), range.end - u);
                 const int buf = i & 1;
@@ -284,15 +282,15 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
                 }
                 tc_fence_after();
-                for (int j = 0; j < n; ++j, ++c) {
-                    const int s = c % STAGES;
-                    if (!mbar_wait(full0 + 8 * s, (c / STAGES) & 1, abort_flag)) {
+                for (int j = 0; j < n; ++j) {
+                    if (!mbar_wait(full0 + 8 * s, lap, abort_flag)) {
                         *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
                     }
                     tc_fence_after();
                     const uint32_t w_addr = smem_u32(smem + s * STAGE_BYTES);
                     il_mma_x4(tmem + buf * BN, smem_desc(w_addr), smem_desc(w_addr + W_BYTES), idesc, j > 0 ? 1u : 0u);
                     tc_commit(empty0 + 8 * s);
+                    if (++s == STAGES) { s = 0; lap ^= 1; }
                 }
                 if (ok) tc_commit(acc_full0 + 8 * buf);
                 u += n;
