@@ -135,6 +135,7 @@ int8_weigh_plain_kernel(const IaArgs a) {
 // to the next.
 constexpr int IR_THREADS = 128, IR_WARPS = 4, IR_SEQS = 1024, IR_STAGES = 3;
 constexpr int IR_EXTRA = 3;
+constexpr long long IR_KEPT_MOST = 1LL << 26;  // floats
 constexpr float IR_NONE = -1e30f;               // a maximum over no key: finite, so that nothing below needs to ask for it
 constexpr int IR_SIDE = 12;                  // beside a stage's page: its scales of keys and of values, and its id
 constexpr int IR_LEAST_X = -80, IR_MOST_X = 120;
@@ -177,7 +178,7 @@ struct IrBatch {
 // A run of pages of one tile and kv head: what of it lies in a block's range.
 struct IrSegment {
     int b, kvh, tile, page, n;           // pages page .. page + n - 1 of the sequence (n may be 0)
-    long long first, last, next;         // the units of the tile's first and last page, and the one behind the segment
+    long long first, last, at, next;     // the units of the tile's first and last page, the segment's first, and the one behind it
     bool begins, whole;                  // has the tile's first page; all of them
 };
 
@@ -209,6 +210,7 @@ __device__ __forceinline__ IrSegment ir_locate(const IrBatch& B, long long u, lo
     g.first = u - (r - before) + B.extra;
     g.last = g.first + units - B.extra - 1;
     const long long from = max(u, g.first);
+    g.at = from;
     g.next = min(g.last + 1, end);
     g.n = (int)max(0LL, g.next - from);
     g.page = B.first_page(s, t0) + (int)(from - g.first);
@@ -474,7 +476,7 @@ __device__ __forceinline__ void ir_put(const IaArgs& a, const IrSeq& s, int tile
 
 template <int HD, int NT, bool WIDE>
 __global__ void __launch_bounds__(IR_THREADS, NT == 1 ? 4 : 2)
-int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict__ pieces, int* __restrict__ error_word,
+int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict__ pieces, float* __restrict__ kept, int* __restrict__ error_word,
                  const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     // probabilities are summed times 2^OFFSET and may exceed that by 2^LAZY before the reference maximum is moved; with f below 2
     // and both in float16, 2^(OFFSET + LAZY + 1) stays below 2^16
@@ -602,6 +604,8 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
                     for (int k = 0; k < TILES; ++k) { o[k][i][0] *= a0; o[k][i][1] *= a1; o[k][i][2] *= a0; o[k][i][3] *= a1; }
                 }
             }
+            if (NT == 1 && kept && g < group)                      // the scores as they are, for what accounts for them
+                *reinterpret_cast<float4*>(kept + (((seg.at + p) * IR_WARPS + warp) * group + g) * 16 + 4 * t) = make_float4(sc[0][0], sc[0][1], sc[0][2], sc[0][3]);
             uint32_t p_hi[NT][2], p_lo[NT][2];
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
@@ -755,6 +759,57 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     }
 }
 
+// What single tokens attend to, from the scores that int8_rows_kernel kept: a page a warp, a lane four keys of every second head.
+__global__ void __launch_bounds__(IR_THREADS)
+int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict__ kept) {
+    extern __shared__ unsigned char smem_raw[];
+    long long* cum = (long long*)smem_raw;
+    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    __shared__ long long warp_total[IR_WARPS];
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, false, IR_EXTRA};
+    const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
+    const int blocks = ir_dealt(total), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.n_q / a.n_kv;
+    const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
+    for (long long u = begin; u < end;) {
+        const IrSegment seg = ir_locate(B, u, end);
+        u = seg.next;
+        const IrSeq s = seqs[seg.b];
+        if (seg.n == 0) continue;
+        // lanes 0 - 15 take heads 0, 2, .., the others 1, 3, ..: of up to 8
+        float ref[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int h = 2 * i + (lane >> 4);
+            ref[i] = h < group ? a.lse[(size_t)s.row0 * a.n_q + seg.kvh * group + h] * 1.4426950408889634f : INFINITY;
+        }
+        const int part = (lane & 15) >> 2, t = lane & 3;
+#pragma unroll 2
+        for (int p = warp; p < seg.n; p += IR_WARPS) {
+            const float* src = kept + (seg.at + p) * (IR_WARPS * 16) * group;
+            const int page = min(seg.page + p, a.max_pages - 1), id = min(max(a.page_table[(size_t)s.slot * a.max_pages + page], 0), a.n_pages - 1);
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int h = 2 * i + (lane >> 4);
+                if (h < group) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(src + (part * group + h) * 16 + 4 * t));
+                    sum.x += ir_ex2(v.x - ref[i]); sum.y += ir_ex2(v.y - ref[i]); sum.z += ir_ex2(v.z - ref[i]); sum.w += ir_ex2(v.w - ref[i]);
+                }
+            }
+            sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16); sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
+            sum.z += __shfl_xor_sync(0xffffffffu, sum.z, 16); sum.w += __shfl_xor_sync(0xffffffffu, sum.w, 16);
+            // keys t, t + 4, t + 8, t + 12 of 16: the lower half adds the first two, the upper the others; one addition a key, so in
+            // one order, and nobody waits for it
+            float* w = a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + 16 * part + t + (lane & 16 ? 8 : 0);
+            const float x = lane & 16 ? sum.z : sum.x, y = lane & 16 ? sum.w : sum.y;
+            if (x > 0.f) atomicAdd(w, x);
+            if (y > 0.f) atomicAdd(w + 4, y);
+        }
+    }
+}
+
 // What the last rows of every sequence attend to, from their lse: the keys once more, 8 NT of the (row, head) columns at a time, QB
 // such batches beside each page.  A key belongs to one block, which adds its columns' probabilities up in one order and then to the
 // key's weight.
@@ -774,6 +829,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
     long long* cum = (long long*)(bars + 2 * IR_STAGES);
     IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
     __shared__ float qf[QB * C], lse2[QB * C];
+    __shared__ int last_of[QB * C];                                // the last key a column sees
     __shared__ long long warp_total[IR_WARPS];
     __shared__ int sm_abort[2];
     volatile int* abort_flag = sm_abort;
@@ -810,6 +866,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
             ir_queries<HD, NT, WIDE>(a, s.row0, s.n_new, seg.kvh, column0 + q * C, qs + q * Q_WORDS, qf + q * C);
         for (int c = threadIdx.x; c < batches * C; c += IR_THREADS) {
             const int token = (column0 + c) / group;
+            last_of[c] = s.start + token;
             lse2[c] = token < s.n_new ? a.lse[(size_t)(s.row0 + token) * a.n_q + seg.kvh * group + (column0 + c) % group] * 1.4426950408889634f : INFINITY;
         }
         __syncthreads();
@@ -832,7 +889,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
                 ir_scores<HD, NT>(keys, qs + q * Q_WORDS, warp, lane, sc);
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    const int c = q * C + 8 * i + g, at = s.start + (column0 + c) / group;
+                    const int c = q * C + 8 * i + g, at = last_of[c];
                     const float by = qf[c] * ks, ref = lse2[c];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -889,7 +946,7 @@ template <typename K> static int ir_configure(K kernel, size_t smem) {
     return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
 }
 
-struct IrPlan { int nt, tts, blocks; size_t piece; };
+struct IrPlan { int nt, tts, blocks; size_t piece; long long kept; };      // floats of a piece; of the scores that are kept
 
 template <int HD, int NT, bool WIDE> static int ir_blocks(int n_seqs) {
     static int blocks = 0;
@@ -915,39 +972,50 @@ template <int HD, int NT, bool WIDE> static int ir_blocks(int n_seqs) {
 
 static bool ir_takes(int n_q, int n_kv, int head_dim) { return (head_dim == 64 || head_dim == 128) && n_q / n_kv <= 32; }
 
-static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim) {
+static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim, int weigh_last) {
     IrPlan p{};
     const int group = n_q / n_kv;
     const long long most = (long long)max_new * group;
     p.nt = most <= 8 ? 1 : most <= 16 ? 2 : 4;
-    while (p.tts < 6 && (2 << p.tts) * group <= 8 * p.nt) ++p.tts;
+    while (p.tts < 6 && (1 << p.tts) < max_new && (2 << p.tts) * group <= 8 * p.nt) ++p.tts;
     const int n = std::min(n_seqs, IR_SEQS);
 #define IR_BLOCKS(H_, N_, W_) { p.blocks = ir_blocks<H_, N_, W_>(n); p.piece = ir_piece<H_, N_>(); }
     IR_EACH(head_dim, p.nt, wide, IR_BLOCKS);
 #undef IR_BLOCKS
     const long long units = ((long long)(rows >> p.tts) + n_seqs) * n_kv * max_pages;
     p.blocks = (int)std::min<long long>(p.blocks, std::max(1LL, units));
+    // single tokens that keep account: their scores are kept, a sixteenth to an eighth of what the pages hold, where that has a
+    // bound (of the longest sequence there can be) that a scratch may have; else the keys are read once more.  16 sequences of 8,192,
+    // 32 heads of 64 in float32: 59 us so, 73 with the keys read again.
+    const long long kept = (long long)n * n_kv * (max_pages + IR_EXTRA) * 64 * group;
+    p.kept = weigh_last > 0 && max_new == 1 && p.nt == 1 && kept <= IR_KEPT_MOST ? kept : 0;
     return p;
 }
 
 // float32 elements of scratch that the launch needs.
-SSB_API long long ssb_int8_attention_scratch(int dtype, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim) {
+SSB_API long long ssb_int8_attention_scratch(int dtype, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim,
+                                             int weigh_last) {
     if (n_seqs <= 0 || rows <= 0 || n_kv <= 0 || !ir_takes(n_q, n_kv, head_dim)) return 0;
-    const IrPlan p = ir_plan(dtype == SSB_F32, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
-    return p.blocks < 0 ? 0 : 2LL * p.blocks * (long long)p.piece;
+    const IrPlan p = ir_plan(dtype == SSB_F32, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, weigh_last);
+    return p.blocks < 0 ? 0 : 2LL * p.blocks * (long long)p.piece + p.kept;
 }
 
 template <int HD, int NT, bool WIDE>
 static int ir_rows(const IaArgs& a, const IrPlan& p, float* pieces, int* error_word, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+    float* kept = p.kept ? pieces + 2LL * p.blocks * (long long)p.piece : nullptr;
     for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
         const int n = std::min(IR_SEQS, a.n_seqs - s0);
         // not as a dependent of what came before: blocks that wait beside another launch's are dealt to SMs unevenly (64 sequences of
         // 1 to 8,192 tokens, one call behind another: 111 us, 162 as dependents)
         int rc = ssb_launch(int8_rows_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), ir_smem<HD, NT>(n), stream, false, a, s0, n, p.tts,
-                            pieces, error_word, mk, mv);
+                            pieces, kept, error_word, mk, mv);
         if (rc) return rc;
         rc = ssb_launch(int8_finish_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IrSeq) + 8) + 8, stream, true,
                         a, s0, n, p.tts, (const float*)pieces);
+        if (rc) return rc;
+        if (kept)
+            rc = ssb_launch(int8_account_kernel, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IrSeq) + 8) + 8, stream, true, a, s0, n,
+                            (const float*)kept);
         if (rc) return rc;
     }
     return 0;
@@ -1021,10 +1089,10 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
     rc = ir_map(&mv, v, (long long)n_pages * n_kv * 64, head_dim);
     if (rc) return rc;
     if (!scratch) return SSB_ERR_BAD_SIZE;
-    const IrPlan p = ir_plan(wide, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
+    const IrPlan p = ir_plan(wide, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, weigh_last);
     if (p.blocks < 0) return SSB_ERR_UNSUPPORTED;
 #define IR_ROWS(H_, N_, W_) rc = ir_rows<H_, N_, W_>(a, p, scratch, error_word, mk, mv, stream)
     IR_EACH(head_dim, p.nt, wide, IR_ROWS);
 #undef IR_ROWS
-    return rc || weigh_last <= 0 ? rc : ia_weigh(a, wide, max_new, error_word, mk, stream);
+    return rc || weigh_last <= 0 || p.kept ? rc : ia_weigh(a, wide, max_new, error_word, mk, stream);
 }

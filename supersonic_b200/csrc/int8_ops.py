@@ -28,7 +28,7 @@ _SIGNATURES = {
     "ssb_int8_evict": ("int8_cache", [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
     "ssb_int8_attention": ("int8_attention", [_P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I,
                                               _I, _I, _I, _I, _F, _P, _P, _P]),
-    "ssb_int8_attention_scratch": ("int8_attention", [_I] * 8),
+    "ssb_int8_attention_scratch": ("int8_attention", [_I] * 9),
     "ssb_int8_quantize_rows": ("int8_linear", [_P, _I, _I, _P, _I, _P, _I, _I, _P]),
     "ssb_int8_linear": ("int8_linear", [_P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
     "ssb_int8_linear_scratch": ("int8_linear", [_I, _I, _I]),
@@ -190,7 +190,7 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
     if max_new <= 0:
         raise KernelError(f"attention: max_new {max_new} new tokens")
     code, width = _CODES[q.dtype], page_table.shape[1]
-    scratch = torch.empty(_fn("ssb_int8_attention_scratch")(code, B, rows, max_new, width, n_q, n_kv, dim), dtype=torch.float32, device=q.device)
+    scratch = torch.empty(_fn("ssb_int8_attention_scratch")(code, B, rows, max_new, width, n_q, n_kv, dim, weigh_last), dtype=torch.float32, device=q.device)
     ops.note_bounded_wait_launches(1)
     _check(_fn("ssb_int8_attention")(
         q_at, ldq, code, o_at, ldo, 0 if lse is None else lse.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(),
