@@ -48,44 +48,75 @@ def _fn(name: str):
     return f
 
 
+_INT32, _INT8, _FLOAT32 = torch.int32, torch.int8, torch.float32
+_SIZES = {torch.float32: 4, torch.bfloat16: 2}
+_DIMS = (16, 32, 64, 128, 256)
+
+
 def _ints(t: torch.Tensor, name: str, n: int) -> int:
     """The address of ``n`` int32 values in a row on the device."""
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_cuda or not (n <= 1 or t.stride(0) == 1):
+    if t.dtype is not _INT32 or t.shape != (n,) or not t.is_cuda or not t.is_contiguous():
         raise KernelError(f"{name} must be {n} contiguous int32 values on a CUDA device, is {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _rows(t: torch.Tensor, name: str, rows: int, width: int, dtype=None) -> Tuple[int, int]:
     """(address, row stride) of a matrix of at least ``width`` columns whose rows start on 16 bytes."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or not t.is_cuda or t.dtype not in _CODES \
-            or (dtype is not None and t.dtype != dtype):
+    size, shape = _SIZES.get(t.dtype), t.shape
+    if size is None or len(shape) != 2 or shape[0] != rows or shape[1] < width or not t.is_cuda or (dtype is not None and t.dtype is not dtype):
         raise KernelError(f"{name} must be [{rows}, {width}] of {dtype or 'float32 or bfloat16'} on a CUDA device, "
-                          f"is {t.dtype} {tuple(t.shape)}")
-    at, ld = t.data_ptr(), t.stride(0) if rows > 1 else width + -width % 8
-    if t.stride(1) != 1 and width > 1 or (at | ld * t.element_size()) % 16 or ld < width:
+                          f"is {t.dtype} {tuple(shape)}")
+    at, (ld, step) = t.data_ptr(), t.stride()
+    if rows == 1:
+        ld = width + -width % 8
+    if (step != 1 and width > 1) or (at | ld * size) % 16 or ld < width:
         raise KernelError(f"{name}: rows of contiguous elements that start on 16 bytes")
     return at, ld
 
 
-def _pages(pages: Int8Pages, table: torch.Tensor, name: str = "page_table") -> Tuple[int, int, int, int]:
-    """(pages, kv heads, head size, block) of a cache entry that holds together, and of its table."""
+def _pages(pages: Int8Pages, table: torch.Tensor):
+    """(pages, kv heads, head size, block) of a cache entry that holds together, the addresses of its five tensors (0: no weight), and
+    its table's address, rows and width.  One condition over all of it: this runs in every call of a decode step."""
     k, v, ks, vs, weight = pages
-    if k.dim() != 4 or k.dtype != torch.int8 or v.dtype != torch.int8 or k.shape != v.shape or k.shape[2] != 64 or not k.is_cuda \
-            or not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
-        raise KernelError(f"pages: k and v must be contiguous int8 [pages, kv heads, 64, head size] on a CUDA device, are {k.dtype} "
-                          f"{tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    n_pages, n_kv, _, dim = k.shape
-    per = ks.shape[-1]
-    if ks.shape != (n_pages, n_kv, per) or per not in (1, 2, 4) or vs.shape != ks.shape or ks.dtype != torch.float32 \
-            or vs.dtype != torch.float32 or not ks.is_contiguous() or not vs.is_contiguous() or not ks.is_cuda or not vs.is_cuda:
-        raise KernelError(f"pages: scales must be contiguous float32 [{n_pages}, {n_kv}, 4, 2 or 1], are {tuple(ks.shape)} and {tuple(vs.shape)}")
-    if weight is not None and (weight.shape != (n_pages, n_kv, 64) or weight.dtype != torch.float32 or not weight.is_contiguous()):
-        raise KernelError(f"pages: weight must be contiguous float32 [{n_pages}, {n_kv}, 64], is {weight.dtype} {tuple(weight.shape)}")
-    if dim not in (16, 32, 64, 128, 256):
-        raise KernelError(f"pages: heads of 16, 32, 64, 128 or 256, not {dim}")
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_cuda or not table.is_contiguous():
-        raise KernelError(f"{name} must be contiguous int32 [rows, pages a sequence] on a CUDA device")
-    return n_pages, n_kv, dim, 64 // per
+    shape, scales, tab = k.shape, ks.shape, table.shape
+    if (len(shape) == 4 and v.shape == shape and shape[2] == 64 and shape[3] in _DIMS and k.dtype is _INT8 and v.dtype is _INT8
+            and k.is_cuda and v.is_cuda and k.is_contiguous() and v.is_contiguous()
+            and len(scales) == 3 and vs.shape == scales and scales[:2] == shape[:2] and scales[2] in (1, 2, 4)
+            and ks.dtype is _FLOAT32 and vs.dtype is _FLOAT32 and ks.is_cuda and vs.is_cuda and ks.is_contiguous() and vs.is_contiguous()
+            and (weight is None or (weight.shape == shape[:3] and weight.dtype is _FLOAT32 and weight.is_cuda and weight.is_contiguous()))
+            and table.dtype is _INT32 and len(tab) == 2 and table.is_cuda and table.is_contiguous()):
+        k_at, v_at = k.data_ptr(), v.data_ptr()
+        if (k_at | v_at) % 16 == 0:
+            at = (k_at, v_at, ks.data_ptr(), vs.data_ptr(), 0 if weight is None else weight.data_ptr())
+            return shape[0], shape[1], shape[3], 64 // scales[2], at, table.data_ptr(), tab[0], tab[1]
+    raise KernelError(
+        "pages: k and v must be int8 [pages, kv heads, 64, 16 32 64 128 or 256], their scales float32 [pages, kv heads, 4 2 or 1], weight "
+        "float32 [pages, kv heads, 64] or None, the page table int32 [rows, pages a sequence], all contiguous on a CUDA device; are "
+        f"{k.dtype} {tuple(shape)}, {v.dtype} {tuple(v.shape)}, {ks.dtype} {tuple(scales)}, {vs.dtype} {tuple(vs.shape)}, "
+        f"{None if weight is None else (weight.dtype, tuple(weight.shape))} and {table.dtype} {tuple(tab)}")
+
+
+_error_words = {}
+_scratch_sizes = {}
+
+
+def _error_word(device: torch.device) -> int:
+    """The address of the device's error word (:func:`.ops.tc_error_word`), for a launch with bounded waits, which counts as unread."""
+    ops.note_bounded_wait_launches(1)
+    at = _error_words.get(device)
+    if at is None:
+        at = _error_words[device] = ops.tc_error_word(device).data_ptr()
+    return at
+
+
+def _scratch_size(name: str, *sizes: int) -> int:
+    """What the library says a launch of these sizes needs."""
+    n = _scratch_sizes.get((name, sizes))
+    if n is None:
+        if len(_scratch_sizes) > 4096:
+            _scratch_sizes.clear()
+        n = _scratch_sizes[name, sizes] = _fn(name)(*sizes)
+    return n
 
 
 def append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], pos: torch.Tensor, place: torch.Tensor,
@@ -99,7 +130,7 @@ def append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.T
     A block's scale is max(its scale so far, max |x| * (1/127) over its new tokens, 2^-100); when it grows, the block's earlier codes
     are rounded again under it.  NaN counts as zero and an infinity as 2^127.  The tokens of a sequence come in
     consecutive rows, in order; rows with a negative slot, or a place outside the table, are passed over."""
-    n_pages, n_kv, dim, block = _pages(pages, page_table)
+    n_pages, n_kv, dim, block, at, table, slots, per_seq = _pages(pages, page_table)
     T, width = qkv.shape[0], (n_q + 2 * n_kv) * dim
     if n_q < 0:
         raise KernelError(f"append: {n_q} query heads")
@@ -115,24 +146,23 @@ def append(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.T
         cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
     _check(_fn("ssb_int8_append")(
         q_at, ldq, _CODES[qkv.dtype], o_at, ldo, cos_at, sin_at, positions, rot, _ints(pos, "pos", T), _ints(place, "place", T),
-        _ints(slot, "slot", T), T, page_table.data_ptr(), page_table.shape[0], page_table.shape[1], pages.k.data_ptr(),
-        pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(),
-        0 if pages.weight is None else pages.weight.data_ptr(), n_pages, n_q, n_kv, dim, block, _stream()), "int8_append")
+        _ints(slot, "slot", T), T, table, slots, per_seq, *at, n_pages, n_q, n_kv, dim, block, _stream()), "int8_append")
 
 
 def read(pages: Int8Pages, page_table: torch.Tensor, seq_slot: torch.Tensor, lengths: torch.Tensor, k_out: torch.Tensor,
          v_out: torch.Tensor) -> None:
     """The values a cache stands for: ``k_out``, ``v_out`` [sequences, most, kv heads, head size] (float32 or bfloat16) get the
     first ``lengths`` (and at most ``most``) tokens of every sequence; what is behind them stays."""
-    n_pages, n_kv, dim, block = _pages(pages, page_table)
-    B, most = k_out.shape[0], k_out.shape[1]
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if t.shape != (B, most, n_kv, dim) or t.dtype not in _CODES or t.dtype != k_out.dtype or not t.is_cuda or not t.is_contiguous() \
-                or t.data_ptr() % 16:
-            raise KernelError(f"read: {name} must be contiguous [sequences, most, {n_kv}, {dim}], is {t.dtype} {tuple(t.shape)}")
+    n_pages, n_kv, dim, block, at, table, slots, per_seq = _pages(pages, page_table)
+    shape = k_out.shape
+    if len(shape) != 4 or shape[2] != n_kv or shape[3] != dim or v_out.shape != shape or k_out.dtype not in _CODES \
+            or v_out.dtype is not k_out.dtype or not k_out.is_cuda or not v_out.is_cuda or not k_out.is_contiguous() \
+            or not v_out.is_contiguous() or (k_out.data_ptr() | v_out.data_ptr()) % 16:
+        raise KernelError(f"read: k_out and v_out must be contiguous [sequences, most, {n_kv}, {dim}] of float32 or bfloat16, are "
+                          f"{k_out.dtype} {tuple(shape)} and {v_out.dtype} {tuple(v_out.shape)}")
+    B, most = shape[0], shape[1]
     _check(_fn("ssb_int8_read")(
-        pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), page_table.data_ptr(),
-        page_table.shape[0], page_table.shape[1], n_pages, _ints(seq_slot, "seq_slot", B), _ints(lengths, "lengths", B), B,
+        *at[:4], table, slots, per_seq, n_pages, _ints(seq_slot, "seq_slot", B), _ints(lengths, "lengths", B), B,
         k_out.data_ptr(), v_out.data_ptr(), _CODES[k_out.dtype], most, n_kv, dim, block, _stream()), "int8_read")
 
 
@@ -146,7 +176,7 @@ def evict(pages: Int8Pages, page_table: torch.Tensor, seq_slot: torch.Tensor, le
     under the largest scale of their new block, weights as they are.  ``kept`` (int32 [sequences, kv heads, keep]) gets the places
     that stayed, -1 behind the last.  Afterwards a sequence has min(length, keep) tokens, in ``new_table``'s row; its old pages
     can be given back.  Keys stay rotated by the positions they had."""
-    n_pages, n_kv, dim, block = _pages(pages, page_table)
+    n_pages, n_kv, dim, block, at, table, slots, per_seq = _pages(pages, page_table)
     B = seq_slot.shape[0]
     if pages.weight is None:
         raise KernelError("evict: the pages keep no weights (Int8Pages.weight)")
@@ -158,8 +188,7 @@ def evict(pages: Int8Pages, page_table: torch.Tensor, seq_slot: torch.Tensor, le
     if kept.dtype != torch.int32 or kept.shape != (B, n_kv, keep) or not kept.is_cuda or not kept.is_contiguous():
         raise KernelError(f"evict: kept must be contiguous int32 [{B}, {n_kv}, {keep}], is {kept.dtype} {tuple(kept.shape)}")
     _check(_fn("ssb_int8_evict")(
-        pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), pages.weight.data_ptr(),
-        page_table.data_ptr(), page_table.shape[0], page_table.shape[1], n_pages, _ints(seq_slot, "seq_slot", B),
+        *at, table, slots, per_seq, n_pages, _ints(seq_slot, "seq_slot", B),
         _ints(lengths, "lengths", B), B, new_table.data_ptr(), new_table.shape[1], n_kv, dim, block, keep, first, recent,
         kept.data_ptr(), _stream()), "int8_evict")
 
@@ -173,7 +202,7 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
     ``lse`` (float32 [rows, n_q]) gets the logarithm of a row's sum of exponentials.  ``weigh_last``: that many last rows of every
     sequence add their probabilities, summed over the query heads of a kv head, to ``pages.weight``.  Rows of a sequence with a
     negative slot are zeros, and their ``lse`` minus infinity."""
-    n_pages, n_kv, dim, block = _pages(pages, page_table)
+    n_pages, n_kv, dim, block, at, table, slots, width = _pages(pages, page_table)
     rows, B = q.shape[0], seq_slot.shape[0]
     if n_q <= 0 or n_q % n_kv:
         raise KernelError(f"attention: {n_q} query heads do not split over {n_kv} kv heads")
@@ -184,20 +213,18 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, n_q) or not lse.is_cuda or not lse.is_contiguous()):
         raise KernelError(f"attention: lse must be contiguous float32 [{rows}, {n_q}], is {lse.dtype} {tuple(lse.shape)}")
     if weigh_last and lse is None:
-        lse = torch.empty((rows, n_q), dtype=torch.float32, device=q.device)
+        lse = torch.empty((rows, n_q), dtype=_FLOAT32, device=q.device)
     if rows == 0 or B == 0:
         return
     if max_new <= 0:
         raise KernelError(f"attention: max_new {max_new} new tokens")
-    code, width = _CODES[q.dtype], page_table.shape[1]
-    scratch = torch.empty(_fn("ssb_int8_attention_scratch")(code, B, rows, max_new, width, n_q, n_kv, dim, weigh_last), dtype=torch.float32, device=q.device)
-    ops.note_bounded_wait_launches(1)
+    code, device = _CODES[q.dtype], q.device
+    scratch = torch.empty(_scratch_size("ssb_int8_attention_scratch", code, B, rows, max_new, width, n_q, n_kv, dim, weigh_last),
+                          dtype=_FLOAT32, device=device)
     _check(_fn("ssb_int8_attention")(
-        q_at, ldq, code, o_at, ldo, 0 if lse is None else lse.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(),
-        pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), 0 if pages.weight is None else pages.weight.data_ptr(),
-        page_table.data_ptr(), page_table.shape[0], width, n_pages, _ints(cu_new, "cu_new", B + 1),
-        _ints(seq_start, "seq_start", B), _ints(seq_slot, "seq_slot", B), B, rows, max_new, n_q, n_kv, dim, block, int(window or 0),
-        weigh_last, scale, scratch.data_ptr(), ops.tc_error_word(q.device).data_ptr(), _stream()), "int8_attention")
+        q_at, ldq, code, o_at, ldo, 0 if lse is None else lse.data_ptr(), *at, table, slots, width, n_pages,
+        _ints(cu_new, "cu_new", B + 1), _ints(seq_start, "seq_start", B), _ints(seq_slot, "seq_slot", B), B, rows, max_new, n_q, n_kv,
+        dim, block, window or 0, weigh_last, scale, scratch.data_ptr(), _error_word(device), _stream()), "int8_attention")
 
 
 # ---- matrix products ------------------------------------------------------------------------------------------------
@@ -227,7 +254,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, ou
     channel's.  ``accumulate`` adds to a float32 ``out``.  k: a multiple of 16 up to 133,136; n: a multiple of 8."""
     rows, k = x.shape
     n = weight.shape[0]
-    if weight.dtype != torch.int8 or weight.dim() != 2 or weight.shape[1] != k or not weight.is_cuda or weight.stride(1) != 1 \
+    if weight.dtype is not _INT8 or weight.dim() != 2 or weight.shape[1] != k or not weight.is_cuda or weight.stride(1) != 1 \
             or (weight.data_ptr() | weight.stride(0)) % 16:
         raise KernelError(f"linear: weight must be int8 [n, {k}] with rows on 16 bytes, is {weight.dtype} {tuple(weight.shape)}")
     if k % 16 or not 0 < k <= MOST_K or n % 8:
@@ -240,8 +267,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, ou
         raise KernelError("linear: results are added in float32 only")
     if rows == 0 or n == 0:
         return
-    scratch = torch.empty(_fn("ssb_int8_linear_scratch")(rows, n, k), dtype=torch.int8, device=x.device)
-    ops.note_bounded_wait_launches(1)
+    device = x.device
+    scratch = torch.empty(_scratch_size("ssb_int8_linear_scratch", rows, n, k), dtype=_INT8, device=device)
     _check(_fn("ssb_int8_linear")(x_at, ldx, _CODES[x.dtype], weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), o_at, ldo,
-                                  _CODES[out.dtype], rows, n, k, 1 if accumulate else 0, scratch.data_ptr(),
-                                  ops.tc_error_word(x.device).data_ptr(), _stream()), "int8_linear")
+                                  _CODES[out.dtype], rows, n, k, 1 if accumulate else 0, scratch.data_ptr(), _error_word(device),
+                                  _stream()), "int8_linear")
