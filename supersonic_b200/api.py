@@ -51,6 +51,13 @@ class Engine:
         return teacher_forced(self.model, sequences, decode_step)
 
 
+    def int8_session(self, max_tokens: int, budget: Optional[int] = None, **kw):
+        """The loaded model's sequences with its projections, keys and values in 8 bits, and with ``budget`` cut down to their first,
+        latest and most attended tokens (``engine/int8_session.py``)."""
+        from .engine.int8_session import Int8Session
+        return Int8Session(self.model, max_tokens, budget=budget, **kw)
+
+
 def load(model_dir: Optional[str] = None, dtype: str = "bfloat16", device: int = 0,
          context_size: Optional[int] = None, batch_size: int = 1, max_tokens: Optional[int] = None,
          step_token_budget: Optional[int] = None, preset: Optional[str] = None, random_seed: int = 0,
