@@ -588,7 +588,7 @@ static IlPlan il_plan(int M, int N, int K) {
     p.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
     p.m_tiles = (M + p.bn - 1) / p.bn;
     p.n_tiles = (N + IL_BM - 1) / IL_BM;
-    p.blocks = (int)std::min<long long>(sms, (long long)p.m_tiles * p.n_tiles * k_blocks);
+    p.blocks = (int)std::min<long long>(sms, std::max<long long>(1, (long long)p.m_tiles * p.n_tiles * k_blocks / 4));
     p.counters = (size_t)p.blocks * 4;
     p.pieces = (size_t)p.blocks * 2 * p.bn * IL_BM * 4;
     return p;
