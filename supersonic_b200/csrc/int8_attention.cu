@@ -994,8 +994,9 @@ static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_page
 
 // float32 elements of scratch that the launch needs.
 SSB_API long long ssb_int8_attention_scratch(int dtype, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim,
-                                             int weigh_last) {
+                                             int weigh_last, float scale) {
     if (n_seqs <= 0 || rows <= 0 || n_kv <= 0 || !ir_takes(n_q, n_kv, head_dim)) return 0;
+    if (ia_tc_takes(dtype, head_dim, max_new, scale)) return ia_tc_scratch(n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
     const IrPlan p = ir_plan(dtype == SSB_F32, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, weigh_last);
     return p.blocks < 0 ? 0 : 2LL * p.blocks * (long long)p.piece + p.kept;
 }
@@ -1077,12 +1078,13 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
         }
         return ssb_launch_status();
     }
-    const bool wide = dtype == SSB_F32, prompt = ia_tc_takes(a, dtype, max_new);
+    const bool wide = dtype == SSB_F32, prompt = ia_tc_takes(dtype, head_dim, max_new, scale);
     CUtensorMap mk, mv;
     int rc = prompt && weigh_last <= 0 ? 0 : ir_map(&mk, k, (long long)n_pages * n_kv * 64, head_dim);
     if (rc) return rc;
     if (prompt) {
-        rc = ia_tc_launch(a, max_new, error_word, stream);
+        if (ldq % 8 || ldo % 8 || (((uintptr_t)q | (uintptr_t)out) & 15)) return SSB_ERR_BAD_SIZE;
+        rc = ia_tc_launch(a, max_new, scratch, error_word, stream);
         if (rc || weigh_last <= 0) return rc;
         return ia_weigh(a, wide, max_new, error_word, mk, stream);
     }

@@ -21,6 +21,7 @@ struct IaArgs {
     float scale;
 };
 
-// Prompts of bfloat16 rows on tcgen05 (int8_attention_tc.cu): whether it takes these, and the launch.
-bool ia_tc_takes(const IaArgs& a, int dtype, int max_new);
-int ia_tc_launch(const IaArgs& a, int max_new, int* error_word, cudaStream_t stream);
+// Prompts of bfloat16 rows on tcgen05 (int8_attention_tc.cu): whether it takes these, the float32 scratch it needs, and the launch.
+bool ia_tc_takes(int dtype, int head_dim, int max_new, float scale);
+long long ia_tc_scratch(int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim);
+int ia_tc_launch(const IaArgs& a, int max_new, float* scratch, int* error_word, cudaStream_t stream);

@@ -33,7 +33,7 @@ constexpr float IT_LAZY = 12.f;            // how far, in the log2 domain, a max
 constexpr float IT_LEAST = 7.888609052210118e-31f;
 struct ItSeq { int row0, n_new, start, slot; };
 struct ItTile { int row, head, p0, rows, turns; };
-struct ItUnit { int turns, kb_lo, kvh, slot, last; ItTile tile[2]; };       // no turns: the block is done; last: the sequence's last key
+struct ItUnit { int turns, kb_lo, kvh, slot, last, part; ItTile tile[2]; };       // no turns: the block is done; last: the sequence's last key; part: of the keys, or -1: all
 __host__ __device__ constexpr int it_threads(int tiles) { return 256 + 128 * tiles; }
 constexpr int IT_BARS = 6 + 8 + 6 + IT_SCALES;
 __host__ __device__ constexpr size_t it_smem(int tiles, int hd) {
@@ -43,6 +43,37 @@ __host__ __device__ constexpr size_t it_smem(int tiles, int hd) {
 // Registers a thread of the three kinds of warps: 4 that control, 4 that convert, 4 a tile that take the softmax.
 constexpr int IT_REGS_CONTROL = 48, IT_REGS_CONVERT = 96;
 __host__ __device__ constexpr int it_regs_softmax(int tiles) { return tiles == 2 ? 184 : 232; }
+
+// The turns of a unit: items (row tile, head of the group) TILES * level and, with two tiles, the one behind it.  Keys begin at the
+// page that the first tile of the pair sees first, for a tile that is alone too: a row's turns, and with them its sums, are the same in
+// a unit of either size.
+template <int TILES> struct ItSpan {
+    int kb_lo, most, nb[TILES];          // first page; turns of the longer tile; of each
+    __device__ ItSpan(int start, int n_new, int group, int window, int level) : kb_lo(0), most(0) {
+        const int n_items = ((n_new + IT_BM - 1) / IT_BM) * group;
+#pragma unroll
+        for (int x = 0; x < TILES; ++x) {
+            const int item = TILES * level + x, tile = item / group;
+            const int p0 = start + tile * IT_BM, rows = item < n_items ? min(IT_BM, n_new - tile * IT_BM) : 0;
+            if (x == 0) {
+                const int first = start + (item & ~1) / group * IT_BM;
+                kb_lo = (window > 0 && first - window + 1 > 0) ? (first - window + 1) >> 6 : 0;
+            }
+            nb[x] = rows > 0 ? (((p0 + rows - 1) >> 6) - kb_lo + 2) >> 1 : 0;
+            most = max(most, nb[x]);
+        }
+    }
+};
+// Where there are fewer units than SMs a unit's turns are cut into up to ``parts`` runs of ``each`` turns, four at least, that are units
+// of their own; int8_join_kernel puts them together.
+struct ItCut {
+    int parts, each;
+    __device__ ItCut(int turns, int most_parts) {
+        parts = min(most_parts, max(1, turns / 4));
+        each = (turns + parts - 1) / parts;
+        parts = (turns + each - 1) / max(1, each);
+    }
+};
 
 __device__ __forceinline__ void it_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // A from tensor memory (8 columns a step of 16 keys), B's descriptor 128 units (16 rows of 128 bytes) a step: four steps.
@@ -120,7 +151,8 @@ template <bool KEYS> __device__ __forceinline__ uint4 it_operand(uint32_t w0, ui
 
 template <int HD, int TILES>
 __global__ void __launch_bounds__(it_threads(TILES), 1)
-int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map_q, int s0, int n_seqs, int levels, int* __restrict__ error_word) {
+int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map_q, int s0, int n_seqs, int levels, int parts,
+                         float* __restrict__ part_o, float2* __restrict__ part_ml, int* __restrict__ error_word) {
     constexpr uint32_t TMEM_COLS = 256 * TILES, S0 = 0, O0 = IT_BN * TILES;       // scores, later probabilities; outputs behind them
     constexpr int HALVES = HD / 64;
     constexpr uint32_t Q_BYTES = IT_BM * HD * 2, PAGE_BYTES = 64 * HD * 2, KV_BYTES = 2 * PAGE_BYTES;
@@ -192,10 +224,12 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
             // The units of the launch go from the latest position to the first, over sequences and kv heads; a block takes every
             // gridDim.x-th of them, forwards and backwards in turn.
             int base = 0, level = levels - 1;                    // units before this level's
-            int n_units = 0;
+            int n_units = 0, taken = 0;                          // units published, and looked at (some have no turn)
             bool ok = true;
             while (ok) {
-                const int u = n_units * (int)gridDim.x + ((n_units & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+                const int all = taken * (int)gridDim.x + ((taken & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+                const int u = all / parts, part = all - u * parts;
+                ++taken;
                 while (level >= 0) {
                     int here = 0, next = 0;                      // levels next..level are reached by the same sequences
                     for (int c = 0; c < n_seqs; c += 32) {
@@ -229,25 +263,22 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                         member -= n;
                     }
                     const ItSeq q = seqs[b];
-                    const int n_items = ((q.n_new + IT_BM - 1) / IT_BM) * group;
+                    const ItSpan<TILES> span(q.start, q.n_new, group, window, level);
+                    const ItCut cut(span.most, parts);
+                    const int skip = part * cut.each;
+                    if (skip >= span.most) continue;             // fewer parts than others have
+                    kb_lo = span.kb_lo + 2 * skip;
 #pragma unroll
                     for (int x = 0; x < TILES; ++x) {
-                        const int item = TILES * level + x;
-                        const int tile = item / group;
-                        const int p0 = q.start + tile * IT_BM, rows = item < n_items ? min(IT_BM, q.n_new - tile * IT_BM) : 0;
+                        const int item = TILES * level + x, tile = item / group;
                         t_head[x] = kvh * group + item % group;
                         t_row[x] = q.row0 + tile * IT_BM;
-                        // Keys begin at the page that the first tile of the pair sees first, for a tile that is alone too: a
-                        // row's turns, and with them its sums, are the same in a unit of either size
-                        if (x == 0) {
-                            const int first = q.start + (item & ~1) / group * IT_BM;
-                            kb_lo = (window > 0 && first - window + 1 > 0) ? (first - window + 1) >> 6 : 0;
-                        }
-                        nb[x] = rows > 0 ? (((p0 + rows - 1) >> 6) - kb_lo + 2) >> 1 : 0;    // turns, from page kb_lo on
+                        nb[x] = min(max(span.nb[x] - skip, 0), cut.each);
                         nb_max = max(nb_max, nb[x]);
                         q_tiles += nb[x] > 0;
-                        if (lane == 0) unit.tile[x] = ItTile{t_row[x], t_head[x], p0, rows, nb[x]};
+                        if (lane == 0) unit.tile[x] = ItTile{t_row[x], t_head[x], q.start + tile * IT_BM, min(IT_BM, q.n_new - tile * IT_BM), nb[x]};
                     }
+                    if (lane == 0) unit.part = cut.parts > 1 ? part : -1;
                     if (lane == 0) { unit.slot = q.slot; unit.last = q.start + q.n_new - 1; }
                 }
                 if (lane == 0) {
@@ -448,6 +479,7 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
             if (nb_max == 0) break;
             const int kb_lo = units[n & 1].kb_lo;
             const ItTile tile = units[n & 1].tile[x];
+            const int part = units[n & 1].part;
             __syncwarp();
             if (lane == 0) it_arrive(u_empty0 + 8 * (n & 1));
             const int n_mine = tile.turns, p0 = tile.p0, pos = p0 + r;
@@ -549,8 +581,24 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                 if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
             } else {
                 tc_fence_after();
-                const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
                 const size_t row = (size_t)(tile.row + r);
+                if (part >= 0) {                                 // a part: sums as they are, the reference and the sum of weights
+                    const size_t at = ((size_t)part * a.rows + row) * a.n_q + tile.head;
+#pragma unroll 1
+                    for (int i = 0; i < HD / 32; ++i) {
+                        uint32_t o[32];
+                        it_ld32(t_o + i * 32, o);
+                        it_ld_wait();
+                        if (r < tile.rows) {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q)
+                                *reinterpret_cast<uint4*>(part_o + at * HD + i * 32 + 4 * q) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+                        }
+                    }
+                    if (r < tile.rows) part_ml[at] = make_float2(m_ref, l_run);
+                    continue;
+                }
+                const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
                 uint4* dst = reinterpret_cast<uint4*>((bf16*)a.out + row * a.ldo + (size_t)tile.head * HD);
 #pragma unroll
                 for (int i = 0; i < HD / 32; ++i) {
@@ -583,13 +631,78 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
     }
 }
 
-bool ia_tc_takes(const IaArgs& a, int dtype, int max_new) {
-    return dtype == SSB_BF16 && (a.head_dim == 64 || a.head_dim == 128) && max_new >= 64 && a.scale > 0.f && a.ldq % 8 == 0 && a.ldo % 8 == 0 &&
-           (((uintptr_t)a.q | (uintptr_t)a.out) & 15) == 0;
+// Rows whose keys were cut into parts: a thread four dims of a row's head.
+template <int HD, int TILES>
+__global__ void __launch_bounds__(256)
+int8_join_kernel(const IaArgs a, int s0, int n_seqs, int parts, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int d = (int)(e % (HD / 4)) * 4, head = (int)(e / (HD / 4) % a.n_q);
+    const long long row_of = e / (HD / 4) / a.n_q;
+    if (row_of >= a.rows) return;
+    const int row = (int)row_of, group = a.n_q / a.n_kv;
+    int lo = s0, hi = s0 + n_seqs - 1;                           // the last sequence that begins at or before the row
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.cu_new[mid] <= row) lo = mid; else hi = mid - 1;
+    }
+    const int row0 = a.cu_new[lo], n_new = a.cu_new[lo + 1] - row0, start = a.seq_start[lo], slot = a.seq_slot[lo];
+    if (slot < 0 || slot >= a.n_slots || start < 0 || row < row0 || row >= row0 + n_new) return;
+    const int item = (row - row0) / IT_BM * group + head % group;
+    const ItSpan<TILES> span(start, n_new, group, a.window, item / TILES);
+    const ItCut cut(span.most, parts);
+    if (cut.parts <= 1) return;
+    const int turns = TILES == 2 && (item & 1) ? span.nb[TILES - 1] : span.nb[0];
+    const int mine = (turns + cut.each - 1) / cut.each;          // parts that reach the row's tile
+    float m = -INFINITY, l = 0.f;
+    for (int p = 0; p < mine; ++p) m = fmaxf(m, __ldcg(part_ml + ((size_t)p * a.rows + row) * a.n_q + head).x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < mine; ++p) {
+        const size_t at = ((size_t)p * a.rows + row) * a.n_q + head;
+        const float2 ml = __ldcg(part_ml + at);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_o + at * HD + d));
+        const float by = ml.x == -INFINITY ? 0.f : it_ex2(ml.x - m);
+        o.x = fmaf(v.x, by, o.x); o.y = fmaf(v.y, by, o.y); o.z = fmaf(v.z, by, o.z); o.w = fmaf(v.w, by, o.w);
+        l = fmaf(ml.y, by, l);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * inv, o.y * inv), y = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>((bf16*)a.out + (size_t)row * a.ldo + (size_t)head * HD + d) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    if (d == 0 && a.lse) a.lse[(size_t)row * a.n_q + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// From 64 new tokens of a sequence on: half of a tile's rows.
+bool ia_tc_takes(int dtype, int head_dim, int max_new, float scale) {
+    return dtype == SSB_BF16 && (head_dim == 64 || head_dim == 128) && max_new >= 64 && scale > 0.f;
+}
+
+// Tiles a unit, and parts that a unit's keys are cut into at most.
+struct ItPlan { int tiles, levels, parts; };
+static ItPlan it_plan(int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim) {
+    ItPlan p{};
+    const int group = n_q / n_kv, sms = ssb_sm_count();
+    const int pairs = (((max_new + IT_BM - 1) / IT_BM) * group + 1) / 2;
+    p.tiles = (long long)n_kv * n_seqs * pairs <= sms / 2 ? 1 : 2;
+    p.levels = p.tiles == 1 ? ((max_new + IT_BM - 1) / IT_BM) * group : pairs;
+    // units there can be: every sequence may end in a tile and a unit that is not full
+    const long long units = std::min((long long)n_kv * n_seqs * p.levels, n_kv * (((long long)rows / IT_BM + n_seqs) * group / p.tiles + n_seqs));
+    // parts for two rounds of the SMs, of at least four turns of the longest sequence there can be, in a scratch of up to 256 MB
+    p.parts = (int)std::max(1LL, std::min({2LL * sms / std::max(1LL, units), (long long)(max_pages + 1) / 8, 16LL,
+                                           (1LL << 26) / ((long long)rows * n_q * (head_dim + 2))}));
+    return p;
+}
+// float32 elements that parts are kept in.
+long long ia_tc_scratch(int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim) {
+    const ItPlan p = it_plan(n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
+    return p.parts > 1 ? (long long)p.parts * rows * n_q * (head_dim + 2) : 0;
 }
 
 template <int HD, int TILES>
-static int it_launch(const IaArgs& a, const CUtensorMap& mq, int s0, int n, int levels, long long grid, int* error_word, cudaStream_t stream) {
+static int it_launch(const IaArgs& a, const CUtensorMap& mq, int s0, int n, const ItPlan& p, long long grid, float* scratch, int* error_word,
+                     cudaStream_t stream) {
     constexpr size_t smem = it_smem(TILES, HD);
     static bool configured = false;
     if (!configured) {
@@ -602,25 +715,29 @@ static int it_launch(const IaArgs& a, const CUtensorMap& mq, int s0, int n, int 
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
-    return ssb_launch(int8_attention_tc_kernel<HD, TILES>, dim3((unsigned)grid), dim3(it_threads(TILES)), smem, stream, true, a, mq, s0, n, levels,
-                      error_word);
+    float* part_o = scratch;
+    float2* part_ml = p.parts > 1 ? reinterpret_cast<float2*>(scratch + (size_t)p.parts * a.rows * a.n_q * HD) : nullptr;
+    const int rc = ssb_launch(int8_attention_tc_kernel<HD, TILES>, dim3((unsigned)grid), dim3(it_threads(TILES)), smem, stream, true, a, mq, s0, n,
+                              p.levels, p.parts, part_o, part_ml, error_word);
+    if (rc || p.parts == 1) return rc;
+    return ssb_launch(int8_join_kernel<HD, TILES>, dim3((unsigned)(((long long)a.rows * a.n_q * (HD / 4) + 255) / 256)), dim3(256), 0, stream, true,
+                      a, s0, n, p.parts, (const float*)part_o, (const float2*)part_ml);
 }
 
-int ia_tc_launch(const IaArgs& a, int max_new, int* error_word, cudaStream_t stream) {
+int ia_tc_launch(const IaArgs& a, int max_new, float* scratch, int* error_word, cudaStream_t stream) {
     CUtensorMap mq;
     int rc = make_map(&mq, a.q, a.rows, a.n_q * a.head_dim, a.ldq, IT_BM);
     if (rc) return rc;
-    const int group = a.n_q / a.n_kv, sms = ssb_sm_count();
-    const int pairs = (((max_new + IT_BM - 1) / IT_BM) * group + 1) / 2;
-    const int tiles = (long long)a.n_kv * a.n_seqs * pairs <= sms / 2 ? 1 : 2;
-    const int levels = tiles == 1 ? ((max_new + IT_BM - 1) / IT_BM) * group : pairs;
+    const ItPlan p = it_plan(a.n_seqs, a.rows, max_new, a.max_pages, a.n_q, a.n_kv, a.head_dim);
+    if (p.parts > 1 && !scratch) return SSB_ERR_BAD_SIZE;
+    const int group = a.n_q / a.n_kv, sms = ssb_sm_count(), tiles = p.tiles;
     for (int s0 = 0; s0 < a.n_seqs; s0 += IT_SEQS) {
         const int n = std::min(IT_SEQS, a.n_seqs - s0);
-        // a block for every SM, and no more than there can be units: each sequence may end in a tile and a unit that is not full
-        const long long rows_units = a.n_kv * (((long long)a.rows / IT_BM + n) * group / tiles + n);
-        const long long grid = std::min({(long long)sms, (long long)a.n_kv * n * levels, rows_units});
-        if (a.head_dim == 64) rc = tiles == 1 ? it_launch<64, 1>(a, mq, s0, n, levels, grid, error_word, stream) : it_launch<64, 2>(a, mq, s0, n, levels, grid, error_word, stream);
-        else rc = tiles == 1 ? it_launch<128, 1>(a, mq, s0, n, levels, grid, error_word, stream) : it_launch<128, 2>(a, mq, s0, n, levels, grid, error_word, stream);
+        // a block for every SM, and no more than there can be units
+        const long long units = std::min((long long)a.n_kv * n * p.levels, a.n_kv * (((long long)a.rows / IT_BM + n) * group / tiles + n)) * p.parts;
+        const long long grid = std::min((long long)sms, units);
+        if (a.head_dim == 64) rc = tiles == 1 ? it_launch<64, 1>(a, mq, s0, n, p, grid, scratch, error_word, stream) : it_launch<64, 2>(a, mq, s0, n, p, grid, scratch, error_word, stream);
+        else rc = tiles == 1 ? it_launch<128, 1>(a, mq, s0, n, p, grid, scratch, error_word, stream) : it_launch<128, 2>(a, mq, s0, n, p, grid, scratch, error_word, stream);
         if (rc) return rc;
     }
     return 0;

@@ -406,3 +406,18 @@ def test_linear_on_a_side_stream_and_no_wait_runs_out(rows):
     side.synchronize()
     ops.check_device_errors()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dim,n_q,n_kv,window", [(128, 4, 1, None), (64, 6, 2, None), (128, 3, 3, 700), (64, 4, 1, 1500)])
+def test_attention_of_few_new_tokens_behind_many(dim, n_q, n_kv, window):
+    """Few tiles of rows and many keys: the keys are cut into parts, as many as each sequence has room for."""
+    rng = np.random.default_rng(dim + n_q)
+    _check_attention(rng, [2100, 3, 900, 5000], [70, 130, 64, 1], n_q, n_kv, dim, 16, "bf16", window=window, weigh=2)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_attention_of_a_few_tokens_a_sequence(kind):
+    """Between one token and a tile of them: rows of several tokens and heads share a block's columns."""
+    rng = np.random.default_rng(11)
+    for n_q, n_kv, dim in ((4, 1, 64), (6, 2, 128), (8, 8, 64), (16, 1, 128)):
+        _check_attention(rng, [300, 61, 0, 1000], [3, 7, 16, 33], n_q, n_kv, dim, 32, kind, weigh=5)
