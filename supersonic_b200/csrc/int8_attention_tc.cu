@@ -41,8 +41,10 @@ __host__ __device__ constexpr size_t it_smem(int tiles, int hd) {
            IT_BARS * 8 + 32 + 1024;
 }
 // Registers a thread of the three kinds of warps: 4 that control, 4 that convert, 4 a tile that take the softmax.
-constexpr int IT_REGS_CONTROL = 48, IT_REGS_CONVERT = 96;
-__host__ __device__ constexpr int it_regs_softmax(int tiles) { return tiles == 2 ? 184 : 232; }
+__host__ __device__ constexpr int it_blocks(int tiles, int hd) { return tiles == 1 && hd == 64 ? 2 : 1; }       // an SM
+constexpr int IT_REGS_CONTROL = 48;
+__host__ __device__ constexpr int it_regs_convert(int tiles, int hd) { return it_blocks(tiles, hd) == 2 ? 72 : 96; }
+__host__ __device__ constexpr int it_regs_softmax(int tiles, int hd) { return it_blocks(tiles, hd) == 2 ? 120 : tiles == 2 ? 184 : 232; }
 
 // The turns of a unit: items (row tile, head of the group) TILES * level and, with two tiles, the one behind it.  Keys begin at the
 // page that the first tile of the pair sees first, for a tile that is alone too: a row's turns, and with them its sums, are the same in
@@ -150,7 +152,7 @@ template <bool KEYS> __device__ __forceinline__ uint4 it_operand(uint32_t w0, ui
 }
 
 template <int HD, int TILES>
-__global__ void __launch_bounds__(it_threads(TILES), 1)
+__global__ void __launch_bounds__(it_threads(TILES), it_blocks(TILES, HD))
 int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map_q, int s0, int n_seqs, int levels, int parts,
                          float* __restrict__ part_o, float2* __restrict__ part_ml, int* __restrict__ error_word) {
     constexpr uint32_t TMEM_COLS = 256 * TILES, S0 = 0, O0 = IT_BN * TILES;       // scores, later probabilities; outputs behind them
@@ -368,7 +370,7 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
             if (!ok) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); }
         }
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(IT_REGS_CONVERT));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(it_regs_convert(TILES, HD)));
         const int id = threadIdx.x - 128;
         const int per = 64 >> a.shift;
         const int row_of = id / (HD / 16), c = id % (HD / 16);    // of the pieces id, id + 128, ...: rows 128 / (HD / 16) apart
@@ -459,7 +461,7 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
         }
         if (!ok && lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_PRODUCER); }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(it_regs_softmax(TILES)));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(it_regs_softmax(TILES, HD)));
         // softmax and output: one query row per thread; warps 8-11 tile 0, warps 12-15 tile 1
         const int x = TILES == 1 ? 0 : (warp - 8) >> 2;
         const int quarter = warp & 3;                            // the lanes of tensor memory this warp may touch
@@ -682,16 +684,28 @@ bool ia_tc_takes(int dtype, int head_dim, int max_new, float scale) {
 // Tiles a unit, and parts that a unit's keys are cut into at most.
 struct ItPlan { int tiles, levels, parts; };
 static ItPlan it_plan(int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim) {
+    const int group = n_q / n_kv, sms = ssb_sm_count(), items = ((max_new + IT_BM - 1) / IT_BM) * group;
+    const long long turns = (max_pages + 1) / 2;                 // of the longest sequence there can be
+    // parts of four turns at least, in a scratch of up to 256 MB
+    const long long most = std::min({turns / 4, 16LL, (1LL << 26) / ((long long)rows * n_q * (head_dim + 2))});
+    // Of one or two tiles a unit and the numbers of parts, what is done first: rounds of the SMs times the turns of a part, and three
+    // more for its beginning and end.  A turn of two tiles is 1.65 of one's at head size 128; at 64, where single tiles run two blocks
+    // an SM, the same, and one that has its SM to itself 0.78.  us with one tile and with two, heads x size: 500 tokens behind 16,001, 32 x 64 184 and 181, 32 x 128 314 and
+    // 196; 300 behind 3,000, 8 x 64 23.3 and 28.2, 8 x 128 27.8 and 33.8; two of 600 behind 1,000, 32 x 128 90 and 98, 32 x 64 67 and 73; four of 2,048,
+    // 32 x 128 323 and 206, 32 x 64 192 and 184.
     ItPlan p{};
-    const int group = n_q / n_kv, sms = ssb_sm_count();
-    const int pairs = (((max_new + IT_BM - 1) / IT_BM) * group + 1) / 2;
-    p.tiles = (long long)n_kv * n_seqs * pairs <= sms / 2 ? 1 : 2;
-    p.levels = p.tiles == 1 ? ((max_new + IT_BM - 1) / IT_BM) * group : pairs;
-    // units there can be: every sequence may end in a tile and a unit that is not full
-    const long long units = std::min((long long)n_kv * n_seqs * p.levels, n_kv * (((long long)rows / IT_BM + n_seqs) * group / p.tiles + n_seqs));
-    // parts for two rounds of the SMs, of at least four turns of the longest sequence there can be, in a scratch of up to 256 MB
-    p.parts = (int)std::max(1LL, std::min({2LL * sms / std::max(1LL, units), (long long)(max_pages + 1) / 8, 16LL,
-                                           (1LL << 26) / ((long long)rows * n_q * (head_dim + 2))}));
+    double best = 0;
+    for (int tiles = 2; tiles >= 1; --tiles) {
+        const int levels = (items + tiles - 1) / tiles;
+        // units there can be: every sequence may end in a tile and a unit that is not full
+        const long long units = std::min((long long)n_kv * n_seqs * levels, n_kv * (((long long)rows / IT_BM + n_seqs) * group / tiles + n_seqs));
+        const long long slots = (long long)sms * it_blocks(tiles, head_dim);
+        for (long long n = 1; n <= std::max(1LL, most); ++n) {
+            const double turn = tiles == 2 ? (head_dim == 128 ? 1.65 : 1.0) : head_dim == 64 && units * n <= sms ? 0.78 : 1.0;
+            const double cost = (double)((units * n + slots - 1) / slots) * (double)((turns + n - 1) / n + 3) * turn;
+            if (p.parts == 0 || cost < best) { best = cost; p = ItPlan{tiles, levels, (int)n}; }
+        }
+    }
     return p;
 }
 // float32 elements that parts are kept in.
@@ -709,7 +723,7 @@ static int it_launch(const IaArgs& a, const CUtensorMap& mq, int s0, int n, cons
         cudaFuncAttributes attr;
         cudaError_t e = cudaFuncGetAttributes(&attr, int8_attention_tc_kernel<HD, TILES>);
         // what the softmax warps take must be what the others give: a kernel built with fewer registers a thread would wait for good
-        if (e == cudaSuccess && attr.numRegs * it_threads(TILES) < 128 * (IT_REGS_CONTROL + IT_REGS_CONVERT + TILES * it_regs_softmax(TILES)))
+        if (e == cudaSuccess && attr.numRegs * it_threads(TILES) < 128 * (IT_REGS_CONTROL + it_regs_convert(TILES, HD) + TILES * it_regs_softmax(TILES, HD)))
             return SSB_ERR_UNSUPPORTED;
         if (e == cudaSuccess) e = cudaFuncSetAttribute(int8_attention_tc_kernel<HD, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
@@ -735,7 +749,7 @@ int ia_tc_launch(const IaArgs& a, int max_new, float* scratch, int* error_word, 
         const int n = std::min(IT_SEQS, a.n_seqs - s0);
         // a block for every SM, and no more than there can be units
         const long long units = std::min((long long)a.n_kv * n * p.levels, a.n_kv * (((long long)a.rows / IT_BM + n) * group / tiles + n)) * p.parts;
-        const long long grid = std::min((long long)sms, units);
+        const long long grid = std::min((long long)sms * it_blocks(tiles, a.head_dim), units);
         if (a.head_dim == 64) rc = tiles == 1 ? it_launch<64, 1>(a, mq, s0, n, p, grid, scratch, error_word, stream) : it_launch<64, 2>(a, mq, s0, n, p, grid, scratch, error_word, stream);
         else rc = tiles == 1 ? it_launch<128, 1>(a, mq, s0, n, p, grid, scratch, error_word, stream) : it_launch<128, 2>(a, mq, s0, n, p, grid, scratch, error_word, stream);
         if (rc) return rc;
