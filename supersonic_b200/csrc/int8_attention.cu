@@ -708,40 +708,48 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
             mbar_wait(full0 + 8 * (i % IR_STAGES), (i / IR_STAGES) & 1, abort_flag + 1);
 }
 
-// Tiles whose pages lay in several blocks' ranges: block c takes the one that began in c's range and went on behind it.
+// Tiles whose pages lay in several blocks' ranges: block c, whose range may begin in the middle of one and end in another, takes its share
+// of each one's sums, half a block a tile: a column's four dims a thread where there are many, else several threads with a part of
+// the pieces each, put together by shuffles.  (A tile a block, whichever had its first page: one sequence of 4,000 tokens, whose 8
+// tiles are 74 pieces each, @@ us.)
 template <int HD, int NT, bool WIDE>
 __global__ void __launch_bounds__(IR_THREADS)
 int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __restrict__ pieces) {
     constexpr float OFFSET = WIDE ? 13.f : 2.f;
-    constexpr int C = 8 * NT;
+    constexpr int C = 8 * NT, HALF = IR_THREADS / 2;
     extern __shared__ unsigned char smem_raw[];
     long long* cum = (long long*)smem_raw;
     IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
     __shared__ long long warp_total[IR_WARPS];
+    __shared__ float others[2][6][32];
     IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
     ssb_pdl_launch_dependents();
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     ssb_pdl_wait();
-    const int blocks = ir_dealt(total), c0 = blockIdx.x;
-    const long long begin = ir_begin(total, c0, blocks), end = ir_begin(total, c0 + 1, blocks);
+    const int blocks = ir_dealt(total), c = blockIdx.x, half = threadIdx.x / HALF, thread = threadIdx.x % HALF, lane = threadIdx.x & 31;
+    const long long begin = ir_begin(total, c, blocks), end = ir_begin(total, c + 1, blocks);
     if (begin >= end) return;
-    // the tile whose unit is the range's last: its first page may be here or (the range ends among its extra units) elsewhere
-    const IrSegment seg = ir_locate(B, end - 1, end);
-    if (seg.first < begin || seg.first >= end || seg.last < end) return;
-    const int c1 = ir_owner(seg.last, total, blocks);
-    auto piece = [&](int c) { return pieces + (size_t)(2 * c + (c == c0)) * ir_piece<HD, NT>(); };
-    for (int e = threadIdx.x; e < C * (HD / 4); e += IR_THREADS) {
-        const int col = e / (HD / 4), d = e % (HD / 4) * 4;
+    const IrSegment seg = ir_locate(B, half ? end - 1 : begin, end);
+    const IrSeq s = seqs[seg.b];
+    const int c0 = ir_owner(seg.first, total, blocks), c1 = ir_owner(seg.last, total, blocks), n_pieces = c1 - c0 + 1;
+    if (n_pieces < 2 || c < c0 || c > c1) return;              // the same for the whole half
+    const int live = min(C, min(1 << tts, s.n_new - (seg.tile << tts)) * (a.n_q / a.n_kv)) * (HD / 4);
+    int e0 = (int)((long long)live * (c - c0) / n_pieces), e1 = (int)((long long)live * (c - c0 + 1) / n_pieces);
+    if (half ? seg.first - B.extra <= begin : seg.last >= end - 1) (half ? e0 : e1) = (e0 + e1) / 2;        // both halves have this tile
+    auto piece = [&](int i) { return pieces + (size_t)(2 * i + (i == c0)) * ir_piece<HD, NT>(); };
+    for (; e0 < e1; e0 += HALF) {
+        const int n = min(HALF, e1 - e0), width = n > 32 ? HALF : n > 1 ? 1 << (32 - __clz(n - 1)) : 1, groups = HALF / width;
+        const int e = e0 + min(thread % width, n - 1), col = e / (HD / 4), d = e % (HD / 4) * 4;
         float top = IR_NONE, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         constexpr int AT_ONCE = 4;                                 // pieces asked for together
-        for (int c = c0; c <= c1; c += AT_ONCE) {
+        for (int i0 = c0 + thread / width; i0 <= c1; i0 += AT_ONCE * groups) {
             float pm[AT_ONCE], pl[AT_ONCE];
             float4 pv[AT_ONCE];
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
-                const float* p = piece(min(c + i, c1));
-                pm[i] = c + i <= c1 ? __ldcg(p + C * HD + col) : IR_NONE;
+                const float* p = piece(min(i0 + i * groups, c1));
+                pm[i] = i0 + i * groups <= c1 ? __ldcg(p + C * HD + col) : IR_NONE;
                 pl[i] = __ldcg(p + C * HD + C + col);
                 pv[i] = __ldcg(reinterpret_cast<const float4*>(p + col * HD + d));
             }
@@ -750,12 +758,27 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
             top = now;
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
-                const float by = c + i <= c1 ? ir_ex2(pm[i] - now) : 0.f;
+                const float by = i0 + i * groups <= c1 ? ir_ex2(pm[i] - now) : 0.f;
                 v.x = fmaf(pv[i].x, by, v.x); v.y = fmaf(pv[i].y, by, v.y); v.z = fmaf(pv[i].z, by, v.z); v.w = fmaf(pv[i].w, by, v.w);
                 sum = fmaf(pl[i], by, sum);
             }
         }
-        ir_put<HD, WIDE>(a, seqs[seg.b], seg.tile, tts, seg.kvh, col, d, v, top, sum, OFFSET);
+        auto add = [&](float t, float l, float x, float y, float z, float w) {
+            const float now = fmaxf(top, t), keep = ir_ex2(top - now), by = ir_ex2(t - now);
+            top = now;
+            sum = sum * keep + l * by;
+            v.x = v.x * keep + x * by; v.y = v.y * keep + y * by; v.z = v.z * keep + z * by; v.w = v.w * keep + w * by;
+        };
+        for (int o = width; o < 32; o <<= 1)
+            add(__shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o), __shfl_xor_sync(0xffffffffu, v.x, o),
+                __shfl_xor_sync(0xffffffffu, v.y, o), __shfl_xor_sync(0xffffffffu, v.z, o), __shfl_xor_sync(0xffffffffu, v.w, o));
+        if (groups > 1) {                                          // the half's two warps
+            float (&o)[6][32] = others[half];
+            if (thread >= 32) { o[0][lane] = top; o[1][lane] = sum; o[2][lane] = v.x; o[3][lane] = v.y; o[4][lane] = v.z; o[5][lane] = v.w; }
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(HALF) : "memory");
+            if (thread < 32) add(o[0][lane], o[1][lane], o[2][lane], o[3][lane], o[4][lane], o[5][lane]);
+        }
+        if (thread < n) ir_put<HD, WIDE>(a, s, seg.tile, tts, seg.kvh, col, d, v, top, sum, OFFSET);
     }
 }
 
