@@ -36,7 +36,7 @@ struct I8Append {
     int8_t* codes[2];             // keys, values
     float* scale[2];
     float* weight;                // or null
-    int ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block, chunk, kv_warps;
+    int ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block, chunk, kv_blocks;
 };
 
 constexpr int I8_APPEND_WARPS = 4, I8_Q_HEADS = 8;
@@ -49,6 +49,8 @@ constexpr int I8_APPEND_WARPS = 4, I8_Q_HEADS = 8;
 //    whether they begin one: 18,000 rows of 48 heads 153 us).
 //  * queries: ROWS rows of up to 8 heads, the rotation tables' rows read once for all of them.
 // KV, Q: which kinds of warps the launch has; where there are many rows each kind has a launch of its own, and its own number of registers.
+// 17,000 rows of 32 heads over 8 of 128 in bfloat16: 64 us for keys and values, bound by the instructions of rotating, rounding and
+// writing them, and 42 us for queries, at the rate of a copy.
 template <typename T, int LANES, bool KV, bool Q>
 __global__ void __launch_bounds__(32 * I8_APPEND_WARPS, KV ? 4 : 8)
 int8_append_kernel(const I8Append a) {
@@ -58,7 +60,14 @@ int8_append_kernel(const I8Append a) {
     const int lane = threadIdx.x & 31, l = lane % LANES, r_of = lane / LANES, half = a.rot / 2;
     const bool turned = a.cos_t != nullptr && l < a.rot / 16;
     const int e0 = l < a.rot / 16 ? 8 * l : a.rot + 16 * (l - a.rot / 16), e1 = l < a.rot / 16 ? half + 8 * l : e0 + 8;
+    // the two kinds' blocks lie among one another in proportion
     int w = blockIdx.x * I8_APPEND_WARPS + (threadIdx.x >> 5);
+    bool queries = !KV;
+    if (KV && Q) {
+        const long long before = (long long)blockIdx.x * a.kv_blocks / gridDim.x, then = (long long)(blockIdx.x + 1) * a.kv_blocks / gridDim.x;
+        queries = then == before;
+        w = (int)(queries ? blockIdx.x - before : before) * I8_APPEND_WARPS + (threadIdx.x >> 5);
+    }
 
     auto page_of = [&](int s, int p) -> int {                 // or -1: no place
         if (s < 0 || s >= a.n_slots || p < 0 || (p >> 6) >= a.max_pages) return -1;
@@ -79,8 +88,7 @@ int8_append_kernel(const I8Append a) {
             y[i] = __fadd_rn(__fmul_rn(u, s[i]), __fmul_rn(v, c[i]));
         }
     };
-    if (Q && (!KV || w >= a.kv_warps)) {                       // queries
-        if (KV) w -= a.kv_warps;
+    if (Q && queries) {
         const int blocks = (a.n_q + I8_Q_HEADS - 1) / I8_Q_HEADS, head0 = w % blocks * I8_Q_HEADS, row = w / blocks * ROWS + r_of;
         if (row >= a.T) return;
         const int sl = a.slot[row], pl = a.place[row];
@@ -223,15 +231,18 @@ SSB_API int ssb_int8_append(const void* qkv, int ldq, int dtype, void* out, int 
     if (rot % 16 || rot > head_dim || n_kv <= 0 || n_q < 0 || (block != 16 && block != 32 && block != 64)) return SSB_ERR_BAD_SIZE;
     I8Append a{qkv, out, cos_t, sin_t, pos, place, slot, page_table, {(int8_t*)k, (int8_t*)v}, {k_scale, v_scale}, weight,
                ldq, ldo, T, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, rot, positions, block};
-    // a warp a row while there are few; else a chunk of rows, of which two or so begin a run
-    const bool many = T > 256;
-    a.chunk = many ? std::min(block, 32) : 1;
+    // A warp a row while there are few; else a chunk of rows, of which two or so begin a run; and a launch for each kind of warps where
+    // there are so many that the keys' registers cost the queries more than a second launch.  32 heads over 8 of 128, us with one
+    // launch of a row a warp, of chunks of 8, and two launches with chunks of 16: 2 x 256 tokens 9.7, -, 14.1; 4 x 256 16.0, 10.4, 18.5;
+    // 4 x 512 31.4, 20.8, 26.3; 1,024 single tokens 29.6, 26.1, 39.9; 4 x 1,024 57.8, 38.2, 36.4; 16 x 1,024 -, 136, 116.
+    const bool many = T > 2048;
+    a.chunk = many ? std::min(block, 32) : T > 256 ? 8 : 1;
     const int rows = 32 / std::max(1, head_dim / 16);
     const long long kv = (long long)((T + a.chunk - 1) / a.chunk) * 2 * n_kv;
     const long long q = (long long)((T + rows - 1) / std::max(1, rows)) * ((n_q + I8_Q_HEADS - 1) / I8_Q_HEADS);
-    const long long blocks = (kv + q + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS;
-    if (blocks > 0x7fffffffLL || kv > 0x7fffffffLL) return SSB_ERR_BAD_SIZE;
-    a.kv_warps = (int)kv;
+    const long long kv_blocks = (kv + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS, blocks = kv_blocks + (q + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS;
+    if (blocks * I8_APPEND_WARPS > 0x7fffffffLL) return SSB_ERR_BAD_SIZE;
+    a.kv_blocks = (int)kv_blocks;
     const dim3 threads(32 * I8_APPEND_WARPS), kv_grid((unsigned)((kv + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS)),
         q_grid((unsigned)((q + I8_APPEND_WARPS - 1) / I8_APPEND_WARPS));
     int rc = 0;
@@ -316,6 +327,9 @@ __device__ __forceinline__ uint32_t i8_rank(float x) {
 
 constexpr int I8_SELECT_THREADS = 512, I8_SELECT_WARPS = I8_SELECT_THREADS / 32, I8_BINS = 2048;
 constexpr int I8_SELECT_KEEP = 16384;      // ranks a block keeps in shared memory; further ones are read again
+// Ranks of no number, which go from that of minus infinity, 0x007fffff, to that of infinity, 0xff800000: of a place behind the end; of one
+// whose page is not there, below every number; of one that stays whatever it weighs.
+constexpr uint32_t I8_NEVER = 0u, I8_NOWHERE = 1u << 21, I8_SURE = 0xffffffffu;
 
 __device__ __forceinline__ int4 i8_cluster_int4(const int* mine, unsigned rank) {
     uint32_t remote;
@@ -330,15 +344,16 @@ __device__ __forceinline__ int i8_cluster_int(const int* mine, unsigned rank) {
 
 // kept[b, head] = the places that stay, in order: the first ``first``, the last ``recent``, and of the others the heaviest, equal
 // ones by their place; -1 behind them.  A cluster of 1, 4 or 8 blocks a (sequence, kv head), each with a run of whole pages of the
-// sequence and each warp with a run of whole 32 places of its block's: the rank of the last one that stays is found 11, 11 and 10 bits
+// sequence and each warp with a run of whole 128 places of its block's: the rank of the last one that stays is found 11, 11 and 10 bits
 // at a time, by counting (every block adds the cluster's counts up for itself), then every warp writes its places behind those of the
-// warps and blocks before it.  Ranks lie in shared memory and the loops over them stay loops: 32 ranks a thread in registers, every
-// loop unrolled, is code that runs once, and took longer to fetch than to run (sequences of 700 tokens 9 us and 32).
+// warps and blocks before it.  Ranks lie in shared memory, four places a lane and turn, and the loops over them stay loops: 32 ranks a
+// thread in registers, every loop unrolled, is code that runs once, and took longer to fetch than to run (sequences of 700 tokens 9 us
+// and 32).  What bounds it is the instructions of those loops: @@
 __global__ void __launch_bounds__(I8_SELECT_THREADS, 2)
 int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ page_table, int n_slots, int max_pages, int n_pages,
                    const int* __restrict__ seq_slot, const int* __restrict__ lengths, int n_kv, int keep, int first, int recent,
                    int cluster, int held, int* __restrict__ kept) {
-    extern __shared__ uint32_t ranks[];
+    extern __shared__ __align__(16) uint32_t ranks[];
     __shared__ __align__(16) int count[I8_BINS], total[I8_BINS];
     __shared__ int warp_sum[2][32];
     __shared__ int chosen, still;
@@ -357,30 +372,41 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
     const int pages = (n + I8_PAGE - 1) / I8_PAGE, share = (pages + cluster - 1) / cluster * I8_PAGE;
     const int j0 = min(rank_in * share, n), j1 = min(j0 + share, n);        // this block's places
     const int lo = first, hi = n - recent;                     // places that have to be chosen from
-    auto fetch = [&](int j) -> uint32_t {
+    const int per_warp = ((j1 - j0 + I8_SELECT_WARPS - 1) / I8_SELECT_WARPS + 127) / 128 * 128, w0 = min(j0 + warp * per_warp, j1), w1 = min(w0 + per_warp, j1);
+    const bool wide = ((uintptr_t)weight & 15) == 0;
+    auto fetch = [&](int j) -> uint4 {                         // of four places, which share a page
+        if (j >= w1) return make_uint4(I8_NEVER, I8_NEVER, I8_NEVER, I8_NEVER);
         const int page = pt[j >> 6];
-        return page < 0 || page >= n_pages ? 0u : i8_rank(weight[((size_t)page * n_kv + head) * I8_PAGE + (j & 63)]);
+        const bool there = page >= 0 && page < n_pages;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (there) {
+            const float* at = weight + ((size_t)page * n_kv + head) * I8_PAGE + (j & 63);
+            f = wide ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+        }
+        auto rank = [&](int i, float x) { return i >= w1 ? I8_NEVER : i < lo || i >= hi ? I8_SURE : there ? i8_rank(x) : I8_NOWHERE; };
+        return make_uint4(rank(j, f.x), rank(j + 1, f.y), rank(j + 2, f.z), rank(j + 3, f.w));
     };
-    const int per_warp = ((j1 - j0 + I8_SELECT_WARPS - 1) / I8_SELECT_WARPS + 31) / 32 * 32, w0 = min(j0 + warp * per_warp, j1), w1 = min(w0 + per_warp, j1);
     for (int i = threadIdx.x; i < I8_BINS; i += I8_SELECT_THREADS) count[i] = 0;
-    const int kept_in = min(held / I8_SELECT_WARPS / 32 * 32, per_warp);     // of the warp's places, in shared memory
+    const int kept_in = min(held / I8_SELECT_WARPS / 128 * 128, per_warp);   // of the warp's places, in shared memory
     uint32_t* own = ranks + warp * kept_in;
-#pragma unroll 8
-    for (int j = w0 + lane; j < min(w0 + kept_in, w1); j += 32) own[j - w0] = fetch(j);
+#pragma unroll 4
+    for (int j = w0 + 4 * lane; j < min(w0 + kept_in, w1); j += 128) *reinterpret_cast<uint4*>(own + (j - w0)) = fetch(j);
     __syncthreads();
-    // f(place, rank) for each of the warp's places, 32 at a time
+    // f(first place, ranks) for each four of the lane's places, 128 of the warp's at a time
     auto each = [&](auto&& f) {
-        for (int j = w0 + lane; j - lane < w1; j += 32) f(j, j >= w1 ? 0u : j - w0 < kept_in ? own[j - w0] : fetch(j));
+        for (int j = w0 + 4 * lane; j - 4 * lane < w1; j += 128)
+            f(j, j >= w1 ? make_uint4(I8_NEVER, I8_NEVER, I8_NEVER, I8_NEVER) : j - w0 < kept_in ? *reinterpret_cast<const uint4*>(own + (j - w0)) : fetch(j));
     };
 
     uint32_t prefix = 0;                                       // the bits found so far
     int left = keep - first - recent;                          // of those with the prefix, how many stay
-    for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
+    for (int shift = left > 0 ? 21 : -1; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
         const int bits = shift == 0 ? 10 : 11;
         const uint32_t above = shift == 21 ? 0u : ~0u << (shift + bits);
-        each([&](int j, uint32_t r) {
-            if (((r ^ prefix) & above) == 0 && j >= lo && j < min(w1, hi)) atomicAdd(&count[(r >> shift) & ((1 << bits) - 1)], 1);
-        });
+        auto counted = [&](uint32_t r) {
+            if (((r ^ prefix) & above) == 0 && r - 1u < I8_SURE - 1u) atomicAdd(&count[(r >> shift) & ((1 << bits) - 1)], 1);
+        };
+        each([&](int, const uint4& r) { counted(r.x); counted(r.y); counted(r.z); counted(r.w); });
         if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
         // four bins a thread, the highest first: how many lie above them.  In a cluster every block adds up its share of the bins over
         // the blocks and fetches the other shares' totals (each adding all of them up for itself moved 64 KB a block and pass through
@@ -429,26 +455,20 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
             over += c[i];
         }
         __syncthreads();
-        if (left > 0) { prefix |= (uint32_t)chosen << shift; left = still; }
-        else prefix = 0xffffffffu;                             // none of them stays
-        if (left <= 0) break;
+        prefix |= (uint32_t)chosen << shift;
+        left = still;
         for (int i = threadIdx.x; i < I8_BINS; i += I8_SELECT_THREADS) count[i] = 0;        // nobody reads them any more
         __syncthreads();
     }
+    if (left == 0) prefix = I8_SURE - 1;                       // none that has to be chosen stays
     // how many tie and how many stay for sure; then those before this block and warp
-    auto look = [&](int j, uint32_t r, bool& sure, bool& tie) {
-        const bool in = j < w1, free = in && j >= lo && j < hi;
-        tie = free && r == prefix && left > 0;
-        sure = in && (!free || r > prefix);
-    };
     int ties = 0, sures = 0;
-    each([&](int j, uint32_t r) {
-        bool sure, tie;
-        look(j, r, sure, tie);
-        ties += __popc(__ballot_sync(0xffffffffu, tie));
-        sures += __popc(__ballot_sync(0xffffffffu, sure));
+    each([&](int, const uint4& r) {
+        ties += (r.x == prefix) + (r.y == prefix) + (r.z == prefix) + (r.w == prefix);
+        sures += (r.x > prefix) + (r.y > prefix) + (r.z > prefix) + (r.w > prefix);
     });
-    __syncthreads();
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    sures = __reduce_add_sync(0xffffffffu, sures);
     if (lane == 0) { warp_sum[0][warp] = ties; warp_sum[1][warp] = sures; }
     __syncthreads();
     if (threadIdx.x < 2) {
@@ -456,19 +476,30 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
         for (int w = 0; w < I8_SELECT_WARPS; ++w) sum += warp_sum[threadIdx.x][w];
         mine[threadIdx.x] = sum;
     }
-    if (cluster > 1) ssb_cluster_sync(); else __syncthreads();
+    if (cluster > 1) ssb_cluster_sync();
     int ties_before = 0, sures_before = 0;
     for (int r = 0; r < rank_in; ++r) { ties_before += i8_cluster_int(mine, r); sures_before += i8_cluster_int(mine + 1, r); }
     for (int w = 0; w < warp; ++w) { ties_before += warp_sum[0][w]; sures_before += warp_sum[1][w]; }
-    each([&](int j, uint32_t r) {
-        bool sure, tie;
-        look(j, r, sure, tie);
-        const unsigned t = __ballot_sync(0xffffffffu, tie), u = __ballot_sync(0xffffffffu, sure), below = (1u << lane) - 1;
-        const int tie_at = ties_before + __popc(t & below);
-        const int at = sures_before + __popc(u & below) + min(tie_at, left);
-        if ((sure || (tie && tie_at < left)) && at < keep) dst[at] = j;
-        ties_before += __popc(t);
-        sures_before += __popc(u);
+    each([&](int j, const uint4& r) {
+        auto packed = [&](uint32_t x) { return (x > prefix ? 1 : 0) + (x == prefix ? 1 << 16 : 0); };
+        const int four = packed(r.x) + packed(r.y) + packed(r.z) + packed(r.w);
+        int incl = four;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        int sure_at = sures_before + ((incl - four) & 0xffff), tie_at = ties_before + ((incl - four) >> 16);
+        auto put = [&](int i, uint32_t x) {
+            const int at = sure_at + min(tie_at, left);
+            if ((x > prefix || (x == prefix && tie_at < left)) && at < keep) dst[at] = i;
+            sure_at += x > prefix;
+            tie_at += x == prefix;
+        };
+        put(j, r.x); put(j + 1, r.y); put(j + 2, r.z); put(j + 3, r.w);
+        incl = __shfl_sync(0xffffffffu, incl, 31);
+        sures_before += incl & 0xffff;
+        ties_before += incl >> 16;
     });
     if (cluster > 1) ssb_cluster_sync();                       // no block leaves while another may read its counts
 }
@@ -486,23 +517,22 @@ int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restri
     constexpr int PIECES = (2 * I8_PAGE * LANES + I8_MOVE_THREADS - 1) / I8_MOVE_THREADS;
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
-    const int to = blockIdx.x, head = blockIdx.y, b = blockIdx.z, s = seq_slot[b];
-    if (s < 0 || s >= n_slots) return;
-    const int target = new_table[(size_t)b * new_pages + to];
-    if (target < 0 || target >= n_pages) return;
+    // what does not wait for anything else is asked for together
+    const int to = blockIdx.x, head = blockIdx.y, b = blockIdx.z, mine = to * I8_PAGE + (int)threadIdx.x;
+    const int s = seq_slot[b], target = new_table[(size_t)b * new_pages + to];
+    const int j = threadIdx.x < I8_PAGE && mine < keep ? kept[((size_t)b * n_kv + head) * keep + mine] : -1;
+    if (s < 0 || s >= n_slots || target < 0 || target >= n_pages) return;
     const int per = I8_PAGE / block;
     __shared__ long long from[I8_PAGE];                        // the row's place among all rows, or -1
     __shared__ float scale[2][I8_PAGE];
     const size_t head_at = (size_t)target * n_kv + head;
     if (threadIdx.x < I8_PAGE) {
-        const int i = to * I8_PAGE + (int)threadIdx.x, j = i < keep ? kept[((size_t)b * n_kv + head) * keep + i] : -1;
         long long row = -1;
         if (j >= 0 && (j >> 6) < max_pages) {
             const int page = page_table[(size_t)s * max_pages + (j >> 6)];
             if (page >= 0 && page < n_pages) row = ((long long)page * n_kv + head) * I8_PAGE + (j & 63);
         }
         from[threadIdx.x] = row;
-        if (weight && row >= 0) weight[head_at * I8_PAGE + threadIdx.x] = weight[row];
     }
     __syncthreads();
     uint4 c[PIECES];
@@ -516,6 +546,9 @@ int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restri
         const int which = threadIdx.x / I8_PAGE, row = threadIdx.x % I8_PAGE;
         const float mine = from[row] >= 0 ? (which ? v_scale : k_scale)[from[row] / block] : 0.f;
         scale[which][row] = mine;
+    } else if (weight && threadIdx.x < 3 * I8_PAGE) {
+        const int row = threadIdx.x - 2 * I8_PAGE;
+        if (from[row] >= 0) weight[head_at * I8_PAGE + row] = weight[from[row]];
     }
     __syncthreads();
 #pragma unroll
@@ -548,9 +581,9 @@ SSB_API int ssb_int8_evict(void* k, void* v, float* k_scale, float* v_scale, flo
         return SSB_ERR_BAD_SIZE;
     // blocks a (sequence, kv head) by the longest sequence there can be
     const long long longest = (long long)max_pages * I8_PAGE;
-    const int cluster = longest <= 8192 ? 1 : longest <= 32768 ? 4 : 8;
-    // a warp's share of a block's places, in whole 32, as the kernel has it for the longest
-    const long long block_most = ((long long)max_pages + cluster - 1) / cluster * I8_PAGE, warp_most = ((block_most + I8_SELECT_WARPS - 1) / I8_SELECT_WARPS + 31) / 32 * 32;
+    const int cluster = longest <= 4096 ? 1 : longest <= 65536 ? 4 : 8;
+    // a warp's share of a block's places, in whole 128, as the kernel has it for the longest
+    const long long block_most = ((long long)max_pages + cluster - 1) / cluster * I8_PAGE, warp_most = ((block_most + I8_SELECT_WARPS - 1) / I8_SELECT_WARPS + 127) / 128 * 128;
     const int held = (int)std::min<long long>(I8_SELECT_KEEP, warp_most * I8_SELECT_WARPS);
     static bool configured = false;
     if (!configured) {

@@ -224,6 +224,42 @@ def test_append(kind, dim, n_q, n_kv, block, rot):
             assert np.array_equal(got.cpu().numpy(), ref)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("counts", [[250, 3, 200, 67], [1] * 300, [2100, 33, 1, 500]])
+def test_append_of_many_tokens(kind, block, counts):
+    """Steps of hundreds and thousands of tokens behind tokens that are there, then one more step of one token each."""
+    from supersonic_b200.csrc import int8_ops
+    rng = np.random.default_rng(len(counts) + block)
+    dtype, n_q, n_kv, dim, rot = TYPES[kind], 3, 2, 64, 64
+    held = [5 + 3 * b % 40 for b in range(len(counts))]
+    cache, table, _ = _random_cache(rng, [h + n + 1 for h, n in zip(held, counts)], n_kv, dim, block)
+    cos, sin = (f(np.arange(2300)[:, None] / 50.0 * np.exp(-np.arange(rot // 2) / 7.0)).astype(np.float32) for f in (np.cos, np.sin))
+    tables = [torch.from_numpy(t).to(DEV) for t in (cos, sin)]
+    for n_new in (counts, [1] * len(counts)):
+        pages, T = _pages_of(cache), sum(n_new)
+        x = rng.normal(size=(T, n_q + 2 * n_kv, dim)) * np.exp(rng.normal(size=(T, 1, 1)))
+        xt = torch.from_numpy(x).to(DEV).to(dtype).reshape(T, -1)
+        x = xt.float().cpu().numpy().reshape(x.shape)
+        place = np.concatenate([np.arange(h, h + n) for h, n in zip(held, n_new)]).astype(np.int32)
+        slot = np.concatenate([np.full(n, b) for b, n in enumerate(n_new)]).astype(np.int32)
+        out = torch.zeros_like(xt)
+        int8_ops.append(xt, *tables, _ints(place), _ints(place), _ints(slot), torch.from_numpy(table).to(DEV), pages, out, n_q)
+        turned = x.copy()
+        turned[:, : n_q + n_kv] = plain.rotate(x[:, : n_q + n_kv], cos[place][:, None], sin[place][:, None])
+        want, row = turned.copy(), 0
+        for b, n in enumerate(n_new):
+            rows = slice(row, row + n)
+            row += n
+            back = cache.append(turned[rows, n_q:n_q + n_kv], turned[rows, n_q + n_kv:], table[b], held[b])
+            want[rows, n_q:n_q + n_kv], want[rows, n_q + n_kv:] = back
+            held[b] += n
+        rounded = torch.from_numpy(want).to(dtype).float().numpy()
+        assert np.array_equal(out.float().cpu().numpy().reshape(want.shape), rounded)
+        for got, ref in zip(pages, (*cache.codes, *cache.scale, cache.weight)):
+            assert np.array_equal(got.cpu().numpy(), ref)
+
+
 def test_append_of_numbers_that_have_no_code():
     from supersonic_b200.csrc import int8_ops
     from supersonic_b200.cache import Int8Pages
@@ -309,6 +345,28 @@ def test_evict_long_sequences(n, keep):
         middle = 4 + np.argsort(-w[4:n - 20], kind="stable")[:keep - 24]
         want = np.sort(np.concatenate([np.arange(4), middle, np.arange(n - 20, n)]))
         assert np.array_equal(kept[0, h].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("n,keep", [(5000, 300), (140001, 6000)])
+def test_evict_with_weights_off_16_bytes(n, keep):
+    """Weights that begin anywhere, in sequences of which a block holds more places than it keeps ranks, too."""
+    from supersonic_b200.cache import Int8Pages
+    from supersonic_b200.csrc import int8_ops
+    rng = np.random.default_rng(n)
+    cache, table, targets = _random_cache(rng, [n], 1, 16, 64, spare=-(-keep // 64))
+    pages = _pages_of(cache)
+    off = torch.zeros(pages.weight.numel() + 1, dtype=torch.float32, device=DEV)
+    weight = off[1:].view(pages.weight.shape)
+    weight.copy_(pages.weight)
+    kept = torch.zeros((1, 1, keep), dtype=torch.int32, device=DEV)
+    int8_ops.evict(Int8Pages(*pages[:4], weight), torch.from_numpy(table).to(DEV), _ints([0]), _ints([n]), torch.from_numpy(targets).to(DEV),
+                   keep, 0, 33, kept)
+    w = cache.weight[table[0], 0].reshape(-1)[:n - 33]
+    want = np.sort(np.concatenate([np.argsort(-w, kind="stable")[:keep - 33], np.arange(n - 33, n)]))
+    got = kept[0, 0].cpu().numpy()
+    assert np.array_equal(got, want)
+    moved = weight.cpu().numpy()[targets[0, :-(-keep // 64)], 0].reshape(-1)[:keep]
+    assert np.array_equal(moved, cache.weight[table[0], 0].reshape(-1)[got])
 
 
 # ---- products ---------------------------------------------------------------------------------------------------------
