@@ -711,7 +711,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
 // Tiles whose pages lay in several blocks' ranges: block c, whose range may begin in the middle of one and end in another, takes its share
 // of each one's sums, half a block a tile: a column's four dims a thread where there are many, else several threads with a part of
 // the pieces each, put together by shuffles.  (A tile a block, whichever had its first page: one sequence of 4,000 tokens, whose 8
-// tiles are 74 pieces each, @@ us.)
+// tiles are 74 pieces each, 34 us instead of 15.)
 template <int HD, int NT, bool WIDE>
 __global__ void __launch_bounds__(IR_THREADS)
 int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __restrict__ pieces) {

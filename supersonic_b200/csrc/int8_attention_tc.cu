@@ -676,9 +676,12 @@ int8_join_kernel(const IaArgs a, int s0, int n_seqs, int parts, const float* __r
     if (d == 0 && a.lse) a.lse[(size_t)row * a.n_q + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// From 64 new tokens of a sequence on: half of a tile's rows.
+// From 17 or 33 new tokens of a sequence on, by the head size.  us with the kernel of rows and with this one, 32 heads over 8: of 128,
+// 16 x 2,000 tokens and 12 new 91 and 99, 16 new 92 and 99, 24 new 126 and 99; 4,000 tokens and 16 new 27 and 30, 24 new 33 and 31; of 64,
+// 16 x 8,000 and 16 new 170 and 330, 32 new 317 and 330; 16,000 and 24 new 46 and 50, 32 new 54 and 50.  (What one sequence holds is not
+// known here: with few keys, 64 x 300 tokens, this one is ahead from 12 new on.)
 bool ia_tc_takes(int dtype, int head_dim, int max_new, float scale) {
-    return dtype == SSB_BF16 && (head_dim == 64 || head_dim == 128) && max_new >= 64 && scale > 0.f;
+    return dtype == SSB_BF16 && (head_dim == 64 || head_dim == 128) && max_new > (head_dim == 128 ? 16 : 32) && scale > 0.f;
 }
 
 // Tiles a unit, and parts that a unit's keys are cut into at most.

@@ -157,12 +157,17 @@ __device__ __forceinline__ void il_mma_pair_x4(uint32_t tmem_d, uint64_t desc_a,
                  "tcgen05.mma.cta_group::2.kind::i8 [%0], a3, b3, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, q;\n}"
                  ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
 }
-__device__ __forceinline__ void il_ld16(uint32_t taddr, int (&r)[16]) {
+template <int N> __device__ __forceinline__ void il_ld16(uint32_t taddr, int (&r)[N], int i) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
                  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "=r"(r[i + 0]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7]),
+                   "=r"(r[i + 8]), "=r"(r[i + 9]), "=r"(r[i + 10]), "=r"(r[i + 11]), "=r"(r[i + 12]), "=r"(r[i + 13]), "=r"(r[i + 14]), "=r"(r[i + 15])
                  : "r"(taddr) : "memory");
+}
+// N columns of the lane's row of tensor memory.
+template <int N> __device__ __forceinline__ void il_ld(uint32_t taddr, int (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 16) il_ld16(taddr + i, r, i);
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float il_result(int sum, float sx, float sw) { return __fmul_rn(__fmul_rn((float)sum, sx), sw); }
@@ -198,7 +203,7 @@ struct IlRange {
 
 template <int BN> constexpr int il_columns() { return 2 * BN < 32 ? 32 : 2 * BN; }
 template <int BN, int STAGES> constexpr size_t il_smem() {
-    return (size_t)STAGES * (IL_BM + BN) * IL_BK + (2 * STAGES + 4) * 8 + 32 + 1024;
+    return (size_t)STAGES * (IL_BM + BN) * IL_BK + 4 * BN * 4 + (2 * STAGES + 4) * 8 + 32 + 1024;
 }
 
 template <int BN, int STAGES>
@@ -208,7 +213,8 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     constexpr uint32_t W_BYTES = IL_BM * IL_BK, X_BYTES = BN * IL_BK, STAGE_BYTES = W_BYTES + X_BYTES;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = (uint64_t*)(smem + STAGES * STAGE_BYTES);      // full[STAGES], empty[STAGES], acc_full[2], acc_empty[2]
+    float* row_scales = (float*)(smem + STAGES * STAGE_BYTES);      // of a tile's rows, an epilogue warp's own
+    uint64_t* bars = (uint64_t*)(row_scales + 4 * BN);              // full[STAGES], empty[STAGES], acc_full[2], acc_empty[2]
     uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 4);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);     // [0]: a role gave up; [1]: stays zero
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -298,13 +304,22 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
     } else {
         ssb_pdl_wait();
+        constexpr int CH = 16;                                    // columns at a time
         const int quarter = warp & 3, in_tile = quarter * 32 + lane;
+        float* scales = row_scales + quarter * BN;
         int i = 0;
         for (long long u = range.begin; u < range.end; ++i) {
             const int tile = (int)(u / k_blocks), kb0 = (int)(u - (long long)tile * k_blocks);
             const int n = (int)min((long long)(k_blocks - kb0), range.end - u), buf = i & 1;
             const int m0 = tile % m_tiles * BN, col = tile / m_tiles * IL_BM + in_tile;       // this thread's output channel
             u += n;
+            // all that does not wait for the sums comes before them: scales, and which blocks have pieces of the tile
+            const int rows = min(BN, o.M - m0);
+            for (int r = lane; r < rows; r += 32) scales[r] = o.sx[m0 + r];
+            const float sw = col < o.N ? o.sw[col] : 0.f;
+            const long long first = (long long)tile * k_blocks;
+            const int c0_block = n == k_blocks ? 0 : range.owner(first), c1_block = n == k_blocks ? 0 : range.owner(first + k_blocks - 1);
+            __syncwarp();
             // the four warps meet below: they go on together or not at all
             if (il_any_of_four(!mbar_wait(acc_full0 + 8 * buf, (i >> 1) & 1, abort_flag))) {
                 if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
@@ -312,67 +327,60 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
             tc_fence_after();
             const uint32_t acc = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
-            const float sw = col < o.N ? o.sw[col] : 0.f;
-            auto finish = [&](int c0, const int (&sum)[16]) {      // 16 rows of x, from tile column c0
-                const int m1 = m0 + c0, live = min(16, o.M - m1);
-                if (live <= 0) return;                             // the same for the whole warp
-                const float mine = o.sx[min(m1 + (lane & 15), o.M - 1)];
-                float y[16];
+            // a block's pieces: of the tile that its range begins in the middle of (or that is all it has), and of its last; four
+            // columns of a channel lie together
+            auto piece = [&](int c) { return reinterpret_cast<int4*>(pieces) + (size_t)(2 * c + (c == c0_block)) * (BN / 4) * IL_BM + in_tile; };
+            bool mine = true;                                      // whether this block writes the tile's results
+            if (n < k_blocks) {
+                int4* dst = piece(blockIdx.x);
+#pragma unroll 1
+                for (int c0 = 0; c0 < rows; c0 += CH) {
+                    int sum[CH];
+                    il_ld<CH>(acc + c0, sum);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = il_result(sum[e], __shfl_sync(0xffffffffu, mine, e), sw);
-                if (col >= o.N) return;
-                if (!o.is_f32) {
-                    bf16* dst = (bf16*)o.out + (size_t)m1 * o.ldo + col;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (e < live) dst[(size_t)e * o.ldo] = __float2bfloat16_rn(y[e]);
-                } else {
-                    float* dst = (float*)o.out + (size_t)m1 * o.ldo + col;
-                    if (o.add) {
-                        float was[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) was[e] = e < live ? dst[(size_t)e * o.ldo] : 0.f;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) y[e] += was[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (e < live) dst[(size_t)e * o.ldo] = y[e];
-                }
-            };
-            const int rows = min(BN, o.M - m0);
-            if (n == k_blocks) {
-                for (int c0 = 0; c0 < rows; c0 += 16) {
-                    int sum[16];
-                    il_ld16(acc + c0, sum);
-                    finish(c0, sum);
-                }
-            } else {
-                // a block's pieces: of the tile that its range begins in the middle of (or that is all it has), and of its last
-                const long long first = (long long)tile * k_blocks;
-                const int c0_block = range.owner(first), c1_block = range.owner(first + k_blocks - 1);
-                auto piece = [&](int c) { return pieces + ((size_t)(2 * c + (c == c0_block)) * BN) * IL_BM + in_tile; };
-                int* mine = piece(blockIdx.x);
-                for (int c0 = 0; c0 < rows; c0 += 16) {
-                    int sum[16];
-                    il_ld16(acc + c0, sum);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) mine[(size_t)(c0 + e) * IL_BM] = sum[e];
+                    for (int e = 0; e < CH; e += 4)
+                        if (c0 + e < rows) dst[(size_t)((c0 + e) / 4) * IL_BM] = make_int4(sum[e], sum[e + 1], sum[e + 2], sum[e + 3]);
                 }
                 __threadfence();
                 il_any_of_four(false);
-                const bool last = il_any_of_four(threadIdx.x == 64 && atomicAdd(arrived + c0_block, n) + n == k_blocks);
-                if (last) {
-                    __threadfence();
-                    for (int c0 = 0; c0 < rows; c0 += 16) {
-                        int sum[16] = {};
-                        for (int c = c0_block; c <= c1_block; ++c) {
-                            const int* src = piece(c) + (size_t)c0 * IL_BM;
+                mine = il_any_of_four(threadIdx.x == 64 && atomicAdd(arrived + c0_block, n) + n == k_blocks);
+                if (mine) __threadfence();
+            }
+#pragma unroll 1
+            for (int c0 = 0; mine && c0 < rows; c0 += CH) {        // rows of x
+                const int live = col < o.N ? rows - c0 : 0;
+                const size_t at = (size_t)(m0 + c0) * o.ldo + col;
+                float was[CH];
+                if (o.add)
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) sum[e] += __ldcg(src + (size_t)e * IL_BM);
+                    for (int e = 0; e < CH; ++e) was[e] = e < live ? ((const float*)o.out)[at + (size_t)e * o.ldo] : 0.f;
+                int sum[CH];
+                if (n == k_blocks) {
+                    il_ld<CH>(acc + c0, sum);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) sum[e] = 0;
+#pragma unroll 4
+                    for (int c = c0_block; c <= c1_block; ++c) {
+                        const int4* src = piece(c) + (size_t)(c0 / 4) * IL_BM;
+#pragma unroll
+                        for (int e = 0; e < CH; e += 4) {
+                            const int4 v = c0 + e < rows ? __ldcg(src + (size_t)(e / 4) * IL_BM) : make_int4(0, 0, 0, 0);
+                            sum[e] += v.x; sum[e + 1] += v.y; sum[e + 2] += v.z; sum[e + 3] += v.w;
                         }
-                        finish(c0, sum);
                     }
+                }
+                float y[CH];
+#pragma unroll
+                for (int e = 0; e < CH; ++e) y[e] = il_result(sum[e], scales[c0 + e], sw);
+                if (!o.is_f32) {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e)
+                        if (e < live) ((bf16*)o.out)[at + (size_t)e * o.ldo] = __float2bfloat16_rn(y[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e)
+                        if (e < live) ((float*)o.out)[at + (size_t)e * o.ldo] = o.add ? y[e] + was[e] : y[e];
                 }
             }
             tc_fence_before();
@@ -576,22 +584,45 @@ struct IlPlan {
     int bn, m_tiles, n_tiles, blocks;      // bn 0: tiles on pairs
     size_t counters, pieces;               // in scratch, behind the rows' scales (bytes)
 };
+// The kernel, its tile and its blocks, by what they are estimated to take (us; k-blocks of 128 codes):
+//  * a block of the streaming kernel 0.36 a k-block, 0.45 with 128 rows a tile, 0.6 where those are all there are (nothing then shares
+//    a fetch of weights); beginning and ending 9; the pieces of a tile 0.012 a piece and row, and 4 where tiles are cut wherever a
+//    block's share ends instead of into equal parts;
+//  * a pair 0.37 a k-block of 256 x 256, 8 for beginning and ending, 0.09 a tile that begins cold.
+// Parts have four k-blocks at least, eight in tiles of 64 rows and more, whose pieces are larger.  us measured on both sides, rows x
+// channels x k: shares that end anywhere and equal parts, 1 x 16,384 x 2,048 12.4 and 9.6, 8 x 4,096 x 4,096 10.2 and 8.8, 72 x 16,384
+// x 2,048 21.3 and 14.2; parts of four and of eight, 1 x 2,048 x 2,048 7.0 and 8.4, 72 x 1,024 x 4,096 (64 rows a tile) 13.9 and 13.0;
+// tiles of 64 rows, of 128, and pairs, 72 x 28,672 x 4,096 45, 36 and 36, 128 x 1,024 x 4,096 13.8, 19.3 and 18.8, 128 x 28,672 x 4,096
+// 49, 45 and 38, 256 x 4,096 x 14,336 47, 41 and 50, 512 x 4,096 x 4,096 29, 33 and 22.  Tiles of 256 rows in the streaming kernel were
+// behind one of these everywhere (256 x 4,096 x 14,336 49).
 static IlPlan il_plan(int M, int N, int K) {
-    IlPlan p{};
     const int sms = ssb_sm_count(), k_blocks = (K + IL_BK - 1) / IL_BK;
-    const long long pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256);
-    if (M > 256 && pair_tiles >= sms / 4) {
-        p.m_tiles = (M + 255) / 256;
-        p.n_tiles = (N + 255) / 256;
-        return p;
+    IlPlan best{};
+    double least = 0;
+    auto consider = [&](double cost, int bn, int m_tiles, int n_tiles, int blocks) {
+        if (best.m_tiles && cost >= least) return;
+        least = cost;
+        best = IlPlan{bn, m_tiles, n_tiles, blocks, (size_t)blocks * 4, (size_t)blocks * 2 * bn * IL_BM * 4};
+    };
+    for (int bn = M <= 16 ? 16 : M <= 32 ? 32 : 64; bn <= 128; bn *= 2) {
+        const int m_tiles = (M + bn - 1) / bn, n_tiles = (N + IL_BM - 1) / IL_BM;
+        const long long tiles = (long long)m_tiles * n_tiles, units = tiles * k_blocks;
+        const double each = bn < 128 ? 0.36 : m_tiles == 1 ? 0.6 : 0.45;
+        const double piece = 0.012 * std::min(bn, M);
+        const int any = (int)std::min<long long>(sms, std::max(1LL, units / 4));
+        consider(9 + each * (double)((units + any - 1) / any) + 4 + piece * (double)((any + tiles - 1) / tiles), bn, m_tiles, n_tiles, any);
+        if (tiles <= sms) {
+            const int parts = std::min(sms / (int)tiles, std::max(1, k_blocks / (bn <= 32 ? 4 : 8)));
+            consider(9 + each * ((k_blocks + parts - 1) / parts) + (parts > 1 ? piece * parts : 0), bn, m_tiles, n_tiles, (int)tiles * parts);
+        }
+        if (M <= bn) break;
     }
-    p.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-    p.m_tiles = (M + p.bn - 1) / p.bn;
-    p.n_tiles = (N + IL_BM - 1) / IL_BM;
-    p.blocks = (int)std::min<long long>(sms, std::max<long long>(1, (long long)p.m_tiles * p.n_tiles * k_blocks / 4));
-    p.counters = (size_t)p.blocks * 4;
-    p.pieces = (size_t)p.blocks * 2 * p.bn * IL_BM * 4;
-    return p;
+    if (M > 64) {
+        const int m_tiles = (M + 255) / 256, n_tiles = (N + 255) / 256, pairs = sms / 2;
+        const long long tiles = (long long)m_tiles * n_tiles;
+        consider(8 + 0.37 * (double)((tiles + pairs - 1) / pairs) * k_blocks + 0.09 * (double)std::min<long long>(tiles, pairs), 0, m_tiles, n_tiles, 0);
+    }
+    return best;
 }
 static size_t il_round(size_t n) { return (n + 127) & ~(size_t)127; }
 
@@ -642,7 +673,6 @@ SSB_API int ssb_int8_linear(const void* x, int ldx, int dtype, const void* w, in
         case 32: return il_stream<32, 10>(mw, mx, o, p, K, counters, pieces, error_word, stream);
         case 64: return il_stream<64, 8>(mw, mx, o, p, K, counters, pieces, error_word, stream);
         case 128: return il_stream<128, 6>(mw, mx, o, p, K, counters, pieces, error_word, stream);
-        case 256: return il_stream<256, 4>(mw, mx, o, p, K, counters, pieces, error_word, stream);
     }
     static int max_pairs = 0;
     if (!max_pairs) {
