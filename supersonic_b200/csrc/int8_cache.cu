@@ -55,7 +55,9 @@ template <typename T, int LANES, bool KV, bool Q>
 __global__ void __launch_bounds__(32 * I8_APPEND_WARPS, KV ? 4 : 8)
 int8_append_kernel(const I8Append a) {
     constexpr int ROWS = 32 / LANES, KEEP = 4, HD = 16 * LANES;
-    ssb_pdl_wait();
+    // queries that follow the keys' launch touch nothing of its, and what it waited for is there: they wait for it at their end, so
+    // that they run beside its last blocks and whoever waits for them has waited for both
+    if (KV) ssb_pdl_wait();
     ssb_pdl_launch_dependents();
     const int lane = threadIdx.x & 31, l = lane % LANES, r_of = lane / LANES, half = a.rot / 2;
     const bool turned = a.cos_t != nullptr && l < a.rot / 16;
@@ -90,22 +92,24 @@ int8_append_kernel(const I8Append a) {
     };
     if (Q && queries) {
         const int blocks = (a.n_q + I8_Q_HEADS - 1) / I8_Q_HEADS, head0 = w % blocks * I8_Q_HEADS, row = w / blocks * ROWS + r_of;
-        if (row >= a.T) return;
-        const int sl = a.slot[row], pl = a.place[row];
-        float c[8], s[8];
-        const bool turns = tables(turned ? a.pos[row] : -1, c, s);
-        const T* src = (const T*)a.qkv + (size_t)row * a.ldq;
-        T* dst = (T*)a.out + (size_t)row * a.ldo;
-        if (sl < 0 || sl >= a.n_slots || pl < 0 || (pl >> 6) >= a.max_pages) return;
+        if (row < a.T) {
+            const int sl = a.slot[row], pl = a.place[row];
+            float c[8], s[8];
+            const bool turns = tables(turned ? a.pos[row] : -1, c, s);
+            const T* src = (const T*)a.qkv + (size_t)row * a.ldq;
+            T* dst = (T*)a.out + (size_t)row * a.ldo;
+            if (sl >= 0 && sl < a.n_slots && pl >= 0 && (pl >> 6) < a.max_pages)
 #pragma unroll 4
-        for (int h = head0; h < min(head0 + I8_Q_HEADS, a.n_q); ++h) {
-            float x[8], y[8];
-            i8_load8(src + h * HD + e0, x);
-            i8_load8(src + h * HD + e1, y);
-            if (turns) turn(x, y, c, s);
-            i8_store8(dst + h * HD + e0, x);
-            i8_store8(dst + h * HD + e1, y);
+                for (int h = head0; h < min(head0 + I8_Q_HEADS, a.n_q); ++h) {
+                    float x[8], y[8];
+                    i8_load8(src + h * HD + e0, x);
+                    i8_load8(src + h * HD + e1, y);
+                    if (turns) turn(x, y, c, s);
+                    i8_store8(dst + h * HD + e0, x);
+                    i8_store8(dst + h * HD + e1, y);
+                }
         }
+        if (!KV) ssb_pdl_wait();
         return;
     }
     if (!KV) return;
@@ -131,8 +135,7 @@ int8_append_kernel(const I8Append a) {
     }
     for (; leads; leads &= leads - 1) {
         const int at = __ffs(leads) - 1, lead = row0 + at;
-        const int s0 = __shfl_sync(0xffffffffu, my_slot, at), p0 = __shfl_sync(0xffffffffu, my_place, at), page = __shfl_sync(0xffffffffu, my_page, at);
-        if (page < 0) continue;
+        const int s0 = __shfl_sync(0xffffffffu, my_slot, at), p0 = __shfl_sync(0xffffffffu, my_place, at);
         const int in_block = p0 & (a.block - 1), in_page = p0 & (I8_PAGE - 1), most_n = a.block - in_block;
         // rows that go on from the first: in the chunk by its lanes, behind it (a run may cross its end) by asking
         const unsigned after = at == 31 ? 0u : goes_on >> (at + 1);
@@ -147,10 +150,6 @@ int8_append_kernel(const I8Append a) {
                 more = got == 32 && n < most_n;
             }
         }
-        const size_t head_at = (size_t)page * a.n_kv + kvh;
-        const int per = I8_PAGE / a.block;
-        float* scale_at = a.scale[which] + head_at * per + in_page / a.block;
-        const float old = in_block ? *scale_at : 0.f;
         float x[KEEP][8], y[KEEP][8];
         uint32_t top = 0;
         bool wild = false;                                     // a number of the run is none, or too large
@@ -184,6 +183,13 @@ int8_append_kernel(const I8Append a) {
         };
         const int last = (n - 1) / (KEEP * ROWS) * (KEEP * ROWS);
         for (int first = 0; first <= last; first += KEEP * ROWS) load(first);
+        // the page only now: the rows do not wait for its id
+        const int page = __shfl_sync(0xffffffffu, my_page, at);
+        if (page < 0) continue;
+        const size_t head_at = (size_t)page * a.n_kv + kvh;
+        const int per = I8_PAGE / a.block;
+        float* scale_at = a.scale[which] + head_at * per + in_page / a.block;
+        const float old = in_block ? *scale_at : 0.f;
         top = __reduce_max_sync(0xffffffffu, top);
         if (top >= I8_WILD) {
             wild = true;
@@ -348,7 +354,8 @@ __device__ __forceinline__ int i8_cluster_int(const int* mine, unsigned rank) {
 // at a time, by counting (every block adds the cluster's counts up for itself), then every warp writes its places behind those of the
 // warps and blocks before it.  Ranks lie in shared memory, four places a lane and turn, and the loops over them stay loops: 32 ranks a
 // thread in registers, every loop unrolled, is code that runs once, and took longer to fetch than to run (sequences of 700 tokens 9 us
-// and 32).  What bounds it is the instructions of those loops: @@
+// and 32).  What bounds it is the time of its phases one after another (fetching, three counts with the cluster's sums, two walks):
+// 4 x 8 selections among 60,000 to 131,000 places 34 us, with a place a lane and turn 40; 12 MB of weights would be read in 2.
 __global__ void __launch_bounds__(I8_SELECT_THREADS, 2)
 int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ page_table, int n_slots, int max_pages, int n_pages,
                    const int* __restrict__ seq_slot, const int* __restrict__ lengths, int n_kv, int keep, int first, int recent,
@@ -507,7 +514,8 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
 constexpr int I8_MOVE_THREADS = 256;
 
 // The kept tokens of one destination page and kv head: codes under the largest scale of their new block, weights beside them.  A
-// thread's pieces of codes are on their way while the block's scales are compared.
+// thread's pieces of codes are on their way while the block's scales are compared.  4 x 8 times 4,096 tokens of 128: 67 MB in 25 us,
+// 2.7 TB/s; bound by fetches that wait for one another (the place, its page, the codes and scale under it).
 template <int LANES>
 __global__ void __launch_bounds__(I8_MOVE_THREADS)
 int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restrict__ k_scale, float* __restrict__ v_scale,
@@ -579,7 +587,9 @@ SSB_API int ssb_int8_evict(void* k, void* v, float* k_scale, float* v_scale, flo
     if (head_dim % 16 || head_dim <= 0 || n_kv <= 0 || (block != 16 && block != 32 && block != 64) || keep <= 0 || first < 0 ||
         recent < 0 || (long long)first + recent > keep || (long long)new_pages * I8_PAGE < keep || n_seqs > 65535 || n_kv > 65535)
         return SSB_ERR_BAD_SIZE;
-    // blocks a (sequence, kv head) by the longest sequence there can be
+    // blocks a (sequence, kv head) by the longest sequence there can be.  us of selecting 512 and moving them with 1, 4 and 8 blocks (a
+    // place a lane and turn): 8 x 4,000 places 32.8, 32.5 and 48; 8 x 8,000 38.8, 35.2 and 51; 8 x 32,000 117, 45 and 62; 64,000 179,
+    // 35.7 and 33.3; 4 x 131,000 503, 122 and 83.  Above 65,536 the ranks of four blocks' places do not fit their shared memory.
     const long long longest = (long long)max_pages * I8_PAGE;
     const int cluster = longest <= 4096 ? 1 : longest <= 65536 ? 4 : 8;
     // a warp's share of a block's places, in whole 128, as the kernel has it for the longest
