@@ -134,7 +134,9 @@ int8_weigh_plain_kernel(const IaArgs a) {
 // others go to scratch, and int8_finish_kernel puts them together in the order of the keys.  Nothing is left from one launch
 // to the next.
 constexpr int IR_THREADS = 128, IR_WARPS = 4, IR_SEQS = 1024, IR_STAGES = 3;
-constexpr int IR_EXTRA = 3;
+// What beginning and ending a tile costs, in pages.  us with 0, 1, 3, 6, 8 and 11: 64 sequences of 1 to 8,192 135, 130, 110, 102.6, 105
+// and 109; 32 of 20 to 4,000 (64 dims) 51, 39, 31, 29.9, 30.9 and 32.7; 64 of 2,000 with 3, 6 and 11 58.4, 59.8 and 60.7.
+constexpr int IR_EXTRA = 6;
 constexpr long long IR_KEPT_MOST = 1LL << 26;  // floats
 constexpr float IR_NONE = -1e30f;               // a maximum over no key: finite, so that nothing below needs to ask for it
 constexpr int IR_SIDE = 12;                  // beside a stage's page: its scales of keys and of values, and its id
@@ -474,6 +476,11 @@ __device__ __forceinline__ void ir_put(const IaArgs& a, const IrSeq& s, int tile
     if (d == 0 && a.lse) a.lse[row * a.n_q + head] = l == 0.f ? -INFINITY : (m - offset + log2f(l)) * 0.6931471805599453f;
 }
 
+// Single tokens and few rows.  64 sequences of 1 to 8,192 tokens, 32 heads over 8 of 128, bfloat16: 102 us with the joining, 5.5 TB/s, bound by the pages
+// in flight (three a block, four blocks an SM); 16 of 8,000, 32 over 8 of 64, float32: 45 us, 3 TB/s, by instructions (a page has half
+// the bytes there, and probabilities go in two halves).  NT, tiles of 8 columns: the fewest that hold the group (and up to 4 where
+// neighbouring tokens fill them): 8 x 4,000 single tokens of a group of 4 with 1, 2 and 4 tiles 28, 38 and 57 us, four new tokens 39, 39
+// and 58.
 template <int HD, int NT, bool WIDE>
 __global__ void __launch_bounds__(IR_THREADS, NT == 1 ? 4 : 2)
 int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict__ pieces, float* __restrict__ kept, int* __restrict__ error_word,
@@ -783,6 +790,7 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
 }
 
 // What single tokens attend to, from the scores that int8_rows_kernel kept: a page a warp, a lane four keys of every second head.
+// 16 sequences of 8,000, 32 heads over 8: 17 MB of scores in 13 us.
 __global__ void __launch_bounds__(IR_THREADS)
 int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict__ kept) {
     extern __shared__ unsigned char smem_raw[];
@@ -1030,7 +1038,7 @@ static int ir_rows(const IaArgs& a, const IrPlan& p, float* pieces, int* error_w
     for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
         const int n = std::min(IR_SEQS, a.n_seqs - s0);
         // not as a dependent of what came before: blocks that wait beside another launch's are dealt to SMs unevenly (64 sequences of
-        // 1 to 8,192 tokens, one call behind another: 111 us, 162 as dependents)
+        // 1 to 8,192 tokens, one call behind another: 111 us, 162 as dependents, when a tile's cost was counted as 3 pages)
         int rc = ssb_launch(int8_rows_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), ir_smem<HD, NT>(n), stream, false, a, s0, n, p.tts,
                             pieces, kept, error_word, mk, mv);
         if (rc) return rc;

@@ -49,8 +49,8 @@ constexpr int I8_APPEND_WARPS = 4, I8_Q_HEADS = 8;
 //    whether they begin one: 18,000 rows of 48 heads 153 us).
 //  * queries: ROWS rows of up to 8 heads, the rotation tables' rows read once for all of them.
 // KV, Q: which kinds of warps the launch has; where there are many rows each kind has a launch of its own, and its own number of registers.
-// 17,000 rows of 32 heads over 8 of 128 in bfloat16: 64 us for keys and values, bound by the instructions of rotating, rounding and
-// writing them, and 42 us for queries, at the rate of a copy.
+// 14,800 rows of 32 heads over 8 of 128 in bfloat16: 60 us for keys and values, 2.5 TB/s, bound by fetches one after another (places, rows,
+// tables) under four warps a scheduler; 43 us for queries, 5.7 TB/s.
 template <typename T, int LANES, bool KV, bool Q>
 __global__ void __launch_bounds__(32 * I8_APPEND_WARPS, KV ? 4 : 8)
 int8_append_kernel(const I8Append a) {
@@ -273,7 +273,8 @@ SSB_API int ssb_int8_append(const void* qkv, int ldq, int dtype, void* out, int 
 }
 
 // ---- values back ----------------------------------------------------------------------------------------------------
-// out[b, i, head] = values of token i of sequence b, i < lengths[b] (and < most); 16 numbers a thread.
+// out[b, i, head] = values of token i of sequence b, i < lengths[b] (and < most); 16 numbers a thread.  4 x 4,096 tokens of 8 heads of
+// 128 to bfloat16: 101 MB in 22 us, 4.6 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256)
 int8_read_kernel(const int8_t* __restrict__ k, const int8_t* __restrict__ v, const float* __restrict__ k_scale,
