@@ -424,6 +424,26 @@ def test_linear_of_the_largest_sums(rows):
     assert (out[:, 3] == float(want)).all() and (out[:, 0] == -float(want)).all()
 
 
+@pytest.mark.parametrize("n,k", [(1024, 4096), (4096, 1152), (28672, 1024), (2056, 8208), (16384, 2048), (520, 14336)])
+@pytest.mark.parametrize("rows", [1, 9, 31, 50, 72, 128, 200, 320, 700])
+def test_linear_has_the_formulas_bits_however_it_is_cut(rows, n, k):
+    """Whole tiles, equal parts of tiles, shares that end anywhere and pairs: exact sums, then the formula's two float32 products."""
+    from supersonic_b200.csrc import int8_ops
+    gen = torch.Generator(device=DEV).manual_seed(rows + n)
+    x = torch.randn((rows, k), generator=gen, device=DEV).to(torch.bfloat16)
+    w = torch.randint(-127, 128, (n, k), generator=gen, device=DEV, dtype=torch.int8)
+    sw = torch.rand((n,), generator=gen, device=DEV) + 0.01
+    codes, scales = torch.zeros((rows, k), dtype=torch.int8, device=DEV), torch.zeros(rows, device=DEV)
+    int8_ops.quantize_rows(x, codes, scales)
+    sums = torch.cat([codes.double() @ part.double().T for part in w.split(4096)], dim=1)      # whole numbers below 2^53: exact
+    want = sums.float() * scales[:, None] * sw
+    base = torch.randn((rows, n), generator=gen, device=DEV)
+    out, added = torch.full((rows, n), float("nan"), device=DEV), base.clone()
+    int8_ops.linear(x, w, sw, out)
+    int8_ops.linear(x, w, sw, added, accumulate=True)
+    assert torch.equal(out, want) and torch.equal(added, want + base)
+
+
 def test_linear_reads_and_writes_parts_of_wider_matrices():
     from supersonic_b200.csrc import int8_ops
     x = torch.randn((70, 512), device=DEV).bfloat16()
