@@ -4,6 +4,7 @@
 // with codes kc, vc and their blocks' scales ks, vs.  The rows that keep account add exp(s_ij - lse_i), summed over the query
 // heads of a kv head, to the weight of key j.
 #include "int8_attention.cuh"
+#include "packed_call.cuh"
 #include "tc_helpers.cuh"
 #include <cuda_fp16.h>
 #include <math.h>
@@ -1129,3 +1130,5 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
 #undef IR_ROWS
     return rc || weigh_last <= 0 || p.kept ? rc : ia_weigh(a, wide, max_new, error_word, mk, stream);
 }
+
+SSB_PACKED(ssb_int8_attention)

@@ -10,6 +10,7 @@
 // The reference keeps keys in int8 and values in int4 for one of its lanes, a scale per block of tokens and channel
 // (kernels/certified_kv_bridge_cuda.cu:32-420); this cache has one scale per block of tokens and head, and both in int8.
 #include "int8_codes.cuh"
+#include "packed_call.cuh"
 #include <algorithm>
 
 typedef __nv_bfloat16 bf16;
@@ -621,3 +622,7 @@ SSB_API int ssb_int8_evict(void* k, void* v, float* k_scale, float* v_scale, flo
 #undef I8_MOVE
     return SSB_ERR_BAD_SIZE;
 }
+
+SSB_PACKED(ssb_int8_append)
+SSB_PACKED(ssb_int8_read)
+SSB_PACKED(ssb_int8_evict)

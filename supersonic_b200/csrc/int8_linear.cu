@@ -12,6 +12,7 @@
 // The reference's 8-bit lane of this architecture multiplies int8 weights by activations of the model's type
 // (crates/runner/src/llama31_engine.rs:289-430).
 #include "int8_codes.cuh"
+#include "packed_call.cuh"
 #include "tc_helpers.cuh"
 #include "tc_rows.cuh"
 #include <algorithm>
@@ -702,3 +703,6 @@ SSB_API int ssb_int8_linear(const void* x, int ldx, int dtype, const void* w, in
     return ssb_launch(int8_pair_kernel, dim3(2 * pairs), dim3(IL_THREADS), IL_PAIR_SMEM, stream, true, mx, mw, o, p.m_tiles, p.n_tiles,
                       (K + IL_BK - 1) / IL_BK, std::min(16, p.m_tiles), error_word);
 }
+
+SSB_PACKED(ssb_int8_quantize_rows)
+SSB_PACKED(ssb_int8_linear)

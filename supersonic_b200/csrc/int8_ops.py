@@ -10,7 +10,8 @@ The modelled project's 8-bit lanes: an int8/int4 tiered cache (kernels/certified
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
+from struct import Struct, error as StructError
 from typing import Optional, Tuple
 
 import torch
@@ -18,7 +19,7 @@ import torch
 from ..cache import Int8Pages
 from . import ops
 from .build import load_library
-from .ops import KernelError, _CODES, _check, _stream
+from .ops import KernelError, _CODES, _check
 
 _P, _I, _F = c_void_p, c_int, c_float
 _SIGNATURES = {
@@ -33,17 +34,29 @@ _SIGNATURES = {
     "ssb_int8_linear": ("int8_linear", [_P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
     "ssb_int8_linear_scratch": ("int8_linear", [_I, _I, _I]),
 }
+_FORMATS = {_P: "P", _I: "i", _F: "f"}
 _functions = {}
 
 
 def _fn(name: str):
-    """The library's function with its argument types set: ctypes then converts plain integers itself, at a fraction of the cost
-    of one object an argument."""
+    """The library's function.  Arguments of a launch go as one run of bytes (packed_call.cuh): one conversion instead of up to 31, at a
+    third of the cost; a number that its type does not hold is an error."""
     f = _functions.get(name)
     if f is None:
         library, types = _SIGNATURES[name]
-        f = getattr(load_library(library), name)
-        f.restype, f.argtypes = c_longlong if name.endswith("_scratch") else c_int, types
+        if name.endswith("_scratch"):
+            f = getattr(load_library(library), name)
+            f.restype, f.argtypes = c_longlong, types
+        else:
+            call, pack = getattr(load_library(library), name + "_packed"), Struct("@" + "".join(_FORMATS[t] for t in types)).pack
+            call.restype, call.argtypes = c_int, [c_char_p]
+
+            def f(*args):
+                try:
+                    packed = pack(*args)
+                except (StructError, OverflowError) as e:
+                    raise KernelError(f"{name}: {e}") from None
+                return call(packed)
         _functions[name] = f
     return f
 
@@ -79,21 +92,30 @@ def _pages(pages: Int8Pages, table: torch.Tensor):
     its table's address, rows and width.  One condition over all of it: this runs in every call of a decode step."""
     k, v, ks, vs, weight = pages
     shape, scales, tab = k.shape, ks.shape, table.shape
-    if (len(shape) == 4 and v.shape == shape and shape[2] == 64 and shape[3] in _DIMS and k.dtype is _INT8 and v.dtype is _INT8
-            and k.is_cuda and v.is_cuda and k.is_contiguous() and v.is_contiguous()
-            and len(scales) == 3 and vs.shape == scales and scales[:2] == shape[:2] and scales[2] in (1, 2, 4)
-            and ks.dtype is _FLOAT32 and vs.dtype is _FLOAT32 and ks.is_cuda and vs.is_cuda and ks.is_contiguous() and vs.is_contiguous()
-            and (weight is None or (weight.shape == shape[:3] and weight.dtype is _FLOAT32 and weight.is_cuda and weight.is_contiguous()))
-            and table.dtype is _INT32 and len(tab) == 2 and table.is_cuda and table.is_contiguous()):
-        k_at, v_at = k.data_ptr(), v.data_ptr()
-        if (k_at | v_at) % 16 == 0:
-            at = (k_at, v_at, ks.data_ptr(), vs.data_ptr(), 0 if weight is None else weight.data_ptr())
-            return shape[0], shape[1], shape[3], 64 // scales[2], at, table.data_ptr(), tab[0], tab[1]
+    if len(shape) == 4 and len(scales) == 3 and len(tab) == 2:
+        n_pages, n_kv, page, dim = shape
+        scale_pages, scale_heads, per = scales
+        if (page == 64 and dim in _DIMS and v.shape == shape and k.dtype is _INT8 and v.dtype is _INT8
+                and k.is_cuda and v.is_cuda and k.is_contiguous() and v.is_contiguous()
+                and scale_pages == n_pages and scale_heads == n_kv and per in (1, 2, 4) and vs.shape == scales
+                and ks.dtype is _FLOAT32 and vs.dtype is _FLOAT32 and ks.is_cuda and vs.is_cuda and ks.is_contiguous() and vs.is_contiguous()
+                and (weight is None or (weight.shape == (n_pages, n_kv, 64) and weight.dtype is _FLOAT32 and weight.is_cuda
+                                        and weight.is_contiguous()))
+                and table.dtype is _INT32 and table.is_cuda and table.is_contiguous()):
+            k_at, v_at = k.data_ptr(), v.data_ptr()
+            if (k_at | v_at) % 16 == 0:
+                at = (k_at, v_at, ks.data_ptr(), vs.data_ptr(), 0 if weight is None else weight.data_ptr())
+                return n_pages, n_kv, dim, 64 // per, at, table.data_ptr(), tab[0], tab[1]
     raise KernelError(
         "pages: k and v must be int8 [pages, kv heads, 64, 16 32 64 128 or 256], their scales float32 [pages, kv heads, 4 2 or 1], weight "
         "float32 [pages, kv heads, 64] or None, the page table int32 [rows, pages a sequence], all contiguous on a CUDA device; are "
         f"{k.dtype} {tuple(shape)}, {v.dtype} {tuple(v.shape)}, {ks.dtype} {tuple(scales)}, {vs.dtype} {tuple(vs.shape)}, "
         f"{None if weight is None else (weight.dtype, tuple(weight.shape))} and {table.dtype} {tuple(tab)}")
+
+
+def _stream() -> int:
+    """The current stream's handle."""
+    return ops._stream().value or 0
 
 
 _error_words = {}
