@@ -695,9 +695,9 @@ static ItPlan it_plan(int n_seqs, int rows, int max_new, int max_pages, int n_q,
     const long long most = std::min({turns / 4, 16LL, (1LL << 26) / ((long long)rows * n_q * (head_dim + 2))});
     // Of one or two tiles a unit and the numbers of parts, what is done first: rounds of the SMs times the turns of a part, and three
     // more for its beginning and end.  A turn of two tiles is 1.65 of one's at head size 128; at 64, where single tiles run two blocks
-    // an SM, the same, and one that has its SM to itself 0.78.  us with one tile and with two, heads x size: 500 tokens behind 16,001, 32 x 64 184 and 181, 32 x 128 314 and
-    // 196; 300 behind 3,000, 8 x 64 23.3 and 28.2, 8 x 128 27.8 and 33.8; two of 600 behind 1,000, 32 x 128 90 and 98, 32 x 64 67 and 73; four of 2,048,
-    // 32 x 128 323 and 206, 32 x 64 192 and 184.
+    // an SM, the same, and one that has its SM to itself 0.78.  us with one tile and with two, heads x size: 500 tokens behind 16,001,
+    // 32 x 64 184 and 181, 32 x 128 314 and 196; 300 behind 3,000, 8 x 64 23.3 and 28.2, 8 x 128 27.8 and 33.8; two of 600 behind
+    // 1,000, 32 x 128 90 and 98, 32 x 64 67 and 73; four of 2,048, 32 x 128 323 and 206, 32 x 64 192 and 184.
     ItPlan p{};
     double best = 0;
     for (int tiles = 2; tiles >= 1; --tiles) {

@@ -220,7 +220,7 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
               lse: Optional[torch.Tensor] = None, weigh_last: int = 0) -> None:
     """Causal attention of packed sequences over an 8-bit cache that holds the step's keys already.  ``q`` and ``out`` [rows,
     n_q x head size]; sequence b brings rows ``cu_new[b]`` to ``cu_new[b + 1]`` (at most ``max_new``; none is allowed), held
-    ``seq_start[b]`` tokens before them, and its row i sees the keys at places start + i - ``window`` + 1 (None: 0) to start + i.
+    ``seq_start[b]`` tokens before them, and its row i sees the keys at places start + i - ``window`` + 1 (None or 0: 0) to start + i.
     ``lse`` (float32 [rows, n_q]) gets the logarithm of a row's sum of exponentials.  ``weigh_last``: that many last rows of every
     sequence add their probabilities, summed over the query heads of a kv head, to ``pages.weight``.  Rows of a sequence with a
     negative slot are zeros, and their ``lse`` minus infinity."""
@@ -238,8 +238,8 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
         lse = torch.empty((rows, n_q), dtype=_FLOAT32, device=q.device)
     if rows == 0 or B == 0:
         return
-    if max_new <= 0:
-        raise KernelError(f"attention: max_new {max_new} new tokens")
+    if max_new <= 0 or (window or 0) < 0:
+        raise KernelError(f"attention: max_new {max_new} new tokens, window {window}")
     code, device = _CODES[q.dtype], q.device
     scratch = torch.empty(_scratch_size("ssb_int8_attention_scratch", code, B, rows, max_new, width, n_q, n_kv, dim, weigh_last, scale),
                           dtype=_FLOAT32, device=device)

@@ -499,3 +499,13 @@ def test_attention_of_a_few_tokens_a_sequence(kind):
     rng = np.random.default_rng(11)
     for n_q, n_kv, dim in ((4, 1, 64), (6, 2, 128), (8, 8, 64), (16, 1, 128)):
         _check_attention(rng, [300, 61, 0, 1000], [3, 7, 16, 33], n_q, n_kv, dim, 32, kind, weigh=5)
+
+
+def test_numbers_that_do_not_fit_their_type_are_refused():
+    from supersonic_b200.cache import Int8Pages
+    from supersonic_b200.csrc import int8_ops, ops
+    pages = Int8Pages.allocate(1, 1, 64, 16, device=DEV)
+    q = torch.zeros((1, 64), dtype=torch.bfloat16, device=DEV)
+    for window in (2 ** 40, -1):
+        with pytest.raises(ops.KernelError):
+            int8_ops.attention(q, pages, _ints([[0]]), _ints([0, 1]), _ints([0]), _ints([0]), 1, torch.zeros_like(q), 1, 0.125, window=window)
