@@ -733,17 +733,18 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
     ssb_pdl_launch_dependents();
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
-    ssb_pdl_wait();
     const int blocks = ir_dealt(total), c = blockIdx.x, half = threadIdx.x / HALF, thread = threadIdx.x % HALF, lane = threadIdx.x & 31;
     const long long begin = ir_begin(total, c, blocks), end = ir_begin(total, c + 1, blocks);
-    if (begin >= end) return;
+    // every block waits for the pieces, those without a share too: whoever waits for this launch has waited for them
+    if (begin >= end) { ssb_pdl_wait(); return; }
     const IrSegment seg = ir_locate(B, half ? end - 1 : begin, end);
     const IrSeq s = seqs[seg.b];
     const int c0 = ir_owner(seg.first, total, blocks), c1 = ir_owner(seg.last, total, blocks), n_pieces = c1 - c0 + 1;
-    if (n_pieces < 2 || c < c0 || c > c1) return;              // the same for the whole half
     const int live = min(C, min(1 << tts, s.n_new - (seg.tile << tts)) * (a.n_q / a.n_kv)) * (HD / 4);
     int e0 = (int)((long long)live * (c - c0) / n_pieces), e1 = (int)((long long)live * (c - c0 + 1) / n_pieces);
     if (half ? seg.first - B.extra <= begin : seg.last >= end - 1) (half ? e0 : e1) = (e0 + e1) / 2;        // both halves have this tile
+    ssb_pdl_wait();
+    if (n_pieces < 2 || c < c0 || c > c1) return;              // the same for the whole half
     auto piece = [&](int i) { return pieces + (size_t)(2 * i + (i == c0)) * ir_piece<HD, NT>(); };
     for (; e0 < e1; e0 += HALF) {
         const int n = min(HALF, e1 - e0), width = n > 32 ? HALF : n > 1 ? 1 << (32 - __clz(n - 1)) : 1, groups = HALF / width;
