@@ -99,27 +99,35 @@ class Int8Session:
     def _write_table(self, slots) -> None:
         for slot in slots:
             pages = self.held[slot]
-            if len(pages) > self.table_host.shape[1]:
-                raise CacheFull(f"a sequence of {self.length[slot]} tokens spans {len(pages)} pages, its table has {self.table_host.shape[1]}")
             self.table_host[slot, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
         self.table.copy_(self.table_host)
+
+    def _reserve(self, slots, counts) -> None:
+        """Pages for these new tokens, and their rows of the page table: for all of the sequences, or (CacheFull) for none."""
+        grown = []
+        for slot, n in zip(slots, counts):
+            spans = pages_for(self.length[slot] + n)
+            if spans > self.table_host.shape[1]:
+                raise CacheFull(f"a sequence of {self.length[slot] + n} tokens spans {spans} pages, its table has {self.table_host.shape[1]}")
+            if spans > len(self.held[slot]):
+                grown.append((slot, spans - len(self.held[slot])))
+        pages = self._take(sum(n for _, n in grown))
+        for slot, n in grown:
+            self.held[slot] += pages[:n]
+            del pages[:n]
+        if grown:
+            self._write_table([slot for slot, _ in grown])
 
     # ---- the step ------------------------------------------------------------------------
     def step(self, entries: Sequence[StepEntry]) -> torch.Tensor:
         """Run the entries' tokens; float32 logits [wanted, vocab], as :meth:`Model.step` gives them."""
+        for e in entries:
+            if e.slot not in self.open_slots:
+                raise ValueError(f"slot {e.slot} is not open")
         packed = pack_entries(entries, [self.position[e.slot] for e in entries], self.model.vocab_size)
         self.model._check_positions(packed.max_total)
         slots, counts = packed.slots, packed.counts
-        grown = []
-        for slot, n in zip(slots, counts):
-            if slot not in self.open_slots:
-                raise ValueError(f"slot {slot} is not open")
-            need = pages_for(self.length[slot] + n) - len(self.held[slot])
-            if need > 0:
-                self.held[slot] += self._take(need)
-                grown.append(slot)
-        if grown:
-            self._write_table(grown)
+        self._reserve(slots, counts)
         starts = [self.length[s] for s in slots]
         places = [np.arange(a, a + n) for a, n in zip(starts, counts)]
         flat = np.concatenate([packed.flat] + places + [starts]).astype(np.int32)      # the step's integers, then the cache's

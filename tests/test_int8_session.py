@@ -1,0 +1,129 @@
+"""What an 8-bit session keeps account of (slots, pages, the page table, cuts), on the CPU: its step is replaced by one that writes
+every token to its place through the page table and whose logits depend on all that the sequence then holds."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from supersonic_b200.cache import CacheFull
+from supersonic_b200.csrc import int8_ops, ops
+from supersonic_b200.engine import StepEntry
+from supersonic_b200.engine.int8_session import Int8Session
+
+VOCAB = 97
+
+
+class Session(Int8Session):
+    """Logits of a row: one for (sum over the tokens held up to it of (place + 1) times token) % VOCAB."""
+
+    def __init__(self, max_tokens, step_token_budget=4096, **kw):
+        model = SimpleNamespace(device=torch.device("cpu"), dtype=torch.float32, blocks=[], spec=SimpleNamespace(schedule=[]),
+                                vocab_size=VOCAB, step_token_budget=step_token_budget, use_graphs=False, _check_positions=lambda n: None)
+        super().__init__(model, max_tokens, **kw)
+        n_pages = len(self.free)
+        self.store = torch.full((n_pages, 64), -1)
+        self.layers = [SimpleNamespace(pages=SimpleNamespace(k=torch.zeros((n_pages, 1, 1, 1))))]      # what is cut: the store
+        self.steps = []
+
+    def _forward(self, packed, ints):
+        rows, flat = [], packed.flat
+        T = packed.n_tokens
+        place = ints[flat.shape[0]:flat.shape[0] + T].tolist()
+        self.steps.append(T)
+        for t in range(T):
+            slot = int(flat[2 * T + t])
+            self.store[self.table[slot, place[t] // 64], place[t] % 64] = int(flat[t])
+            held = self.tokens(slot, place[t] + 1)
+            assert all(x >= 0 for x in held)
+            rows.append(torch.nn.functional.one_hot(torch.tensor(expected(held)), VOCAB).float())
+        want = flat[-packed.n_want:] if packed.n_want else []
+        return torch.stack([rows[int(w)] for w in want]) if packed.n_want else torch.zeros((0, VOCAB))
+
+    def tokens(self, slot, n):
+        """The first ``n`` tokens of a sequence, by the table that a step reads"""
+        return [int(self.store[self.table[slot, j // 64], j % 64]) for j in range(n)]
+
+    def account(self):
+        return [list(h) for h in self.held], sorted(self.free), self.table.clone(), list(self.position), list(self.length), set(self.open_slots)
+
+    def unchanged_since(self, before):
+        now = self.account()
+        return all(torch.equal(a, b) if torch.is_tensor(a) else a == b for a, b in zip(before, now)) and torch.equal(self.table, self.table_host)
+
+
+def expected(tokens):
+    return sum((i + 1) * t for i, t in enumerate(tokens)) % VOCAB
+
+
+@pytest.fixture(autouse=True)
+def on_the_host(monkeypatch):
+    monkeypatch.setattr(ops, "check_device_errors", lambda device=None: None)
+
+
+def prompt(n, seed=0):
+    return [(7 * seed + 3 * i + i * i) % VOCAB for i in range(n)]
+
+
+def run(session, *entries):
+    """Steps the entries (slot, tokens) and checks every logit."""
+    held = {slot: session.tokens(slot, session.length[slot]) for slot, _ in entries}
+    logits = session.step([StepEntry(slot, tokens, list(range(len(tokens)))) for slot, tokens in entries])
+    want = [expected(held[slot] + list(tokens[:i + 1])) for slot, tokens in entries for i in range(len(tokens))]
+    assert logits.argmax(-1).tolist() == want
+
+
+# ---- steps that are refused ---------------------------------------------------------------------------------------
+def test_a_step_refused_for_want_of_pages_changes_nothing():
+    session = Session(64 * 4)
+    a, b, c = session.open(), session.open(), session.open()
+    run(session, (a, prompt(60, 1)))
+    before = session.account()
+    with pytest.raises(CacheFull):
+        session.step([StepEntry(b, prompt(10, 2), [9]), StepEntry(c, prompt(200, 3), [199])])
+    assert session.unchanged_since(before)
+    run(session, (b, prompt(10, 2)))                               # as if nothing had been: a's page is its own
+    run(session, (a, [5]), (b, [6]))
+    assert session.tokens(a, 61) == prompt(60, 1) + [5]
+    for s in (a, b, c):
+        session.close(s)
+    assert sorted(session.free) == list(range(4))
+
+
+def test_a_step_with_a_sequence_that_is_not_open_changes_nothing():
+    session = Session(64 * 4, max_sequences=3)
+    a, b = session.open(), session.open()
+    run(session, (a, prompt(60, 1)))
+    before = session.account()
+    for other in (2, 3, -1):                                       # not open, and no slot at all
+        with pytest.raises(ValueError):
+            session.step([StepEntry(b, prompt(10, 2), [9]), StepEntry(other, [1], [0])])
+        assert session.unchanged_since(before)
+    run(session, (b, prompt(10, 2)), (a, [4]))
+
+
+def test_a_step_of_tokens_outside_the_vocabulary_changes_nothing():
+    session = Session(64 * 4)
+    a = session.open()
+    before = session.account()
+    for bad in ([StepEntry(a, [1, VOCAB], [0])], [StepEntry(a, [], [])], [StepEntry(a, [1], [1])], [StepEntry(a, [1], [0])] * 2, []):
+        with pytest.raises(ValueError):
+            session.step(bad)
+        assert session.unchanged_since(before)
+    run(session, (a, [3]))
+
+
+def test_a_sequence_wider_than_its_table_is_refused_every_time():
+    session = Session(64 * 16)
+    session.table_host = session.table_host[:, :3].contiguous()     # room for 192 tokens a sequence
+    session.table = session.table_host.clone()
+    a, b = session.open(), session.open()
+    run(session, (a, prompt(64, 1)))
+    before = session.account()
+    for _ in range(2):
+        with pytest.raises(CacheFull):
+            session.step([StepEntry(b, prompt(193, 2), [0])])
+        assert session.unchanged_since(before)
+    run(session, (b, prompt(192, 2)))
+    with pytest.raises(CacheFull):
+        session.step([StepEntry(b, [1], [0])])
+    run(session, (a, [1]))
