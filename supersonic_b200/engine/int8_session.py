@@ -218,9 +218,11 @@ class Int8Session:
     # ---- greedy generation ---------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 8, stop_token_ids: Sequence[int] = ()) -> List[List[int]]:
         """Greedy tokens for each prompt, all prompts in one batch."""
-        slots = [self.open() for _ in prompts]
+        slots: List[int] = []
         out: List[List[int]] = [[] for _ in prompts]
         try:
+            for _ in prompts:
+                slots.append(self.open())
             live = list(range(len(prompts)))
             entries = [StepEntry(s, p, [len(p) - 1]) for s, p in zip(slots, prompts)]
             while live and max_new_tokens > 0:

@@ -127,3 +127,21 @@ def test_a_sequence_wider_than_its_table_is_refused_every_time():
     with pytest.raises(CacheFull):
         session.step([StepEntry(b, [1], [0])])
     run(session, (a, [1]))
+
+
+# ---- generation ---------------------------------------------------------------------------------------------------
+def greedy(tokens, n):
+    out = []
+    for _ in range(n):
+        out.append(expected(list(tokens) + out))
+    return out
+
+
+def test_a_refused_generate_gives_its_slots_back():
+    session = Session(64 * 8, max_sequences=2)
+    prompts = [prompt(5, i) for i in range(3)]
+    for refused in (prompts, [[1], []], [prompt(513)]):              # more than there are slots; an empty prompt; no room
+        with pytest.raises((CacheFull, ValueError)):
+            session.generate(refused, 2)
+        assert not session.open_slots and sorted(session.free) == list(range(8))
+    assert session.generate(prompts[:2], 4) == [greedy(p, 4) for p in prompts[:2]]
