@@ -102,32 +102,53 @@ class Int8Session:
             self.table_host[slot, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
         self.table.copy_(self.table_host)
 
-    def _reserve(self, slots, counts) -> None:
-        """Pages for these new tokens, and their rows of the page table: for all of the sequences, or (CacheFull) for none."""
-        grown = []
+    def _reserve(self, slots, counts) -> List[List[int]]:
+        """Pages for these new tokens, and their rows of the page table: for all of the sequences, or (CacheFull) for none.  Returns
+        the groups of sequences that are cut behind the step (:meth:`_cuts`), for which there is room then."""
+        spans, grown, cut = {}, [], []
         for slot, n in zip(slots, counts):
-            spans = pages_for(self.length[slot] + n)
-            if spans > self.table_host.shape[1]:
-                raise CacheFull(f"a sequence of {self.length[slot] + n} tokens spans {spans} pages, its table has {self.table_host.shape[1]}")
-            if spans > len(self.held[slot]):
-                grown.append((slot, spans - len(self.held[slot])))
-        pages = self._take(sum(n for _, n in grown))
+            total = self.length[slot] + n
+            if pages_for(total) > self.table_host.shape[1]:
+                raise CacheFull(f"a sequence of {total} tokens spans {pages_for(total)} pages, its table has {self.table_host.shape[1]}")
+            spans[slot] = max(len(self.held[slot]), pages_for(total))
+            if spans[slot] > len(self.held[slot]):
+                grown.append((slot, spans[slot] - len(self.held[slot])))
+            if self.budget is not None and total >= self.budget + self.slack:
+                cut.append(slot)
+        more = sum(n for _, n in grown)
+        groups = self._cuts(cut, len(self.free) - more, spans) if more <= len(self.free) else []
+        pages = self._take(more)
         for slot, n in grown:
             self.held[slot] += pages[:n]
             del pages[:n]
         if grown:
             self._write_table([slot for slot, _ in grown])
+        return groups
+
+    def _cuts(self, slots: List[int], free: int, spans) -> List[List[int]]:
+        """Sequences of ``spans[slot]`` pages in the groups that they are cut in: a cut sequence moves to pages of its own beside its old
+        ones, so as many go together as ``free`` pages hold, and a group's old pages make room for the next."""
+        per, groups = pages_for(self.budget or 0), []
+        while slots:
+            n = min(len(slots), free // per)
+            if n == 0:
+                raise CacheFull(f"cutting a sequence takes {per} pages of 64 tokens beside its own, {free} are free")
+            groups.append(slots[:n])
+            free += sum(spans[s] for s in slots[:n]) - n * per
+            slots = slots[n:]
+        return groups
 
     # ---- the step ------------------------------------------------------------------------
     def step(self, entries: Sequence[StepEntry]) -> torch.Tensor:
-        """Run the entries' tokens; float32 logits [wanted, vocab], as :meth:`Model.step` gives them."""
+        """Run the entries' tokens; float32 logits [wanted, vocab], as :meth:`Model.step` gives them.  A step that is refused, for want
+        of pages for its tokens or for the cuts behind it too, has changed nothing."""
         for e in entries:
             if e.slot not in self.open_slots:
                 raise ValueError(f"slot {e.slot} is not open")
         packed = pack_entries(entries, [self.position[e.slot] for e in entries], self.model.vocab_size)
         self.model._check_positions(packed.max_total)
         slots, counts = packed.slots, packed.counts
-        self._reserve(slots, counts)
+        cuts = self._reserve(slots, counts)
         starts = [self.length[s] for s in slots]
         places = [np.arange(a, a + n) for a, n in zip(starts, counts)]
         flat = np.concatenate([packed.flat] + places + [starts]).astype(np.int32)      # the step's integers, then the cache's
@@ -138,8 +159,8 @@ class Int8Session:
         for slot, n in zip(slots, counts):
             self.position[slot] += n
             self.length[slot] += n
-        if self.budget is not None:
-            self._evict([s for s in slots if self.length[s] >= self.budget + self.slack])
+        for group in cuts:
+            self._evict(group)
         return logits
 
     def _captured(self, packed, flat) -> torch.Tensor:
@@ -194,14 +215,6 @@ class Int8Session:
     def _evict(self, slots: List[int]) -> None:
         """Cut these sequences down to the budget: every layer moves what it keeps to the same new pages, the old ones are free again."""
         budget, per = self.budget, pages_for(self.budget)
-        while slots and len(self.free) < per * len(slots):    # not room for all at once: some, whose old pages make room for others
-            n = len(self.free) // per
-            if n == 0:
-                self._take(per)                               # raises
-            self._evict(slots[:n])
-            slots = slots[n:]
-        if not slots:
-            return
         B = len(slots)
         new = [self._take(per) for _ in slots]
         as_ints = lambda x: torch.tensor(x, dtype=torch.int32, device=self.device)               # noqa: E731

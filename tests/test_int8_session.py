@@ -145,3 +145,69 @@ def test_a_refused_generate_gives_its_slots_back():
             session.generate(refused, 2)
         assert not session.open_slots and sorted(session.free) == list(range(8))
     assert session.generate(prompts[:2], 4) == [greedy(p, 4) for p in prompts[:2]]
+
+
+# ---- a budget -----------------------------------------------------------------------------------------------------
+@pytest.fixture
+def cuts(monkeypatch):
+    """Cuts that keep the first ``first`` and the latest tokens, moved as the operator moves them; (tokens before, kept) of each."""
+    log = []
+
+    def evict(pages, table, seq_slot, lengths, new_table, keep, first, recent, kept):
+        for b, (slot, n) in enumerate(zip(seq_slot.tolist(), lengths.tolist())):
+            held = session.tokens(slot, n)
+            stay = held if n <= keep else held[:first] + held[n - (keep - first):]
+            for j, t in enumerate(stay):
+                session.store[new_table[b, j // 64], j % 64] = t
+            log.append((n, len(stay)))
+    monkeypatch.setattr(int8_ops, "evict", evict)
+
+    def make(*a, **kw):
+        nonlocal session
+        session = Session(*a, **kw)
+        return session
+    session = None
+    return SimpleNamespace(make=make, log=log)
+
+
+def test_a_sequence_is_cut_whenever_it_outgrows_its_budget(cuts):
+    session = cuts.make(64 * 8, budget=100, slack=20, first=3)
+    a = session.open()
+    run(session, (a, prompt(150, 1)))
+    assert cuts.log == [(150, 100)] and session.length[a] == 100 and session.position[a] == 150
+    assert session.tokens(a, 100) == prompt(150, 1)[:3] + prompt(150, 1)[-97:]
+    for t in range(45):
+        run(session, (a, [t]))
+    assert cuts.log == [(150, 100), (120, 100), (120, 100)] and session.position[a] == 195
+    session.close(a)
+    assert sorted(session.free) == list(range(8))
+
+
+def test_a_step_whose_cut_has_no_room_changes_nothing(cuts):
+    session = cuts.make(192, budget=128, slack=64)                   # three pages, and two more for the cut at 192 tokens
+    a = session.open()
+    run(session, (a, prompt(191, 1)))
+    before = session.account()
+    for _ in range(2):
+        with pytest.raises(CacheFull):
+            session.step([StepEntry(a, [1], [0])])
+        assert session.unchanged_since(before) and not cuts.log
+    assert session.tokens(a, 191) == prompt(191, 1)
+
+
+def test_cuts_make_room_for_one_another(cuts):
+    """Two sequences of three pages, and room for the pages of one cut: the first one's old pages are the second one's new ones."""
+    session = cuts.make(64 * 8, budget=128, slack=1)
+    a, b = session.open(), session.open()
+    run(session, (a, prompt(128, 1)), (b, prompt(128, 2)))
+    run(session, (a, [5]), (b, [6]))
+    assert cuts.log == [(129, 128), (129, 128)]
+    assert session.tokens(a, 128)[-1] == 5 and session.tokens(b, 128)[-1] == 6 and len(session.free) == 4
+    before = session.account()
+    c = session.open()
+    run(session, (c, prompt(128, 3)))
+    with pytest.raises(CacheFull):                                   # two pages for the new tokens, none for a cut
+        session.step([StepEntry(a, [7], [0]), StepEntry(b, [8], [0])])
+    session.close(c)
+    run(session, (a, [7]))
+    assert sorted(session.free + session.held[a] + session.held[b]) == list(range(8)) and before[3][a] + 1 == session.position[a]
