@@ -27,7 +27,7 @@ from ..csrc.kernel_sets import NormedInput
 from ..parts.attention import Attention
 from ..parts.block import PreNormBlock
 from ..parts.feed_forward import SwiGLU
-from .batch import StepEntry, batch_over, pack_entries
+from .batch import StepEntry, batch_over, pack_entries, plan_chunks
 from .model import Model, StepContext
 
 
@@ -67,6 +67,7 @@ class Int8Session:
             self.layers.append(layer)
         if len(model.spec.schedule) != len(self.layers) or any(s.layer != i for i, s in enumerate(model.spec.schedule)):
             raise ValueError("an 8-bit session runs every layer once, in order")
+        self.n_pages = n_pages
         self.free = list(range(n_pages - 1, -1, -1))
         self.held: List[List[int]] = [[] for _ in range(max_sequences)]
         self.position = [0] * max_sequences          # tokens given
@@ -102,28 +103,55 @@ class Int8Session:
             self.table_host[slot, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
         self.table.copy_(self.table_host)
 
-    def _reserve(self, slots, counts) -> List[List[int]]:
-        """Pages for these new tokens, and their rows of the page table: for all of the sequences, or (CacheFull) for none.  Returns
-        the groups of sequences that are cut behind the step (:meth:`_cuts`), for which there is room then."""
-        spans, grown, cut = {}, [], []
+    def _plan(self, slots, counts) -> list:
+        """A step of these new tokens as chunks, each a list of (entry, first, end) and the groups of sequences that are cut behind it
+        (:meth:`_cuts`); CacheFull if there is no room for one of them.
+
+        A chunk has the model's ``step_token_budget`` tokens at most.  A sequence that fits its row of the page table, and the cache
+        beside the pages of its cut, is cut behind its last token.  One that does not is cut behind every chunk in which it outgrows its
+        budget, and chunks are as small as leaves room for that."""
+        width, per, limit = self.table_host.shape[1], pages_for(self.budget or 0), self.model.step_token_budget
+        length, spans, free = {s: self.length[s] for s in slots}, {s: len(self.held[s]) for s in slots}, len(self.free)
+        whole = [True] * len(slots)
+        if self.budget is not None:
+            cut_at = self.budget + self.slack
+            for i, (slot, n) in enumerate(zip(slots, counts)):
+                pages = pages_for(length[slot] + n)
+                whole[i] = pages <= width and (length[slot] + n < cut_at or pages + per <= self.n_pages)
+            if not all(whole):
+                limit = max(1, min(limit, min(width, self.n_pages - per) * PAGE_TOKENS - cut_at + 1))
+        chunks = []
+        for pieces in plan_chunks(counts, limit):
+            cut = []
+            for i, first, end in pieces:
+                slot = slots[i]
+                length[slot] += end - first
+                pages = max(spans[slot], pages_for(length[slot]))
+                if pages > width:
+                    raise CacheFull(f"a sequence of {length[slot]} tokens spans {pages} pages, its table has {width}")
+                free -= pages - spans[slot]
+                spans[slot] = pages
+                if self.budget is not None and length[slot] >= cut_at and (end == counts[i] or not whole[i]):
+                    cut.append(slot)
+            if free < 0:
+                raise CacheFull(f"{-free} more pages of 64 tokens are needed than are free")
+            groups = self._cuts(cut, free, spans)
+            for slot in cut:
+                free += spans[slot] - per
+                spans[slot], length[slot] = per, self.budget
+            chunks.append((pieces, groups))
+        return chunks
+
+    def _reserve(self, slots, counts) -> None:
+        """Pages for these new tokens, and their rows of the page table."""
+        grown = []
         for slot, n in zip(slots, counts):
-            total = self.length[slot] + n
-            if pages_for(total) > self.table_host.shape[1]:
-                raise CacheFull(f"a sequence of {total} tokens spans {pages_for(total)} pages, its table has {self.table_host.shape[1]}")
-            spans[slot] = max(len(self.held[slot]), pages_for(total))
-            if spans[slot] > len(self.held[slot]):
-                grown.append((slot, spans[slot] - len(self.held[slot])))
-            if self.budget is not None and total >= self.budget + self.slack:
-                cut.append(slot)
-        more = sum(n for _, n in grown)
-        groups = self._cuts(cut, len(self.free) - more, spans) if more <= len(self.free) else []
-        pages = self._take(more)
-        for slot, n in grown:
-            self.held[slot] += pages[:n]
-            del pages[:n]
+            more = pages_for(self.length[slot] + n) - len(self.held[slot])
+            if more > 0:
+                self.held[slot] += self._take(more)
+                grown.append(slot)
         if grown:
-            self._write_table([slot for slot, _ in grown])
-        return groups
+            self._write_table(grown)
 
     def _cuts(self, slots: List[int], free: int, spans) -> List[List[int]]:
         """Sequences of ``spans[slot]`` pages in the groups that they are cut in: a cut sequence moves to pages of its own beside its old
@@ -140,15 +168,30 @@ class Int8Session:
 
     # ---- the step ------------------------------------------------------------------------
     def step(self, entries: Sequence[StepEntry]) -> torch.Tensor:
-        """Run the entries' tokens; float32 logits [wanted, vocab], as :meth:`Model.step` gives them.  A step that is refused, for want
-        of pages for its tokens or for the cuts behind it too, has changed nothing."""
+        """Run the entries' tokens; float32 logits [wanted, vocab], as :meth:`Model.step` gives them.  More tokens than the model's
+        ``step_token_budget`` run as several steps.  A step that is refused, for want of pages for its tokens or for the cuts behind it
+        too, has changed nothing."""
         for e in entries:
             if e.slot not in self.open_slots:
                 raise ValueError(f"slot {e.slot} is not open")
         packed = pack_entries(entries, [self.position[e.slot] for e in entries], self.model.vocab_size)
         self.model._check_positions(packed.max_total)
+        chunks = self._plan(packed.slots, packed.counts)
+        if len(chunks) == 1:
+            return self._run(packed, chunks[0][1])
+        rows, order = [], []
+        for pieces, cuts in chunks:
+            part = [StepEntry(entries[i].slot, entries[i].tokens[first:end], [w - first for w in entries[i].want if first <= w < end])
+                    for i, first, end in pieces]
+            rows.append(self._run(pack_entries(part, [self.position[e.slot] for e in part]), cuts))
+            order += [(i, j) for i, first, end in pieces for j, w in enumerate(entries[i].want) if first <= w < end]
+        back = sorted(range(len(order)), key=order.__getitem__)       # an entry's wanted rows come in the order it named them
+        return torch.cat(rows)[torch.tensor(back, dtype=torch.int64, device=self.device)]
+
+    def _run(self, packed, cuts) -> torch.Tensor:
+        """One chunk, and the cuts behind it."""
         slots, counts = packed.slots, packed.counts
-        cuts = self._reserve(slots, counts)
+        self._reserve(slots, counts)
         starts = [self.length[s] for s in slots]
         places = [np.arange(a, a + n) for a, n in zip(starts, counts)]
         flat = np.concatenate([packed.flat] + places + [starts]).astype(np.int32)      # the step's integers, then the cache's

@@ -211,3 +211,50 @@ def test_cuts_make_room_for_one_another(cuts):
     session.close(c)
     run(session, (a, [7]))
     assert sorted(session.free + session.held[a] + session.held[b]) == list(range(8)) and before[3][a] + 1 == session.position[a]
+
+
+def test_prompts_longer_than_the_table_are_cut_on_their_way(cuts):
+    """A budget bounds what a prompt holds, not how long it is: what does not fit the table runs in chunks with a cut behind each."""
+    session = cuts.make(64 * 16, step_token_budget=150, budget=100, slack=30, first=3)
+    a, b = session.open(), session.open()
+    tokens, other = prompt(1000, 1), prompt(40, 2)
+    logits = session.step([StepEntry(b, other, [39]), StepEntry(a, tokens, [999, 0, 500])])
+    assert session.position[a] == 1000 and session.position[b] == 40 and all(n <= 150 for n in session.steps)
+    assert 100 <= session.length[a] < 130 and session.tokens(a, 3) == tokens[:3]
+    assert session.tokens(a, session.length[a])[3:] == tokens[1000 - session.length[a] + 3:]
+    assert logits.shape == (4, VOCAB) and logits.argmax(-1).tolist()[0] == expected(other) and logits.argmax(-1).tolist()[2] == expected(tokens[:1])
+    assert session.generate([prompt(700, 3)], 3) and not session.open_slots - {a, b}
+    session.close(a)
+    session.close(b)
+    assert sorted(session.free) == list(range(16))
+
+
+def test_prompts_longer_than_the_cache_are_cut_on_their_way(cuts):
+    """Chunks are as small as leaves room for a cut, whatever a step may have."""
+    session = cuts.make(64 * 8, step_token_budget=4096, budget=100, slack=30)
+    a = session.open()
+    session.step([StepEntry(a, prompt(2000, 1), [1999])])
+    assert session.position[a] == 2000 and session.length[a] < 130
+    assert max(session.steps) <= 64 * 6 - 129 and len(cuts.log) >= 2000 // 384
+
+
+def test_a_prompt_that_fits_its_table_is_cut_behind_its_last_token(cuts):
+    session = cuts.make(64 * 16, step_token_budget=150, budget=100, slack=30)       # a table of 5 pages
+    a, b = session.open(), session.open()
+    run(session, (a, prompt(320, 1)), (b, prompt(60, 2)))
+    assert session.steps == [150, 150, 80] and cuts.log == [(320, 100)]
+
+
+def test_steps_of_more_tokens_than_the_models_run_in_chunks():
+    session = Session(64 * 16, step_token_budget=100)
+    a, b = session.open(), session.open()
+    run(session, (a, prompt(130, 1)), (b, prompt(250, 2)))
+    assert session.steps == [100, 100, 100, 80]
+    run(session, *[(s, [1]) for s in (a, b)])
+    before = session.account()
+    with pytest.raises(CacheFull):                                   # the last chunk has no room: none of them runs
+        session.step([StepEntry(a, prompt(300, 3), [0]), StepEntry(b, prompt(600, 4), [0])])
+    assert session.unchanged_since(before)
+    session.close(a)
+    session.close(b)
+    assert sorted(session.free) == list(range(16))
