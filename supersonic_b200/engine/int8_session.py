@@ -52,12 +52,18 @@ class Int8Session:
         if budget is not None and (budget <= 0 or slack < 1 or first < 0 or self.recent < 0 or first + self.recent > budget):
             raise ValueError(f"a budget of {budget} tokens has no room for the first {first} and the latest {self.recent}")
         n_pages = pages_for(max_tokens)
+        stops = model.spec.schedule
+        if [s.layer for s in stops] != list(range(len(model.blocks))) or len({s.cache for s in stops}) != len(stops) \
+                or any(s.before is not None or not s.writes_cache for s in stops) or hasattr(getattr(model, "embedding", None), "cache_need"):
+            raise ValueError("an 8-bit session runs every layer once, in order, each with a cache of its own and nothing between them")
         self.layers: List[_Layer] = []
         for b in model.blocks:
             mixer, ff, rotary = b.mixer, getattr(b, "feed_forward", None), getattr(b, "position", None)
             if type(b) is not PreNormBlock or not isinstance(mixer, Attention) or not isinstance(ff, SwiGLU) or ff.act is not None \
                     or getattr(rotary, "rotary_tables", None) is None or rotary.interleaved or rotary.rotary_dim % 16:
                 raise ValueError("an 8-bit session runs layers of rotary attention and a silu-gated feed-forward behind pre-norms")
+            if mixer.window is not None and budget is not None:
+                raise ValueError("a window counts positions, which a sequence's places are no longer once it was cut to a budget")
             layer = _Layer(b, Int8Pages.allocate(n_pages, mixer.n_kv, mixer.head_dim, block, weights=budget is not None, device=self.device))
             for name, w in (("qkv", mixer.w_qkv), ("o", mixer.w_o), ("gate_up", ff.w_gate_up), ("down", ff.w_down)):
                 codes = torch.empty(w.shape, dtype=torch.int8, device=self.device)
@@ -65,8 +71,6 @@ class Int8Session:
                 int8_ops.quantize_rows(w, codes, scale)
                 layer.weights[name] = (codes, scale)
             self.layers.append(layer)
-        if len(model.spec.schedule) != len(self.layers) or any(s.layer != i for i, s in enumerate(model.spec.schedule)):
-            raise ValueError("an 8-bit session runs every layer once, in order")
         self.n_pages = n_pages
         self.free = list(range(n_pages - 1, -1, -1))
         self.held: List[List[int]] = [[] for _ in range(max_sequences)]

@@ -258,3 +258,32 @@ def test_steps_of_more_tokens_than_the_models_run_in_chunks():
     session.close(a)
     session.close(b)
     assert sorted(session.free) == list(range(16))
+
+
+# ---- models that are refused --------------------------------------------------------------------------------------
+def _model(window=None, stops=((0, 0), (1, 1)), embedding=None, **kw):
+    from supersonic_b200.config.base import ScheduleEntry
+    from supersonic_b200.parts.attention import Attention
+    from supersonic_b200.parts.block import PreNormBlock
+    from supersonic_b200.parts.feed_forward import SwiGLU
+
+    def block():
+        mixer, ff = Attention.__new__(Attention), SwiGLU.__new__(SwiGLU)
+        vars(mixer).update(n_q=1, n_kv=1, head_dim=16, window=window, scale=1.0, w_qkv=torch.zeros((48, 16)), w_o=torch.zeros((16, 16)))
+        vars(ff).update(act=None, inter=16, layout="stacked", w_gate_up=torch.zeros((32, 16)), w_down=torch.zeros((16, 16)))
+        return PreNormBlock(mixer, ff, None, None, SimpleNamespace(rotary_tables=lambda: None, interleaved=False, rotary_dim=16))
+    schedule = [ScheduleEntry(*stop, **(kw if i == 1 else {})) for i, stop in enumerate(stops)]
+    return SimpleNamespace(device=torch.device("cpu"), dtype=torch.float32, blocks=[block(), block()], vocab_size=VOCAB, use_graphs=False,
+                           spec=SimpleNamespace(schedule=schedule), step_token_budget=64, embedding=embedding, _check_positions=lambda n: None)
+
+
+def test_models_that_a_session_would_run_wrongly_are_refused(monkeypatch):
+    monkeypatch.setattr(int8_ops, "quantize_rows", lambda *a: None)
+    Int8Session(_model(), 256)
+    Int8Session(_model(window=100), 256)
+    for model in (_model(before=(0, 0)), _model(writes_cache=False), _model(stops=((0, 0), (1, 0))), _model(stops=((1, 0), (0, 1))),
+                  _model(embedding=SimpleNamespace(cache_need=lambda: None))):
+        with pytest.raises(ValueError):
+            Int8Session(model, 256)
+    with pytest.raises(ValueError):                                  # a window counts positions, a cut cache has places
+        Int8Session(_model(window=100), 256, budget=64)
