@@ -27,9 +27,9 @@ int8_attention_plain_kernel(const IaArgs a) {
         const int mid = (lo + hi + 1) >> 1;
         if (a.cu_new[mid] <= row) lo = mid; else hi = mid - 1;
     }
-    const int s = row < a.cu_new[a.n_seqs] && row >= a.cu_new[0] ? a.seq_slot[lo] : -1;
-    const int at = a.seq_start[lo] + row - a.cu_new[lo];
-    const int last = s < 0 || s >= a.n_slots ? -1 : min(at, a.max_pages * IA_PAGE - 1);
+    const IaSeq seq = ia_sequence(a, lo);
+    const int s = row >= seq.row0 && row < seq.row0 + seq.n_new ? seq.slot : -1, at = seq.start + row - seq.row0;
+    const int last = s < 0 ? -1 : (int)min((long long)at, (long long)a.max_pages * IA_PAGE - 1);
     const int from = a.window > 0 ? max(0, at - a.window + 1) : 0;
     float q[2][4], o[2][4] = {};
 #pragma unroll
@@ -40,7 +40,7 @@ int8_attention_plain_kernel(const IaArgs a) {
     float m = -INFINITY, l = 0.f;
     for (int j = from; j <= last; ++j) {
         const int page = a.page_table[(size_t)s * a.max_pages + (j >> 6)];
-        if (page < 0 || page >= a.n_pages) continue;
+        if (!ia_in_pool(a, page)) continue;
         const size_t r = ((size_t)page * a.n_kv + kvh) * IA_PAGE + (j & 63);
         float d = 0.f;
 #pragma unroll
@@ -81,15 +81,15 @@ template <typename T>
 __global__ void __launch_bounds__(128)
 int8_weigh_plain_kernel(const IaArgs a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, words = a.head_dim / 4, group = a.n_q / a.n_kv;
-    const int kvh = blockIdx.y, b = blockIdx.z, s = a.seq_slot[b];
-    const int row0 = a.cu_new[b], n_new = a.cu_new[b + 1] - row0, start = a.seq_start[b];
-    if (s < 0 || s >= a.n_slots || n_new <= 0) return;
+    const int kvh = blockIdx.y;
+    const auto [row0, n_new, start, s] = ia_sequence(a, blockIdx.z);
+    if (s < 0 || n_new <= 0) return;
     const int i0 = max(0, n_new - a.weigh_last);
-    const int end = min(start + n_new, a.max_pages * IA_PAGE);
+    const int end = (int)min((long long)start + n_new, (long long)a.max_pages * IA_PAGE);
     const int begin = a.window > 0 ? max(0, start + i0 - a.window + 1) : 0;
     for (int j = begin + (int)blockIdx.x * 4 + warp; j < end; j += gridDim.x * 4) {
         const int page = a.page_table[(size_t)s * a.max_pages + (j >> 6)];
-        if (page < 0 || page >= a.n_pages) continue;
+        if (!ia_in_pool(a, page)) continue;
         const size_t r = ((size_t)page * a.n_kv + kvh) * IA_PAGE + (j & 63);
         const float ks = a.scale * a.k_scale[r >> a.shift];
         float sum = 0.f;
@@ -142,14 +142,14 @@ constexpr long long IR_KEPT_MOST = 1LL << 26;  // floats
 constexpr float IR_NONE = -1e30f;               // a maximum over no key: finite, so that nothing below needs to ask for it
 constexpr int IR_SIDE = 12;                  // beside a stage's page: its scales of keys and of values, and its id
 constexpr int IR_LEAST_X = -80, IR_MOST_X = 120;
+constexpr float IR_NO_PAGE = -1.f;           // in the place of the scales of a page id that names no page
+__device__ const float ir_no_page = IR_NO_PAGE;
 
-struct IrSeq { int row0, n_new, start, slot; };
-
-// What the dealing needs: tokens a tile (1 << tts), the window, and the batch with the units before each sequence.
+// What the dealing needs: tokens a tile (1 << tts), the window, the table's width, and the batch with the units before each sequence.
 struct IrBatch {
-    const IrSeq* seqs;
+    const IaSeq* seqs;
     const long long* cum;                // [n_seqs + 1]
-    int n_seqs, n_kv, tts, window;
+    int n_seqs, n_kv, tts, window, pages;
     bool one_tile;                       // a sequence's rows are one tile, however many
     int extra;                           // what beginning and ending a tile costs, in pages: units without a page before its first
 
@@ -166,16 +166,21 @@ struct IrBatch {
         const long long r0 = (a & 63) >> tts;
         return (a >> 6) * t + ramp(r0 + t) - ramp(r0);
     }
-    __device__ int tiles(const IrSeq& s) const { return s.slot < 0 || s.n_new <= 0 ? 0 : one_tile ? 1 : (s.n_new + (1 << tts) - 1) >> tts; }
+    __device__ int tiles(const IaSeq& s) const { return s.slot < 0 || s.n_new <= 0 ? 0 : one_tile ? 1 : (s.n_new + (1 << tts) - 1) >> tts; }
     // units of the first t tiles of a sequence: the pages that each sees, and the extra ones
-    __device__ long long units_before(const IrSeq& s, long long t) const {
-        if (one_tile) return t * (((s.start + s.n_new - 1) >> 6) - first_page(s, 0) + 1 + extra);
-        return t * (1 + extra) + floors(t, (long long)s.start + (1 << tts) - 1) - (window > 0 ? floors(t, (long long)s.start - window + 1) : 0);
+    __device__ long long units_before(const IaSeq& s, long long t) const {
+        if (one_tile) return t * (min((s.start + s.n_new - 1) >> 6, pages - 1) - first_page(s, 0) + 1 + extra);
+        const long long hi = (long long)s.start + (1 << tts) - 1;
+        return t * (1 + extra) + (window > 0 ? floors(t, min(hi, last_place())) - floors(t, first_place(s)) : floors(t, hi));
     }
-    __device__ int first_page(const IrSeq& s, int tile) const {
-        const long long lo = (long long)s.start + ((long long)tile << tts) - window + 1;
+    __device__ int first_page(const IaSeq& s, int tile) const {
+        const long long lo = first_place(s) + ((long long)tile << tts);
         return window > 0 && lo > 0 ? (int)(lo >> 6) : 0;
     }
+    // Of a window's first row, no farther than the table's last place: so the first tile has one page at least and the table's at most
+    // wherever it starts (without a window a start is the last place at most).  What the others have of pages behind that is unseen.
+    __device__ long long last_place() const { return (long long)pages * IA_PAGE - 1; }
+    __device__ long long first_place(const IaSeq& s) const { return min((long long)s.start - window + 1, last_place()); }
 };
 
 // A run of pages of one tile and kv head: what of it lies in a block's range.
@@ -191,7 +196,7 @@ __device__ __forceinline__ IrSegment ir_locate(const IrBatch& B, long long u, lo
         const int mid = (lo + hi + 1) >> 1;
         if (B.cum[mid] <= u) lo = mid; else hi = mid - 1;
     }
-    const IrSeq s = B.seqs[lo];
+    const IaSeq s = B.seqs[lo];
     IrSegment g;
     g.b = lo;
     const int tiles = B.tiles(s);
@@ -223,13 +228,12 @@ __device__ __forceinline__ IrSegment ir_locate(const IrBatch& B, long long u, lo
 }
 
 // Reads the batch and sums its units up; every thread of the block gets the total.
-__device__ __forceinline__ long long ir_read_batch(const IaArgs& a, int s0, int n_seqs, IrBatch& B, IrSeq* seqs, long long* cum,
+__device__ __forceinline__ long long ir_read_batch(const IaArgs& a, int s0, int n_seqs, IrBatch& B, IaSeq* seqs, long long* cum,
                                                    long long* warp_total, int last = 0) {
     for (int b = threadIdx.x; b < n_seqs; b += IR_THREADS) {
-        const int row0 = a.cu_new[s0 + b], slot = a.seq_slot[s0 + b];
-        const int n_new = a.cu_new[s0 + b + 1] - row0, start = a.seq_start[s0 + b];
-        const int skip = last > 0 && n_new > last ? n_new - last : 0;        // with ``last``, that many last rows only
-        seqs[b] = IrSeq{row0 + skip, n_new - skip, start + skip, slot < a.n_slots && start >= 0 ? slot : -1};
+        const IaSeq s = ia_sequence(a, s0 + b);
+        const int skip = last > 0 && s.n_new > last ? s.n_new - last : 0;    // with ``last``, that many last rows only
+        seqs[b] = IaSeq{s.row0 + skip, s.n_new - skip, s.start + skip, s.slot};
     }
     __syncthreads();
     const int per = (n_seqs + IR_THREADS - 1) / IR_THREADS, b0 = (int)threadIdx.x * per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -416,15 +420,17 @@ __device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFee
         f.left = f.seg.n;
         f.ids_from = -1;
     }
-    const IrSeq s = B.seqs[f.seg.b];
+    const IaSeq s = B.seqs[f.seg.b];
     const int i = f.seg.n - f.left;
     if (f.ids_from < 0 || i - f.ids_from >= 32) {
-        // a tile that is not full may count a page behind the sequence's last: the last again, which no row of it sees
-        const int page = min(min(f.seg.page + i + lane, (s.start + s.n_new - 1) >> 6), a.max_pages - 1);
-        f.ids = min(max(a.page_table[(size_t)s.slot * a.max_pages + page], 0), a.n_pages - 1);
+        // a tile that is not full may count a page behind the sequence's last: the last again, which no row of it sees; what lies behind
+        // the table is no page
+        const int page = f.seg.page + i + lane;
+        const int named = a.page_table[(size_t)s.slot * a.max_pages + min(min(page, (s.start + s.n_new - 1) >> 6), B.pages - 1)];
+        f.ids = page < B.pages && ia_in_pool(a, named) ? named : -1;
         f.ids_from = i;
     }
-    const int id = __shfl_sync(0xffffffffu, f.ids, i - f.ids_from);
+    const int named = __shfl_sync(0xffffffffu, f.ids, i - f.ids_from), id = max(named, 0);      // of no page: any, unseen
     const int st = f.stage;
     bool ok = true;
     if (lane == 0) ok = ir_wait(empty0 + 8 * st, f.lap ^ 1, abort_flag);
@@ -432,12 +438,12 @@ __device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFee
     if (!ok) return false;
     const size_t head = (size_t)id * a.n_kv + f.seg.kvh;
     if (lane < 2 * per) {
-        const float* src = (lane < per ? a.k_scale : a.v_scale) + head * per + (lane & (per - 1));
+        const float* src = named >= 0 ? (lane < per ? a.k_scale : a.v_scale) + head * per + (lane & (per - 1)) : &ir_no_page;
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(scales + IR_SIDE * st + lane)), "l"(src) : "memory");
     }
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full0 + 8 * st) : "memory");
     if (lane == 0) {
-        scales[IR_SIDE * st + 8] = __int_as_float(id);            // before this lane's arrival at the barrier, below
+        if (!VALUES) scales[IR_SIDE * st + 8] = __int_as_float(named);       // before this lane's arrival at the barrier, below
         const uint32_t dst = smem_u32(stages + st * ir_stage_bytes<HD, VALUES>());
         mbar_expect_tx(full0 + 8 * st, ir_stage_bytes<HD, VALUES>());
         tma_load_2d(dst, &map_k, full0 + 8 * st, 0, (int)(head * 64));
@@ -454,7 +460,7 @@ template <int HD, int NT> constexpr int ir_work_words() {
     return 8 * NT * ir_acc_ld<HD>() > NT * ir_q_words<HD>() ? 8 * NT * ir_acc_ld<HD>() : NT * ir_q_words<HD>();
 }
 template <int HD, int NT> constexpr size_t ir_smem(int n_seqs) {
-    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, true>() + (size_t)ir_work_words<HD, NT>() * 4 + IR_STAGES * IR_SIDE * 4 + 2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IrSeq) + 8) + 8;
+    return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, true>() + (size_t)ir_work_words<HD, NT>() * 4 + IR_STAGES * IR_SIDE * 4 + 2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IaSeq) + 8) + 8;
 }
 // floats of a piece: a column's sums, its maximum and its sum of weights
 template <int HD, int NT> constexpr int ir_piece() { return 8 * NT * (HD + 2); }
@@ -467,7 +473,7 @@ template <> __device__ __forceinline__ void ir_store4<bf16>(bf16* p, float4 v) {
 }
 // What a column's result is written as.
 template <int HD, bool WIDE>
-__device__ __forceinline__ void ir_put(const IaArgs& a, const IrSeq& s, int tile, int tts, int kvh, int col, int d, float4 o, float m, float l, float offset) {
+__device__ __forceinline__ void ir_put(const IaArgs& a, const IaSeq& s, int tile, int tts, int kvh, int col, int d, float4 o, float m, float l, float offset) {
     using T = typename std::conditional<WIDE, float, bf16>::type;
     const int group = a.n_q / a.n_kv, token = (tile << tts) + col / group, head = kvh * group + col % group;
     if (col / group >= (1 << tts) || token >= s.n_new) return;
@@ -499,7 +505,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
     float* scales = acc + ir_work_words<HD, NT>();                                // [stage][keys' | values' | page id]
     uint64_t* bars = (uint64_t*)(scales + IR_STAGES * IR_SIDE);                         // full, empty
     long long* cum = (long long*)(bars + 2 * IR_STAGES);
-    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    IaSeq* seqs = (IaSeq*)(cum + n_seqs + 1);
     __shared__ float warp_m[IR_WARPS][C], warp_l[IR_WARPS][C], qf[C];
     __shared__ long long warp_total[IR_WARPS];
     __shared__ int sm_abort[2];
@@ -514,7 +520,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, a.max_pages, false, IR_EXTRA};
     // dependents may start once all that came before this launch is done: they read the batch and the pages ahead of their own wait
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
@@ -544,7 +550,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
     for (long long u = begin; u < end;) {
         const IrSegment seg = ir_locate(B, u, end);
         if (seg.n == 0) { u = seg.next; continue; }
-        const IrSeq s = seqs[seg.b];
+        const IaSeq s = seqs[seg.b];
         const int token0 = seg.tile << tts, n_tokens = min(1 << tts, s.n_new - token0);
         ir_queries<HD, NT, WIDE>(a, s.row0 + token0, n_tokens, seg.kvh, 0, qs, qf);
         __syncthreads();
@@ -581,9 +587,9 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
             const float ks = scales[IR_SIDE * st + block_at], vs = scales[IR_SIDE * st + (64 >> a.shift) + block_at];
             float sc[NT][4];
             ir_scores<HD, NT>(keys, qs, warp, lane, sc);
-            // vs = f 2^x; what is no scale belongs to keys that nobody sees
+            // vs = f 2^x; what is no scale belongs to keys that nobody sees, and x = -inf leaves nothing of a page that is none
             const int x = min(max((int)(__float_as_uint(vs) >> 23 & 255) - 127, IR_LEAST_X), IR_MOST_X);
-            const float fx = (float)x, down = __uint_as_float((uint32_t)(127 - x) << 23), f = fabsf(vs) < 3e38f ? vs * down : 0.f;
+            const float fx = vs == IR_NO_PAGE ? -INFINITY : (float)x, down = __uint_as_float((uint32_t)(127 - x) << 23), f = fabsf(vs) < 3e38f ? vs * down : 0.f;
             const bool inside = key0 >= all_lo && key0 + 15 <= all_hi;
             float worst = -INFINITY;
 #pragma unroll
@@ -727,10 +733,10 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     constexpr int C = 8 * NT, HALF = IR_THREADS / 2;
     extern __shared__ unsigned char smem_raw[];
     long long* cum = (long long*)smem_raw;
-    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    IaSeq* seqs = (IaSeq*)(cum + n_seqs + 1);
     __shared__ long long warp_total[IR_WARPS];
     __shared__ float others[2][6][32];
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, a.max_pages, false, IR_EXTRA};
     ssb_pdl_launch_dependents();
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     const int blocks = ir_dealt(total), c = blockIdx.x, half = threadIdx.x / HALF, thread = threadIdx.x % HALF, lane = threadIdx.x & 31;
@@ -738,7 +744,7 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     // every block waits for the pieces, those without a share too: whoever waits for this launch has waited for them
     if (begin >= end) { ssb_pdl_wait(); return; }
     const IrSegment seg = ir_locate(B, half ? end - 1 : begin, end);
-    const IrSeq s = seqs[seg.b];
+    const IaSeq s = seqs[seg.b];
     const int c0 = ir_owner(seg.first, total, blocks), c1 = ir_owner(seg.last, total, blocks), n_pieces = c1 - c0 + 1;
     const int live = min(C, min(1 << tts, s.n_new - (seg.tile << tts)) * (a.n_q / a.n_kv)) * (HD / 4);
     int e0 = (int)((long long)live * (c - c0) / n_pieces), e1 = (int)((long long)live * (c - c0 + 1) / n_pieces);
@@ -797,9 +803,9 @@ __global__ void __launch_bounds__(IR_THREADS)
 int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict__ kept) {
     extern __shared__ unsigned char smem_raw[];
     long long* cum = (long long*)smem_raw;
-    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    IaSeq* seqs = (IaSeq*)(cum + n_seqs + 1);
     __shared__ long long warp_total[IR_WARPS];
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, false, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, a.max_pages, false, IR_EXTRA};
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     const int blocks = ir_dealt(total), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.n_q / a.n_kv;
     const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
@@ -808,7 +814,7 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
     for (long long u = begin; u < end;) {
         const IrSegment seg = ir_locate(B, u, end);
         u = seg.next;
-        const IrSeq s = seqs[seg.b];
+        const IaSeq s = seqs[seg.b];
         if (seg.n == 0) continue;
         // lanes 0 - 15 take heads 0, 2, .., the others 1, 3, ..: of up to 8
         float ref[4];
@@ -821,7 +827,8 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
 #pragma unroll 2
         for (int p = warp; p < seg.n; p += IR_WARPS) {
             const float* src = kept + (seg.at + p) * (IR_WARPS * 16) * group;
-            const int page = min(seg.page + p, a.max_pages - 1), id = min(max(a.page_table[(size_t)s.slot * a.max_pages + page], 0), a.n_pages - 1);
+            const int id = a.page_table[(size_t)s.slot * a.max_pages + min(seg.page + p, a.max_pages - 1)];
+            const bool there = ia_in_pool(a, id);
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -837,8 +844,8 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
             // one order, and nobody waits for it
             float* w = a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + 16 * part + t + (lane & 16 ? 8 : 0);
             const float x = lane & 16 ? sum.z : sum.x, y = lane & 16 ? sum.w : sum.y;
-            if (x > 0.f) atomicAdd(w, x);
-            if (y > 0.f) atomicAdd(w + 4, y);
+            if (there && x > 0.f) atomicAdd(w, x);
+            if (there && y > 0.f) atomicAdd(w + 4, y);
         }
     }
 }
@@ -848,7 +855,7 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
 // key's weight.
 template <int HD, int NT, int QB> constexpr size_t ir_weigh_smem(int n_seqs) {
     return 1024 + (size_t)IR_STAGES * ir_stage_bytes<HD, false>() + (size_t)QB * NT * ir_q_words<HD>() * 4 + IR_STAGES * IR_SIDE * 4 +
-           2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IrSeq) + 8) + 8;
+           2 * IR_STAGES * 8 + (size_t)n_seqs * (sizeof(IaSeq) + 8) + 8;
 }
 template <int HD, int NT, int QB, bool WIDE>
 __global__ void __launch_bounds__(IR_THREADS)
@@ -860,7 +867,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
     float* scales = (float*)(qs + QB * Q_WORDS);
     uint64_t* bars = (uint64_t*)(scales + IR_STAGES * IR_SIDE);
     long long* cum = (long long*)(bars + 2 * IR_STAGES);
-    IrSeq* seqs = (IrSeq*)(cum + n_seqs + 1);
+    IaSeq* seqs = (IaSeq*)(cum + n_seqs + 1);
     __shared__ float qf[QB * C], lse2[QB * C];
     __shared__ int last_of[QB * C];                                // the last key a column sees
     __shared__ long long warp_total[IR_WARPS];
@@ -876,7 +883,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, true, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, a.max_pages, true, IR_EXTRA};
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total, a.weigh_last);
     const int blocks = ir_dealt(total);
     const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
@@ -892,7 +899,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
     for (long long u = begin; u < end;) {
         const IrSegment seg = ir_locate(B, u, end);
         if (seg.n == 0) { u = seg.next; continue; }
-        const IrSeq s = seqs[seg.b];
+        const IaSeq s = seqs[seg.b];
         __syncthreads();                                           // the segment before is done with its queries
         const int batches = min(QB, (s.n_new * group - column0 + C - 1) / C);      // may be none
         for (int q = 0; q < batches; ++q)
@@ -944,7 +951,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
             x += __shfl_xor_sync(0xffffffffu, up1 ? x0 : x1, 8);
             x += __shfl_xor_sync(0xffffffffu, x, 4);
             const int key = key0 + t + 4 * (2 * up2 + up1);
-            if (!(lane & 4) && key < s.start + s.n_new && x > 0.f)
+            if (!(lane & 4) && id >= 0 && key < s.start + s.n_new && x > 0.f)
                 atomicAdd(a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + (key & 63), x);
         }
         u = seg.next;
@@ -1035,8 +1042,9 @@ SSB_API long long ssb_int8_attention_scratch(int dtype, int n_seqs, int rows, in
 }
 
 template <int HD, int NT, bool WIDE>
-static int ir_rows(const IaArgs& a, const IrPlan& p, float* pieces, int* error_word, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+static int ir_rows(IaArgs a, const IrPlan& p, float* pieces, int* error_word, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
     float* kept = p.kept ? pieces + 2LL * p.blocks * (long long)p.piece : nullptr;
+    if (kept) a.most_new = 1;                                      // which is what there is room for
     for (int s0 = 0; s0 < a.n_seqs; s0 += IR_SEQS) {
         const int n = std::min(IR_SEQS, a.n_seqs - s0);
         // not as a dependent of what came before: blocks that wait beside another launch's are dealt to SMs unevenly (64 sequences of
@@ -1044,11 +1052,11 @@ static int ir_rows(const IaArgs& a, const IrPlan& p, float* pieces, int* error_w
         int rc = ssb_launch(int8_rows_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), ir_smem<HD, NT>(n), stream, false, a, s0, n, p.tts,
                             pieces, kept, error_word, mk, mv);
         if (rc) return rc;
-        rc = ssb_launch(int8_finish_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IrSeq) + 8) + 8, stream, true,
+        rc = ssb_launch(int8_finish_kernel<HD, NT, WIDE>, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IaSeq) + 8) + 8, stream, true,
                         a, s0, n, p.tts, (const float*)pieces);
         if (rc) return rc;
         if (kept)
-            rc = ssb_launch(int8_account_kernel, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IrSeq) + 8) + 8, stream, true, a, s0, n,
+            rc = ssb_launch(int8_account_kernel, dim3(p.blocks), dim3(IR_THREADS), (size_t)n * (sizeof(IaSeq) + 8) + 8, stream, true, a, s0, n,
                             (const float*)kept);
         if (rc) return rc;
     }
@@ -1097,8 +1105,9 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
         return SSB_ERR_BAD_SIZE;
     if (weigh_last > 0 && (!weight || !lse)) return SSB_ERR_BAD_SIZE;
     if (dtype != SSB_BF16 && dtype != SSB_F32) return SSB_ERR_BAD_DTYPE;
-    const IaArgs a{q, out, lse, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, weight, page_table, cu_new, seq_start, seq_slot,
+    IaArgs a{q, out, lse, (const int8_t*)k, (const int8_t*)v, k_scale, v_scale, weight, page_table, cu_new, seq_start, seq_slot,
                    ldq, ldo, rows, n_seqs, n_slots, max_pages, n_pages, n_q, n_kv, head_dim, block == 16 ? 4 : block == 32 ? 5 : 6, window, weigh_last, scale};
+    a.most_start = (int)std::min((long long)max_pages * IA_PAGE - 1 + std::max(window, 0), 0x7fffff00LL - rows);
     if (!ir_takes(n_q, n_kv, head_dim)) {
         if (weigh_last > 0 && n_seqs > 65535) return SSB_ERR_BAD_SIZE;
         const dim3 grid(rows, (n_q + 3) / 4), wgrid(std::min((max_pages * IA_PAGE + 3) / 4, 512), n_kv, n_seqs);

@@ -31,13 +31,12 @@ constexpr int IT_SEQS = 512;               // sequences a launch: their table li
 constexpr int IT_SCALES = 4;               // turns whose scales are kept
 constexpr float IT_LAZY = 12.f;            // how far, in the log2 domain, a maximum may rise above its row's reference
 constexpr float IT_LEAST = 7.888609052210118e-31f;
-struct ItSeq { int row0, n_new, start, slot; };
 struct ItTile { int row, head, p0, rows, turns; };
-struct ItUnit { int turns, kb_lo, kvh, slot, last, part; ItTile tile[2]; };       // no turns: the block is done; last: the sequence's last key; part: of the keys, or -1: all
+struct ItUnit { int turns, kb_lo, kvh, slot, last, part; ItTile tile[2]; };       // no turns: the block is done; last: the sequence's last key in the table; part: of the keys, or -1: all
 __host__ __device__ constexpr int it_threads(int tiles) { return 256 + 128 * tiles; }
 constexpr int IT_BARS = 6 + 8 + 6 + IT_SCALES;
 __host__ __device__ constexpr size_t it_smem(int tiles, int hd) {
-    return (size_t)tiles * IT_BM * hd * 2 + 2 * 2 * IT_BN * hd * 2 + IT_SEQS * (sizeof(ItSeq) + 4) + IT_SCALES * 8 * 16 + 2 * sizeof(ItUnit) +
+    return (size_t)tiles * IT_BM * hd * 2 + 2 * 2 * IT_BN * hd * 2 + IT_SEQS * (sizeof(IaSeq) + 4) + IT_SCALES * 8 * 16 + 2 * sizeof(ItUnit) +
            IT_BARS * 8 + 32 + 1024;
 }
 // Registers a thread of the three kinds of warps: 4 that control, 4 that convert, 4 a tile that take the softmax.
@@ -48,10 +47,10 @@ __host__ __device__ constexpr int it_regs_softmax(int tiles, int hd) { return it
 
 // The turns of a unit: items (row tile, head of the group) TILES * level and, with two tiles, the one behind it.  Keys begin at the
 // page that the first tile of the pair sees first, for a tile that is alone too: a row's turns, and with them its sums, are the same in
-// a unit of either size.
+// a unit of either size.  All of it in the ``pages`` of the table, of which a tile has one at least.
 template <int TILES> struct ItSpan {
     int kb_lo, most, nb[TILES];          // first page; turns of the longer tile; of each
-    __device__ ItSpan(int start, int n_new, int group, int window, int level) : kb_lo(0), most(0) {
+    __device__ ItSpan(int start, int n_new, int group, int window, int pages, int level) : kb_lo(0), most(0) {
         const int n_items = ((n_new + IT_BM - 1) / IT_BM) * group;
 #pragma unroll
         for (int x = 0; x < TILES; ++x) {
@@ -59,9 +58,9 @@ template <int TILES> struct ItSpan {
             const int p0 = start + tile * IT_BM, rows = item < n_items ? min(IT_BM, n_new - tile * IT_BM) : 0;
             if (x == 0) {
                 const int first = start + (item & ~1) / group * IT_BM;
-                kb_lo = (window > 0 && first - window + 1 > 0) ? (first - window + 1) >> 6 : 0;
+                kb_lo = (window > 0 && first - window + 1 > 0) ? min((first - window + 1) >> 6, pages - 1) : 0;
             }
-            nb[x] = rows > 0 ? (((p0 + rows - 1) >> 6) - kb_lo + 2) >> 1 : 0;
+            nb[x] = rows > 0 ? (min((p0 + rows - 1) >> 6, pages - 1) - kb_lo + 2) >> 1 : 0;
             most = max(most, nb[x]);
         }
     }
@@ -166,7 +165,7 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
     unsigned char* q_s = smem;
     unsigned char* kv_s = smem + TILES * Q_BYTES;                 // two stages of [keys of two pages | values of two pages]
     float4* scales = (float4*)(kv_s + 4 * KV_BYTES);              // [turn & 3][group of 16 keys]: ks scale log2 e, log2 vs, 1 / vs
-    ItSeq* seqs = (ItSeq*)(scales + IT_SCALES * 8);
+    IaSeq* seqs = (IaSeq*)(scales + IT_SCALES * 8);
     int* units_of = (int*)(seqs + IT_SEQS);                       // units of a sequence for one kv head
     ItUnit* units = (ItUnit*)(units_of + IT_SEQS);                // the one that is computed and the next
     uint64_t* bars = (uint64_t*)(units + 2);
@@ -181,12 +180,10 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();                                 // dependents read the batch and the pages ahead of their own wait
     for (int b = threadIdx.x; b < n_seqs; b += it_threads(TILES)) {
-        const int row0 = a.cu_new[s0 + b], n_new = a.cu_new[s0 + b + 1] - row0, start = a.seq_start[s0 + b];
-        int slot = a.seq_slot[s0 + b];
-        if (slot >= a.n_slots || start < 0) slot = -1;
-        seqs[b] = ItSeq{row0, n_new, start, slot};
+        const IaSeq q = ia_sequence(a, s0 + b);
+        seqs[b] = q;
         // (row tile, head of the group) items, heads fastest, TILES a unit
-        units_of[b] = slot < 0 || n_new <= 0 ? 0 : min(levels, (((n_new + IT_BM - 1) / IT_BM) * group + TILES - 1) / TILES);
+        units_of[b] = q.slot < 0 || q.n_new <= 0 ? 0 : min(levels, (((q.n_new + IT_BM - 1) / IT_BM) * group + TILES - 1) / TILES);
     }
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -266,8 +263,8 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                         }
                         member -= n;
                     }
-                    const ItSeq q = seqs[b];
-                    const ItSpan<TILES> span(q.start, q.n_new, group, window, level);
+                    const IaSeq q = seqs[b];
+                    const ItSpan<TILES> span(q.start, q.n_new, group, window, a.max_pages, level);
                     const ItCut cut(span.most, parts);
                     const int skip = part * cut.each;
                     if (skip >= span.most) continue;             // fewer parts than others have
@@ -283,7 +280,7 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                         if (lane == 0) unit.tile[x] = ItTile{t_row[x], t_head[x], q.start + tile * IT_BM, min(IT_BM, q.n_new - tile * IT_BM), nb[x]};
                     }
                     if (lane == 0) unit.part = cut.parts > 1 ? part : -1;
-                    if (lane == 0) { unit.slot = q.slot; unit.last = q.start + q.n_new - 1; }
+                    if (lane == 0) { unit.slot = q.slot; unit.last = (int)min((long long)q.start + q.n_new, (long long)a.max_pages * IA_PAGE) - 1; }
                 }
                 if (lane == 0) {
                     unit.turns = nb_max;
@@ -388,25 +385,26 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
             __syncwarp();
             if (nb == 0) break;
             if (lane == 0) it_arrive(u_empty0 + 8 * (n & 1));
-            // a page past the sequence's last one (odd page counts) is the last one again: its keys lie beyond every query
-            auto page_at = [&](int j, int pg) {
-                return min(max(pt[min(min(kb_lo + 2 * j + pg, last >> 6), a.max_pages - 1)], 0), a.n_pages - 1);
-            };
+            // a page past the sequence's last one (odd page counts) is the last one again: its groups have no scale
+            auto page_at = [&](int j, int pg) { return pt[min(kb_lo + 2 * j + pg, last >> 6)]; };
             uint4 kr[PIECES], vr[PIECES];
             float ks = 0.f, vs = 0.f;
+            bool there = false;
             int ids[2] = {page_at(0, 0), page_at(0, 1)}, ahead[2];
             auto fetch = [&](uint4 (&r)[PIECES], const int8_t* codes, const int (&p)[2]) {
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {               // the first half of the pieces is the first page's
                     const int pg = i / (PIECES / 2), row = (i % (PIECES / 2)) * ROWS + row_of;
-                    r[i] = it_load_once(codes + (((size_t)p[pg] * a.n_kv + kvh) * 64 + row) * HD + 16 * c);
+                    r[i] = it_load_once(codes + (((size_t)(ia_in_pool(a, p[pg]) ? p[pg] : 0) * a.n_kv + kvh) * 64 + row) * HD + 16 * c);
                 }
             };
             auto fetch_scales = [&](const int (&p)[2]) {
                 if (id < 8) {
-                    const size_t at = ((size_t)p[id >> 2] * a.n_kv + kvh) * per + (((id & 3) * 16) >> a.shift);
-                    ks = a.k_scale[at];
-                    vs = a.v_scale[at];
+                    const int page = p[id >> 2];
+                    const size_t at = ((size_t)page * a.n_kv + kvh) * per + (((id & 3) * 16) >> a.shift);
+                    there = ia_in_pool(a, page);
+                    ks = there ? a.k_scale[at] : 0.f;
+                    vs = there ? a.v_scale[at] : 0.f;
                 }
             };
             fetch(kr, a.k, ids);
@@ -436,10 +434,11 @@ int8_attention_tc_kernel(const IaArgs a, const __grid_constant__ CUtensorMap map
                     put(k_dst, kr[i], (c >> 2) * (KV_BYTES / HALVES) + row * 128, row, std::true_type{});
                 }
                 if (id < 8) {
-                    // groups that begin behind the sequence's last key have no scale: theirs count nowhere
-                    const bool has = (kb_lo + 2 * j) * 64 + 16 * id <= last;
+                    // groups that begin behind the sequence's last key, or whose page is none, have no scale: what is added to their
+                    // scores leaves nothing of them
+                    const bool has = there && (kb_lo + 2 * j) * 64 + 16 * id <= last;
                     const float v1 = has ? fmaxf(vs, IT_LEAST) : 1.f, k1 = has ? fmaxf(ks * (a.scale * 1.4426950408889634f), 1e-37f) : 1.f;
-                    scales[(turn & (IT_SCALES - 1)) * 8 + id] = make_float4(k1, log2f(v1), 1.f / v1, 0.f);
+                    scales[(turn & (IT_SCALES - 1)) * 8 + id] = make_float4(k1, has ? log2f(v1) : -INFINITY, 1.f / v1, 0.f);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -651,10 +650,10 @@ int8_join_kernel(const IaArgs a, int s0, int n_seqs, int parts, const float* __r
         const int mid = (lo + hi + 1) >> 1;
         if (a.cu_new[mid] <= row) lo = mid; else hi = mid - 1;
     }
-    const int row0 = a.cu_new[lo], n_new = a.cu_new[lo + 1] - row0, start = a.seq_start[lo], slot = a.seq_slot[lo];
-    if (slot < 0 || slot >= a.n_slots || start < 0 || row < row0 || row >= row0 + n_new) return;
+    const auto [row0, n_new, start, slot] = ia_sequence(a, lo);
+    if (slot < 0 || row < row0 || row >= row0 + n_new) return;
     const int item = (row - row0) / IT_BM * group + head % group;
-    const ItSpan<TILES> span(start, n_new, group, a.window, item / TILES);
+    const ItSpan<TILES> span(start, n_new, group, a.window, a.max_pages, item / TILES);
     const ItCut cut(span.most, parts);
     if (cut.parts <= 1) return;
     const int turns = TILES == 2 && (item & 1) ? span.nb[TILES - 1] : span.nb[0];

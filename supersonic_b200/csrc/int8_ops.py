@@ -223,7 +223,8 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
     ``seq_start[b]`` tokens before them, and its row i sees the keys at places start + i - ``window`` + 1 (None or 0: 0) to start + i.
     ``lse`` (float32 [rows, n_q]) gets the logarithm of a row's sum of exponentials.  ``weigh_last``: that many last rows of every
     sequence add their probabilities, summed over the query heads of a kv head, to ``pages.weight``.  Rows of a sequence with a
-    negative slot are zeros, and their ``lse`` minus infinity."""
+    negative slot are zeros, and their ``lse`` minus infinity.  A place behind the table's end, or under a page id that names no page,
+    holds a key that no row sees."""
     n_pages, n_kv, dim, block, at, table, slots, width = _pages(pages, page_table)
     rows, B = q.shape[0], seq_slot.shape[0]
     if n_q <= 0 or n_q % n_kv:

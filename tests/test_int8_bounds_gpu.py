@@ -1,0 +1,163 @@
+"""Attention over the 8-bit cache at the borders of what it is given: places behind the page table's end, page ids that name no page,
+starts near 2^31.  One definition holds for every kernel: a key is seen if its place is within the row's reach and the table and its
+page id is one of the pool's; a row that sees none is zeros, with minus infinity for its sum."""
+import numpy as np
+import pytest
+import torch
+
+import plain_int8 as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+MOST = 2 ** 31 - 1
+GUARD = 4096
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _cache(rng, table, n_pages, n_kv, dim, block):
+    """Random codes and scales in the pages that the table names; every other page's scales and weights are NaN."""
+    cache = plain.Cache(n_pages, n_kv, dim, block)
+    named = np.unique(table[(table >= 0) & (table < n_pages)])
+    for which in range(2):
+        cache.codes[which][:] = np.clip(np.rint(rng.normal(size=cache.codes[which].shape) * 36), -127, 127)
+        cache.scale[which][:] = np.nan
+        cache.scale[which][named] = 0.02 * np.exp(0.5 * rng.normal(size=cache.scale[which][named].shape))
+    cache.weight[:] = np.nan
+    cache.weight[named] = np.exp(rng.normal(size=cache.weight[named].shape))
+    return cache
+
+
+def _attend(cache, pages, start, window, weigh, q, scale):
+    """(out, lse, weight added [n_kv, places of the table], the largest sum of |q_d k_d| of a score) of one sequence; q float64"""
+    rows, n_q, _ = q.shape
+    group, n_pages = n_q // cache.n_kv, len(cache.codes[0])
+    there = np.repeat((pages >= 0) & (pages < n_pages), plain.PAGE)
+    place = np.flatnonzero(there)
+    k, v = (cache.values(which, pages[(pages >= 0) & (pages < n_pages)], None) for which in range(2))
+    out, lse, added, terms = np.zeros(q.shape), np.full((rows, n_q), -np.inf), np.zeros((cache.n_kv, len(there))), 0.0
+    for i in range(rows):
+        seen = place <= start + i
+        if window:
+            seen &= place > start + i - window
+        if not seen.any():
+            continue
+        for h in range(n_q):
+            ks = k[seen, h // group]
+            s = ks @ q[i, h] * scale
+            terms = max(terms, (np.abs(ks) @ np.abs(q[i, h])).max() * scale)
+            p = np.exp(s - s.max())
+            out[i, h] = p @ v[seen, h // group] / p.sum()
+            lse[i, h] = s.max() + np.log(p.sum())
+            if i >= rows - weigh:
+                added[h // group, place[seen]] += p / p.sum()
+    return out, lse, added, terms
+
+
+def _check(rng, monkeypatch, table, starts, counts, n_q, n_kv, dim, block, kind, window=None, weigh=0):
+    from supersonic_b200.cache import Int8Pages
+    from supersonic_b200.csrc import int8_ops, ops
+    dtype, rows, n_pages = TYPES[kind], sum(counts), int(table[(table >= 0) & (table < MOST)].max()) - 1
+    cache = _cache(rng, table, n_pages, n_kv, dim, block)
+    pages = Int8Pages(*[torch.from_numpy(x).to(DEV) for x in (*cache.codes, *cache.scale, cache.weight.copy())])
+    q = torch.from_numpy(rng.normal(size=(rows, n_q, dim)) * 2).to(dtype)
+    qt = q.to(DEV).reshape(rows, -1)
+    out, lse = torch.full_like(qt, float("nan")), torch.full((rows, n_q), float("nan"), device=DEV)
+    guards, empty = [], torch.empty
+
+    def guarded(shape, *a, **kw):                                     # scratch, with a region behind it that nothing may touch
+        if not isinstance(shape, int) or kw.get("dtype") is not torch.float32:
+            return empty(shape, *a, **kw)
+        whole = torch.full((shape + GUARD,), 12345.0, **kw)
+        guards.append(whole[shape:])
+        return whole[:shape]
+    monkeypatch.setattr(torch, "empty", guarded)
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    scale = dim ** -0.5
+    int8_ops.attention(qt, pages, torch.from_numpy(table).to(DEV), _ints(cu), _ints(starts), _ints(list(range(len(counts)))), max(counts),
+                       out, n_q, scale, window=window, lse=lse, weigh_last=weigh)
+    monkeypatch.undo()
+    ops.check_device_errors()
+    assert all((g == 12345.0).all() for g in guards)
+    out, lse = out.float().cpu().numpy().reshape(rows, n_q, dim), lse.cpu().numpy()
+    weight, want_weight, terms = pages.weight.cpu().numpy(), cache.weight.astype(np.float64), 0.0
+    most_added = np.zeros_like(want_weight)
+    for b, (start, n) in enumerate(zip(starts, counts)):
+        own = slice(cu[b], cu[b + 1])
+        o, l, added, most = _attend(cache, table[b], start, window, weigh, q[own].double().numpy(), scale)
+        terms = max(terms, most)
+        # bounds as in test_int8_gpu.py: the rows' type's rounding, probabilities of 11 bits, float32 sums
+        top = max([np.abs(cache.values(1, [p], 64)).max() for p in table[b] if 0 <= p < n_pages], default=0.0)
+        bound = (2.0 ** -9 + 2.0 ** -10 if kind == "bf16" else 4e-6) * top + (2.0 ** -9 * np.abs(o) if kind == "bf16" else 0)
+        assert (np.abs(out[own] - o) <= bound).all(), b
+        none = np.isneginf(l)
+        assert np.array_equal(np.isneginf(lse[own]), none) and (out[own][none] == 0).all()
+        assert (np.abs(lse[own][~none] - l[~none]) <= 4e-6 * np.maximum(1.0, np.abs(l[~none]))).all()
+        for p, page in enumerate(table[b]):
+            if 0 <= page < n_pages:
+                want_weight[page] += added[:, 64 * p:64 * p + 64]
+                most_added[page] += added[:, 64 * p:64 * p + 64]
+    ok = np.abs(weight - want_weight) <= (1e-5 + 2.0 ** -21 * terms) * (most_added + 1e-3) + 2.0 ** -22 * np.abs(cache.weight)
+    assert (ok | (np.isnan(weight) & np.isnan(want_weight))).all()
+
+
+# head sizes and groups of the kernel of rows (one, two and four tiles of columns), the prompt kernel, and the plain one
+HEADS = [(64, 8, 2), (128, 4, 1), (128, 16, 1), (64, 40, 1), (32, 4, 2)]
+
+
+def _table(rng, n, width):
+    """Pages of ``n`` sequences, in no order; two ids stay outside the pool (see ``_check``: it ends two below the largest)."""
+    ids = rng.permutation(n * width)
+    return (ids + 3).astype(np.int32).reshape(n, width)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,n_q,n_kv", HEADS)
+@pytest.mark.parametrize("window", [None, 50, 1000])
+def test_single_tokens_whose_start_lies_behind_the_table(monkeypatch, kind, dim, n_q, n_kv, window):
+    rng = np.random.default_rng(dim + n_q)
+    starts = [3, 127, 128, 190, 5000, MOST, 64, MOST - 1]
+    _check(rng, monkeypatch, _table(rng, len(starts), 2), starts, [1] * len(starts), n_q, n_kv, dim, 16, kind, window, weigh=1)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,n_q,n_kv", HEADS)
+@pytest.mark.parametrize("window", [None, 50, 1000])
+def test_prompts_whose_start_lies_behind_the_table(monkeypatch, kind, dim, n_q, n_kv, window):
+    rng = np.random.default_rng(dim * n_q)
+    starts, counts = [0, 100, 150, 192, 4000, MOST - 200, 60], [70, 140, 33, 2, 40, 130, 0]
+    _check(rng, monkeypatch, _table(rng, len(starts), 3), starts, counts, n_q, n_kv, dim, 32, kind, window, weigh=20)
+
+
+def _with_holes(table):
+    table[0, 1], table[1, 0], table[2, :], table[3, -1] = -1, MOST, -(2 ** 31), table[table < MOST].max() + 2
+    return table
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,n_q,n_kv", HEADS)
+def test_single_tokens_over_page_ids_that_name_no_page(monkeypatch, kind, dim, n_q, n_kv):
+    rng = np.random.default_rng(dim + n_q)
+    for window in (None, 40):
+        _check(rng, monkeypatch, _with_holes(_table(rng, 4, 4)), [200, 255, 130, 250], [1] * 4, n_q, n_kv, dim, 16, kind, window, weigh=1)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,n_q,n_kv", HEADS)
+def test_prompts_over_page_ids_that_name_no_page(monkeypatch, kind, dim, n_q, n_kv):
+    rng = np.random.default_rng(dim + n_q)
+    for window in (None, 40):
+        _check(rng, monkeypatch, _with_holes(_table(rng, 4, 4)), [0, 100, 3, 200], [200, 140, 130, 56], n_q, n_kv, dim, 64, kind, window, weigh=9)
+
+
+@pytest.mark.parametrize("kind", ["bf16"])
+def test_parts_of_keys_over_page_ids_that_name_no_page(monkeypatch, kind):
+    """Few rows behind many keys: parts of them, some of which see nothing."""
+    rng = np.random.default_rng(9)
+    table = _table(rng, 2, 40)
+    table[0, 3:25], table[1, 8:], = -1, MOST
+    for window in (None, 700):
+        _check(rng, monkeypatch, table.copy(), [2400, 2450], [70, 100], 4, 1, 64, 16, kind, window, weigh=2)
