@@ -9,6 +9,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 #include <algorithm>
+#include <map>
+#include <mutex>
 #include <type_traits>
 
 typedef __nv_bfloat16 bf16;
@@ -988,16 +990,18 @@ template <typename K> static int ir_configure(K kernel, size_t smem) {
 
 struct IrPlan { int nt, tts, blocks; size_t piece; long long kept; };      // floats of a piece; of the scores that are kept
 
+// Blocks of a launch over n_seqs sequences, or -1.  Host threads may ask at the same time for different sizes, and what a thread is told
+// does not depend on who asked before: its scratch is sized by it.
 template <int HD, int NT, bool WIDE> static int ir_blocks(int n_seqs) {
-    static int blocks = 0;
-    static size_t at = 0;
-    const size_t smem = ir_smem<HD, NT>(n_seqs);
-    if (blocks == 0 || at != smem) {
-        if (ir_configure(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(IR_SEQS)) != 0) { cudaGetLastError(); return -1; }
-        blocks = ir_resident(int8_rows_kernel<HD, NT, WIDE>, smem);
-        at = smem;
-    }
-    return blocks;
+    static std::mutex lock;
+    static std::map<std::pair<int, int>, int> known;               // (device, sequences)
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) { cudaGetLastError(); return -1; }
+    const std::lock_guard<std::mutex> held(lock);
+    const auto at = known.find({device, n_seqs});
+    if (at != known.end()) return at->second;
+    if (ir_configure(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(IR_SEQS)) != 0) { cudaGetLastError(); return -1; }
+    return known[{device, n_seqs}] = ir_resident(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(n_seqs));
 }
 #define IR_EACH(HD_, NT_, WIDE_, WHAT_) \
     do { \
@@ -1032,13 +1036,15 @@ static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_page
     return p;
 }
 
+static long long ir_scratch(const IrPlan& p) { return 2LL * p.blocks * (long long)p.piece + p.kept; }
+
 // float32 elements of scratch that the launch needs.
 SSB_API long long ssb_int8_attention_scratch(int dtype, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim,
                                              int weigh_last, float scale) {
     if (n_seqs <= 0 || rows <= 0 || n_kv <= 0 || !ir_takes(n_q, n_kv, head_dim)) return 0;
     if (ia_tc_takes(dtype, head_dim, max_new, scale)) return ia_tc_scratch(n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
     const IrPlan p = ir_plan(dtype == SSB_F32, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, weigh_last);
-    return p.blocks < 0 ? 0 : 2LL * p.blocks * (long long)p.piece + p.kept;
+    return p.blocks < 0 ? 0 : ir_scratch(p);
 }
 
 template <int HD, int NT, bool WIDE>
@@ -1098,7 +1104,7 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
                                const float* k_scale, const float* v_scale, float* weight, const int* page_table, int n_slots,
                                int max_pages, int n_pages, const int* cu_new, const int* seq_start, const int* seq_slot,
                                int n_seqs, int rows, int max_new, int n_q, int n_kv, int head_dim, int block, int window, int weigh_last,
-                               float scale, float* scratch, int* error_word, cudaStream_t stream) {
+                               float scale, float* scratch, long long scratch_size, int* error_word, cudaStream_t stream) {
     if (n_seqs <= 0 || rows <= 0) return 0;
     if (head_dim % 16 || head_dim <= 0 || head_dim > 256 || n_kv <= 0 || n_q % n_kv || (block != 16 && block != 32 && block != 64) ||
         (n_q + 3) / 4 > 65535 || n_kv > 65535 || max_new <= 0 || max_pages <= 0 || n_pages <= 0 || !error_word)
@@ -1126,6 +1132,7 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
     if (rc) return rc;
     if (prompt) {
         if (ldq % 8 || ldo % 8 || (((uintptr_t)q | (uintptr_t)out) & 15)) return SSB_ERR_BAD_SIZE;
+        if (scratch_size < ia_tc_scratch(n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim)) return SSB_ERR_BAD_SIZE;
         rc = ia_tc_launch(a, max_new, scratch, error_word, stream);
         if (rc || weigh_last <= 0) return rc;
         return ia_weigh(a, wide, max_new, error_word, mk, stream);
@@ -1135,6 +1142,7 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
     if (!scratch) return SSB_ERR_BAD_SIZE;
     const IrPlan p = ir_plan(wide, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, weigh_last);
     if (p.blocks < 0) return SSB_ERR_UNSUPPORTED;
+    if (scratch_size < ir_scratch(p)) return SSB_ERR_BAD_SIZE;
 #define IR_ROWS(H_, N_, W_) rc = ir_rows<H_, N_, W_>(a, p, scratch, error_word, mk, mv, stream)
     IR_EACH(head_dim, p.nt, wide, IR_ROWS);
 #undef IR_ROWS

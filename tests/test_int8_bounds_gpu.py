@@ -161,3 +161,80 @@ def test_parts_of_keys_over_page_ids_that_name_no_page(monkeypatch, kind):
     table[0, 3:25], table[1, 8:], = -1, MOST
     for window in (None, 700):
         _check(rng, monkeypatch, table.copy(), [2400, 2450], [70, 100], 4, 1, 64, 16, kind, window, weigh=2)
+
+
+# ---- host threads -------------------------------------------------------------------------------------------------
+def test_the_scratch_of_a_batch_does_not_depend_on_who_asks_beside_it():
+    """Threads that ask for batches of other sizes all the time are told what one that asks alone is told."""
+    import threading
+    from supersonic_b200.csrc import int8_ops
+    ask = int8_ops._fn("ssb_int8_attention_scratch")
+    sizes = [8, 200, 1000, 60, 700, 1]
+    args = lambda n: (1, n, n, 1, 64, 32, 8, 128, 0, 0.125)                                  # noqa: E731
+    want, wrong = {n: ask(*args(n)) for n in sizes}, []
+    assert len(set(want.values())) > 1
+
+    def go(first):
+        for i in range(600):
+            n = sizes[(first + i) % len(sizes)]
+            if ask(*args(n)) != want[n]:
+                wrong.append(n)
+    threads = [threading.Thread(target=go, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, len(wrong)
+
+
+def test_two_host_threads_with_batches_of_different_sizes():
+    import threading
+    from supersonic_b200.cache import Int8Pages
+    from supersonic_b200.csrc import int8_ops, ops
+
+    def batch(n, seed):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        rand = lambda *s: torch.randn(s, generator=gen, device=DEV)                          # noqa: E731
+        pages = Int8Pages(*[(rand(2 * n, 2, 64, 128) * 36).clamp(-127, 127).to(torch.int8) for _ in range(2)],
+                          *[rand(2 * n, 2, 4).abs() + 0.01 for _ in range(2)])
+        table = torch.arange(2 * n, dtype=torch.int32, device=DEV).reshape(n, 2)
+        ints = (_ints(list(range(n + 1))), _ints([(37 * i) % 128 for i in range(n)]), _ints(list(range(n))))
+        q = rand(n, 8 * 128)
+        torch.cuda.synchronize()
+
+        def run():
+            out = torch.empty_like(q)
+            int8_ops.attention(q, pages, table, *ints, 1, out, 8, 0.125)
+            return out
+        return run
+    runs = [batch(8, 1), batch(200, 2)]
+    want, wrong = [r() for r in runs], []
+    torch.cuda.synchronize()
+
+    def go(which):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [runs[which]() for _ in range(100)]
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(which for o in outs if not torch.equal(o, want[which]))
+    threads = [threading.Thread(target=go, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    ops.check_device_errors()
+    assert not wrong
+
+
+@pytest.mark.parametrize("rows,start", [(1, 500), (300, 4000)])
+def test_a_scratch_that_is_too_small_is_refused(monkeypatch, rows, start):
+    from supersonic_b200.cache import Int8Pages
+    from supersonic_b200.csrc import int8_ops, ops
+    pages = Int8Pages.allocate(80, 1, 64, 16, device=DEV)
+    q = torch.zeros((rows, 64), dtype=torch.bfloat16, device=DEV)
+    table = torch.arange(80, dtype=torch.int32, device=DEV).reshape(1, 80)
+    args = (q, pages, table, _ints([0, rows]), _ints([start]), _ints([0]), rows, torch.zeros_like(q), 1, 0.125)
+    size = int8_ops._scratch_size
+    int8_ops.attention(*args)
+    monkeypatch.setattr(int8_ops, "_scratch_size", lambda *a: size(*a) - 1)
+    with pytest.raises(ops.KernelError):
+        int8_ops.attention(*args)
