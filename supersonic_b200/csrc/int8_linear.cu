@@ -37,6 +37,12 @@ __device__ __forceinline__ uint32_t il_block_max(uint32_t m, uint32_t* warp_max)
     return __reduce_max_sync(0xffffffffu, lane < warps ? warp_max[lane] : 0u);
 }
 
+// The launch's first block zeroes the product's counters: one for each of its blocks, a hundred or so.
+__device__ __forceinline__ void il_clear(int* clear, int n_clear) {
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < n_clear; i += blockDim.x) clear[i] = 0;
+}
+
 // A block a row, 8 numbers a thread and turn, all of them in registers between the row's maximum and its codes (NV turns).
 // ``clear``: words that the product counts in, zeroed here.  8,192 x 4,096 in bfloat16: 24 us, 4.2 TB/s.
 template <typename T, int NV>
@@ -47,7 +53,7 @@ int8_quantize_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ code
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
     const int row = blockIdx.x;
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n_clear; i += gridDim.x * blockDim.x) clear[i] = 0;
+    il_clear(clear, n_clear);
     float v[NV][8];
     uint32_t top = 0;
 #pragma unroll
@@ -88,7 +94,7 @@ int8_quantize_any_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ 
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
     const T* src = x + (size_t)blockIdx.x * ldx;
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < n_clear; i += gridDim.x * 256) clear[i] = 0;
+    il_clear(clear, n_clear);
     uint32_t top = 0;
     for (int k = threadIdx.x; k < K; k += 256) top = max(top, __float_as_uint(fabsf(i8_finite(ssb_to_float(src[k])))));
     const float s = fmaxf(__fmul_rn(__uint_as_float(il_block_max(top, warp_max[0])), 1.f / 127.f), I8_LEAST_SCALE), inverse = 1.f / s;

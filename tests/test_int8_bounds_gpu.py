@@ -238,3 +238,20 @@ def test_a_scratch_that_is_too_small_is_refused(monkeypatch, rows, start):
     monkeypatch.setattr(int8_ops, "_scratch_size", lambda *a: size(*a) - 1)
     with pytest.raises(ops.KernelError):
         int8_ops.attention(*args)
+
+
+# ---- products -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,k", [(8_400_000, 4), (67_200_000, 8)])
+def test_rows_beyond_32_bits_of_threads_are_quantised(rows, k):
+    """More rows than a launch's threads can be counted in 32 bits, with 256 and with 32 threads a row."""
+    from supersonic_b200.csrc import int8_ops
+    gen = torch.Generator(device=DEV).manual_seed(rows)
+    x = torch.empty((rows, k), dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    codes, scale = torch.full((rows, k), 99, dtype=torch.int8, device=DEV), torch.zeros(rows, device=DEV)
+    int8_ops.quantize_rows(x, codes, scale)
+    for part in (slice(0, 2000), slice(rows // 2 - 1000, rows // 2 + 1000), slice(rows - 2000, rows)):
+        xs = x[part].float().cpu().numpy()
+        for i in range(0, 2000, 97):
+            want, s = plain.quantize(xs[i])
+            assert np.array_equal(codes[part][i].cpu().numpy(), want) and scale[part][i].item() == s
+    assert (scale > 0).all()
