@@ -1,6 +1,6 @@
 // Matrix products in 8-bit integers: out[m, n] (+)= (sum_k xc[m, k] wc[n, k]) * sx[m] * sw[n], with the rows of x quantised as they
 // come (sx = max |x_row| * (1/127), xc = rint(x / sx)) and weights that lie in codes with a scale per output channel.  The sums are
-// exact: 32-bit integers up to k = 133,136 (127 * 127 * k < 2^31), which is checked.  So a result has the same bits whatever
+// exact: 32-bit integers up to k = 132,096 (127 * 128 * k < 2^31, of weights down to -128), which is checked.  So a result has the same bits whatever
 // kernel, cut of k or batch it was computed in.
 //
 // Three launches' worth of code, two launches a call: the rows' codes; then one of two products on the fifth-generation tensor
@@ -19,7 +19,7 @@
 
 typedef __nv_bfloat16 bf16;
 
-constexpr int IL_MOST_K = 133136;
+constexpr int IL_MOST_K = 132096;
 
 // ---- rows to codes ------------------------------------------------------------------------------------------------
 // rint(x / s), the division correctly rounded (as in i8_encode8).

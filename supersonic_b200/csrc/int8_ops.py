@@ -251,7 +251,7 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
 
 
 # ---- matrix products ------------------------------------------------------------------------------------------------
-MOST_K = 133136        # 127 * 127 * k stays below 2^31
+MOST_K = 132096        # 127 * 128 * k stays below 2^31: rows' codes go to 127, weights may be -128
 
 
 def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
@@ -274,7 +274,7 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> 
 def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, out: torch.Tensor, accumulate: bool = False) -> None:
     """``out`` [rows, n] (+)= x W^T with ``x`` (float32 or bfloat16 [rows, k]) quantised row by row as it comes and ``weight`` int8
     [n, k] with ``weight_scale`` (float32 [n]): the sum of products of codes is an exact integer, times the row's scale, times the
-    channel's.  ``accumulate`` adds to a float32 ``out``.  k: a multiple of 16 up to 133,136; n: a multiple of 8."""
+    channel's.  ``accumulate`` adds to a float32 ``out``.  k: a multiple of 16 up to 132,096; n: a multiple of 8."""
     rows, k = x.shape
     n = weight.shape[0]
     if weight.dtype is not _INT8 or weight.dim() != 2 or weight.shape[1] != k or not weight.is_cuda or weight.stride(1) != 1 \

@@ -255,3 +255,26 @@ def test_rows_beyond_32_bits_of_threads_are_quantised(rows, k):
             want, s = plain.quantize(xs[i])
             assert np.array_equal(codes[part][i].cpu().numpy(), want) and scale[part][i].item() == s
     assert (scale > 0).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_the_largest_sums_of_weights_of_minus_128(rows):
+    """Products of 127 x -128 throughout, at the largest k that is taken: a sum of -(2^31 - 131,072)."""
+    from supersonic_b200.csrc import int8_ops, ops
+    k = int8_ops.MOST_K
+    assert 127 * 128 * k < 2 ** 31 <= 127 * 128 * (k + 16)
+    x = torch.ones((rows, k), device=DEV)
+    x[:, 1::2] = -1
+    w = torch.full((8, k), -128, dtype=torch.int8, device=DEV)
+    w[:, 1::2] = 127                                              # whose sum is k / 2 times 127 x 255
+    w[5, 0::2], w[5, 1::2] = 127, -128
+    w[3] = -128
+    out, same = torch.zeros((rows, 8), device=DEV), torch.zeros((rows, 8), device=DEV)
+    int8_ops.linear(x, w, torch.ones(8, device=DEV), out)
+    by = np.float32(1) / np.float32(127)
+    assert (out[:, 0] == float(-np.float32(127 * 255 * (k // 2)) * by)).all() and (out[:, 5] == -out[:, 0]).all() and (out[:, 3] == 0).all()
+    int8_ops.linear(x.abs(), w, torch.ones(8, device=DEV), same)
+    assert (same[:, 3] == float(-np.float32(127 * 128 * k) * by)).all()
+    wide = torch.zeros((8, k + 16), dtype=torch.int8, device=DEV)
+    with pytest.raises(ops.KernelError):
+        int8_ops.linear(torch.ones((rows, k + 16), device=DEV), wide, torch.ones(8, device=DEV), out)
