@@ -67,14 +67,14 @@ int8_attention_plain_kernel(const IaArgs a) {
                 for (int e = 0; e < 4; ++e) o[w][e] = fmaf(pv, (float)(int8_t)(c >> (8 * e)), o[w][e] * keep);
             }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int w = 0; w < 2; ++w)
         if (lane + 32 * w < words)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 ((T*)a.out)[(size_t)row * a.ldo + (size_t)head * a.head_dim + 4 * (lane + 32 * w) + e] = ssb_from_float<T>(o[w][e] * inv);
-    if (lane == 0 && a.lse) a.lse[(size_t)row * a.n_q + head] = l > 0.f ? m + logf(l) : -INFINITY;
+    if (lane == 0 && a.lse) a.lse[(size_t)row * a.n_q + head] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 // What the last rows of every sequence attend to: a warp a key, over those rows and the heads of the group; the key's weight is its
@@ -799,7 +799,8 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     }
 }
 
-// What single tokens attend to, from the scores that int8_rows_kernel kept: a page a warp, a lane four keys of every second head.
+// What single tokens attend to, from the scores that int8_rows_kernel kept: a page a warp, a lane four keys of every second head.  A row
+// whose sum is no number makes the weights of the keys that it sees none, as the formula has it (eviction ranks those lowest).
 // 16 sequences of 8,000, 32 heads over 8: 17 MB of scores in 13 us.
 __global__ void __launch_bounds__(IR_THREADS)
 int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict__ kept) {
@@ -837,7 +838,8 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
                 const int h = 2 * i + (lane >> 4);
                 if (h < group) {
                     const float4 v = __ldcg(reinterpret_cast<const float4*>(src + (part * group + h) * 16 + 4 * t));
-                    sum.x += ir_ex2(v.x - ref[i]); sum.y += ir_ex2(v.y - ref[i]); sum.z += ir_ex2(v.z - ref[i]); sum.w += ir_ex2(v.w - ref[i]);
+                    auto weight = [&](float x) { return x == -INFINITY ? 0.f : ir_ex2(x - ref[i]); };          // -inf: not seen
+                    sum.x += weight(v.x); sum.y += weight(v.y); sum.z += weight(v.z); sum.w += weight(v.w);
                 }
             }
             sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16); sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
@@ -846,8 +848,8 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
             // one order, and nobody waits for it
             float* w = a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + 16 * part + t + (lane & 16 ? 8 : 0);
             const float x = lane & 16 ? sum.z : sum.x, y = lane & 16 ? sum.w : sum.y;
-            if (there && x > 0.f) atomicAdd(w, x);
-            if (there && y > 0.f) atomicAdd(w + 4, y);
+            if (there && x != 0.f) atomicAdd(w, x);
+            if (there && y != 0.f) atomicAdd(w + 4, y);
         }
     }
 }
@@ -953,7 +955,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
             x += __shfl_xor_sync(0xffffffffu, up1 ? x0 : x1, 8);
             x += __shfl_xor_sync(0xffffffffu, x, 4);
             const int key = key0 + t + 4 * (2 * up2 + up1);
-            if (!(lane & 4) && id >= 0 && key < s.start + s.n_new && x > 0.f)
+            if (!(lane & 4) && id >= 0 && key < s.start + s.n_new && x != 0.f)
                 atomicAdd(a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + (key & 63), x);
         }
         u = seg.next;

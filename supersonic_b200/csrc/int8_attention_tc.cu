@@ -666,7 +666,7 @@ int8_join_kernel(const IaArgs a, int s0, int n_seqs, int parts, const float* __r
         const size_t at = ((size_t)p * a.rows + row) * a.n_q + head;
         const float2 ml = __ldcg(part_ml + at);
         const float4 v = __ldcg(reinterpret_cast<const float4*>(part_o + at * HD + d));
-        const float by = ml.x == -INFINITY ? 0.f : it_ex2(ml.x - m);
+        const float by = ml.x == -INFINITY ? ml.y : it_ex2(ml.x - m);       // a part that saw nothing has a sum of 0, one of no numbers none
         o.x = fmaf(v.x, by, o.x); o.y = fmaf(v.y, by, o.y); o.z = fmaf(v.z, by, o.z); o.w = fmaf(v.w, by, o.w);
         l = fmaf(ml.y, by, l);
     }

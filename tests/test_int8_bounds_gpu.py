@@ -57,15 +57,19 @@ def _attend(cache, pages, start, window, weigh, q, scale):
     return out, lse, added, terms
 
 
-def _check(rng, monkeypatch, table, starts, counts, n_q, n_kv, dim, block, kind, window=None, weigh=0):
+def _check(rng, monkeypatch, table, starts, counts, n_q, n_kv, dim, block, kind, window=None, weigh=0, bad=()):
+    """``bad``: (row, head) of queries that hold a NaN: their results are NaN, and the weights of what they account for."""
     from supersonic_b200.cache import Int8Pages
     from supersonic_b200.csrc import int8_ops, ops
     dtype, rows, n_pages = TYPES[kind], sum(counts), int(table[(table >= 0) & (table < MOST)].max()) - 1
     cache = _cache(rng, table, n_pages, n_kv, dim, block)
     pages = Int8Pages(*[torch.from_numpy(x).to(DEV) for x in (*cache.codes, *cache.scale, cache.weight.copy())])
     q = torch.from_numpy(rng.normal(size=(rows, n_q, dim)) * 2).to(dtype)
-    qt = q.to(DEV).reshape(rows, -1)
-    out, lse = torch.full_like(qt, float("nan")), torch.full((rows, n_q), float("nan"), device=DEV)
+    given = q.clone()
+    for row, head in bad:
+        given[row, head, dim // 3] = float("nan")
+    qt = given.to(DEV).reshape(rows, -1)
+    out, lse = torch.full_like(qt, 7.0), torch.full((rows, n_q), 7.0, device=DEV)
     guards, empty = [], torch.empty
 
     def guarded(shape, *a, **kw):                                     # scratch, with a region behind it that nothing may touch
@@ -84,14 +88,26 @@ def _check(rng, monkeypatch, table, starts, counts, n_q, n_kv, dim, block, kind,
     assert all((g == 12345.0).all() for g in guards)
     out, lse = out.float().cpu().numpy().reshape(rows, n_q, dim), lse.cpu().numpy()
     weight, want_weight, terms = pages.weight.cpu().numpy(), cache.weight.astype(np.float64), 0.0
-    most_added = np.zeros_like(want_weight)
+    most_added, lost = np.zeros_like(want_weight), np.zeros(weight.shape, bool)
     for b, (start, n) in enumerate(zip(starts, counts)):
         own = slice(cu[b], cu[b + 1])
+        spoilt = np.zeros((n, n_q), bool)
+        for row, head in bad:
+            if cu[b] <= row < cu[b + 1]:
+                spoilt[row - cu[b], head] = True
+                if row >= cu[b + 1] - weigh:
+                    for j in range(max(0, start + row - cu[b] - window + 1 if window else 0), start + row - cu[b] + 1):
+                        if 0 <= table[b, j // 64] < n_pages:
+                            lost[table[b, j // 64], head // (n_q // n_kv), j % 64] = True
         o, l, added, most = _attend(cache, table[b], start, window, weigh, q[own].double().numpy(), scale)
         terms = max(terms, most)
         # bounds as in test_int8_gpu.py: the rows' type's rounding, probabilities of 11 bits, float32 sums
         top = max([np.abs(cache.values(1, [p], 64)).max() for p in table[b] if 0 <= p < n_pages], default=0.0)
         bound = (2.0 ** -9 + 2.0 ** -10 if kind == "bf16" else 4e-6) * top + (2.0 ** -9 * np.abs(o) if kind == "bf16" else 0)
+        seen_nan = spoilt & ~np.isneginf(l)
+        assert np.isnan(out[own][seen_nan]).all() and np.isnan(lse[own][seen_nan]).all()
+        o, l = np.where(seen_nan[..., None], 0, o), np.where(seen_nan, 0, l)
+        out[own], lse[own] = np.where(seen_nan[..., None], 0, out[own]), np.where(seen_nan, 0, lse[own])
         assert (np.abs(out[own] - o) <= bound).all(), b
         none = np.isneginf(l)
         assert np.array_equal(np.isneginf(lse[own]), none) and (out[own][none] == 0).all()
@@ -100,6 +116,8 @@ def _check(rng, monkeypatch, table, starts, counts, n_q, n_kv, dim, block, kind,
             if 0 <= page < n_pages:
                 want_weight[page] += added[:, 64 * p:64 * p + 64]
                 most_added[page] += added[:, 64 * p:64 * p + 64]
+    assert np.isnan(weight[lost]).all()
+    weight, want_weight = np.where(lost, 0, weight), np.where(lost, 0, want_weight)
     ok = np.abs(weight - want_weight) <= (1e-5 + 2.0 ** -21 * terms) * (most_added + 1e-3) + 2.0 ** -22 * np.abs(cache.weight)
     assert (ok | (np.isnan(weight) & np.isnan(want_weight))).all()
 
@@ -161,6 +179,18 @@ def test_parts_of_keys_over_page_ids_that_name_no_page(monkeypatch, kind):
     table[0, 3:25], table[1, 8:], = -1, MOST
     for window in (None, 700):
         _check(rng, monkeypatch, table.copy(), [2400, 2450], [70, 100], 4, 1, 64, 16, kind, window, weigh=2)
+
+
+# ---- queries that are no numbers --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,n_q,n_kv", HEADS)
+@pytest.mark.parametrize("starts,counts,weigh", [([3, 127, 150, 60], [1] * 4, 1), ([0, 100, 3], [70, 92, 1], 20), ([1500, 40], [70, 60], 3)])
+def test_a_query_that_is_no_number_spoils_what_it_sees_and_nothing_else(monkeypatch, kind, dim, n_q, n_kv, starts, counts, weigh):
+    rng = np.random.default_rng(dim + n_q)
+    table = _table(rng, len(starts), -(-max(s + n for s, n in zip(starts, counts)) // 64))
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    bad = [(cu[1] - 1, 0), (0, n_q - 1), (cu[2] - 1, n_q // 2)]        # sequences' last rows, and a first one that may not account
+    _check(rng, monkeypatch, table, starts, counts, n_q, n_kv, dim, 16, kind, 90, weigh, bad)
 
 
 # ---- host threads -------------------------------------------------------------------------------------------------
