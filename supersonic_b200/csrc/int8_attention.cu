@@ -827,30 +827,34 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
             ref[i] = h < group ? a.lse[(size_t)s.row0 * a.n_q + seg.kvh * group + h] * 1.4426950408889634f : INFINITY;
         }
         const int part = (lane & 15) >> 2, t = lane & 3;
-#pragma unroll 2
-        for (int p = warp; p < seg.n; p += IR_WARPS) {
-            const float* src = kept + (seg.at + p) * (IR_WARPS * 16) * group;
-            const int id = a.page_table[(size_t)s.slot * a.max_pages + min(seg.page + p, a.max_pages - 1)];
-            const bool there = ia_in_pool(a, id);
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto pages = [&](auto none) {                              // whether a row saw nothing or has no number for its sum: -inf, which it does not see, counts 0
+#pragma unroll (decltype(none)::value ? 1 : 2)
+            for (int p = warp; p < seg.n; p += IR_WARPS) {
+                const float* src = kept + (seg.at + p) * (IR_WARPS * 16) * group;
+                const int id = a.page_table[(size_t)s.slot * a.max_pages + min(seg.page + p, a.max_pages - 1)];
+                const bool there = ia_in_pool(a, id);
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int h = 2 * i + (lane >> 4);
-                if (h < group) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(src + (part * group + h) * 16 + 4 * t));
-                    auto weight = [&](float x) { return x == -INFINITY ? 0.f : ir_ex2(x - ref[i]); };          // -inf: not seen
-                    sum.x += weight(v.x); sum.y += weight(v.y); sum.z += weight(v.z); sum.w += weight(v.w);
+                for (int i = 0; i < 4; ++i) {
+                    const int h = 2 * i + (lane >> 4);
+                    if (h < group) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(src + (part * group + h) * 16 + 4 * t));
+                        auto weight = [&](float x) { return decltype(none)::value && x == -INFINITY ? 0.f : ir_ex2(x - ref[i]); };
+                        sum.x += weight(v.x); sum.y += weight(v.y); sum.z += weight(v.z); sum.w += weight(v.w);
+                    }
                 }
+                sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16); sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
+                sum.z += __shfl_xor_sync(0xffffffffu, sum.z, 16); sum.w += __shfl_xor_sync(0xffffffffu, sum.w, 16);
+                // keys t, t + 4, t + 8, t + 12 of 16: the lower half adds the first two, the upper the others; one addition a key, so in
+                // one order, and nobody waits for it
+                float* w = a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + 16 * part + t + (lane & 16 ? 8 : 0);
+                const float x = lane & 16 ? sum.z : sum.x, y = lane & 16 ? sum.w : sum.y;
+                if (there && x != 0.f) atomicAdd(w, x);
+                if (there && y != 0.f) atomicAdd(w + 4, y);
             }
-            sum.x += __shfl_xor_sync(0xffffffffu, sum.x, 16); sum.y += __shfl_xor_sync(0xffffffffu, sum.y, 16);
-            sum.z += __shfl_xor_sync(0xffffffffu, sum.z, 16); sum.w += __shfl_xor_sync(0xffffffffu, sum.w, 16);
-            // keys t, t + 4, t + 8, t + 12 of 16: the lower half adds the first two, the upper the others; one addition a key, so in
-            // one order, and nobody waits for it
-            float* w = a.weight + ((size_t)id * a.n_kv + seg.kvh) * 64 + 16 * part + t + (lane & 16 ? 8 : 0);
-            const float x = lane & 16 ? sum.z : sum.x, y = lane & 16 ? sum.w : sum.y;
-            if (there && x != 0.f) atomicAdd(w, x);
-            if (there && y != 0.f) atomicAdd(w + 4, y);
-        }
+        };
+        if (__all_sync(0xffffffffu, ref[0] > -INFINITY && ref[1] > -INFINITY && ref[2] > -INFINITY && ref[3] > -INFINITY)) pages(std::false_type{});
+        else pages(std::true_type{});
     }
 }
 
