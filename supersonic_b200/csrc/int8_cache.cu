@@ -515,9 +515,10 @@ int8_select_kernel(const float* __restrict__ weight, const int* __restrict__ pag
 
 constexpr int I8_MOVE_THREADS = 256;
 
-// The kept tokens of one destination page and kv head: codes under the largest scale of their new block, weights beside them.  A
-// thread's pieces of codes are on their way while the block's scales are compared.  4 x 8 times 4,096 tokens of 128: 67 MB in 25 us,
-// 2.7 TB/s; bound by fetches that wait for one another (the place, its page, the codes and scale under it).
+// The kept tokens of one destination page and kv head: codes under the largest scale of their new block, weights beside them; zeros of
+// a token whose page id names no page.  A thread's pieces of codes are on their way while the block's scales are compared.  4 x 8 times
+// 4,096 tokens of 128: 67 MB in 25 us, 2.7 TB/s; bound by fetches that wait for one another (the place, its page, the codes and scale
+// under it).
 template <int LANES>
 __global__ void __launch_bounds__(I8_MOVE_THREADS)
 int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restrict__ k_scale, float* __restrict__ v_scale,
@@ -533,12 +534,13 @@ int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restri
     const int j = threadIdx.x < I8_PAGE && mine < keep ? kept[((size_t)b * n_kv + head) * keep + mine] : -1;
     if (s < 0 || s >= n_slots || target < 0 || target >= n_pages) return;
     const int per = I8_PAGE / block;
-    __shared__ long long from[I8_PAGE];                        // the row's place among all rows, or -1
+    __shared__ long long from[I8_PAGE];                        // the row's place among all rows, -1: nothing is kept there, or -2: kept, but in no page
     __shared__ float scale[2][I8_PAGE];
     const size_t head_at = (size_t)target * n_kv + head;
     if (threadIdx.x < I8_PAGE) {
         long long row = -1;
-        if (j >= 0 && (j >> 6) < max_pages) {
+        if (j >= 0) {
+            row = -2;
             const int page = page_table[(size_t)s * max_pages + (j >> 6)];
             if (page >= 0 && page < n_pages) row = ((long long)page * n_kv + head) * I8_PAGE + (j & 63);
         }
@@ -560,17 +562,21 @@ int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restri
         const int row = threadIdx.x - 2 * I8_PAGE;
         if (from[row] >= 0) weight[head_at * I8_PAGE + row] = weight[from[row]];
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        const int e = threadIdx.x + i * I8_MOVE_THREADS, which = e / (I8_PAGE * LANES), row = e / LANES % I8_PAGE;
-        if (e >= 2 * I8_PAGE * LANES || from[row] < 0) continue;
-        const int first = row / block * block;
+    const bool homeless = __syncthreads_or(threadIdx.x < I8_PAGE && from[threadIdx.x % I8_PAGE] == -2);
+    auto largest = [&](int which, int first) {
         float m = 0.f;
         for (int r = first; r < first + block; r += 4) {
             const float4 f = *reinterpret_cast<const float4*>(&scale[which][r]);
             m = fmaxf(fmaxf(m, fmaxf(f.x, f.y)), fmaxf(f.z, f.w));
         }
+        return m;
+    };
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int e = threadIdx.x + i * I8_MOVE_THREADS, which = e / (I8_PAGE * LANES), row = e / LANES % I8_PAGE;
+        if (e >= 2 * I8_PAGE * LANES || from[row] < 0) continue;
+        const int first = row / block * block;
+        const float m = largest(which, first);
         if (e % LANES == 0 && row == first) (which ? v_scale : k_scale)[head_at * per + row / block] = m;        // the block's first row is kept if any is
         if (scale[which][row] != m) {
             const float ratio = __fdiv_rn(scale[which][row], m);
@@ -579,6 +585,14 @@ int8_move_kernel(int8_t* __restrict__ k, int8_t* __restrict__ v, float* __restri
         }
         reinterpret_cast<uint4*>((which ? v : k) + (head_at * I8_PAGE + row) * (16 * LANES))[e % LANES] = c[i];
     }
+    if (homeless)
+        for (int e = threadIdx.x; e < 2 * I8_PAGE * LANES; e += I8_MOVE_THREADS) {
+            const int which = e / (I8_PAGE * LANES), row = e / LANES % I8_PAGE, first = row / block * block;
+            if (from[row] != -2) continue;
+            reinterpret_cast<uint4*>((which ? v : k) + (head_at * I8_PAGE + row) * (16 * LANES))[e % LANES] = make_uint4(0, 0, 0, 0);
+            if (e % LANES == 0 && row == first) (which ? v_scale : k_scale)[head_at * per + row / block] = largest(which, first);
+            if (e % LANES == 0 && weight && !which) weight[head_at * I8_PAGE + row] = 0.f;
+        }
 }
 
 SSB_API int ssb_int8_evict(void* k, void* v, float* k_scale, float* v_scale, float* weight, const int* page_table, int n_slots,

@@ -197,7 +197,8 @@ def evict(pages: Int8Pages, page_table: torch.Tensor, seq_slot: torch.Tensor, le
     What stays is moved, in its order, to the pages named by ``new_table`` [sequences, pages], which no sequence may hold: codes
     under the largest scale of their new block, weights as they are.  ``kept`` (int32 [sequences, kv heads, keep]) gets the places
     that stayed, -1 behind the last.  Afterwards a sequence has min(length, keep) tokens, in ``new_table``'s row; its old pages
-    can be given back.  Keys stay rotated by the positions they had."""
+    can be given back.  Keys stay rotated by the positions they had.  A place whose page id names no page is the last to be
+    chosen, and zeros where it stays."""
     n_pages, n_kv, dim, block, at, table, slots, per_seq = _pages(pages, page_table)
     B = seq_slot.shape[0]
     if pages.weight is None:

@@ -308,3 +308,42 @@ def test_the_largest_sums_of_weights_of_minus_128(rows):
     wide = torch.zeros((8, k + 16), dtype=torch.int8, device=DEV)
     with pytest.raises(ops.KernelError):
         int8_ops.linear(torch.ones((rows, k + 16), device=DEV), wide, torch.ones(8, device=DEV), out)
+
+
+# ---- eviction -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim,block", [(64, 16), (128, 64), (16, 32)])
+def test_evict_over_page_ids_that_name_no_page(dim, block):
+    """Tokens without a page are the last to be chosen; those that stay all the same are zeros, and spoil nobody's scale."""
+    from supersonic_b200.cache import Int8Pages
+    from supersonic_b200.csrc import int8_ops
+    rng, n_kv, n, keep, first, recent = np.random.default_rng(dim), 2, 700, 500, 10, 70
+    table = np.arange(11, dtype=np.int32)[None, ::-1].copy()
+    table[0, [0, 3, 7, 10]] = -1, MOST, 30, -5                            # the first tokens, the last ones, and some between
+    target = np.arange(11, 19, dtype=np.int32)[None]
+    cache = plain.Cache(20, n_kv, dim, block)
+    for which in range(2):
+        cache.codes[which][:] = np.clip(np.rint(rng.normal(size=cache.codes[which].shape) * 36), -127, 127)
+        cache.scale[which][:] = 0.02 * np.exp(0.5 * rng.normal(size=cache.scale[which].shape))
+    cache.weight[:] = rng.normal(size=cache.weight.shape)
+    cache.weight[table[0, 5], :, ::2] = -np.inf
+    pages = Int8Pages(*[torch.from_numpy(t).to(DEV) for t in (*cache.codes, *cache.scale, cache.weight.copy())])
+    kept = torch.zeros((1, n_kv, keep), dtype=torch.int32, device=DEV)
+    int8_ops.evict(pages, torch.from_numpy(table).to(DEV), _ints([0]), _ints([n]), torch.from_numpy(target).to(DEV), keep, first, recent, kept)
+    out = [torch.full((1, keep, n_kv, dim), 9.0, device=DEV) for _ in range(2)]
+    int8_ops.read(pages, torch.from_numpy(target).to(DEV), _ints([0]), _ints([keep]), *out)
+    there = np.repeat((table[0] >= 0) & (table[0] < 20), 64)[:n]
+    for h in range(n_kv):
+        w = [cache.weight[table[0, j // 64], h, j % 64] if there[j] else 0.0 for j in range(n)]
+        middle = sorted(range(first, n - recent), key=lambda j: (not there[j], -w[j], j))[:keep - first - recent]
+        stay = sorted([*range(first), *middle, *range(n - recent, n)])
+        assert kept[0, h].tolist() == stay
+        for i0 in range(0, keep, block):
+            run = stay[i0:i0 + block]
+            for which in range(2):
+                s = np.array([cache.scale[which][table[0, j // 64], h, j % 64 // block] if there[j] else 0 for j in run], np.float32)
+                for i, j in enumerate(run):
+                    c = cache.codes[which][table[0, j // 64], h, j % 64].astype(np.float32) if there[j] else np.zeros(dim, np.float32)
+                    want = np.rint(c * (s[i] / s.max())) * s.max() if s.max() > 0 else c
+                    assert np.array_equal(out[which][0, i0 + i, h].cpu().numpy(), want), (h, i0 + i)
+        moved = pages.weight[torch.from_numpy(target[0]).long().to(DEV), h].reshape(-1)[:keep].cpu().numpy()
+        assert np.array_equal(moved, [w[j] for j in stay])
