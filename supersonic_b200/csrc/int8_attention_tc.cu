@@ -13,7 +13,8 @@
 // * Scales stay out of the products.  16 keys have one scale of keys, which multiplies their scores where the softmax scales them
 //   anyway, and one of values, whose logarithm goes into the exponent: 2^(s ks + log2 vs - m) is a probability times its value's
 //   scale, at no instruction more than the probability alone; a group's sum is divided by vs once before it counts in the
-//   denominator.  The maximum m is over s ks + log2 vs, so float16 holds what is summed whatever the scales are.
+//   denominator.  The maximum m is over s ks + log2 vs, so float16 holds what is summed; the denominator
+//   has all keys whose values' scales are within 2^90 of one another.
 //
 // A row's reference moves only when a maximum is 2^12 above it (float16 holds up to 2^16), and only then is O rescaled; what lies
 // 2^-14 below the reference is rounded to 2^-25 of it, and a sum is at least 2^-12 of the largest.  Every mbarrier wait is bounded.

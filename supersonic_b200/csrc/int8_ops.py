@@ -225,7 +225,7 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
     ``lse`` (float32 [rows, n_q]) gets the logarithm of a row's sum of exponentials.  ``weigh_last``: that many last rows of every
     sequence add their probabilities, summed over the query heads of a kv head, to ``pages.weight``.  Rows of a sequence with a
     negative slot are zeros, and their ``lse`` minus infinity.  A place behind the table's end, or under a page id that names no page,
-    holds a key that no row sees."""
+    holds a key that no row sees.  The values' scales that a row sees have to be within 2^90 of one another."""
     n_pages, n_kv, dim, block, at, table, slots, width = _pages(pages, page_table)
     rows, B = q.shape[0], seq_slot.shape[0]
     if n_q <= 0 or n_q % n_kv:

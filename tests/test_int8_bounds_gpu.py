@@ -181,6 +181,37 @@ def test_parts_of_keys_over_page_ids_that_name_no_page(monkeypatch, kind):
         _check(rng, monkeypatch, table.copy(), [2400, 2450], [70, 100], 4, 1, 64, 16, kind, window, weigh=2)
 
 
+# ---- batches of several launches, odd groups, scales --------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_more_single_tokens_than_a_launch_takes(monkeypatch, kind):
+    rng, n = np.random.default_rng(3), 1100
+    _check(rng, monkeypatch, _table(rng, n, 2), [(31 * i) % 128 for i in range(n)], [1] * n, 2, 1, 64, 16, kind, weigh=1)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_more_prompts_than_a_launch_takes(monkeypatch, kind):
+    rng, n = np.random.default_rng(4), 530
+    counts = [33 + i % 5 for i in range(n)]
+    _check(rng, monkeypatch, _table(rng, n, 2), [(17 * i) % 90 for i in range(n)], counts, 2, 1, 64, 16, kind, weigh=2)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,n_q,n_kv", [(64, 3, 1), (128, 5, 1), (64, 14, 2)])
+@pytest.mark.parametrize("window", [1, 70, 200])
+def test_odd_groups_in_a_window(monkeypatch, kind, dim, n_q, n_kv, window):
+    rng = np.random.default_rng(n_q)
+    _check(rng, monkeypatch, _table(rng, 3, 7), [0, 150, 300], [260, 130, 40], n_q, n_kv, dim, 32, kind, window, weigh=5)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [150, 1, 30]])
+def test_value_scales_very_far_apart(kind, dim, counts):
+    """Scales of values up to 2^90 of each other."""
+    from test_int8_gpu import _check_attention
+    _check_attention(np.random.default_rng(8), [300, 129, 40], counts, 8, 2, dim, 16, kind, weigh=1, v_spread=45)
+
+
 # ---- queries that are no numbers --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("dim,n_q,n_kv", HEADS)
