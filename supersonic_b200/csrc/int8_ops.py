@@ -276,9 +276,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, ou
     """``out`` [rows, n] (+)= x W^T with ``x`` (float32 or bfloat16 [rows, k]) quantised row by row as it comes and ``weight`` int8
     [n, k] with ``weight_scale`` (float32 [n]): the sum of products of codes is an exact integer, times the row's scale, times the
     channel's.  ``accumulate`` adds to a float32 ``out``.  k: a multiple of 16 up to 132,096; n: a multiple of 8."""
+    if x.dim() != 2 or weight.dim() != 2:
+        raise KernelError(f"linear: x and weight must be matrices, are {tuple(x.shape)} and {tuple(weight.shape)}")
     rows, k = x.shape
     n = weight.shape[0]
-    if weight.dtype is not _INT8 or weight.dim() != 2 or weight.shape[1] != k or not weight.is_cuda or weight.stride(1) != 1 \
+    if weight.dtype is not _INT8 or weight.shape[1] != k or not weight.is_cuda or weight.stride(1) != 1 \
             or (weight.data_ptr() | weight.stride(0)) % 16:
         raise KernelError(f"linear: weight must be int8 [n, {k}] with rows on 16 bytes, is {weight.dtype} {tuple(weight.shape)}")
     if k % 16 or not 0 < k <= MOST_K or n % 8:

@@ -115,3 +115,12 @@ def test_pages_refuse_sizes_they_cannot_have():
             Int8Pages.allocate(**{**dict(n_pages=2, n_kv_heads=1, head_dim=64, device="cpu"), **kw})
     p = Int8Pages.allocate(2, 3, 64, block=32, weights=True, device="cpu")
     assert p.block == 32 and p.bytes_held() == 2 * (2 * 3 * 64 * 64) + 2 * (2 * 3 * 2 * 4) + 2 * 3 * 64 * 4
+
+
+@pytest.mark.parametrize("kw", [{"x": z(32)}, {"x": z(2, 3, 32)}, {"weight": z(16, dtype=torch.int8)}, {"weight": z(2, 16, 32, dtype=torch.int8)},
+                                {"weight": OnDevice.of(torch.tensor(1, dtype=torch.int8))}])
+def test_linear_refuses_what_is_no_matrix(kw):
+    a = dict(x=z(3, 32), weight=z(16, 32, dtype=torch.int8), weight_scale=z(16), out=z(3, 16))
+    a.update(kw)
+    with pytest.raises(KernelError):
+        int8_ops.linear(**a)
