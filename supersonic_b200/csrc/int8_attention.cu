@@ -124,8 +124,9 @@ int8_weigh_plain_kernel(const IaArgs a) {
 // (m16n8k16): codes are whole numbers up to 127, which float16 holds exactly; probabilities are rounded to its 11 bits, or (WIDE,
 // float32 rows) go in two halves.  The scores' registers are the B operand's, so nothing moves between lanes.
 // The scales stay outside the products: a key's goes onto the score; a value's, f * 2^x, into the exponent (x) and onto the
-// probability (f), with the running maximum taken over score + x, so that float16 holds what is summed.  The sum of weights takes
-// what x took off back in float32: keys whose values' scales are within 2^90 of one another all count in it.  The maximum is rounded up to a whole number, in the log2 domain: taking x and it off a score then costs no bits.
+// probability (f), with the running maximum taken over score + x, so that float16 holds what is summed.  The sum of weights takes x
+// back in float32: all keys count in it whose values' scales are within 2^90 of one another.  The maximum is rounded up to a whole
+// number, in the log2 domain: taking x and it off a score then costs no bits.
 //
 // Value codes become float16 in registers: 1024 + (code + 128) is a float16 whose low byte is the code with its sign bit turned, so
 // two keys' four codes take two exclusive-ors, six byte permutations and four subtractions.  Which key is which column or k of
