@@ -146,13 +146,12 @@ constexpr float IR_NONE = -1e30f;               // a maximum over no key: finite
 constexpr int IR_SIDE = 12;                  // beside a stage's page: its scales of keys and of values, and its id
 constexpr int IR_LEAST_X = -80, IR_MOST_X = 120;
 constexpr float IR_NO_PAGE = -1.f;           // in the place of the scales of a page id that names no page
-__device__ const float ir_no_page = IR_NO_PAGE;
 
-// What the dealing needs: tokens a tile (1 << tts), the window, the table's width, and the batch with the units before each sequence.
+// What the dealing needs: tokens a tile (1 << tts), the window, and the batch with the units before each sequence.
 struct IrBatch {
     const IaSeq* seqs;
     const long long* cum;                // [n_seqs + 1]
-    int n_seqs, n_kv, tts, window, pages;
+    int n_seqs, n_kv, tts, window;
     bool one_tile;                       // a sequence's rows are one tile, however many
     int extra;                           // what beginning and ending a tile costs, in pages: units without a page before its first
 
@@ -172,18 +171,13 @@ struct IrBatch {
     __device__ int tiles(const IaSeq& s) const { return s.slot < 0 || s.n_new <= 0 ? 0 : one_tile ? 1 : (s.n_new + (1 << tts) - 1) >> tts; }
     // units of the first t tiles of a sequence: the pages that each sees, and the extra ones
     __device__ long long units_before(const IaSeq& s, long long t) const {
-        if (one_tile) return t * (min((s.start + s.n_new - 1) >> 6, pages - 1) - first_page(s, 0) + 1 + extra);
-        const long long hi = (long long)s.start + (1 << tts) - 1;
-        return t * (1 + extra) + (window > 0 ? floors(t, min(hi, last_place())) - floors(t, first_place(s)) : floors(t, hi));
+        if (one_tile) return t * (((s.start + s.n_new - 1) >> 6) - first_page(s, 0) + 1 + extra);
+        return t * (1 + extra) + floors(t, (long long)s.start + (1 << tts) - 1) - (window > 0 ? floors(t, (long long)s.start - window + 1) : 0);
     }
     __device__ int first_page(const IaSeq& s, int tile) const {
-        const long long lo = first_place(s) + ((long long)tile << tts);
+        const long long lo = (long long)s.start + ((long long)tile << tts) - window + 1;
         return window > 0 && lo > 0 ? (int)(lo >> 6) : 0;
     }
-    // Of a window's first row, no farther than the table's last place: so the first tile has one page at least and the table's at most
-    // wherever it starts (without a window a start is the last place at most).  What the others have of pages behind that is unseen.
-    __device__ long long last_place() const { return (long long)pages * IA_PAGE - 1; }
-    __device__ long long first_place(const IaSeq& s) const { return min((long long)s.start - window + 1, last_place()); }
 };
 
 // A run of pages of one tile and kv head: what of it lies in a block's range.
@@ -426,11 +420,11 @@ __device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFee
     const IaSeq s = B.seqs[f.seg.b];
     const int i = f.seg.n - f.left;
     if (f.ids_from < 0 || i - f.ids_from >= 32) {
-        // a tile that is not full may count a page behind the sequence's last: the last again, which no row of it sees; what lies behind
-        // the table is no page
+        // a tile that is not full may count a page behind the sequence's last: the last again, which no row of it sees; one that starts
+        // behind the table counts pages there, which are none
         const int page = f.seg.page + i + lane;
-        const int named = a.page_table[(size_t)s.slot * a.max_pages + min(min(page, (s.start + s.n_new - 1) >> 6), B.pages - 1)];
-        f.ids = page < B.pages && ia_in_pool(a, named) ? named : -1;
+        const int named = a.page_table[(size_t)s.slot * a.max_pages + min(min(page, (s.start + s.n_new - 1) >> 6), a.max_pages - 1)];
+        f.ids = page < a.max_pages && ia_in_pool(a, named) ? named : -1;
         f.ids_from = i;
     }
     const int named = __shfl_sync(0xffffffffu, f.ids, i - f.ids_from), id = max(named, 0);      // of no page: any, unseen
@@ -440,13 +434,16 @@ __device__ __forceinline__ bool ir_feed(const IaArgs& a, const IrBatch& B, IrFee
     ok = __shfl_sync(0xffffffffu, ok, 0);
     if (!ok) return false;
     const size_t head = (size_t)id * a.n_kv + f.seg.kvh;
-    if (lane < 2 * per) {
-        const float* src = named >= 0 ? (lane < per ? a.k_scale : a.v_scale) + head * per + (lane & (per - 1)) : &ir_no_page;
+    if (named < 0) {
+        if (lane < 2 * per) scales[IR_SIDE * st + lane] = IR_NO_PAGE;
+        __syncwarp();                                              // before lane 0's arrival at the barrier, below
+    } else if (lane < 2 * per) {
+        const float* src = (lane < per ? a.k_scale : a.v_scale) + head * per + (lane & (per - 1));
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(scales + IR_SIDE * st + lane)), "l"(src) : "memory");
     }
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full0 + 8 * st) : "memory");
     if (lane == 0) {
-        if (!VALUES) scales[IR_SIDE * st + 8] = __int_as_float(named);       // before this lane's arrival at the barrier, below
+        if (!VALUES) scales[IR_SIDE * st + 8] = __int_as_float(named);
         const uint32_t dst = smem_u32(stages + st * ir_stage_bytes<HD, VALUES>());
         mbar_expect_tx(full0 + 8 * st, ir_stage_bytes<HD, VALUES>());
         tma_load_2d(dst, &map_k, full0 + 8 * st, 0, (int)(head * 64));
@@ -523,7 +520,7 @@ int8_rows_kernel(const IaArgs a, int s0, int n_seqs, int tts, float* __restrict_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, a.max_pages, false, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
     // dependents may start once all that came before this launch is done: they read the batch and the pages ahead of their own wait
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
@@ -739,7 +736,7 @@ int8_finish_kernel(const IaArgs a, int s0, int n_seqs, int tts, const float* __r
     IaSeq* seqs = (IaSeq*)(cum + n_seqs + 1);
     __shared__ long long warp_total[IR_WARPS];
     __shared__ float others[2][6][32];
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, a.max_pages, false, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, tts, a.window, false, IR_EXTRA};
     ssb_pdl_launch_dependents();
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     const int blocks = ir_dealt(total), c = blockIdx.x, half = threadIdx.x / HALF, thread = threadIdx.x % HALF, lane = threadIdx.x & 31;
@@ -809,7 +806,7 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
     long long* cum = (long long*)smem_raw;
     IaSeq* seqs = (IaSeq*)(cum + n_seqs + 1);
     __shared__ long long warp_total[IR_WARPS];
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, a.max_pages, false, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, false, IR_EXTRA};
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total);
     const int blocks = ir_dealt(total), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.n_q / a.n_kv;
     const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
@@ -833,7 +830,7 @@ int8_account_kernel(const IaArgs a, int s0, int n_seqs, const float* __restrict_
             for (int p = warp; p < seg.n; p += IR_WARPS) {
                 const float* src = kept + (seg.at + p) * (IR_WARPS * 16) * group;
                 const int id = a.page_table[(size_t)s.slot * a.max_pages + min(seg.page + p, a.max_pages - 1)];
-                const bool there = ia_in_pool(a, id);
+                const bool there = seg.page + p < a.max_pages && ia_in_pool(a, id);
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -892,7 +889,7 @@ int8_weigh_kernel(const IaArgs a, int s0, int n_seqs, int column0, int* __restri
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, a.max_pages, true, IR_EXTRA};
+    IrBatch B{nullptr, nullptr, 0, a.n_kv, 0, a.window, true, IR_EXTRA};
     const long long total = ir_read_batch(a, s0, n_seqs, B, seqs, cum, warp_total, a.weigh_last);
     const int blocks = ir_dealt(total);
     const long long begin = ir_begin(total, blockIdx.x, blocks), end = ir_begin(total, blockIdx.x + 1, blocks);
@@ -1023,7 +1020,8 @@ template <int HD, int NT, bool WIDE> static int ir_blocks(int n_seqs) {
 
 static bool ir_takes(int n_q, int n_kv, int head_dim) { return (head_dim == 64 || head_dim == 128) && n_q / n_kv <= 32; }
 
-static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim, int weigh_last) {
+static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim, int window,
+                      int weigh_last) {
     IrPlan p{};
     const int group = n_q / n_kv;
     const long long most = (long long)max_new * group;
@@ -1038,7 +1036,8 @@ static IrPlan ir_plan(bool wide, int n_seqs, int rows, int max_new, int max_page
     // single tokens that keep account: their scores are kept, a sixteenth to an eighth of what the pages hold, where that has a
     // bound (of the longest sequence there can be) that a scratch may have; else the keys are read once more.  16 sequences of 8,192,
     // 32 heads of 64 in float32: 59 us so, 73 with the keys read again.
-    const long long kept = (long long)n * n_kv * (max_pages + IR_EXTRA) * 64 * group;
+    const long long spans = window > 0 ? (window + 62LL) / IA_PAGE + 1 : max_pages;      // pages a token sees at most
+    const long long kept = (long long)n * n_kv * (spans + IR_EXTRA) * 64 * group;
     p.kept = weigh_last > 0 && max_new == 1 && p.nt == 1 && kept <= IR_KEPT_MOST ? kept : 0;
     return p;
 }
@@ -1047,10 +1046,10 @@ static long long ir_scratch(const IrPlan& p) { return 2LL * p.blocks * (long lon
 
 // float32 elements of scratch that the launch needs.
 SSB_API long long ssb_int8_attention_scratch(int dtype, int n_seqs, int rows, int max_new, int max_pages, int n_q, int n_kv, int head_dim,
-                                             int weigh_last, float scale) {
+                                             int window, int weigh_last, float scale) {
     if (n_seqs <= 0 || rows <= 0 || n_kv <= 0 || !ir_takes(n_q, n_kv, head_dim)) return 0;
     if (ia_tc_takes(dtype, head_dim, max_new, scale)) return ia_tc_scratch(n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim);
-    const IrPlan p = ir_plan(dtype == SSB_F32, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, weigh_last);
+    const IrPlan p = ir_plan(dtype == SSB_F32, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, window, weigh_last);
     return p.blocks < 0 ? 0 : ir_scratch(p);
 }
 
@@ -1147,7 +1146,7 @@ SSB_API int ssb_int8_attention(const void* q, int ldq, int dtype, void* out, int
     rc = ir_map(&mv, v, (long long)n_pages * n_kv * 64, head_dim);
     if (rc) return rc;
     if (!scratch) return SSB_ERR_BAD_SIZE;
-    const IrPlan p = ir_plan(wide, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, weigh_last);
+    const IrPlan p = ir_plan(wide, n_seqs, rows, max_new, max_pages, n_q, n_kv, head_dim, window, weigh_last);
     if (p.blocks < 0) return SSB_ERR_UNSUPPORTED;
     if (scratch_size < ir_scratch(p)) return SSB_ERR_BAD_SIZE;
 #define IR_ROWS(H_, N_, W_) rc = ir_rows<H_, N_, W_>(a, p, scratch, error_word, mk, mv, stream)

@@ -26,7 +26,7 @@ struct IaArgs {
 // A sequence of the step's batch as every kernel here takes it: the rows it has of those there are, its slot (negative: it has none, its
 // rows are zeros) and the tokens before it.  A key lies in the table's 64 max_pages places, under a page id of the pool; one behind the
 // table's end or under any other id is seen by nobody.  A start that lies farther behind the end than rows can tell is taken back to
-// where they cannot (most_start), so that positions hold in 32 bits and a single token spans the table's pages at most.
+// where they cannot (most_start): positions hold in 32 bits, and a single token spans the table's pages or its window's at most.
 struct IaSeq { int row0, n_new, start, slot; };
 __device__ __forceinline__ IaSeq ia_sequence(const IaArgs& a, int b) {
     const int row0 = a.cu_new[b], slot = a.seq_slot[b], start = a.seq_start[b];

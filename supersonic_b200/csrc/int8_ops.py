@@ -29,7 +29,7 @@ _SIGNATURES = {
     "ssb_int8_evict": ("int8_cache", [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
     "ssb_int8_attention": ("int8_attention", [_P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I,
                                               _I, _I, _I, _I, _F, _P, _L, _P, _P]),
-    "ssb_int8_attention_scratch": ("int8_attention", [_I] * 9 + [_F]),
+    "ssb_int8_attention_scratch": ("int8_attention", [_I] * 10 + [_F]),
     "ssb_int8_quantize_rows": ("int8_linear", [_P, _I, _I, _P, _I, _P, _I, _I, _P]),
     "ssb_int8_linear": ("int8_linear", [_P, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
     "ssb_int8_linear_scratch": ("int8_linear", [_I, _I, _I]),
@@ -243,7 +243,7 @@ def attention(q: torch.Tensor, pages: Int8Pages, page_table: torch.Tensor, cu_ne
     if max_new <= 0 or (window or 0) < 0:
         raise KernelError(f"attention: max_new {max_new} new tokens, window {window}")
     code, device = _CODES[q.dtype], q.device
-    size = _scratch_size("ssb_int8_attention_scratch", code, B, rows, max_new, width, n_q, n_kv, dim, weigh_last, scale)
+    size = _scratch_size("ssb_int8_attention_scratch", code, B, rows, max_new, width, n_q, n_kv, dim, window or 0, weigh_last, scale)
     scratch = torch.empty(size, dtype=_FLOAT32, device=device)
     _check(_fn("ssb_int8_attention")(
         q_at, ldq, code, o_at, ldo, 0 if lse is None else lse.data_ptr(), *at, table, slots, width, n_pages,

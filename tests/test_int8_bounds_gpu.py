@@ -231,7 +231,7 @@ def test_the_scratch_of_a_batch_does_not_depend_on_who_asks_beside_it():
     from supersonic_b200.csrc import int8_ops
     ask = int8_ops._fn("ssb_int8_attention_scratch")
     sizes = [8, 200, 1000, 60, 700, 1]
-    args = lambda n: (1, n, n, 1, 64, 32, 8, 128, 0, 0.125)                                  # noqa: E731
+    args = lambda n: (1, n, n, 1, 64, 32, 8, 128, 0, 0, 0.125)                               # noqa: E731
     want, wrong = {n: ask(*args(n)) for n in sizes}, []
     assert len(set(want.values())) > 1
 
