@@ -39,9 +39,12 @@ class _Layer:
 
 
 class Int8Session:
-    """``max_tokens``: tokens that the cache holds in all (in whole pages; cutting a sequence takes its budget's pages beside its own); ``budget``: tokens a sequence may keep (None: all), of which
-    the first ``first`` and the latest ``recent`` stay in any case; ``slack``: tokens it may grow beyond that before it is cut down to it
-    again; ``observe``: how many of a step's last rows account for what they attend to."""
+    """``max_tokens``: tokens that the cache holds in all, in whole pages (a sequence that is cut takes its budget's pages beside its own
+    for as long as that lasts); ``budget``: tokens a sequence may keep (None: all), of which the first ``first`` and the latest
+    ``recent`` stay in any case; ``slack``: tokens it may grow beyond that before it is cut down to it again; ``observe``: how many of a
+    step's last rows account for what they attend to.
+
+    The 8-bit weights are made from the model's and lie beside them, as the cache lies beside the model's own (:meth:`bytes_held`)."""
 
     def __init__(self, model: Model, max_tokens: int, max_sequences: int = 64, budget: Optional[int] = None, first: int = 4,
                  recent: Optional[int] = None, slack: int = PAGE_TOKENS, block: int = 16, observe: int = 32):
@@ -125,7 +128,7 @@ class Int8Session:
             if not all(whole):
                 limit = max(1, min(limit, min(width, self.n_pages - per) * PAGE_TOKENS - cut_at + 1))
         chunks = []
-        for pieces in plan_chunks(counts, limit):
+        for pieces in [[(i, 0, n) for i, n in enumerate(counts)]] if sum(counts) <= limit else plan_chunks(counts, limit):
             cut = []
             for i, first, end in pieces:
                 slot = slots[i]
@@ -277,7 +280,8 @@ class Int8Session:
 
     # ---- greedy generation ---------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 8, stop_token_ids: Sequence[int] = ()) -> List[List[int]]:
-        """Greedy tokens for each prompt, all prompts in one batch."""
+        """Greedy tokens for each prompt, all prompts in one batch; a sequence ends at one of ``stop_token_ids`` (the model's own are in
+        its ``spec.stop_token_ids``)."""
         slots: List[int] = []
         out: List[List[int]] = [[] for _ in prompts]
         try:

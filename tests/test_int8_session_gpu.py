@@ -130,3 +130,50 @@ def test_refusals():
     cfg, store, _ = tiny_ronelorn.build("A")
     with pytest.raises(ValueError):
         Int8Session(Model.from_config(cfg, store, dtype="bfloat16", device="cuda:0", max_tokens=256, max_seq_tokens=128), 256)
+
+
+def test_a_refused_step_leaves_the_other_sequences_and_the_session_as_they_were():
+    from supersonic_b200.cache import CacheFull
+    from supersonic_b200.engine import StepEntry
+    from supersonic_b200.engine.int8_session import Int8Session
+    model = _model("D", "float32")
+    rng = np.random.default_rng(8)
+    first, second = (rng.integers(0, model.vocab_size, n).tolist() for n in (60, 70))
+    logits = []
+    for refused in (False, True):
+        session = Int8Session(model, 64 * 5)
+        a, b, c = (session.open() for _ in range(3))
+        rows = [session.step([StepEntry(a, first, [59])])]
+        if refused:
+            with pytest.raises(CacheFull):
+                session.step([StepEntry(b, second, [69]), StepEntry(c, second * 3, [0])])
+            session.close(c)
+            with pytest.raises(ValueError):
+                session.step([StepEntry(b, second, [69]), StepEntry(c, [1], [0])])
+        rows.append(session.step([StepEntry(b, second, [69])]))
+        rows += [session.step([StepEntry(a, [5], [0]), StepEntry(b, [6], [0])]) for _ in range(3)]
+        logits.append(torch.cat(rows))
+    assert torch.equal(*logits)
+
+
+@pytest.mark.parametrize("step_tokens,most", [(100, 100), (4096, 64 * 8 - 64 * 2 - 129 + 1)])
+def test_a_prompt_beyond_the_table_is_cut_on_its_way(monkeypatch, step_tokens, most):
+    """A prompt longer than a budget's table, in steps of the model's tokens, or than leaves room for its cut, in steps that do; the same twice."""
+    from supersonic_b200.engine import StepEntry
+    from supersonic_b200.engine.int8_session import Int8Session
+    model = _model("D", "float32")
+    monkeypatch.setattr(model, "step_token_budget", step_tokens)
+    monkeypatch.setattr(model, "position_limit", None)
+    tokens, logits = np.random.default_rng(9).integers(0, model.vocab_size, 500).tolist(), []
+    for _ in range(2):
+        session, sizes = Int8Session(model, 64 * 8, budget=96, first=4, recent=16, slack=33), []
+        run = session._run
+        monkeypatch.setattr(session, "_run", lambda packed, cuts: (sizes.append(packed.n_tokens), run(packed, cuts))[1])
+        slot = session.open()
+        rows = [session.step([StepEntry(slot, tokens, [499, 3, 250])])]
+        rows += [session.step([StepEntry(slot, [t], [0])]) for t in (1, 2, 3)]
+        assert session.position[slot] == 503 and session.length[slot] < 129 and max(sizes) <= most and sum(sizes) == 503
+        session.close(slot)
+        assert sorted(session.free) == list(range(8))
+        logits.append(torch.cat(rows))
+    assert torch.isfinite(logits[0]).all() and logits[0].shape[0] == 6 and torch.equal(*logits)
