@@ -9,8 +9,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 #include <algorithm>
-#include <map>
-#include <mutex>
+#include <atomic>
 #include <type_traits>
 
 typedef __nv_bfloat16 bf16;
@@ -995,17 +994,20 @@ template <typename K> static int ir_configure(K kernel, size_t smem) {
 struct IrPlan { int nt, tts, blocks; size_t piece; long long kept; };      // floats of a piece; of the scores that are kept
 
 // Blocks of a launch over n_seqs sequences, or -1.  Host threads may ask at the same time for different sizes, and what a thread is told
-// does not depend on who asked before: its scratch is sized by it.
+// does not depend on who asked before: its scratch is sized by it.  Nothing here allocates or locks, so nothing is thrown.
 template <int HD, int NT, bool WIDE> static int ir_blocks(int n_seqs) {
-    static std::mutex lock;
-    static std::map<std::pair<int, int>, int> known;               // (device, sequences)
+    constexpr int DEVICES = 8;                                     // of any others every call asks the driver
+    static std::atomic<int> known[DEVICES][IR_SEQS + 1];           // 0: not asked yet
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) { cudaGetLastError(); return -1; }
-    const std::lock_guard<std::mutex> held(lock);
-    const auto at = known.find({device, n_seqs});
-    if (at != known.end()) return at->second;
-    if (ir_configure(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(IR_SEQS)) != 0) { cudaGetLastError(); return -1; }
-    return known[{device, n_seqs}] = ir_resident(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(n_seqs));
+    std::atomic<int>* at = device < DEVICES ? &known[device][n_seqs] : nullptr;
+    int blocks = at ? at->load(std::memory_order_acquire) : 0;
+    if (blocks == 0) {
+        if (ir_configure(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(IR_SEQS)) != 0) { cudaGetLastError(); return -1; }
+        blocks = ir_resident(int8_rows_kernel<HD, NT, WIDE>, ir_smem<HD, NT>(n_seqs));
+        if (at) at->store(blocks, std::memory_order_release);
+    }
+    return blocks;
 }
 #define IR_EACH(HD_, NT_, WIDE_, WHAT_) \
     do { \
