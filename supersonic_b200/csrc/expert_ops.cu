@@ -225,6 +225,257 @@ SSB_API int ssb_route_softmax(float* z, int ld, const float* bias, int n_tokens,
 }
 
 // ---------------------------------------------------------------------------------------
+// router by scores.  s = softmax(z) or sigmoid(z) over all experts, c = s + correction; the experts form `n_groups` equal groups of
+// neighbours, a group's score is its largest c or the sum of its two largest; of the experts of the `keep` best groups the `top`
+// largest c win, in order, the lower index (expert, group) at equal scores; an expert's weight is its s times `scale`, with
+// `renormalize` divided by the sum of the chosen s (+ 1e-20).  A logit that is NaN counts as minus infinity, whose s is zero, an infinite one as the
+// largest number; a c that is NaN comes last.
+//
+// What is chosen is chosen by c in 64 bits.  c in 32 bits is within RS_NEAR of it, so a warp (a token, its experts in registers)
+// chooses in 32 bits and looks whether two neighbours of its order, the last chosen and the next among them, or a kept and a
+// dropped group, are closer than that: only then (a token in some hundreds) it computes and chooses again in 64 bits, one expert
+// after another.  Without correction c grows with z, and the order is z's own.
+// 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: see the figures at the launch.
+// ---------------------------------------------------------------------------------------
+constexpr int RS_MOST_GROUPS = 32;
+enum { RS_SOFTMAX = 0, RS_SIGMOID = 1 };
+
+struct RsArgs {
+    const float* z; int ld; const float* correction;
+    int n_tokens, n_experts, n_groups, keep, top, kind, by_two, renormalize; float scale;
+    int* expert_of; float* pair_weight;
+};
+// How far c in 32 bits may be from the exact one, twice over: s to 3e-7 (its exponential, its quotient, z - max rounded: where that
+// is large, s is small), the sum's rounding.
+__device__ __forceinline__ float rs_near(float c) { return 2e-6f + 1e-6f * fabsf(c); }
+__device__ __forceinline__ float rs_logit(float z) {
+    return z != z || z == -INFINITY ? -INFINITY : fminf(fmaxf(z, -3.4028234663852886e38f), 3.4028234663852886e38f);
+}
+// A number's bits in an order that is the numbers'; 0 is below all of them (and NaN's).
+__device__ __forceinline__ uint32_t rs_key(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return x != x ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float rs_from_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// All of it in 64 bits, for a token whose choice is close.  ``most``, ``total``: of the softmax.
+__device__ __noinline__ void rs_choose_exactly(const RsArgs& a, const float* zr, int* chosen, int lane) {
+    double most = -INFINITY, total = 0.0;
+    if (a.kind == RS_SOFTMAX) {
+        for (int e = lane; e < a.n_experts; e += 32) most = fmax(most, (double)rs_logit(zr[e]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (most > -INFINITY)
+            for (int e = lane; e < a.n_experts; e += 32) total += exp((double)rs_logit(zr[e]) - most);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    auto choice = [&](int e) -> double {
+        const double z = (double)rs_logit(zr[e]);
+        double s = 0.0;
+        if (z > -INFINITY) s = a.kind == RS_SOFTMAX ? exp(z - most) / total : 1.0 / (1.0 + exp(-z));
+        const double c = s + (a.correction ? (double)a.correction[e] : 0.0);
+        return c != c ? -INFINITY : c;
+    };
+    const int per = a.n_experts / a.n_groups;
+    uint32_t stays = 0xffffffffu;
+    if (a.keep < a.n_groups) {
+        double score = -INFINITY;                         // lane g: group g's
+        for (int g = 0; g < a.n_groups; ++g) {
+            double first = -INFINITY, second = -INFINITY;
+            for (int e = g * per + lane; e < (g + 1) * per; e += 32) {
+                const double c = choice(e);
+                if (c > first) { second = first; first = c; } else if (c > second) second = c;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const double f = __shfl_xor_sync(0xffffffffu, first, o), s = __shfl_xor_sync(0xffffffffu, second, o);
+                second = fmax(fmin(first, f), fmax(second, s));
+                first = fmax(first, f);
+            }
+            if (lane == g) score = a.by_two && per > 1 ? first + second : first;
+        }
+        int before = 0;
+        for (int g = 0; g < a.n_groups; ++g) {
+            const double o = __shfl_sync(0xffffffffu, score, g);
+            before += o > score || (o == score && g < lane);
+        }
+        stays = __ballot_sync(0xffffffffu, lane < a.n_groups && before < a.keep);
+    }
+    double last = INFINITY;
+    int last_e = -1;
+    for (int k = 0; k < a.top; ++k) {                     // the largest behind the last one chosen
+        double best = -INFINITY;
+        int best_e = 0x7fffffff;
+        for (int e = lane; e < a.n_experts; e += 32) {
+            if (!(stays >> (e / per) & 1)) continue;
+            const double c = choice(e);
+            if ((c < last || (c == last && e > last_e)) && (best_e == 0x7fffffff || c > best)) { best = c; best_e = e; }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const double c = __shfl_xor_sync(0xffffffffu, best, o);
+            const int e = __shfl_xor_sync(0xffffffffu, best_e, o);
+            if (e != 0x7fffffff && (best_e == 0x7fffffff || c > best || (c == best && e < best_e))) { best = c; best_e = e; }
+        }
+        last = best;
+        last_e = best_e;
+        if (lane == 0) chosen[k] = best_e;
+    }
+    __syncwarp();
+}
+
+// PER: experts a lane (expert j * 32 + lane).
+template <int PER>
+__global__ void __launch_bounds__(RG_THREADS)
+route_scored_kernel(const RsArgs a) {
+    extern __shared__ float rsc_smem[];                  // per warp: [top] chosen experts, [n_experts + 4 * n_groups] scores of groups' members
+    ssb_pdl_launch_dependents();
+    ssb_pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = blockIdx.x * (RG_THREADS / 32) + warp;
+    if (t >= a.n_tokens) return;
+    const bool grouped = a.keep < a.n_groups;
+    const int words = a.top + (grouped ? a.n_experts + 4 * a.n_groups : 0);
+    int* chosen = (int*)rsc_smem + (size_t)warp * words;
+    float* member = (float*)(chosen + a.top);
+    const float* zr = a.z + (size_t)t * a.ld;
+    float z[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = j * 32 + lane;
+        z[j] = e < a.n_experts ? rs_logit(zr[e]) : -INFINITY;
+    }
+    float most = 0.f, inv = 1.f;
+    if (a.kind == RS_SOFTMAX) {
+        most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) most = fmaxf(most, z[j]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float total = 0.f;
+        if (most > -INFINITY)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) total += expf(z[j] - most);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        inv = 1.f / total;
+    }
+    auto score = [&](float x) { return x == -INFINITY ? 0.f : a.kind == RS_SOFTMAX ? expf(x - most) * inv : 1.f / (1.f + expf(-x)); };
+    uint32_t key[PER];                                   // of c, or without correction of z; 0: no expert, dropped or taken
+    bool near = false;
+    const int per = a.n_experts / a.n_groups;
+    if (a.correction) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = j * 32 + lane;
+            const float c = e < a.n_experts ? score(z[j]) + a.correction[e] : 0.f;
+            key[j] = e < a.n_experts ? rs_key(c) : 0u;
+            if (grouped && e < a.n_experts) member[e + 4 * (e / per)] = c != c ? -INFINITY : c;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = j * 32 + lane;
+            key[j] = e < a.n_experts ? rs_key(z[j]) : 0u;
+            if (grouped && e < a.n_experts) member[e + 4 * (e / per)] = a.by_two && per > 1 ? score(z[j]) : z[j];
+        }
+    }
+    if (grouped) {
+        __syncwarp();
+        // as many lanes a group as there are for each; groups lie 4 words apart, so that those lanes meet no bank twice
+        const int share = a.n_groups <= 1 ? 32 : 1 << (__clz(a.n_groups - 1) - 27);          // 32 / groups, a power of two
+        const int g = lane / share;
+        float first = -INFINITY, second = -INFINITY;
+        if (g < a.n_groups)
+            for (int i = lane % share; i < per; i += share) {
+                const float c = member[g * (per + 4) + i];
+                if (c > first) { second = first; first = c; } else if (c > second) second = c;
+            }
+        for (int o = share / 2; o > 0; o >>= 1) {
+            const float f = __shfl_xor_sync(0xffffffffu, first, o), s = __shfl_xor_sync(0xffffffffu, second, o);
+            second = fmaxf(fminf(first, f), fmaxf(second, s));
+            first = fmaxf(first, f);
+        }
+        const float mine = a.by_two && per > 1 ? first + second : first;
+        int before = 0;
+        for (int o = 0; o < a.n_groups; ++o) {
+            const float other = __shfl_sync(0xffffffffu, mine, o * share);
+            before += other > mine || (other == mine && o < g);
+        }
+        const bool live = g < a.n_groups, kept = live && before < a.keep;
+        const float worst_kept = rs_from_key(__reduce_min_sync(0xffffffffu, kept ? rs_key(mine) : 0xffffffffu));
+        const float best_dropped = rs_from_key(__reduce_max_sync(0xffffffffu, live && !kept ? rs_key(mine) : 0u));
+        // by the largest z alone nothing is rounded
+        if (a.correction || (a.by_two && per > 1)) near = !(worst_kept - best_dropped > 2.f * rs_near(worst_kept));
+        const uint32_t stays = __ballot_sync(0xffffffffu, kept);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (!(stays >> (((j * 32 + lane) / per) * share & 31) & 1)) key[j] = 0u;
+    }
+    float before = INFINITY;
+    for (int k = 0; k <= a.top; ++k) {                   // one more than is chosen, to see how close it was
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) mine = max(mine, key[j]);
+        const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
+        if (a.correction && best) {
+            const float c = rs_from_key(best);
+            near = near || !(before - c > rs_near(c));
+            before = c;
+        }
+        if (k == a.top) break;
+        int at = 0x7fffffff;                             // the lowest expert that has it
+#pragma unroll
+        for (int j = PER - 1; j >= 0; --j)
+            if (key[j] == best) at = j * 32 + lane;
+        at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (j * 32 + lane == at) key[j] = 0u;
+        if (lane == 0) chosen[k] = at;
+    }
+    __syncwarp();
+    if (near) rs_choose_exactly(a, zr, chosen, lane);
+    float sum = 0.f;
+    for (int k = lane; k < a.top; k += 32) sum += score(rs_logit(zr[chosen[k]]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float f = a.renormalize ? a.scale / (sum + 1e-20f) : a.scale;
+    for (int k = lane; k < a.top; k += 32) {
+        const int e = chosen[k];
+        a.expert_of[(size_t)t * a.top + k] = e;
+        a.pair_weight[(size_t)t * a.top + k] = score(rs_logit(zr[e])) * f;
+    }
+}
+
+template <int PER>
+static int rs_launch(const RsArgs& a, int pdl, cudaStream_t stream) {
+    const size_t smem = (size_t)(RG_THREADS / 32) * (a.top + (a.keep < a.n_groups ? a.n_experts + 4 * a.n_groups : 0)) * sizeof(float);
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(route_scored_kernel<PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (int)e;
+    }
+    const int rc = ssb_launch(route_scored_kernel<PER>, dim3((a.n_tokens + RG_THREADS / 32 - 1) / (RG_THREADS / 32)), dim3(RG_THREADS), smem,
+                              stream, pdl != 0, a);
+    return rc ? rc : ssb_launch_status();
+}
+
+SSB_API int ssb_route_scored(const float* z, int ld, const float* correction, int n_tokens, int n_experts, int n_groups, int keep, int top,
+                             int kind, int by_two, int renormalize, float scale, int* expert_of, float* pair_weight, int pdl,
+                             cudaStream_t stream) {
+    if (n_tokens <= 0) return 0;
+    if (n_experts <= 0 || n_experts > 2048 || n_groups <= 0 || n_groups > RS_MOST_GROUPS || n_experts % n_groups || keep < 1 || keep > n_groups ||
+        top < 1 || top > keep * (n_experts / n_groups) || ld < n_experts || kind < RS_SOFTMAX || kind > RS_SIGMOID)
+        return SSB_ERR_BAD_SIZE;
+    const RsArgs a{z, ld, correction, n_tokens, n_experts, n_groups, keep, top, kind, by_two, renormalize, scale, expert_of, pair_weight};
+    if (n_experts <= 64) return rs_launch<2>(a, pdl, stream);
+    if (n_experts <= 256) return rs_launch<8>(a, pdl, stream);
+    if (n_experts <= 512) return rs_launch<16>(a, pdl, stream);
+    return rs_launch<64>(a, pdl, stream);
+}
+
+// ---------------------------------------------------------------------------------------
 // pairs sorted by expert.  One block: counts in shared memory, offsets and the tile list by one
 // thread, then every pair takes the next free row of its expert.  The order inside a group is
 // whatever the adds give; nothing downstream depends on it.

@@ -1,0 +1,1012 @@
+// Products of matrices in microscaled 4-bit floats (the format: fp4_codes.cuh): out[m, n] (+)= sum_k x[m, k] w[n, k], on the
+// fifth-generation tensor cores (tcgen05 kind::mxf4 with a scale for every 32 numbers).  Codes and scales arrive by TMA, codes with the
+// 128-byte swizzle (a k-block of 256 numbers is one swizzle row), scales as they lie; scales go on to tensor memory (tcgen05.cp, each
+// 128 rows x 4 blocks to four columns, in all four lane quarters), where the instructions read them.  Products of codes and their scales
+// are exact; sums are float32 in tensor memory.
+//
+// Two kernels:
+//  * where the weights' bytes or the number of tiles is what bounds it: weights on the M side (128 of them a tile), rows of x on the
+//    N side, and the k-blocks of all tiles dealt out over the SMs, in equal parts of tiles or wherever a tile ends; the same for experts,
+//    whose tiles of rows a list in memory names;
+//  * many rows: tiles of 256 x 256 on pairs of SMs (cta_group::2).
+//
+// What becomes of the sums: stored, added in float32, or (an inner row of a feed-forward) through an activation or a gated unit's inner
+// step and into 4 bits at once, from the float32 sums.
+#include "fp4_codes.cuh"
+#include "packed_call.cuh"
+#include "tc_helpers.cuh"
+#include "tc_rows.cuh"
+#include <algorithm>
+
+typedef __nv_bfloat16 bf16;
+
+constexpr int FL_BM = 128;
+constexpr int FL_THREADS = 192;           // warp 0: TMA, warp 1: MMA + tensor memory, warps 2-5: epilogue
+constexpr int FL_ROW = 128;               // bytes of codes a row and k-block
+constexpr uint32_t FL_CHUNK = F4_CHUNK;
+enum { FL_STORE = 0, FL_GATED = 1, FL_ACT = 2 };
+
+// D float32; A and B E2M1, both K-major; scales powers of two.  ``part``: which half of a scale word (blocks 0 1 or 2 3) A and B use.
+__host__ __device__ constexpr uint32_t fl_idesc(int m, int n, int part) {
+    return ((uint32_t)(2 * part) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
+           ((uint32_t)(2 * part) << 29);
+}
+// 32 lanes x 16 bytes of shared memory that lie together (8-row groups 128 bytes apart), no swizzle.
+__device__ __forceinline__ uint64_t fl_scale_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (8ull << 16) | (8ull << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void fl_copy_scales(uint32_t tmem, uint32_t addr) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(fl_scale_desc(addr)) : "memory");
+}
+__device__ __forceinline__ void fl_copy_scales_pair(uint32_t tmem, uint32_t addr) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(fl_scale_desc(addr)) : "memory");
+}
+// A k-block: four instructions of 64 numbers (32 bytes along the swizzled row: 2 descriptor units); the first two use the scales at
+// sa0 and sb0, the last two those at sa1 and sb1, each pair their first and their second halves (idesc0, idesc1).
+#define FL_MMA_X4(group_)                                                                                                                 \
+    asm volatile("{\n.reg .pred p, q;\n.reg .b64 a1, a2, a3, b1, b2, b3;\n"                                                               \
+                 "setp.ne.b32 p, %9, 0;\nsetp.eq.b32 q, 0, 0;\n"                                                                          \
+                 "add.u64 a1, %1, 2;\nadd.u64 a2, %1, 4;\nadd.u64 a3, %1, 6;\n"                                                           \
+                 "add.u64 b1, %2, 2;\nadd.u64 b2, %2, 4;\nadd.u64 b3, %2, 6;\n"                                                           \
+                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"              \
+                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %4, [%5], [%6], q;\n"              \
+                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %3, [%7], [%8], q;\n"              \
+                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %4, [%7], [%8], q;\n}"             \
+                 ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc0), "r"(idesc1), "r"(sa0), "r"(sb0), "r"(sa1), "r"(sb1),               \
+                 "r"(accumulate) : "memory")
+__device__ __forceinline__ void fl_mma_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc0, uint32_t idesc1, uint32_t sa0,
+                                          uint32_t sb0, uint32_t sa1, uint32_t sb1, uint32_t accumulate) {
+    FL_MMA_X4("1");
+}
+__device__ __forceinline__ void fl_mma_pair_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc0, uint32_t idesc1,
+                                               uint32_t sa0, uint32_t sb0, uint32_t sa1, uint32_t sb1, uint32_t accumulate) {
+    FL_MMA_X4("2");
+}
+__device__ __forceinline__ void fl_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fl_ld16(uint32_t taddr, float (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\ntcgen05.wait::ld.sync.aligned;"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+                   "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+                 : "r"(taddr) : "memory");
+}
+// Whether any thread of the four epilogue warps says so; all of them meet here (barrier 1).
+__device__ __forceinline__ bool fl_any_of_four(bool mine) {
+    uint32_t any;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, 1, 128, p;\nselp.b32 %0, 1, 0, q;\n}"
+                 : "=r"(any) : "r"((uint32_t)mine) : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void fl_meet_four() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+struct FlOut {
+    void* out;                     // FL_STORE: rows of ldo elements; else codes, rows of ldo bytes
+    uint8_t* scales;               // FL_GATED, FL_ACT: of the codes
+    const int* index;              // where a row goes (experts: the pair of a sorted row), or null
+    const float* row_scale;        // FL_GATED: a factor for each row's results, or null
+    int ldo, is_f32, add, M, N;    // rows of x, rows of a weight matrix
+    int kind;                      // FL_GATED: ssb_gate's kind; FL_ACT: ssb_activate's
+    float limit;                   // of ssb_gate, or the factor behind ssb_activate
+    int inner_blocks;              // FL_GATED, FL_ACT: k-blocks of the codes that are written
+};
+// The experts' tiles of rows: tile t holds up to BN rows of expert tile_expert[t], sorted rows tile_row0[t] onwards, which lie at rows
+// t * BN onwards of x (and of codes that are written); meta[0] tiles.  Null: rows as they are.
+struct FlTiles {
+    const int* offsets; const int* tile_expert; const int* tile_row0; const int* meta;
+};
+
+// The launch's work is tiles x k-blocks, dealt out evenly: block c takes units U c / G .. U (c + 1) / G - 1, tiles in order, a tile's
+// k-blocks in order, so that every SM streams the same bytes whatever the sizes.  A tile that lies in one block's range is finished
+// there; of any other the blocks write their sums to memory (at most two such pieces a block) and the one whose piece arrives last adds
+// them up, in the order of k.
+struct FlRange {
+    long long units, begin, end;
+    int k_blocks, blocks;
+    // no more blocks than units: each of them then has some, as whoever adds up a tile's pieces expects
+    __device__ FlRange(long long units_, int k_blocks_, int c, int blocks_) : units(units_), k_blocks(k_blocks_), blocks(blocks_) {
+        begin = c < blocks ? units * c / blocks : units;
+        end = c < blocks ? units * (c + 1) / blocks : units;
+    }
+    __device__ int owner(long long unit) const { return (int)(((unit + 1) * blocks - 1) / units); }       // the block that takes it
+};
+
+constexpr int fl_power(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
+template <int BN, int STAGES> constexpr int fl_columns() { return fl_power(2 * BN + 16 * STAGES); }
+constexpr int FL_INNER_ROWS = 16;         // rows of an inner tile that meet in shared memory at a time
+constexpr int FL_INNER_LD = 132;
+template <int BN, int STAGES> constexpr size_t fl_smem() {
+    return (size_t)STAGES * ((FL_BM + BN) * FL_ROW + 2 * FL_CHUNK) + FL_INNER_ROWS * FL_INNER_LD * 4 + (2 * STAGES + 4) * 8 + 32 + 1024;
+}
+
+// 16 numbers of a block of 32 whose other half the neighbouring lane has: codes to ``dst`` (8 bytes), the block's scale by the even lane.
+__device__ __forceinline__ void fl_put_inner(float (&v)[16], uint8_t* dst, uint8_t* scale, bool live) {
+    uint32_t most = f4_most(v);
+    if (__any_sync(0xffffffffu, most >= F4_WILD)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = f4_finite(v[i]);
+        most = f4_most(v);
+    }
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    const int byte = f4_scale_byte(most);
+    const float inverse = f4_inverse(byte);
+    const uint2 w = make_uint2(f4_encode8(v, inverse), f4_encode8(v + 8, inverse));
+    if (live) {
+        *reinterpret_cast<uint2*>(dst) = w;
+        if ((threadIdx.x & 1) == 0) *scale = (uint8_t)byte;
+    }
+}
+
+template <int BN, int STAGES, int MODE, bool LIST>
+__global__ void __launch_bounds__(FL_THREADS, 1)
+fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_ws,
+                  const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xs, const FlOut o, const FlTiles list,
+                  int m_tiles, int n_tiles, int k_blocks, int* __restrict__ arrived, float* __restrict__ pieces, int* __restrict__ error_word) {
+    constexpr uint32_t W_BYTES = FL_BM * FL_ROW, X_BYTES = BN * FL_ROW, STAGE_BYTES = W_BYTES + X_BYTES + 2 * FL_CHUNK;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* inner = (float*)(smem + STAGES * STAGE_BYTES);           // [FL_INNER_ROWS][FL_INNER_LD]
+    uint64_t* bars = (uint64_t*)(inner + FL_INNER_ROWS * FL_INNER_LD);      // full[STAGES], empty[STAGES], acc_full[2], acc_empty[2]
+    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 4);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);     // [0]: a role gave up; [1]: stays zero
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+    const uint32_t acc_full0 = smem_u32(bars + 2 * STAGES), acc_empty0 = smem_u32(bars + 2 * STAGES + 2);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(acc_full0 + 8 * i, 1); mbar_init(acc_empty0 + 8 * i, 4); }
+        abort_flag[0] = 0;
+        abort_flag[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(fl_columns<BN, STAGES>()) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    if (LIST) { ssb_pdl_wait(); ssb_pdl_launch_dependents(); }      // the list is there
+    // a tile's place: dense, tiles of rows go fastest; of a list, tiles of channels
+    const int listed = LIST ? list.meta[0] : m_tiles;
+    const long long units = (long long)listed * n_tiles * k_blocks;
+    const FlRange range(units, k_blocks, blockIdx.x, LIST ? (int)min((long long)gridDim.x, (units + 3) / 4) : (int)gridDim.x);
+    auto place = [&](int tile, int& m, int& n) {
+        if (LIST) { m = tile / n_tiles; n = tile - m * n_tiles; }
+        else { n = tile / m_tiles; m = tile - n * m_tiles; }
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const int all = (int)(range.end - range.begin), ahead = LIST ? 0 : min(STAGES, all);
+            const int tile0 = (int)(range.begin / k_blocks);
+            const int kb_first = (int)(range.begin - (long long)tile0 * k_blocks);
+            int tile = tile0, kb = kb_first, m, n, e = 0;
+            auto begin = [&]() {
+                place(tile, m, n);
+                if (LIST) e = list.tile_expert[m];
+            };
+            auto next = [&]() {
+                if (++kb == k_blocks) { kb = 0; ++tile; if ((long long)tile * k_blocks < range.end) begin(); }
+            };
+            auto weights = [&](int s) {
+                const uint32_t dst = smem_u32(smem + s * STAGE_BYTES);
+                mbar_expect_tx(full0 + 8 * s, STAGE_BYTES);
+                tma_load_2d(dst, &map_w, full0 + 8 * s, kb * FL_ROW, e * o.N + n * FL_BM);
+                tma_load_2d(dst + W_BYTES + X_BYTES, &map_ws, full0 + 8 * s, 0, (e * n_tiles + n) * k_blocks + kb);
+            };
+            if (all > 0) begin();
+            // the first stages' weights are nobody's output: they come while the rows are still being quantised
+            for (int s = 0; s < ahead; ++s, next()) weights(s);
+            if (!LIST) { ssb_pdl_wait(); ssb_pdl_launch_dependents(); }
+            tile = tile0; kb = kb_first;
+            if (all > 0) begin();
+            int c = 0, s = 0;
+            uint32_t lap = 1;
+            for (; c < all; ++c, next()) {
+                if (c >= ahead) {
+                    if (!mbar_wait(empty0 + 8 * s, lap, abort_flag)) {
+                        *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_PRODUCER); break;
+                    }
+                    weights(s);
+                }
+                const uint32_t x_dst = smem_u32(smem + s * STAGE_BYTES) + W_BYTES;
+                tma_load_2d(x_dst, &map_x, full0 + 8 * s, kb * FL_ROW, m * BN);
+                tma_load_2d(x_dst + X_BYTES + FL_CHUNK, &map_xs, full0 + 8 * s, 0, (LIST ? m : m * BN >> 7) * k_blocks + kb);
+                if (++s == STAGES) { s = 0; lap ^= 1; }
+            }
+            if (*abort_flag)                                       // let copies that were issued land before the block ends
+                for (int i = max(0, c - STAGES); i < c; ++i)
+                    mbar_wait(full0 + 8 * (i % STAGES), (i / STAGES) & 1, abort_flag + 1);
+        }
+    } else if (warp == 1) {
+        if (!LIST) ssb_pdl_wait();                                 // what follows spins on barriers
+        if (lane == 0) {
+            constexpr uint32_t idesc0 = fl_idesc(FL_BM, BN, 0), idesc1 = fl_idesc(FL_BM, BN, 1);
+            bool ok = true;
+            int i = 0, s = 0;
+            uint32_t lap = 0;
+            for (long long u = range.begin; u < range.end && ok; ++i) {
+                const int tile = (int)(u / k_blocks), kb0 = (int)(u - (long long)tile * k_blocks);
+                const int n = (int)min((long long)(k_blocks - kb0), range.end - u), buf = i & 1;
+                int m, unused;
+                place(tile, m, unused);
+                const int rows_at = LIST || BN == 128 ? 0 : (m * BN & 127) / 32;      // 32 rows' scales a column
+                if (!mbar_wait(acc_empty0 + 8 * buf, ((i >> 1) & 1) ^ 1, abort_flag)) {
+                    *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
+                }
+                tc_fence_after();
+                for (int j = 0; j < n; ++j) {
+                    if (!mbar_wait(full0 + 8 * s, lap, abort_flag)) {
+                        *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
+                    }
+                    tc_fence_after();
+                    // a stage has columns of its own for its scales, so what reads them is done when they are written again
+                    const uint32_t w_addr = smem_u32(smem + s * STAGE_BYTES), scales = tmem + 2 * BN + 16 * s;
+                    const uint32_t s_addr = w_addr + W_BYTES + X_BYTES;
+                    fl_copy_scales(scales, s_addr);
+                    fl_copy_scales(scales + 4, s_addr + 512);
+                    fl_copy_scales(scales + 8, s_addr + FL_CHUNK);
+                    fl_copy_scales(scales + 12, s_addr + FL_CHUNK + 512);
+                    fl_mma_x4(tmem + buf * BN, smem_desc(w_addr), smem_desc(w_addr + W_BYTES), idesc0, idesc1, scales,
+                              scales + 8 + rows_at, scales + 4, scales + 12 + rows_at, j > 0 ? 1u : 0u);
+                    tc_commit(empty0 + 8 * s);
+                    if (++s == STAGES) { s = 0; lap ^= 1; }
+                }
+                if (ok) tc_commit(acc_full0 + 8 * buf);
+                u += n;
+            }
+        }
+    } else {
+        if (!LIST) ssb_pdl_wait();
+        constexpr int CH = 16;                                    // rows of x at a time
+        const int quarter = warp & 3, in_tile = quarter * 32 + lane, who = threadIdx.x - 64;
+        int i = 0;
+        for (long long u = range.begin; u < range.end; ++i) {
+            const int tile = (int)(u / k_blocks), kb0 = (int)(u - (long long)tile * k_blocks);
+            const int n = (int)min((long long)(k_blocks - kb0), range.end - u), buf = i & 1;
+            int mt, nt;
+            place(tile, mt, nt);
+            const int m0 = mt * BN, col = nt * FL_BM + in_tile;    // the tile's first row of x, this thread's output channel
+            u += n;
+            // all that does not wait for the sums comes before them
+            int rows, sorted0 = 0;
+            if (LIST) { sorted0 = list.tile_row0[mt]; rows = min(list.offsets[list.tile_expert[mt] + 1] - sorted0, BN); }
+            else rows = min(BN, o.M - m0);
+            const long long first = (long long)tile * k_blocks;
+            const int c0_block = n == k_blocks ? 0 : range.owner(first), c1_block = n == k_blocks ? 0 : range.owner(first + k_blocks - 1);
+            __syncwarp();
+            // the four warps meet below: they go on together or not at all
+            if (fl_any_of_four(!mbar_wait(acc_full0 + 8 * buf, (i >> 1) & 1, abort_flag))) {
+                if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
+            // a block's pieces: of the tile that its range begins in the middle of (or that is all it has), and of its last; four
+            // rows' sums of a channel lie together
+            auto piece = [&](int c) { return reinterpret_cast<float4*>(pieces) + (size_t)(2 * c + (c == c0_block)) * (BN / 4) * FL_BM + in_tile; };
+            bool mine = true;                                      // whether this block writes the tile's results
+            if (n < k_blocks) {
+                float4* dst = piece(blockIdx.x);
+#pragma unroll 1
+                for (int c0 = 0; c0 < rows; c0 += CH) {
+                    float sum[CH];
+                    fl_ld16(acc + c0, sum);
+#pragma unroll
+                    for (int e = 0; e < CH; e += 4)
+                        if (c0 + e < rows) dst[(size_t)((c0 + e) / 4) * FL_BM] = make_float4(sum[e], sum[e + 1], sum[e + 2], sum[e + 3]);
+                }
+                __threadfence();
+                fl_any_of_four(false);
+                bool last = false;
+                if (threadIdx.x == 64) {
+                    last = atomicAdd(arrived + c0_block, n) + n == k_blocks;
+                    if (last) arrived[c0_block] = 0;               // as it was, for the next launch that counts here
+                }
+                mine = fl_any_of_four(last);
+                if (mine) __threadfence();
+            }
+#pragma unroll 1
+            for (int c0 = 0; mine && c0 < rows; c0 += CH) {        // rows of x
+                const int live = col < o.N ? rows - c0 : 0;
+                const size_t at = (size_t)(m0 + c0) * o.ldo + col;
+                float was[CH];
+                __syncwarp();
+                if (MODE == FL_STORE && o.add)
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) was[e] = e < live ? ((const float*)o.out)[at + (size_t)e * o.ldo] : 0.f;
+                float sum[CH];
+                if (n == k_blocks) {
+                    fl_ld16(acc + c0, sum);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < CH; ++e) sum[e] = 0.f;
+#pragma unroll 4
+                    for (int c = c0_block; c <= c1_block; ++c) {
+                        const float4* src = piece(c) + (size_t)(c0 / 4) * FL_BM;
+#pragma unroll
+                        for (int e = 0; e < CH; e += 4) {
+                            const float4 v = c0 + e < rows ? __ldcg(src + (size_t)(e / 4) * FL_BM) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            sum[e] += v.x; sum[e + 1] += v.y; sum[e + 2] += v.z; sum[e + 3] += v.w;
+                        }
+                    }
+                }
+                if (MODE == FL_STORE) {
+                    if (o.index) {
+#pragma unroll
+                        for (int e = 0; e < CH; ++e)
+                            if (e < live) ((float*)o.out)[(size_t)o.index[sorted0 + c0 + e] * o.ldo + col] = sum[e];
+                    } else if (!o.is_f32) {
+#pragma unroll
+                        for (int e = 0; e < CH; ++e)
+                            if (e < live) ((bf16*)o.out)[at + (size_t)e * o.ldo] = __float2bfloat16_rn(sum[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < CH; ++e)
+                            if (e < live) ((float*)o.out)[at + (size_t)e * o.ldo] = o.add ? sum[e] + was[e] : sum[e];
+                    }
+                } else {
+                    // inner rows: a lane holds one channel of 16 rows, a block of 32 channels is wanted in two neighbouring lanes
+                    constexpr int WIDE = MODE == FL_GATED ? 64 : 128;                // inner channels a tile
+                    static_assert(CH == FL_INNER_ROWS, "");
+                    if (MODE == FL_GATED) {
+                        const bool up = lane >= 16;
+                        const int at_ch = quarter * 16 + (lane & 15);
+#pragma unroll
+                        for (int j = 0; j < CH; j += 2) {
+                            // lanes 0-15 finish row j, lanes 16-31 row j + 1
+                            const float own = up ? sum[j + 1] : sum[j], give = up ? sum[j] : sum[j + 1];
+                            const float got = __shfl_xor_sync(0xffffffffu, give, 16);
+                            float z = ssb_gate(up ? got : own, up ? own : got, o.kind, o.limit);
+                            const int r = c0 + j + (up ? 1 : 0);
+                            if (o.row_scale && r < rows) z *= o.row_scale[m0 + r];
+                            inner[(j + (up ? 1 : 0)) * FL_INNER_LD + at_ch] = z;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < CH; ++j) inner[j * FL_INNER_LD + in_tile] = ssb_activate(sum[j], o.kind) * o.limit;
+                    }
+                    fl_meet_four();
+                    // WIDE / 16 half blocks a row
+                    const int width = MODE == FL_GATED ? o.N / 2 : o.N, z0 = nt * WIDE, left = rows - c0;
+#pragma unroll
+                    for (int item = who; item < CH * (WIDE / 16); item += 128) {
+                        const int r = item / (WIDE / 16), half = item % (WIDE / 16), k = z0 + half * 16;
+                        float v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            const float4 q = *reinterpret_cast<const float4*>(inner + r * FL_INNER_LD + half * 16 + e);
+                            v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
+                        }
+                        const int row = m0 + c0 + r;               // of the codes
+                        const int in_list = (LIST ? mt * 128 + c0 + r : row);                     // a listed tile's scales are 128 rows'
+                        fl_put_inner(v, (uint8_t*)o.out + (size_t)row * o.ldo + k / 2,
+                                     o.scales + f4_scale_at(in_list, k / F4_BLOCK, o.inner_blocks), r < left && k < width);
+                        // behind the last channel: scales of zero up to a whole k-block
+                        if (nt == n_tiles - 1 && r < left && half == 0)
+                            for (int b = width / F4_BLOCK; b < 8 * o.inner_blocks; ++b) o.scales[f4_scale_at(in_list, b, o.inner_blocks)] = 0;
+                    }
+                    fl_meet_four();
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) fl_arrive(acc_empty0 + 8 * buf);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(fl_columns<BN, STAGES>()) : "memory");
+    }
+}
+
+// Tiles of 256 rows x 256 channels on pairs of SMs: each block fetches 128 rows and 128 channels a k-block, its rows' scales and those
+// of all 256 channels (35 KB for 512 clocks of products); the leader issues the pair's instructions, each block's tensor memory gets
+// its 128 rows.  Tensor memory has 512 columns: two accumulators of 256 that share 64 of them, and two sets of 24 for scales.  An
+// epilogue begins with the columns that the next tile wants, so the next tile's products run beside the rest of it.  Tiles go in bands
+// of ``group_m`` row tiles, row tiles fastest.
+constexpr int FL_PAIR_STAGES = 5;
+constexpr int FL_PAIR_STAGE_BYTES = 2 * FL_BM * FL_ROW + 3 * F4_CHUNK;
+constexpr int FL_PAIR_ACC = 192;          // columns from the first accumulator to the second
+constexpr int FL_PAIR_SCALES = 448;       // scales' first column
+constexpr size_t FL_PAIR_SMEM = (size_t)FL_PAIR_STAGES * FL_PAIR_STAGE_BYTES + TC_STAGE_BYTES + (2 * FL_PAIR_STAGES + 3) * 8 + 24 + 1024;
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FL_THREADS, 1)
+fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ CUtensorMap map_ws, const FlOut o, int m_tiles, int n_tiles, int k_blocks, int group_m,
+                int* __restrict__ error_word) {
+    constexpr int BN = 256, STAGES = FL_PAIR_STAGES;
+    constexpr uint32_t X_BYTES = FL_BM * FL_ROW, W_BYTES = FL_BM * FL_ROW, STAGE_BYTES = FL_PAIR_STAGE_BYTES;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* put = (float*)(smem + STAGES * STAGE_BYTES);
+    uint64_t* bars = (uint64_t*)(smem + STAGES * STAGE_BYTES + TC_STAGE_BYTES);       // full[STAGES], empty[STAGES], acc_full[2], free
+    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 3);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();                        // 0: the leader
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, tiles = m_tiles * n_tiles;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+    const uint32_t acc_full0 = smem_u32(bars + 2 * STAGES), free0 = smem_u32(bars + 2 * STAGES + 2);
+    auto tile_at = [&](int tile, int& m, int& n) {
+        const int band = tile / (group_m * n_tiles), in_band = tile - band * group_m * n_tiles, rows = min(group_m, m_tiles - band * group_m);
+        m = band * group_m + in_band % rows;
+        n = in_band / rows;
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int i = 0; i < 2; ++i) mbar_init(acc_full0 + 8 * i, 1);
+        mbar_init(free0, 8);
+        abort_flag[0] = 0;
+        abort_flag[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync_all();   // both blocks' barriers are initialised before either signals the other
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        ssb_pdl_wait();
+        if (lane == 0) {
+            ssb_pdl_launch_dependents();
+            const uint32_t leader_full0 = cluster_map(full0, 0);
+            int c = 0;
+            for (int tile = pair; tile < tiles && !*abort_flag; tile += n_pairs) {
+                int m, n;
+                tile_at(tile, m, n);
+                const int mt = 2 * m + (int)rank, n0 = n * BN + (int)rank * FL_BM;
+                for (int kb = 0; kb < k_blocks; ++kb, ++c) {
+                    const int s = c % STAGES;
+                    const uint32_t x_dst = smem_u32(smem + s * STAGE_BYTES), bar = leader_full0 + 8 * s;
+                    if (!mbar_wait(empty0 + 8 * s, ((c / STAGES) & 1) ^ 1, abort_flag)) {
+                        *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_PRODUCER); break;
+                    }
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
+                    tma_load_2d_pair(x_dst, &map_x, bar, kb * FL_ROW, mt * FL_BM);
+                    tma_load_2d_pair(x_dst + X_BYTES, &map_w, bar, kb * FL_ROW, n0);
+                    tma_load_2d_pair(x_dst + X_BYTES + W_BYTES, &map_xs, bar, 0, mt * k_blocks + kb);
+                    tma_load_2d_pair(x_dst + X_BYTES + W_BYTES + FL_CHUNK, &map_ws, bar, 0, 2 * n * k_blocks + kb);
+                    tma_load_2d_pair(x_dst + X_BYTES + W_BYTES + 2 * FL_CHUNK, &map_ws, bar, 0, (2 * n + 1) * k_blocks + kb);
+                }
+            }
+            if (*abort_flag) {
+                // let issued copies land: the leader sees both blocks' bytes on its barriers, the other block gives them time
+                if (rank == 0) {
+                    for (int i = max(0, c - STAGES); i < c; ++i)
+                        mbar_wait(full0 + 8 * (i % STAGES), (i / STAGES) & 1, abort_flag + 1);
+                } else {
+                    const long long t0 = clock64();
+                    while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        ssb_pdl_wait();
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc0 = fl_idesc(256, BN, 0), idesc1 = fl_idesc(256, BN, 1);
+            bool ok = true;
+            int c = 0, i = 0;
+            for (int tile = pair; tile < tiles && ok; tile += n_pairs, ++i) {
+                const uint32_t acc = tmem + (i & 1) * FL_PAIR_ACC;
+                if (i > 0 && !mbar_wait(free0, (i - 1) & 1, abort_flag)) {    // both epilogues have drained the shared columns
+                    *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
+                }
+                tc_fence_after();
+                for (int kb = 0; kb < k_blocks && ok; ++kb, ++c) {
+                    const int s = c % STAGES, before = c - 2;
+                    // this k-block's scales go where those of two k-blocks before were: their products have to be done
+                    if (!mbar_wait(full0 + 8 * s, (c / STAGES) & 1, abort_flag) ||
+                        (before >= 0 && !mbar_wait(empty0 + 8 * (before % STAGES), (before / STAGES) & 1, abort_flag))) {
+                        *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
+                    }
+                    tc_fence_after();
+                    const uint32_t x_addr = smem_u32(smem + s * STAGE_BYTES), s_addr = x_addr + X_BYTES + W_BYTES;
+                    const uint32_t xs = tmem + FL_PAIR_SCALES + (c & 1) * 24, ws = xs + 8;
+                    fl_copy_scales_pair(xs, s_addr);
+                    fl_copy_scales_pair(xs + 4, s_addr + 512);
+                    fl_copy_scales_pair(ws, s_addr + FL_CHUNK);                   // channels 0-127, blocks 0-3
+                    fl_copy_scales_pair(ws + 4, s_addr + 2 * FL_CHUNK);           // channels 128-255
+                    fl_copy_scales_pair(ws + 8, s_addr + FL_CHUNK + 512);         // blocks 4-7
+                    fl_copy_scales_pair(ws + 12, s_addr + 2 * FL_CHUNK + 512);
+                    fl_mma_pair_x4(acc, smem_desc(x_addr), smem_desc(x_addr + X_BYTES), idesc0, idesc1, xs, ws, xs + 4, ws + 8, kb > 0 ? 1u : 0u);
+                    tc_commit_pair(empty0 + 8 * s, 3);              // the stage is free in both blocks
+                }
+                if (ok) tc_commit_pair(acc_full0 + 8 * (i & 1), 3);
+            }
+        }
+    } else {
+        ssb_pdl_wait();
+        const int quarter = warp & 3;
+        float* stage = put + quarter * 32 * TC_STAGE_LD;
+        const uint32_t leader_free = cluster_map(free0, 0);
+        int i = 0;
+        for (int tile = pair; tile < tiles; tile += n_pairs, ++i) {
+            int m, n;
+            tile_at(tile, m, n);
+            const int row0 = (2 * m + (int)rank) * FL_BM + quarter * 32, row = row0 + lane, rows = o.M - row0, buf = i & 1;
+            const float row_scale = MODE == FL_GATED && o.row_scale && row < o.M ? o.row_scale[row] : 1.f;
+            bool ok = mbar_wait(acc_full0 + 8 * buf, (i >> 1) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_EPILOGUE); }
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * FL_PAIR_ACC + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+                const int g = buf == 0 ? (j + 3) & 3 : j;            // the shared 64 columns first
+                uint32_t r[2][32];
+                tc_ld32(acc + g * 64, r[0]);
+                tc_ld32(acc + g * 64 + 32, r[1]);
+                if (j == 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_free);
+                }
+                if (MODE == FL_STORE) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int col = n * BN + g * 64 + h * 32;
+                        if (rows <= 0 || col >= o.N) continue;
+                        const bool whole = col + 32 <= o.N;
+                        if (o.is_f32) {
+                            if (whole) {
+                                char* dst = (char*)((float*)o.out + (size_t)row0 * o.ldo + col);
+                                if (o.add) tc_put_rows<32, true>(stage, r[h], dst, (size_t)o.ldo * 4, rows);
+                                else tc_put_rows<32, false>(stage, r[h], dst, (size_t)o.ldo * 4, rows);
+                            } else if (row < o.M) {
+                                float* dst = (float*)o.out + (size_t)row * o.ldo + col;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (col + e < o.N) dst[e] = o.add ? dst[e] + __uint_as_float(r[h][e]) : __uint_as_float(r[h][e]);
+                            }
+                        } else {
+                            uint32_t packed[16];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1]));
+                                packed[e / 2] = *reinterpret_cast<const uint32_t*>(&p);
+                            }
+                            if (whole) {
+                                tc_put_rows<16, false>(stage, packed, (char*)((bf16*)o.out + (size_t)row0 * o.ldo + col), (size_t)o.ldo * 2, rows);
+                            } else if (row < o.M) {
+                                bf16* dst = (bf16*)o.out + (size_t)row * o.ldo + col;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (col + e < o.N) dst[e] = __float2bfloat16_rn(__uint_as_float(r[h][e]));
+                            }
+                        }
+                    }
+                } else {
+                    // a lane holds 64 sums of its row: a block of 32 inner channels (16 gate, 16 up, twice), or two of them
+                    constexpr int BLOCKS = MODE == FL_GATED ? 1 : 2;
+                    const int width = MODE == FL_GATED ? o.N / 2 : o.N;
+#pragma unroll
+                    for (int h = 0; h < BLOCKS; ++h) {
+                        float v[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            v[e] = MODE == FL_GATED ? ssb_gate(__uint_as_float(r[e >> 4][e & 15]), __uint_as_float(r[e >> 4][16 + (e & 15)]), o.kind, o.limit) * row_scale
+                                                    : ssb_activate(__uint_as_float(r[h][e]), o.kind) * o.limit;
+                        uint32_t most = f4_most(v);
+                        if (most >= F4_WILD) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = f4_finite(v[e]);
+                            most = f4_most(v);
+                        }
+                        const int byte = f4_scale_byte(most), k = (n * 4 + g) * 32 * BLOCKS + h * 32;
+                        const float inverse = f4_inverse(byte);
+                        if (row < o.M && k < width) {
+                            *reinterpret_cast<uint4*>((uint8_t*)o.out + (size_t)row * o.ldo + k / 2) =
+                                make_uint4(f4_encode8(v, inverse), f4_encode8(v + 8, inverse), f4_encode8(v + 16, inverse), f4_encode8(v + 24, inverse));
+                            o.scales[f4_scale_at(row, k / F4_BLOCK, o.inner_blocks)] = (uint8_t)byte;
+                        }
+                    }
+                    // behind the last channel: scales of zero up to a whole k-block
+                    if (j == 0 && n == n_tiles - 1 && row < o.M)
+                        for (int b = width / F4_BLOCK; b < 8 * o.inner_blocks; ++b) o.scales[f4_scale_at(row, b, o.inner_blocks)] = 0;
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    cluster_sync_all();   // neither block leaves while the other may still read its shared memory or signal it
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+    cluster_sync_all();
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+// codes: rows of ``row_bytes`` bytes, boxes of box_rows x 128 bytes
+static int fl_map(CUtensorMap* map, const void* base, long long rows, int row_bytes, int box_rows) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return SSB_ERR_UNSUPPORTED;
+    cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    cuuint32_t box[2] = {FL_ROW, (cuuint32_t)box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : SSB_ERR_BAD_SIZE;
+}
+// scales: ``chunks`` of 1,024 bytes, a chunk a box
+static int fl_scale_map(CUtensorMap* map, const void* base, long long chunks) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return SSB_ERR_UNSUPPORTED;
+    cuuint64_t dims[2] = {F4_CHUNK / 4, (cuuint64_t)chunks};
+    cuuint64_t strides[1] = {F4_CHUNK};
+    cuuint32_t box[2] = {F4_CHUNK / 4, 1};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : SSB_ERR_BAD_SIZE;
+}
+
+struct FlPlan {
+    int bn, m_tiles, n_tiles, blocks;      // bn 0: tiles on pairs
+    size_t pieces;                         // bytes
+};
+static FlPlan fl_plan(int M, int N, int K) {
+    const int sms = ssb_sm_count(), k_blocks = f4_k_blocks(K);
+    FlPlan best{};
+    double least = 0;
+    auto consider = [&](double cost, int bn, int m_tiles, int n_tiles, int blocks) {
+        if (best.m_tiles && cost >= least) return;
+        least = cost;
+        best = FlPlan{bn, m_tiles, n_tiles, blocks, (size_t)blocks * 2 * bn * FL_BM * 4};
+    };
+    for (int bn = M <= 16 ? 16 : M <= 32 ? 32 : 64; bn <= 128; bn *= 2) {
+        const int m_tiles = (M + bn - 1) / bn, n_tiles = (N + FL_BM - 1) / FL_BM;
+        const long long tiles = (long long)m_tiles * n_tiles, units = tiles * k_blocks;
+        const double each = bn < 128 ? 0.36 : m_tiles == 1 ? 0.6 : 0.45;
+        const double piece = 0.012 * std::min(bn, M);
+        const int any = (int)std::min<long long>(sms, std::max(1LL, units / 4));
+        consider(9 + each * (double)((units + any - 1) / any) + 4 + piece * (double)((any + tiles - 1) / tiles), bn, m_tiles, n_tiles, any);
+        if (tiles <= sms) {
+            const int parts = std::min(sms / (int)tiles, std::max(1, k_blocks / (bn <= 32 ? 4 : 8)));
+            consider(9 + each * ((k_blocks + parts - 1) / parts) + (parts > 1 ? piece * parts : 0), bn, m_tiles, n_tiles, (int)tiles * parts);
+        }
+        if (M <= bn) break;
+    }
+    if (M > 64) {
+        const int m_tiles = (M + 255) / 256, n_tiles = (N + 255) / 256, pairs = sms / 2;
+        const long long tiles = (long long)m_tiles * n_tiles;
+        consider(8 + 0.37 * (double)((tiles + pairs - 1) / pairs) * k_blocks + 0.09 * (double)std::min<long long>(tiles, pairs), 0, m_tiles, n_tiles, 0);
+    }
+    return best;
+}
+static size_t fl_round(size_t n) { return (n + 255) & ~(size_t)255; }
+
+constexpr int FL_COUNTERS = 256;          // of a launch: one for each of its blocks
+
+// Scratch of a product of M rows by N x K weights: codes and scales of the rows (of rows that come as numbers), pieces of tiles.
+struct FlScratch {
+    size_t codes, scales, pieces, all;
+    FlScratch(int M, int K, bool numbers, size_t piece_bytes) {
+        codes = 0;
+        scales = numbers ? fl_round((size_t)M * (K / 2)) : 0;
+        pieces = scales + (numbers ? (size_t)((M + 127) / 128) * f4_k_blocks(K) * F4_CHUNK : 0);
+        all = pieces + std::max<size_t>(piece_bytes, 16);
+    }
+};
+SSB_API long long ssb_fp4_linear_scratch(int M, int N, int K, int numbers) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return (long long)FlScratch(M, K, numbers != 0, fl_plan(M, N, K).pieces).all;
+}
+
+template <int BN, int STAGES, int MODE, bool LIST>
+static int fl_stream(const CUtensorMap& mw, const CUtensorMap& mws, const CUtensorMap& mx, const CUtensorMap& mxs, const FlOut& o,
+                     const FlTiles& list, int m_tiles, int n_tiles, int blocks, int K, int* counters, float* pieces, int* error_word,
+                     cudaStream_t stream) {
+    constexpr size_t smem = fl_smem<BN, STAGES>();
+    static_assert(smem <= 227 * 1024, "");
+    static bool configured = false;
+    if (!configured) {
+        cudaError_t e = cudaFuncSetAttribute(fp4_stream_kernel<BN, STAGES, MODE, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    return ssb_launch(fp4_stream_kernel<BN, STAGES, MODE, LIST>, dim3(blocks), dim3(FL_THREADS), smem, stream, true, mw, mws, mx, mxs, o, list,
+                      m_tiles, n_tiles, f4_k_blocks(K), counters, pieces, error_word);
+}
+
+template <int MODE>
+static int fl_pair(const CUtensorMap& mx, const CUtensorMap& mxs, const CUtensorMap& mw, const CUtensorMap& mws, const FlOut& o, const FlPlan& p,
+                   int K, int* error_word, cudaStream_t stream) {
+    static_assert(FL_PAIR_SMEM <= 227 * 1024, "");
+    static int max_pairs = 0;
+    if (!max_pairs) {
+        cudaError_t e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FL_PAIR_SMEM);
+        if (e != cudaSuccess) return (int)e;
+        const int sms = ssb_sm_count();
+        // how many pairs the device holds at once (a GPC with an odd SM left over holds one fewer)
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(sms & ~1);
+        cfg.blockDim = dim3(FL_THREADS);
+        cfg.dynamicSmemBytes = FL_PAIR_SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, fp4_pair_kernel<MODE>, &cfg) != cudaSuccess || clusters <= 0) {
+            cudaGetLastError();
+            clusters = sms / 2;
+        }
+        max_pairs = std::min(clusters, sms / 2);
+    }
+    const int pairs = std::min(p.m_tiles * p.n_tiles, max_pairs);
+    return ssb_launch(fp4_pair_kernel<MODE>, dim3(2 * pairs), dim3(FL_THREADS), FL_PAIR_SMEM, stream, true, mx, mxs, mw, mws, o, p.m_tiles,
+                      p.n_tiles, f4_k_blocks(K), std::min(16, p.m_tiles), error_word);
+}
+
+template <int MODE>
+static int fl_dense(const void* x, const void* xs, const void* w, const void* ws, const FlOut& o, int K, int* counters, float* pieces,
+                    const FlPlan& p, int* error_word, cudaStream_t stream) {
+    const int k_blocks = f4_k_blocks(K);
+    CUtensorMap mw, mws, mx, mxs;
+    int rc = fl_map(&mx, x, o.M, K / 2, p.bn ? p.bn : FL_BM);
+    if (!rc) rc = fl_map(&mw, w, o.N, K / 2, FL_BM);
+    if (!rc) rc = fl_scale_map(&mxs, xs, (long long)((o.M + 127) / 128) * k_blocks);
+    if (!rc) rc = fl_scale_map(&mws, ws, (long long)((o.N + 127) / 128) * k_blocks);
+    if (rc) return rc;
+    const FlTiles none{};
+    switch (p.bn) {
+        case 16: return fl_stream<16, 10, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
+        case 32: return fl_stream<32, 9, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
+        case 64: return fl_stream<64, 8, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
+        case 128: return fl_stream<128, 6, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
+    }
+    return fl_pair<MODE>(mx, mxs, mw, mws, o, p, K, error_word, stream);
+}
+
+SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* codes, void* scales, int rows, int K, int per_expert, int inter,
+                             int* clear, int n_clear, cudaStream_t stream);
+SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void* codes, void* scales, int pairs, int top, int K,
+                                   const int* slot, int tile_rows, cudaStream_t stream);
+
+// A product of dense weights.  x: rows of dtype (ldx elements apart), which are quantised first, or (dtype -1) codes with the scales xs.
+// counters: FL_COUNTERS words (``n_clear`` of them and behind them are zeroed on the way where x is quantised; else the launch needs
+// them zero); the launch leaves them zero.  scratch: ssb_fp4_linear_scratch bytes.
+template <int MODE>
+static int fl_product(const void* x, long long ldx, int dtype, const void* xs, const void* w, const void* ws, const FlOut& o, int K,
+                      void* scratch, int* counters, int n_clear, int* error_word, cudaStream_t stream) {
+    if (o.M < 0 || o.N <= 0 || K <= 0 || K % F4_BLOCK || o.N % 8 || !scratch || !counters || !error_word) return SSB_ERR_BAD_SIZE;
+    if (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws | (uintptr_t)o.out | (uintptr_t)o.scales | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
+    if (o.M == 0) return 0;
+    const FlPlan p = fl_plan(o.M, o.N, K);
+    if (p.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
+    const FlScratch at(o.M, K, dtype >= 0, p.pieces);
+    char* base = (char*)scratch;
+    if (dtype >= 0) {
+        const int rc = ssb_fp4_quantize(x, ldx, dtype, base + at.codes, base + at.scales, o.M, K, o.M, 0, counters, n_clear, stream);
+        if (rc) return rc;
+        x = base + at.codes;
+        xs = base + at.scales;
+    }
+    return fl_dense<MODE>(x, xs, w, ws, o, K, counters, (float*)(base + at.pieces), p, error_word, stream);
+}
+
+SSB_API int ssb_fp4_linear(const void* x, long long ldx, int dtype, const void* xs, const void* w, const void* ws, void* out, int ldo,
+                           int out_dtype, int M, int N, int K, int add, void* scratch, int* counters, int* error_word, cudaStream_t stream) {
+    if ((out_dtype != SSB_F32 && out_dtype != SSB_BF16) || (add && out_dtype != SSB_F32)) return SSB_ERR_BAD_DTYPE;
+    const FlOut o{out, nullptr, nullptr, nullptr, ldo, out_dtype == SSB_F32, add, M, N, 0, 0.f, 0};
+    return fl_product<FL_STORE>(x, ldx, dtype, xs, w, ws, o, K, scratch, counters, FL_COUNTERS, error_word, stream);
+}
+
+// The inner rows of a feed-forward in 4 bits.  gated: w holds 16 gate rows and their 16 up rows in turn, N = 2 x inner channels, kind and
+// limit as ssb_gate's; else kind as ssb_activate's and limit a factor.  counters: as above, and as many behind them for the product that
+// reads the inner rows.
+SSB_API int ssb_fp4_inner(const void* x, long long ldx, int dtype, const void* xs, const void* w, const void* ws, void* codes, void* scales,
+                          int M, int N, int K, int gated, int kind, float limit, const float* row_scale, void* scratch, int* counters,
+                          int* error_word, cudaStream_t stream) {
+    const int inner = gated ? N / 2 : N;
+    if (inner % F4_BLOCK || (gated && N % 2) || kind < 0 || kind > 2 || (row_scale && !gated)) return SSB_ERR_BAD_SIZE;
+    const FlOut o{codes, (uint8_t*)scales, nullptr, row_scale, inner / 2, 0, 0, M, N, kind, limit, f4_k_blocks(inner)};
+    return gated ? fl_product<FL_GATED>(x, ldx, dtype, xs, w, ws, o, K, scratch, counters, 2 * FL_COUNTERS, error_word, stream)
+                 : fl_product<FL_ACT>(x, ldx, dtype, xs, w, ws, o, K, scratch, counters, 2 * FL_COUNTERS, error_word, stream);
+}
+
+// ---- experts ----------------------------------------------------------------------------------------------------------
+// Pairs (token, choice) by expert, one block: counts in shared memory, first rows and first tiles of the experts by one warp, then every
+// pair takes the next row of its expert.  ``slot``: where a pair's row goes among tiles of BN rows (-1: its expert is none), ``order``:
+// the pair of a sorted row.  The order inside an expert is whatever the adds give; nothing that is written depends on it.
+__global__ void __launch_bounds__(1024)
+fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int bn, int* __restrict__ offsets, int* __restrict__ order,
+                 int* __restrict__ slot, int* __restrict__ tile_expert, int* __restrict__ tile_row0, int* __restrict__ meta,
+                 int* __restrict__ clear, int n_clear) {
+    extern __shared__ int counts[];                                // [experts] counts, then the next row; [experts] first row, [experts] first tile
+    int *row0 = counts + experts, *tile0 = row0 + experts;
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
+    for (int i = threadIdx.x; i < n_clear; i += blockDim.x) clear[i] = 0;
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[e] = 0;
+    __syncthreads();
+    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
+        const int e = expert_of[p];
+        if ((unsigned)e < (unsigned)experts) atomicAdd(&counts[e], 1);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int row = 0, tile = 0;
+        for (int e0 = 0; e0 < experts; e0 += 32) {
+            const int e = e0 + threadIdx.x, n = e < experts ? counts[e] : 0, t = (n + bn - 1) / bn;
+            int r_sum = n, t_sum = t;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int r = __shfl_up_sync(0xffffffffu, r_sum, d), q = __shfl_up_sync(0xffffffffu, t_sum, d);
+                if (threadIdx.x >= d) { r_sum += r; t_sum += q; }
+            }
+            if (e < experts) {
+                row0[e] = row + r_sum - n;
+                tile0[e] = tile + t_sum - t;
+                offsets[e] = row0[e];
+            }
+            row += __shfl_sync(0xffffffffu, r_sum, 31);
+            tile += __shfl_sync(0xffffffffu, t_sum, 31);
+        }
+        if (threadIdx.x == 0) { offsets[experts] = row; meta[0] = tile; }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        for (int i = 0; i < counts[e]; i += bn) {
+            tile_expert[tile0[e] + i / bn] = e;
+            tile_row0[tile0[e] + i / bn] = row0[e] + i;
+        }
+        counts[e] = 0;
+    }
+    __syncthreads();
+    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
+        const int e = expert_of[p];
+        int to = -1;
+        if ((unsigned)e < (unsigned)experts) {
+            const int i = atomicAdd(&counts[e], 1);
+            to = (tile0[e] + i / bn) * bn + i % bn;
+            order[row0[e] + i] = p;
+        }
+        slot[p] = to;
+    }
+}
+
+// out[t] (+)= sum over the choices j, in their order, of weight[t, j] * y[t, j]; choices of no expert count nothing.
+template <typename T>
+__global__ void __launch_bounds__(256)
+fp4_combine_kernel(const float* __restrict__ y, const int* __restrict__ slot, const float* __restrict__ weight, T* __restrict__ out,
+                   long long ldo, int tokens, int top, int width, int add) {
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
+    const int per_row = width / 8;
+    const long long pieces = (long long)tokens * per_row, step = (long long)gridDim.x * blockDim.x;
+    for (long long p = (long long)blockIdx.x * blockDim.x + threadIdx.x; p < pieces; p += step) {
+        const int t = (int)(p / per_row), c = (int)(p - (long long)t * per_row) * 8;
+        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < top; ++j) {
+            const int pair = t * top + j;
+            if (slot[pair] < 0) continue;
+            const float w = weight[pair];
+            float v[8];
+            f4_load8(y + (size_t)pair * width + c, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] = fmaf(w, v[i], sum[i]);
+        }
+        T* dst = out + t * ldo + c;
+        if (add) {
+            float v[8];
+            f4_load8(dst, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += v[i];
+        }
+        f4_store8(dst, sum);
+    }
+}
+
+// Rows a tile, by how many an expert has on average: no more than the step has tokens, and little of a tile empty.
+static int fl_list_rows(int tokens, int top, int experts) {
+    const long long mean = (long long)tokens * top / experts;
+    return tokens <= 16 || mean <= 8 ? 16 : tokens <= 32 || mean <= 16 ? 32 : tokens <= 64 || mean <= 48 ? 64 : 128;
+}
+struct FlExperts {
+    int bn, tiles, blocks;                 // rows a tile, tiles at most, blocks of a product
+    size_t counters, offsets, order, slot, tile_expert, tile_row0, meta, x, xs, z, zs, y, pieces, all;
+    FlExperts(int tokens, int top, int experts, int K, int inter) {
+        const int pairs = tokens * top;
+        bn = fl_list_rows(tokens, top, experts);
+        tiles = pairs / bn + std::min(experts, pairs);
+        blocks = ssb_sm_count();
+        const size_t rows = (size_t)tiles * bn, chunks = (size_t)tiles * F4_CHUNK;
+        size_t at = 0;
+        auto take = [&](size_t bytes) { const size_t was = at; at += fl_round(bytes); return was; };
+        counters = take(2 * FL_COUNTERS * 4);
+        offsets = take((size_t)(experts + 1) * 4);
+        order = take((size_t)pairs * 4);
+        slot = take((size_t)pairs * 4);
+        tile_expert = take((size_t)tiles * 4);
+        tile_row0 = take((size_t)tiles * 4);
+        meta = take(4);
+        x = take(rows * (K / 2));
+        xs = take(chunks * f4_k_blocks(K));
+        z = take(rows * (inter / 2));
+        zs = take(chunks * f4_k_blocks(inter));
+        y = take((size_t)pairs * K * 4);
+        pieces = take((size_t)blocks * 2 * bn * FL_BM * 4);
+        all = at;
+    }
+};
+SSB_API long long ssb_fp4_experts_scratch(int tokens, int top, int experts, int K, int inter) {
+    if (tokens <= 0 || top <= 0 || experts <= 0 || K <= 0 || inter <= 0) return 0;
+    return (long long)FlExperts(tokens, top, experts, K, inter).all;
+}
+
+template <int MODE>
+static int fl_listed(const void* x, const void* xs, const void* w, const void* ws, const FlOut& o, const FlTiles& list, const FlExperts& at,
+                     int experts, int K, int* counters, float* pieces, int* error_word, cudaStream_t stream) {
+    const int k_blocks = f4_k_blocks(K), n_tiles = (o.N + FL_BM - 1) / FL_BM;
+    CUtensorMap mw, mws, mx, mxs;
+    int rc = fl_map(&mx, x, (long long)at.tiles * at.bn, K / 2, at.bn);
+    if (!rc) rc = fl_map(&mw, w, (long long)experts * o.N, K / 2, FL_BM);
+    if (!rc) rc = fl_scale_map(&mxs, xs, (long long)at.tiles * k_blocks);
+    if (!rc) rc = fl_scale_map(&mws, ws, (long long)experts * n_tiles * k_blocks);
+    if (rc) return rc;
+    switch (at.bn) {
+        case 16: return fl_stream<16, 10, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+        case 32: return fl_stream<32, 9, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+        case 64: return fl_stream<64, 8, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+    }
+    return fl_stream<128, 6, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+}
+
+// out[t] (+)= sum_j weight[t, j] E(x_t) of expert expert_of[t, j]; w1: [experts][N1][K], w2: [experts][K][inter].
+SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* expert_of, const float* weight, const void* w1, const void* ws1,
+                            const void* w2, const void* ws2, void* out, long long ldo, int out_dtype, int tokens, int top, int experts, int K,
+                            int inter, int gated, int kind, float limit, int add, void* scratch, int* error_word, cudaStream_t stream) {
+    if (tokens < 0 || top <= 0 || experts <= 0 || experts > 4096 || K <= 0 || K % F4_BLOCK || inter <= 0 || inter % F4_BLOCK || kind < 0 || kind > 2 ||
+        !scratch || !error_word || (long long)tokens * top > (1 << 24)) return SSB_ERR_BAD_SIZE;
+    if (((uintptr_t)x | (uintptr_t)w1 | (uintptr_t)ws1 | (uintptr_t)w2 | (uintptr_t)ws2 | (uintptr_t)out | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
+    if ((dtype != SSB_F32 && dtype != SSB_BF16) || (out_dtype != SSB_F32 && out_dtype != SSB_BF16) || (add && out_dtype != SSB_F32)) return SSB_ERR_BAD_DTYPE;
+    if (tokens == 0) return 0;
+    const FlExperts at(tokens, top, experts, K, inter);
+    if (at.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
+    char* base = (char*)scratch;
+    auto ints = [&](size_t o) { return (int*)(base + o); };
+    const int pairs = tokens * top;
+    int rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(1024), (size_t)experts * 12, stream, true, expert_of, pairs, experts, at.bn, ints(at.offsets),
+                        ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta), ints(at.counters), 2 * FL_COUNTERS);
+    if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, pairs, top, K, ints(at.slot), at.bn, stream);
+    if (rc) return rc;
+    const FlTiles list{ints(at.offsets), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta)};
+    float* pieces = (float*)(base + at.pieces);
+    const FlOut first{base + at.z, (uint8_t*)(base + at.zs), nullptr, nullptr, inter / 2, 0, 0, tokens, gated ? 2 * inter : inter, kind, limit, f4_k_blocks(inter)};
+    rc = gated ? fl_listed<FL_GATED>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream)
+               : fl_listed<FL_ACT>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream);
+    if (rc) return rc;
+    const FlOut second{base + at.y, nullptr, ints(at.order), nullptr, K, 1, 0, tokens, K, 0, 0.f, 0};
+    rc = fl_listed<FL_STORE>(base + at.z, base + at.zs, w2, ws2, second, list, at, experts, inter, ints(at.counters) + FL_COUNTERS, pieces, error_word, stream);
+    if (rc) return rc;
+    const float* y = (const float*)(base + at.y);
+    const dim3 grid((unsigned)std::min<long long>(((long long)tokens * (K / 8) + 255) / 256, 8 * ssb_sm_count()));
+    if (out_dtype == SSB_BF16)
+        return ssb_launch(fp4_combine_kernel<bf16>, grid, dim3(256), 0, stream, true, y, ints(at.slot), weight, (bf16*)out, ldo, tokens, top, K, add);
+    return ssb_launch(fp4_combine_kernel<float>, grid, dim3(256), 0, stream, true, y, ints(at.slot), weight, (float*)out, ldo, tokens, top, K, add);
+}
+
+SSB_PACKED(ssb_fp4_linear)
+SSB_PACKED(ssb_fp4_inner)
+SSB_PACKED(ssb_fp4_experts)

@@ -1,0 +1,261 @@
+"""Python faces of the kernels in microscaled 4-bit floats: rows into 4 bits and back, matrix products of 4-bit rows and weights, and
+feed-forwards whose inner rows never leave 4 bits.
+
+Like :mod:`.ops`, every function checks what its kernel assumes, raises :class:`KernelError`, and launches on the current stream;
+nothing synchronises.  Weights, and rows that several products read, are :class:`~supersonic_b200.weights.Fp4Matrix`.
+
+A number's block is 32 neighbours along its row.  With m the block's largest magnitude (NaN counts as zero, an infinity as the largest
+finite number), its scale is 2^(floor(log2 m) - 2) (2^-127 at least, and where m is 0), and a number becomes the one of 0, 0.5, 1, 1.5,
+2, 3, 4, 6 (times the scale, with its sign) that is nearest, between two the one with the even code; what is above 6 becomes 6.
+Products of codes and their scales are exact, and are summed in float32.
+
+The modelled project's 4-bit lanes multiply int4 weights by activations of the model's type
+(crates/runner/src/llama31_engine.rs:289-430).
+"""
+from __future__ import annotations
+
+from ctypes import c_float, c_int, c_longlong, c_void_p
+from struct import Struct, error as StructError
+from typing import Optional, Union
+
+import torch
+
+from ..weights.fp4 import FP4_BLOCK, Fp4Matrix
+from . import ops
+from .build import load_library
+from .int8_ops import _error_word, _rows, _stream
+from .ops import KernelError, _CODES, _check
+
+_P, _I, _F, _L = c_void_p, c_int, c_float, c_longlong
+_SIGNATURES = {
+    "ssb_fp4_quantize": [_P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _I, _P],
+    "ssb_fp4_values": [_P, _P, _P, _L, _I, _I, _I, _I, _I, _P],
+    "ssb_fp4_linear": [_P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P],
+    "ssb_fp4_inner": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P],
+    "ssb_fp4_experts": [_P, _L, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
+    "ssb_fp4_linear_scratch": [_I] * 4,
+    "ssb_fp4_experts_scratch": [_I] * 5,
+}
+_FORMATS = {_P: "P", _I: "i", _F: "f", _L: "q"}
+_functions = {}
+_scratch_sizes = {}
+_COUNTERS = 256                # words a product counts in
+
+
+def _fn(name: str):
+    """The library's function; arguments of a launch go as one run of bytes (packed_call.cuh)."""
+    f = _functions.get(name)
+    if f is None:
+        types = _SIGNATURES[name]
+        if name.endswith("_scratch"):
+            f = getattr(load_library("fp4"), name)
+            f.restype, f.argtypes = c_longlong, types
+        else:
+            call, pack = getattr(load_library("fp4"), name + "_packed"), Struct("@" + "".join(_FORMATS[t] for t in types)).pack
+            call.restype = c_int
+
+            def f(*args):
+                try:
+                    packed = pack(*args)
+                except (StructError, OverflowError) as e:
+                    raise KernelError(f"{name}: {e}") from None
+                return call(packed)
+        _functions[name] = f
+    return f
+
+
+def _scratch_size(name: str, *sizes) -> int:
+    """What the library says a launch of these sizes needs."""
+    n = _scratch_sizes.get((name, sizes))
+    if n is None:
+        if len(_scratch_sizes) > 4096:
+            _scratch_sizes.clear()
+        n = _scratch_sizes[name, sizes] = _fn(name)(*sizes)
+    return n
+
+
+def _here(*tensors) -> torch.device:
+    """The current device, on which all of these have to be."""
+    device = tensors[0].device
+    if device.type != "cuda" or device.index != torch.cuda.current_device() or any(t.device != device for t in tensors):
+        raise KernelError(f"tensors must be on the current CUDA device, are on {sorted({str(t.device) for t in tensors})}")
+    return device
+
+
+def _matrix_rows(t: torch.Tensor, name: str, m: Fp4Matrix):
+    """(address, row stride, rows) of a tensor of a 4-bit matrix's shape, all its rows equally far apart."""
+    if tuple(t.shape) != m.shape or t.dtype not in _CODES or not t.is_cuda:
+        raise KernelError(f"{name} must be float32 or bfloat16 {m.shape} on a CUDA device, is {t.dtype} {tuple(t.shape)}")
+    if t.dim() == 3:
+        if not t.is_contiguous():
+            raise KernelError(f"{name}: matrices of several experts are contiguous")
+        t = t.view(-1, t.shape[-1])
+    return _rows(t, name, t.shape[0], t.shape[1]) + (t.shape[0],)
+
+
+def quantize(x: torch.Tensor, matrix: Fp4Matrix) -> None:
+    """``matrix`` gets the numbers of ``x`` (float32 or bfloat16, of its shape; of a gated matrix the gate rows, then the up rows)."""
+    at, ld, rows = _matrix_rows(x, "x", matrix)
+    _here(x, matrix.codes)
+    n, k = matrix.shape[-2:]
+    _check(_fn("ssb_fp4_quantize")(at, ld, _CODES[x.dtype], matrix.codes.data_ptr(), matrix.scales.data_ptr(), rows, k, n,
+                                   n // 2 if matrix.gated else 0, 0, 0, _stream()), "fp4_quantize")
+
+
+def values(matrix: Fp4Matrix, out: torch.Tensor) -> None:
+    """``out`` (float32 or bfloat16, of its shape) gets the numbers that ``matrix`` stands for, which both types hold exactly (down to
+    2^-128); of a gated matrix the gate rows, then the up rows."""
+    at, ld, rows = _matrix_rows(out, "out", matrix)
+    _here(out, matrix.codes)
+    n, k = matrix.shape[-2:]
+    _check(_fn("ssb_fp4_values")(matrix.codes.data_ptr(), matrix.scales.data_ptr(), at, ld, _CODES[out.dtype], rows, k, n,
+                                 n // 2 if matrix.gated else 0, _stream()), "fp4_values")
+
+
+Rows = Union[torch.Tensor, Fp4Matrix]
+
+
+def _operands(what: str, x: Rows, weight: Fp4Matrix):
+    """(rows, x's address, row stride, type code and scales' address) of rows that a dense weight takes."""
+    if not isinstance(weight, Fp4Matrix) or len(weight.shape) != 2:
+        raise KernelError(f"{what}: weight must be a 4-bit matrix [n, k], is {weight if isinstance(weight, Fp4Matrix) else type(weight)}")
+    n, k = weight.shape
+    if n % 8:
+        raise KernelError(f"{what}: n {n} must be a multiple of 8")
+    if isinstance(x, Fp4Matrix):
+        if len(x.shape) != 2 or x.shape[1] != k or x.gated:
+            raise KernelError(f"{what}: rows of {k} numbers, not {x}")
+        return x.shape[0], x.codes.data_ptr(), 0, -1, x.scales.data_ptr()
+    if x.dim() != 2:
+        raise KernelError(f"{what}: x must be a matrix, is {tuple(x.shape)}")
+    at, ld = _rows(x, "x", x.shape[0], k)
+    if x.shape[1] != k:
+        raise KernelError(f"{what}: rows of {k} numbers, not {tuple(x.shape)}")
+    return x.shape[0], at, ld, _CODES[x.dtype], 0
+
+
+def _counters(x: Rows, n: int, device) -> torch.Tensor:
+    """The words that a product counts in: zeroed by the launch that quantises its rows, or zero as they are."""
+    if not isinstance(x, Fp4Matrix):
+        return torch.empty(n, dtype=torch.int32, device=device)
+    left, x._scratch = x._scratch, None                    # whoever takes them has them alone
+    return torch.zeros(n, dtype=torch.int32, device=device) if left is None or n > _COUNTERS else left
+
+
+def _of(x: Rows) -> torch.Tensor:
+    return x.codes if isinstance(x, Fp4Matrix) else x
+
+
+def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = False) -> None:
+    """``out`` [rows, n] (+)= x W^T with ``x`` [rows, k] (float32 or bfloat16, quantised as it comes, or a 4-bit matrix) and ``weight``
+    [n, k].  ``accumulate`` adds to a float32 ``out``.  n: a multiple of 8."""
+    rows, x_at, ldx, code, xs_at = _operands("linear", x, weight)
+    if weight.gated:
+        raise KernelError("linear: a gated unit's first matrix goes through gate_up")
+    n, k = weight.shape
+    o_at, ldo = _rows(out, "out", rows, n)
+    if out.shape[1] != n:
+        raise KernelError(f"linear: out must be [{rows}, {n}], is {tuple(out.shape)}")
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError("linear: results are added in float32 only")
+    device = _here(out, weight.codes, _of(x))
+    if rows == 0:
+        return
+    counters = _counters(x, _COUNTERS, device)
+    scratch = torch.empty(_scratch_size("ssb_fp4_linear_scratch", rows, n, k, code >= 0), dtype=torch.int8, device=device)
+    _check(_fn("ssb_fp4_linear")(x_at, ldx, code, xs_at, weight.codes.data_ptr(), weight.scales.data_ptr(), o_at, ldo, _CODES[out.dtype],
+                                 rows, n, k, 1 if accumulate else 0, scratch.data_ptr(), counters.data_ptr(), _error_word(device),
+                                 _stream()), "fp4_linear")
+
+
+def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_scale: Optional[torch.Tensor]) -> Fp4Matrix:
+    rows, x_at, ldx, code, xs_at = _operands(what, x, weight)
+    n, k = weight.shape
+    inter = n // 2 if weight.gated else n
+    if inter % FP4_BLOCK:
+        raise KernelError(f"{what}: {inter} inner channels must be a multiple of {FP4_BLOCK}")
+    device = _here(weight.codes, _of(x))
+    if rows == 0:
+        raise KernelError(f"{what}: no rows")
+    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (rows,) or not row_scale.is_contiguous()
+                                  or row_scale.device != device):
+        raise KernelError(f"{what}: row_scale must be {rows} contiguous float32 values")
+    z = Fp4Matrix(torch.empty((rows, inter // 2), dtype=torch.uint8, device=device),
+                  torch.empty((-(-rows // 128) * -(-inter // 256), 1024), dtype=torch.uint8, device=device), (rows, inter))
+    counters = _counters(x, 2 * _COUNTERS, device)
+    scratch = torch.empty(_scratch_size("ssb_fp4_linear_scratch", rows, n, k, code >= 0), dtype=torch.int8, device=device)
+    _check(_fn("ssb_fp4_inner")(x_at, ldx, code, xs_at, weight.codes.data_ptr(), weight.scales.data_ptr(), z.codes.data_ptr(),
+                                z.scales.data_ptr(), rows, n, k, 1 if weight.gated else 0, kind, limit,
+                                0 if row_scale is None else row_scale.data_ptr(), scratch.data_ptr(), counters.data_ptr(),
+                                _error_word(device), _stream()), "fp4_inner")
+    z._scratch = counters[_COUNTERS:]
+    return z
+
+
+def gate_up(x: Rows, weight: Fp4Matrix, act=None, row_scale: Optional[torch.Tensor] = None) -> Fp4Matrix:
+    """The inner rows of a gated unit, f(x Wgate^T, x Wup^T) * row_scale from the float32 sums, in 4 bits [rows, inter].  ``weight``: a
+    gated matrix [2 x inter, k].  ``act``: None for silu(g) u, or (kind, limit) as :func:`.ops.gated_activation` takes them;
+    ``row_scale``: a float32 factor for each row."""
+    if not isinstance(weight, Fp4Matrix) or not weight.gated:
+        raise KernelError("gate_up: weight must be a gated 4-bit matrix")
+    kind, limit = act if act else ("silu", 0.0)
+    if kind not in ops.GATE_KINDS_FF:
+        raise KernelError(f"gate_up: {kind!r} is not known (known: {sorted(ops.GATE_KINDS_FF)})")
+    return _inner("gate_up", x, weight, ops.GATE_KINDS_FF[kind], float(limit), row_scale)
+
+
+def activated(x: Rows, weight: Fp4Matrix, act: str, scale: float = 1.0) -> Fp4Matrix:
+    """The inner rows of a feed-forward without gate, act(x W^T) * scale from the float32 sums, in 4 bits [rows, inter].  ``act``: one of
+    ``ops.ACTIVATIONS``."""
+    if act not in ops.ACTIVATIONS:
+        raise KernelError(f"activated: {act!r} is not known (known: {sorted(ops.ACTIVATIONS)})")
+    if isinstance(weight, Fp4Matrix) and weight.gated:
+        raise KernelError("activated: a gated unit's first matrix goes through gate_up")
+    return _inner("activated", x, weight, ops.ACTIVATIONS[act], float(scale), None)
+
+
+MOST_PAIRS = 1 << 24           # (token, choice) pairs of a call
+
+
+def experts(x: torch.Tensor, expert_of: torch.Tensor, pair_weight: torch.Tensor, first: Fp4Matrix, down: Fp4Matrix, out: torch.Tensor,
+            act=None, accumulate: bool = False) -> None:
+    """``out`` [tokens, k] (+)= sum over a token's choices j of pair_weight[t, j] * E(x_t), E the unit of expert ``expert_of[t, j]``:
+    down(f(gate x, up x)) with a gated ``first`` [experts, 2 x inter, k] (``act`` as :func:`gate_up` takes it), down(act(up x)) with
+    ``first`` [experts, inter, k] (``act``: one of ``ops.ACTIVATIONS``); ``down`` [experts, k, inter].  Rows and inner rows go into 4
+    bits, an inner row from the float32 sums; choices are summed in float32, in their order.  A choice that names no expert counts
+    nothing.  ``expert_of`` int32 and ``pair_weight`` float32 [tokens, top]; ``accumulate`` adds to a float32 ``out``."""
+    if not (isinstance(first, Fp4Matrix) and isinstance(down, Fp4Matrix) and len(first.shape) == len(down.shape) == 3):
+        raise KernelError("experts: first and down must be 4-bit matrices of several experts")
+    E, n, k = first.shape
+    inter = n // 2 if first.gated else n
+    if down.shape != (E, k, inter) or down.gated or k % FP4_BLOCK or inter % FP4_BLOCK:
+        raise KernelError(f"experts: first {first} takes a down of {[E, k, inter]}, not {down}")
+    if first.gated:
+        kind, limit = act if act else ("silu", 0.0)
+        kinds = ops.GATE_KINDS_FF
+    else:
+        kind, limit, kinds = act, 1.0, ops.ACTIVATIONS
+    if kind not in kinds:
+        raise KernelError(f"experts: {kind!r} is not known (known: {sorted(kinds)})")
+    if x.dim() != 2 or x.shape[1] != k or out.shape != x.shape:
+        raise KernelError(f"experts: x and out must be [tokens, {k}], are {tuple(x.shape)} and {tuple(out.shape)}")
+    tokens = x.shape[0]
+    x_at, ldx = _rows(x, "x", tokens, k)
+    o_at, ldo = _rows(out, "out", tokens, k)
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError("experts: results are added in float32 only")
+    device = _here(x, out, expert_of, pair_weight, first.codes, down.codes)
+    top = expert_of.shape[-1] if expert_of.dim() == 2 else 0
+    if top < 1 or expert_of.dtype != torch.int32 or pair_weight.dtype != torch.float32 or expert_of.shape != (tokens, top) \
+            or pair_weight.shape != (tokens, top) or not expert_of.is_contiguous() or not pair_weight.is_contiguous():
+        raise KernelError(f"experts: expert_of and pair_weight must be contiguous int32 and float32 [{tokens}, top], are {expert_of.dtype} "
+                          f"{tuple(expert_of.shape)} and {pair_weight.dtype} {tuple(pair_weight.shape)}")
+    if tokens * top > MOST_PAIRS or E > 4096:
+        raise KernelError(f"experts: {tokens} tokens of {top} choices among {E} experts are more than {MOST_PAIRS} pairs or 4096 experts")
+    if tokens == 0:
+        return
+    scratch = torch.empty(_scratch_size("ssb_fp4_experts_scratch", tokens, top, E, k, inter), dtype=torch.int8, device=device)
+    _check(_fn("ssb_fp4_experts")(x_at, ldx, _CODES[x.dtype], expert_of.data_ptr(), pair_weight.data_ptr(), first.codes.data_ptr(),
+                                  first.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), o_at, ldo, _CODES[out.dtype],
+                                  tokens, top, E, k, inter, 1 if first.gated else 0, kinds[kind], float(limit), 1 if accumulate else 0,
+                                  scratch.data_ptr(), _error_word(device), _stream()), "fp4_experts")

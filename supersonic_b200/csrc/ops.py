@@ -1740,6 +1740,45 @@ def route_softmax(logits: torch.Tensor, n_experts: int, renormalize: bool, scale
         "route_softmax")
 
 
+SCORES = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = ("max", "two")
+ROUTE_MOST_EXPERTS, ROUTE_MOST_GROUPS = 2048, 32
+
+
+def route_scored(logits: torch.Tensor, n_experts: int, expert_of: torch.Tensor, pair_weight: torch.Tensor, scores: str = "softmax",
+                 correction: Optional[torch.Tensor] = None, groups: int = 1, keep: Optional[int] = None, group_score: str = "two",
+                 renormalize: bool = True, scale: float = 1.0, pdl: bool = False) -> None:
+    """Per token, from float32 router logits [tokens, >= n_experts]: s = softmax(z) over all experts, or sigmoid(z); the ``top`` experts
+    with the largest c = s + ``correction`` (float32 [n_experts]; a bias that only chooses), in order, among the experts of the
+    ``keep`` (all) best of ``groups`` equal groups of neighbours.  A group's score is its largest c (``group_score`` "max") or the sum
+    of its two largest ("two").  pair_weight = s * scale of the chosen, with ``renormalize`` divided by the sum of their s (+ 1e-20).
+    Ties go to the lower index.  A NaN among the logits counts as minus infinity, whose s is zero, an infinite one as the largest number;
+    a c that is NaN comes last."""
+    _need(logits, "logits", torch.float32, 2)
+    _need(expert_of, "expert_of", torch.int32, 2); _need(pair_weight, "pair_weight", torch.float32, 2)
+    T, top = logits.shape[0], expert_of.shape[1]
+    keep = groups if keep is None else keep
+    if logits.shape[1] < n_experts or tuple(expert_of.shape) != (T, top) or tuple(pair_weight.shape) != (T, top) \
+            or not (expert_of.is_contiguous() and pair_weight.is_contiguous()):
+        raise KernelError("route_scored: logits [tokens, >= experts]; expert_of and pair_weight [tokens, top], contiguous")
+    if scores not in SCORES or group_score not in GROUP_SCORES:
+        raise KernelError(f"route_scored: scores {scores!r} of {sorted(SCORES)}, group_score {group_score!r} of {list(GROUP_SCORES)}")
+    if not 1 <= n_experts <= ROUTE_MOST_EXPERTS or not 1 <= groups <= ROUTE_MOST_GROUPS or n_experts % groups or not 1 <= keep <= groups \
+            or not 1 <= top <= keep * (n_experts // groups):
+        raise KernelError(f"route_scored: {top} of {n_experts} experts (up to {ROUTE_MOST_EXPERTS}) in {groups} equal groups (up to "
+                          f"{ROUTE_MOST_GROUPS}), {keep} of them kept")
+    if correction is not None:
+        _need(correction, "correction", torch.float32, 1)
+        if correction.shape[0] != n_experts:
+            raise KernelError("route_scored: one correction per expert")
+    if any(t is not None and t.device.index != torch.cuda.current_device() for t in (logits, expert_of, pair_weight, correction)):
+        raise KernelError("route_scored: tensors must be on the current CUDA device")
+    _check(_fn("expert_ops", "ssb_route_scored")(
+        _ptr(logits), c_int(logits.stride(0)), _ptr(correction), c_int(T), c_int(n_experts), c_int(groups), c_int(keep), c_int(top),
+        c_int(SCORES[scores]), c_int(1 if group_score == "two" else 0), c_int(1 if renormalize else 0), c_float(scale),
+        _ptr(expert_of), _ptr(pair_weight), c_int(1 if pdl else 0), _stream()), "route_scored")
+
+
 def expert_tiles_bound(n_pairs: int, n_experts: int, tile_rows: int) -> int:
     """The most row tiles ``n_pairs`` pairs spread over ``n_experts`` groups can make."""
     return n_pairs // tile_rows + min(n_experts, n_pairs)

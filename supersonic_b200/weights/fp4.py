@@ -1,0 +1,94 @@
+"""A matrix in microscaled 4-bit floats (MXFP4): 32 neighbours along a row share a scale 2^(byte - 127), a number is a sign and one of
+0, 0.5, 1, 1.5, 2, 3, 4, 6.
+
+``codes`` (uint8 ``[n, k / 2]``, of several experts ``[experts, n, k / 2]``) hold two numbers a byte, the earlier one in the low half.
+``scales`` lie in runs of 1,024 bytes for 128 rows and 256 numbers of k, as the tensor cores read them: in a run two halves of four
+blocks, in a half 16 bytes for each of 32 lanes, which are the four blocks of rows lane, lane + 32, lane + 64 and lane + 96.  Rows of a
+run behind the matrix's last and blocks behind its last hold zeros (rows: anything, in matrices of a step's rows).  ``gated``: the
+matrix is a gated unit's first product; of its gate rows and up rows, 16 gate rows and the 16 up rows of the same channels lie in turn.
+
+The modelled project's 4-bit lanes keep int4 codes with a float scale a group (crates/runner/src/llama31_engine.rs:289-430).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+FP4_BLOCK = 32
+_RUN_ROWS, _RUN_BLOCKS = 128, 8
+
+
+class Fp4Matrix:
+    """``shape`` is that of the numbers: (n, k), or (experts, n, k)."""
+
+    __slots__ = ("codes", "scales", "shape", "gated", "_scratch")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, gated: bool = False):
+        shape = tuple(int(s) for s in shape)
+        n, k = shape[-2:] if len(shape) in (2, 3) else (0, 0)
+        if n <= 0 or k <= 0 or k % FP4_BLOCK or min(shape) <= 0:
+            raise ValueError(f"a 4-bit matrix has shape [n, k] or [experts, n, k] with k a multiple of {FP4_BLOCK}, not {shape}")
+        if gated and n % (2 * FP4_BLOCK):
+            raise ValueError(f"a gated unit has as many gate as up rows, a multiple of {FP4_BLOCK} of each; {n} rows in all")
+        runs = (shape[0] if len(shape) == 3 else 1) * -(-n // _RUN_ROWS) * -(-k // (FP4_BLOCK * _RUN_BLOCKS))
+        if codes.dtype != torch.uint8 or tuple(codes.shape) != shape[:-1] + (k // 2,) or not codes.is_contiguous():
+            raise ValueError(f"codes must be contiguous uint8 {shape[:-1] + (k // 2,)}, are {codes.dtype} {tuple(codes.shape)}")
+        if scales.dtype != torch.uint8 or tuple(scales.shape) != (runs, 1024) or not scales.is_contiguous() or scales.device != codes.device:
+            raise ValueError(f"scales must be contiguous uint8 {(runs, 1024)} beside the codes, are {scales.dtype} {tuple(scales.shape)}")
+        self.codes, self.scales, self.shape, self.gated, self._scratch = codes, scales, shape, gated, None
+
+    @classmethod
+    def empty(cls, *shape: int, device="cuda", gated: bool = False) -> "Fp4Matrix":
+        """Zeros of ``shape``, for ``fp4_ops.quantize`` to fill."""
+        if len(shape) not in (2, 3) or min(shape) <= 0 or shape[-1] % FP4_BLOCK:
+            raise ValueError(f"a 4-bit matrix has shape [n, k] or [experts, n, k] with k a multiple of {FP4_BLOCK}, not {shape}")
+        runs = (shape[0] if len(shape) == 3 else 1) * -(-shape[-2] // _RUN_ROWS) * -(-shape[-1] // (FP4_BLOCK * _RUN_BLOCKS))
+        return cls(torch.zeros(shape[:-1] + (shape[-1] // 2,), dtype=torch.uint8, device=device),
+                   torch.zeros((runs, 1024), dtype=torch.uint8, device=device), shape, gated)
+
+    @classmethod
+    def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, gated: bool = False) -> "Fp4Matrix":
+        """From codes as above and scales in rows, uint8 ``[n, k / 32]`` (``[experts, n, k / 32]``), as model files hold them (255, a scale
+        that is no number, is refused).  ``gated``: rows are the gate rows, then the up rows."""
+        shape = tuple(codes.shape[:-1]) + (2 * codes.shape[-1],) if codes.dim() in (2, 3) else ()
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not shape or shape[-1] % FP4_BLOCK \
+                or tuple(scales.shape) != shape[:-1] + (shape[-1] // FP4_BLOCK,) or scales.device != codes.device:
+            raise ValueError(f"codes uint8 [.., n, k / 2] and scales uint8 [.., n, k / {FP4_BLOCK}] on one device, are {codes.dtype} "
+                             f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
+        if bool((scales == 255).any()):
+            raise ValueError("a scale of 255 is no number")
+        if gated:
+            codes, scales = (interleaved(t) for t in (codes, scales))
+        n, blocks = scales.shape[-2:]
+        s = scales.reshape(-1, n, blocks)
+        s = torch.nn.functional.pad(s, (0, -blocks % _RUN_BLOCKS, 0, -n % _RUN_ROWS))
+        # [experts, tile, 4, 32 lanes, k-block, half, 4] -> [experts, tile, k-block, half, lane, 4 rows, 4 blocks]
+        s = s.view(s.shape[0], s.shape[1] // _RUN_ROWS, 4, 32, s.shape[2] // _RUN_BLOCKS, 2, 4).permute(0, 1, 4, 5, 3, 2, 6)
+        return cls(codes.contiguous(), s.reshape(-1, 1024).contiguous(), shape, gated)
+
+    def plain_scales(self) -> torch.Tensor:
+        """The scales in rows, uint8 ``[.., n, k / 32]`` (rows in the order that the codes have)."""
+        n, k = self.shape[-2:]
+        tiles, k_blocks = -(-n // _RUN_ROWS), -(-k // (FP4_BLOCK * _RUN_BLOCKS))
+        s = self.scales.view(-1, tiles, k_blocks, 2, 32, 4, 4).permute(0, 1, 5, 4, 2, 3, 6)
+        s = s.reshape(-1, tiles * _RUN_ROWS, k_blocks * _RUN_BLOCKS)[:, :n, : k // FP4_BLOCK]
+        return s.reshape(self.shape[:-1] + (k // FP4_BLOCK,)).contiguous()
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def bytes_held(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self) -> str:
+        return f"Fp4Matrix({list(self.shape)}{', gated' if self.gated else ''}, {self.device})"
+
+
+def interleaved(t: torch.Tensor) -> torch.Tensor:
+    """Rows (the last but one dimension) that are a gated unit's gate rows, then its up rows: 16 of each in turn."""
+    n = t.shape[-2]
+    if n % 32:
+        raise ValueError(f"{n} rows are not 16 gate and 16 up rows in turn")
+    return t.unflatten(-2, (2, n // 32, 16)).transpose(-4, -3).flatten(-4, -2)
