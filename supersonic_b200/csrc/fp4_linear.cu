@@ -15,7 +15,6 @@
 #include "fp4_codes.cuh"
 #include "packed_call.cuh"
 #include "tc_helpers.cuh"
-#include "tc_rows.cuh"
 #include <algorithm>
 
 typedef __nv_bfloat16 bf16;
@@ -71,6 +70,11 @@ __device__ __forceinline__ void fl_ld16(uint32_t taddr, float (&r)[16]) {
                  : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
                    "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
                  : "r"(taddr) : "memory");
+}
+// An arrival at the pair's leader that orders tensor memory alone (by the tcgen05 fences around it): a release at cluster scope waits
+// for whatever this thread has on its way to or from memory, 1,290 clocks where scales are being fetched ahead.
+__device__ __forceinline__ void fl_arrive_leader(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // Whether any thread of the four epilogue warps says so; all of them meet here (barrier 1).
 __device__ __forceinline__ bool fl_any_of_four(bool mine) {
@@ -408,44 +412,84 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 }
 
 // Tiles of 256 rows x 256 channels on pairs of SMs: each block fetches 128 rows and 128 channels a k-block, its rows' scales and those
-// of all 256 channels (35 KB for 512 clocks of products); the leader issues the pair's instructions, each block's tensor memory gets
-// its 128 rows.  Tensor memory has 512 columns: two accumulators of 256 that share 64 of them, and two sets of 24 for scales.  An
-// epilogue begins with the columns that the next tile wants, so the next tile's products run beside the rest of it.  Tiles go in bands
-// of ``group_m`` row tiles, row tiles fastest.
-constexpr int FL_PAIR_STAGES = 5;
-constexpr int FL_PAIR_STAGE_BYTES = 2 * FL_BM * FL_ROW + 3 * F4_CHUNK;
-constexpr int FL_PAIR_ACC = 192;          // columns from the first accumulator to the second
-constexpr int FL_PAIR_SCALES = 448;       // scales' first column
-constexpr size_t FL_PAIR_SMEM = (size_t)FL_PAIR_STAGES * FL_PAIR_STAGE_BYTES + TC_STAGE_BYTES + (2 * FL_PAIR_STAGES + 3) * 8 + 24 + 1024;
+// of all 256 channels; the leader issues the pair's instructions, each block's tensor memory gets its 128 rows.  Tensor memory has 512
+// columns: two accumulators of 256 that share 128 of them, and five times 24 for a k-block's scales.  An epilogue begins with the
+// columns that the next tile wants, and hands them over as soon as they are in registers.
+//
+// Scales are brought to tensor memory by four warps with tcgen05.st: tcgen05.cp runs in order with the products and took 0.19 us of a
+// k-block's 0.66 (six of them; 8,192 x 14,336 x 4,096: 266 us).  They come through a ring of their own, by cp.async: a TMA copy is behind
+// the codes that were asked for before it, and the way through registers then has to be waited for (357 us).
+//
+// Tiles go in bands of ``group_m`` row tiles, row tiles fastest; of experts (LIST), a list's tile of rows with all its channels.
+constexpr int FL_PAIR_STAGES = 6;
+constexpr int FL_PAIR_STAGE_BYTES = 2 * FL_BM * FL_ROW;
+constexpr int FL_PAIR_RING = 4;           // k-blocks of scales in shared memory
+constexpr int FL_PAIR_SETS = 5;           // and in tensor memory
+constexpr int FL_PAIR_ACC = 128;          // columns from the first accumulator to the second
+constexpr int FL_PAIR_SCALES = 384;       // scales' first column
+constexpr int FL_PAIR_WARPS = 14;         // 0: TMA, 1: MMA + tensor memory, 2-5: scales, 6-13: epilogue
+constexpr int FL_PAIR_PUT = 32 * 20;      // words in which an epilogue warp's rows meet
+constexpr int FL_PAIR_BARS = 2 * FL_PAIR_STAGES + FL_PAIR_SETS + 3;
+constexpr size_t FL_PAIR_SMEM = (size_t)FL_PAIR_STAGES * FL_PAIR_STAGE_BYTES + FL_PAIR_RING * 3 * F4_CHUNK + 8 * FL_PAIR_PUT * 4 + FL_PAIR_BARS * 8 + 24 + 1024;
 
-template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FL_THREADS, 1)
-fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_w,
-                const __grid_constant__ CUtensorMap map_ws, const FlOut o, int m_tiles, int n_tiles, int k_blocks, int group_m,
-                int* __restrict__ error_word) {
+__device__ __forceinline__ void fl_cp16(uint32_t dst, const void* src, bool live) {         // zeros where it is not live
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void fl_st8(uint32_t taddr, const uint4& a, const uint4& b) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+}
+// tc_put_rows with a place for each row: ``at``, the lane's row of dst.
+template <int WORDS, bool ADD>
+__device__ __forceinline__ void fl_put_rows(float* stage, const uint32_t* v, char* dst, size_t row_bytes, int at, int rows) {
+    constexpr int LD = WORDS + 4, PER = WORDS / 4, ROWS = 32 / PER;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < WORDS; j += 4)
+        *reinterpret_cast<uint4*>(stage + lane * LD + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += ROWS) {
+        const int r = r0 + lane / PER, c = lane % PER * 4, row = __shfl_sync(0xffffffffu, at, r);
+        const float4 x = *reinterpret_cast<const float4*>(stage + r * LD + c);
+        if (r < rows) {
+            float4* to = reinterpret_cast<float4*>(dst + (size_t)row * row_bytes) + lane % PER;
+            if (ADD) atomicAdd(to, x);
+            else *to = x;
+        }
+    }
+    __syncwarp();
+}
+
+template <int MODE, bool LIST>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32 * FL_PAIR_WARPS, 1)
+fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const uint8_t* __restrict__ xs,
+                const uint8_t* __restrict__ ws, int x_runs, const FlOut o, const FlTiles list, int m_tiles, int n_tiles, int k_blocks,
+                int group_m, int* __restrict__ error_word) {
     constexpr int BN = 256, STAGES = FL_PAIR_STAGES;
     constexpr uint32_t X_BYTES = FL_BM * FL_ROW, W_BYTES = FL_BM * FL_ROW, STAGE_BYTES = FL_PAIR_STAGE_BYTES;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* put = (float*)(smem + STAGES * STAGE_BYTES);
-    uint64_t* bars = (uint64_t*)(smem + STAGES * STAGE_BYTES + TC_STAGE_BYTES);       // full[STAGES], empty[STAGES], acc_full[2], free
-    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 3);
+    unsigned char* ring = smem + STAGES * STAGE_BYTES;
+    float* put = (float*)(ring + FL_PAIR_RING * 3 * FL_CHUNK);
+    uint64_t* bars = (uint64_t*)(put + 8 * FL_PAIR_PUT);            // full, empty [STAGES], ready [SETS], acc_full[2], free
+    uint32_t* tmem_slot = (uint32_t*)(bars + FL_PAIR_BARS);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();                        // 0: the leader
-    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, tiles = m_tiles * n_tiles;
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
-    const uint32_t acc_full0 = smem_u32(bars + 2 * STAGES), free0 = smem_u32(bars + 2 * STAGES + 2);
-    auto tile_at = [&](int tile, int& m, int& n) {
-        const int band = tile / (group_m * n_tiles), in_band = tile - band * group_m * n_tiles, rows = min(group_m, m_tiles - band * group_m);
-        m = band * group_m + in_band % rows;
-        n = in_band / rows;
-    };
+    const uint32_t ready0 = smem_u32(bars + 2 * STAGES);            // scales are in both blocks' tensor memory: at the leader, as full
+    const uint32_t acc_full0 = ready0 + 8 * FL_PAIR_SETS, free0 = acc_full0 + 16;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < FL_PAIR_SETS; ++s) mbar_init(ready0 + 8 * s, 8);
         for (int i = 0; i < 2; ++i) mbar_init(acc_full0 + 8 * i, 1);
-        mbar_init(free0, 8);
+        mbar_init(free0, 16);
         abort_flag[0] = 0;
         abort_flag[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -459,33 +503,38 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     cluster_sync_all();   // both blocks' barriers are initialised before either signals the other
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    ssb_pdl_wait();       // rows, scales and a list are there
+    if (threadIdx.x == 0) ssb_pdl_launch_dependents();
+    const int tiles = (LIST ? list.meta[0] : m_tiles) * n_tiles;
+    auto tile_at = [&](int tile, int& m, int& n) {
+        if (LIST) { m = tile / n_tiles; n = tile - m * n_tiles; return; }
+        const int band = tile / (group_m * n_tiles), in_band = tile - band * group_m * n_tiles, rows = min(group_m, m_tiles - band * group_m);
+        m = band * group_m + in_band % rows;
+        n = in_band / rows;
+    };
 
     if (warp == 0) {
-        ssb_pdl_wait();
         if (lane == 0) {
-            ssb_pdl_launch_dependents();
             const uint32_t leader_full0 = cluster_map(full0, 0);
             int c = 0;
             for (int tile = pair; tile < tiles && !*abort_flag; tile += n_pairs) {
                 int m, n;
                 tile_at(tile, m, n);
-                const int mt = 2 * m + (int)rank, n0 = n * BN + (int)rank * FL_BM;
+                const int e = LIST ? list.tile_expert[m] : 0;
+                const int mt = 2 * m + (int)rank, n0 = e * o.N + n * BN + (int)rank * FL_BM;
                 for (int kb = 0; kb < k_blocks; ++kb, ++c) {
                     const int s = c % STAGES;
                     const uint32_t x_dst = smem_u32(smem + s * STAGE_BYTES), bar = leader_full0 + 8 * s;
                     if (!mbar_wait(empty0 + 8 * s, ((c / STAGES) & 1) ^ 1, abort_flag)) {
                         *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_PRODUCER); break;
                     }
-                    if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * (X_BYTES + W_BYTES));
                     tma_load_2d_pair(x_dst, &map_x, bar, kb * FL_ROW, mt * FL_BM);
                     tma_load_2d_pair(x_dst + X_BYTES, &map_w, bar, kb * FL_ROW, n0);
-                    tma_load_2d_pair(x_dst + X_BYTES + W_BYTES, &map_xs, bar, 0, mt * k_blocks + kb);
-                    tma_load_2d_pair(x_dst + X_BYTES + W_BYTES + FL_CHUNK, &map_ws, bar, 0, 2 * n * k_blocks + kb);
-                    tma_load_2d_pair(x_dst + X_BYTES + W_BYTES + 2 * FL_CHUNK, &map_ws, bar, 0, (2 * n + 1) * k_blocks + kb);
                 }
             }
             if (*abort_flag) {
-                // let issued copies land: the leader sees both blocks' bytes on its barriers, the other block gives them time
+                // let issued copies land: the leader sees both blocks' codes on its barriers, the other block gives them time
                 if (rank == 0) {
                     for (int i = max(0, c - STAGES); i < c; ++i)
                         mbar_wait(full0 + 8 * (i % STAGES), (i / STAGES) & 1, abort_flag + 1);
@@ -496,50 +545,105 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             }
         }
     } else if (warp == 1) {
-        ssb_pdl_wait();
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc0 = fl_idesc(256, BN, 0), idesc1 = fl_idesc(256, BN, 1);
             bool ok = true;
             int c = 0, i = 0;
             for (int tile = pair; tile < tiles && ok; tile += n_pairs, ++i) {
                 const uint32_t acc = tmem + (i & 1) * FL_PAIR_ACC;
-                if (i > 0 && !mbar_wait(free0, (i - 1) & 1, abort_flag)) {    // both epilogues have drained the shared columns
+                if (i > 0 && !mbar_wait(free0, (i - 1) & 1, abort_flag)) {    // both epilogues have the shared columns
                     *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
                 }
-                tc_fence_after();
                 for (int kb = 0; kb < k_blocks && ok; ++kb, ++c) {
-                    const int s = c % STAGES, before = c - 2;
-                    // this k-block's scales go where those of two k-blocks before were: their products have to be done
-                    if (!mbar_wait(full0 + 8 * s, (c / STAGES) & 1, abort_flag) ||
-                        (before >= 0 && !mbar_wait(empty0 + 8 * (before % STAGES), (before / STAGES) & 1, abort_flag))) {
+                    const int s = c % STAGES, set = c % FL_PAIR_SETS;
+                    if (!mbar_wait(ready0 + 8 * set, (c / FL_PAIR_SETS) & 1, abort_flag) || !mbar_wait(full0 + 8 * s, (c / STAGES) & 1, abort_flag)) {
                         *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
                     }
                     tc_fence_after();
-                    const uint32_t x_addr = smem_u32(smem + s * STAGE_BYTES), s_addr = x_addr + X_BYTES + W_BYTES;
-                    const uint32_t xs = tmem + FL_PAIR_SCALES + (c & 1) * 24, ws = xs + 8;
-                    fl_copy_scales_pair(xs, s_addr);
-                    fl_copy_scales_pair(xs + 4, s_addr + 512);
-                    fl_copy_scales_pair(ws, s_addr + FL_CHUNK);                   // channels 0-127, blocks 0-3
-                    fl_copy_scales_pair(ws + 4, s_addr + 2 * FL_CHUNK);           // channels 128-255
-                    fl_copy_scales_pair(ws + 8, s_addr + FL_CHUNK + 512);         // blocks 4-7
-                    fl_copy_scales_pair(ws + 12, s_addr + 2 * FL_CHUNK + 512);
-                    fl_mma_pair_x4(acc, smem_desc(x_addr), smem_desc(x_addr + X_BYTES), idesc0, idesc1, xs, ws, xs + 4, ws + 8, kb > 0 ? 1u : 0u);
+                    const uint32_t x_addr = smem_u32(smem + s * STAGE_BYTES), x_sc = tmem + FL_PAIR_SCALES + set * 24, w_sc = x_sc + 8;
+                    fl_mma_pair_x4(acc, smem_desc(x_addr), smem_desc(x_addr + X_BYTES), idesc0, idesc1, x_sc, w_sc, x_sc + 4, w_sc + 8, kb > 0 ? 1u : 0u);
                     tc_commit_pair(empty0 + 8 * s, 3);              // the stage is free in both blocks
                 }
                 if (ok) tc_commit_pair(acc_full0 + 8 * (i & 1), 3);
             }
         }
+    } else if (warp < 6) {
+        // a lane's 16 bytes of each 512 are four columns of its lane, in this warp's quarter of the lanes as in the others
+        const uint32_t leader_ready0 = cluster_map(ready0, 0), columns = tmem + FL_PAIR_SCALES + ((uint32_t)(warp & 3) << 21);
+        const int runs = (o.N + FL_BM - 1) / FL_BM, who = threadIdx.x - 64;       // runs of a weight matrix's scales
+        // what is loaded next: k-block ahead_kb of tile ahead_tile; 192 pieces of 16 bytes, a row's run, then two of channels
+        int ahead_tile = pair, ahead_kb = 0, slot_in = 0;
+        const uint8_t *src_x = xs, *src_0 = ws, *src_1 = ws;
+        bool live_x = false, live_1 = false;
+        auto load = [&]() {
+            if (ahead_tile < tiles) {
+                if (ahead_kb == 0) {
+                    int m, n;
+                    tile_at(ahead_tile, m, n);
+                    const int run_x = 2 * m + (int)rank, run_w = (LIST ? list.tile_expert[m] : 0) * runs + 2 * n;
+                    live_x = run_x < x_runs;                        // behind the last run: zeros
+                    live_1 = 2 * n + 1 < runs;
+                    src_x = xs + (size_t)(live_x ? run_x : 0) * k_blocks * FL_CHUNK;
+                    src_0 = ws + (size_t)run_w * k_blocks * FL_CHUNK;
+                    src_1 = live_1 ? src_0 + (size_t)k_blocks * FL_CHUNK : ws;
+                }
+                const size_t at = (size_t)ahead_kb * FL_CHUNK + (who & 63) * 16;
+                const uint32_t dst = smem_u32(ring + slot_in * 3 * FL_CHUNK) + who * 16;
+                fl_cp16(dst, (who < 64 ? src_x : src_0) + at, who < 64 ? live_x : true);
+                if (who < 64) fl_cp16(dst + 2 * FL_CHUNK, src_1 + at, live_1);
+                if (++ahead_kb == k_blocks) { ahead_kb = 0; ahead_tile += n_pairs; }
+            }
+            if (++slot_in == FL_PAIR_RING) slot_in = 0;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int i = 0; i < FL_PAIR_RING - 1; ++i) load();
+        int c = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += n_pairs)
+            for (int kb = 0; kb < k_blocks && ok; ++kb, ++c) {
+                const int slot = c % FL_PAIR_RING, set = c % FL_PAIR_SETS, before = c - FL_PAIR_SETS;
+                asm volatile("cp.async.wait_group %0;" ::"n"(FL_PAIR_RING - 2) : "memory");
+                // the set's last products are done
+                if (before >= 0) ok = mbar_wait(empty0 + 8 * (before % STAGES), (before / STAGES) & 1, abort_flag);
+                // the four warps go on together or not at all; what they copied is there, and the slot before this one has been read
+                uint32_t bad;
+                asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, 2, 128, p;\nselp.b32 %0, 1, 0, q;\n}"
+                             : "=r"(bad) : "r"((uint32_t)!ok) : "memory");
+                ok = !bad;
+                if (!ok) {
+                    if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); }
+                    break;
+                }
+                tc_fence_after();
+                load();
+                const uint4* src = reinterpret_cast<const uint4*>(ring + slot * 3 * FL_CHUNK) + lane;
+                const uint4 x0 = src[0], x1 = src[32], a0 = src[64], a1 = src[96], b0 = src[128], b1 = src[160];
+                fl_st8(columns + set * 24, x0, x1);                 // rows: blocks 0-3, 4-7
+                fl_st8(columns + set * 24 + 8, a0, b0);             // blocks 0-3: channels 0-127, 128-255
+                fl_st8(columns + set * 24 + 16, a1, b1);            // blocks 4-7
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) fl_arrive_leader(leader_ready0 + 8 * set);
+            }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
-        ssb_pdl_wait();
-        const int quarter = warp & 3;
-        float* stage = put + quarter * 32 * TC_STAGE_LD;
+        const int quarter = warp & 3, half = (warp - 6) >> 2;
+        float* stage = put + (warp - 6) * FL_PAIR_PUT;
         const uint32_t leader_free = cluster_map(free0, 0);
         int i = 0;
         for (int tile = pair; tile < tiles; tile += n_pairs, ++i) {
             int m, n;
             tile_at(tile, m, n);
-            const int row0 = (2 * m + (int)rank) * FL_BM + quarter * 32, row = row0 + lane, rows = o.M - row0, buf = i & 1;
-            const float row_scale = MODE == FL_GATED && o.row_scale && row < o.M ? o.row_scale[row] : 1.f;
+            // this warp's 32 rows: the first of them in the matrix (among a list's tiles) and how many there are
+            const int in_tile = (int)rank * FL_BM + quarter * 32, row0 = m * BN + in_tile, row = row0 + lane, buf = i & 1;
+            int rows = o.M - row0, to = row;
+            if (LIST) {
+                const int first = list.tile_row0[m];
+                rows = min(list.offsets[list.tile_expert[m] + 1] - first, BN) - in_tile;
+                if (o.index && lane < rows) to = o.index[first + in_tile + lane];
+            }
+            const float row_scale = MODE == FL_GATED && o.row_scale && lane < rows ? o.row_scale[row] : 1.f;
             bool ok = mbar_wait(acc_full0 + 8 * buf, (i >> 1) & 1, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
@@ -549,29 +653,33 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             tc_fence_after();
             const uint32_t acc = tmem + buf * FL_PAIR_ACC + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-            for (int j = 0; j < 4; ++j) {
-                const int g = buf == 0 ? (j + 3) & 3 : j;            // the shared 64 columns first
+            for (int j = 0; j < 2; ++j) {
+                const int g = half + 2 * (j ^ buf ^ 1);              // the shared 128 columns first
                 uint32_t r[2][32];
                 tc_ld32(acc + g * 64, r[0]);
                 tc_ld32(acc + g * 64 + 32, r[1]);
                 if (j == 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(leader_free);
+                    if (lane == 0) fl_arrive_leader(leader_free);
                 }
+                if (rows <= 0) continue;
                 if (MODE == FL_STORE) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int col = n * BN + g * 64 + h * 32;
-                        if (rows <= 0 || col >= o.N) continue;
+                        if (col >= o.N) continue;
                         const bool whole = col + 32 <= o.N;
                         if (o.is_f32) {
                             if (whole) {
-                                char* dst = (char*)((float*)o.out + (size_t)row0 * o.ldo + col);
-                                if (o.add) tc_put_rows<32, true>(stage, r[h], dst, (size_t)o.ldo * 4, rows);
-                                else tc_put_rows<32, false>(stage, r[h], dst, (size_t)o.ldo * 4, rows);
-                            } else if (row < o.M) {
-                                float* dst = (float*)o.out + (size_t)row * o.ldo + col;
+                                char* dst = (char*)((float*)o.out + col);
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    if (o.add) fl_put_rows<16, true>(stage, r[h] + 16 * q, dst + 64 * q, (size_t)o.ldo * 4, to, rows);
+                                    else fl_put_rows<16, false>(stage, r[h] + 16 * q, dst + 64 * q, (size_t)o.ldo * 4, to, rows);
+                                }
+                            } else if (lane < rows) {
+                                float* dst = (float*)o.out + (size_t)to * o.ldo + col;
 #pragma unroll
                                 for (int e = 0; e < 32; ++e)
                                     if (col + e < o.N) dst[e] = o.add ? dst[e] + __uint_as_float(r[h][e]) : __uint_as_float(r[h][e]);
@@ -584,9 +692,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                                 packed[e / 2] = *reinterpret_cast<const uint32_t*>(&p);
                             }
                             if (whole) {
-                                tc_put_rows<16, false>(stage, packed, (char*)((bf16*)o.out + (size_t)row0 * o.ldo + col), (size_t)o.ldo * 2, rows);
-                            } else if (row < o.M) {
-                                bf16* dst = (bf16*)o.out + (size_t)row * o.ldo + col;
+                                fl_put_rows<16, false>(stage, packed, (char*)((bf16*)o.out + col), (size_t)o.ldo * 2, to, rows);
+                            } else if (lane < rows) {
+                                bf16* dst = (bf16*)o.out + (size_t)to * o.ldo + col;
 #pragma unroll
                                 for (int e = 0; e < 32; ++e)
                                     if (col + e < o.N) dst[e] = __float2bfloat16_rn(__uint_as_float(r[h][e]));
@@ -602,7 +710,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                         float v[32];
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            v[e] = MODE == FL_GATED ? ssb_gate(__uint_as_float(r[e >> 4][e & 15]), __uint_as_float(r[e >> 4][16 + (e & 15)]), o.kind, o.limit) * row_scale
+                            v[e] = MODE == FL_GATED ? ssb_gate_fast(__uint_as_float(r[e >> 4][e & 15]), __uint_as_float(r[e >> 4][16 + (e & 15)]), o.kind, o.limit) * row_scale
                                                     : ssb_activate(__uint_as_float(r[h][e]), o.kind) * o.limit;
                         uint32_t most = f4_most(v);
                         if (most >= F4_WILD) {
@@ -612,14 +720,14 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                         }
                         const int byte = f4_scale_byte(most), k = (n * 4 + g) * 32 * BLOCKS + h * 32;
                         const float inverse = f4_inverse(byte);
-                        if (row < o.M && k < width) {
+                        if (lane < rows && k < width) {
                             *reinterpret_cast<uint4*>((uint8_t*)o.out + (size_t)row * o.ldo + k / 2) =
                                 make_uint4(f4_encode8(v, inverse), f4_encode8(v + 8, inverse), f4_encode8(v + 16, inverse), f4_encode8(v + 24, inverse));
                             o.scales[f4_scale_at(row, k / F4_BLOCK, o.inner_blocks)] = (uint8_t)byte;
                         }
                     }
                     // behind the last channel: scales of zero up to a whole k-block
-                    if (j == 0 && n == n_tiles - 1 && row < o.M)
+                    if (j == 0 && half == 0 && n == n_tiles - 1 && lane < rows)
                         for (int b = width / F4_BLOCK; b < 8 * o.inner_blocks; ++b) o.scales[f4_scale_at(row, b, o.inner_blocks)] = 0;
                 }
             }
@@ -728,34 +836,36 @@ static int fl_stream(const CUtensorMap& mw, const CUtensorMap& mws, const CUtens
                       m_tiles, n_tiles, f4_k_blocks(K), counters, pieces, error_word);
 }
 
-template <int MODE>
-static int fl_pair(const CUtensorMap& mx, const CUtensorMap& mxs, const CUtensorMap& mw, const CUtensorMap& mws, const FlOut& o, const FlPlan& p,
-                   int K, int* error_word, cudaStream_t stream) {
+template <int MODE, bool LIST>
+static int fl_pair(const CUtensorMap& mx, const CUtensorMap& mw, const void* xs, const void* ws, int x_runs, const FlOut& o,
+                   const FlTiles& list, int m_tiles, int n_tiles, int K, int* error_word, cudaStream_t stream) {
     static_assert(FL_PAIR_SMEM <= 227 * 1024, "");
+    auto kernel = fp4_pair_kernel<MODE, LIST>;
     static int max_pairs = 0;
     if (!max_pairs) {
-        cudaError_t e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FL_PAIR_SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FL_PAIR_SMEM);
         if (e != cudaSuccess) return (int)e;
         const int sms = ssb_sm_count();
         // how many pairs the device holds at once (a GPC with an odd SM left over holds one fewer)
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(sms & ~1);
-        cfg.blockDim = dim3(FL_THREADS);
+        cfg.blockDim = dim3(32 * FL_PAIR_WARPS);
         cfg.dynamicSmemBytes = FL_PAIR_SMEM;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr; cfg.numAttrs = 1;
         int clusters = 0;
-        if (cudaOccupancyMaxActiveClusters(&clusters, fp4_pair_kernel<MODE>, &cfg) != cudaSuccess || clusters <= 0) {
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters <= 0) {
             cudaGetLastError();
             clusters = sms / 2;
         }
         max_pairs = std::min(clusters, sms / 2);
     }
-    const int pairs = std::min(p.m_tiles * p.n_tiles, max_pairs);
-    return ssb_launch(fp4_pair_kernel<MODE>, dim3(2 * pairs), dim3(FL_THREADS), FL_PAIR_SMEM, stream, true, mx, mxs, mw, mws, o, p.m_tiles,
-                      p.n_tiles, f4_k_blocks(K), std::min(16, p.m_tiles), error_word);
+    const int pairs = (int)std::min<long long>((long long)m_tiles * n_tiles, max_pairs);
+    return ssb_launch(kernel, dim3(2 * pairs), dim3(32 * FL_PAIR_WARPS), FL_PAIR_SMEM, stream, true, mx, mw, (const uint8_t*)xs,
+                      (const uint8_t*)ws, x_runs, o, list, m_tiles,
+                      n_tiles, f4_k_blocks(K), std::min(16, m_tiles), error_word);
 }
 
 template <int MODE>
@@ -775,7 +885,7 @@ static int fl_dense(const void* x, const void* xs, const void* w, const void* ws
         case 64: return fl_stream<64, 8, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
         case 128: return fl_stream<128, 6, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
     }
-    return fl_pair<MODE>(mx, mxs, mw, mws, o, p, K, error_word, stream);
+    return fl_pair<MODE, false>(mx, mw, xs, ws, (o.M + 127) / 128, o, none, p.m_tiles, p.n_tiles, K, error_word, stream);
 }
 
 SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* codes, void* scales, int rows, int K, int per_expert, int inter,
@@ -921,7 +1031,7 @@ fp4_combine_kernel(const float* __restrict__ y, const int* __restrict__ slot, co
 // Rows a tile, by how many an expert has on average: no more than the step has tokens, and little of a tile empty.
 static int fl_list_rows(int tokens, int top, int experts) {
     const long long mean = (long long)tokens * top / experts;
-    return tokens <= 16 || mean <= 8 ? 16 : tokens <= 32 || mean <= 16 ? 32 : tokens <= 64 || mean <= 48 ? 64 : 128;
+    return tokens <= 16 || mean <= 8 ? 16 : tokens <= 32 || mean <= 16 ? 32 : tokens <= 64 || mean <= 48 ? 64 : mean <= 96 ? 128 : 256;
 }
 struct FlExperts {
     int bn, tiles, blocks;                 // rows a tile, tiles at most, blocks of a product
@@ -931,7 +1041,7 @@ struct FlExperts {
         bn = fl_list_rows(tokens, top, experts);
         tiles = pairs / bn + std::min(experts, pairs);
         blocks = ssb_sm_count();
-        const size_t rows = (size_t)tiles * bn, chunks = (size_t)tiles * F4_CHUNK;
+        const size_t rows = (size_t)tiles * bn, chunks = (size_t)tiles * (bn > 128 ? 2 : 1) * F4_CHUNK;
         size_t at = 0;
         auto take = [&](size_t bytes) { const size_t was = at; at += fl_round(bytes); return was; };
         counters = take(2 * FL_COUNTERS * 4);
@@ -946,7 +1056,7 @@ struct FlExperts {
         z = take(rows * (inter / 2));
         zs = take(chunks * f4_k_blocks(inter));
         y = take((size_t)pairs * K * 4);
-        pieces = take((size_t)blocks * 2 * bn * FL_BM * 4);
+        pieces = bn <= 128 ? take((size_t)blocks * 2 * bn * FL_BM * 4) : at;
         all = at;
     }
 };
@@ -960,17 +1070,18 @@ static int fl_listed(const void* x, const void* xs, const void* w, const void* w
                      int experts, int K, int* counters, float* pieces, int* error_word, cudaStream_t stream) {
     const int k_blocks = f4_k_blocks(K), n_tiles = (o.N + FL_BM - 1) / FL_BM;
     CUtensorMap mw, mws, mx, mxs;
-    int rc = fl_map(&mx, x, (long long)at.tiles * at.bn, K / 2, at.bn);
+    int rc = fl_map(&mx, x, (long long)at.tiles * at.bn, K / 2, std::min(at.bn, FL_BM));
     if (!rc) rc = fl_map(&mw, w, (long long)experts * o.N, K / 2, FL_BM);
-    if (!rc) rc = fl_scale_map(&mxs, xs, (long long)at.tiles * k_blocks);
+    if (!rc) rc = fl_scale_map(&mxs, xs, (long long)at.tiles * (at.bn > 128 ? 2 : 1) * k_blocks);
     if (!rc) rc = fl_scale_map(&mws, ws, (long long)experts * n_tiles * k_blocks);
     if (rc) return rc;
     switch (at.bn) {
         case 16: return fl_stream<16, 10, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
         case 32: return fl_stream<32, 9, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
         case 64: return fl_stream<64, 8, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+        case 128: return fl_stream<128, 6, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
     }
-    return fl_stream<128, 6, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+    return fl_pair<MODE, true>(mx, mw, xs, ws, 2 * at.tiles, o, list, at.tiles, (o.N + 255) / 256, K, error_word, stream);
 }
 
 // out[t] (+)= sum_j weight[t, j] E(x_t) of expert expert_of[t, j]; w1: [experts][N1][K], w2: [experts][K][inter].

@@ -9,7 +9,7 @@ constexpr int FR_THREADS = 256;
 constexpr int FR_TURNS = 4;               // units a half-warp has in flight
 
 // Where a row goes: row r of a matrix of several experts' rows, or (slot) pair r's row, a copy of its token's, in tiles of ``tile_rows``
-// whose scales have a run of 128 rows each.
+// whose scales have runs of their own.
 struct FrRows {
     int per_expert, inter;                 // rows of a matrix; of a gated unit's first, how many of them are gate rows
     const int* slot; int top, tile_rows;
@@ -63,7 +63,7 @@ fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict_
                 at = to.slot[row];
                 if (at < 0) continue;
                 const int tile = (int)at / to.tile_rows;
-                r = tile * 128 + (int)at - tile * to.tile_rows;
+                r = tile * max(to.tile_rows, 128) + (int)at - tile * to.tile_rows;
             } else {
                 const int expert = row / to.per_expert;
                 r = f4_laid_row(row - expert * to.per_expert, to.inter);
