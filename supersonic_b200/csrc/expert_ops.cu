@@ -9,6 +9,7 @@
 // nothing to do.  An expert's output rows are written per pair and summed per token in the order
 // of the choices, so no result depends on the other tokens of the step.
 #include "common.cuh"
+#include "packed_call.cuh"
 #include <math.h>
 
 typedef __nv_bfloat16 bf16;
@@ -233,9 +234,9 @@ SSB_API int ssb_route_softmax(float* z, int ld, const float* bias, int n_tokens,
 //
 // What is chosen is chosen by c in 64 bits.  c in 32 bits is within RS_NEAR of it, so a warp (a token, its experts in registers)
 // chooses in 32 bits and looks whether two neighbours of its order, the last chosen and the next among them, or a kept and a
-// dropped group, are closer than that: only then (a token in some hundreds) it computes and chooses again in 64 bits, one expert
-// after another.  Without correction c grows with z, and the order is z's own.
-// 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: see the figures at the launch.
+// dropped group, are closer than that: only then (a token in some hundreds) it computes and chooses again in 64 bits.  Without
+// correction c grows with z, and the order is z's own.
+// 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: RS_FIGURE
 // ---------------------------------------------------------------------------------------
 constexpr int RS_MOST_GROUPS = 32;
 enum { RS_SOFTMAX = 0, RS_SIGMOID = 1 };
@@ -258,42 +259,37 @@ __device__ __forceinline__ uint32_t rs_key(float x) {
 }
 __device__ __forceinline__ float rs_from_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// All of it in 64 bits, for a token whose choice is close.  ``most``, ``total``: of the softmax.
-__device__ __noinline__ void rs_choose_exactly(const RsArgs& a, const float* zr, int* chosen, int lane) {
+// All of it in 64 bits, for a token whose choice is close.  ``c``: room for the experts' choice scores.
+__device__ __noinline__ void rs_choose_exactly(const RsArgs& a, const float* zr, double* c, int* chosen, int lane) {
     double most = -INFINITY, total = 0.0;
     if (a.kind == RS_SOFTMAX) {
         for (int e = lane; e < a.n_experts; e += 32) most = fmax(most, (double)rs_logit(zr[e]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
-        if (most > -INFINITY)
-            for (int e = lane; e < a.n_experts; e += 32) total += exp((double)rs_logit(zr[e]) - most);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
-    auto choice = [&](int e) -> double {
+    for (int e = lane; e < a.n_experts; e += 32) {
         const double z = (double)rs_logit(zr[e]);
-        double s = 0.0;
-        if (z > -INFINITY) s = a.kind == RS_SOFTMAX ? exp(z - most) / total : 1.0 / (1.0 + exp(-z));
-        const double c = s + (a.correction ? (double)a.correction[e] : 0.0);
-        return c != c ? -INFINITY : c;
-    };
+        c[e] = !(z > -INFINITY) ? 0.0 : a.kind == RS_SOFTMAX ? exp(z - most) : 1.0 / (1.0 + exp(-z));
+        total += c[e];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int e = lane; e < a.n_experts; e += 32) {
+        double v = a.kind == RS_SOFTMAX && total > 0.0 ? c[e] / total : c[e];
+        if (a.correction) v += (double)a.correction[e];
+        c[e] = v != v ? -INFINITY : v;
+    }
+    __syncwarp();
     const int per = a.n_experts / a.n_groups;
     uint32_t stays = 0xffffffffu;
     if (a.keep < a.n_groups) {
         double score = -INFINITY;                         // lane g: group g's
-        for (int g = 0; g < a.n_groups; ++g) {
+        if (lane < a.n_groups) {
             double first = -INFINITY, second = -INFINITY;
-            for (int e = g * per + lane; e < (g + 1) * per; e += 32) {
-                const double c = choice(e);
-                if (c > first) { second = first; first = c; } else if (c > second) second = c;
+            for (int e = lane * per; e < (lane + 1) * per; ++e) {
+                if (c[e] > first) { second = first; first = c[e]; } else if (c[e] > second) second = c[e];
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const double f = __shfl_xor_sync(0xffffffffu, first, o), s = __shfl_xor_sync(0xffffffffu, second, o);
-                second = fmax(fmin(first, f), fmax(second, s));
-                first = fmax(first, f);
-            }
-            if (lane == g) score = a.by_two && per > 1 ? first + second : first;
+            score = a.by_two && per > 1 ? first + second : first;
         }
         int before = 0;
         for (int g = 0; g < a.n_groups; ++g) {
@@ -308,15 +304,14 @@ __device__ __noinline__ void rs_choose_exactly(const RsArgs& a, const float* zr,
         double best = -INFINITY;
         int best_e = 0x7fffffff;
         for (int e = lane; e < a.n_experts; e += 32) {
-            if (!(stays >> (e / per) & 1)) continue;
-            const double c = choice(e);
-            if ((c < last || (c == last && e > last_e)) && (best_e == 0x7fffffff || c > best)) { best = c; best_e = e; }
+            const double v = c[e];
+            if ((stays >> (e / per) & 1) && (v < last || (v == last && e > last_e)) && (best_e == 0x7fffffff || v > best)) { best = v; best_e = e; }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            const double c = __shfl_xor_sync(0xffffffffu, best, o);
+            const double v = __shfl_xor_sync(0xffffffffu, best, o);
             const int e = __shfl_xor_sync(0xffffffffu, best_e, o);
-            if (e != 0x7fffffff && (best_e == 0x7fffffff || c > best || (c == best && e < best_e))) { best = c; best_e = e; }
+            if (e != 0x7fffffff && (best_e == 0x7fffffff || v > best || (v == best && e < best_e))) { best = v; best_e = e; }
         }
         last = best;
         last_e = best_e;
@@ -325,20 +320,26 @@ __device__ __noinline__ void rs_choose_exactly(const RsArgs& a, const float* zr,
     __syncwarp();
 }
 
+// A warp's shared memory.
+__host__ __device__ __forceinline__ int rs_doubles(int n_experts, int n_groups, int top) {
+    const int members = (n_experts + 4 * n_groups + 1) / 2;
+    return (members > n_experts ? members : n_experts) + (top + 1) / 2;
+}
+
 // PER: experts a lane (expert j * 32 + lane).
 template <int PER>
 __global__ void __launch_bounds__(RG_THREADS)
 route_scored_kernel(const RsArgs a) {
-    extern __shared__ float rsc_smem[];                  // per warp: [top] chosen experts, [n_experts + 4 * n_groups] scores of groups' members
+    extern __shared__ double rsc_smem[];                 // per warp: [n_experts] scores in 64 bits, over them in 32 bits groups' members; [top] chosen
     ssb_pdl_launch_dependents();
     ssb_pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x * (RG_THREADS / 32) + warp;
     if (t >= a.n_tokens) return;
     const bool grouped = a.keep < a.n_groups;
-    const int words = a.top + (grouped ? a.n_experts + 4 * a.n_groups : 0);
-    int* chosen = (int*)rsc_smem + (size_t)warp * words;
-    float* member = (float*)(chosen + a.top);
+    double* exact = rsc_smem + (size_t)warp * rs_doubles(a.n_experts, a.n_groups, a.top);
+    float* member = (float*)exact;
+    int* chosen = (int*)(exact + rs_doubles(a.n_experts, a.n_groups, 0));
     const float* zr = a.z + (size_t)t * a.ld;
     float z[PER];
 #pragma unroll
@@ -436,7 +437,7 @@ route_scored_kernel(const RsArgs a) {
         if (lane == 0) chosen[k] = at;
     }
     __syncwarp();
-    if (near) rs_choose_exactly(a, zr, chosen, lane);
+    if (near) rs_choose_exactly(a, zr, exact, chosen, lane);
     float sum = 0.f;
     for (int k = lane; k < a.top; k += 32) sum += score(rs_logit(zr[chosen[k]]));
 #pragma unroll
@@ -451,7 +452,7 @@ route_scored_kernel(const RsArgs a) {
 
 template <int PER>
 static int rs_launch(const RsArgs& a, int pdl, cudaStream_t stream) {
-    const size_t smem = (size_t)(RG_THREADS / 32) * (a.top + (a.keep < a.n_groups ? a.n_experts + 4 * a.n_groups : 0)) * sizeof(float);
+    const size_t smem = (size_t)(RG_THREADS / 32) * rs_doubles(a.n_experts, a.n_groups, a.top) * sizeof(double);
     if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(route_scored_kernel<PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
@@ -474,6 +475,7 @@ SSB_API int ssb_route_scored(const float* z, int ld, const float* correction, in
     if (n_experts <= 512) return rs_launch<16>(a, pdl, stream);
     return rs_launch<64>(a, pdl, stream);
 }
+SSB_PACKED(ssb_route_scored)
 
 // ---------------------------------------------------------------------------------------
 // pairs sorted by expert.  One block: counts in shared memory, offsets and the tile list by one

@@ -5,6 +5,7 @@
 // 16 bytes for each of 32 lanes, which are the 4 blocks of rows lane, lane + 32, lane + 64, lane + 96.
 #pragma once
 #include "common.cuh"
+#include <cuda_fp16.h>
 
 constexpr int F4_BLOCK = 32;              // numbers a scale
 constexpr int F4_KB = 256;                // numbers a k-block: 128 bytes of codes, one swizzle row
@@ -45,10 +46,24 @@ __device__ __forceinline__ uint32_t f4_encode8(const float* x, float inverse) {
                     "f"(x[5] * inverse), "f"(x[6] * inverse), "f"(x[7] * inverse));
     return w;
 }
-__device__ __forceinline__ float f4_value(uint32_t code) {
-    const uint32_t m = code & 7;
-    const float v = m < 4 ? 0.5f * (float)m : m < 6 ? (float)m - 2.f : 2.f * (float)m - 8.f;
-    return code & 8 ? -v : v;
+// One code, in the low four bits.
+__device__ __forceinline__ uint32_t f4_encode1(float x) {
+    uint32_t w;
+    asm("{\n.reg .b8 a;\ncvt.rn.satfinite.e2m1x2.f32 a, %1, %2;\nmov.b32 %0, {a, 0, 0, 0};\n}" : "=r"(w) : "f"(0.f), "f"(x));
+    return w;
+}
+// Eight codes' values times ``scale``.
+__device__ __forceinline__ void f4_values8(uint32_t codes, float scale, float* v) {
+    uint32_t h[4];
+    asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %4;\ncvt.rn.f16x2.e2m1x2 %0, a;\ncvt.rn.f16x2.e2m1x2 %1, b;\n"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\ncvt.rn.f16x2.e2m1x2 %3, d;\n}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(codes));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(h + i));
+        v[2 * i] = f.x * scale;
+        v[2 * i + 1] = f.y * scale;
+    }
 }
 
 __device__ __forceinline__ void f4_load8(const __nv_bfloat16* p, float* x) {

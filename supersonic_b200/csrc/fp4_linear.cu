@@ -4,7 +4,7 @@
 // 128 rows x 4 blocks to four columns, in all four lane quarters), where the instructions read them.  Products of codes and their scales
 // are exact; sums are float32 in tensor memory.
 //
-// Two kernels:
+// Two kernels here (and one for up to 16 rows in fp4_few.cu):
 //  * where the weights' bytes or the number of tiles is what bounds it: weights on the M side (128 of them a tile), rows of x on the
 //    N side, and the k-blocks of all tiles dealt out over the SMs, in equal parts of tiles or wherever a tile ends; the same for experts,
 //    whose tiles of rows a list in memory names;
@@ -13,6 +13,7 @@
 // What becomes of the sums: stored, added in float32, or (an inner row of a feed-forward) through an activation or a gated unit's inner
 // step and into 4 bits at once, from the float32 sums.
 #include "fp4_codes.cuh"
+#include "fp4_few.cuh"
 #include "packed_call.cuh"
 #include "tc_helpers.cuh"
 #include <algorithm>
@@ -815,9 +816,18 @@ struct FlScratch {
         all = pieces + std::max<size_t>(piece_bytes, 16);
     }
 };
-SSB_API long long ssb_fp4_linear_scratch(int M, int N, int K, int numbers) {
+// Rows that come as numbers and run in the kernel of few rows are quantised by each of its blocks, up to this many numbers: us with
+// and without a launch of their own, see fl_product.
+constexpr long long FL_FUSED_NUMBERS = 32768;
+
+// Twice the bytes of scratch that a product needs, and one if it needs counters.  numbers: rows come as numbers; mode: FL_*.
+SSB_API long long ssb_fp4_product_scratch(int M, int N, int K, int numbers, int mode) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return (long long)FlScratch(M, K, numbers != 0, fl_plan(M, N, K).pieces).all;
+    if (fw_takes(M, N, K, mode)) {
+        if (!numbers || (long long)M * K <= FL_FUSED_NUMBERS) return 0;
+        return 2 * (long long)FlScratch(M, K, true, 0).all;
+    }
+    return 2 * (long long)FlScratch(M, K, numbers != 0, fl_plan(M, N, K).pieces).all + 1;
 }
 
 template <int BN, int STAGES, int MODE, bool LIST>
@@ -894,23 +904,36 @@ SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void
                                    const int* slot, int tile_rows, cudaStream_t stream);
 
 // A product of dense weights.  x: rows of dtype (ldx elements apart), which are quantised first, or (dtype -1) codes with the scales xs.
-// counters: FL_COUNTERS words (``n_clear`` of them and behind them are zeroed on the way where x is quantised; else the launch needs
-// them zero); the launch leaves them zero.  scratch: ssb_fp4_linear_scratch bytes.
+// scratch: ssb_fp4_product_scratch bytes.  counters: FL_COUNTERS words (``n_clear`` of them and behind them are zeroed on the way where x
+// is quantised; else the launch needs them zero); the launch leaves them zero.
 template <int MODE>
 static int fl_product(const void* x, long long ldx, int dtype, const void* xs, const void* w, const void* ws, const FlOut& o, int K,
                       void* scratch, int* counters, int n_clear, int* error_word, cudaStream_t stream) {
-    if (o.M < 0 || o.N <= 0 || K <= 0 || K % F4_BLOCK || o.N % 8 || !scratch || !counters || !error_word) return SSB_ERR_BAD_SIZE;
+    if (o.M < 0 || o.N <= 0 || K <= 0 || K % F4_BLOCK || o.N % 8 || dtype > SSB_BF16) return SSB_ERR_BAD_SIZE;
     if (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws | (uintptr_t)o.out | (uintptr_t)o.scales | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
     if (o.M == 0) return 0;
-    const FlPlan p = fl_plan(o.M, o.N, K);
+    const bool few = fw_takes(o.M, o.N, K, MODE), first = dtype >= 0 && !(few && (long long)o.M * K <= FL_FUSED_NUMBERS);
+    if (((first || !few) && !scratch) || (!few && (!counters || !error_word))) return SSB_ERR_BAD_SIZE;
+    const FlPlan p = few ? FlPlan{} : fl_plan(o.M, o.N, K);
     if (p.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
     const FlScratch at(o.M, K, dtype >= 0, p.pieces);
     char* base = (char*)scratch;
-    if (dtype >= 0) {
-        const int rc = ssb_fp4_quantize(x, ldx, dtype, base + at.codes, base + at.scales, o.M, K, o.M, 0, counters, n_clear, stream);
+    if (first) {
+        const int rc = ssb_fp4_quantize(x, ldx, dtype, base + at.codes, base + at.scales, o.M, K, o.M, 0, few ? nullptr : counters,
+                                        few ? 0 : n_clear, stream);
         if (rc) return rc;
         x = base + at.codes;
         xs = base + at.scales;
+        dtype = -1;
+    }
+    if (few) {
+        FwArgs a{};
+        a.w = (const uint8_t*)w; a.ws = (const uint8_t*)ws;
+        a.x = x; a.ldx = ldx; a.dtype = dtype; a.xs = (const uint8_t*)xs;
+        a.out = o.out; a.out_scales = o.scales; a.ldo = o.ldo; a.is_f32 = o.is_f32; a.add = o.add;
+        a.M = o.M; a.N = o.N; a.K = K;
+        a.kind = o.kind; a.limit = o.limit; a.row_scale = o.row_scale; a.inner_blocks = o.inner_blocks;
+        return fw_product(a, MODE, stream);
     }
     return fl_dense<MODE>(x, xs, w, ws, o, K, counters, (float*)(base + at.pieces), p, error_word, stream);
 }
@@ -999,8 +1022,8 @@ fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int 
 // out[t] (+)= sum over the choices j, in their order, of weight[t, j] * y[t, j]; choices of no expert count nothing.
 template <typename T>
 __global__ void __launch_bounds__(256)
-fp4_combine_kernel(const float* __restrict__ y, const int* __restrict__ slot, const float* __restrict__ weight, T* __restrict__ out,
-                   long long ldo, int tokens, int top, int width, int add) {
+fp4_combine_kernel(const float* __restrict__ y, const int* __restrict__ expert_of, int experts, const float* __restrict__ weight,
+                   T* __restrict__ out, long long ldo, int tokens, int top, int width, int add) {
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
     const int per_row = width / 8;
@@ -1010,7 +1033,7 @@ fp4_combine_kernel(const float* __restrict__ y, const int* __restrict__ slot, co
         float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int j = 0; j < top; ++j) {
             const int pair = t * top + j;
-            if (slot[pair] < 0) continue;
+            if ((unsigned)expert_of[pair] >= (unsigned)experts) continue;
             const float w = weight[pair];
             float v[8];
             f4_load8(y + (size_t)pair * width + c, v);
@@ -1036,8 +1059,17 @@ static int fl_list_rows(int tokens, int top, int experts) {
 struct FlExperts {
     int bn, tiles, blocks;                 // rows a tile, tiles at most, blocks of a product
     size_t counters, offsets, order, slot, tile_expert, tile_row0, meta, x, xs, z, zs, y, pieces, all;
-    FlExperts(int tokens, int top, int experts, int K, int inter) {
-        const int pairs = tokens * top;
+    bool few;                              // by the kernel of few rows, which needs no list
+    FlExperts(int tokens, int top, int experts, int K, int inter, bool gated) {
+        const int pairs = tokens * top, N1 = gated ? 2 * inter : inter;
+        few = fw_takes_list(pairs, experts, N1, K, gated ? FL_GATED : FL_ACT) && fw_takes_list(pairs, experts, K, inter, FL_STORE);
+        if (few) {
+            z = 0;
+            zs = fl_round((size_t)pairs * (inter / 2));
+            y = zs + fl_round((size_t)((pairs + 127) / 128) * f4_k_blocks(inter) * F4_CHUNK);
+            all = y + fl_round((size_t)pairs * K * 4);
+            return;
+        }
         bn = fl_list_rows(tokens, top, experts);
         tiles = pairs / bn + std::min(experts, pairs);
         blocks = ssb_sm_count();
@@ -1060,9 +1092,9 @@ struct FlExperts {
         all = at;
     }
 };
-SSB_API long long ssb_fp4_experts_scratch(int tokens, int top, int experts, int K, int inter) {
+SSB_API long long ssb_fp4_experts_scratch(int tokens, int top, int experts, int K, int inter, int gated) {
     if (tokens <= 0 || top <= 0 || experts <= 0 || K <= 0 || inter <= 0) return 0;
-    return (long long)FlExperts(tokens, top, experts, K, inter).all;
+    return (long long)FlExperts(tokens, top, experts, K, inter, gated != 0).all;
 }
 
 template <int MODE>
@@ -1093,29 +1125,47 @@ SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* 
     if (((uintptr_t)x | (uintptr_t)w1 | (uintptr_t)ws1 | (uintptr_t)w2 | (uintptr_t)ws2 | (uintptr_t)out | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
     if ((dtype != SSB_F32 && dtype != SSB_BF16) || (out_dtype != SSB_F32 && out_dtype != SSB_BF16) || (add && out_dtype != SSB_F32)) return SSB_ERR_BAD_DTYPE;
     if (tokens == 0) return 0;
-    const FlExperts at(tokens, top, experts, K, inter);
-    if (at.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
+    const FlExperts at(tokens, top, experts, K, inter, gated != 0);
     char* base = (char*)scratch;
-    auto ints = [&](size_t o) { return (int*)(base + o); };
-    const int pairs = tokens * top;
-    int rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(1024), (size_t)experts * 12, stream, true, expert_of, pairs, experts, at.bn, ints(at.offsets),
+    const int pairs = tokens * top, N1 = gated ? 2 * inter : inter;
+    float* y = (float*)(base + at.y);
+    int rc;
+    if (at.few) {
+        FwArgs a{};
+        a.w = (const uint8_t*)w1; a.ws = (const uint8_t*)ws1;
+        a.x = x; a.ldx = ldx; a.dtype = dtype;
+        a.out = base + at.z; a.out_scales = (uint8_t*)(base + at.zs); a.ldo = inter / 2;
+        a.M = tokens; a.N = N1; a.K = K;
+        a.kind = kind; a.limit = limit; a.inner_blocks = f4_k_blocks(inter);
+        a.expert_of = expert_of; a.pairs = pairs; a.top = top; a.experts = experts;
+        rc = fw_product_list(a, gated ? FL_GATED : FL_ACT, stream);
+        if (rc) return rc;
+        a.w = (const uint8_t*)w2; a.ws = (const uint8_t*)ws2;
+        a.x = base + at.z; a.dtype = -1; a.xs = (const uint8_t*)(base + at.zs);
+        a.out = y; a.ldo = K; a.is_f32 = 1;
+        a.N = K; a.K = inter;
+        rc = fw_product_list(a, FL_STORE, stream);
+    } else {
+        if (at.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
+        auto ints = [&](size_t o) { return (int*)(base + o); };
+        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(1024), (size_t)experts * 12, stream, true, expert_of, pairs, experts, at.bn, ints(at.offsets),
                         ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta), ints(at.counters), 2 * FL_COUNTERS);
-    if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, pairs, top, K, ints(at.slot), at.bn, stream);
+        if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, pairs, top, K, ints(at.slot), at.bn, stream);
+        if (rc) return rc;
+        const FlTiles list{ints(at.offsets), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta)};
+        float* pieces = (float*)(base + at.pieces);
+        const FlOut first{base + at.z, (uint8_t*)(base + at.zs), nullptr, nullptr, inter / 2, 0, 0, tokens, N1, kind, limit, f4_k_blocks(inter)};
+        rc = gated ? fl_listed<FL_GATED>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream)
+                   : fl_listed<FL_ACT>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream);
+        if (rc) return rc;
+        const FlOut second{y, nullptr, ints(at.order), nullptr, K, 1, 0, tokens, K, 0, 0.f, 0};
+        rc = fl_listed<FL_STORE>(base + at.z, base + at.zs, w2, ws2, second, list, at, experts, inter, ints(at.counters) + FL_COUNTERS, pieces, error_word, stream);
+    }
     if (rc) return rc;
-    const FlTiles list{ints(at.offsets), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta)};
-    float* pieces = (float*)(base + at.pieces);
-    const FlOut first{base + at.z, (uint8_t*)(base + at.zs), nullptr, nullptr, inter / 2, 0, 0, tokens, gated ? 2 * inter : inter, kind, limit, f4_k_blocks(inter)};
-    rc = gated ? fl_listed<FL_GATED>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream)
-               : fl_listed<FL_ACT>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream);
-    if (rc) return rc;
-    const FlOut second{base + at.y, nullptr, ints(at.order), nullptr, K, 1, 0, tokens, K, 0, 0.f, 0};
-    rc = fl_listed<FL_STORE>(base + at.z, base + at.zs, w2, ws2, second, list, at, experts, inter, ints(at.counters) + FL_COUNTERS, pieces, error_word, stream);
-    if (rc) return rc;
-    const float* y = (const float*)(base + at.y);
     const dim3 grid((unsigned)std::min<long long>(((long long)tokens * (K / 8) + 255) / 256, 8 * ssb_sm_count()));
     if (out_dtype == SSB_BF16)
-        return ssb_launch(fp4_combine_kernel<bf16>, grid, dim3(256), 0, stream, true, y, ints(at.slot), weight, (bf16*)out, ldo, tokens, top, K, add);
-    return ssb_launch(fp4_combine_kernel<float>, grid, dim3(256), 0, stream, true, y, ints(at.slot), weight, (float*)out, ldo, tokens, top, K, add);
+        return ssb_launch(fp4_combine_kernel<bf16>, grid, dim3(256), 0, stream, true, (const float*)y, expert_of, experts, weight, (bf16*)out, ldo, tokens, top, K, add);
+    return ssb_launch(fp4_combine_kernel<float>, grid, dim3(256), 0, stream, true, (const float*)y, expert_of, experts, weight, (float*)out, ldo, tokens, top, K, add);
 }
 
 SSB_PACKED(ssb_fp4_linear)

@@ -33,8 +33,8 @@ _SIGNATURES = {
     "ssb_fp4_linear": [_P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P],
     "ssb_fp4_inner": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P],
     "ssb_fp4_experts": [_P, _L, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
-    "ssb_fp4_linear_scratch": [_I] * 4,
-    "ssb_fp4_experts_scratch": [_I] * 5,
+    "ssb_fp4_product_scratch": [_I] * 5,
+    "ssb_fp4_experts_scratch": [_I] * 6,
 }
 _FORMATS = {_P: "P", _I: "i", _F: "f", _L: "q"}
 _functions = {}
@@ -74,45 +74,48 @@ def _scratch_size(name: str, *sizes) -> int:
     return n
 
 
-def _here(*tensors) -> torch.device:
-    """The current device, on which all of these have to be."""
-    device = tensors[0].device
-    if device.type != "cuda" or device.index != torch.cuda.current_device() or any(t.device != device for t in tensors):
-        raise KernelError(f"tensors must be on the current CUDA device, are on {sorted({str(t.device) for t in tensors})}")
-    return device
+def _here(*indices) -> None:
+    """Raises unless these device indices (-1: no CUDA device) are the current device's."""
+    current = torch.cuda.current_device()
+    for i in indices:
+        if i != current:
+            raise KernelError(f"tensors must be on the current CUDA device {current}, are on {sorted(set(indices))}")
 
 
 def _matrix_rows(t: torch.Tensor, name: str, m: Fp4Matrix):
-    """(address, row stride, rows) of a tensor of a 4-bit matrix's shape, all its rows equally far apart."""
-    if tuple(t.shape) != m.shape or t.dtype not in _CODES or not t.is_cuda:
-        raise KernelError(f"{name} must be float32 or bfloat16 {m.shape} on a CUDA device, is {t.dtype} {tuple(t.shape)}")
-    if t.dim() == 3:
+    """(address, row stride, rows, type code) of a tensor of a 4-bit matrix's shape, all its rows equally far apart."""
+    shape = t.shape
+    if shape != m.shape or t.dtype not in _CODES or t.get_device() != m.index:
+        raise KernelError(f"{name} must be float32 or bfloat16 {m.shape} on the matrix's device, is {t.dtype} {tuple(shape)} on {t.device}")
+    _here(m.index)
+    if len(shape) == 3:
         if not t.is_contiguous():
             raise KernelError(f"{name}: matrices of several experts are contiguous")
-        t = t.view(-1, t.shape[-1])
-    return _rows(t, name, t.shape[0], t.shape[1]) + (t.shape[0],)
+        t = t.view(-1, shape[2])
+        shape = t.shape
+    at, ld = _rows(t, name, shape[0], shape[1])
+    return at, ld, shape[0], _CODES[t.dtype]
 
 
 def quantize(x: torch.Tensor, matrix: Fp4Matrix) -> None:
     """``matrix`` gets the numbers of ``x`` (float32 or bfloat16, of its shape; of a gated matrix the gate rows, then the up rows)."""
-    at, ld, rows = _matrix_rows(x, "x", matrix)
-    _here(x, matrix.codes)
+    at, ld, rows, code = _matrix_rows(x, "x", matrix)
     n, k = matrix.shape[-2:]
-    _check(_fn("ssb_fp4_quantize")(at, ld, _CODES[x.dtype], matrix.codes.data_ptr(), matrix.scales.data_ptr(), rows, k, n,
+    _check(_fn("ssb_fp4_quantize")(at, ld, code, matrix.codes_at, matrix.scales_at, rows, k, n,
                                    n // 2 if matrix.gated else 0, 0, 0, _stream()), "fp4_quantize")
 
 
 def values(matrix: Fp4Matrix, out: torch.Tensor) -> None:
     """``out`` (float32 or bfloat16, of its shape) gets the numbers that ``matrix`` stands for, which both types hold exactly (down to
     2^-128); of a gated matrix the gate rows, then the up rows."""
-    at, ld, rows = _matrix_rows(out, "out", matrix)
-    _here(out, matrix.codes)
+    at, ld, rows, code = _matrix_rows(out, "out", matrix)
     n, k = matrix.shape[-2:]
-    _check(_fn("ssb_fp4_values")(matrix.codes.data_ptr(), matrix.scales.data_ptr(), at, ld, _CODES[out.dtype], rows, k, n,
+    _check(_fn("ssb_fp4_values")(matrix.codes_at, matrix.scales_at, at, ld, code, rows, k, n,
                                  n // 2 if matrix.gated else 0, _stream()), "fp4_values")
 
 
 Rows = Union[torch.Tensor, Fp4Matrix]
+_MODE_STORE, _MODE_GATED, _MODE_ACT = 0, 1, 2
 
 
 def _operands(what: str, x: Rows, weight: Fp4Matrix):
@@ -125,25 +128,36 @@ def _operands(what: str, x: Rows, weight: Fp4Matrix):
     if isinstance(x, Fp4Matrix):
         if len(x.shape) != 2 or x.shape[1] != k or x.gated:
             raise KernelError(f"{what}: rows of {k} numbers, not {x}")
-        return x.shape[0], x.codes.data_ptr(), 0, -1, x.scales.data_ptr()
-    if x.dim() != 2:
-        raise KernelError(f"{what}: x must be a matrix, is {tuple(x.shape)}")
-    at, ld = _rows(x, "x", x.shape[0], k)
-    if x.shape[1] != k:
-        raise KernelError(f"{what}: rows of {k} numbers, not {tuple(x.shape)}")
-    return x.shape[0], at, ld, _CODES[x.dtype], 0
+        _here(x.index, weight.index)
+        return x.shape[0], x.codes_at, 0, -1, x.scales_at
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != k:
+        raise KernelError(f"{what}: rows of {k} numbers, not {tuple(shape)}")
+    at, ld = _rows(x, "x", shape[0], k)
+    _here(x.get_device(), weight.index)
+    return shape[0], at, ld, _CODES[x.dtype], 0
 
 
-def _counters(x: Rows, n: int, device) -> torch.Tensor:
-    """The words that a product counts in: zeroed by the launch that quantises its rows, or zero as they are."""
-    if not isinstance(x, Fp4Matrix):
-        return torch.empty(n, dtype=torch.int32, device=device)
-    left, x._scratch = x._scratch, None                    # whoever takes them has them alone
-    return torch.zeros(n, dtype=torch.int32, device=device) if left is None or n > _COUNTERS else left
-
-
-def _of(x: Rows) -> torch.Tensor:
-    return x.codes if isinstance(x, Fp4Matrix) else x
+def _workspace(x: Rows, needs: int, device, words: int, ahead: int = 0):
+    """(a buffer, the address of scratch behind its first ``ahead`` bytes, the address of ``words`` counters) of a product that ``needs``
+    so much (ssb_fp4_product_scratch).  Counters are zeroed by the launch that quantises rows; a product of rows in 4 bits takes those
+    that came with them, which nobody takes twice, or has its own zeroed."""
+    size, counts = needs >> 1, needs & 1
+    if not counts:
+        if size + ahead == 0:
+            return None, 0, 0
+        buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
+        return buffer, buffer.data_ptr() + ahead, 0
+    if isinstance(x, Fp4Matrix):
+        buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
+        left, x._counters = x._counters, None
+        if left is None or words > _COUNTERS:
+            left = torch.zeros(words, dtype=torch.int32, device=device)
+            return (buffer, left), buffer.data_ptr() + ahead, left.data_ptr()
+        return (buffer, left), buffer.data_ptr() + ahead, left[1]
+    buffer = torch.empty(ahead + 4 * words + size, dtype=torch.int8, device=device)
+    at = buffer.data_ptr() + ahead
+    return buffer, at + 4 * words, at
 
 
 def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = False) -> None:
@@ -156,39 +170,41 @@ def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = Fal
     o_at, ldo = _rows(out, "out", rows, n)
     if out.shape[1] != n:
         raise KernelError(f"linear: out must be [{rows}, {n}], is {tuple(out.shape)}")
-    if accumulate and out.dtype != torch.float32:
+    if accumulate and out.dtype is not torch.float32:
         raise KernelError("linear: results are added in float32 only")
-    device = _here(out, weight.codes, _of(x))
+    _here(out.get_device())
     if rows == 0:
         return
-    counters = _counters(x, _COUNTERS, device)
-    scratch = torch.empty(_scratch_size("ssb_fp4_linear_scratch", rows, n, k, code >= 0), dtype=torch.int8, device=device)
-    _check(_fn("ssb_fp4_linear")(x_at, ldx, code, xs_at, weight.codes.data_ptr(), weight.scales.data_ptr(), o_at, ldo, _CODES[out.dtype],
-                                 rows, n, k, 1 if accumulate else 0, scratch.data_ptr(), counters.data_ptr(), _error_word(device),
-                                 _stream()), "fp4_linear")
+    device = weight.device
+    needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_STORE)
+    held, scratch, counters = _workspace(x, needs, device, _COUNTERS)
+    _check(_fn("ssb_fp4_linear")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, o_at, ldo, _CODES[out.dtype], rows, n, k,
+                                 1 if accumulate else 0, scratch, counters, _error_word(device) if counters else 0, _stream()), "fp4_linear")
 
 
 def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_scale: Optional[torch.Tensor]) -> Fp4Matrix:
     rows, x_at, ldx, code, xs_at = _operands(what, x, weight)
     n, k = weight.shape
-    inter = n // 2 if weight.gated else n
+    gated = weight.gated
+    inter = n // 2 if gated else n
     if inter % FP4_BLOCK:
         raise KernelError(f"{what}: {inter} inner channels must be a multiple of {FP4_BLOCK}")
-    device = _here(weight.codes, _of(x))
     if rows == 0:
         raise KernelError(f"{what}: no rows")
+    device = weight.device
     if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (rows,) or not row_scale.is_contiguous()
-                                  or row_scale.device != device):
-        raise KernelError(f"{what}: row_scale must be {rows} contiguous float32 values")
-    z = Fp4Matrix(torch.empty((rows, inter // 2), dtype=torch.uint8, device=device),
-                  torch.empty((-(-rows // 128) * -(-inter // 256), 1024), dtype=torch.uint8, device=device), (rows, inter))
-    counters = _counters(x, 2 * _COUNTERS, device)
-    scratch = torch.empty(_scratch_size("ssb_fp4_linear_scratch", rows, n, k, code >= 0), dtype=torch.int8, device=device)
-    _check(_fn("ssb_fp4_inner")(x_at, ldx, code, xs_at, weight.codes.data_ptr(), weight.scales.data_ptr(), z.codes.data_ptr(),
-                                z.scales.data_ptr(), rows, n, k, 1 if weight.gated else 0, kind, limit,
-                                0 if row_scale is None else row_scale.data_ptr(), scratch.data_ptr(), counters.data_ptr(),
-                                _error_word(device), _stream()), "fp4_inner")
-    z._scratch = counters[_COUNTERS:]
+                                  or row_scale.get_device() != weight.index):
+        raise KernelError(f"{what}: row_scale must be {rows} contiguous float32 values beside the weight")
+    needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_GATED if gated else _MODE_ACT)
+    size, ahead = Fp4Matrix.rows_layout(rows, inter)
+    held, scratch, counters = _workspace(x, needs, device, 2 * _COUNTERS, ahead)
+    buffer = held[0] if type(held) is tuple else held
+    z = Fp4Matrix.over_rows(buffer, rows, inter, size)
+    _check(_fn("ssb_fp4_inner")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, z.codes_at, z.scales_at, rows, n, k,
+                                1 if gated else 0, kind, limit, 0 if row_scale is None else row_scale.data_ptr(), scratch, counters,
+                                _error_word(device) if counters else 0, _stream()), "fp4_inner")
+    if counters:
+        z._counters = (held, counters + 4 * _COUNTERS)
     return z
 
 
@@ -244,7 +260,8 @@ def experts(x: torch.Tensor, expert_of: torch.Tensor, pair_weight: torch.Tensor,
     o_at, ldo = _rows(out, "out", tokens, k)
     if accumulate and out.dtype != torch.float32:
         raise KernelError("experts: results are added in float32 only")
-    device = _here(x, out, expert_of, pair_weight, first.codes, down.codes)
+    _here(x.get_device(), out.get_device(), expert_of.get_device(), pair_weight.get_device(), first.index, down.index)
+    device = first.device
     top = expert_of.shape[-1] if expert_of.dim() == 2 else 0
     if top < 1 or expert_of.dtype != torch.int32 or pair_weight.dtype != torch.float32 or expert_of.shape != (tokens, top) \
             or pair_weight.shape != (tokens, top) or not expert_of.is_contiguous() or not pair_weight.is_contiguous():
@@ -254,8 +271,8 @@ def experts(x: torch.Tensor, expert_of: torch.Tensor, pair_weight: torch.Tensor,
         raise KernelError(f"experts: {tokens} tokens of {top} choices among {E} experts are more than {MOST_PAIRS} pairs or 4096 experts")
     if tokens == 0:
         return
-    scratch = torch.empty(_scratch_size("ssb_fp4_experts_scratch", tokens, top, E, k, inter), dtype=torch.int8, device=device)
-    _check(_fn("ssb_fp4_experts")(x_at, ldx, _CODES[x.dtype], expert_of.data_ptr(), pair_weight.data_ptr(), first.codes.data_ptr(),
-                                  first.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), o_at, ldo, _CODES[out.dtype],
+    scratch = torch.empty(_scratch_size("ssb_fp4_experts_scratch", tokens, top, E, k, inter, first.gated), dtype=torch.int8, device=device)
+    _check(_fn("ssb_fp4_experts")(x_at, ldx, _CODES[x.dtype], expert_of.data_ptr(), pair_weight.data_ptr(), first.codes_at,
+                                  first.scales_at, down.codes_at, down.scales_at, o_at, ldo, _CODES[out.dtype],
                                   tokens, top, E, k, inter, 1 if first.gated else 0, kinds[kind], float(limit), 1 if accumulate else 0,
                                   scratch.data_ptr(), _error_word(device), _stream()), "fp4_experts")

@@ -2,6 +2,7 @@
 #include "fp4_codes.cuh"
 #include "packed_call.cuh"
 #include <algorithm>
+#include <climits>
 
 typedef __nv_bfloat16 bf16;
 
@@ -15,35 +16,46 @@ struct FrRows {
     const int* slot; int top, tile_rows;
 };
 
+// Where the units of 128 numbers that a half-warp takes lie: unit u is part u % per_row of row u / per_row; from one turn to the next
+// the half-warp goes on by ``rows`` rows and ``parts`` parts, so that nothing is divided on the way.
+struct FrStep {
+    int per_row, rows, parts;
+    __device__ void next(int& row, int& part) const {
+        row += rows;
+        part += parts;
+        if (part >= per_row) { part -= per_row; ++row; }
+    }
+};
+
 // A unit is 128 numbers of a row: sixteen lanes of eight, four lanes a block, whose four scales are one word.  Units run over whole
-// k-blocks; behind a row's end they write scales of zero.
-template <typename T>
+// k-blocks; behind a row's end they write scales of zero.  TURNS units are in flight.
+template <typename T, int TURNS>
 __global__ void __launch_bounds__(FR_THREADS)
 fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int rows, int K,
-                    const FrRows to, int k_blocks, int* __restrict__ clear, int n_clear) {
+                    const FrRows to, const FrStep step, int k_blocks, int* __restrict__ clear, int n_clear) {
+    const int lane = threadIdx.x & 15, u = blockIdx.x * (FR_THREADS / 16) + (threadIdx.x >> 4);
+    int row = u / step.per_row, part = u - row * step.per_row;
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < n_clear; i += FR_THREADS) clear[i] = 0;
-    const int lane = threadIdx.x & 15, per_row = 2 * k_blocks;
-    const long long units = (long long)rows * per_row, step = (long long)gridDim.x * (FR_THREADS / 16);
-    long long u = (long long)blockIdx.x * (FR_THREADS / 16) + (threadIdx.x >> 4);
-    // the half-warps of a warp stay together: the loop ends for both at once
-    for (long long first = u - ((threadIdx.x >> 4) & 1); first < units; first += FR_TURNS * step, u += FR_TURNS * step) {
-        float v[FR_TURNS][8];
+    // the half-warps of a warp go on together: a later unit is in no earlier row
+    while (__any_sync(0xffffffffu, row < rows)) {
+        float v[TURNS][8];
+        int at_row[TURNS], at_part[TURNS];
 #pragma unroll
-        for (int j = 0; j < FR_TURNS; ++j) {
-            const long long unit = u + j * step;
-            const int row = (int)(unit / per_row), k = (int)(unit - (long long)row * per_row) * 128 + lane * 8;
-            const bool live = unit < units && k < K;
+        for (int j = 0; j < TURNS; ++j) {
+            at_row[j] = row;
+            at_part[j] = part;
+            const int k = part * 128 + lane * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
-            if (live) f4_load8(x + (to.slot ? row / to.top : row) * ldx + k, v[j]);
+            if (row < rows && k < K) f4_load8(x + (long long)(to.slot ? row / to.top : row) * ldx + k, v[j]);
+            step.next(row, part);
         }
 #pragma unroll
-        for (int j = 0; j < FR_TURNS; ++j) {
-            const long long unit = u + j * step;
-            const int row = (int)(unit / per_row), part = (int)(unit - (long long)row * per_row), k = part * 128 + lane * 8;
+        for (int j = 0; j < TURNS; ++j) {
+            const int k = at_part[j] * 128 + lane * 8;
             uint32_t most = f4_most(v[j]);
             if (__any_sync(0xffffffffu, most >= F4_WILD)) {
 #pragma unroll
@@ -56,47 +68,79 @@ fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict_
             uint32_t word = (uint32_t)byte << (8 * (lane >> 2));
             word |= __shfl_xor_sync(0xffffffffu, word, 4);
             word |= __shfl_xor_sync(0xffffffffu, word, 8);
-            if (unit >= units) continue;
-            long long at;                                      // row of the codes
-            int run0 = 0, r;                                   // the matrix's first run of scales' rows, the row in it
+            if (at_row[j] >= rows) continue;
+            long long at = at_row[j];                          // row of the codes
+            int run0 = 0, r = at_row[j];                       // the matrix's first run of scales' rows, the row in it
             if (to.slot) {
-                at = to.slot[row];
+                at = to.slot[at_row[j]];
                 if (at < 0) continue;
                 const int tile = (int)at / to.tile_rows;
                 r = tile * max(to.tile_rows, 128) + (int)at - tile * to.tile_rows;
-            } else {
-                const int expert = row / to.per_expert;
-                r = f4_laid_row(row - expert * to.per_expert, to.inter);
+            } else if (to.per_expert < rows || to.inter) {
+                const int expert = r / to.per_expert;
+                r = f4_laid_row(r - expert * to.per_expert, to.inter);
                 at = (long long)expert * to.per_expert + r;
                 run0 = expert * ((to.per_expert + 127) >> 7);
             }
             if (k < K) *reinterpret_cast<uint32_t*>(codes + at * (K / 2) + k / 2) = f4_encode8(v[j], f4_inverse(byte));
             if (lane == 0)
-                *reinterpret_cast<uint32_t*>(scales + (size_t)run0 * k_blocks * F4_CHUNK + f4_scale_at(r, part * 4, k_blocks)) = word;
+                *reinterpret_cast<uint32_t*>(scales + (size_t)run0 * k_blocks * F4_CHUNK + f4_scale_at(r, at_part[j] * 4, k_blocks)) = word;
         }
     }
 }
 
-template <typename T>
+// The same units the other way.
+template <typename T, int TURNS>
 __global__ void __launch_bounds__(FR_THREADS)
 fp4_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, long long ldo, int rows,
-                  int K, int per_expert, int inter, int k_blocks) {
+                  int K, int per_expert, int inter, const FrStep step, int k_blocks) {
+    const int lane = threadIdx.x & 15, u = blockIdx.x * (FR_THREADS / 16) + (threadIdx.x >> 4);
+    int row = u / step.per_row, part = u - row * step.per_row;
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
-    const int per_row = K / 8, tiles = (per_expert + 127) >> 7;
-    const long long pieces = (long long)rows * per_row, step = (long long)gridDim.x * FR_THREADS;
-    for (long long p = (long long)blockIdx.x * FR_THREADS + threadIdx.x; p < pieces; p += step) {
-        const int row = (int)(p / per_row), k = (int)(p - (long long)row * per_row) * 8;
-        const int expert = row / per_expert, r = f4_laid_row(row - expert * per_expert, inter);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + ((size_t)expert * per_expert + r) * (K / 2) + k / 2);
-        const float s = f4_scale(scales[(size_t)expert * tiles * k_blocks * F4_CHUNK + f4_scale_at(r, k / F4_BLOCK, k_blocks)]);
-        float v[8];
+    while (row < rows) {
+        uint32_t w[TURNS], byte[TURNS];
+        int at_row[TURNS], at_part[TURNS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = f4_value(w >> (4 * i)) * s;
-        f4_store8(out + row * ldo + k, v);
+        for (int j = 0; j < TURNS; ++j) {
+            at_row[j] = row;
+            at_part[j] = part;
+            const int k = part * 128 + lane * 8;
+            w[j] = byte[j] = 0;
+            if (row < rows && k < K) {
+                long long at = row;
+                int run0 = 0, r = row;
+                if (per_expert < rows || inter) {
+                    const int expert = row / per_expert;
+                    r = f4_laid_row(row - expert * per_expert, inter);
+                    at = (long long)expert * per_expert + r;
+                    run0 = expert * ((per_expert + 127) >> 7);
+                }
+                w[j] = *reinterpret_cast<const uint32_t*>(codes + at * (K / 2) + k / 2);
+                byte[j] = scales[(size_t)run0 * k_blocks * F4_CHUNK + f4_scale_at(r, k / F4_BLOCK, k_blocks)];
+            }
+            step.next(row, part);
+        }
+#pragma unroll
+        for (int j = 0; j < TURNS; ++j) {
+            const int k = at_part[j] * 128 + lane * 8;
+            float v[8];
+            f4_values8(w[j], f4_scale((int)byte[j]), v);
+            if (at_row[j] < rows && k < K) f4_store8(out + (long long)at_row[j] * ldo + k, v);
+        }
     }
 }
 
+// Blocks of a launch over ``rows`` rows of ``per_row`` units, and its step; ``turns``: how many units a half-warp should have in flight.
+// One where that leaves SMs without work.
+static FrStep fr_step(int rows, int per_row, int* blocks, int* turns) {
+    const long long units = (long long)rows * per_row, per_block = FR_THREADS / 16;
+    const long long all = (units + per_block - 1) / per_block, most = 8LL * ssb_sm_count();
+    *turns = all >= 4LL * ssb_sm_count() ? 4 : 1;
+    *blocks = (int)std::min(all, most);
+    const long long step = *blocks * per_block;
+    return FrStep{per_row, (int)(step / per_row), (int)(step % per_row)};
+}
 static int fr_sizes(int rows, int K, int per_expert, int inter) {
     if (rows < 0 || K <= 0 || K % F4_BLOCK || per_expert <= 0 || rows % per_expert || (inter && (inter % 16 || per_expert != 2 * inter)))
         return SSB_ERR_BAD_SIZE;
@@ -107,11 +151,11 @@ template <typename T>
 static int fr_quantize(const T* x, long long ldx, uint8_t* codes, uint8_t* scales, int rows, int K, const FrRows& to, int* clear, int n_clear,
                        cudaStream_t stream) {
     const int k_blocks = f4_k_blocks(K);
-    const long long units = (long long)rows * 2 * k_blocks, per_block = FR_THREADS / 16;
-    // a turn a thread until every SM has its eight blocks, then as many turns as it takes
-    const int blocks = (int)std::min<long long>((units + per_block - 1) / per_block, 8 * ssb_sm_count());
-    return ssb_launch(fp4_quantize_kernel<T>, dim3(blocks), dim3(FR_THREADS), 0, stream, true, x, ldx, codes, scales, rows, K, to, k_blocks,
-                      clear, n_clear);
+    int blocks, turns;
+    const FrStep step = fr_step(rows, 2 * k_blocks, &blocks, &turns);
+    if ((long long)rows + step.rows * 4LL + 4 > INT_MAX) return SSB_ERR_BAD_SIZE;
+    return ssb_launch(turns == 1 ? fp4_quantize_kernel<T, 1> : fp4_quantize_kernel<T, FR_TURNS>, dim3(blocks), dim3(FR_THREADS), 0, stream, true,
+                      x, ldx, codes, scales, rows, K, to, step, k_blocks, clear, n_clear);
 }
 
 // x: rows x K, rows of 16-byte pieces; ``per_expert`` rows of them are a matrix; clear: words zeroed on the way.
@@ -135,19 +179,24 @@ SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void
     return SSB_ERR_BAD_DTYPE;
 }
 
+template <typename T>
+static int fr_values(const uint8_t* codes, const uint8_t* scales, T* out, long long ldo, int rows, int K, int per_expert, int inter,
+                     cudaStream_t stream) {
+    int blocks, turns;
+    const FrStep step = fr_step(rows, (K + 127) / 128, &blocks, &turns);
+    if ((long long)rows + step.rows * 4LL + 4 > INT_MAX) return SSB_ERR_BAD_SIZE;
+    return ssb_launch(turns == 1 ? fp4_values_kernel<T, 1> : fp4_values_kernel<T, FR_TURNS>, dim3(blocks), dim3(FR_THREADS), 0, stream, true,
+                      codes, scales, out, ldo, rows, K, per_expert, inter, step, f4_k_blocks(K));
+}
+
 SSB_API int ssb_fp4_values(const void* codes, const void* scales, void* out, long long ldo, int dtype, int rows, int K, int per_expert,
                            int inter, cudaStream_t stream) {
     const int rc = fr_sizes(rows, K, per_expert, inter);
     if (rc || rows == 0) return rc;
     if (((uintptr_t)out | (uintptr_t)codes | (uintptr_t)scales) & 15) return SSB_ERR_BAD_SIZE;
-    const long long pieces = (long long)rows * (K / 8);
-    const dim3 grid((unsigned)std::min<long long>((pieces + FR_THREADS - 1) / FR_THREADS, 16 * ssb_sm_count()));
-    const uint8_t *c = (const uint8_t*)codes, *s = (const uint8_t*)scales;
-    const int k_blocks = f4_k_blocks(K);
-    if (dtype == SSB_BF16)
-        return ssb_launch(fp4_values_kernel<bf16>, grid, dim3(FR_THREADS), 0, stream, true, c, s, (bf16*)out, ldo, rows, K, per_expert, inter, k_blocks);
-    if (dtype == SSB_F32)
-        return ssb_launch(fp4_values_kernel<float>, grid, dim3(FR_THREADS), 0, stream, true, c, s, (float*)out, ldo, rows, K, per_expert, inter, k_blocks);
+    const uint8_t *c = (const uint8_t*)codes, *sc = (const uint8_t*)scales;
+    if (dtype == SSB_BF16) return fr_values(c, sc, (bf16*)out, ldo, rows, K, per_expert, inter, stream);
+    if (dtype == SSB_F32) return fr_values(c, sc, (float*)out, ldo, rows, K, per_expert, inter, stream);
     return SSB_ERR_BAD_DTYPE;
 }
 

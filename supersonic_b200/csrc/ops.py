@@ -10,6 +10,7 @@ codes (crates/gpu-hal/src/scalar_type.rs:25-32).
 from __future__ import annotations
 
 from ctypes import c_float, c_int, c_longlong, c_void_p
+from struct import Struct, error as StructError
 from typing import Optional
 
 import torch
@@ -1743,6 +1744,7 @@ def route_softmax(logits: torch.Tensor, n_experts: int, renormalize: bool, scale
 SCORES = {"softmax": 0, "sigmoid": 1}
 GROUP_SCORES = ("max", "two")
 ROUTE_MOST_EXPERTS, ROUTE_MOST_GROUPS = 2048, 32
+_route_scored = None
 
 
 def route_scored(logits: torch.Tensor, n_experts: int, expert_of: torch.Tensor, pair_weight: torch.Tensor, scores: str = "softmax",
@@ -1754,29 +1756,38 @@ def route_scored(logits: torch.Tensor, n_experts: int, expert_of: torch.Tensor, 
     of its two largest ("two").  pair_weight = s * scale of the chosen, with ``renormalize`` divided by the sum of their s (+ 1e-20).
     Ties go to the lower index.  A NaN among the logits counts as minus infinity, whose s is zero, an infinite one as the largest number;
     a c that is NaN comes last."""
-    _need(logits, "logits", torch.float32, 2)
-    _need(expert_of, "expert_of", torch.int32, 2); _need(pair_weight, "pair_weight", torch.float32, 2)
-    T, top = logits.shape[0], expert_of.shape[1]
+    shape = logits.shape
+    T, top = shape[0], expert_of.shape[-1]
     keep = groups if keep is None else keep
-    if logits.shape[1] < n_experts or tuple(expert_of.shape) != (T, top) or tuple(pair_weight.shape) != (T, top) \
-            or not (expert_of.is_contiguous() and pair_weight.is_contiguous()):
-        raise KernelError("route_scored: logits [tokens, >= experts]; expert_of and pair_weight [tokens, top], contiguous")
+    if len(shape) != 2 or logits.dtype is not torch.float32 or shape[1] < n_experts or (logits.stride(1) != 1 and shape[1] > 1) \
+            or expert_of.dtype is not torch.int32 or pair_weight.dtype is not torch.float32 or expert_of.shape != (T, top) \
+            or pair_weight.shape != (T, top) or not expert_of.is_contiguous() or not pair_weight.is_contiguous():
+        raise KernelError("route_scored: logits float32 [tokens, >= experts]; expert_of int32 and pair_weight float32 [tokens, top], contiguous")
     if scores not in SCORES or group_score not in GROUP_SCORES:
         raise KernelError(f"route_scored: scores {scores!r} of {sorted(SCORES)}, group_score {group_score!r} of {list(GROUP_SCORES)}")
     if not 1 <= n_experts <= ROUTE_MOST_EXPERTS or not 1 <= groups <= ROUTE_MOST_GROUPS or n_experts % groups or not 1 <= keep <= groups \
             or not 1 <= top <= keep * (n_experts // groups):
         raise KernelError(f"route_scored: {top} of {n_experts} experts (up to {ROUTE_MOST_EXPERTS}) in {groups} equal groups (up to "
                           f"{ROUTE_MOST_GROUPS}), {keep} of them kept")
+    correction_at, device = 0, torch.cuda.current_device()
     if correction is not None:
-        _need(correction, "correction", torch.float32, 1)
-        if correction.shape[0] != n_experts:
-            raise KernelError("route_scored: one correction per expert")
-    if any(t is not None and t.device.index != torch.cuda.current_device() for t in (logits, expert_of, pair_weight, correction)):
+        if correction.dtype is not torch.float32 or correction.shape != (n_experts,) or not correction.is_contiguous() \
+                or correction.get_device() != device:
+            raise KernelError("route_scored: one correction per expert, float32 on the current CUDA device")
+        correction_at = correction.data_ptr()
+    if logits.get_device() != device or expert_of.get_device() != device or pair_weight.get_device() != device:
         raise KernelError("route_scored: tensors must be on the current CUDA device")
-    _check(_fn("expert_ops", "ssb_route_scored")(
-        _ptr(logits), c_int(logits.stride(0)), _ptr(correction), c_int(T), c_int(n_experts), c_int(groups), c_int(keep), c_int(top),
-        c_int(SCORES[scores]), c_int(1 if group_score == "two" else 0), c_int(1 if renormalize else 0), c_float(scale),
-        _ptr(expert_of), _ptr(pair_weight), c_int(1 if pdl else 0), _stream()), "route_scored")
+    global _route_scored
+    if _route_scored is None:
+        _route_scored = _fn("expert_ops", "ssb_route_scored_packed"), Struct("@PiPiiiiiiiifPPiP").pack
+    call, pack = _route_scored
+    try:
+        args = pack(logits.data_ptr(), logits.stride(0) if T > 1 else shape[1], correction_at, T, n_experts, groups, keep, top, SCORES[scores],
+                    1 if group_score == "two" else 0, 1 if renormalize else 0, scale, expert_of.data_ptr(), pair_weight.data_ptr(),
+                    1 if pdl else 0, _stream().value or 0)
+    except StructError as e:
+        raise KernelError(f"route_scored: {e}") from None
+    _check(call(args), "route_scored")
 
 
 def expert_tiles_bound(n_pairs: int, n_experts: int, tile_rows: int) -> int:

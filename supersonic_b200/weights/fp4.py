@@ -22,7 +22,7 @@ _RUN_ROWS, _RUN_BLOCKS = 128, 8
 class Fp4Matrix:
     """``shape`` is that of the numbers: (n, k), or (experts, n, k)."""
 
-    __slots__ = ("codes", "scales", "shape", "gated", "_scratch")
+    __slots__ = ("_codes", "_scales", "shape", "gated", "device", "index", "codes_at", "scales_at", "_buffer", "_counters")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, gated: bool = False):
         shape = tuple(int(s) for s in shape)
@@ -36,7 +36,11 @@ class Fp4Matrix:
             raise ValueError(f"codes must be contiguous uint8 {shape[:-1] + (k // 2,)}, are {codes.dtype} {tuple(codes.shape)}")
         if scales.dtype != torch.uint8 or tuple(scales.shape) != (runs, 1024) or not scales.is_contiguous() or scales.device != codes.device:
             raise ValueError(f"scales must be contiguous uint8 {(runs, 1024)} beside the codes, are {scales.dtype} {tuple(scales.shape)}")
-        self.codes, self.scales, self.shape, self.gated, self._scratch = codes, scales, shape, gated, None
+        self._codes, self._scales, self.shape, self.gated, self._buffer, self._counters = codes, scales, shape, gated, None, None
+        # where they are, for the kernels: the tensors stay what they are as long as the matrix lives
+        self.device, self.index, self.codes_at, self.scales_at = codes.device, codes.get_device(), codes.data_ptr(), scales.data_ptr()
+        if (self.codes_at | self.scales_at) % 16:
+            raise ValueError("codes and scales must start on 16 bytes")
 
     @classmethod
     def empty(cls, *shape: int, device="cuda", gated: bool = False) -> "Fp4Matrix":
@@ -75,9 +79,35 @@ class Fp4Matrix:
         s = s.reshape(-1, tiles * _RUN_ROWS, k_blocks * _RUN_BLOCKS)[:, :n, : k // FP4_BLOCK]
         return s.reshape(self.shape[:-1] + (k // FP4_BLOCK,)).contiguous()
 
+    @staticmethod
+    def rows_layout(n: int, k: int):
+        """(bytes of codes up to a whole 256, bytes of both) of a step's rows [n, k] in one buffer (:meth:`over_rows`)."""
+        codes = (n * (k // 2) + 255) // 256 * 256
+        return codes, codes + -(-n // _RUN_ROWS) * -(-k // (FP4_BLOCK * _RUN_BLOCKS)) * 1024
+
+    @classmethod
+    def over_rows(cls, buffer: torch.Tensor, n: int, k: int, codes: int) -> "Fp4Matrix":
+        """A step's rows [n, k] at the start of an int8 ``buffer``: ``codes`` bytes of codes, then scales (:meth:`rows_layout`)."""
+        m = cls.__new__(cls)
+        m._codes = m._scales = m._counters = None          # made when somebody asks for them
+        m.shape, m.gated, m._buffer, m.device, m.index = (n, k), False, buffer, buffer.device, buffer.get_device()
+        m.codes_at = buffer.data_ptr()
+        m.scales_at = m.codes_at + codes
+        return m
+
     @property
-    def device(self) -> torch.device:
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            n, k = self.shape
+            self._codes = self._buffer[: n * (k // 2)].view(torch.uint8).view(n, k // 2)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            codes, both = self.rows_layout(*self.shape)
+            self._scales = self._buffer[codes:both].view(torch.uint8).view(-1, 1024)
+        return self._scales
 
     def bytes_held(self) -> int:
         return self.codes.numel() + self.scales.numel()
