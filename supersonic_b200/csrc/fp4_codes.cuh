@@ -52,6 +52,21 @@ __device__ __forceinline__ uint32_t f4_encode1(float x) {
     asm("{\n.reg .b8 a;\ncvt.rn.satfinite.e2m1x2.f32 a, %1, %2;\nmov.b32 %0, {a, 0, 0, 0};\n}" : "=r"(w) : "f"(0.f), "f"(x));
     return w;
 }
+// A warp's 32 numbers, one a lane, as a block: codes into ``row`` (of codes), the scale of row r's block; nothing from channel ``width`` on.
+__device__ __forceinline__ void f4_put_block(float z, uint8_t* row, uint8_t* scales, int r, int k, int width, int k_blocks) {
+    const int lane = threadIdx.x & 31;
+    z = f4_finite(z);
+    const int byte = f4_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(z) & 0x7fffffffu));
+    // a lane's code into its place among the eight of a word
+    uint32_t w = f4_encode1(z * f4_inverse(byte)) << (4 * (lane & 7));
+    w |= __shfl_xor_sync(0xffffffffu, w, 1);
+    w |= __shfl_xor_sync(0xffffffffu, w, 2);
+    w |= __shfl_xor_sync(0xffffffffu, w, 4);
+    if (k < width) {
+        if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(row + (k + lane) / 2) = w;
+        if (lane == 0) scales[f4_scale_at(r, k / F4_BLOCK, k_blocks)] = (uint8_t)byte;
+    }
+}
 // Eight codes' values times ``scale``.
 __device__ __forceinline__ void f4_values8(uint32_t codes, float scale, float* v) {
     uint32_t h[4];

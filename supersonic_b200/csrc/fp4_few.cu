@@ -66,39 +66,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
     int tiles = 1;
     if (LIST) {
         ssb_pdl_wait();
-        // pairs by expert, in their order; a tile: ROWS neighbours of one expert
-        int e = -1, first = 0, place = 0;
-        if (tid < a.pairs) {
-            e = a.expert_of[tid];
-            if ((unsigned)e >= (unsigned)a.experts) e = -1;
-            tile_first[tid] = e;
-        }
-        __syncthreads();
-        int same = 0;
-        if (e >= 0)
-            for (int q = 0; q < a.pairs; ++q) {
-                const int f = tile_first[q];
-                first += f >= 0 && f < e;
-                place += f == e && q < tid;
-                same += f == e;
-            }
-        __syncthreads();
-        if (tid < a.pairs) pair_of[tid] = -1;
-        if (tid < FW_MOST_PAIRS) tile_rows[tid] = 0;
-        __syncthreads();
-        const bool starts = e >= 0 && place % ROWS == 0;
-        if (e >= 0) pair_of[first + place] = tid;
-        if (starts) tile_rows[first + place] = min(ROWS, same - place);          // at its first row's place for now
-        __syncthreads();
-        int before = 0, all = 0, rows_here = 0;
-        if (starts) {
-            rows_here = tile_rows[first + place];
-            for (int q = 0; q < first + place; ++q) before += tile_rows[q] > 0;
-        }
-        all = __syncthreads_count(starts);
-        if (starts) { tile_rows[before] = rows_here; tile_first[before] = first + place; tile_expert[before] = e; }
-        __syncthreads();
-        tiles = all;
+        tiles = fw_sort_pairs<ROWS>(a.expert_of, a.pairs, a.experts, pair_of, tile_first, tile_rows, tile_expert);
     }
     const int c_tiles = (a.N + CH - 1) / CH, items = tiles * c_tiles;
     const int begin = (int)((long long)items * blockIdx.x / gridDim.x), end = (int)((long long)items * (blockIdx.x + 1) / gridDim.x);
@@ -288,18 +256,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
                 } else {
                     z = ssb_activate(total(r, q * 32 + lane), a.kind) * a.limit;
                 }
-                z = f4_finite(z);
-                const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(z) & 0x7fffffffu);
-                const int byte = f4_scale_byte(most);
-                // a lane's code into its place among the eight of a word
-                uint32_t w = f4_encode1(z * f4_inverse(byte)) << (4 * (lane & 7));
-                w |= __shfl_xor_sync(0xffffffffu, w, 1);
-                w |= __shfl_xor_sync(0xffffffffu, w, 2);
-                w |= __shfl_xor_sync(0xffffffffu, w, 4);
-                if (k < width) {
-                    if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>((uint8_t*)a.out + (size_t)out_row * a.ldo + (k + lane) / 2) = w;
-                    if (lane == 0) a.out_scales[f4_scale_at(out_row, k / F4_BLOCK, a.inner_blocks)] = (uint8_t)byte;
-                }
+                f4_put_block(z, (uint8_t*)a.out + (size_t)out_row * a.ldo, a.out_scales, out_row, k, width, a.inner_blocks);
                 // behind the last channel: scales of zero up to a whole k-block
                 if (q == 0 && ch0 + CH >= a.N && width / F4_BLOCK + lane < 8 * a.inner_blocks && lane < 8)
                     a.out_scales[f4_scale_at(out_row, width / F4_BLOCK + lane, a.inner_blocks)] = 0;
@@ -349,7 +306,10 @@ static FwPlan fw_plan(int M, int N, int K, int mode, int tiles) {
     }
     const size_t fixed = fw_fixed(8 * p.nb, k_blocks, p.k_warps, list);
     if (fixed >= FW_MOST_SMEM) return p;
-    p.slots = (int)std::min<size_t>(5, (FW_MOST_SMEM - fixed) / (FW_WARPS * FW_SLOT));
+    // no more than a block's steps want: what is left lets the next launch's blocks begin beside these
+    const long long items = (long long)std::max(tiles, 1) * ((N + 16 * (FW_WARPS / p.k_warps) - 1) / (16 * (FW_WARPS / p.k_warps)));
+    const long long steps = (items + sms - 1) / sms * ((k_blocks + p.k_warps - 1) / p.k_warps);
+    p.slots = (int)std::min<long long>(std::min<long long>(5, std::max<long long>(2, steps)), (FW_MOST_SMEM - fixed) / (FW_WARPS * FW_SLOT));
     if (p.slots < 2) p.slots = 0;
     p.smem = fixed + (size_t)p.slots * FW_WARPS * FW_SLOT;
     return p;

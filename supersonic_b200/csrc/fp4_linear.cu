@@ -15,76 +15,10 @@
 #include "fp4_codes.cuh"
 #include "fp4_few.cuh"
 #include "packed_call.cuh"
-#include "tc_helpers.cuh"
+#include "fp4_tc.cuh"
 #include <algorithm>
 
 typedef __nv_bfloat16 bf16;
-
-constexpr int FL_BM = 128;
-constexpr int FL_THREADS = 192;           // warp 0: TMA, warp 1: MMA + tensor memory, warps 2-5: epilogue
-constexpr int FL_ROW = 128;               // bytes of codes a row and k-block
-constexpr uint32_t FL_CHUNK = F4_CHUNK;
-enum { FL_STORE = 0, FL_GATED = 1, FL_ACT = 2 };
-
-// D float32; A and B E2M1, both K-major; scales powers of two.  ``part``: which half of a scale word (blocks 0 1 or 2 3) A and B use.
-__host__ __device__ constexpr uint32_t fl_idesc(int m, int n, int part) {
-    return ((uint32_t)(2 * part) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
-           ((uint32_t)(2 * part) << 29);
-}
-// 32 lanes x 16 bytes of shared memory that lie together (8-row groups 128 bytes apart), no swizzle.
-__device__ __forceinline__ uint64_t fl_scale_desc(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (8ull << 16) | (8ull << 32) | (1ull << 46);
-}
-__device__ __forceinline__ void fl_copy_scales(uint32_t tmem, uint32_t addr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(fl_scale_desc(addr)) : "memory");
-}
-__device__ __forceinline__ void fl_copy_scales_pair(uint32_t tmem, uint32_t addr) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(fl_scale_desc(addr)) : "memory");
-}
-// A k-block: four instructions of 64 numbers (32 bytes along the swizzled row: 2 descriptor units); the first two use the scales at
-// sa0 and sb0, the last two those at sa1 and sb1, each pair their first and their second halves (idesc0, idesc1).
-#define FL_MMA_X4(group_)                                                                                                                 \
-    asm volatile("{\n.reg .pred p, q;\n.reg .b64 a1, a2, a3, b1, b2, b3;\n"                                                               \
-                 "setp.ne.b32 p, %9, 0;\nsetp.eq.b32 q, 0, 0;\n"                                                                          \
-                 "add.u64 a1, %1, 2;\nadd.u64 a2, %1, 4;\nadd.u64 a3, %1, 6;\n"                                                           \
-                 "add.u64 b1, %2, 2;\nadd.u64 b2, %2, 4;\nadd.u64 b3, %2, 6;\n"                                                           \
-                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"              \
-                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %4, [%5], [%6], q;\n"              \
-                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %3, [%7], [%8], q;\n"              \
-                 "tcgen05.mma.cta_group::" group_ ".kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %4, [%7], [%8], q;\n}"             \
-                 ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc0), "r"(idesc1), "r"(sa0), "r"(sb0), "r"(sa1), "r"(sb1),               \
-                 "r"(accumulate) : "memory")
-__device__ __forceinline__ void fl_mma_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc0, uint32_t idesc1, uint32_t sa0,
-                                          uint32_t sb0, uint32_t sa1, uint32_t sb1, uint32_t accumulate) {
-    FL_MMA_X4("1");
-}
-__device__ __forceinline__ void fl_mma_pair_x4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc0, uint32_t idesc1,
-                                               uint32_t sa0, uint32_t sb0, uint32_t sa1, uint32_t sb1, uint32_t accumulate) {
-    FL_MMA_X4("2");
-}
-__device__ __forceinline__ void fl_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void fl_ld16(uint32_t taddr, float (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\ntcgen05.wait::ld.sync.aligned;"
-                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
-                   "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-                 : "r"(taddr) : "memory");
-}
-// An arrival at the pair's leader that orders tensor memory alone (by the tcgen05 fences around it): a release at cluster scope waits
-// for whatever this thread has on its way to or from memory, 1,290 clocks where scales are being fetched ahead.
-__device__ __forceinline__ void fl_arrive_leader(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
-// Whether any thread of the four epilogue warps says so; all of them meet here (barrier 1).
-__device__ __forceinline__ bool fl_any_of_four(bool mine) {
-    uint32_t any;
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, 1, 128, p;\nselp.b32 %0, 1, 0, q;\n}"
-                 : "=r"(any) : "r"((uint32_t)mine) : "memory");
-    return any != 0;
-}
-__device__ __forceinline__ void fl_meet_four() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
 struct FlOut {
     void* out;                     // FL_STORE: rows of ldo elements; else codes, rows of ldo bytes
@@ -117,30 +51,9 @@ struct FlRange {
     __device__ int owner(long long unit) const { return (int)(((unit + 1) * blocks - 1) / units); }       // the block that takes it
 };
 
-constexpr int fl_power(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
 template <int BN, int STAGES> constexpr int fl_columns() { return fl_power(2 * BN + 16 * STAGES); }
-constexpr int FL_INNER_ROWS = 16;         // rows of an inner tile that meet in shared memory at a time
-constexpr int FL_INNER_LD = 132;
 template <int BN, int STAGES> constexpr size_t fl_smem() {
     return (size_t)STAGES * ((FL_BM + BN) * FL_ROW + 2 * FL_CHUNK) + FL_INNER_ROWS * FL_INNER_LD * 4 + (2 * STAGES + 4) * 8 + 32 + 1024;
-}
-
-// 16 numbers of a block of 32 whose other half the neighbouring lane has: codes to ``dst`` (8 bytes), the block's scale by the even lane.
-__device__ __forceinline__ void fl_put_inner(float (&v)[16], uint8_t* dst, uint8_t* scale, bool live) {
-    uint32_t most = f4_most(v);
-    if (__any_sync(0xffffffffu, most >= F4_WILD)) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = f4_finite(v[i]);
-        most = f4_most(v);
-    }
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    const int byte = f4_scale_byte(most);
-    const float inverse = f4_inverse(byte);
-    const uint2 w = make_uint2(f4_encode8(v, inverse), f4_encode8(v + 8, inverse));
-    if (live) {
-        *reinterpret_cast<uint2*>(dst) = w;
-        if ((threadIdx.x & 1) == 0) *scale = (uint8_t)byte;
-    }
 }
 
 template <int BN, int STAGES, int MODE, bool LIST>
@@ -230,41 +143,43 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
     } else if (warp == 1) {
         if (!LIST) ssb_pdl_wait();                                 // what follows spins on barriers
-        if (lane == 0) {
-            constexpr uint32_t idesc0 = fl_idesc(FL_BM, BN, 0), idesc1 = fl_idesc(FL_BM, BN, 1);
-            bool ok = true;
-            int i = 0, s = 0;
-            uint32_t lap = 0;
-            for (long long u = range.begin; u < range.end && ok; ++i) {
-                const int tile = (int)(u / k_blocks), kb0 = (int)(u - (long long)tile * k_blocks);
-                const int n = (int)min((long long)(k_blocks - kb0), range.end - u), buf = i & 1;
-                int m, unused;
-                place(tile, m, unused);
-                const int rows_at = LIST || BN == 128 ? 0 : (m * BN & 127) / 32;      // 32 rows' scales a column
-                if (!mbar_wait(acc_empty0 + 8 * buf, ((i >> 1) & 1) ^ 1, abort_flag)) {
-                    *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
-                }
+        constexpr uint32_t idesc0 = fl_idesc(FL_BM, BN, 0), idesc1 = fl_idesc(FL_BM, BN, 1);
+        const bool issues = fl_elect();
+        const uint64_t w_desc = smem_desc(smem_u32(smem)), x_desc = smem_desc(smem_u32(smem) + W_BYTES);
+        bool ok = true;
+        int i = 0, s = 0;
+        uint32_t lap = 0;
+        for (long long u = range.begin; u < range.end && ok; ++i) {
+            const int tile = (int)(u / k_blocks), kb0 = (int)(u - (long long)tile * k_blocks);
+            const int n = (int)min((long long)(k_blocks - kb0), range.end - u), buf = i & 1;
+            int m, unused;
+            place(tile, m, unused);
+            const int rows_at = LIST || BN == 128 ? 0 : (m * BN & 127) / 32;          // 32 rows' scales a column
+            ok = mbar_wait(acc_empty0 + 8 * buf, ((i >> 1) & 1) ^ 1, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break; }
+            tc_fence_after();
+            for (int j = 0; j < n; ++j) {
+                ok = mbar_wait(full0 + 8 * s, lap, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break; }
                 tc_fence_after();
-                for (int j = 0; j < n; ++j) {
-                    if (!mbar_wait(full0 + 8 * s, lap, abort_flag)) {
-                        *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
-                    }
-                    tc_fence_after();
-                    // a stage has columns of its own for its scales, so what reads them is done when they are written again
-                    const uint32_t w_addr = smem_u32(smem + s * STAGE_BYTES), scales = tmem + 2 * BN + 16 * s;
-                    const uint32_t s_addr = w_addr + W_BYTES + X_BYTES;
+                // a stage has columns of its own for its scales, so what reads them is done when they are written again
+                const uint32_t s_addr = smem_u32(smem) + s * STAGE_BYTES + W_BYTES + X_BYTES, scales = tmem + 2 * BN + 16 * s;
+                const uint32_t step = s * (STAGE_BYTES >> 4);
+                if (issues) {
                     fl_copy_scales(scales, s_addr);
                     fl_copy_scales(scales + 4, s_addr + 512);
                     fl_copy_scales(scales + 8, s_addr + FL_CHUNK);
                     fl_copy_scales(scales + 12, s_addr + FL_CHUNK + 512);
-                    fl_mma_x4(tmem + buf * BN, smem_desc(w_addr), smem_desc(w_addr + W_BYTES), idesc0, idesc1, scales,
-                              scales + 8 + rows_at, scales + 4, scales + 12 + rows_at, j > 0 ? 1u : 0u);
+                    fl_mma_x4(tmem + buf * BN, w_desc + step, x_desc + step, idesc0, idesc1, scales, scales + 8 + rows_at, scales + 4,
+                              scales + 12 + rows_at, j > 0 ? 1u : 0u);
                     tc_commit(empty0 + 8 * s);
-                    if (++s == STAGES) { s = 0; lap ^= 1; }
                 }
-                if (ok) tc_commit(acc_full0 + 8 * buf);
-                u += n;
+                __syncwarp();
+                if (++s == STAGES) { s = 0; lap ^= 1; }
             }
+            if (ok && issues) tc_commit(acc_full0 + 8 * buf);
+            __syncwarp();
+            u += n;
         }
     } else {
         if (!LIST) ssb_pdl_wait();
@@ -367,7 +282,7 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                             // lanes 0-15 finish row j, lanes 16-31 row j + 1
                             const float own = up ? sum[j + 1] : sum[j], give = up ? sum[j] : sum[j + 1];
                             const float got = __shfl_xor_sync(0xffffffffu, give, 16);
-                            float z = ssb_gate(up ? got : own, up ? own : got, o.kind, o.limit);
+                            float z = ssb_gate_fast(up ? got : own, up ? own : got, o.kind, o.limit);
                             const int r = c0 + j + (up ? 1 : 0);
                             if (o.row_scale && r < rows) z *= o.row_scale[m0 + r];
                             inner[(j + (up ? 1 : 0)) * FL_INNER_LD + at_ch] = z;
@@ -417,29 +332,22 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 // columns: two accumulators of 256 that share 128 of them, and five times 24 for a k-block's scales.  An epilogue begins with the
 // columns that the next tile wants, and hands them over as soon as they are in registers.
 //
-// Scales are brought to tensor memory by four warps with tcgen05.st: tcgen05.cp runs in order with the products and took 0.19 us of a
-// k-block's 0.66 (six of them; 8,192 x 14,336 x 4,096: 266 us).  They come through a ring of their own, by cp.async: a TMA copy is behind
-// the codes that were asked for before it, and the way through registers then has to be waited for (357 us).
+// Scales come to tensor memory through the registers of four warps (tcgen05.st), which fetch them some k-blocks ahead: tcgen05.cp runs
+// in order with the products and took 0.19 us of a k-block's 0.66 (six of them; 8,192 x 14,336 x 4,096: 266 us); through shared memory
+// by TMA they stand behind the codes that were asked for before them (357 us), and by cp.async a k-block takes these warps 850 clocks.
 //
 // Tiles go in bands of ``group_m`` row tiles, row tiles fastest; of experts (LIST), a list's tile of rows with all its channels.
 constexpr int FL_PAIR_STAGES = 6;
 constexpr int FL_PAIR_STAGE_BYTES = 2 * FL_BM * FL_ROW;
-constexpr int FL_PAIR_RING = 4;           // k-blocks of scales in shared memory
-constexpr int FL_PAIR_SETS = 5;           // and in tensor memory
+constexpr int FL_PAIR_SETS = 5;           // k-blocks whose scales are in tensor memory
+constexpr int FL_PAIR_AHEAD = 3;          // and in registers, on their way
 constexpr int FL_PAIR_ACC = 128;          // columns from the first accumulator to the second
 constexpr int FL_PAIR_SCALES = 384;       // scales' first column
 constexpr int FL_PAIR_WARPS = 14;         // 0: TMA, 1: MMA + tensor memory, 2-5: scales, 6-13: epilogue
 constexpr int FL_PAIR_PUT = 32 * 20;      // words in which an epilogue warp's rows meet
 constexpr int FL_PAIR_BARS = 2 * FL_PAIR_STAGES + FL_PAIR_SETS + 3;
-constexpr size_t FL_PAIR_SMEM = (size_t)FL_PAIR_STAGES * FL_PAIR_STAGE_BYTES + FL_PAIR_RING * 3 * F4_CHUNK + 8 * FL_PAIR_PUT * 4 + FL_PAIR_BARS * 8 + 24 + 1024;
+constexpr size_t FL_PAIR_SMEM = (size_t)FL_PAIR_STAGES * FL_PAIR_STAGE_BYTES + 8 * FL_PAIR_PUT * 4 + FL_PAIR_BARS * 8 + 24 + 1024;
 
-__device__ __forceinline__ void fl_cp16(uint32_t dst, const void* src, bool live) {         // zeros where it is not live
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void fl_st8(uint32_t taddr, const uint4& a, const uint4& b) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"r"(taddr), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
-}
 // tc_put_rows with a place for each row: ``at``, the lane's row of dst.
 template <int WORDS, bool ADD>
 __device__ __forceinline__ void fl_put_rows(float* stage, const uint32_t* v, char* dst, size_t row_bytes, int at, int rows) {
@@ -471,8 +379,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     constexpr uint32_t X_BYTES = FL_BM * FL_ROW, W_BYTES = FL_BM * FL_ROW, STAGE_BYTES = FL_PAIR_STAGE_BYTES;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    unsigned char* ring = smem + STAGES * STAGE_BYTES;
-    float* put = (float*)(ring + FL_PAIR_RING * 3 * FL_CHUNK);
+    float* put = (float*)(smem + STAGES * STAGE_BYTES);
     uint64_t* bars = (uint64_t*)(put + 8 * FL_PAIR_PUT);            // full, empty [STAGES], ready [SETS], acc_full[2], free
     uint32_t* tmem_slot = (uint32_t*)(bars + FL_PAIR_BARS);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
@@ -546,88 +453,88 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             constexpr uint32_t idesc0 = fl_idesc(256, BN, 0), idesc1 = fl_idesc(256, BN, 1);
+            const bool issues = fl_elect();
+            const uint64_t x_desc = smem_desc(smem_u32(smem)), w_desc = smem_desc(smem_u32(smem) + X_BYTES);
             bool ok = true;
-            int c = 0, i = 0;
+            int i = 0, s = 0, set = 0;
+            uint32_t lap = 0, set_lap = 0;
             for (int tile = pair; tile < tiles && ok; tile += n_pairs, ++i) {
                 const uint32_t acc = tmem + (i & 1) * FL_PAIR_ACC;
-                if (i > 0 && !mbar_wait(free0, (i - 1) & 1, abort_flag)) {    // both epilogues have the shared columns
-                    *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
-                }
-                for (int kb = 0; kb < k_blocks && ok; ++kb, ++c) {
-                    const int s = c % STAGES, set = c % FL_PAIR_SETS;
-                    if (!mbar_wait(ready0 + 8 * set, (c / FL_PAIR_SETS) & 1, abort_flag) || !mbar_wait(full0 + 8 * s, (c / STAGES) & 1, abort_flag)) {
-                        *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break;
-                    }
+                if (i > 0) ok = mbar_wait(free0, (i - 1) & 1, abort_flag);            // both epilogues have the shared columns
+                if (!__all_sync(0xffffffffu, ok)) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break; }
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    ok = mbar_wait(ready0 + 8 * set, set_lap, abort_flag) && mbar_wait(full0 + 8 * s, lap, abort_flag);
+                    if (!__all_sync(0xffffffffu, ok)) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); ok = false; break; }
                     tc_fence_after();
-                    const uint32_t x_addr = smem_u32(smem + s * STAGE_BYTES), x_sc = tmem + FL_PAIR_SCALES + set * 24, w_sc = x_sc + 8;
-                    fl_mma_pair_x4(acc, smem_desc(x_addr), smem_desc(x_addr + X_BYTES), idesc0, idesc1, x_sc, w_sc, x_sc + 4, w_sc + 8, kb > 0 ? 1u : 0u);
-                    tc_commit_pair(empty0 + 8 * s, 3);              // the stage is free in both blocks
+                    const uint32_t x_sc = tmem + FL_PAIR_SCALES + set * 24, w_sc = x_sc + 8, step = s * (STAGE_BYTES >> 4);
+                    if (issues) {
+                        fl_mma_pair_x4(acc, x_desc + step, w_desc + step, idesc0, idesc1, x_sc, w_sc, x_sc + 4, w_sc + 8, kb > 0 ? 1u : 0u);
+                        tc_commit_pair(empty0 + 8 * s, 3);          // the stage is free in both blocks
+                    }
+                    __syncwarp();
+                    if (++s == STAGES) { s = 0; lap ^= 1; }
+                    if (++set == FL_PAIR_SETS) { set = 0; set_lap ^= 1; }
                 }
-                if (ok) tc_commit_pair(acc_full0 + 8 * (i & 1), 3);
+                if (ok && issues) tc_commit_pair(acc_full0 + 8 * (i & 1), 3);
+                __syncwarp();
             }
         }
     } else if (warp < 6) {
         // a lane's 16 bytes of each 512 are four columns of its lane, in this warp's quarter of the lanes as in the others
         const uint32_t leader_ready0 = cluster_map(ready0, 0), columns = tmem + FL_PAIR_SCALES + ((uint32_t)(warp & 3) << 21);
-        const int runs = (o.N + FL_BM - 1) / FL_BM, who = threadIdx.x - 64;       // runs of a weight matrix's scales
-        // what is loaded next: k-block ahead_kb of tile ahead_tile; 192 pieces of 16 bytes, a row's run, then two of channels
-        int ahead_tile = pair, ahead_kb = 0, slot_in = 0;
-        const uint8_t *src_x = xs, *src_0 = ws, *src_1 = ws;
-        bool live_x = false, live_1 = false;
-        auto load = [&]() {
-            if (ahead_tile < tiles) {
-                if (ahead_kb == 0) {
-                    int m, n;
-                    tile_at(ahead_tile, m, n);
-                    const int run_x = 2 * m + (int)rank, run_w = (LIST ? list.tile_expert[m] : 0) * runs + 2 * n;
-                    live_x = run_x < x_runs;                        // behind the last run: zeros
-                    live_1 = 2 * n + 1 < runs;
-                    src_x = xs + (size_t)(live_x ? run_x : 0) * k_blocks * FL_CHUNK;
-                    src_0 = ws + (size_t)run_w * k_blocks * FL_CHUNK;
-                    src_1 = live_1 ? src_0 + (size_t)k_blocks * FL_CHUNK : ws;
-                }
-                const size_t at = (size_t)ahead_kb * FL_CHUNK + (who & 63) * 16;
-                const uint32_t dst = smem_u32(ring + slot_in * 3 * FL_CHUNK) + who * 16;
-                fl_cp16(dst, (who < 64 ? src_x : src_0) + at, who < 64 ? live_x : true);
-                if (who < 64) fl_cp16(dst + 2 * FL_CHUNK, src_1 + at, live_1);
-                if (++ahead_kb == k_blocks) { ahead_kb = 0; ahead_tile += n_pairs; }
+        const int runs = (o.N + FL_BM - 1) / FL_BM;                 // of a weight matrix's scales
+        // what is fetched next: k-block in_kb of tile in_tile; of rows x, of channels 0-127 a, 128-255 b, blocks 0-3 and 4-7
+        struct { uint4 x0, x1, a0, a1, b0, b1; } w[FL_PAIR_AHEAD];
+        int in_tile = pair, in_kb = 0;
+        const uint8_t *src_x = xs, *src_a = ws, *src_b = ws;
+        bool live_x = false, live_b = false;                        // behind the last run: zeros
+        auto load = [&](auto& to) {
+            if (in_tile >= tiles) return;
+            if (in_kb == 0) {
+                int m, n;
+                tile_at(in_tile, m, n);
+                const int run_x = 2 * m + (int)rank, run_w = (LIST ? list.tile_expert[m] : 0) * runs + 2 * n;
+                live_x = run_x < x_runs;
+                live_b = 2 * n + 1 < runs;
+                src_x = xs + (size_t)(live_x ? run_x : 0) * k_blocks * FL_CHUNK + lane * 16;
+                src_a = ws + (size_t)run_w * k_blocks * FL_CHUNK + lane * 16;
+                src_b = live_b ? src_a + (size_t)k_blocks * FL_CHUNK : src_a;
             }
-            if (++slot_in == FL_PAIR_RING) slot_in = 0;
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            const size_t at = (size_t)in_kb * FL_CHUNK;
+            auto get = [&](const uint8_t* p, bool live) { return live ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0); };
+            to.x0 = get(src_x + at, live_x); to.x1 = get(src_x + at + 512, live_x);
+            to.a0 = get(src_a + at, true); to.a1 = get(src_a + at + 512, true);
+            to.b0 = get(src_b + at, live_b); to.b1 = get(src_b + at + 512, live_b);
+            if (++in_kb == k_blocks) { in_kb = 0; in_tile += n_pairs; }
         };
-        for (int i = 0; i < FL_PAIR_RING - 1; ++i) load();
-        int c = 0;
+#pragma unroll
+        for (int q = 0; q < FL_PAIR_AHEAD; ++q) load(w[q]);
+        const int my_tiles = pair < tiles ? (tiles - pair + n_pairs - 1) / n_pairs : 0, all = my_tiles * k_blocks;
         bool ok = true;
-        for (int tile = pair; tile < tiles && ok; tile += n_pairs)
-            for (int kb = 0; kb < k_blocks && ok; ++kb, ++c) {
-                const int slot = c % FL_PAIR_RING, set = c % FL_PAIR_SETS, before = c - FL_PAIR_SETS;
-                asm volatile("cp.async.wait_group %0;" ::"n"(FL_PAIR_RING - 2) : "memory");
+        for (int c0 = 0; c0 < all && ok; c0 += FL_PAIR_AHEAD) {
+#pragma unroll
+            for (int q = 0; q < FL_PAIR_AHEAD; ++q) {
+                const int c = c0 + q, set = c % FL_PAIR_SETS, before = c - FL_PAIR_SETS;
+                if (c >= all || !ok) continue;
                 // the set's last products are done
-                if (before >= 0) ok = mbar_wait(empty0 + 8 * (before % STAGES), (before / STAGES) & 1, abort_flag);
-                // the four warps go on together or not at all; what they copied is there, and the slot before this one has been read
-                uint32_t bad;
-                asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, 2, 128, p;\nselp.b32 %0, 1, 0, q;\n}"
-                             : "=r"(bad) : "r"((uint32_t)!ok) : "memory");
-                ok = !bad;
+                if (before >= 0) ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * (before % STAGES), (before / STAGES) & 1, abort_flag));
                 if (!ok) {
                     if (lane == 0) { *abort_flag = 1; atomicCAS(error_word, 0, TC_ERR_MMA); }
-                    break;
+                    continue;
                 }
                 tc_fence_after();
-                load();
-                const uint4* src = reinterpret_cast<const uint4*>(ring + slot * 3 * FL_CHUNK) + lane;
-                const uint4 x0 = src[0], x1 = src[32], a0 = src[64], a1 = src[96], b0 = src[128], b1 = src[160];
-                fl_st8(columns + set * 24, x0, x1);                 // rows: blocks 0-3, 4-7
-                fl_st8(columns + set * 24 + 8, a0, b0);             // blocks 0-3: channels 0-127, 128-255
-                fl_st8(columns + set * 24 + 16, a1, b1);            // blocks 4-7
+                fl_st8(columns + set * 24, w[q].x0, w[q].x1);       // rows: blocks 0-3, 4-7
+                fl_st8(columns + set * 24 + 8, w[q].a0, w[q].b0);   // blocks 0-3: channels 0-127, 128-255
+                fl_st8(columns + set * 24 + 16, w[q].a1, w[q].b1);  // blocks 4-7
+                load(w[q]);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) fl_arrive_leader(leader_ready0 + 8 * set);
             }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
     } else {
         const int quarter = warp & 3, half = (warp - 6) >> 2;
         float* stage = put + (warp - 6) * FL_PAIR_PUT;
@@ -744,31 +651,6 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
-// codes: rows of ``row_bytes`` bytes, boxes of box_rows x 128 bytes
-static int fl_map(CUtensorMap* map, const void* base, long long rows, int row_bytes, int box_rows) {
-    EncodeTiledFn enc = encode_tiled();
-    if (!enc) return SSB_ERR_UNSUPPORTED;
-    cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
-    cuuint32_t box[2] = {FL_ROW, (cuuint32_t)box_rows};
-    cuuint32_t elem[2] = {1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : SSB_ERR_BAD_SIZE;
-}
-// scales: ``chunks`` of 1,024 bytes, a chunk a box
-static int fl_scale_map(CUtensorMap* map, const void* base, long long chunks) {
-    EncodeTiledFn enc = encode_tiled();
-    if (!enc) return SSB_ERR_UNSUPPORTED;
-    cuuint64_t dims[2] = {F4_CHUNK / 4, (cuuint64_t)chunks};
-    cuuint64_t strides[1] = {F4_CHUNK};
-    cuuint32_t box[2] = {F4_CHUNK / 4, 1};
-    cuuint32_t elem[2] = {1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : SSB_ERR_BAD_SIZE;
-}
-
 struct FlPlan {
     int bn, m_tiles, n_tiles, blocks;      // bn 0: tiles on pairs
     size_t pieces;                         // bytes
@@ -816,17 +698,16 @@ struct FlScratch {
         all = pieces + std::max<size_t>(piece_bytes, 16);
     }
 };
-// Rows that come as numbers and run in the kernel of few rows are quantised by each of its blocks, up to this many numbers: us with
-// and without a launch of their own, see fl_product.
-constexpr long long FL_FUSED_NUMBERS = 32768;
+// The kernel of few rows takes products where there is little to read; where the weights' bytes count, its instructions a weight do too
+// (fl_product).
+constexpr long long FL_FEW_NUMBERS = 32768, FL_FEW_WEIGHTS = 5 << 20;
+static bool fl_few(int M, int N, int K, int mode) {
+    return (long long)M * K <= FL_FEW_NUMBERS && (long long)N * K <= FL_FEW_WEIGHTS && fw_takes(M, N, K, mode);
+}
 
 // Twice the bytes of scratch that a product needs, and one if it needs counters.  numbers: rows come as numbers; mode: FL_*.
 SSB_API long long ssb_fp4_product_scratch(int M, int N, int K, int numbers, int mode) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
-    if (fw_takes(M, N, K, mode)) {
-        if (!numbers || (long long)M * K <= FL_FUSED_NUMBERS) return 0;
-        return 2 * (long long)FlScratch(M, K, true, 0).all;
-    }
+    if (M <= 0 || N <= 0 || K <= 0 || fl_few(M, N, K, mode)) return 0;
     return 2 * (long long)FlScratch(M, K, numbers != 0, fl_plan(M, N, K).pieces).all + 1;
 }
 
@@ -890,7 +771,7 @@ static int fl_dense(const void* x, const void* xs, const void* w, const void* ws
     if (rc) return rc;
     const FlTiles none{};
     switch (p.bn) {
-        case 16: return fl_stream<16, 10, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
+        case 16: return fl_stream<16, 5, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
         case 32: return fl_stream<32, 9, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
         case 64: return fl_stream<64, 8, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
         case 128: return fl_stream<128, 6, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
@@ -899,7 +780,7 @@ static int fl_dense(const void* x, const void* xs, const void* w, const void* ws
 }
 
 SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* codes, void* scales, int rows, int K, int per_expert, int inter,
-                             int* clear, int n_clear, cudaStream_t stream);
+                             int* clear, int n_clear, int early, cudaStream_t stream);
 SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void* codes, void* scales, int pairs, int top, int K,
                                    const int* slot, int tile_rows, cudaStream_t stream);
 
@@ -912,20 +793,8 @@ static int fl_product(const void* x, long long ldx, int dtype, const void* xs, c
     if (o.M < 0 || o.N <= 0 || K <= 0 || K % F4_BLOCK || o.N % 8 || dtype > SSB_BF16) return SSB_ERR_BAD_SIZE;
     if (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws | (uintptr_t)o.out | (uintptr_t)o.scales | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
     if (o.M == 0) return 0;
-    const bool few = fw_takes(o.M, o.N, K, MODE), first = dtype >= 0 && !(few && (long long)o.M * K <= FL_FUSED_NUMBERS);
-    if (((first || !few) && !scratch) || (!few && (!counters || !error_word))) return SSB_ERR_BAD_SIZE;
-    const FlPlan p = few ? FlPlan{} : fl_plan(o.M, o.N, K);
-    if (p.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
-    const FlScratch at(o.M, K, dtype >= 0, p.pieces);
-    char* base = (char*)scratch;
-    if (first) {
-        const int rc = ssb_fp4_quantize(x, ldx, dtype, base + at.codes, base + at.scales, o.M, K, o.M, 0, few ? nullptr : counters,
-                                        few ? 0 : n_clear, stream);
-        if (rc) return rc;
-        x = base + at.codes;
-        xs = base + at.scales;
-        dtype = -1;
-    }
+    const bool few = fl_few(o.M, o.N, K, MODE);
+    if (!error_word || (!few && (!scratch || !counters))) return SSB_ERR_BAD_SIZE;
     if (few) {
         FwArgs a{};
         a.w = (const uint8_t*)w; a.ws = (const uint8_t*)ws;
@@ -934,6 +803,16 @@ static int fl_product(const void* x, long long ldx, int dtype, const void* xs, c
         a.M = o.M; a.N = o.N; a.K = K;
         a.kind = o.kind; a.limit = o.limit; a.row_scale = o.row_scale; a.inner_blocks = o.inner_blocks;
         return fw_product(a, MODE, stream);
+    }
+    const FlPlan p = fl_plan(o.M, o.N, K);
+    if (p.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
+    const FlScratch at(o.M, K, dtype >= 0, p.pieces);
+    char* base = (char*)scratch;
+    if (dtype >= 0) {
+        const int rc = ssb_fp4_quantize(x, ldx, dtype, base + at.codes, base + at.scales, o.M, K, o.M, 0, counters, n_clear, 1, stream);
+        if (rc) return rc;
+        x = base + at.codes;
+        xs = base + at.scales;
     }
     return fl_dense<MODE>(x, xs, w, ws, o, K, counters, (float*)(base + at.pieces), p, error_word, stream);
 }
@@ -1056,13 +935,17 @@ static int fl_list_rows(int tokens, int top, int experts) {
     const long long mean = (long long)tokens * top / experts;
     return tokens <= 16 || mean <= 8 ? 16 : tokens <= 32 || mean <= 16 ? 32 : tokens <= 64 || mean <= 48 ? 64 : mean <= 96 ? 128 : 256;
 }
+// Whether experts run in the kernel of few rows.
+static bool fl_few_pairs(int pairs, int experts, int K, int inter) {
+    return pairs <= 16 && fw_takes_list(pairs, experts, 2 * inter, K, FL_GATED) && fw_takes_list(pairs, experts, K, inter, FL_STORE);
+}
 struct FlExperts {
     int bn, tiles, blocks;                 // rows a tile, tiles at most, blocks of a product
     size_t counters, offsets, order, slot, tile_expert, tile_row0, meta, x, xs, z, zs, y, pieces, all;
     bool few;                              // by the kernel of few rows, which needs no list
-    FlExperts(int tokens, int top, int experts, int K, int inter, bool gated) {
-        const int pairs = tokens * top, N1 = gated ? 2 * inter : inter;
-        few = fw_takes_list(pairs, experts, N1, K, gated ? FL_GATED : FL_ACT) && fw_takes_list(pairs, experts, K, inter, FL_STORE);
+    FlExperts(int tokens, int top, int experts, int K, int inter) {
+        const int pairs = tokens * top;
+        few = fl_few_pairs(pairs, experts, K, inter);
         if (few) {
             z = 0;
             zs = fl_round((size_t)pairs * (inter / 2));
@@ -1094,7 +977,7 @@ struct FlExperts {
 };
 SSB_API long long ssb_fp4_experts_scratch(int tokens, int top, int experts, int K, int inter, int gated) {
     if (tokens <= 0 || top <= 0 || experts <= 0 || K <= 0 || inter <= 0) return 0;
-    return (long long)FlExperts(tokens, top, experts, K, inter, gated != 0).all;
+    return (long long)FlExperts(tokens, top, experts, K, inter).all;
 }
 
 template <int MODE>
@@ -1108,7 +991,7 @@ static int fl_listed(const void* x, const void* xs, const void* w, const void* w
     if (!rc) rc = fl_scale_map(&mws, ws, (long long)experts * n_tiles * k_blocks);
     if (rc) return rc;
     switch (at.bn) {
-        case 16: return fl_stream<16, 10, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+        case 16: return fl_stream<16, 5, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
         case 32: return fl_stream<32, 9, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
         case 64: return fl_stream<64, 8, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
         case 128: return fl_stream<128, 6, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
@@ -1125,7 +1008,7 @@ SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* 
     if (((uintptr_t)x | (uintptr_t)w1 | (uintptr_t)ws1 | (uintptr_t)w2 | (uintptr_t)ws2 | (uintptr_t)out | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
     if ((dtype != SSB_F32 && dtype != SSB_BF16) || (out_dtype != SSB_F32 && out_dtype != SSB_BF16) || (add && out_dtype != SSB_F32)) return SSB_ERR_BAD_DTYPE;
     if (tokens == 0) return 0;
-    const FlExperts at(tokens, top, experts, K, inter, gated != 0);
+    const FlExperts at(tokens, top, experts, K, inter);
     char* base = (char*)scratch;
     const int pairs = tokens * top, N1 = gated ? 2 * inter : inter;
     float* y = (float*)(base + at.y);

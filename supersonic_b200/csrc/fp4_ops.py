@@ -28,13 +28,13 @@ from .ops import KernelError, _CODES, _check
 
 _P, _I, _F, _L = c_void_p, c_int, c_float, c_longlong
 _SIGNATURES = {
-    "ssb_fp4_quantize": [_P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _I, _P],
+    "ssb_fp4_quantize": [_P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _P],
     "ssb_fp4_values": [_P, _P, _P, _L, _I, _I, _I, _I, _I, _P],
     "ssb_fp4_linear": [_P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P],
     "ssb_fp4_inner": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P],
     "ssb_fp4_experts": [_P, _L, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
     "ssb_fp4_product_scratch": [_I] * 5,
-    "ssb_fp4_experts_scratch": [_I] * 6,
+    "ssb_fp4_experts_scratch": [_I] * 5,
 }
 _FORMATS = {_P: "P", _I: "i", _F: "f", _L: "q"}
 _functions = {}
@@ -102,7 +102,7 @@ def quantize(x: torch.Tensor, matrix: Fp4Matrix) -> None:
     at, ld, rows, code = _matrix_rows(x, "x", matrix)
     n, k = matrix.shape[-2:]
     _check(_fn("ssb_fp4_quantize")(at, ld, code, matrix.codes_at, matrix.scales_at, rows, k, n,
-                                   n // 2 if matrix.gated else 0, 0, 0, _stream()), "fp4_quantize")
+                                   n // 2 if matrix.gated else 0, 0, 0, 0, _stream()), "fp4_quantize")
 
 
 def values(matrix: Fp4Matrix, out: torch.Tensor) -> None:
@@ -179,7 +179,7 @@ def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = Fal
     needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_STORE)
     held, scratch, counters = _workspace(x, needs, device, _COUNTERS)
     _check(_fn("ssb_fp4_linear")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, o_at, ldo, _CODES[out.dtype], rows, n, k,
-                                 1 if accumulate else 0, scratch, counters, _error_word(device) if counters else 0, _stream()), "fp4_linear")
+                                 1 if accumulate else 0, scratch, counters, _error_word(device), _stream()), "fp4_linear")
 
 
 def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_scale: Optional[torch.Tensor]) -> Fp4Matrix:
@@ -202,7 +202,7 @@ def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_s
     z = Fp4Matrix.over_rows(buffer, rows, inter, size)
     _check(_fn("ssb_fp4_inner")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, z.codes_at, z.scales_at, rows, n, k,
                                 1 if gated else 0, kind, limit, 0 if row_scale is None else row_scale.data_ptr(), scratch, counters,
-                                _error_word(device) if counters else 0, _stream()), "fp4_inner")
+                                _error_word(device), _stream()), "fp4_inner")
     if counters:
         z._counters = (held, counters + 4 * _COUNTERS)
     return z
@@ -271,7 +271,7 @@ def experts(x: torch.Tensor, expert_of: torch.Tensor, pair_weight: torch.Tensor,
         raise KernelError(f"experts: {tokens} tokens of {top} choices among {E} experts are more than {MOST_PAIRS} pairs or 4096 experts")
     if tokens == 0:
         return
-    scratch = torch.empty(_scratch_size("ssb_fp4_experts_scratch", tokens, top, E, k, inter, first.gated), dtype=torch.int8, device=device)
+    scratch = torch.empty(_scratch_size("ssb_fp4_experts_scratch", tokens, top, E, k, inter), dtype=torch.int8, device=device)
     _check(_fn("ssb_fp4_experts")(x_at, ldx, _CODES[x.dtype], expert_of.data_ptr(), pair_weight.data_ptr(), first.codes_at,
                                   first.scales_at, down.codes_at, down.scales_at, o_at, ldo, _CODES[out.dtype],
                                   tokens, top, E, k, inter, 1 if first.gated else 0, kinds[kind], float(limit), 1 if accumulate else 0,

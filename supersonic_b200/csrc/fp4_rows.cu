@@ -32,11 +32,11 @@ struct FrStep {
 template <typename T, int TURNS>
 __global__ void __launch_bounds__(FR_THREADS)
 fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int rows, int K,
-                    const FrRows to, const FrStep step, int k_blocks, int* __restrict__ clear, int n_clear) {
+                    const FrRows to, const FrStep step, int k_blocks, int* __restrict__ clear, int n_clear, int early) {
     const int lane = threadIdx.x & 15, u = blockIdx.x * (FR_THREADS / 16) + (threadIdx.x >> 4);
     int row = u / step.per_row, part = u - row * step.per_row;
     ssb_pdl_wait();
-    ssb_pdl_launch_dependents();                               // what was written before this launch is there: weights may be read ahead
+    if (early) ssb_pdl_launch_dependents();                    // what was written before this launch is there: weights may be read ahead
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < n_clear; i += FR_THREADS) clear[i] = 0;
     // the half-warps of a warp go on together: a later unit is in no earlier row
@@ -149,24 +149,25 @@ static int fr_sizes(int rows, int K, int per_expert, int inter) {
 
 template <typename T>
 static int fr_quantize(const T* x, long long ldx, uint8_t* codes, uint8_t* scales, int rows, int K, const FrRows& to, int* clear, int n_clear,
-                       cudaStream_t stream) {
+                       int early, cudaStream_t stream) {
     const int k_blocks = f4_k_blocks(K);
     int blocks, turns;
     const FrStep step = fr_step(rows, 2 * k_blocks, &blocks, &turns);
     if ((long long)rows + step.rows * 4LL + 4 > INT_MAX) return SSB_ERR_BAD_SIZE;
     return ssb_launch(turns == 1 ? fp4_quantize_kernel<T, 1> : fp4_quantize_kernel<T, FR_TURNS>, dim3(blocks), dim3(FR_THREADS), 0, stream, true,
-                      x, ldx, codes, scales, rows, K, to, step, k_blocks, clear, n_clear);
+                      x, ldx, codes, scales, rows, K, to, step, k_blocks, clear, n_clear, early);
 }
 
-// x: rows x K, rows of 16-byte pieces; ``per_expert`` rows of them are a matrix; clear: words zeroed on the way.
+// x: rows x K, rows of 16-byte pieces; ``per_expert`` rows of them are a matrix; clear: words zeroed on the way.  early: the next
+// launch may begin meanwhile, which it must not if it takes the codes for weights and reads ahead.
 SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* codes, void* scales, int rows, int K, int per_expert, int inter,
-                             int* clear, int n_clear, cudaStream_t stream) {
+                             int* clear, int n_clear, int early, cudaStream_t stream) {
     const int rc = fr_sizes(rows, K, per_expert, inter);
     if (rc || rows == 0) return rc;
     if (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales) & 15) return SSB_ERR_BAD_SIZE;
     const FrRows to{per_expert, inter, nullptr, 1, 128};
-    if (dtype == SSB_BF16) return fr_quantize((const bf16*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, rows, K, to, clear, n_clear, stream);
-    if (dtype == SSB_F32) return fr_quantize((const float*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, rows, K, to, clear, n_clear, stream);
+    if (dtype == SSB_BF16) return fr_quantize((const bf16*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, rows, K, to, clear, n_clear, early, stream);
+    if (dtype == SSB_F32) return fr_quantize((const float*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, rows, K, to, clear, n_clear, early, stream);
     return SSB_ERR_BAD_DTYPE;
 }
 
@@ -174,8 +175,8 @@ SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* code
 SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void* codes, void* scales, int pairs, int top, int K,
                                    const int* slot, int tile_rows, cudaStream_t stream) {
     const FrRows to{pairs, 0, slot, top, tile_rows};
-    if (dtype == SSB_BF16) return fr_quantize((const bf16*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, pairs, K, to, nullptr, 0, stream);
-    if (dtype == SSB_F32) return fr_quantize((const float*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, pairs, K, to, nullptr, 0, stream);
+    if (dtype == SSB_BF16) return fr_quantize((const bf16*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, pairs, K, to, nullptr, 0, 1, stream);
+    if (dtype == SSB_F32) return fr_quantize((const float*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, pairs, K, to, nullptr, 0, 1, stream);
     return SSB_ERR_BAD_DTYPE;
 }
 
