@@ -8,8 +8,6 @@
 // as many instructions, are taken apart into float16 ones by the compiler: 36 million instructions for what takes half of them so.)
 // tcgen05 with its own scales needs a tile's 128 channels and their rows in tensor memory before the first product and a way back after
 // the last: one row x 2,048 x 2,048 takes it 8.3 us.
-//
-// The same for experts: every block sorts the step's pairs (token, choice) by expert for itself, a tile is up to 8 rows of an expert.
 #include "fp4_codes.cuh"
 #include "fp4_few.cuh"
 #include <algorithm>
@@ -49,7 +47,7 @@ __device__ __forceinline__ void fw_cp4(uint32_t dst, const void* src, bool live)
 // A row's codes in shared memory, 16 bytes more than whole k-blocks apart: eight rows' pieces meet no bank twice.
 __host__ __device__ constexpr int fw_row_bytes(int k_blocks) { return k_blocks * 128 + 16; }
 
-template <int NB, int MODE, bool LIST>
+template <int NB, int MODE>
 __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) {
     constexpr int ROWS = 8 * NB;
     extern __shared__ __align__(16) unsigned char fw_smem[];
@@ -59,16 +57,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
     unsigned char* x_s = fw_smem;                                    // [ROWS][row_bytes]
     float* sx_s = (float*)(x_s + ROWS * row_bytes);                  // [all_blocks][ROWS]
     float* red = sx_s + all_blocks * ROWS;                           // [2][k_warps][ROWS][LD]
-    int* list_s = (int*)(red + 2 * a.k_warps * ROWS * LD);           // LIST: [4][FW_MOST_PAIRS] + 1
-    int *pair_of = list_s, *tile_first = list_s + FW_MOST_PAIRS, *tile_rows = tile_first + FW_MOST_PAIRS, *tile_expert = tile_rows + FW_MOST_PAIRS;
-    unsigned char* ring = (unsigned char*)(LIST ? list_s + 4 * FW_MOST_PAIRS + 4 : list_s) + warp * a.slots * FW_SLOT;
-
-    int tiles = 1;
-    if (LIST) {
-        ssb_pdl_wait();
-        tiles = fw_sort_pairs<ROWS>(a.expert_of, a.pairs, a.experts, pair_of, tile_first, tile_rows, tile_expert);
-    }
-    const int c_tiles = (a.N + CH - 1) / CH, items = tiles * c_tiles;
+    unsigned char* ring = (unsigned char*)(red + 2 * a.k_warps * ROWS * LD) + warp * a.slots * FW_SLOT;
+    const int items = (a.N + CH - 1) / CH;
     const int begin = (int)((long long)items * blockIdx.x / gridDim.x), end = (int)((long long)items * (blockIdx.x + 1) / gridDim.x);
     const int steps = kw < a.k_blocks ? (a.k_blocks - kw + a.k_warps - 1) / a.k_warps : 0;      // of this warp, a tile
 
@@ -79,14 +69,13 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
     auto load = [&]() {
         if (in_item < end && steps > 0) {
             if (in_step == 0) {
-                const int tile = LIST ? in_item / c_tiles : 0, e = LIST ? tile_expert[tile] : 0, ch0 = (in_item - tile * c_tiles) * CH + cg * 16;
-                const int runs = (a.N + 127) >> 7, ch = ch0 + (lane >> 1);
-                src = a.w + ((size_t)e * a.N + min(ch0, a.N - 1)) * (a.K / 2);      // clamped where nothing is read
+                const int ch0 = in_item * CH + cg * 16, ch = ch0 + (lane >> 1);
+                src = a.w + (size_t)min(ch0, a.N - 1) * (a.K / 2);                  // clamped where nothing is read
 #pragma unroll
                 for (int q = 0; q < 4; ++q) live_row[q] = ch0 + (lane >> 3) + 4 * q < a.N;
                 live_scale = ch < a.N;
                 const int c = live_scale ? ch : 0;
-                src_scale = a.ws + (size_t)e * runs * a.k_blocks * F4_CHUNK + f4_scale_at(c, (lane & 1) * 4, a.k_blocks);
+                src_scale = a.ws + f4_scale_at(c, (lane & 1) * 4, a.k_blocks);
             }
             const int kb = kw + in_step * a.k_warps, at = kb * 128 + (lane & 7) * 16;
             unsigned char* slot = ring + in_slot * FW_SLOT;
@@ -105,15 +94,14 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
     };
     // weights are nobody's output: the first of them come while whatever writes the rows still runs
     for (int i = 0; i + 1 < a.slots; ++i) load();
-    if (!LIST) ssb_pdl_wait();
+    ssb_pdl_wait();
     ssb_pdl_launch_dependents();
 
-    int out_slot = 0, have = -1;                                     // the tile whose rows are in shared memory
+    int out_slot = 0;
+    const int rows = a.M;
     for (int item = begin; item < end; ++item) {
-        const int tile = LIST ? item / c_tiles : 0, ch0 = (item - tile * c_tiles) * CH;
-        const int rows = LIST ? tile_rows[tile] : a.M, first = LIST ? tile_first[tile] : 0;
-        if (tile != have) {
-            have = tile;
+        const int ch0 = item * CH;
+        if (item == begin) {                                         // the rows, which stay
             if (a.dtype < 0) {
                 // 16 bytes of codes a thread and turn, a word of four blocks' scales; behind K zeros
                 const int per_row = a.k_blocks * 8, words = a.k_blocks * 2;
@@ -124,7 +112,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
                         const int u = u0 + j * FW_THREADS, r = u / per_row, at = (u - r * per_row) * 16;
                         v[j] = make_uint4(0, 0, 0, 0);
                         if (u < rows * per_row && at < a.K / 2)
-                            v[j] = *reinterpret_cast<const uint4*>((const uint8_t*)a.x + (size_t)(LIST ? pair_of[first + r] : r) * (a.K / 2) + at);
+                            v[j] = *reinterpret_cast<const uint4*>((const uint8_t*)a.x + (size_t)r * (a.K / 2) + at);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -134,7 +122,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
                 }
                 for (int u = tid; u < rows * words; u += FW_THREADS) {
                     const int r = u / words, i = u - r * words;
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(a.xs + f4_scale_at(LIST ? pair_of[first + r] : r, 4 * i, a.k_blocks));
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(a.xs + f4_scale_at(r, 4 * i, a.k_blocks));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) sx_s[(4 * i + j) * ROWS + r] = f4_scale(w >> (8 * j) & 255);
                 }
@@ -149,7 +137,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
                         if (u < units && k < a.K) {
-                            const size_t row = LIST ? pair_of[first + r] / a.top : r;
+                            const size_t row = r;
                             if (a.dtype == SSB_BF16) f4_load8((const bf16*)a.x + row * a.ldx + k, v[j]);
                             else f4_load8((const float*)a.x + row * a.ldx + k, v[j]);
                         }
@@ -238,7 +226,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
                 const int r = i / CH, ch = i - r * CH;
                 if (ch0 + ch >= a.N) continue;
                 const float s = total(r, ch);
-                const size_t at = (size_t)(LIST ? pair_of[first + r] : r) * a.ldo + ch0 + ch;
+                const size_t at = (size_t)r * a.ldo + ch0 + ch;
                 if (a.is_f32) ((float*)a.out)[at] = a.add ? ((float*)a.out)[at] + s : s;
                 else ((bf16*)a.out)[at] = __float2bfloat16_rn(s);
             }
@@ -247,19 +235,19 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
             constexpr int WIDE = MODE == FW_GATED ? 64 : 32;         // channels of W a block
             const int per = CH / WIDE, width = MODE == FW_GATED ? a.N / 2 : a.N;
             for (int i = warp; i < rows * per; i += FW_WARPS) {
-                const int r = i / per, q = i - r * per, out_row = LIST ? pair_of[first + r] : r, k = (ch0 / WIDE + q) * 32;
+                const int r = i / per, q = i - r * per, k = (ch0 / WIDE + q) * 32;
                 float z;
                 if (MODE == FW_GATED) {
                     const int ch = q * 64 + (lane >> 4) * 32 + (lane & 15);
                     z = ssb_gate_fast(total(r, ch), total(r, ch + 16), a.kind, a.limit);
-                    if (a.row_scale) z *= a.row_scale[out_row];
+                    if (a.row_scale) z *= a.row_scale[r];
                 } else {
                     z = ssb_activate(total(r, q * 32 + lane), a.kind) * a.limit;
                 }
-                f4_put_block(z, (uint8_t*)a.out + (size_t)out_row * a.ldo, a.out_scales, out_row, k, width, a.inner_blocks);
+                f4_put_block(z, (uint8_t*)a.out + (size_t)r * a.ldo, a.out_scales, r, k, width, a.inner_blocks);
                 // behind the last channel: scales of zero up to a whole k-block
                 if (q == 0 && ch0 + CH >= a.N && width / F4_BLOCK + lane < 8 * a.inner_blocks && lane < 8)
-                    a.out_scales[f4_scale_at(out_row, width / F4_BLOCK + lane, a.inner_blocks)] = 0;
+                    a.out_scales[f4_scale_at(r, width / F4_BLOCK + lane, a.inner_blocks)] = 0;
             }
         }
     }
@@ -267,15 +255,14 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
-static size_t fw_fixed(int rows, int k_blocks, int k_warps, bool list) {
+static size_t fw_fixed(int rows, int k_blocks, int k_warps) {
     const int ch = 16 * (FW_WARPS / k_warps);
-    return (size_t)rows * fw_row_bytes(k_blocks) + (size_t)k_blocks * 8 * rows * 4 + (size_t)2 * k_warps * rows * (ch + 4) * 4 +
-           (list ? (4 * FW_MOST_PAIRS + 4) * 4 : 0);
+    return (size_t)rows * fw_row_bytes(k_blocks) + (size_t)k_blocks * 8 * rows * 4 + (size_t)2 * k_warps * rows * (ch + 4) * 4;
 }
 
-template <int NB, int MODE, bool LIST>
+template <int NB, int MODE>
 static int fw_launch(const FwArgs& a, int blocks, size_t smem, cudaStream_t stream) {
-    auto kernel = fp4_few_kernel<NB, MODE, LIST>;
+    auto kernel = fp4_few_kernel<NB, MODE>;
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FW_MOST_SMEM);
@@ -284,60 +271,46 @@ static int fw_launch(const FwArgs& a, int blocks, size_t smem, cudaStream_t stre
     }
     return ssb_launch(kernel, dim3(blocks), dim3(FW_THREADS), smem, stream, true, a);
 }
-// How a product of M rows (a list: of tiles of 8) by N x K weights runs; slots 0: not by this kernel.
+
+// How a product of M rows by N x K weights runs; slots 0: not by this kernel.
 struct FwPlan { int nb, k_warps, slots, blocks; size_t smem; };
-static FwPlan fw_plan(int M, int N, int K, int mode, int tiles) {
+static FwPlan fw_plan(int M, int N, int K, int mode) {
     FwPlan p{};
     const int k_blocks = f4_k_blocks(K), sms = ssb_sm_count();
-    const bool list = tiles > 0;
     if (M > 16) return p;
-    p.nb = M <= 8 || list ? 1 : 2;
+    p.nb = M <= 8 ? 1 : 2;
     // channels a tile and warps along k: as few steps of a warp as can be, one after another on the fullest SM; a gated tile is 64
     // channels (32 inner ones, a block) at least, an ungated one of inner channels 32
-    long long least = 0;
+    long long least = 0, steps = 0;
     for (int k_warps = mode == FW_STORE ? 16 : mode == FW_GATED ? 4 : 8; k_warps >= 1; k_warps /= 2) {
-        const int ch = 16 * (FW_WARPS / k_warps), c_tiles = (N + ch - 1) / ch;
-        const long long items = (long long)std::max(tiles, 1) * c_tiles;
-        const long long cost = (items + sms - 1) / sms * (2 * ((k_blocks + k_warps - 1) / k_warps) + 1);          // a tile's end is half a step
+        const int ch = 16 * (FW_WARPS / k_warps), items = (N + ch - 1) / ch, rounds = (items + sms - 1) / sms;
+        const int deep = (k_blocks + k_warps - 1) / k_warps;
+        const long long cost = (long long)rounds * (2 * deep + 1);            // a tile's end is half a step
         if (p.k_warps && cost >= least) continue;
         least = cost;
+        steps = (long long)rounds * deep;
         p.k_warps = k_warps;
-        p.blocks = (int)std::min<long long>(items, sms);
+        p.blocks = std::min(items, sms);
     }
-    const size_t fixed = fw_fixed(8 * p.nb, k_blocks, p.k_warps, list);
+    const size_t fixed = fw_fixed(8 * p.nb, k_blocks, p.k_warps);
     if (fixed >= FW_MOST_SMEM) return p;
-    // no more than a block's steps want: what is left lets the next launch's blocks begin beside these
-    const long long items = (long long)std::max(tiles, 1) * ((N + 16 * (FW_WARPS / p.k_warps) - 1) / (16 * (FW_WARPS / p.k_warps)));
-    const long long steps = (items + sms - 1) / sms * ((k_blocks + p.k_warps - 1) / p.k_warps);
+    // no more slots than a block's steps want: what is left lets the next launch's blocks begin beside these
     p.slots = (int)std::min<long long>(std::min<long long>(5, std::max<long long>(2, steps)), (FW_MOST_SMEM - fixed) / (FW_WARPS * FW_SLOT));
     if (p.slots < 2) p.slots = 0;
     p.smem = fixed + (size_t)p.slots * FW_WARPS * FW_SLOT;
     return p;
 }
-bool fw_takes(int M, int N, int K, int mode) { return fw_plan(M, N, K, mode, 0).slots > 0; }
-bool fw_takes_list(int pairs, int experts, int N, int K, int mode) {
-    return pairs <= FW_MOST_PAIRS && pairs <= 4 * experts && fw_plan(8, N, K, mode, std::min(pairs, experts)).slots > 0;
-}
+bool fw_takes(int M, int N, int K, int mode) { return fw_plan(M, N, K, mode).slots > 0; }
 
 int fw_product(FwArgs a, int mode, cudaStream_t stream) {
-    const FwPlan p = fw_plan(a.M, a.N, a.K, mode, 0);
+    const FwPlan p = fw_plan(a.M, a.N, a.K, mode);
     if (p.slots == 0) return SSB_ERR_UNSUPPORTED;
     a.k_warps = p.k_warps;
     a.slots = p.slots;
     a.k_blocks = f4_k_blocks(a.K);
     if (p.nb == 1)
-        return mode == FW_STORE ? fw_launch<1, FW_STORE, false>(a, p.blocks, p.smem, stream)
-               : mode == FW_GATED ? fw_launch<1, FW_GATED, false>(a, p.blocks, p.smem, stream) : fw_launch<1, FW_ACT, false>(a, p.blocks, p.smem, stream);
-    return mode == FW_STORE ? fw_launch<2, FW_STORE, false>(a, p.blocks, p.smem, stream)
-           : mode == FW_GATED ? fw_launch<2, FW_GATED, false>(a, p.blocks, p.smem, stream) : fw_launch<2, FW_ACT, false>(a, p.blocks, p.smem, stream);
-}
-int fw_product_list(FwArgs a, int mode, cudaStream_t stream) {
-    const FwPlan p = fw_plan(8, a.N, a.K, mode, std::min(a.pairs, a.experts));
-    if (p.slots == 0) return SSB_ERR_UNSUPPORTED;
-    a.k_warps = p.k_warps;
-    a.slots = p.slots;
-    a.k_blocks = f4_k_blocks(a.K);
-    const int blocks = ssb_sm_count();
-    return mode == FW_STORE ? fw_launch<1, FW_STORE, true>(a, blocks, p.smem, stream)
-           : mode == FW_GATED ? fw_launch<1, FW_GATED, true>(a, blocks, p.smem, stream) : fw_launch<1, FW_ACT, true>(a, blocks, p.smem, stream);
+        return mode == FW_STORE ? fw_launch<1, FW_STORE>(a, p.blocks, p.smem, stream)
+               : mode == FW_GATED ? fw_launch<1, FW_GATED>(a, p.blocks, p.smem, stream) : fw_launch<1, FW_ACT>(a, p.blocks, p.smem, stream);
+    return mode == FW_STORE ? fw_launch<2, FW_STORE>(a, p.blocks, p.smem, stream)
+           : mode == FW_GATED ? fw_launch<2, FW_GATED>(a, p.blocks, p.smem, stream) : fw_launch<2, FW_ACT>(a, p.blocks, p.smem, stream);
 }

@@ -92,7 +92,10 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     // a tile's place: dense, tiles of rows go fastest; of a list, tiles of channels
     const int listed = LIST ? list.meta[0] : m_tiles;
     const long long units = (long long)listed * n_tiles * k_blocks;
-    const FlRange range(units, k_blocks, blockIdx.x, LIST ? (int)min((long long)gridDim.x, (units + 3) / 4) : (int)gridDim.x);
+    // of a list as many blocks as tiles, or equal parts of tiles, where there are no more tiles than blocks
+    const int list_tiles = listed * n_tiles, blocks = (int)gridDim.x;
+    const FlRange range(units, k_blocks, blockIdx.x,
+                        !LIST || list_tiles > blocks || list_tiles == 0 ? blocks : list_tiles * max(1, min(blocks / list_tiles, k_blocks / 4)));
     auto place = [&](int tile, int& m, int& n) {
         if (LIST) { m = tile / n_tiles; n = tile - m * n_tiles; }
         else { n = tile / m_tiles; m = tile - n * m_tiles; }
@@ -209,10 +212,10 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             const uint32_t acc = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
             // a block's pieces: of the tile that its range begins in the middle of (or that is all it has), and of its last; four
             // rows' sums of a channel lie together
-            auto piece = [&](int c) { return reinterpret_cast<float4*>(pieces) + (size_t)(2 * c + (c == c0_block)) * (BN / 4) * FL_BM + in_tile; };
+            auto sums_of = [&](int c) { return reinterpret_cast<float4*>(pieces) + (size_t)(2 * c + (c == c0_block)) * (BN / 4) * FL_BM + in_tile; };
             bool mine = true;                                      // whether this block writes the tile's results
             if (n < k_blocks) {
-                float4* dst = piece(blockIdx.x);
+                float4* dst = sums_of(blockIdx.x);
 #pragma unroll 1
                 for (int c0 = 0; c0 < rows; c0 += CH) {
                     float sum[CH];
@@ -248,7 +251,7 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                     for (int e = 0; e < CH; ++e) sum[e] = 0.f;
 #pragma unroll 4
                     for (int c = c0_block; c <= c1_block; ++c) {
-                        const float4* src = piece(c) + (size_t)(c0 / 4) * FL_BM;
+                        const float4* src = sums_of(c) + (size_t)(c0 / 4) * FL_BM;
 #pragma unroll
                         for (int e = 0; e < CH; e += 4) {
                             const float4 v = c0 + e < rows ? __ldcg(src + (size_t)(e / 4) * FL_BM) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -271,14 +274,16 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                             if (e < live) ((float*)o.out)[at + (size_t)e * o.ldo] = o.add ? sum[e] + was[e] : sum[e];
                     }
                 } else {
-                    // inner rows: a lane holds one channel of 16 rows, a block of 32 channels is wanted in two neighbouring lanes
-                    constexpr int WIDE = MODE == FL_GATED ? 64 : 128;                // inner channels a tile
-                    static_assert(CH == FL_INNER_ROWS, "");
+                    // inner rows: a lane holds one channel of 16 rows, a block of 32 channels is wanted in neighbouring lanes
+                    constexpr int WIDE = MODE == FL_GATED ? 64 : 128, V = WIDE / 8, PER = WIDE / V;     // inner channels a tile, a thread, threads a row
+                    static_assert(CH == FL_INNER_ROWS && CH * PER == 128, "");
+                    const int width = MODE == FL_GATED ? o.N / 2 : o.N, left = rows - c0;
                     if (MODE == FL_GATED) {
                         const bool up = lane >= 16;
                         const int at_ch = quarter * 16 + (lane & 15);
 #pragma unroll
                         for (int j = 0; j < CH; j += 2) {
+                            if (j >= left) break;
                             // lanes 0-15 finish row j, lanes 16-31 row j + 1
                             const float own = up ? sum[j + 1] : sum[j], give = up ? sum[j] : sum[j + 1];
                             const float got = __shfl_xor_sync(0xffffffffu, give, 16);
@@ -289,26 +294,23 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                         }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < CH; ++j) inner[j * FL_INNER_LD + in_tile] = ssb_activate(sum[j], o.kind) * o.limit;
+                        for (int j = 0; j < CH; ++j)
+                            if (j < left) inner[j * FL_INNER_LD + in_tile] = ssb_activate(sum[j], o.kind) * o.limit;
                     }
                     fl_meet_four();
-                    // WIDE / 16 half blocks a row
-                    const int width = MODE == FL_GATED ? o.N / 2 : o.N, z0 = nt * WIDE, left = rows - c0;
+                    const int r = who / PER, piece = who % PER, k = nt * WIDE + piece * V;
+                    if ((who & ~31) / PER < left) {                  // some of this warp's rows are there
+                        float v[V];
 #pragma unroll
-                    for (int item = who; item < CH * (WIDE / 16); item += 128) {
-                        const int r = item / (WIDE / 16), half = item % (WIDE / 16), k = z0 + half * 16;
-                        float v[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            const float4 q = *reinterpret_cast<const float4*>(inner + r * FL_INNER_LD + half * 16 + e);
+                        for (int e = 0; e < V; e += 4) {
+                            const float4 q = *reinterpret_cast<const float4*>(inner + r * FL_INNER_LD + piece * V + e);
                             v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
                         }
-                        const int row = m0 + c0 + r;               // of the codes
-                        const int in_list = (LIST ? mt * 128 + c0 + r : row);                     // a listed tile's scales are 128 rows'
-                        fl_put_inner(v, (uint8_t*)o.out + (size_t)row * o.ldo + k / 2,
-                                     o.scales + f4_scale_at(in_list, k / F4_BLOCK, o.inner_blocks), r < left && k < width);
+                        const int row = m0 + c0 + r, in_list = LIST ? mt * 128 + c0 + r : row;       // of the codes; a listed tile's scales are 128 rows'
+                        fl_put_inner<V>(v, (uint8_t*)o.out + (size_t)row * o.ldo + k / 2,
+                                        o.scales + f4_scale_at(in_list, k / F4_BLOCK, o.inner_blocks), r < left && k < width);
                         // behind the last channel: scales of zero up to a whole k-block
-                        if (nt == n_tiles - 1 && r < left && half == 0)
+                        if (nt == n_tiles - 1 && r < left && piece == 0)
                             for (int b = width / F4_BLOCK; b < 8 * o.inner_blocks; ++b) o.scales[f4_scale_at(in_list, b, o.inner_blocks)] = 0;
                     }
                     fl_meet_four();
@@ -898,6 +900,107 @@ fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int 
     }
 }
 
+constexpr int FL_SORTED_PAIRS = 256;      // (token, choice) pairs that a block sorts for itself
+// The pairs (token, choice) by expert, in their order, for a block that has them to itself (pairs <= FL_SORTED_PAIRS <= its threads): tile
+// t, up to ROWS neighbours of one expert tile_expert[t], is pair_of[tile_first[t]], ..., tile_rows[t] of them.  Pairs whose expert is
+// none are left out.  All threads call it; the number of tiles.
+template <int ROWS>
+__device__ __forceinline__ int fl_sort_pairs(const int* __restrict__ expert_of, int pairs, int experts, int* pair_of, int* tile_first,
+                                             int* tile_rows, int* tile_expert) {
+    const int tid = threadIdx.x;
+    int e = -1, first = 0, place = 0, same = 0;
+    if (tid < pairs) {
+        e = expert_of[tid];
+        if ((unsigned)e >= (unsigned)experts) e = -1;
+        tile_first[tid] = e;
+    }
+    __syncthreads();
+    if (e >= 0)
+#pragma unroll 8
+        for (int q = 0; q < pairs; ++q) {
+            const int f = tile_first[q];
+            first += f >= 0 && f < e;
+            place += f == e && q < tid;
+            same += f == e;
+        }
+    if (tid < FL_SORTED_PAIRS) tile_rows[tid] = 0;
+    __syncthreads();
+    const bool starts = e >= 0 && place % ROWS == 0;
+    const int rows = min(ROWS, same - place);
+    if (e >= 0) pair_of[first + place] = tid;
+    if (starts) tile_rows[first + place] = 1;
+    __syncthreads();
+    int before = 0;
+    if (starts)
+#pragma unroll 8
+        for (int q = 0; q < first + place; ++q) before += tile_rows[q];
+    const int tiles = __syncthreads_count(starts);
+    if (starts) { tile_first[before] = first + place; tile_rows[before] = rows; tile_expert[before] = e; }
+    __syncthreads();
+    return tiles;
+}
+
+bool fw_takes(int M, int N, int K, int mode);
+bool fw_takes_list(int pairs, int experts, int N, int K, int mode);
+int fw_product(FwArgs a, int mode, cudaStream_t stream);
+int fw_product_list(FwArgs a, int mode, cudaStream_t stream);
+
+// Tiles of up to FL_SORTED_PAIRS pairs beside their rows into 4 bits, in one launch: every block sorts the pairs for itself, and takes
+// k-blocks of rows by its warps (a lane eight numbers, four lanes a block).
+template <typename T, int BN>
+__global__ void __launch_bounds__(256)
+fp4_place_kernel(const int* __restrict__ expert_of, int pairs, int experts, int top, const T* __restrict__ x, long long ldx, int K, int k_blocks,
+                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int* __restrict__ offsets, int* __restrict__ order,
+                 int* __restrict__ tile_expert, int* __restrict__ tile_row0, int* __restrict__ meta, int* __restrict__ clear, int n_clear) {
+    __shared__ int pair_of[FL_SORTED_PAIRS], first_of[FL_SORTED_PAIRS], rows_of[FL_SORTED_PAIRS], expert[FL_SORTED_PAIRS];
+    static_assert(FL_SORTED_PAIRS == 256, "a thread a pair");
+    ssb_pdl_wait();
+    ssb_pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles = fl_sort_pairs<BN>(expert_of, pairs, experts, pair_of, first_of, rows_of, expert);
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < n_clear; i += 256) clear[i] = 0;
+        for (int t = threadIdx.x; t < tiles; t += 256) {
+            tile_expert[t] = expert[t];
+            tile_row0[t] = first_of[t];
+            // where an expert's rows end, which is all that the products ask of it
+            if (t + 1 == tiles || expert[t + 1] != expert[t]) offsets[expert[t] + 1] = first_of[t] + rows_of[t];
+        }
+        if (threadIdx.x < pairs) order[threadIdx.x] = pair_of[threadIdx.x];
+        if (threadIdx.x == 0) meta[0] = tiles;
+    }
+    const int sorted = tiles ? first_of[tiles - 1] + rows_of[tiles - 1] : 0;
+    for (int task = blockIdx.x * 8 + warp; task < sorted * k_blocks; task += gridDim.x * 8) {
+        const int i = task / k_blocks, kb = task - i * k_blocks, k = kb * F4_KB + lane * 8, pair = pair_of[i];
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = 0.f;
+        if (k < K) f4_load8(x + (size_t)(pair / top) * ldx + k, v);
+        int t = 0;                                                   // its tile
+        for (int base = 0; base < tiles; base += 32) {
+            const int q = base + lane;
+            const uint32_t hit = __ballot_sync(0xffffffffu, q < tiles && first_of[q] <= i);
+            t += __popc(hit);
+        }
+        --t;
+        const int r = i - first_of[t];
+        uint32_t most = f4_most(v);
+        if (__any_sync(0xffffffffu, most >= F4_WILD)) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = f4_finite(v[q]);
+            most = f4_most(v);
+        }
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int byte = f4_scale_byte(most);
+        uint32_t word = (uint32_t)byte << (8 * ((lane & 15) >> 2));
+        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+        if (k < K) *reinterpret_cast<uint32_t*>(codes + (size_t)(t * BN + r) * (K / 2) + k / 2) = f4_encode8(v, f4_inverse(byte));
+        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + f4_scale_at(t * 128 + r, kb * 8 + (lane >> 4) * 4, k_blocks)) = word;
+    }
+}
+
 // out[t] (+)= sum over the choices j, in their order, of weight[t, j] * y[t, j]; choices of no expert count nothing.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -935,24 +1038,11 @@ static int fl_list_rows(int tokens, int top, int experts) {
     const long long mean = (long long)tokens * top / experts;
     return tokens <= 16 || mean <= 8 ? 16 : tokens <= 32 || mean <= 16 ? 32 : tokens <= 64 || mean <= 48 ? 64 : mean <= 96 ? 128 : 256;
 }
-// Whether experts run in the kernel of few rows.
-static bool fl_few_pairs(int pairs, int experts, int K, int inter) {
-    return pairs <= 16 && fw_takes_list(pairs, experts, 2 * inter, K, FL_GATED) && fw_takes_list(pairs, experts, K, inter, FL_STORE);
-}
 struct FlExperts {
     int bn, tiles, blocks;                 // rows a tile, tiles at most, blocks of a product
     size_t counters, offsets, order, slot, tile_expert, tile_row0, meta, x, xs, z, zs, y, pieces, all;
-    bool few;                              // by the kernel of few rows, which needs no list
     FlExperts(int tokens, int top, int experts, int K, int inter) {
         const int pairs = tokens * top;
-        few = fl_few_pairs(pairs, experts, K, inter);
-        if (few) {
-            z = 0;
-            zs = fl_round((size_t)pairs * (inter / 2));
-            y = zs + fl_round((size_t)((pairs + 127) / 128) * f4_k_blocks(inter) * F4_CHUNK);
-            all = y + fl_round((size_t)pairs * K * 4);
-            return;
-        }
         bn = fl_list_rows(tokens, top, experts);
         tiles = pairs / bn + std::min(experts, pairs);
         blocks = ssb_sm_count();
@@ -1013,37 +1103,32 @@ SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* 
     const int pairs = tokens * top, N1 = gated ? 2 * inter : inter;
     float* y = (float*)(base + at.y);
     int rc;
-    if (at.few) {
-        FwArgs a{};
-        a.w = (const uint8_t*)w1; a.ws = (const uint8_t*)ws1;
-        a.x = x; a.ldx = ldx; a.dtype = dtype;
-        a.out = base + at.z; a.out_scales = (uint8_t*)(base + at.zs); a.ldo = inter / 2;
-        a.M = tokens; a.N = N1; a.K = K;
-        a.kind = kind; a.limit = limit; a.inner_blocks = f4_k_blocks(inter);
-        a.expert_of = expert_of; a.pairs = pairs; a.top = top; a.experts = experts;
-        rc = fw_product_list(a, gated ? FL_GATED : FL_ACT, stream);
-        if (rc) return rc;
-        a.w = (const uint8_t*)w2; a.ws = (const uint8_t*)ws2;
-        a.x = base + at.z; a.dtype = -1; a.xs = (const uint8_t*)(base + at.zs);
-        a.out = y; a.ldo = K; a.is_f32 = 1;
-        a.N = K; a.K = inter;
-        rc = fw_product_list(a, FL_STORE, stream);
+    if (at.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
+    auto ints = [&](size_t o) { return (int*)(base + o); };
+    if (pairs <= FL_SORTED_PAIRS && at.bn == 16) {
+        const int k_blocks = f4_k_blocks(K);
+        const dim3 grid((unsigned)std::min(ssb_sm_count(), (pairs * k_blocks + 7) / 8));
+        auto place = [&](auto kernel, auto* numbers) {
+            return ssb_launch(kernel, grid, dim3(256), 0, stream, true, expert_of, pairs, experts, top, numbers, ldx, K, k_blocks,
+                              (uint8_t*)(base + at.x), (uint8_t*)(base + at.xs), ints(at.offsets), ints(at.order), ints(at.tile_expert),
+                              ints(at.tile_row0), ints(at.meta), ints(at.counters), 2 * FL_COUNTERS);
+        };
+        rc = dtype == SSB_BF16 ? place(fp4_place_kernel<bf16, 16>, (const bf16*)x) : place(fp4_place_kernel<float, 16>, (const float*)x);
     } else {
-        if (at.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
-        auto ints = [&](size_t o) { return (int*)(base + o); };
-        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(1024), (size_t)experts * 12, stream, true, expert_of, pairs, experts, at.bn, ints(at.offsets),
-                        ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta), ints(at.counters), 2 * FL_COUNTERS);
+        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(1024), (size_t)experts * 12, stream, true, expert_of, pairs, experts, at.bn,
+                        ints(at.offsets), ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta),
+                        ints(at.counters), 2 * FL_COUNTERS);
         if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, pairs, top, K, ints(at.slot), at.bn, stream);
-        if (rc) return rc;
-        const FlTiles list{ints(at.offsets), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta)};
-        float* pieces = (float*)(base + at.pieces);
-        const FlOut first{base + at.z, (uint8_t*)(base + at.zs), nullptr, nullptr, inter / 2, 0, 0, tokens, N1, kind, limit, f4_k_blocks(inter)};
-        rc = gated ? fl_listed<FL_GATED>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream)
-                   : fl_listed<FL_ACT>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream);
-        if (rc) return rc;
-        const FlOut second{y, nullptr, ints(at.order), nullptr, K, 1, 0, tokens, K, 0, 0.f, 0};
-        rc = fl_listed<FL_STORE>(base + at.z, base + at.zs, w2, ws2, second, list, at, experts, inter, ints(at.counters) + FL_COUNTERS, pieces, error_word, stream);
     }
+    if (rc) return rc;
+    const FlTiles list{ints(at.offsets), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta)};
+    float* pieces = (float*)(base + at.pieces);
+    const FlOut first{base + at.z, (uint8_t*)(base + at.zs), nullptr, nullptr, inter / 2, 0, 0, tokens, N1, kind, limit, f4_k_blocks(inter)};
+    rc = gated ? fl_listed<FL_GATED>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream)
+               : fl_listed<FL_ACT>(base + at.x, base + at.xs, w1, ws1, first, list, at, experts, K, ints(at.counters), pieces, error_word, stream);
+    if (rc) return rc;
+    const FlOut second{y, nullptr, ints(at.order), nullptr, K, 1, 0, tokens, K, 0, 0.f, 0};
+    rc = fl_listed<FL_STORE>(base + at.z, base + at.zs, w2, ws2, second, list, at, experts, inter, ints(at.counters) + FL_COUNTERS, pieces, error_word, stream);
     if (rc) return rc;
     const dim3 grid((unsigned)std::min<long long>(((long long)tokens * (K / 8) + 255) / 256, 8 * ssb_sm_count()));
     if (out_dtype == SSB_BF16)

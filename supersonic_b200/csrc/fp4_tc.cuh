@@ -80,21 +80,28 @@ __device__ __forceinline__ void fl_meet_four() { asm volatile("barrier.cta.sync 
 constexpr int fl_power(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
 constexpr int FL_INNER_ROWS = 16;         // rows of an inner tile that meet in shared memory at a time
 constexpr int FL_INNER_LD = 132;
-// 16 numbers of a block of 32 whose other half the neighbouring lane has: codes to ``dst`` (8 bytes), the block's scale by the even lane.
-__device__ __forceinline__ void fl_put_inner(float (&v)[16], uint8_t* dst, uint8_t* scale, bool live) {
+// V (8 or 16) numbers of a block of 32 whose others the neighbouring lanes have: codes to ``dst`` (V / 2 bytes), the block's scale by the
+// first of its lanes.
+template <int V>
+__device__ __forceinline__ void fl_put_inner(float (&v)[V], uint8_t* dst, uint8_t* scale, bool live) {
+    constexpr int LANES = 32 / V;
     uint32_t most = f4_most(v);
     if (__any_sync(0xffffffffu, most >= F4_WILD)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = f4_finite(v[i]);
+        for (int i = 0; i < V; ++i) v[i] = f4_finite(v[i]);
         most = f4_most(v);
     }
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
     const int byte = f4_scale_byte(most);
     const float inverse = f4_inverse(byte);
-    const uint2 w = make_uint2(f4_encode8(v, inverse), f4_encode8(v + 8, inverse));
+    uint32_t w[V / 8];
+#pragma unroll
+    for (int i = 0; i < V / 8; ++i) w[i] = f4_encode8(v + 8 * i, inverse);
     if (live) {
-        *reinterpret_cast<uint2*>(dst) = w;
-        if ((threadIdx.x & 1) == 0) *scale = (uint8_t)byte;
+        if (V == 16) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[V / 8 - 1]);
+        else *reinterpret_cast<uint32_t*>(dst) = w[0];
+        if ((threadIdx.x & (LANES - 1)) == 0) *scale = (uint8_t)byte;
     }
 }
 
