@@ -783,7 +783,7 @@ static int fl_dense(const void* x, const void* xs, const void* w, const void* ws
 
 SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* codes, void* scales, int rows, int K, int per_expert, int inter,
                              int* clear, int n_clear, int early, cudaStream_t stream);
-SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void* codes, void* scales, int pairs, int top, int K,
+SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void* codes, void* scales, int tokens, int top, int K,
                                    const int* slot, int tile_rows, cudaStream_t stream);
 
 // A product of dense weights.  x: rows of dtype (ldx elements apart), which are quantised first, or (dtype -1) codes with the scales xs.
@@ -840,63 +840,93 @@ SSB_API int ssb_fp4_inner(const void* x, long long ldx, int dtype, const void* x
 }
 
 // ---- experts ----------------------------------------------------------------------------------------------------------
-// Pairs (token, choice) by expert, one block: counts in shared memory, first rows and first tiles of the experts by one warp, then every
-// pair takes the next row of its expert.  ``slot``: where a pair's row goes among tiles of BN rows (-1: its expert is none), ``order``:
-// the pair of a sorted row.  The order inside an expert is whatever the adds give; nothing that is written depends on it.
-__global__ void __launch_bounds__(1024)
+// Pairs (token, choice) by expert, one block.  A warp has a run of neighbouring pairs and counts of its own: it counts them by expert, the
+// counts of the warps before it say where its pairs go, and it places them.  ``slot``: where a pair's row goes among tiles of BN rows
+// (-1: its expert is none), ``order``: the pair of a sorted row.  The order of an expert's pairs inside a warp's run is whatever the adds
+// give; nothing that leaves the call depends on it.  12,288 pairs of 64 experts: GROUP_FIGURE us (counts that all warps share 16, ranks by
+// match.any 26).
+constexpr int FL_GROUP_WARPS = 32;
+
+__global__ void __launch_bounds__(32 * FL_GROUP_WARPS)
 fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int bn, int* __restrict__ offsets, int* __restrict__ order,
                  int* __restrict__ slot, int* __restrict__ tile_expert, int* __restrict__ tile_row0, int* __restrict__ meta,
-                 int* __restrict__ clear, int n_clear) {
-    extern __shared__ int counts[];                                // [experts] counts, then the next row; [experts] first row, [experts] first tile
-    int *row0 = counts + experts, *tile0 = row0 + experts;
+                 int* __restrict__ clear, int n_clear, int n_warps) {
+    extern __shared__ int counts[];                                // [n_warps][experts]; then [experts] first row, first tile
+    int *row0 = counts + n_warps * experts, *tile0 = row0 + experts;
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = (pairs + n_warps - 1) / n_warps;
+    const int lo = min(pairs, warp * run), hi = warp < n_warps ? min(pairs, lo + run) : lo;
     for (int i = threadIdx.x; i < n_clear; i += blockDim.x) clear[i] = 0;
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[e] = 0;
+    for (int e = threadIdx.x; e < n_warps * experts; e += blockDim.x) counts[e] = 0;
     __syncthreads();
-    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
-        const int e = expert_of[p];
-        if ((unsigned)e < (unsigned)experts) atomicAdd(&counts[e], 1);
+    int* mine = counts + min(warp, n_warps - 1) * experts;
+    auto expert_at = [&](int p) {
+        const int e = p < hi ? expert_of[p] : -1;
+        return (unsigned)e < (unsigned)experts ? e : -1;
+    };
+    constexpr int AHEAD = 8;                                       // loads in flight
+    for (int p0 = lo; p0 < hi; p0 += 32 * AHEAD) {
+        int es[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) es[q] = expert_at(p0 + 32 * q + lane);
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            if (es[q] >= 0) atomicAdd(mine + es[q], 1);
+        }
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {      // an expert's counts become the rows before each warp's
+        int sum = 0;
+        for (int w = 0; w < n_warps; ++w) {
+            const int n = counts[w * experts + e];
+            counts[w * experts + e] = sum;
+            sum += n;
+        }
+        row0[e] = sum;
+    }
+    __syncthreads();
+    if (warp == 0) {
         int row = 0, tile = 0;
         for (int e0 = 0; e0 < experts; e0 += 32) {
-            const int e = e0 + threadIdx.x, n = e < experts ? counts[e] : 0, t = (n + bn - 1) / bn;
+            const int e = e0 + lane, n = e < experts ? row0[e] : 0, t = (n + bn - 1) / bn;
             int r_sum = n, t_sum = t;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const int r = __shfl_up_sync(0xffffffffu, r_sum, d), q = __shfl_up_sync(0xffffffffu, t_sum, d);
-                if (threadIdx.x >= d) { r_sum += r; t_sum += q; }
+                if (lane >= d) { r_sum += r; t_sum += q; }
             }
             if (e < experts) {
                 row0[e] = row + r_sum - n;
                 tile0[e] = tile + t_sum - t;
-                offsets[e] = row0[e];
+                offsets[e + 1] = row + r_sum;                      // where an expert's rows end
             }
             row += __shfl_sync(0xffffffffu, r_sum, 31);
             tile += __shfl_sync(0xffffffffu, t_sum, 31);
         }
-        if (threadIdx.x == 0) { offsets[experts] = row; meta[0] = tile; }
+        if (lane == 0) { offsets[0] = 0; meta[0] = tile; }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-        for (int i = 0; i < counts[e]; i += bn) {
+    for (int e = threadIdx.x; e < experts; e += blockDim.x)
+        for (int i = 0; row0[e] + i < offsets[e + 1]; i += bn) {
             tile_expert[tile0[e] + i / bn] = e;
             tile_row0[tile0[e] + i / bn] = row0[e] + i;
         }
-        counts[e] = 0;
-    }
-    __syncthreads();
-    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
-        const int e = expert_of[p];
-        int to = -1;
-        if ((unsigned)e < (unsigned)experts) {
-            const int i = atomicAdd(&counts[e], 1);
-            to = (tile0[e] + i / bn) * bn + i % bn;
-            order[row0[e] + i] = p;
+    for (int p0 = lo; p0 < hi; p0 += 32 * AHEAD) {
+        int es[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) es[q] = expert_at(p0 + 32 * q + lane);
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            const int e = es[q], p = p0 + 32 * q + lane;
+            int to = -1;
+            if (e >= 0) {
+                const int i = atomicAdd(mine + e, 1);
+                to = (tile0[e] + i / bn) * bn + i % bn;
+                order[row0[e] + i] = p;
+            }
+            if (p < hi) slot[p] = to;
         }
-        slot[p] = to;
     }
 }
 
@@ -1013,14 +1043,23 @@ fp4_combine_kernel(const float* __restrict__ y, const int* __restrict__ expert_o
     for (long long p = (long long)blockIdx.x * blockDim.x + threadIdx.x; p < pieces; p += step) {
         const int t = (int)(p / per_row), c = (int)(p - (long long)t * per_row) * 8;
         float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int j = 0; j < top; ++j) {
-            const int pair = t * top + j;
-            if ((unsigned)expert_of[pair] >= (unsigned)experts) continue;
-            const float w = weight[pair];
-            float v[8];
-            f4_load8(y + (size_t)pair * width + c, v);
+        for (int j0 = 0; j0 < top; j0 += 4) {                      // four choices in flight
+            float v[4][8], w[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] = fmaf(w, v[i], sum[i]);
+            for (int q = 0; q < 4; ++q) {
+                const int pair = t * top + j0 + q;
+                w[q] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[q][i] = 0.f;
+                if (j0 + q < top && (unsigned)expert_of[pair] < (unsigned)experts) {
+                    w[q] = weight[pair];
+                    f4_load8(y + (size_t)pair * width + c, v[q]);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] = fmaf(w[q], v[q][i], sum[i]);
         }
         T* dst = out + t * ldo + c;
         if (add) {
@@ -1094,7 +1133,7 @@ SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* 
                             const void* w2, const void* ws2, void* out, long long ldo, int out_dtype, int tokens, int top, int experts, int K,
                             int inter, int gated, int kind, float limit, int add, void* scratch, int* error_word, cudaStream_t stream) {
     if (tokens < 0 || top <= 0 || experts <= 0 || experts > 4096 || K <= 0 || K % F4_BLOCK || inter <= 0 || inter % F4_BLOCK || kind < 0 || kind > 2 ||
-        !scratch || !error_word || (long long)tokens * top > (1 << 24)) return SSB_ERR_BAD_SIZE;
+        !scratch || !error_word || (long long)tokens * top > (1 << 24)) return SSB_ERR_BAD_SIZE;          // 4,096: of the grouping's shared memory
     if (((uintptr_t)x | (uintptr_t)w1 | (uintptr_t)ws1 | (uintptr_t)w2 | (uintptr_t)ws2 | (uintptr_t)out | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
     if ((dtype != SSB_F32 && dtype != SSB_BF16) || (out_dtype != SSB_F32 && out_dtype != SSB_BF16) || (add && out_dtype != SSB_F32)) return SSB_ERR_BAD_DTYPE;
     if (tokens == 0) return 0;
@@ -1115,10 +1154,12 @@ SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* 
         };
         rc = dtype == SSB_BF16 ? place(fp4_place_kernel<bf16, 16>, (const bf16*)x) : place(fp4_place_kernel<float, 16>, (const float*)x);
     } else {
-        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(1024), (size_t)experts * 12, stream, true, expert_of, pairs, experts, at.bn,
-                        ints(at.offsets), ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta),
-                        ints(at.counters), 2 * FL_COUNTERS);
-        if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, pairs, top, K, ints(at.slot), at.bn, stream);
+        // as many warps as shared memory has room for their counts
+        const int n_warps = std::max(1, std::min(FL_GROUP_WARPS, 48 * 1024 / (4 * experts) - 2));
+        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(32 * FL_GROUP_WARPS), (size_t)experts * (n_warps + 2) * 4, stream, true, expert_of, pairs,
+                        experts, at.bn, ints(at.offsets), ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta),
+                        ints(at.counters), 2 * FL_COUNTERS, n_warps);
+        if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, tokens, top, K, ints(at.slot), at.bn, stream);
     }
     if (rc) return rc;
     const FlTiles list{ints(at.offsets), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta)};

@@ -9,8 +9,8 @@ typedef __nv_bfloat16 bf16;
 constexpr int FR_THREADS = 256;
 constexpr int FR_TURNS = 4;               // units a half-warp has in flight
 
-// Where a row goes: row r of a matrix of several experts' rows, or (slot) pair r's row, a copy of its token's, in tiles of ``tile_rows``
-// whose scales have runs of their own.
+// Where a row goes: row r of a matrix of several experts' rows, or (slot) the rows of its ``top`` pairs, in tiles of ``tile_rows`` whose
+// scales have runs of their own.
 struct FrRows {
     int per_expert, inter;                 // rows of a matrix; of a gated unit's first, how many of them are gate rows
     const int* slot; int top, tile_rows;
@@ -29,7 +29,7 @@ struct FrStep {
 
 // A unit is 128 numbers of a row: sixteen lanes of eight, four lanes a block, whose four scales are one word.  Units run over whole
 // k-blocks; behind a row's end they write scales of zero.  TURNS units are in flight.
-template <typename T, int TURNS>
+template <typename T, int TURNS, bool PAIRS>
 __global__ void __launch_bounds__(FR_THREADS)
 fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int rows, int K,
                     const FrRows to, const FrStep step, int k_blocks, int* __restrict__ clear, int n_clear, int early) {
@@ -50,7 +50,7 @@ fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict_
             const int k = part * 128 + lane * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
-            if (row < rows && k < K) f4_load8(x + (long long)(to.slot ? row / to.top : row) * ldx + k, v[j]);
+            if (row < rows && k < K) f4_load8(x + (long long)row * ldx + k, v[j]);
             step.next(row, part);
         }
 #pragma unroll
@@ -69,22 +69,25 @@ fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict_
             word |= __shfl_xor_sync(0xffffffffu, word, 4);
             word |= __shfl_xor_sync(0xffffffffu, word, 8);
             if (at_row[j] >= rows) continue;
-            long long at = at_row[j];                          // row of the codes
-            int run0 = 0, r = at_row[j];                       // the matrix's first run of scales' rows, the row in it
-            if (to.slot) {
-                at = to.slot[at_row[j]];
-                if (at < 0) continue;
-                const int tile = (int)at / to.tile_rows;
-                r = tile * max(to.tile_rows, 128) + (int)at - tile * to.tile_rows;
-            } else if (to.per_expert < rows || to.inter) {
-                const int expert = r / to.per_expert;
-                r = f4_laid_row(r - expert * to.per_expert, to.inter);
-                at = (long long)expert * to.per_expert + r;
-                run0 = expert * ((to.per_expert + 127) >> 7);
+            const uint32_t code = f4_encode8(v[j], f4_inverse(byte));
+            for (int copy = 0; copy < (PAIRS ? to.top : 1); ++copy) {
+                long long at = at_row[j];                      // row of the codes
+                int run0 = 0, r = at_row[j];                   // the matrix's first run of scales' rows, the row in it
+                if (PAIRS) {
+                    at = to.slot[at_row[j] * to.top + copy];
+                    if (at < 0) continue;
+                    const int tile = (int)at / to.tile_rows;
+                    r = tile * max(to.tile_rows, 128) + (int)at - tile * to.tile_rows;
+                } else if (to.per_expert < rows || to.inter) {
+                    const int expert = r / to.per_expert;
+                    r = f4_laid_row(r - expert * to.per_expert, to.inter);
+                    at = (long long)expert * to.per_expert + r;
+                    run0 = expert * ((to.per_expert + 127) >> 7);
+                }
+                if (k < K) *reinterpret_cast<uint32_t*>(codes + at * (K / 2) + k / 2) = code;
+                if (lane == 0)
+                    *reinterpret_cast<uint32_t*>(scales + (size_t)run0 * k_blocks * F4_CHUNK + f4_scale_at(r, at_part[j] * 4, k_blocks)) = word;
             }
-            if (k < K) *reinterpret_cast<uint32_t*>(codes + at * (K / 2) + k / 2) = f4_encode8(v[j], f4_inverse(byte));
-            if (lane == 0)
-                *reinterpret_cast<uint32_t*>(scales + (size_t)run0 * k_blocks * F4_CHUNK + f4_scale_at(r, at_part[j] * 4, k_blocks)) = word;
         }
     }
 }
@@ -154,7 +157,9 @@ static int fr_quantize(const T* x, long long ldx, uint8_t* codes, uint8_t* scale
     int blocks, turns;
     const FrStep step = fr_step(rows, 2 * k_blocks, &blocks, &turns);
     if ((long long)rows + step.rows * 4LL + 4 > INT_MAX) return SSB_ERR_BAD_SIZE;
-    return ssb_launch(turns == 1 ? fp4_quantize_kernel<T, 1> : fp4_quantize_kernel<T, FR_TURNS>, dim3(blocks), dim3(FR_THREADS), 0, stream, true,
+    auto kernel = to.slot ? (turns == 1 ? fp4_quantize_kernel<T, 1, true> : fp4_quantize_kernel<T, FR_TURNS, true>)
+                          : (turns == 1 ? fp4_quantize_kernel<T, 1, false> : fp4_quantize_kernel<T, FR_TURNS, false>);
+    return ssb_launch(kernel, dim3(blocks), dim3(FR_THREADS), 0, stream, true,
                       x, ldx, codes, scales, rows, K, to, step, k_blocks, clear, n_clear, early);
 }
 
@@ -171,12 +176,12 @@ SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* code
     return SSB_ERR_BAD_DTYPE;
 }
 
-// The pairs' rows, pair p's from row p / top of x, to the rows that ``slot`` names (-1: none) in tiles of ``tile_rows``.
-SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void* codes, void* scales, int pairs, int top, int K,
+// The tokens' rows, each to the rows that its ``top`` pairs' ``slot`` names (-1: none) in tiles of ``tile_rows``.
+SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void* codes, void* scales, int tokens, int top, int K,
                                    const int* slot, int tile_rows, cudaStream_t stream) {
-    const FrRows to{pairs, 0, slot, top, tile_rows};
-    if (dtype == SSB_BF16) return fr_quantize((const bf16*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, pairs, K, to, nullptr, 0, 1, stream);
-    if (dtype == SSB_F32) return fr_quantize((const float*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, pairs, K, to, nullptr, 0, 1, stream);
+    const FrRows to{tokens, 0, slot, top, tile_rows};
+    if (dtype == SSB_BF16) return fr_quantize((const bf16*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, tokens, K, to, nullptr, 0, 1, stream);
+    if (dtype == SSB_F32) return fr_quantize((const float*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, tokens, K, to, nullptr, 0, 1, stream);
     return SSB_ERR_BAD_DTYPE;
 }
 
