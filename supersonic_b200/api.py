@@ -62,7 +62,7 @@ def load(model_dir: Optional[str] = None, dtype: str = "bfloat16", device: int =
          context_size: Optional[int] = None, batch_size: int = 1, max_tokens: Optional[int] = None,
          step_token_budget: Optional[int] = None, preset: Optional[str] = None, random_seed: int = 0,
          allow_unexpected_tensors: bool = False, use_graphs: bool = True,
-         deterministic: bool = False) -> Engine:
+         deterministic: bool = False, weight_format: Optional[str] = None) -> Engine:
     """Load ``model_dir`` (config.json + safetensors), or build the named ``preset`` with random
     weights made on the device from ``random_seed`` (no folder is read or written).  The cache holds
     ``max_tokens`` tokens in all, by default ``batch_size`` sequences of ``context_size`` tokens
@@ -71,7 +71,10 @@ def load(model_dir: Optional[str] = None, dtype: str = "bfloat16", device: int =
     memory a batch of long prompts needs beside the cache.  Weights, cache and workspace are checked
     against the device's free memory before anything is loaded.  ``deterministic``: the bfloat16
     path without float atomics, so that the same batch gives the same bits every run and sampled
-    tokens are reproducible from their seed (the float32 path always is)."""
+    tokens are reproducible from their seed (the float32 path always is).  ``weight_format="mxfp4"``:
+    the projections of attention and the feed-forwards (experts among them) as 4-bit floats with a scale
+    for every 32 (``csrc/fp4_ops.py``), made from the model's weights as it is loaded; rows go into
+    4 bits too where they meet them.  Norms, embedding, head and the other mixers stay as they are."""
     from .cache import PAGE_TOKENS
     from .config import load_config, preset_config
     if (model_dir is None) == (preset is None):
@@ -80,7 +83,7 @@ def load(model_dir: Optional[str] = None, dtype: str = "bfloat16", device: int =
     ctx = context_size or min(getattr(cfg, "max_position_embeddings", 8192), 8192)
     ctx = -(-ctx // PAGE_TOKENS) * PAGE_TOKENS
     total = max_tokens or ctx * max(batch_size, 1)
-    extra = {"use_graphs": use_graphs, "deterministic": deterministic}
+    extra = {"use_graphs": use_graphs, "deterministic": deterministic, "weight_format": weight_format}
     if step_token_budget is not None:
         extra["step_token_budget"] = step_token_budget
     dev = f"cuda:{device}"

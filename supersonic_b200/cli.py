@@ -49,6 +49,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--batch-size", type=int, default=1, help="sequences decoded in parallel")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"],
                     help="bfloat16 (serving kernels) or float32 (true 32-bit path)")
+    ap.add_argument("--weight-format", default=None, choices=["mxfp4"],
+                    help="hold the projections and feed-forwards in this format (4-bit floats); default: as --dtype says")
     ap.add_argument("--emit-stage-timings", action="store_true",
                     help="print [stage] lines: device time by stage (projections, attention, mlp, norms, head, sampling)")
     ap.add_argument("--emit-generated-json", action="store_true",
@@ -146,7 +148,8 @@ def main(argv=None) -> int:
     t0 = time.time()
     try:
         engine = load(args.model_dir, dtype=args.dtype, device=args.device, context_size=context,
-                      batch_size=min(batch, len(prompts)), preset=preset, random_seed=args.random_seed)
+                      batch_size=min(batch, len(prompts)), preset=preset, random_seed=args.random_seed,
+                      weight_format=args.weight_format)
     except (MemoryPreflightError, ConfigError) as e:
         err(str(e))
         return 1

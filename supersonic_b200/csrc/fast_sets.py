@@ -13,6 +13,7 @@ from typing import Dict, Optional
 
 import torch
 
+from ..weights.fp4 import Fp4Matrix
 from . import ops
 from .kernel_sets import NormedInput, PlainKernels, as_tensor
 
@@ -94,6 +95,9 @@ class FastKernels(PlainKernels):
         return True
 
     def linear(self, x, weight, out, accumulate=False):
+        if isinstance(weight, Fp4Matrix):
+            super().linear(x, weight, out, accumulate)
+            return
         rows = x.n_rows if isinstance(x, NormedInput) else x.shape[0]
         x = as_tensor(x)
         if (out.dtype == torch.float32 or not accumulate) and ops.gemm_tc_ok(x, weight, out):
@@ -324,7 +328,7 @@ class FastKernels(PlainKernels):
         rows = batch.n_tokens
         if getattr(position, "interleaved", False):
             return False                      # the fused rotations pair (i, i + half)
-        if not (self.fuse_rope_prefill and tables and not batch.is_decode
+        if isinstance(w_qkv, Fp4Matrix) or not (self.fuse_rope_prefill and tables and not batch.is_decode
                 and w_qkv.dtype == torch.bfloat16 and head_dim in (64, 128)):
             return False
         n, k = w_qkv.shape

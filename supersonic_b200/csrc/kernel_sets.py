@@ -11,7 +11,8 @@ from typing import Optional
 
 import torch
 
-from . import ops
+from ..weights.fp4 import Fp4Matrix
+from . import fp4_ops, ops
 
 
 class NormedInput:
@@ -91,8 +92,11 @@ class PlainKernels:
         ops.rmsnorm(x, weight, eps, out, rows, pdl=self._chain(out.shape[0]))
 
     def linear(self, x, weight, out, accumulate=False):
-        """out (+)= x @ weight^T; ``x`` may be a :class:`NormedInput`."""
+        """out (+)= x @ weight^T; ``x`` may be a :class:`NormedInput`, ``weight`` a 4-bit matrix."""
         x = as_tensor(x)
+        if isinstance(weight, Fp4Matrix):
+            fp4_ops.linear(x, weight, out, accumulate)
+            return
         ops.gemm_nt_plain(x, weight, out, accumulate, pdl=self._chain(x.shape[0]))
 
     def pack_gate_up(self, gate, up):
@@ -424,6 +428,26 @@ class PlainKernels:
         logits = torch.empty((x.shape[0], weight.shape[0]), dtype=torch.float32, device=x.device)
         self.linear(x, weight, logits)
         ops.route_softmax(logits, n_experts, renormalize, scale, expert_of, pair_weight, pdl=self._chain(logits.shape[0]), bias=bias)
+
+    def route_scored(self, x, weight, n_experts, expert_of, pair_weight, scores, correction, groups, keep, group_score, renormalize, scale):
+        """The router's product (logits x @ weight^T in float32) and the choice (``ops.route_scored``)."""
+        logits = torch.empty((x.shape[0], weight.shape[0]), dtype=torch.float32, device=x.device)
+        self.linear(x, weight, logits)
+        ops.route_scored(logits, n_experts, expert_of, pair_weight, scores, correction, groups, keep, group_score, renormalize, scale,
+                         pdl=self._chain(logits.shape[0]))
+
+    # ---- feed-forwards whose weights are 4-bit matrices ---------------------------------
+    def fp4_gated_unit(self, x, first, down, residual, act=None, row_scale=None):
+        """residual += down(f(gate x, up x) * row_scale), rows and inner rows in 4 bits."""
+        fp4_ops.linear(fp4_ops.gate_up(as_tensor(x), first, act, row_scale), down, residual, accumulate=True)
+
+    def fp4_dense_unit(self, x, up, down, residual, act, scale=1.0):
+        """residual += down(act(up x) * scale), rows and inner rows in 4 bits."""
+        fp4_ops.linear(fp4_ops.activated(as_tensor(x), up, act, scale), down, residual, accumulate=True)
+
+    def fp4_experts(self, x, expert_of, pair_weight, first, down, residual, act=None):
+        """residual += the weighted sum of the chosen experts' units, rows and inner rows in 4 bits."""
+        fp4_ops.experts(as_tensor(x), expert_of, pair_weight, first, down, residual, act, accumulate=True)
 
     def group_by_expert(self, expert_of, n_experts, groups, x=None):
         """``groups``: the dict of int32 tensors a grouped product reads (offsets, order, tile_expert,

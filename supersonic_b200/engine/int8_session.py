@@ -55,6 +55,8 @@ class Int8Session:
         if budget is not None and (budget <= 0 or slack < 1 or first < 0 or self.recent < 0 or first + self.recent > budget):
             raise ValueError(f"a budget of {budget} tokens has no room for the first {first} and the latest {self.recent}")
         n_pages = pages_for(max_tokens)
+        if getattr(model, "weight_format", None) is not None:
+            raise ValueError(f"an 8-bit session makes its weights from the model's, which are in {model.weight_format}")
         stops = model.spec.schedule
         if [s.layer for s in stops] != list(range(len(model.blocks))) or len({s.cache for s in stops}) != len(stops) \
                 or any(s.before is not None or not s.writes_cache for s in stops) or hasattr(getattr(model, "embedding", None), "cache_need"):

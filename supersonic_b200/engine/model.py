@@ -25,12 +25,15 @@ from ..config import ModelSpec, load_config, spec_from_config
 from ..csrc.kernel_sets import kernel_set_for
 from ..parts import (BLOCKS, EMBEDDINGS, FEED_FORWARDS, HEADS, MIXERS, NORMS, POSITION_ENCODINGS, STREAM_ADAPTERS,
                      BuildContext, WeightAccess, lookup)
-from ..weights import WeightStore
+from ..weights import Fp4Matrix, WeightStore
 from .batch import (NotOnHost, PackedStep, StepBatch, StepEntry, batch_over, decode_pages_bucket, pack_entries,
                     pack_step, plan_chunks)
 
 _DTYPES = {"float32": torch.float32, "fp32": torch.float32, "f32": torch.float32,
            "bfloat16": torch.bfloat16, "bf16": torch.bfloat16}
+
+
+WEIGHT_FORMATS = (None, "mxfp4")          # as the matrices are in the path's type; 4-bit floats (``parts/fp4.py``)
 
 
 def parse_dtype(dtype) -> torch.dtype:
@@ -195,8 +198,13 @@ class Model:
                  max_tokens: int = 4096, max_seq_tokens: Optional[int] = None,
                  max_slots: Optional[int] = None, kernels: Optional[str] = None, config=None,
                  use_graphs: bool = True, step_token_budget: int = 32768, preflight: bool = True,
-                 deterministic: bool = False):
+                 deterministic: bool = False, weight_format: Optional[str] = None):
         spec.validate()
+        if weight_format not in WEIGHT_FORMATS:
+            raise ValueError(f"weight_format {weight_format!r} is not known (known: {WEIGHT_FORMATS})")
+        if weight_format is not None and deterministic:
+            raise ValueError("4-bit products cut their sums by the step's rows: they have no deterministic form")
+        self.weight_format = weight_format
         self.spec, self.config = spec, config
         self.dtype = parse_dtype(dtype)
         self.device = torch.device(device)
@@ -208,7 +216,7 @@ class Model:
         # weights + cache + the largest step's activations against free memory, before anything is loaded
         from . import preflight as _preflight
         self.memory_estimate = (_preflight.check if preflight else _preflight.estimate_only)(
-            spec, store, self.dtype, self.device, max_tokens, max_seq, max_slots, int(step_token_budget))
+            spec, store, self.dtype, self.device, max_tokens, max_seq, max_slots, int(step_token_budget), weight_format)
         weights = WeightAccess(store, self.device)
         build = BuildContext(self.device, self.dtype, self.kernels, weights, max_positions=max_seq + 64)
 
@@ -217,15 +225,20 @@ class Model:
 
         self.embedding = part(EMBEDDINGS, "embedding", spec.embedding)
         self.blocks = []
+        in_fp4 = []
         for b in spec.blocks:
             mixer = part(MIXERS, "mixer", b.mixer)
             ff = part(FEED_FORWARDS, "feed-forward", b.feed_forward) if b.feed_forward else None
             n1 = part(NORMS, "norm", b.mixer_norm) if b.mixer_norm else None
             n2 = part(NORMS, "norm", b.feed_forward_norm) if b.feed_forward_norm else None
             pos = part(POSITION_ENCODINGS, "position encoding", b.position) if b.position else None
+            if weight_format is not None:                     # block by block: one block's matrices are there in both forms
+                in_fp4 += [p.to_fp4() for p in (mixer, ff) if hasattr(p, "to_fp4")]
             # an arrangement with constants or tensors of its own gets them like any other part
             own = {"params": b.params, "weights": b.weights, "build": build} if (b.params or b.weights) else {}
             self.blocks.append(lookup(BLOCKS, b.kind, "block")(mixer, ff, n1, n2, pos, **own))
+        if weight_format is not None and not any(in_fp4):
+            raise ValueError(f"weight_format {weight_format!r}: no part of this model has matrices that it can hold in that format")
         self.final_norm = part(NORMS, "norm", spec.final_norm)
         self.head = part(HEADS, "head", spec.head)
         self.adapters = [part(STREAM_ADAPTERS, "stream adapter", a) for a in spec.adapters]
@@ -504,6 +517,9 @@ class Model:
                     if key not in seen:
                         seen.add(key)
                         out.append(v)
+            elif isinstance(v, Fp4Matrix):
+                take(v.codes)
+                take(v.scales)
             elif isinstance(v, (list, tuple)):
                 for e in v:
                     take(e, depth)
@@ -520,7 +536,7 @@ class Model:
         return sum(t.untyped_storage().nbytes() for t in self.weight_tensors())
 
     def matrix_elements(self) -> int:
-        """Elements of the two-dimensional weights a token passes through (the head aside)."""
+        """Elements of the two-dimensional weights a token passes through (the head aside; of 4-bit matrices bytes)."""
         head = {t.untyped_storage().data_ptr() for t in vars(self.head).values() if isinstance(t, torch.Tensor)}
         return sum(t.untyped_storage().nbytes() // t.element_size() for t in self.weight_tensors()
                    if t.dim() == 2 and t.untyped_storage().data_ptr() not in head)

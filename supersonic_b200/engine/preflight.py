@@ -64,10 +64,28 @@ def _part_specs(spec):
     yield from spec.adapters
 
 
-def weight_bytes(spec, store, dtype: torch.dtype) -> int:
+def _fp4_names(spec):
+    """Names of the tensors that 4-bit matrices are made of, block by block."""
+    for b in spec.blocks:
+        names = set()
+        for ps, table, what in ((b.mixer, MIXERS, "mixer"), (b.feed_forward, FEED_FORWARDS, "feed-forward")):
+            roles = getattr(lookup(table, ps.kind, what), "fp4_roles", ()) if ps is not None else ()
+            names |= {n for r, n in (ps.weights.items() if roles else ()) if any(r == x or (x.endswith(".") and r.startswith(x)) for x in roles)}
+        yield names
+
+
+def weight_bytes(spec, store, dtype: torch.dtype, weight_format: Optional[str] = None) -> int:
     """Matrices are kept in ``dtype``; vectors (norm weights) as stored.  A tensor two parts name
-    (a tied head) is counted once."""
+    (a tied head) is counted once.  In a 4-bit format: 17 bytes for 32 numbers of the matrices that have it, and once the largest
+    block's matrices as they are loaded (a matrix whose sizes have no such form is larger than is counted here)."""
     item = torch.empty((), dtype=dtype).element_size()
+    if weight_format is not None:
+        def numel(n):
+            return int(torch.Size(store.shape(n)).numel()) if n in store else 0
+        blocks = list(_fp4_names(spec))
+        held = set().union(*blocks) if blocks else set()
+        whole = weight_bytes(spec, store, dtype) - item * sum(numel(n) for n in held)
+        return whole + sum(numel(n) for n in held) * 17 // 32 + item * max([sum(numel(n) for n in names) for names in blocks] + [0])
     names = {n for p in _part_specs(spec) for n in p.weights.values()}
     names |= {n for b in spec.blocks for n in b.weights.values()}
     total = 0
@@ -127,18 +145,18 @@ def workspace_bytes(spec, dtype: torch.dtype, step_tokens: int, decode_rows: int
 
 
 def estimate(spec, store, dtype: torch.dtype, max_tokens: int, max_seq_tokens: int,
-             max_slots: Optional[int], step_token_budget: int) -> MemoryEstimate:
+             max_slots: Optional[int], step_token_budget: int, weight_format: Optional[str] = None) -> MemoryEstimate:
     from ..cache.sequence_cache import pages_for
     slots = max_slots if max_slots is not None else min(pages_for(max_tokens), 4096)
     return MemoryEstimate(
-        weights=weight_bytes(spec, store, dtype),
+        weights=weight_bytes(spec, store, dtype, weight_format),
         cache=SequenceCache.bytes_needed(cache_needs(spec), max_tokens, max_seq_tokens, dtype, max_slots),
         workspace=workspace_bytes(spec, dtype, min(step_token_budget, max_tokens), min(slots, 256)))
 
 
-def check(spec, store, dtype, device, max_tokens, max_seq_tokens, max_slots, step_token_budget) -> MemoryEstimate:
+def check(spec, store, dtype, device, max_tokens, max_seq_tokens, max_slots, step_token_budget, weight_format=None) -> MemoryEstimate:
     """Estimate, compare with what the device has free, raise :class:`MemoryPreflightError`."""
-    est = estimate(spec, store, dtype, max_tokens, max_seq_tokens, max_slots, step_token_budget)
+    est = estimate(spec, store, dtype, max_tokens, max_seq_tokens, max_slots, step_token_budget, weight_format)
     device = torch.device(device)
     if device.type == "cuda":
         free, total = torch.cuda.mem_get_info(device)
@@ -151,5 +169,6 @@ def check(spec, store, dtype, device, max_tokens, max_seq_tokens, max_slots, ste
     return est
 
 
-def estimate_only(spec, store, dtype, device, max_tokens, max_seq_tokens, max_slots, step_token_budget) -> MemoryEstimate:
-    return estimate(spec, store, dtype, max_tokens, max_seq_tokens, max_slots, step_token_budget)
+def estimate_only(spec, store, dtype, device, max_tokens, max_seq_tokens, max_slots, step_token_budget,
+                  weight_format=None) -> MemoryEstimate:
+    return estimate(spec, store, dtype, max_tokens, max_seq_tokens, max_slots, step_token_budget, weight_format)

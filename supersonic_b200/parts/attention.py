@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from ..cache import PAGE_SHIFT, KvNeed
+from .fp4 import fp4_fits, fp4_of
 from .registry import BuildContext, register_mixer
 
 
@@ -51,6 +52,16 @@ class Attention:
         self.w_qkv = torch.cat([q, k, v], dim=0).contiguous()
         self.w_q = self.w_qkv[: self.n_q * self.head_dim]     # for a stop that only reads a cache
         self.dtype = build.dtype
+
+    fp4_roles = ("q", "k", "v", "o")
+
+    def to_fp4(self) -> bool:
+        """The projections as 4-bit matrices; False (and nothing changes) where their sizes have no such form."""
+        if not all(fp4_fits(w) for w in (self.w_qkv, self.w_o)):
+            return False
+        self.w_qkv, self.w_o = fp4_of(self.w_qkv), fp4_of(self.w_o)
+        self.w_q = self.w_qkv.first_rows(self.n_q * self.head_dim)
+        return True
 
     def cache_need(self):
         return KvNeed(self.n_kv, self.head_dim, self.window)

@@ -14,6 +14,10 @@ chosen experts and their weights:
 * ``softmax``: scores s = softmax(W x + b) over all experts in float32 (the bias b is optional); the experts with the largest scores are chosen;
   the weights are their s times ``scale``, with ``renormalize`` divided by their sum (+ 1e-20), which is the softmax over
   the chosen experts' logits alone.
+* ``scored``: scores s = softmax(W x) or sigmoid(W x) (``scores``) over all experts; experts are chosen by s + correction (a stored
+  vector, optional) among those of the ``keep`` best of ``groups`` equal groups of neighbours, a group's score being its largest choice
+  score or the sum of its two largest (``group_score`` "max", "two"); the weights are the chosen experts' s times ``scale``, with
+  ``renormalize`` divided by their sum (+ 1e-20).
 
 A shared expert runs for every token; with ``shared.gate`` its result is multiplied by sigmoid(w_sg . x), one number
 per token.
@@ -30,6 +34,8 @@ from typing import Dict
 import torch
 
 from ..csrc.kernel_sets import as_tensor
+from ..weights.fp4 import Fp4Matrix
+from .fp4 import fp4_fits, fp4_of
 from .registry import BuildContext, register_feed_forward
 
 ROUTERS: Dict[str, type] = {}
@@ -141,6 +147,43 @@ class SoftmaxRouter:
                                   bias=self.bias)
 
 
+@register_router("scored")
+class ScoredRouter:
+    """params: ``scores`` ("softmax" or "sigmoid"), ``groups`` (1), ``keep`` (all groups), ``group_score`` ("two"), ``renormalize`` (True),
+    ``scale`` (1.0); weights: ``weight`` [experts, hidden], ``correction`` [experts] (optional).  The logits are a product of their own
+    with a float32 result, as the other routers'; what is close is chosen in 64 bits (``ops.route_scored``)."""
+
+    def __init__(self, params, weights, build: BuildContext, n_experts: int, top: int):
+        from ..csrc.ops import GROUP_SCORES, ROUTE_MOST_EXPERTS, ROUTE_MOST_GROUPS, SCORES
+        self.n_experts, self.top = n_experts, top
+        self.scores, self.group_score = str(params.get("scores", "softmax")), str(params.get("group_score", "two"))
+        self.groups = int(params.get("groups") or 1)
+        self.keep = int(params.get("keep") or self.groups)
+        self.renormalize, self.scale = bool(params.get("renormalize", True)), float(params.get("scale", 1.0))
+        if self.scores not in SCORES or self.group_score not in GROUP_SCORES:
+            raise ValueError(f"scored router: scores {self.scores!r} of {sorted(SCORES)}, group_score {self.group_score!r} of {list(GROUP_SCORES)}")
+        if n_experts > ROUTE_MOST_EXPERTS or not 1 <= self.groups <= ROUTE_MOST_GROUPS or n_experts % self.groups \
+                or not 1 <= self.keep <= self.groups or not 1 <= top <= self.keep * (n_experts // self.groups):
+            raise ValueError(f"scored router: {top} of {n_experts} experts (up to {ROUTE_MOST_EXPERTS}) in {self.groups} equal groups (up to "
+                             f"{ROUTE_MOST_GROUPS}), {self.keep} of them kept")
+        w = build.weights.as_dtype(weights["weight"], build.dtype)
+        if w.dim() != 2 or w.shape[0] != n_experts:
+            raise ValueError(f"{weights['weight']} has shape {tuple(w.shape)}, expected [{n_experts}, hidden]")
+        pad = (-n_experts) % 8                   # rows of the product's result stay a multiple of 8 wide
+        if pad:
+            w = torch.cat([w, torch.zeros((pad, w.shape[1]), dtype=w.dtype, device=w.device)], dim=0)
+        self.weight = w.contiguous()
+        self.correction = None
+        if weights.get("correction"):
+            self.correction = build.weights.stored(weights["correction"]).float().contiguous()
+            if tuple(self.correction.shape) != (n_experts,):
+                raise ValueError(f"{weights['correction']} has shape {tuple(self.correction.shape)}, expected ({n_experts},)")
+
+    def route(self, ctx, x, expert_of, pair_weight):
+        ctx.kernels.route_scored(x, self.weight, self.n_experts, expert_of, pair_weight, self.scores, self.correction, self.groups, self.keep,
+                                 self.group_score, self.renormalize, self.scale)
+
+
 def group_buffers(kernels, n_tokens: int, top: int, n_experts: int, hidden: int, inter: int, device) -> dict:
     """The int32 buffers that sorting the step's (token, choice) pairs by expert fills and the grouped products read, with
     the sizes a kernel set asks for."""
@@ -216,27 +259,47 @@ class Experts:
         shared = 3 * int(params["shared"]["intermediate_size"]) if params.get("shared") else 0
         return int(params["top"]) * (inner * int(params["expert_size"]) + 3 * int(params["hidden_size"])) + shared
 
+    fp4_roles = ("gate.", "up.", "down.", "shared.gate", "shared.up", "shared.down")
+
+    def to_fp4(self) -> bool:
+        """The experts' matrices (and the shared one's) as 4-bit ones; False (and nothing changes) where their sizes have no such form."""
+        if not (fp4_fits(self.w_down) and fp4_fits(self.w_first) and self.inter % 32 == 0 and self.E <= 4096):
+            return False
+        self.w_first, self.w_down = fp4_of(self.w_first, gated=self.gated), fp4_of(self.w_down)
+        if self.shared is not None:
+            self.shared.to_fp4()
+        return True
+
+    @property
+    def in_fp4(self) -> bool:
+        return isinstance(self.w_down, Fp4Matrix)
+
     @property
     def sums_choices(self) -> bool:
         """Whether the result is the weighted sum over the choices alone: a block may then take ``terms`` and sum itself."""
-        return self.shared is None
+        return self.shared is None and not self.in_fp4
 
     def terms(self, ctx, x):
         """(y [tokens x top, hidden] float32, the choices' weights [tokens, top], top)."""
         return self._choices(ctx, as_tensor(x))[:2] + (self.top,)
 
     def forward(self, ctx, x, residual):
-        y, pair_weight, shared_scale = self._choices(ctx, as_tensor(x))
-        ctx.kernels.expert_combine(residual, y, pair_weight, self.top)
+        if self.in_fp4:
+            xt = as_tensor(x)
+            expert_of, pair_weight, shared_scale = self._route(ctx, xt)
+            ctx.kernels.fp4_experts(xt, expert_of, pair_weight, self.w_first, self.w_down, residual, self.act)
+        else:
+            y, pair_weight, shared_scale = self._choices(ctx, as_tensor(x))
+            ctx.kernels.expert_combine(residual, y, pair_weight, self.top)
         if self.shared is not None:
             if shared_scale is None:
                 self.shared.forward(ctx, x, residual)
             else:
                 self.shared.forward(ctx, x, residual, row_scale=shared_scale)
 
-    def _choices(self, ctx, xt):
+    def _route(self, ctx, xt):
+        """The tokens' experts, their weights, and the shared expert's factor a token (None: no gate)."""
         T, dev, top = xt.shape[0], xt.device, self.top
-        P = T * top
         expert_of = torch.empty((T, top), dtype=torch.int32, device=dev)
         pair_weight = torch.empty((T, top), dtype=torch.float32, device=dev)
         shared_scale = None
@@ -245,6 +308,12 @@ class Experts:
             self.router.route(ctx, xt, expert_of, pair_weight, extra_out=shared_scale)
         else:
             self.router.route(ctx, xt, expert_of, pair_weight)
+        return expert_of, pair_weight, shared_scale
+
+    def _choices(self, ctx, xt):
+        T, dev, top = xt.shape[0], xt.device, self.top
+        P = T * top
+        expert_of, pair_weight, shared_scale = self._route(ctx, xt)
         groups = group_buffers(ctx.kernels, T, top, self.E, self.hidden, self.inter, dev)
         ctx.kernels.group_by_expert(expert_of, self.E, groups, xt)
         z = torch.empty((P, self.inter), dtype=self.dtype, device=dev)

@@ -6,6 +6,8 @@ from __future__ import annotations
 
 import torch
 
+from ..weights.fp4 import Fp4Matrix
+from .fp4 import fp4_fits, fp4_of
 from .registry import BuildContext, register_feed_forward
 
 
@@ -53,9 +55,25 @@ class SwiGLU:
         """Elements per token this part holds while it runs: gate and up, and their product."""
         return 3 * int(params["intermediate_size"])
 
+    fp4_roles = ("gate", "up", "down")
+
+    def to_fp4(self) -> bool:
+        """The unit's matrices as 4-bit ones; False (and nothing changes) where their sizes have no such form."""
+        if not (fp4_fits(self.w_down) and fp4_fits(self.w_gate_up) and self.inter % 32 == 0):
+            return False
+        w = self.w_gate_up
+        if self.layout == "interleaved":                       # [8 gate | 8 up] per 16 rows: the gate rows, then the up rows
+            w = w.view(self.inter // 8, 2, 8, -1).transpose(0, 1).reshape(w.shape)
+        self.w_gate_up, self.layout = fp4_of(w, gated=True), "fp4"
+        self.w_down = fp4_of(self.w_down)
+        return True
+
     def forward(self, ctx, x, residual, row_scale=None):
         """``row_scale``: one float32 factor per token on the unit's result (applied to the inner rows, which the
         last product maps linearly)."""
+        if self.layout == "fp4":
+            ctx.kernels.fp4_gated_unit(x, self.w_gate_up, self.w_down, residual, self.act, row_scale)
+            return
         z = torch.empty((residual.shape[0], self.inter), dtype=self.dtype, device=residual.device)
         if self.act is None and row_scale is None:
             ctx.kernels.gate_up_swiglu(x, self.w_gate_up, self.layout, z)
@@ -92,7 +110,19 @@ class DenseFeedForward:
     def activation_elements(params) -> int:
         return 2 * int(params["intermediate_size"])
 
+    fp4_roles = ("up", "down")
+
+    def to_fp4(self) -> bool:
+        """The matrices as 4-bit ones; False (and nothing changes) where their sizes have no such form."""
+        if not (fp4_fits(self.w_up) and fp4_fits(self.w_down) and self.inter % 32 == 0):
+            return False
+        self.w_up, self.w_down = fp4_of(self.w_up), fp4_of(self.w_down)
+        return True
+
     def forward(self, ctx, x, residual):
+        if isinstance(self.w_up, Fp4Matrix):
+            ctx.kernels.fp4_dense_unit(x, self.w_up, self.w_down, residual, self.activation, self.out_scale)
+            return
         z = torch.empty((residual.shape[0], self.inter), dtype=self.dtype, device=residual.device)
         ctx.kernels.linear_activation(x, self.w_up, z, self.activation, self.out_scale)
         ctx.kernels.linear(z, self.w_down, residual, accumulate=True)

@@ -71,6 +71,13 @@ class Fp4Matrix:
         s = s.view(s.shape[0], s.shape[1] // _RUN_ROWS, 4, 32, s.shape[2] // _RUN_BLOCKS, 2, 4).permute(0, 1, 4, 5, 3, 2, 6)
         return cls(codes.contiguous(), s.reshape(-1, 1024).contiguous(), shape, gated)
 
+    def first_rows(self, n: int) -> "Fp4Matrix":
+        """The first ``n`` rows, in the same memory."""
+        if len(self.shape) != 2 or self.gated or not 0 < n <= self.shape[0]:
+            raise ValueError(f"no first {n} rows of {self}")
+        runs = -(-n // _RUN_ROWS) * -(-self.shape[1] // (FP4_BLOCK * _RUN_BLOCKS))
+        return Fp4Matrix(self.codes[:n], self.scales[:runs], (n, self.shape[1]))
+
     def plain_scales(self) -> torch.Tensor:
         """The scales in rows, uint8 ``[.., n, k / 32]`` (rows in the order that the codes have)."""
         n, k = self.shape[-2:]
