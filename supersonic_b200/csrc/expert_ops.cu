@@ -230,13 +230,14 @@ SSB_API int ssb_route_softmax(float* z, int ld, const float* bias, int n_tokens,
 // neighbours, a group's score is its largest c or the sum of its two largest; of the experts of the `keep` best groups the `top`
 // largest c win, in order, the lower index (expert, group) at equal scores; an expert's weight is its s times `scale`, with
 // `renormalize` divided by the sum of the chosen s (+ 1e-20).  A logit that is NaN counts as minus infinity, whose s is zero, an infinite one as the
-// largest number; a c that is NaN comes last.
+// largest number; a c that is NaN comes last.  Without correction the larger logit comes first, also where both have the same s.
 //
 // What is chosen is chosen by c in 64 bits.  c in 32 bits is within RS_NEAR of it, so a warp (a token, its experts in registers)
 // chooses in 32 bits and looks whether two neighbours of its order, the last chosen and the next among them, or a kept and a
 // dropped group, are closer than that: only then (a token in some hundreds) it computes and chooses again in 64 bits.  Without
 // correction c grows with z, and the order is z's own.
-// 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: RS_FIGURE
+// 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: 34 us (49 with the 64-bit scores of close choices in local
+// memory); the logits' 8.4 MB take 1.4.  The order's rounds bound it: two reductions of a warp each, one after another.
 // ---------------------------------------------------------------------------------------
 constexpr int RS_MOST_GROUPS = 32;
 enum { RS_SOFTMAX = 0, RS_SIGMOID = 1 };
@@ -297,6 +298,11 @@ __device__ __noinline__ void rs_choose_exactly(const RsArgs& a, const float* zr,
             before += o > score || (o == score && g < lane);
         }
         stays = __ballot_sync(0xffffffffu, lane < a.n_groups && before < a.keep);
+    }
+    if (!a.correction) {                                  // c grows with z, also where 64 bits no longer show it
+        __syncwarp();
+        for (int e = lane; e < a.n_experts; e += 32) c[e] = (double)rs_logit(zr[e]);
+        __syncwarp();
     }
     double last = INFINITY;
     int last_e = -1;

@@ -21,9 +21,6 @@ __device__ __forceinline__ uint64_t fl_scale_desc(uint32_t addr) {
 __device__ __forceinline__ void fl_copy_scales(uint32_t tmem, uint32_t addr) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(fl_scale_desc(addr)) : "memory");
 }
-__device__ __forceinline__ void fl_copy_scales_pair(uint32_t tmem, uint32_t addr) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(fl_scale_desc(addr)) : "memory");
-}
 // One lane of the warp, all of whose lanes call it together.  A warp issues its products from code that all its lanes run, under this
 // lane's predicate: descriptors and addresses are then in uniform registers as the instructions want them.  (One lane alone in a branch
 // moves each of them there, some twenty for four instructions: 875 clocks a k-block with its waits, whatever the tile.)

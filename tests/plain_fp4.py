@@ -112,6 +112,10 @@ def route(logits, correction, scores, groups, keep, by, top, renormalize, scale)
         c = [-math.inf if v != v else v for v in c]
         per = len(c) // groups
         best = [sum(sorted(c[g * per:(g + 1) * per], reverse=True)[: 1 if by == "max" else 2]) for g in range(groups)]
+        if correction is None:                   # s grows with z, also where 64 bits no longer show it (exp(-1e30), sigmoid(40) and (41))
+            c = z
+            if by == "max" or per == 1:
+                best = [max(c[g * per:(g + 1) * per]) for g in range(groups)]
         kept = sorted(range(groups), key=lambda g: (-best[g], g))[:keep]
         chosen = sorted((e for g in kept for e in range(g * per, (g + 1) * per)), key=lambda e: (-c[e], e))[:top]
         f = scale / (math.fsum(s[e] for e in chosen) + 1e-20) if renormalize else scale
