@@ -657,6 +657,15 @@ struct FlPlan {
     int bn, m_tiles, n_tiles, blocks;      // bn 0: tiles on pairs
     size_t pieces;                         // bytes
 };
+// What a product is expected to take, in microseconds, by a fit to measured times of all forms over 1 .. 1,024 rows and 4 to 117
+// million weights:
+//  * a block of the streaming kernel takes 3.8 + 0.046 a row, and 0.37 a k-block of 128 weight rows whatever its rows; pieces of split
+//    tiles 2.2 and, each, 0.1 + 0.01 a row;
+//  * a pair 6.5, 0.43 a k-block of 256 x 256 and 0.03 for each tile beside it.
+// At 2,048 x 2,048: 48 rows by tiles of 64 that are whole 9.1, in 2 parts 10.7; at 4,096 x 14,336: 1 row whole 25, in 4 parts 12.1, dealt
+// out over all SMs 13.5; 128 rows by 64 in 2 parts 20.7, by 128 in 4 22.2, on pairs 30; at 14,336 x 4,096: 64 rows by 64 14.0, 128 by 128
+// 17.2, on pairs 15.7; 1,024 rows by 128 70, on pairs 35.  Tiles of 16 and 32 rows are only where one holds all rows: the next one's
+// scales would begin between the columns that a product can name.
 static FlPlan fl_plan(int M, int N, int K) {
     const int sms = ssb_sm_count(), k_blocks = f4_k_blocks(K);
     FlPlan best{};
@@ -667,22 +676,21 @@ static FlPlan fl_plan(int M, int N, int K) {
         best = FlPlan{bn, m_tiles, n_tiles, blocks, (size_t)blocks * 2 * bn * FL_BM * 4};
     };
     for (int bn = M <= 16 ? 16 : M <= 32 ? 32 : 64; bn <= 128; bn *= 2) {
-        const int m_tiles = (M + bn - 1) / bn, n_tiles = (N + FL_BM - 1) / FL_BM;
+        const int m_tiles = (M + bn - 1) / bn, n_tiles = (N + FL_BM - 1) / FL_BM, rows = std::min(bn, M);
         const long long tiles = (long long)m_tiles * n_tiles, units = tiles * k_blocks;
-        const double each = bn < 128 ? 0.36 : m_tiles == 1 ? 0.6 : 0.45;
-        const double piece = 0.012 * std::min(bn, M);
-        const int any = (int)std::min<long long>(sms, std::max(1LL, units / 4));
-        consider(9 + each * (double)((units + any - 1) / any) + 4 + piece * (double)((any + tiles - 1) / tiles), bn, m_tiles, n_tiles, any);
-        if (tiles <= sms) {
-            const int parts = std::min(sms / (int)tiles, std::max(1, k_blocks / (bn <= 32 ? 4 : 8)));
-            consider(9 + each * ((k_blocks + parts - 1) / parts) + (parts > 1 ? piece * parts : 0), bn, m_tiles, n_tiles, (int)tiles * parts);
-        }
+        const double block = 3.8 + 0.046 * rows, piece = 0.1 + 0.01 * rows;
+        if (tiles <= sms)
+            for (int parts = 1; parts <= std::min(sms / (int)tiles, k_blocks); ++parts)
+                consider(block + 0.37 * ((k_blocks + parts - 1) / parts) + (parts > 1 ? 2.2 + piece * parts : 0), bn, m_tiles, n_tiles, (int)tiles * parts);
+        const int any = (int)std::min<long long>(sms, units);
+        const double share = (double)tiles / any;
+        consider(block + 0.37 * ((double)units / any) + 3.7 + piece * std::max(2.0, 1 / share) + share * (0.7 + 0.046 * rows), bn, m_tiles, n_tiles, any);
         if (M <= bn) break;
     }
     if (M > 64) {
         const int m_tiles = (M + 255) / 256, n_tiles = (N + 255) / 256, pairs = sms / 2;
         const long long tiles = (long long)m_tiles * n_tiles;
-        consider(8 + 0.37 * (double)((tiles + pairs - 1) / pairs) * k_blocks + 0.09 * (double)std::min<long long>(tiles, pairs), 0, m_tiles, n_tiles, 0);
+        consider(6.5 + 0.43 * (double)((tiles + pairs - 1) / pairs) * k_blocks + 0.03 * (double)std::min<long long>(tiles, pairs), 0, m_tiles, n_tiles, 0);
     }
     return best;
 }
@@ -700,11 +708,22 @@ struct FlScratch {
         all = pieces + std::max<size_t>(piece_bytes, 16);
     }
 };
-// The kernel of few rows takes products where there is little to read; where the weights' bytes count, its instructions a weight do too
-// (fl_product).
-constexpr long long FL_FEW_NUMBERS = 32768, FL_FEW_WEIGHTS = 5 << 20;
+// The kernel of few rows (its time is for rows that come as numbers; the others' with their launch before it) takes products where there
+// is little to read; where the weights' bytes count, its instructions a weight and a row do too.  Up to 8 rows: 1 x 4,096 x 4,096 5.2 us
+// (8.0 by tiles of 16), 8 rows 7.2 (8.1); 8 x 8,192 x 4,096 10.0 (9.7), 4 x 4,096 x 14,336 15.7 (12.8).  Above: 16 x 4,096 x 2,048 6.6
+// (7.2), 16 x 8,192 x 2,048 8.4 (7.5).  Inner rows are put into 4 bits a block of 32 at a time, which is fewer and longer strips of
+// weights: 8 x 2,048 x 2,048 5.8 (7.1), 16 8.6 (7.6), 8 x 4,096 x 4,096 9.6 (8.3), 1 x 1,024 x 8,192 11.5 (8.0).  They are taken where the
+// product behind them is as well, as its counters come from a launch that quantises.
+constexpr long long FL_FEW_NUMBERS = 32768, FL_FEW_INNER = 16384, FL_FEW_WEIGHTS = 24 << 20, FL_FEW_WEIGHTS_16 = 8 << 20;
 static bool fl_few(int M, int N, int K, int mode) {
-    return (long long)M * K <= FL_FEW_NUMBERS && (long long)N * K <= FL_FEW_WEIGHTS && fw_takes(M, N, K, mode);
+    if ((long long)N * K > (M <= 8 ? FL_FEW_WEIGHTS : FL_FEW_WEIGHTS_16)) return false;
+    if (mode == FL_STORE) {
+        if ((long long)M * K > FL_FEW_NUMBERS) return false;
+    } else {
+        const int inter = mode == FL_GATED ? N / 2 : N;
+        if (M > 8 || K > 4096 || (long long)M * K > FL_FEW_INNER || (long long)M * inter > FL_FEW_NUMBERS) return false;
+    }
+    return fw_takes(M, N, K, mode);
 }
 
 // Twice the bytes of scratch that a product needs, and one if it needs counters.  numbers: rows come as numbers; mode: FL_*.
@@ -843,7 +862,7 @@ SSB_API int ssb_fp4_inner(const void* x, long long ldx, int dtype, const void* x
 // Pairs (token, choice) by expert, one block.  A warp has a run of neighbouring pairs and counts of its own: it counts them by expert, the
 // counts of the warps before it say where its pairs go, and it places them.  ``slot``: where a pair's row goes among tiles of BN rows
 // (-1: its expert is none), ``order``: the pair of a sorted row.  The order of an expert's pairs inside a warp's run is whatever the adds
-// give; nothing that leaves the call depends on it.  12,288 pairs of 64 experts: GROUP_FIGURE us (counts that all warps share 16, ranks by
+// give; nothing that leaves the call depends on it.  12,288 pairs of 64 experts: 14.7 us (counts that all warps share 16, ranks by
 // match.any 26).
 constexpr int FL_GROUP_WARPS = 32;
 
@@ -970,10 +989,6 @@ __device__ __forceinline__ int fl_sort_pairs(const int* __restrict__ expert_of, 
     return tiles;
 }
 
-bool fw_takes(int M, int N, int K, int mode);
-bool fw_takes_list(int pairs, int experts, int N, int K, int mode);
-int fw_product(FwArgs a, int mode, cudaStream_t stream);
-int fw_product_list(FwArgs a, int mode, cudaStream_t stream);
 
 // Tiles of up to FL_SORTED_PAIRS pairs beside their rows into 4 bits, in one launch: every block sorts the pairs for itself, and takes
 // k-blocks of rows by its warps (a lane eight numbers, four lanes a block).
@@ -1072,17 +1087,24 @@ fp4_combine_kernel(const float* __restrict__ y, const int* __restrict__ expert_o
     }
 }
 
-// Rows a tile, by how many an expert has on average: no more than the step has tokens, and little of a tile empty.
-static int fl_list_rows(int tokens, int top, int experts) {
+// Rows a tile, by how many an expert has on average.  Tiles of 16 where most experts fill one; tiles on SM pairs where an expert fills
+// more; between them, where sums are long enough to hide the larger tile's epilogue, tiles of 64.  Microseconds, all measured with tiles of
+// 16 / 64 / 256:  64 experts of 2,048 x 1,408, 6 a token: a mean of 6 rows 72 / 80 / 89, of 12 82 / 103 / 93, of 18 103 / 115 / 95, of 48
+// 172 / 165 / 104;  256 of 7,168 x 512: 16 rows 521 / 653 / 564, 24 692 / 798 / 606;  16 of 4,096 x 6,400: 4 rows 121 / 122 / 155, 12
+// 142 / 131 / 158, 32 263 / 152 / 161, 48 353 / 176 / 167;  8 of 4,096 x 14,336: 12 rows 154 / 139 / 176, 32 304 / 161 / 178, 48 374 /
+// 181 / 179.  (Of 32: 5 to 10 % less than these where a mean of 12 to 20 meets sums of some 3,000, nothing elsewhere; of 128: never least.)
+static int fl_list_rows(int tokens, int top, int experts, int K, int inter) {
     const long long mean = (long long)tokens * top / experts;
-    return tokens <= 16 || mean <= 8 ? 16 : tokens <= 32 || mean <= 16 ? 32 : tokens <= 64 || mean <= 48 ? 64 : mean <= 96 ? 128 : 256;
+    if (tokens <= 16 || mean <= 8) return 16;
+    if (K >= 4096 && inter >= 4096) return mean <= 40 ? 64 : 256;
+    return mean <= 16 ? 16 : 256;
 }
 struct FlExperts {
     int bn, tiles, blocks;                 // rows a tile, tiles at most, blocks of a product
     size_t counters, offsets, order, slot, tile_expert, tile_row0, meta, x, xs, z, zs, y, pieces, all;
     FlExperts(int tokens, int top, int experts, int K, int inter) {
         const int pairs = tokens * top;
-        bn = fl_list_rows(tokens, top, experts);
+        bn = fl_list_rows(tokens, top, experts, K, inter);
         tiles = pairs / bn + std::min(experts, pairs);
         blocks = ssb_sm_count();
         const size_t rows = (size_t)tiles * bn, chunks = (size_t)tiles * (bn > 128 ? 2 : 1) * F4_CHUNK;
@@ -1100,7 +1122,7 @@ struct FlExperts {
         z = take(rows * (inter / 2));
         zs = take(chunks * f4_k_blocks(inter));
         y = take((size_t)pairs * K * 4);
-        pieces = bn <= 128 ? take((size_t)blocks * 2 * bn * FL_BM * 4) : at;
+        pieces = bn < 256 ? take((size_t)blocks * 2 * bn * FL_BM * 4) : at;
         all = at;
     }
 };
@@ -1119,12 +1141,10 @@ static int fl_listed(const void* x, const void* xs, const void* w, const void* w
     if (!rc) rc = fl_scale_map(&mxs, xs, (long long)at.tiles * (at.bn > 128 ? 2 : 1) * k_blocks);
     if (!rc) rc = fl_scale_map(&mws, ws, (long long)experts * n_tiles * k_blocks);
     if (rc) return rc;
-    switch (at.bn) {
-        case 16: return fl_stream<16, 5, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
-        case 32: return fl_stream<32, 9, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
-        case 64: return fl_stream<64, 8, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
-        case 128: return fl_stream<128, 6, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
-    }
+    if (at.bn == 16)
+        return fl_stream<16, 5, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+    if (at.bn == 64)
+        return fl_stream<64, 8, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
     return fl_pair<MODE, true>(mx, mw, xs, ws, 2 * at.tiles, o, list, at.tiles, (o.N + 255) / 256, K, error_word, stream);
 }
 
