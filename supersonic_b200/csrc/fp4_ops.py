@@ -125,6 +125,8 @@ def _operands(what: str, x: Rows, weight: Fp4Matrix):
     n, k = weight.shape
     if n % 8:
         raise KernelError(f"{what}: n {n} must be a multiple of 8")
+    if weight._buffer is not None:             # a product reads its weights ahead of the launch before it
+        raise KernelError(f"{what}: a unit's inner rows are rows, not weights")
     if isinstance(x, Fp4Matrix):
         if len(x.shape) != 2 or x.shape[1] != k or x.gated:
             raise KernelError(f"{what}: rows of {k} numbers, not {x}")
@@ -175,6 +177,8 @@ def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = Fal
     _here(out.get_device())
     if rows == 0:
         return
+    if o_at == x_at:
+        raise KernelError("linear: out must not be x")
     device = weight.device
     needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_STORE)
     held, scratch, counters = _workspace(x, needs, device, _COUNTERS)

@@ -76,7 +76,9 @@ class Fp4Matrix:
         if len(self.shape) != 2 or self.gated or not 0 < n <= self.shape[0]:
             raise ValueError(f"no first {n} rows of {self}")
         runs = -(-n // _RUN_ROWS) * -(-self.shape[1] // (FP4_BLOCK * _RUN_BLOCKS))
-        return Fp4Matrix(self.codes[:n], self.scales[:runs], (n, self.shape[1]))
+        m = Fp4Matrix(self.codes[:n], self.scales[:runs], (n, self.shape[1]))
+        m._buffer = self._buffer
+        return m
 
     def plain_scales(self) -> torch.Tensor:
         """The scales in rows, uint8 ``[.., n, k / 32]`` (rows in the order that the codes have)."""

@@ -131,6 +131,19 @@ def test_linear_refuses(kw):
         fp4_ops.linear(kw.get("x", z(3, 64)), kw.get("w", matrix(16, 64)), kw.get("out", z(3, 16)), accumulate=kw.get("add", False))
 
 
+def test_inner_rows_are_no_weights_and_results_no_rows():
+    size, both = Fp4Matrix.rows_layout(64, 64)
+    rows = Fp4Matrix.over_rows(torch.zeros(both, dtype=torch.int8), 64, 64, size)
+    rows.index = 0
+    for weight in (rows, rows.first_rows(32)):
+        weight.index = 0
+        with pytest.raises(KernelError, match="not weights"):
+            fp4_ops.linear(z(4, 64), weight, z(4, weight.shape[0]))
+    x = z(4, 64)
+    with pytest.raises(KernelError, match="must not be x"):
+        fp4_ops.linear(x, matrix(64, 64), x)
+
+
 @pytest.mark.parametrize("call", [
     lambda: fp4_ops.gate_up(z(3, 64), matrix(64, 64)), lambda: fp4_ops.gate_up(z(3, 64), matrix(64, 64, gated=True), ("tanh", 0.0)),
     lambda: fp4_ops.gate_up(z(0, 64), matrix(64, 64, gated=True)), lambda: fp4_ops.gate_up(z(3, 32), matrix(64, 64, gated=True)),
