@@ -865,44 +865,50 @@ SSB_API int ssb_fp4_inner(const void* x, long long ldx, int dtype, const void* x
 // give; nothing that leaves the call depends on it.  12,288 pairs of 64 experts: 14.7 us (counts that all warps share 16, ranks by
 // match.any 26).
 constexpr int FL_GROUP_WARPS = 32;
+// Words from one warp's counts to the next's: an odd number, so that an expert's counts lie in as many banks.
+__host__ __device__ __forceinline__ int fl_group_stride(int experts, int n_warps) { return n_warps > 1 ? experts | 1 : experts; }
 
 __global__ void __launch_bounds__(32 * FL_GROUP_WARPS)
 fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int bn, int* __restrict__ offsets, int* __restrict__ order,
                  int* __restrict__ slot, int* __restrict__ tile_expert, int* __restrict__ tile_row0, int* __restrict__ meta,
                  int* __restrict__ clear, int n_clear, int n_warps) {
-    extern __shared__ int counts[];                                // [n_warps][experts]; then [experts] first row, first tile
-    int *row0 = counts + n_warps * experts, *tile0 = row0 + experts;
+    extern __shared__ int counts[];                                // [n_warps] rows of ``stride`` for the experts; two more: first row, first tile
+    const int stride = fl_group_stride(experts, n_warps);
+    int *row0 = counts + n_warps * stride, *tile0 = row0 + stride;
     ssb_pdl_wait();
     ssb_pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = (pairs + n_warps - 1) / n_warps;
     const int lo = min(pairs, warp * run), hi = warp < n_warps ? min(pairs, lo + run) : lo;
     for (int i = threadIdx.x; i < n_clear; i += blockDim.x) clear[i] = 0;
-    for (int e = threadIdx.x; e < n_warps * experts; e += blockDim.x) counts[e] = 0;
+    for (int e = threadIdx.x; e < n_warps * stride; e += blockDim.x) counts[e] = 0;
     __syncthreads();
-    int* mine = counts + min(warp, n_warps - 1) * experts;
-    auto expert_at = [&](int p) {
-        const int e = p < hi ? expert_of[p] : -1;
-        return (unsigned)e < (unsigned)experts ? e : -1;
-    };
-    constexpr int AHEAD = 8;                                       // loads in flight
-    for (int p0 = lo; p0 < hi; p0 += 32 * AHEAD) {
-        int es[AHEAD];
-#pragma unroll
-        for (int q = 0; q < AHEAD; ++q) es[q] = expert_at(p0 + 32 * q + lane);
+    int* mine = counts + min(warp, n_warps - 1) * stride;
+    constexpr int AHEAD = 16;                                      // loads in flight, kept where they are a warp's whole run
+    int es[AHEAD];
+    auto load = [&](int p0) {
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
-            if (es[q] >= 0) atomicAdd(mine + es[q], 1);
+            const int p = p0 + 32 * q + lane, e = p < hi ? expert_of[p] : -1;
+            es[q] = (unsigned)e < (unsigned)experts ? e : -1;
         }
+    };
+    for (int p0 = lo; p0 < hi; p0 += 32 * AHEAD) {
+        load(p0);
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+            if (es[q] >= 0) atomicAdd(mine + es[q], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {      // an expert's counts become the rows before each warp's
-        int sum = 0;
-        for (int w = 0; w < n_warps; ++w) {
-            const int n = counts[w * experts + e];
-            counts[w * experts + e] = sum;
-            sum += n;
+    for (int e = warp; e < experts; e += FL_GROUP_WARPS) {         // an expert's counts become the rows before each warp's
+        const int n = lane < n_warps ? counts[lane * stride + e] : 0;
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int before = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += before;
         }
-        row0[e] = sum;
+        if (lane < n_warps) counts[lane * stride + e] = sum - n;
+        if (lane == 31) row0[e] = sum;
     }
     __syncthreads();
     if (warp == 0) {
@@ -927,21 +933,19 @@ fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int 
     }
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += blockDim.x)
-        for (int i = 0; row0[e] + i < offsets[e + 1]; i += bn) {
-            tile_expert[tile0[e] + i / bn] = e;
-            tile_row0[tile0[e] + i / bn] = row0[e] + i;
+        for (int t = tile0[e], end = e + 1 < experts ? tile0[e + 1] : meta[0]; t < end; ++t) {
+            tile_expert[t] = e;
+            tile_row0[t] = row0[e] + (t - tile0[e]) * bn;
         }
     for (int p0 = lo; p0 < hi; p0 += 32 * AHEAD) {
-        int es[AHEAD];
-#pragma unroll
-        for (int q = 0; q < AHEAD; ++q) es[q] = expert_at(p0 + 32 * q + lane);
+        if (run > 32 * AHEAD) load(p0);
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
             const int e = es[q], p = p0 + 32 * q + lane;
             int to = -1;
             if (e >= 0) {
                 const int i = atomicAdd(mine + e, 1);
-                to = (tile0[e] + i / bn) * bn + i % bn;
+                to = tile0[e] * bn + i;                            // an expert's tiles are neighbours
                 order[row0[e] + i] = p;
             }
             if (p < hi) slot[p] = to;
@@ -1175,8 +1179,8 @@ SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* 
         rc = dtype == SSB_BF16 ? place(fp4_place_kernel<bf16, 16>, (const bf16*)x) : place(fp4_place_kernel<float, 16>, (const float*)x);
     } else {
         // as many warps as shared memory has room for their counts
-        const int n_warps = std::max(1, std::min(FL_GROUP_WARPS, 48 * 1024 / (4 * experts) - 2));
-        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(32 * FL_GROUP_WARPS), (size_t)experts * (n_warps + 2) * 4, stream, true, expert_of, pairs,
+        const int n_warps = std::max(1, std::min(FL_GROUP_WARPS, 48 * 1024 / (4 * (experts | 1)) - 2));
+        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(32 * FL_GROUP_WARPS), (size_t)fl_group_stride(experts, n_warps) * (n_warps + 2) * 4, stream, true, expert_of, pairs,
                         experts, at.bn, ints(at.offsets), ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta),
                         ints(at.counters), 2 * FL_COUNTERS, n_warps);
         if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, tokens, top, K, ints(at.slot), at.bn, stream);

@@ -320,7 +320,7 @@ def test_units_one_after_another_on_two_streams():
 # ---- experts ----------------------------------------------------------------------------------------------------------
 EXPERTS = [(1, 64, 32, 4, 2), (1, 2048, 1408, 64, 6), (3, 512, 96, 8, 3), (16, 256, 320, 64, 6), (37, 288, 64, 16, 7), (40, 128, 96, 3, 2),
            (100, 512, 288, 16, 4), (64, 256, 128, 256, 8), (300, 256, 160, 8, 2), (700, 320, 96, 16, 4), (900, 256, 544, 4, 1), (33, 96, 64, 1, 1),
-           (300, 256, 160, 40, 2), (40, 4096, 4096, 4, 1), (130, 4096, 4128, 8, 2)]
+           (300, 256, 160, 40, 2), (40, 4096, 4096, 4, 1), (130, 4096, 4128, 8, 2), (70, 32, 32, 4096, 5), (40, 64, 32, 301, 11)]
 
 
 def choices(g, tokens, experts, top, lopsided=True):
