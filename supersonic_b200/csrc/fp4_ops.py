@@ -23,8 +23,8 @@ import torch
 from ..weights.fp4 import FP4_BLOCK, Fp4Matrix
 from . import ops
 from .build import load_library
-from .int8_ops import _error_word, _rows, _stream
-from .ops import KernelError, _CODES, _check
+from .int8_ops import _SIZES
+from .ops import KernelError, _CODES, _check, _raw_stream
 
 _P, _I, _F, _L = c_void_p, c_int, c_float, c_longlong
 _SIGNATURES = {
@@ -74,12 +74,38 @@ def _scratch_size(name: str, *sizes) -> int:
     return n
 
 
-def _here(*indices) -> None:
-    """Raises unless these device indices (-1: no CUDA device) are the current device's."""
+def _stream(*indices) -> int:
+    """The current stream's handle; raises unless these device indices (-1: no CUDA device) are the current device's."""
     current = torch.cuda.current_device()
     for i in indices:
         if i != current:
             raise KernelError(f"tensors must be on the current CUDA device {current}, are on {sorted(set(indices))}")
+    return _raw_stream(current) if _raw_stream is not None else ops._stream().value or 0
+
+
+_error_words = {}
+
+
+def _error_word(m: Fp4Matrix) -> int:
+    """The address of the device's error word (:func:`.ops.tc_error_word`), for a launch with bounded waits, which counts as unread."""
+    ops.note_bounded_wait_launches(1)
+    at = _error_words.get(m.index)
+    if at is None:
+        at = _error_words[m.index] = ops.tc_error_word(m.device).data_ptr()
+    return at
+
+
+def _rows(t: torch.Tensor, name: str, rows: int, width: int):
+    """(address, row stride) of a matrix [rows, width] whose rows start on 16 bytes; its device is checked where it is launched."""
+    size, shape = _SIZES.get(t.dtype), t.shape
+    if size is None or len(shape) != 2 or shape[0] != rows or shape[1] != width:
+        raise KernelError(f"{name} must be [{rows}, {width}] of float32 or bfloat16, is {t.dtype} {tuple(shape)}")
+    at, (ld, step) = t.data_ptr(), t.stride()
+    if rows == 1:
+        ld = width + -width % 8
+    if (step != 1 and width > 1) or (at | ld * size) % 16 or ld < width:
+        raise KernelError(f"{name}: rows of contiguous elements that start on 16 bytes")
+    return at, ld
 
 
 def _matrix_rows(t: torch.Tensor, name: str, m: Fp4Matrix):
@@ -87,7 +113,6 @@ def _matrix_rows(t: torch.Tensor, name: str, m: Fp4Matrix):
     shape = t.shape
     if shape != m.shape or t.dtype not in _CODES or t.get_device() != m.index:
         raise KernelError(f"{name} must be float32 or bfloat16 {m.shape} on the matrix's device, is {t.dtype} {tuple(shape)} on {t.device}")
-    _here(m.index)
     if len(shape) == 3:
         if not t.is_contiguous():
             raise KernelError(f"{name}: matrices of several experts are contiguous")
@@ -102,7 +127,7 @@ def quantize(x: torch.Tensor, matrix: Fp4Matrix) -> None:
     at, ld, rows, code = _matrix_rows(x, "x", matrix)
     n, k = matrix.shape[-2:]
     _check(_fn("ssb_fp4_quantize")(at, ld, code, matrix.codes_at, matrix.scales_at, rows, k, n,
-                                   n // 2 if matrix.gated else 0, 0, 0, 0, _stream()), "fp4_quantize")
+                                   n // 2 if matrix.gated else 0, 0, 0, 0, _stream(matrix.index)), "fp4_quantize")
 
 
 def values(matrix: Fp4Matrix, out: torch.Tensor) -> None:
@@ -111,7 +136,7 @@ def values(matrix: Fp4Matrix, out: torch.Tensor) -> None:
     at, ld, rows, code = _matrix_rows(out, "out", matrix)
     n, k = matrix.shape[-2:]
     _check(_fn("ssb_fp4_values")(matrix.codes_at, matrix.scales_at, at, ld, code, rows, k, n,
-                                 n // 2 if matrix.gated else 0, _stream()), "fp4_values")
+                                 n // 2 if matrix.gated else 0, _stream(matrix.index)), "fp4_values")
 
 
 Rows = Union[torch.Tensor, Fp4Matrix]
@@ -119,7 +144,7 @@ _MODE_STORE, _MODE_GATED, _MODE_ACT = 0, 1, 2
 
 
 def _operands(what: str, x: Rows, weight: Fp4Matrix):
-    """(rows, x's address, row stride, type code and scales' address) of rows that a dense weight takes."""
+    """(rows, x's address, row stride, type code, scales' address and device) of rows that a dense weight takes."""
     if not isinstance(weight, Fp4Matrix) or len(weight.shape) != 2:
         raise KernelError(f"{what}: weight must be a 4-bit matrix [n, k], is {weight if isinstance(weight, Fp4Matrix) else type(weight)}")
     n, k = weight.shape
@@ -130,20 +155,18 @@ def _operands(what: str, x: Rows, weight: Fp4Matrix):
     if isinstance(x, Fp4Matrix):
         if len(x.shape) != 2 or x.shape[1] != k or x.gated:
             raise KernelError(f"{what}: rows of {k} numbers, not {x}")
-        _here(x.index, weight.index)
-        return x.shape[0], x.codes_at, 0, -1, x.scales_at
+        return x.shape[0], x.codes_at, 0, -1, x.scales_at, x.index
     shape = x.shape
     if len(shape) != 2 or shape[1] != k:
         raise KernelError(f"{what}: rows of {k} numbers, not {tuple(shape)}")
     at, ld = _rows(x, "x", shape[0], k)
-    _here(x.get_device(), weight.index)
-    return shape[0], at, ld, _CODES[x.dtype], 0
+    return shape[0], at, ld, _CODES[x.dtype], 0, x.get_device()
 
 
 def _workspace(x: Rows, needs: int, device, words: int, ahead: int = 0):
     """(a buffer, the address of scratch behind its first ``ahead`` bytes, the address of ``words`` counters) of a product that ``needs``
     so much (ssb_fp4_product_scratch).  Counters are zeroed by the launch that quantises rows; a product of rows in 4 bits takes those
-    that came with them, which nobody takes twice, or has its own zeroed."""
+    that came with them, and the scratch of the launch that made them where it has room, which nobody takes twice, or has its own zeroed."""
     size, counts = needs >> 1, needs & 1
     if not counts:
         if size + ahead == 0:
@@ -151,12 +174,15 @@ def _workspace(x: Rows, needs: int, device, words: int, ahead: int = 0):
         buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
         return buffer, buffer.data_ptr() + ahead, 0
     if isinstance(x, Fp4Matrix):
-        buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
         left, x._counters = x._counters, None
-        if left is None or words > _COUNTERS:
-            left = torch.zeros(words, dtype=torch.int32, device=device)
-            return (buffer, left), buffer.data_ptr() + ahead, left.data_ptr()
-        return (buffer, left), buffer.data_ptr() + ahead, left[1]
+        if left is not None and words <= _COUNTERS:
+            if ahead == 0 and size <= left[3]:
+                return left, left[2], left[1]
+            buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
+            return (buffer, left), buffer.data_ptr() + ahead, left[1]
+        buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
+        left = torch.zeros(words, dtype=torch.int32, device=device)
+        return (buffer, left), buffer.data_ptr() + ahead, left.data_ptr()
     buffer = torch.empty(ahead + 4 * words + size, dtype=torch.int8, device=device)
     at = buffer.data_ptr() + ahead
     return buffer, at + 4 * words, at
@@ -165,29 +191,27 @@ def _workspace(x: Rows, needs: int, device, words: int, ahead: int = 0):
 def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = False) -> None:
     """``out`` [rows, n] (+)= x W^T with ``x`` [rows, k] (float32 or bfloat16, quantised as it comes, or a 4-bit matrix) and ``weight``
     [n, k].  ``accumulate`` adds to a float32 ``out``.  n: a multiple of 8."""
-    rows, x_at, ldx, code, xs_at = _operands("linear", x, weight)
+    rows, x_at, ldx, code, xs_at, index = _operands("linear", x, weight)
     if weight.gated:
         raise KernelError("linear: a gated unit's first matrix goes through gate_up")
     n, k = weight.shape
     o_at, ldo = _rows(out, "out", rows, n)
-    if out.shape[1] != n:
-        raise KernelError(f"linear: out must be [{rows}, {n}], is {tuple(out.shape)}")
     if accumulate and out.dtype is not torch.float32:
         raise KernelError("linear: results are added in float32 only")
-    _here(out.get_device())
+    if rows and o_at == x_at:
+        raise KernelError("linear: out must not be x")
+    stream = _stream(index, weight.index, out.get_device())
     if rows == 0:
         return
-    if o_at == x_at:
-        raise KernelError("linear: out must not be x")
     device = weight.device
     needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_STORE)
     held, scratch, counters = _workspace(x, needs, device, _COUNTERS)
     _check(_fn("ssb_fp4_linear")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, o_at, ldo, _CODES[out.dtype], rows, n, k,
-                                 1 if accumulate else 0, scratch, counters, _error_word(device), _stream()), "fp4_linear")
+                                 1 if accumulate else 0, scratch, counters, _error_word(weight), stream), "fp4_linear")
 
 
 def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_scale: Optional[torch.Tensor]) -> Fp4Matrix:
-    rows, x_at, ldx, code, xs_at = _operands(what, x, weight)
+    rows, x_at, ldx, code, xs_at, index = _operands(what, x, weight)
     n, k = weight.shape
     gated = weight.gated
     inter = n // 2 if gated else n
@@ -199,6 +223,7 @@ def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_s
     if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (rows,) or not row_scale.is_contiguous()
                                   or row_scale.get_device() != weight.index):
         raise KernelError(f"{what}: row_scale must be {rows} contiguous float32 values beside the weight")
+    stream = _stream(index, weight.index)
     needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_GATED if gated else _MODE_ACT)
     size, ahead = Fp4Matrix.rows_layout(rows, inter)
     held, scratch, counters = _workspace(x, needs, device, 2 * _COUNTERS, ahead)
@@ -206,9 +231,9 @@ def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_s
     z = Fp4Matrix.over_rows(buffer, rows, inter, size)
     _check(_fn("ssb_fp4_inner")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, z.codes_at, z.scales_at, rows, n, k,
                                 1 if gated else 0, kind, limit, 0 if row_scale is None else row_scale.data_ptr(), scratch, counters,
-                                _error_word(device), _stream()), "fp4_inner")
+                                _error_word(weight), stream), "fp4_inner")
     if counters:
-        z._counters = (held, counters + 4 * _COUNTERS)
+        z._counters = (held, counters + 4 * _COUNTERS, scratch, needs >> 1)
     return z
 
 
@@ -264,7 +289,6 @@ def experts(x: torch.Tensor, expert_of: torch.Tensor, pair_weight: torch.Tensor,
     o_at, ldo = _rows(out, "out", tokens, k)
     if accumulate and out.dtype != torch.float32:
         raise KernelError("experts: results are added in float32 only")
-    _here(x.get_device(), out.get_device(), expert_of.get_device(), pair_weight.get_device(), first.index, down.index)
     device = first.device
     top = expert_of.shape[-1] if expert_of.dim() == 2 else 0
     if top < 1 or expert_of.dtype != torch.int32 or pair_weight.dtype != torch.float32 or expert_of.shape != (tokens, top) \
@@ -273,10 +297,11 @@ def experts(x: torch.Tensor, expert_of: torch.Tensor, pair_weight: torch.Tensor,
                           f"{tuple(expert_of.shape)} and {pair_weight.dtype} {tuple(pair_weight.shape)}")
     if tokens * top > MOST_PAIRS or E > 4096:
         raise KernelError(f"experts: {tokens} tokens of {top} choices among {E} experts are more than {MOST_PAIRS} pairs or 4096 experts")
+    stream = _stream(x.get_device(), out.get_device(), expert_of.get_device(), pair_weight.get_device(), first.index, down.index)
     if tokens == 0:
         return
     scratch = torch.empty(_scratch_size("ssb_fp4_experts_scratch", tokens, top, E, k, inter), dtype=torch.int8, device=device)
     _check(_fn("ssb_fp4_experts")(x_at, ldx, _CODES[x.dtype], expert_of.data_ptr(), pair_weight.data_ptr(), first.codes_at,
                                   first.scales_at, down.codes_at, down.scales_at, o_at, ldo, _CODES[out.dtype],
                                   tokens, top, E, k, inter, 1 if first.gated else 0, kinds[kind], float(limit), 1 if accumulate else 0,
-                                  scratch.data_ptr(), _error_word(device), _stream()), "fp4_experts")
+                                  scratch.data_ptr(), _error_word(first), stream), "fp4_experts")

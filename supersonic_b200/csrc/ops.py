@@ -1784,7 +1784,7 @@ def route_scored(logits: torch.Tensor, n_experts: int, expert_of: torch.Tensor, 
     try:
         args = pack(logits.data_ptr(), logits.stride(0) if T > 1 else shape[1], correction_at, T, n_experts, groups, keep, top, SCORES[scores],
                     1 if group_score == "two" else 0, 1 if renormalize else 0, scale, expert_of.data_ptr(), pair_weight.data_ptr(),
-                    1 if pdl else 0, _stream().value or 0)
+                    1 if pdl else 0, _raw_stream(device) if _raw_stream is not None else _stream().value or 0)
     except StructError as e:
         raise KernelError(f"route_scored: {e}") from None
     _check(call(args), "route_scored")
