@@ -338,22 +338,28 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 // in order with the products and took 0.19 us of a k-block's 0.66 (six of them; 8,192 x 14,336 x 4,096: 266 us); through shared memory
 // by TMA they stand behind the codes that were asked for before them (357 us), and by cp.async a k-block takes these warps 850 clocks.
 //
-// Tiles go in bands of ``group_m`` row tiles, row tiles fastest; of experts (LIST), a list's tile of rows with all its channels.
-constexpr int FL_PAIR_STAGES = 6;
+// Results leave in runs of 128 bytes, which takes the place of a sixth stage of codes (of 64 bytes with six: 8,192 x 14,336 x 4,096 209 us
+// for 206, 2,048 tokens' experts 159 for 151).
+//
+// Tiles go in bands of ``group_m`` row tiles, row tiles fastest; of experts (LIST), a list's tile of rows with all its channels.  Bands of
+// 32 where there are many tiles of channels, of 16 where there are few: 8,192 x 14,336 x 4,096 181 us (by 16 191), 16,384 x 28,672 x 2,048
+// 405 (426); 8,192 x 4,096 x 14,336 187 (179), 32,768 x 4,096 x 4,096 210 (205).
+constexpr int FL_PAIR_STAGES = 5;
 constexpr int FL_PAIR_STAGE_BYTES = 2 * FL_BM * FL_ROW;
 constexpr int FL_PAIR_SETS = 5;           // k-blocks whose scales are in tensor memory
 constexpr int FL_PAIR_AHEAD = 3;          // and in registers, on their way
 constexpr int FL_PAIR_ACC = 128;          // columns from the first accumulator to the second
 constexpr int FL_PAIR_SCALES = 384;       // scales' first column
 constexpr int FL_PAIR_WARPS = 14;         // 0: TMA, 1: MMA + tensor memory, 2-5: scales, 6-13: epilogue
-constexpr int FL_PAIR_PUT = 32 * 20;      // words in which an epilogue warp's rows meet
+constexpr int FL_PAIR_PUT = 32 * 36;      // words in which an epilogue warp's rows meet
 constexpr int FL_PAIR_BARS = 2 * FL_PAIR_STAGES + FL_PAIR_SETS + 3;
+static_assert(FL_PAIR_SETS <= FL_PAIR_STAGES, "a set's last products are told by the stage that they freed, which must not have been freed again");
 constexpr size_t FL_PAIR_SMEM = (size_t)FL_PAIR_STAGES * FL_PAIR_STAGE_BYTES + 8 * FL_PAIR_PUT * 4 + FL_PAIR_BARS * 8 + 24 + 1024;
 
-// tc_put_rows with a place for each row: ``at``, the lane's row of dst.
-template <int WORDS, bool ADD>
+// A lane's 32 words of its row, a warp's rows in runs of 128 bytes through ``stage``; ``at``: the lane's row of dst.
+template <bool ADD>
 __device__ __forceinline__ void fl_put_rows(float* stage, const uint32_t* v, char* dst, size_t row_bytes, int at, int rows) {
-    constexpr int LD = WORDS + 4, PER = WORDS / 4, ROWS = 32 / PER;
+    constexpr int WORDS = 32, LD = WORDS + 4, PER = WORDS / 4, ROWS = 32 / PER;
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int j = 0; j < WORDS; j += 4)
@@ -574,41 +580,35 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     if (lane == 0) fl_arrive_leader(leader_free);
                 }
                 if (rows <= 0) continue;
-                if (MODE == FL_STORE) {
+                if (MODE == FL_STORE && !o.is_f32 && n * BN + g * 64 + 64 <= o.N) {
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) {
+                        const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1]));
+                        packed[e / 2] = *reinterpret_cast<const uint32_t*>(&p);
+                    }
+                    fl_put_rows<false>(stage, packed, (char*)((bf16*)o.out + n * BN + g * 64), (size_t)o.ldo * 2, to, rows);
+                } else if (MODE == FL_STORE) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int col = n * BN + g * 64 + h * 32;
                         if (col >= o.N) continue;
-                        const bool whole = col + 32 <= o.N;
                         if (o.is_f32) {
-                            if (whole) {
+                            if (col + 32 <= o.N) {
                                 char* dst = (char*)((float*)o.out + col);
-#pragma unroll
-                                for (int q = 0; q < 2; ++q) {
-                                    if (o.add) fl_put_rows<16, true>(stage, r[h] + 16 * q, dst + 64 * q, (size_t)o.ldo * 4, to, rows);
-                                    else fl_put_rows<16, false>(stage, r[h] + 16 * q, dst + 64 * q, (size_t)o.ldo * 4, to, rows);
-                                }
+                                if (o.add) fl_put_rows<true>(stage, r[h], dst, (size_t)o.ldo * 4, to, rows);
+                                else fl_put_rows<false>(stage, r[h], dst, (size_t)o.ldo * 4, to, rows);
                             } else if (lane < rows) {
                                 float* dst = (float*)o.out + (size_t)to * o.ldo + col;
 #pragma unroll
                                 for (int e = 0; e < 32; ++e)
                                     if (col + e < o.N) dst[e] = o.add ? dst[e] + __uint_as_float(r[h][e]) : __uint_as_float(r[h][e]);
                             }
-                        } else {
-                            uint32_t packed[16];
+                        } else if (lane < rows) {
+                            bf16* dst = (bf16*)o.out + (size_t)to * o.ldo + col;
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1]));
-                                packed[e / 2] = *reinterpret_cast<const uint32_t*>(&p);
-                            }
-                            if (whole) {
-                                fl_put_rows<16, false>(stage, packed, (char*)((bf16*)o.out + col), (size_t)o.ldo * 2, to, rows);
-                            } else if (lane < rows) {
-                                bf16* dst = (bf16*)o.out + (size_t)to * o.ldo + col;
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (col + e < o.N) dst[e] = __float2bfloat16_rn(__uint_as_float(r[h][e]));
-                            }
+                            for (int e = 0; e < 32; ++e)
+                                if (col + e < o.N) dst[e] = __float2bfloat16_rn(__uint_as_float(r[h][e]));
                         }
                     }
                 } else {
@@ -777,7 +777,7 @@ static int fl_pair(const CUtensorMap& mx, const CUtensorMap& mw, const void* xs,
     const int pairs = (int)std::min<long long>((long long)m_tiles * n_tiles, max_pairs);
     return ssb_launch(kernel, dim3(2 * pairs), dim3(32 * FL_PAIR_WARPS), FL_PAIR_SMEM, stream, true, mx, mw, (const uint8_t*)xs,
                       (const uint8_t*)ws, x_runs, o, list, m_tiles,
-                      n_tiles, f4_k_blocks(K), std::min(16, m_tiles), error_word);
+                      n_tiles, f4_k_blocks(K), std::min(n_tiles >= 32 ? 32 : 16, m_tiles), error_word);
 }
 
 template <int MODE>
