@@ -236,8 +236,8 @@ SSB_API int ssb_route_softmax(float* z, int ld, const float* bias, int n_tokens,
 // chooses in 32 bits and looks whether two neighbours of its order, the last chosen and the next among them, or a kept and a
 // dropped group, are closer than that: only then (a token in a thousand) it computes the groups' scores, or the candidates', in 64
 // bits.  Without correction c grows with z, and the order is z's own.
-// 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: 20 us; instructions bound it (the logits' 8.4 MB
-// take 1.3).  Choosing round by round, a reduction over the warp for the largest and
+// 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: 19 us; 1,400 instructions
+// a token and what they wait for bound it (the logits' 8.4 MB take 1.3).  Choosing round by round, a reduction over the warp for the largest and
 // one for its expert, and with all scores of a close token in 64 bits, it took 34; in that form with the latter in local memory 49.
 // ---------------------------------------------------------------------------------------
 constexpr int RS_MOST_GROUPS = 32;
@@ -375,9 +375,10 @@ __device__ __forceinline__ uint32_t rs_sorted_at(uint32_t key, int place) {
     return __shfl_sync(0xffffffffu, key, place);
 }
 
-// PER: experts a lane (expert j * 32 + lane).
+// PER: experts a lane (expert j * 32 + lane).  Eight blocks an SM where registers allow it: 8,192 tokens of 512 experts 32.6 us (39.6 as they
+// come), of 256 18.6 (19.3; ten blocks 20.8).
 template <int PER>
-__global__ void __launch_bounds__(RG_THREADS)
+__global__ void __launch_bounds__(RG_THREADS, PER <= 16 ? 8 : 1)
 route_scored_kernel(const RsArgs a) {
     // per warp: [n_experts] scores in 64 bits, over them in 32 bits groups' members, or 32 candidates and their order; [top] chosen
     extern __shared__ double rsc_smem[];

@@ -338,6 +338,9 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 // in order with the products and took 0.19 us of a k-block's 0.66 (six of them; 8,192 x 14,336 x 4,096: 266 us); through shared memory
 // by TMA they stand behind the codes that were asked for before them (357 us), and by cp.async a k-block takes these warps 850 clocks.
 //
+// 8,192 x 14,336 x 4,096: 179 us, 5.4 PFLOP/s, the tensor pipe busy 73 % of the cycles.  Bound by codes on their way from L2 (two sides of
+// 256 a tile, some 46 bytes a clock and SM) and by results on theirs (without them 35 us less).
+//
 // Results leave in runs of 128 bytes, which takes the place of a sixth stage of codes (of 64 bytes with six: 8,192 x 14,336 x 4,096 209 us
 // for 206, 2,048 tokens' experts 159 for 151).
 //
@@ -862,8 +865,8 @@ SSB_API int ssb_fp4_inner(const void* x, long long ldx, int dtype, const void* x
 // Pairs (token, choice) by expert, one block.  A warp has a run of neighbouring pairs and counts of its own: it counts them by expert, the
 // counts of the warps before it say where its pairs go, and it places them.  ``slot``: where a pair's row goes among tiles of BN rows
 // (-1: its expert is none), ``order``: the pair of a sorted row.  The order of an expert's pairs inside a warp's run is whatever the adds
-// give; nothing that leaves the call depends on it.  12,288 pairs of 64 experts: 14.7 us (counts that all warps share 16, ranks by
-// match.any 26).
+// give; nothing that leaves the call depends on it.  12,288 pairs of 64 experts: 13 us, steps one
+// after another on one SM (loaded twice and summed by a thread an expert 15; counts that all warps share 16; ranks by match.any 26).
 constexpr int FL_GROUP_WARPS = 32;
 // Words from one warp's counts to the next's: an odd number, so that an expert's counts lie in as many banks.
 __host__ __device__ __forceinline__ int fl_group_stride(int experts, int n_warps) { return n_warps > 1 ? experts | 1 : experts; }
@@ -995,7 +998,8 @@ __device__ __forceinline__ int fl_sort_pairs(const int* __restrict__ expert_of, 
 
 
 // Tiles of up to FL_SORTED_PAIRS pairs beside their rows into 4 bits, in one launch: every block sorts the pairs for itself, and takes
-// k-blocks of rows by its warps (a lane eight numbers, four lanes a block).
+// k-blocks of rows by its warps (a lane eight numbers, four lanes a block).  One token's experts (64 of 2,048 x 1,408, 6 chosen) 17.2 us, by
+// the two launches of many pairs 20.1; 16 tokens' 52.0 and 54.5.
 template <typename T, int BN>
 __global__ void __launch_bounds__(256)
 fp4_place_kernel(const int* __restrict__ expert_of, int pairs, int experts, int top, const T* __restrict__ x, long long ldx, int K, int k_blocks,

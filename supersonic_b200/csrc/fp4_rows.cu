@@ -29,6 +29,11 @@ struct FrStep {
 
 // A unit is 16 V numbers of a row: sixteen lanes of V, 32 / V lanes a block, scales in words of four.  Units run over whole
 // k-blocks; behind a row's end they write scales of zero.  TURNS units are in flight.
+//
+// Instructions bound it where there are many rows (144 for 256 numbers of bfloat16 with V = 8, places and scale bytes more than half of
+// them), so a lane takes sixteen numbers, two units in flight: 8,192 x 4,096 19.9 us (87 MB, 4.4 TB/s; eight numbers, one unit 23.7),
+// 14,336 x 4,096 32 (40).  Few rows are a launch and a dependent fetch or two, on as many SMs as can be: 64 x 2,048 1.5 us (2.0 by sixteen),
+// 512 x 2,048 1.9 (2.1); they cross at about 1,024 x 2,048 (2.6, 2.5).
 template <typename T, int TURNS, int V, bool PAIRS>
 __global__ void __launch_bounds__(FR_THREADS)
 fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int rows, int K,
@@ -103,7 +108,8 @@ fp4_quantize_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict_
     }
 }
 
-// The same units the other way.
+// The way back, units of 128 numbers: 14,336 x 4,096 to bfloat16 30.5 us (149 MB, 4.9 TB/s), with one unit in flight 32; 64 x 2,048 1.26 with
+// one in flight, 1.7 with four.
 template <typename T, int TURNS>
 __global__ void __launch_bounds__(FR_THREADS)
 fp4_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, long long ldo, int rows,
