@@ -109,7 +109,7 @@ def test_quantize_reads_and_values_writes_parts_of_wider_matrices():
 LINEAR = [(1, 8, 32), (1, 2048, 2048), (2, 136, 288), (8, 1000, 4096), (9, 64, 96), (16, 2040, 2080), (4, 8192, 1024),       # few rows
           (16, 4096, 8192), (3, 16384, 512), (17, 264, 544), (32, 1024, 4096), (33, 2048, 2048), (64, 4096, 1024), (65, 128, 256),
           (100, 1536, 4096), (128, 640, 2016), (129, 4096, 256), (200, 2048, 4096), (300, 264, 288), (257, 256, 32), (1000, 1032, 800),
-          (2048, 2048, 512)]
+          (2048, 2048, 512), (70000, 64, 32), (300, 8, 64), (90, 8, 1024), (2, 64, 65536), (1, 40, 32768), (16, 24, 2048), (65, 40, 4096)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
@@ -315,6 +315,63 @@ def test_units_one_after_another_on_two_streams():
         main.wait_stream(side)
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(outs[2], want[0])
+
+
+@pytest.mark.parametrize("rows", [8, 20, 300])
+def test_units_captured_and_replayed_at_the_same_time(rows):
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(12)
+    (first, _), (down, _) = weight(g, 2 * 1536, 2048, gated=True, spread=0.01), weight(g, 2048, 1536)
+    x = randn(g, rows, 2048, dtype=torch.bfloat16)
+
+    def unit(x, out):
+        fp4_ops.linear(fp4_ops.gate_up(x, first), down, out, accumulate=True)
+    graphs = []
+    for _ in range(2):
+        xs, out, graph = x.clone(), torch.zeros((rows, 2048), device=DEV), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            unit(xs, out)
+            unit(xs, out)
+        graphs.append((graph, xs, out, torch.cuda.Stream()))
+    for turn in range(3):
+        wants = []
+        for graph, xs, out, stream in graphs:
+            xs.copy_(randn(g, rows, 2048, dtype=torch.bfloat16))
+            out.zero_()
+            want = torch.zeros_like(out)
+            for _ in range(6):
+                unit(xs, want)
+            wants.append(want)
+        torch.cuda.synchronize()
+        for graph, xs, out, stream in graphs:
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for (_, _, out, _), want in zip(graphs, wants))
+
+
+@pytest.mark.parametrize("rows", [3, 20, 200])
+def test_inner_rows_made_before_a_capture(rows):
+    """The captured product keeps the counters and the scratch that came with the rows; eager ones beside it have their own."""
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(13)
+    (first, _), (down, _) = weight(g, 2 * 4096, 1024, gated=True, spread=0.01), weight(g, 512, 4096)
+    x = randn(g, rows, 1024, dtype=torch.bfloat16)
+    want = torch.empty((rows, 512), device=DEV)
+    fp4_ops.linear(fp4_ops.gate_up(x, first), down, want)
+    z, out, graph = fp4_ops.gate_up(x, first), torch.empty((rows, 512), device=DEV), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        fp4_ops.linear(z, down, out)
+    held = [torch.full((1 << 16,), i, dtype=torch.uint8, device=DEV) for i in range(64)]       # whatever was given back is written over
+    other = torch.empty_like(out)
+    for _ in range(4):
+        out.zero_()
+        graph.replay()
+        fp4_ops.linear(z, down, other)
+        assert torch.equal(out, want) and torch.equal(other, want)
+    assert all(bool((t == i).all()) for i, t in enumerate(held))
 
 
 # ---- experts ----------------------------------------------------------------------------------------------------------
@@ -631,6 +688,33 @@ def test_a_model_in_4_bits_generates_what_it_scores(model_folders, name, dtype):
     assert int(logits[0].argmax()) == got[2][0]
     with pytest.raises(ValueError):
         eng.int8_session(max_tokens=1024)
+
+
+def test_experts_on_two_streams_and_of_other_types():
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(24)
+    (first, fv), (down, dv) = weight(g, 16, 192, 256, gated=True, spread=0.02), weight(g, 16, 256, 96)
+    runs = []
+    for tokens in (6, 200):
+        x, (e, w) = randn(g, tokens, 256), choices(g, tokens, 16, 4)
+        check_experts(x, e, w, first, fv, down, dv, None, torch.bfloat16)
+        want = torch.empty((tokens, 256), device=DEV)
+        fp4_ops.experts(x, e, w, first, down, want)
+        runs.append((x, e, w, want, torch.empty_like(want), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for x, e, w, want, out, stream in runs:
+            with torch.cuda.stream(stream):
+                fp4_ops.experts(x, e, w, first, down, out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, _, _, want, out, _ in runs)
+
+
+def test_the_command_runs_a_model_in_4_bits(capsys):
+    from supersonic_b200.cli import main
+    args = ["--preset", "tiny-a", "--random-seed", "2", "--prompt-ids", "5,17,3", "--max-new-tokens", "4"]
+    assert main(args + ["--weight-format", "mxfp4"]) == 0
+    assert "generated_tokens=4" in "".join(capsys.readouterr())
 
 
 def test_designs_with_experts_load_in_4_bits():
