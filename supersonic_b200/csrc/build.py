@@ -59,7 +59,7 @@ LIBRARIES: Dict[str, Dict[str, List[str]]] = {
     "int8_cache": {"sources": ["int8_cache.cu"], "flags": [], "link": []},
     "int8_attention": {"sources": ["int8_attention.cu", "int8_attention_tc.cu"], "flags": [], "link": []},
     "int8_linear": {"sources": ["int8_linear.cu"], "flags": [], "link": []},
-    "fp4": {"sources": ["fp4_rows.cu", "fp4_few.cu", "fp4_linear.cu"], "flags": [], "link": []},
+    "fp4": {"sources": ["fp4_rows.cu", "fp4_few.cu", "fp4_step.cu", "fp4_linear.cu"], "flags": [], "link": []},
     "random_fill": {"sources": ["random_fill.cu"], "flags": [], "link": []},
     # the host side's native core: no CUDA in it, so it is compiled by the C++ compiler alone
     "host_runtime": {"sources": ["runtime.cpp"], "flags": [], "link": [], "dir": os.path.join(os.path.dirname(_HERE), "host"),

@@ -4,7 +4,7 @@
 // 128 rows x 4 blocks to four columns, in all four lane quarters), where the instructions read them.  Products of codes and their scales
 // are exact; sums are float32 in tensor memory.
 //
-// Two kernels here (and one for up to 16 rows in fp4_few.cu):
+// Two kernels here (and one for up to 16 rows in fp4_few.cu, one for up to 32 in fp4_step.cu):
 //  * where the weights' bytes or the number of tiles is what bounds it: weights on the M side (128 of them a tile), rows of x on the
 //    N side, and the k-blocks of all tiles dealt out over the SMs, in equal parts of tiles or wherever a tile ends; the same for experts,
 //    whose tiles of rows a list in memory names;
@@ -14,6 +14,7 @@
 // step and into 4 bits at once, from the float32 sums.
 #include "fp4_codes.cuh"
 #include "fp4_few.cuh"
+#include "fp4_step.cuh"
 #include "packed_call.cuh"
 #include "fp4_tc.cuh"
 #include <algorithm>
@@ -274,46 +275,8 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
                             if (e < live) ((float*)o.out)[at + (size_t)e * o.ldo] = o.add ? sum[e] + was[e] : sum[e];
                     }
                 } else {
-                    // inner rows: a lane holds one channel of 16 rows, a block of 32 channels is wanted in neighbouring lanes
-                    constexpr int WIDE = MODE == FL_GATED ? 64 : 128, V = WIDE / 8, PER = WIDE / V;     // inner channels a tile, a thread, threads a row
-                    static_assert(CH == FL_INNER_ROWS && CH * PER == 128, "");
-                    const int width = MODE == FL_GATED ? o.N / 2 : o.N, left = rows - c0;
-                    if (MODE == FL_GATED) {
-                        const bool up = lane >= 16;
-                        const int at_ch = quarter * 16 + (lane & 15);
-#pragma unroll
-                        for (int j = 0; j < CH; j += 2) {
-                            if (j >= left) break;
-                            // lanes 0-15 finish row j, lanes 16-31 row j + 1
-                            const float own = up ? sum[j + 1] : sum[j], give = up ? sum[j] : sum[j + 1];
-                            const float got = __shfl_xor_sync(0xffffffffu, give, 16);
-                            float z = ssb_gate_fast(up ? got : own, up ? own : got, o.kind, o.limit);
-                            const int r = c0 + j + (up ? 1 : 0);
-                            if (o.row_scale && r < rows) z *= o.row_scale[m0 + r];
-                            inner[(j + (up ? 1 : 0)) * FL_INNER_LD + at_ch] = z;
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < CH; ++j)
-                            if (j < left) inner[j * FL_INNER_LD + in_tile] = ssb_activate(sum[j], o.kind) * o.limit;
-                    }
-                    fl_meet_four();
-                    const int r = who / PER, piece = who % PER, k = nt * WIDE + piece * V;
-                    if ((who & ~31) / PER < left) {                  // some of this warp's rows are there
-                        float v[V];
-#pragma unroll
-                        for (int e = 0; e < V; e += 4) {
-                            const float4 q = *reinterpret_cast<const float4*>(inner + r * FL_INNER_LD + piece * V + e);
-                            v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
-                        }
-                        const int row = m0 + c0 + r, in_list = LIST ? mt * 128 + c0 + r : row;       // of the codes; a listed tile's scales are 128 rows'
-                        fl_put_inner<V>(v, (uint8_t*)o.out + (size_t)row * o.ldo + k / 2,
-                                        o.scales + f4_scale_at(in_list, k / F4_BLOCK, o.inner_blocks), r < left && k < width);
-                        // behind the last channel: scales of zero up to a whole k-block
-                        if (nt == n_tiles - 1 && r < left && piece == 0)
-                            for (int b = width / F4_BLOCK; b < 8 * o.inner_blocks; ++b) o.scales[f4_scale_at(in_list, b, o.inner_blocks)] = 0;
-                    }
-                    fl_meet_four();
+                    fl_inner_tile<MODE>(sum, inner, quarter, lane, who, c0, m0, LIST ? mt * 128 : m0, rows, nt, n_tiles, o.N, o.kind, o.limit,
+                                        o.row_scale, (uint8_t*)o.out, o.ldo, o.scales, o.inner_blocks);      // a listed tile's scales are 128 rows'
                 }
             }
             tc_fence_before();
@@ -711,27 +674,21 @@ struct FlScratch {
         all = pieces + std::max<size_t>(piece_bytes, 16);
     }
 };
-// The kernel of few rows (its time is for rows that come as numbers; the others' with their launch before it) takes products where there
-// is little to read; where the weights' bytes count, its instructions a weight and a row do too.  Up to 8 rows: 1 x 4,096 x 4,096 5.2 us
-// (8.0 by tiles of 16), 8 rows 7.2 (8.1); 8 x 8,192 x 4,096 10.0 (9.7), 4 x 4,096 x 14,336 15.7 (12.8).  Above: 16 x 4,096 x 2,048 6.6
-// (7.2), 16 x 8,192 x 2,048 8.4 (7.5).  Inner rows are put into 4 bits a block of 32 at a time, which is fewer and longer strips of
-// weights: 8 x 2,048 x 2,048 5.8 (7.1), 16 8.6 (7.6), 8 x 4,096 x 4,096 9.6 (8.3), 1 x 1,024 x 8,192 11.5 (8.0).  They are taken where the
-// product behind them is as well, as its counters come from a launch that quantises.
-constexpr long long FL_FEW_NUMBERS = 32768, FL_FEW_INNER = 16384, FL_FEW_WEIGHTS = 24 << 20, FL_FEW_WEIGHTS_16 = 8 << 20;
+// The kernel of few rows takes products where there is little to read (its time here, and with their rows' launch the other's, by tiles of
+// 16 on clusters): 1 x 2,048 x 2,048 3.5 us (5.2), 8 rows 3.9 (5.4), 16 rows 5.7 (5.9); 1 x 4,096 x 4,096 5.2 (7.2), 8 rows 7.2 (7.2);
+// 1 x 6,144 x 4,096 7.3 (7.9), 8 rows 9.2 (8.0).  Inner rows are put into 4 bits a block of 32 at a time, which is fewer and longer strips
+// of weights: 1 x 2,048 x 2,048 5.1 (5.3), 8 rows 5.8 (5.7), 16 rows 8.6 (6.4); 1 x 4,096 x 4,096 7.0 (7.3); 1 x 1,024 x 8,192 11.5 (8.0).
+constexpr long long FL_FEW_NUMBERS = 32768, FL_FEW_INNER = 16384;
 static bool fl_few(int M, int N, int K, int mode) {
-    if ((long long)N * K > (M <= 8 ? FL_FEW_WEIGHTS : FL_FEW_WEIGHTS_16)) return false;
-    if (mode == FL_STORE) {
-        if ((long long)M * K > FL_FEW_NUMBERS) return false;
-    } else {
-        const int inter = mode == FL_GATED ? N / 2 : N;
-        if (M > 8 || K > 4096 || (long long)M * K > FL_FEW_INNER || (long long)M * inter > FL_FEW_NUMBERS) return false;
-    }
+    if ((long long)N * K > (M <= 4 ? 24 << 20 : M <= 8 ? 16 << 20 : 4 << 20)) return false;
+    if (mode == FL_STORE ? (long long)M * K > FL_FEW_NUMBERS : M > 8 || K > 4096 || (long long)M * K > FL_FEW_INNER) return false;
     return fw_takes(M, N, K, mode);
 }
 
 // Twice the bytes of scratch that a product needs, and one if it needs counters.  numbers: rows come as numbers; mode: FL_*.
 SSB_API long long ssb_fp4_product_scratch(int M, int N, int K, int numbers, int mode) {
     if (M <= 0 || N <= 0 || K <= 0 || fl_few(M, N, K, mode)) return 0;
+    if (fs_parts(M, N, K)) return numbers ? 2 * (long long)FlScratch(M, K, true, 0).all : 0;
     return 2 * (long long)FlScratch(M, K, numbers != 0, fl_plan(M, N, K).pieces).all + 1;
 }
 
@@ -818,20 +775,28 @@ static int fl_product(const void* x, long long ldx, int dtype, const void* xs, c
     if (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws | (uintptr_t)o.out | (uintptr_t)o.scales | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
     if (o.M == 0) return 0;
     const bool few = fl_few(o.M, o.N, K, MODE);
-    if (!error_word || (!few && (!scratch || !counters))) return SSB_ERR_BAD_SIZE;
-    if (few) {
+    const int parts = few ? 0 : fs_parts(o.M, o.N, K);
+    if (!error_word || (!few && dtype >= 0 && !scratch) || (!few && !parts && (!scratch || !counters))) return SSB_ERR_BAD_SIZE;
+    char* base = (char*)scratch;
+    if (few || parts) {
+        if (parts && dtype >= 0) {
+            const FlScratch at(o.M, K, true, 0);
+            const int rc = ssb_fp4_quantize(x, ldx, dtype, base + at.codes, base + at.scales, o.M, K, o.M, 0, nullptr, 0, 1, stream);
+            if (rc) return rc;
+            x = base + at.codes;
+            xs = base + at.scales;
+        }
         FwArgs a{};
         a.w = (const uint8_t*)w; a.ws = (const uint8_t*)ws;
         a.x = x; a.ldx = ldx; a.dtype = dtype; a.xs = (const uint8_t*)xs;
         a.out = o.out; a.out_scales = o.scales; a.ldo = o.ldo; a.is_f32 = o.is_f32; a.add = o.add;
         a.M = o.M; a.N = o.N; a.K = K;
         a.kind = o.kind; a.limit = o.limit; a.row_scale = o.row_scale; a.inner_blocks = o.inner_blocks;
-        return fw_product(a, MODE, stream);
+        return few ? fw_product(a, MODE, stream) : fs_product(a, MODE, parts, error_word, stream);
     }
     const FlPlan p = fl_plan(o.M, o.N, K);
     if (p.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;
     const FlScratch at(o.M, K, dtype >= 0, p.pieces);
-    char* base = (char*)scratch;
     if (dtype >= 0) {
         const int rc = ssb_fp4_quantize(x, ldx, dtype, base + at.codes, base + at.scales, o.M, K, o.M, 0, counters, n_clear, 1, stream);
         if (rc) return rc;

@@ -102,6 +102,53 @@ __device__ __forceinline__ void fl_put_inner(float (&v)[V], uint8_t* dst, uint8_
     }
 }
 
+// Up to 16 rows' sums of a tile of 128 channels (a thread of four warps one channel) become inner rows in 4 bits; all four warps call it.
+// Rows c0, ... of ``rows``; row m0 of the codes and row s0 of the scales are the tile's first.  A block of 32 channels is wanted in
+// neighbouring lanes: they meet in ``inner``.
+template <int MODE>
+__device__ __forceinline__ void fl_inner_tile(const float (&sum)[FL_INNER_ROWS], float* inner, int quarter, int lane, int who, int c0, int m0, int s0,
+                                              int rows, int nt, int n_tiles, int N, int kind, float limit, const float* row_scale,
+                                              uint8_t* codes, long long ld, uint8_t* scales, int inner_blocks) {
+    constexpr int CH = FL_INNER_ROWS, WIDE = MODE == FL_GATED ? 64 : 128, V = WIDE / 8, PER = WIDE / V;     // inner channels a tile, a thread, threads a row
+    static_assert(CH * PER == 128, "");
+    const int width = MODE == FL_GATED ? N / 2 : N, left = rows - c0;
+    if (MODE == FL_GATED) {
+        const bool up = lane >= 16;
+        const int at_ch = quarter * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < CH; j += 2) {
+            if (j >= left) break;
+            // lanes 0-15 finish row j, lanes 16-31 row j + 1
+            const float own = up ? sum[j + 1] : sum[j], give = up ? sum[j] : sum[j + 1];
+            const float got = __shfl_xor_sync(0xffffffffu, give, 16);
+            float z = ssb_gate_fast(up ? got : own, up ? own : got, kind, limit);
+            const int r = c0 + j + (up ? 1 : 0);
+            if (row_scale && r < rows) z *= row_scale[m0 + r];
+            inner[(j + (up ? 1 : 0)) * FL_INNER_LD + at_ch] = z;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+            if (j < left) inner[j * FL_INNER_LD + quarter * 32 + lane] = ssb_activate(sum[j], kind) * limit;
+    }
+    fl_meet_four();
+    const int r = who / PER, piece = who % PER, k = nt * WIDE + piece * V;
+    if ((who & ~31) / PER < left) {                  // some of this warp's rows are there
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(inner + r * FL_INNER_LD + piece * V + e);
+            v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
+        }
+        fl_put_inner<V>(v, codes + (size_t)(m0 + c0 + r) * ld + k / 2, scales + f4_scale_at(s0 + c0 + r, k / F4_BLOCK, inner_blocks),
+                        r < left && k < width);
+        // behind the last channel: scales of zero up to a whole k-block
+        if (nt == n_tiles - 1 && r < left && piece == 0)
+            for (int b = width / F4_BLOCK; b < 8 * inner_blocks; ++b) scales[f4_scale_at(s0 + c0 + r, b, inner_blocks)] = 0;
+    }
+    fl_meet_four();
+}
+
 __device__ __forceinline__ void fl_st8(uint32_t taddr, const uint4& a, const uint4& b) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  ::"r"(taddr), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
