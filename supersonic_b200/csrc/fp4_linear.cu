@@ -628,10 +628,10 @@ struct FlPlan {
 //  * a block of the streaming kernel takes 3.8 + 0.046 a row, and 0.37 a k-block of 128 weight rows whatever its rows; pieces of split
 //    tiles 2.2 and, each, 0.1 + 0.01 a row;
 //  * a pair 6.5, 0.43 a k-block of 256 x 256 and 0.03 for each tile beside it.
-// At 2,048 x 2,048: 48 rows by tiles of 64 that are whole 9.1, in 2 parts 10.7; at 4,096 x 14,336: 1 row whole 25, in 4 parts 12.1, dealt
-// out over all SMs 13.5; 128 rows by 64 in 2 parts 20.7, by 128 in 4 22.2, on pairs 30; at 14,336 x 4,096: 64 rows by 64 14.0, 128 by 128
-// 17.2, on pairs 15.7; 1,024 rows by 128 70, on pairs 35.  Tiles of 16 and 32 rows are only where one holds all rows: the next one's
-// scales would begin between the columns that a product can name.
+// At 2,048 x 2,048: 48 rows by tiles of 64 that are whole 9.1, in 2 parts 10.7; at 4,096 x 14,336: 64 rows by 64 in 2 parts 20.4, in 4 16.7,
+// dealt out over all SMs 20.8; 128 rows by 64 in 2 parts 20.7, by 128 in 4 22.2, on pairs 30; at 14,336 x 4,096: 64 rows by 64 14.0, 128
+// by 128 17.2, on pairs 15.7; 1,024 rows by 128 70, on pairs 35.  Tiles of 16 and 32 rows are only where one holds all rows: the next one's
+// scales would begin between the columns that a product can name (and only where there are more tiles than SMs: else fp4_step.cu).
 static FlPlan fl_plan(int M, int N, int K) {
     const int sms = ssb_sm_count(), k_blocks = f4_k_blocks(K);
     FlPlan best{};

@@ -180,14 +180,17 @@ def test_linear_reads_and_writes_parts_of_wider_matrices(rows):
     assert bool((out[:, :64] == 3).all()) and bool((out[:, 200:] == 3).all())
 
 
-def test_linear_of_no_rows_and_a_weight_just_made():
+@pytest.mark.parametrize("rows", [4, 20, 50, 100])
+@pytest.mark.parametrize("numbers", [True, False])
+def test_linear_of_no_rows_and_a_weight_just_made(rows, numbers):
     from supersonic_b200.csrc import fp4_ops
     from supersonic_b200.weights import Fp4Matrix
     g = gen(8)
-    x, w = randn(g, 4, 2048), torch.randn((2048, 2048), generator=g, device=DEV)
+    x, w = randn(g, rows, 2048), torch.randn((2048, 2048), generator=g, device=DEV)
     fp4_ops.linear(x[:0], rows4(w), torch.empty((0, 2048), device=DEV))
     xv = pf.rounded(x.double())
-    m, out = Fp4Matrix.empty(2048, 2048), torch.empty((4, 2048), device=DEV)
+    x = x if numbers else rows4(x)
+    m, out = Fp4Matrix.empty(2048, 2048), torch.empty((rows, 2048), device=DEV)
     for turn in range(20):                                        # the product is launched behind the kernel that writes its weights
         fresh = w * 2.0 ** turn
         fp4_ops.quantize(fresh, m)
