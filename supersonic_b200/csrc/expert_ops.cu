@@ -256,7 +256,7 @@ __device__ __forceinline__ float rs_logit(float z) {
 }
 // A number's bits in an order that is the numbers'; 0 is below all of them (and NaN's).
 __device__ __forceinline__ uint32_t rs_key(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.f);         // (both zeros are one)
     return x != x ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float rs_from_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }

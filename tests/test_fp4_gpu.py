@@ -527,6 +527,17 @@ def test_route_of_close_and_equal_scores(scores):
 
 
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("n, groups, keep", [(24, 1, 1), (24, 8, 3), (128, 1, 1), (512, 16, 5)])
+def test_route_of_zeros_of_both_signs(n, groups, keep, scores):
+    g = gen(34)
+    logits = torch.randint(-2, 2, (40, n), generator=g, device=DEV).float() * 0.5
+    logits[torch.rand((40, n), generator=g, device=DEV) < 0.4] = -0.0
+    for by in ("max", "two"):
+        check_route(logits, n, 5, None, scores, groups, keep, by)
+        check_route(logits, n, 5, torch.full((n,), -0.0, device=DEV), scores, groups, keep, by)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 def test_route_of_rows_that_are_masked_or_wild(scores):
     g = gen(32)
     inf, nan = float("inf"), float("nan")
