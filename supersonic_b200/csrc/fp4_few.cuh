@@ -1,4 +1,4 @@
-// What the kernel of few rows (fp4_few.cu) is asked for.
+// What the kernels of few rows (fp4_few.cu, fp4_step.cu) are asked for.
 #pragma once
 #include "common.cuh"
 

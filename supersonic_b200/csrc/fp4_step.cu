@@ -15,7 +15,7 @@
 typedef __nv_bfloat16 bf16;
 
 constexpr int FS_STAGES = 5;
-constexpr int FS_MOST_SUMS = 96;          // rows of the other blocks' sums in a cluster's first
+constexpr int FS_MOST_SUMS = 96;          // rows of sums that a cluster's first block gets: three others, 32 each
 
 template <int BN> constexpr int fs_columns() { return fl_power(BN + 16 * FS_STAGES); }
 template <int BN> constexpr int fs_stage() { return FL_BM * FL_ROW + BN * FL_ROW + 2 * (int)FL_CHUNK; }
