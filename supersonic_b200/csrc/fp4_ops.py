@@ -164,26 +164,28 @@ def _operands(what: str, x: Rows, weight: Fp4Matrix):
 
 
 def _workspace(x: Rows, needs: int, device, words: int, ahead: int = 0):
-    """(a buffer, the address of scratch behind its first ``ahead`` bytes, the address of ``words`` counters) of a product that ``needs``
-    so much (ssb_fp4_product_scratch).  Counters are zeroed by the launch that quantises rows; a product of rows in 4 bits takes those
-    that came with them, and the scratch of the launch that made them where it has room, which nobody takes twice, or has its own zeroed."""
+    """(a buffer or None, the address of scratch behind its first ``ahead`` bytes, the address of ``words`` counters) of a product that
+    ``needs`` so much (ssb_fp4_product_scratch).  Counters are zeroed by the launch that quantises rows; a product of rows in 4 bits takes
+    those that came with them, and the scratch of the launch that made them where it has room, which nobody takes twice and which lie in the
+    rows' own buffer, there as long as the rows are; or it has its own zeroed."""
     size, counts = needs >> 1, needs & 1
     if not counts:
         if size + ahead == 0:
             return None, 0, 0
         buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
         return buffer, buffer.data_ptr() + ahead, 0
-    if isinstance(x, Fp4Matrix):
+    own = isinstance(x, Fp4Matrix)
+    if own:
         left, x._counters = x._counters, None
-        if left is not None and words <= _COUNTERS:
-            if ahead == 0 and size <= left[3]:
-                return left, left[2], left[1]
-            buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
-            return (buffer, left), buffer.data_ptr() + ahead, left[1]
-        buffer = torch.empty(ahead + size, dtype=torch.int8, device=device)
-        left = torch.zeros(words, dtype=torch.int32, device=device)
-        return (buffer, left), buffer.data_ptr() + ahead, left.data_ptr()
+        if left is not None and ahead == 0 and words <= _COUNTERS:
+            counters, scratch, room = left
+            if size <= room:
+                return None, scratch, counters
+            buffer = torch.empty(size, dtype=torch.int8, device=device)
+            return buffer, buffer.data_ptr(), counters
     buffer = torch.empty(ahead + 4 * words + size, dtype=torch.int8, device=device)
+    if own:
+        buffer[ahead:ahead + 4 * words].zero_()
     at = buffer.data_ptr() + ahead
     return buffer, at + 4 * words, at
 
@@ -226,14 +228,13 @@ def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_s
     stream = _stream(index, weight.index)
     needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_GATED if gated else _MODE_ACT)
     size, ahead = Fp4Matrix.rows_layout(rows, inter)
-    held, scratch, counters = _workspace(x, needs, device, 2 * _COUNTERS, ahead)
-    buffer = held[0] if type(held) is tuple else held
+    buffer, scratch, counters = _workspace(x, needs, device, 2 * _COUNTERS, ahead)
     z = Fp4Matrix.over_rows(buffer, rows, inter, size)
     _check(_fn("ssb_fp4_inner")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, z.codes_at, z.scales_at, rows, n, k,
                                 1 if gated else 0, kind, limit, 0 if row_scale is None else row_scale.data_ptr(), scratch, counters,
                                 _error_word(weight), stream), "fp4_inner")
     if counters:
-        z._counters = (held, counters + 4 * _COUNTERS, scratch, needs >> 1)
+        z._counters = (counters + 4 * _COUNTERS, scratch, needs >> 1)          # of z's own buffer
     return z
 
 

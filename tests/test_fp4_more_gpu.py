@@ -1,0 +1,67 @@
+"""More of the 4-bit operators on the device: whose memory launches work in, forms that few sizes take, and extremes."""
+import pytest
+import torch
+
+import plain_fp4 as pf
+from test_fp4_gpu import DEV, TYPES, check, check_experts, check_inner, check_route, choices, gen, randn, rows4, weight
+
+pytestmark = pytest.mark.gpu
+
+
+def written_over():
+    """Small and larger tensors, so that whatever was given back to the allocator is written over."""
+    return [torch.full((n,), i % 251, dtype=torch.uint8, device=DEV) for n in (2048, 1 << 16) for i in range(128)]
+
+
+def unchanged(held):
+    return all(bool((t == i % 128 % 251).all()) for i, t in enumerate(held))
+
+
+# ---- whose memory ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("numbers", [True, False])
+@pytest.mark.parametrize("rows", [3, 40, 64, 200, 300])
+def test_a_captured_product_of_rows_made_before(rows, numbers):
+    """Inner rows from rows of either kind; the product that reads them is captured and replayed, whatever is allocated since."""
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(rows)
+    (first, _), (down, dv) = weight(g, 2 * 4096, 1024, gated=True, spread=0.01), weight(g, 512, 4096)
+    x = randn(g, rows, 1024, dtype=torch.bfloat16)
+    x = x if numbers else rows4(x)
+    z, out, graph = fp4_ops.gate_up(x, first), torch.empty((rows, 512), device=DEV), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        fp4_ops.linear(z, down, out)
+    held = written_over()
+    zv = pf.values(z)
+    for _ in range(4):
+        out.fill_(float("nan"))
+        graph.replay()
+        check(out, zv @ dv.t(), pf.sum_slack(zv, dv))
+    assert unchanged(held)
+
+
+@pytest.mark.parametrize("numbers", [True, False])
+@pytest.mark.parametrize("rows", [16, 40, 300])
+def test_inner_rows_read_on_another_stream(rows, numbers):
+    """The second product on another stream, while the first one goes on allocating and writing."""
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(rows + 1)
+    (first, _), (down, _) = weight(g, 2 * 2048, 1024, gated=True, spread=0.01), weight(g, 1024, 2048)
+    x = randn(g, rows, 1024, dtype=torch.bfloat16)
+    x = x if numbers else rows4(x)
+    want, out = torch.empty((rows, 1024), device=DEV), torch.empty((rows, 1024), device=DEV)
+    fp4_ops.linear(fp4_ops.gate_up(x, first), down, want)
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    busy = torch.zeros((1 << 24,), device=DEV)
+    for _ in range(6):
+        z = fp4_ops.gate_up(x, first)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                busy.add_(1.0)                                    # the product waits behind these
+            fp4_ops.linear(z, down, out.fill_(float("nan")))
+        held = written_over()
+        main.wait_stream(side)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and unchanged(held)
+        del z
