@@ -270,7 +270,7 @@ static int fw_launch(const FwArgs& a, int blocks, size_t smem, cudaStream_t stre
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
-    return ssb_launch(kernel, dim3(blocks), dim3(FW_THREADS), smem, stream, true, a);
+    return ssb_launch(kernel, dim3(blocks), dim3(FW_THREADS), smem, stream, a.early != 0, a);
 }
 
 // How a product of M rows by N x K weights runs; slots 0: not by this kernel.

@@ -698,8 +698,8 @@ SSB_API long long ssb_fp4_product_scratch(int M, int N, int K, int numbers, int 
 
 template <int BN, int STAGES, int MODE, bool LIST>
 static int fl_stream(const CUtensorMap& mw, const CUtensorMap& mws, const CUtensorMap& mx, const CUtensorMap& mxs, const FlOut& o,
-                     const FlTiles& list, int m_tiles, int n_tiles, int blocks, int K, int* counters, float* pieces, int* error_word,
-                     cudaStream_t stream) {
+                     const FlTiles& list, int m_tiles, int n_tiles, int blocks, int K, bool early, int* counters, float* pieces,
+                     int* error_word, cudaStream_t stream) {
     constexpr size_t smem = fl_smem<BN, STAGES>();
     static_assert(smem <= 227 * 1024, "");
     static bool configured = false;
@@ -708,7 +708,7 @@ static int fl_stream(const CUtensorMap& mw, const CUtensorMap& mws, const CUtens
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
-    return ssb_launch(fp4_stream_kernel<BN, STAGES, MODE, LIST>, dim3(blocks), dim3(FL_THREADS), smem, stream, true, mw, mws, mx, mxs, o, list,
+    return ssb_launch(fp4_stream_kernel<BN, STAGES, MODE, LIST>, dim3(blocks), dim3(FL_THREADS), smem, stream, early, mw, mws, mx, mxs, o, list,
                       m_tiles, n_tiles, f4_k_blocks(K), counters, pieces, error_word);
 }
 
@@ -745,8 +745,8 @@ static int fl_pair(const CUtensorMap& mx, const CUtensorMap& mw, const void* xs,
 }
 
 template <int MODE>
-static int fl_dense(const void* x, const void* xs, const void* w, const void* ws, const FlOut& o, int K, int* counters, float* pieces,
-                    const FlPlan& p, int* error_word, cudaStream_t stream) {
+static int fl_dense(const void* x, const void* xs, const void* w, const void* ws, const FlOut& o, int K, bool early, int* counters,
+                    float* pieces, const FlPlan& p, int* error_word, cudaStream_t stream) {
     const int k_blocks = f4_k_blocks(K);
     CUtensorMap mw, mws, mx, mxs;
     int rc = fl_map(&mx, x, o.M, K / 2, p.bn ? p.bn : FL_BM);
@@ -756,10 +756,10 @@ static int fl_dense(const void* x, const void* xs, const void* w, const void* ws
     if (rc) return rc;
     const FlTiles none{};
     switch (p.bn) {
-        case 16: return fl_stream<16, 5, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
-        case 32: return fl_stream<32, 9, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
-        case 64: return fl_stream<64, 8, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
-        case 128: return fl_stream<128, 6, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, counters, pieces, error_word, stream);
+        case 16: return fl_stream<16, 5, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, early, counters, pieces, error_word, stream);
+        case 32: return fl_stream<32, 9, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, early, counters, pieces, error_word, stream);
+        case 64: return fl_stream<64, 8, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, early, counters, pieces, error_word, stream);
+        case 128: return fl_stream<128, 6, MODE, false>(mw, mws, mx, mxs, o, none, p.m_tiles, p.n_tiles, p.blocks, K, early, counters, pieces, error_word, stream);
     }
     return fl_pair<MODE, false>(mx, mw, xs, ws, (o.M + 127) / 128, o, none, p.m_tiles, p.n_tiles, K, error_word, stream);
 }
@@ -770,11 +770,13 @@ SSB_API int ssb_fp4_quantize_pairs(const void* x, long long ldx, int dtype, void
                                    const int* slot, int tile_rows, cudaStream_t stream);
 
 // A product of dense weights.  x: rows of dtype (ldx elements apart), which are quantised first, or (dtype -1) codes with the scales xs.
+// settled: the weights were written before the launch in front of this call began; else a product that nothing is quantised for waits for
+// all that is in front of it (behind a launch that quantises rows they are there: that one waited).
 // scratch: ssb_fp4_product_scratch bytes.  counters: FL_COUNTERS words (``n_clear`` of them and behind them are zeroed on the way where x
 // is quantised; else the launch needs them zero); the launch leaves them zero.
 template <int MODE>
 static int fl_product(const void* x, long long ldx, int dtype, const void* xs, const void* w, const void* ws, const FlOut& o, int K,
-                      void* scratch, int* counters, int n_clear, int* error_word, cudaStream_t stream) {
+                      int settled, void* scratch, int* counters, int n_clear, int* error_word, cudaStream_t stream) {
     if (o.M < 0 || o.N <= 0 || K <= 0 || K % F4_BLOCK || o.N % 8 || dtype > SSB_BF16) return SSB_ERR_BAD_SIZE;
     if (((uintptr_t)x | (uintptr_t)xs | (uintptr_t)w | (uintptr_t)ws | (uintptr_t)o.out | (uintptr_t)o.scales | (uintptr_t)scratch) & 15) return SSB_ERR_BAD_SIZE;
     if (o.M == 0) return 0;
@@ -796,6 +798,7 @@ static int fl_product(const void* x, long long ldx, int dtype, const void* xs, c
         a.out = o.out; a.out_scales = o.scales; a.ldo = o.ldo; a.is_f32 = o.is_f32; a.add = o.add;
         a.M = o.M; a.N = o.N; a.K = K;
         a.kind = o.kind; a.limit = o.limit; a.row_scale = o.row_scale; a.inner_blocks = o.inner_blocks;
+        a.early = settled || (parts && dtype >= 0);
         return few ? fw_product(a, MODE, stream) : fs_product(a, MODE, parts, error_word, stream);
     }
     const FlPlan p = fl_plan(o.M, o.N, K);
@@ -807,27 +810,27 @@ static int fl_product(const void* x, long long ldx, int dtype, const void* xs, c
         x = base + at.codes;
         xs = base + at.scales;
     }
-    return fl_dense<MODE>(x, xs, w, ws, o, K, counters, (float*)(base + at.pieces), p, error_word, stream);
+    return fl_dense<MODE>(x, xs, w, ws, o, K, settled || dtype >= 0, counters, (float*)(base + at.pieces), p, error_word, stream);
 }
 
 SSB_API int ssb_fp4_linear(const void* x, long long ldx, int dtype, const void* xs, const void* w, const void* ws, void* out, int ldo,
-                           int out_dtype, int M, int N, int K, int add, void* scratch, int* counters, int* error_word, cudaStream_t stream) {
+                           int out_dtype, int M, int N, int K, int add, int settled, void* scratch, int* counters, int* error_word, cudaStream_t stream) {
     if ((out_dtype != SSB_F32 && out_dtype != SSB_BF16) || (add && out_dtype != SSB_F32)) return SSB_ERR_BAD_DTYPE;
     const FlOut o{out, nullptr, nullptr, nullptr, ldo, out_dtype == SSB_F32, add, M, N, 0, 0.f, 0};
-    return fl_product<FL_STORE>(x, ldx, dtype, xs, w, ws, o, K, scratch, counters, FL_COUNTERS, error_word, stream);
+    return fl_product<FL_STORE>(x, ldx, dtype, xs, w, ws, o, K, settled, scratch, counters, FL_COUNTERS, error_word, stream);
 }
 
 // The inner rows of a feed-forward in 4 bits.  gated: w holds 16 gate rows and their 16 up rows in turn, N = 2 x inner channels, kind and
 // limit as ssb_gate's; else kind as ssb_activate's and limit a factor.  counters: as above, and as many behind them for the product that
 // reads the inner rows.
 SSB_API int ssb_fp4_inner(const void* x, long long ldx, int dtype, const void* xs, const void* w, const void* ws, void* codes, void* scales,
-                          int M, int N, int K, int gated, int kind, float limit, const float* row_scale, void* scratch, int* counters,
-                          int* error_word, cudaStream_t stream) {
+                          int M, int N, int K, int gated, int kind, float limit, const float* row_scale, int settled, void* scratch,
+                          int* counters, int* error_word, cudaStream_t stream) {
     const int inner = gated ? N / 2 : N;
     if (inner % F4_BLOCK || (gated && N % 2) || kind < 0 || kind > 2 || (row_scale && !gated)) return SSB_ERR_BAD_SIZE;
     const FlOut o{codes, (uint8_t*)scales, nullptr, row_scale, inner / 2, 0, 0, M, N, kind, limit, f4_k_blocks(inner)};
-    return gated ? fl_product<FL_GATED>(x, ldx, dtype, xs, w, ws, o, K, scratch, counters, 2 * FL_COUNTERS, error_word, stream)
-                 : fl_product<FL_ACT>(x, ldx, dtype, xs, w, ws, o, K, scratch, counters, 2 * FL_COUNTERS, error_word, stream);
+    return gated ? fl_product<FL_GATED>(x, ldx, dtype, xs, w, ws, o, K, settled, scratch, counters, 2 * FL_COUNTERS, error_word, stream)
+                 : fl_product<FL_ACT>(x, ldx, dtype, xs, w, ws, o, K, settled, scratch, counters, 2 * FL_COUNTERS, error_word, stream);
 }
 
 // ---- experts ----------------------------------------------------------------------------------------------------------
@@ -1119,9 +1122,9 @@ static int fl_listed(const void* x, const void* xs, const void* w, const void* w
     if (!rc) rc = fl_scale_map(&mws, ws, (long long)experts * n_tiles * k_blocks);
     if (rc) return rc;
     if (at.bn == 16)
-        return fl_stream<16, 5, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+        return fl_stream<16, 5, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, true, counters, pieces, error_word, stream);
     if (at.bn == 64)
-        return fl_stream<64, 8, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, counters, pieces, error_word, stream);
+        return fl_stream<64, 8, MODE, true>(mw, mws, mx, mxs, o, list, 0, n_tiles, at.blocks, K, true, counters, pieces, error_word, stream);
     return fl_pair<MODE, true>(mx, mw, xs, ws, 2 * at.tiles, o, list, at.tiles, (o.N + 255) / 256, K, error_word, stream);
 }
 

@@ -30,8 +30,8 @@ _P, _I, _F, _L = c_void_p, c_int, c_float, c_longlong
 _SIGNATURES = {
     "ssb_fp4_quantize": [_P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _P],
     "ssb_fp4_values": [_P, _P, _P, _L, _I, _I, _I, _I, _I, _P],
-    "ssb_fp4_linear": [_P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P],
-    "ssb_fp4_inner": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P],
+    "ssb_fp4_linear": [_P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P],
+    "ssb_fp4_inner": [_P, _L, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _I, _P, _P, _P, _P],
     "ssb_fp4_experts": [_P, _L, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P],
     "ssb_fp4_product_scratch": [_I] * 5,
     "ssb_fp4_experts_scratch": [_I] * 5,
@@ -126,6 +126,7 @@ def quantize(x: torch.Tensor, matrix: Fp4Matrix) -> None:
     """``matrix`` gets the numbers of ``x`` (float32 or bfloat16, of its shape; of a gated matrix the gate rows, then the up rows)."""
     at, ld, rows, code = _matrix_rows(x, "x", matrix)
     n, k = matrix.shape[-2:]
+    matrix.written()
     _check(_fn("ssb_fp4_quantize")(at, ld, code, matrix.codes_at, matrix.scales_at, rows, k, n,
                                    n // 2 if matrix.gated else 0, 0, 0, 0, _stream(matrix.index)), "fp4_quantize")
 
@@ -209,7 +210,8 @@ def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = Fal
     needs = _scratch_size("ssb_fp4_product_scratch", rows, n, k, code >= 0, _MODE_STORE)
     held, scratch, counters = _workspace(x, needs, device, _COUNTERS)
     _check(_fn("ssb_fp4_linear")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, o_at, ldo, _CODES[out.dtype], rows, n, k,
-                                 1 if accumulate else 0, scratch, counters, _error_word(weight), stream), "fp4_linear")
+                                 1 if accumulate else 0, 1 if weight.reads_ahead(stream) else 0, scratch, counters, _error_word(weight),
+                                 stream), "fp4_linear")
 
 
 def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_scale: Optional[torch.Tensor]) -> Fp4Matrix:
@@ -231,8 +233,8 @@ def _inner(what: str, x: Rows, weight: Fp4Matrix, kind: int, limit: float, row_s
     buffer, scratch, counters = _workspace(x, needs, device, 2 * _COUNTERS, ahead)
     z = Fp4Matrix.over_rows(buffer, rows, inter, size)
     _check(_fn("ssb_fp4_inner")(x_at, ldx, code, xs_at, weight.codes_at, weight.scales_at, z.codes_at, z.scales_at, rows, n, k,
-                                1 if gated else 0, kind, limit, 0 if row_scale is None else row_scale.data_ptr(), scratch, counters,
-                                _error_word(weight), stream), "fp4_inner")
+                                1 if gated else 0, kind, limit, 0 if row_scale is None else row_scale.data_ptr(),
+                                1 if weight.reads_ahead(stream) else 0, scratch, counters, _error_word(weight), stream), "fp4_inner")
     if counters:
         z._counters = (counters + 4 * _COUNTERS, scratch, needs >> 1)          # of z's own buffer
     return z

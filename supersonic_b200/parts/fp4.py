@@ -18,4 +18,4 @@ def fp4_of(weight, gated: bool = False) -> Fp4Matrix:
     from ..csrc import fp4_ops
     out = Fp4Matrix.empty(*weight.shape, device=weight.device, gated=gated)
     fp4_ops.quantize(weight, out)
-    return out
+    return out.settle()

@@ -22,7 +22,8 @@ _RUN_ROWS, _RUN_BLOCKS = 128, 8
 class Fp4Matrix:
     """``shape`` is that of the numbers: (n, k), or (experts, n, k)."""
 
-    __slots__ = ("_codes", "_scales", "shape", "gated", "device", "index", "codes_at", "scales_at", "_buffer", "_counters")
+    __slots__ = ("_codes", "_scales", "shape", "gated", "device", "index", "codes_at", "scales_at", "_buffer", "_counters",
+                 "_writes", "_known", "_streams", "_captured", "_settled")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, gated: bool = False):
         shape = tuple(int(s) for s in shape)
@@ -37,6 +38,7 @@ class Fp4Matrix:
         if scales.dtype != torch.uint8 or tuple(scales.shape) != (runs, 1024) or not scales.is_contiguous() or scales.device != codes.device:
             raise ValueError(f"scales must be contiguous uint8 {(runs, 1024)} beside the codes, are {scales.dtype} {tuple(scales.shape)}")
         self._codes, self._scales, self.shape, self.gated, self._buffer, self._counters = codes, scales, shape, gated, None, None
+        self._writes, self._known, self._settled = [0], None, None
         # where they are, for the kernels: the tensors stay what they are as long as the matrix lives
         self.device, self.index, self.codes_at, self.scales_at = codes.device, codes.get_device(), codes.data_ptr(), scales.data_ptr()
         if (self.codes_at | self.scales_at) % 16:
@@ -78,7 +80,49 @@ class Fp4Matrix:
         runs = -(-n // _RUN_ROWS) * -(-self.shape[1] // (FP4_BLOCK * _RUN_BLOCKS))
         m = Fp4Matrix(self.codes[:n], self.scales[:runs], (n, self.shape[1]))
         m._buffer = self._buffer
+        m._writes, m._settled = self._writes, self._settled
         return m
+
+    # A product may fetch its weights while the launch in front of it still runs, and such a launch sees for certain only what was written
+    # before the launch in front of that one ended.  So the first product on a stream behind a write is launched behind everything; the
+    # stream's next ones may read ahead.  Writes are counted: this package's (``written``), torch's by the tensors' versions.
+    def written(self) -> None:
+        """Said by whoever writes codes or scales other than through torch (``fp4_ops.quantize`` does)."""
+        self._writes[0] += 1
+
+    def _version(self):
+        try:
+            return self._writes[0] + self._codes._version + self._scales._version
+        except RuntimeError:                                   # tensors of inference mode count no versions
+            return None
+
+    def reads_ahead(self, stream: int) -> bool:
+        """Whether a product on this stream (its handle, the current one) may read the matrix ahead of its turn; that it is launched now
+        is noted."""
+        version = self._version()
+        if version is None:                                    # what torch writes is not seen: only what was settled, and not written by a kernel since
+            return self._settled == ("writes", self._writes[0])
+        if version == self._settled:
+            return True
+        if version != self._known:
+            self._known, self._streams, self._captured = version, set(), set()
+        if stream in self._streams:
+            return True
+        # a captured launch orders nothing that runs outside its graph
+        seen = self._captured if torch.cuda.is_current_stream_capturing() else self._streams
+        if stream in seen:
+            return True
+        seen.add(stream)
+        return False
+
+    def settle(self) -> "Fp4Matrix":
+        """Waits for the device, after which products on any stream may read the matrix ahead, until it is written again.  (Of tensors made
+        in inference mode: until ``written`` is said.)"""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+        version = self._version()
+        self._settled = ("writes", self._writes[0]) if version is None else version
+        return self
 
     def plain_scales(self) -> torch.Tensor:
         """The scales in rows, uint8 ``[.., n, k / 32]`` (rows in the order that the codes have)."""
@@ -99,6 +143,7 @@ class Fp4Matrix:
         """A step's rows [n, k] at the start of an int8 ``buffer``: ``codes`` bytes of codes, then scales (:meth:`rows_layout`)."""
         m = cls.__new__(cls)
         m._codes = m._scales = m._counters = None          # made when somebody asks for them
+        m._writes, m._known, m._settled = [0], None, None
         m.shape, m.gated, m._buffer, m.device, m.index = (n, k), False, buffer, buffer.device, buffer.get_device()
         m.codes_at = buffer.data_ptr()
         m.scales_at = m.codes_at + codes

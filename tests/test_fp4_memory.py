@@ -9,9 +9,7 @@ COUNTERS = 4 * 256                                                # bytes that a
 
 
 def matrix(*shape, gated=False):
-    m = Fp4Matrix.empty(*shape, device="cpu", gated=gated)
-    m.index = 0
-    return m
+    return Fp4Matrix.empty(*shape, device="cpu", gated=gated)
 
 
 @pytest.fixture
@@ -25,6 +23,7 @@ def launches(monkeypatch):
     monkeypatch.setattr(fp4_ops, "_stream", lambda *indices: 0)
     monkeypatch.setattr(fp4_ops, "_error_word", lambda m: 0)
     monkeypatch.setattr(fp4_ops, "_scratch_size", lambda name, *sizes: 2 * 4096 + 1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return made
 
 
@@ -56,3 +55,78 @@ def test_scratch_without_room_is_the_second_products_own(launches, monkeypatch):
     fp4_ops.linear(z, matrix(64, 64), torch.zeros((40, 64)))
     *_, scratch, counters, _, _ = launches[-1][1]
     assert inside(counters, COUNTERS, z._buffer) and not inside(scratch, 1, z._buffer)
+
+
+# ---- weights that were just written: a product may read them ahead of its turn only behind another one on its stream ----------
+AHEAD = -5                                                        # where a product's arguments say that it may
+
+
+def product(launches, w, x=None):
+    fp4_ops.linear(torch.zeros((3, 64)) if x is None else x, w, torch.zeros((3, w.shape[0])))
+    return launches[-1][1][AHEAD]
+
+
+@pytest.mark.parametrize("write", [
+    lambda m: fp4_ops.quantize(torch.zeros((64, 64)), m), lambda m: m.codes.fill_(3), lambda m: m.scales[0].fill_(120),
+    lambda m: m.codes[3:5].copy_(torch.ones((2, 32), dtype=torch.uint8)), lambda m: m.first_rows(16).codes.zero_(),
+    lambda m: fp4_ops.quantize(torch.zeros((16, 64)), m.first_rows(16)), lambda m: m.written(),
+])
+def test_the_first_product_behind_a_write_waits_for_it(launches, write):
+    m = matrix(64, 64)
+    assert [product(launches, m) for _ in range(3)] == [0, 1, 1]
+    write(m)
+    assert [product(launches, m) for _ in range(3)] == [0, 1, 1]
+    m.settle()
+    assert product(launches, m) == 1
+    write(m)
+    assert [product(launches, m) for _ in range(2)] == [0, 1]
+
+
+def test_every_stream_has_a_first_product(launches, monkeypatch):
+    m, at = matrix(64, 64), 0
+    monkeypatch.setattr(fp4_ops, "_stream", lambda *indices: at)
+    seen = []
+    for at in (7, 7, 9, 7, 9):
+        seen.append(product(launches, m))
+    assert seen == [0, 1, 0, 1, 1]
+
+
+def test_a_captured_product_orders_nothing_outside_its_graph(launches, monkeypatch):
+    m, capturing = matrix(64, 64), True
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    assert [product(launches, m) for _ in range(2)] == [0, 1]
+    capturing = False
+    assert [product(launches, m) for _ in range(2)] == [0, 1]
+    capturing = True
+    assert product(launches, m) == 1                              # written before the capture
+
+
+def test_tensors_of_inference_mode_are_read_ahead_when_settled(launches):
+    with torch.inference_mode():
+        m = matrix(64, 64)
+        assert [product(launches, m) for _ in range(2)] == [0, 0]
+        m.settle()
+        assert product(launches, m) == 1
+        fp4_ops.quantize(torch.zeros((64, 64)), m)
+        assert [product(launches, m) for _ in range(2)] == [0, 0]
+    assert [product(launches, m) for _ in range(2)] == [0, 0]
+
+
+def test_units_look_at_both_matrices_and_views_are_matrices_too(launches):
+    first, down = matrix(128, 64, gated=True), matrix(64, 64).settle()
+    z = fp4_ops.gate_up(torch.zeros((3, 64)), first)
+    assert launches[-1][1][AHEAD] == 0
+    assert product(launches, down, z) == 1
+    fp4_ops.gate_up(torch.zeros((3, 64)), first)
+    assert launches[-1][1][AHEAD] == 1
+    view = down.first_rows(16)
+    assert product(launches, view) == 1
+    down.written()
+    assert [product(launches, view) for _ in range(2)] == [0, 1]
+    assert product(launches, down) == 0
+
+
+def test_the_parts_matrices_are_settled(launches):
+    from supersonic_b200.parts.fp4 import fp4_of
+    w = fp4_of(torch.zeros((64, 64)))
+    assert w.reads_ahead(0) and w.reads_ahead(5) and not matrix(64, 64).reads_ahead(0)

@@ -65,3 +65,30 @@ def test_inner_rows_read_on_another_stream(rows, numbers):
         torch.cuda.synchronize()
         assert torch.equal(out, want) and unchanged(held)
         del z
+
+
+# ---- weights that were just written ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows, n, k", [(1, 2048, 2048), (12, 1024, 4096), (40, 2048, 1024), (300, 1024, 512), (4, 19000, 256)])
+@pytest.mark.parametrize("numbers", [True, False])
+def test_products_behind_writes_of_every_kind(rows, n, k, numbers):
+    """Codes copied by torch, a matrix made of parts on the spot, a view of one that was quantised: the next launch is the product."""
+    from supersonic_b200.csrc import fp4_ops
+    from supersonic_b200.weights import Fp4Matrix
+    g = gen(rows + n)
+    x = randn(g, rows, k)
+    sources = [rows4(torch.randn((n, k), generator=g, device=DEV) * 2.0 ** i) for i in range(3)]
+    xv, x = pf.rounded(x.double()), x if numbers else rows4(x)
+    wants = [(xv @ pf.values(m).t(), pf.sum_slack(xv, pf.values(m))) for m in sources]
+    plain = [(m.codes.clone(), m.plain_scales()) for m in sources]
+    m, out, some = Fp4Matrix.empty(n, k), torch.empty((rows, n), device=DEV), n // 16 * 8
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for source, parts, (want, slack) in zip(sources, plain, wants):
+            m.scales.copy_(source.scales)
+            m.codes.copy_(source.codes)
+            fp4_ops.linear(x, m, out)
+            check(out, want, slack)
+            fp4_ops.linear(x, Fp4Matrix.from_parts(*parts), out.zero_())
+            check(out, want, slack)
+            fp4_ops.linear(x, m.first_rows(some), out[:, :some].zero_())
+            check(out, want, slack)
