@@ -45,6 +45,11 @@ __device__ __forceinline__ void fw_cp4(uint32_t dst, const void* src, bool live)
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
 
+// Sums are held times 2^-11, which a row's scales bring in and the tile's end takes out: a block's products (up to 1,152, multiples of 0.25)
+// times its row's scale are exact then for every scale from 2^-127 to 2^127, and what is too large is so as a whole.  (A sum below 2^-115 has
+// float32's smallest steps times 2^11.  The smaller of the two scales first, 1 x 4,096 x 4,096: 5.65 us for 5.12; a look at each step's
+// scales 5.38.)
+constexpr float FW_HELD = 4.8828125e-4f, FW_WHOLE = 2048.f;
 // A row's codes in shared memory, 16 bytes more than whole k-blocks apart: eight rows' pieces meet no bank twice.
 __host__ __device__ constexpr int fw_row_bytes(int k_blocks) { return k_blocks * 128 + 16; }
 
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
                     const int r = u / words, i = u - r * words;
                     const uint32_t w = *reinterpret_cast<const uint32_t*>(a.xs + f4_scale_at(r, 4 * i, a.k_blocks));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sx_s[(4 * i + j) * ROWS + r] = f4_scale(w >> (8 * j) & 255);
+                    for (int j = 0; j < 4; ++j) sx_s[(4 * i + j) * ROWS + r] = f4_scale(w >> (8 * j) & 255) * FW_HELD;
                 }
             } else {
                 // eight numbers a thread and turn, four neighbouring threads a block of 32; behind K zeros
@@ -157,7 +162,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
                         const int byte = f4_scale_byte(most);
                         if (u < units) {
                             *reinterpret_cast<uint32_t*>(x_s + r * row_bytes + i * 4) = f4_encode8(v[j], f4_inverse(byte));
-                            if ((i & 3) == 0) sx_s[(i >> 2) * ROWS + r] = f4_scale(byte);
+                            if ((i & 3) == 0) sx_s[(i >> 2) * ROWS + r] = f4_scale(byte) * FW_HELD;
                         }
                     }
                 }
@@ -197,10 +202,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
                     const float2 sx = *reinterpret_cast<const float2*>(sx_s + (blk0 + b) * ROWS + 8 * nb + 2 * t4);
                     float d[4];
                     fw_mma(d, lo, hi, x);
-                    sum[nb][0] = fmaf(d[0] * c_lo, sx.x, sum[nb][0]);
-                    sum[nb][1] = fmaf(d[1] * c_lo, sx.y, sum[nb][1]);
-                    sum[nb][2] = fmaf(d[2] * c_hi, sx.x, sum[nb][2]);
-                    sum[nb][3] = fmaf(d[3] * c_hi, sx.y, sum[nb][3]);
+                    sum[nb][0] = fmaf(d[0] * sx.x, c_lo, sum[nb][0]);
+                    sum[nb][1] = fmaf(d[1] * sx.y, c_lo, sum[nb][1]);
+                    sum[nb][2] = fmaf(d[2] * sx.x, c_hi, sum[nb][2]);
+                    sum[nb][3] = fmaf(d[3] * sx.y, c_hi, sum[nb][3]);
                 }
             }
             __syncwarp();                                            // the slot has been read
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fp4_few_kernel(const FwArgs a) 
         auto total = [&](int r, int ch) {
             float s = 0.f;
             for (int k = 0; k < a.k_warps; ++k) s += parts[(k * ROWS + r) * LD + ch];
-            return s;
+            return s * FW_WHOLE;
         };
         if (MODE == FW_STORE) {
             for (int i = tid; i < rows * CH; i += FW_THREADS) {

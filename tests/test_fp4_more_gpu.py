@@ -92,3 +92,35 @@ def test_products_behind_writes_of_every_kind(rows, n, k, numbers):
             check(out, want, slack)
             fp4_ops.linear(x, m.first_rows(some), out[:, :some].zero_())
             check(out, want, slack)
+
+
+# ---- scales at the ends of their range ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("numbers", [True, False])
+@pytest.mark.parametrize("rows, n, k", [(1, 136, 512), (8, 136, 512), (12, 136, 512), (12, 136, 4096), (30, 264, 512), (40, 264, 512), (100, 136, 512),
+                                        (300, 264, 512), (3, 19000, 512), (24, 19000, 512)])
+def test_products_of_scales_at_the_ends(rows, n, k, numbers):
+    """Weight scales from 2^-126 to 2^125 against rows of the opposite ones, so that a product of codes with one of its scales alone would leave
+    float32 (1,152 2^125) while the whole is of ordinary size; beside them blocks whose products are too small for it."""
+    from supersonic_b200.csrc import fp4_ops
+    from supersonic_b200.weights import Fp4Matrix
+    g = gen(rows + k)
+
+    def ints(low, high, *shape):
+        return torch.randint(low, high, shape, generator=g, device=DEV)
+    blocks = k // 32
+    ends = torch.tensor([1, 250, 60, 190, 2, 252, 127, 5, 240, 10], device=DEV)[torch.arange(blocks, device=DEV) % 10]
+    other = (254 - ends).clamp(2, 252)
+    other[6] = ends[6] = 1                                        # 2^-252 times codes
+    jitter = lambda t, c: (t + ints(-3, 4, c, blocks)).clamp(0, 252).to(torch.uint8)
+    wm = Fp4Matrix.from_parts(ints(0, 256, n, k // 2).to(torch.uint8), jitter(ends, n))
+    xm = Fp4Matrix.from_parts(ints(0, 256, rows, k // 2).to(torch.uint8), jitter(other, rows))
+    if numbers:
+        x = torch.empty((rows, k), device=DEV)
+        fp4_ops.values(xm, x)
+        xv = pf.rounded(x.double())                               # (a block whose largest code is below 4 gets a smaller scale)
+    else:
+        x, xv = xm, pf.values(xm)
+    wv = pf.values(wm)
+    out = torch.empty((rows, n), device=DEV)
+    fp4_ops.linear(x, wm, out)
+    check(out, xv @ wv.t(), pf.sum_slack(xv, wv))
