@@ -836,13 +836,17 @@ SSB_API int ssb_fp4_inner(const void* x, long long ldx, int dtype, const void* x
 // ---- experts ----------------------------------------------------------------------------------------------------------
 // Pairs (token, choice) by expert, one block.  A warp has a run of neighbouring pairs and counts of its own: it counts them by expert, the
 // counts of the warps before it say where its pairs go, and it places them.  ``slot``: where a pair's row goes among tiles of BN rows
-// (-1: its expert is none), ``order``: the pair of a sorted row.  The order of an expert's pairs inside a warp's run is whatever the adds
-// give; nothing that leaves the call depends on it.  12,288 pairs of 64 experts: 13 us, steps one
-// after another on one SM (loaded twice and summed by a thread an expert 15; counts that all warps share 16; ranks by match.any 26).
+// (-1: its expert is none), ``order``: the pair of a sorted row.  RANKED: an expert's pairs keep their order.  Which of its tiles a pair is in
+// may then decide where its sums are cut, so lists whose tiles are cut are ranked; where every tile is whole (on SM pairs) the order inside a
+// warp's run is whatever the adds give, and nothing that leaves the call depends on it.  12,288 pairs of 64 experts: 13 us, steps one
+// after another on one SM (loaded twice and summed by a thread an expert 15; counts that all warps share 16; ranks by match.any 26).  Ranked, a call for 700 tokens with 3 of 256 experts takes 54.9 us for 53.4, for 85
+// with 6 of 64 37.5 as before: by ballots over the bits of an expert's number, and no further than the run goes (every unrolled turn that is
+// passed over is instructions to be fetched, 2 us in all).
 constexpr int FL_GROUP_WARPS = 32;
 // Words from one warp's counts to the next's: an odd number, so that an expert's counts lie in as many banks.
 __host__ __device__ __forceinline__ int fl_group_stride(int experts, int n_warps) { return n_warps > 1 ? experts | 1 : experts; }
 
+template <bool RANKED>
 __global__ void __launch_bounds__(32 * FL_GROUP_WARPS)
 fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int bn, int* __restrict__ offsets, int* __restrict__ order,
                  int* __restrict__ slot, int* __restrict__ tile_expert, int* __restrict__ tile_row0, int* __restrict__ meta,
@@ -912,14 +916,32 @@ fp4_group_kernel(const int* __restrict__ expert_of, int pairs, int experts, int 
             tile_expert[t] = e;
             tile_row0[t] = row0[e] + (t - tile0[e]) * bn;
         }
+    const int bits = 32 - __clz(experts - 1);
     for (int p0 = lo; p0 < hi; p0 += 32 * AHEAD) {
         if (run > 32 * AHEAD) load(p0);
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
+            if (RANKED && p0 + 32 * q >= hi) break;
             const int e = es[q], p = p0 + 32 * q + lane;
-            int to = -1;
+            int to = -1, i = 0;
+            if (RANKED) {                                          // the first lane of each expert counts for all of them
+                uint32_t same = __ballot_sync(0xffffffffu, e >= 0);          // the lanes of this one's expert, bit by bit of its number
+                for (int b = 0; b < bits; ++b) {
+                    const bool set = e >> b & 1;
+                    const uint32_t all = __ballot_sync(0xffffffffu, set);
+                    same &= set ? all : ~all;
+                }
+                const int first = e >= 0 ? __ffs(same) - 1 : lane;
+                if (lane == first && e >= 0) {
+                    i = mine[e];
+                    mine[e] = i + __popc(same);
+                }
+                i = __shfl_sync(0xffffffffu, i, first) + __popc(same & ((1u << lane) - 1));
+                __syncwarp();
+            } else if (e >= 0) {
+                i = atomicAdd(mine + e, 1);
+            }
             if (e >= 0) {
-                const int i = atomicAdd(mine + e, 1);
                 to = tile0[e] * bn + i;                            // an expert's tiles are neighbours
                 order[row0[e] + i] = p;
             }
@@ -1156,7 +1178,7 @@ SSB_API int ssb_fp4_experts(const void* x, long long ldx, int dtype, const int* 
     } else {
         // as many warps as shared memory has room for their counts
         const int n_warps = std::max(1, std::min(FL_GROUP_WARPS, 48 * 1024 / (4 * (experts | 1)) - 2));
-        rc = ssb_launch(fp4_group_kernel, dim3(1), dim3(32 * FL_GROUP_WARPS), (size_t)fl_group_stride(experts, n_warps) * (n_warps + 2) * 4, stream, true, expert_of, pairs,
+        rc = ssb_launch(at.bn < 256 ? fp4_group_kernel<true> : fp4_group_kernel<false>, dim3(1), dim3(32 * FL_GROUP_WARPS), (size_t)fl_group_stride(experts, n_warps) * (n_warps + 2) * 4, stream, true, expert_of, pairs,
                         experts, at.bn, ints(at.offsets), ints(at.order), ints(at.slot), ints(at.tile_expert), ints(at.tile_row0), ints(at.meta),
                         ints(at.counters), 2 * FL_COUNTERS, n_warps);
         if (!rc) rc = ssb_fp4_quantize_pairs(x, ldx, dtype, base + at.x, base + at.xs, tokens, top, K, ints(at.slot), at.bn, stream);

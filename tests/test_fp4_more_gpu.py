@@ -124,3 +124,22 @@ def test_products_of_scales_at_the_ends(rows, n, k, numbers):
     out = torch.empty((rows, n), device=DEV)
     fp4_ops.linear(x, wm, out)
     check(out, xv @ wv.t(), pf.sum_slack(xv, wv))
+
+
+# ---- experts: many tiles, cut wherever a block's share ends ----------------------------------------------------------------------
+@pytest.mark.parametrize("tokens, k, inter, experts, top", [(85, 1024, 480, 64, 6), (700, 512, 288, 256, 3), (600, 288, 96, 40, 1), (150, 4096, 4096, 4, 1)])
+def test_experts_in_cut_tiles_have_the_same_bits_in_every_run(tokens, k, inter, experts, top):
+    """More tiles than blocks, popular experts with several of them, more pairs than one block sorts for itself."""
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(tokens)
+    x = randn(g, tokens, k, dtype=torch.bfloat16)
+    (first, fv), (down, dv) = weight(g, experts, 2 * inter, k, gated=True, spread=0.02), weight(g, experts, k, inter)
+    e, w = choices(g, tokens, experts, top)
+    out = check_experts(x, e, w, first, fv, down, dv, None, torch.float32)
+    again = torch.empty_like(out)
+    for _ in range(20):
+        fp4_ops.experts(x, e, w, first, down, again)
+        assert torch.equal(again, out)
+    # the tokens in another order are other tiles
+    order = torch.randperm(tokens, generator=g, device=DEV)
+    check_experts(x[order], e[order].contiguous(), w[order].contiguous(), first, fv, down, dv, None, torch.float32)
