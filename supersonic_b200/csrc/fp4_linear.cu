@@ -1128,7 +1128,7 @@ struct FlExperts {
         all = at;
     }
 };
-SSB_API long long ssb_fp4_experts_scratch(int tokens, int top, int experts, int K, int inter, int gated) {
+SSB_API long long ssb_fp4_experts_scratch(int tokens, int top, int experts, int K, int inter) {
     if (tokens <= 0 || top <= 0 || experts <= 0 || K <= 0 || inter <= 0) return 0;
     return (long long)FlExperts(tokens, top, experts, K, inter).all;
 }

@@ -130,3 +130,24 @@ def test_the_parts_matrices_are_settled(launches):
     from supersonic_b200.parts.fp4 import fp4_of
     w = fp4_of(torch.zeros((64, 64)))
     assert w.reads_ahead(0) and w.reads_ahead(5) and not matrix(64, 64).reads_ahead(0)
+
+
+# ---- what Python declares of the library's functions is what the sources say ---------------------------------------------------
+def declared(name):
+    """The kinds of a C entry's arguments, from its definition."""
+    import os
+    import re
+    folder = os.path.dirname(fp4_ops.__file__)
+    for f in sorted(os.listdir(folder)):
+        if f.startswith("fp4_") and f.endswith(".cu"):
+            with open(os.path.join(folder, f), encoding="utf-8") as fh:
+                got = re.search(r"SSB_API (?:int|long long) " + name + r"\(([^)]*)\) \{", fh.read())
+            if got:
+                kinds = [" ".join(a.split()[:-1]) + "*" * (a.split()[-1][0] == "*") for a in got.group(1).split(",")]
+                return ["P" if "*" in k or k == "cudaStream_t" else {"int": "i", "long long": "q", "float": "f"}[k] for k in kinds]
+    raise AssertionError(f"no definition of {name}")
+
+
+@pytest.mark.parametrize("name", sorted(fp4_ops._SIGNATURES))
+def test_signatures(name):
+    assert [fp4_ops._FORMATS[t] for t in fp4_ops._SIGNATURES[name]] == declared(name)
