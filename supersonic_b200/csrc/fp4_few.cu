@@ -11,6 +11,7 @@
 // taken: fl_few.
 #include "fp4_codes.cuh"
 #include "fp4_few.cuh"
+#include "per_device.h"
 #include <algorithm>
 
 typedef __nv_bfloat16 bf16;
@@ -269,11 +270,13 @@ static size_t fw_fixed(int rows, int k_blocks, int k_warps) {
 template <int NB, int MODE>
 static int fw_launch(const FwArgs& a, int blocks, size_t smem, cudaStream_t stream) {
     auto kernel = fp4_few_kernel<NB, MODE>;
-    static bool configured = false;
-    if (!configured) {
+    static SsbPerDevice<bool> set;
+    bool* configured = set.here();
+    if (!configured) return SSB_ERR_UNSUPPORTED;
+    if (!*configured) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FW_MOST_SMEM);
         if (e != cudaSuccess) return (int)e;
-        configured = true;
+        *configured = true;
     }
     return ssb_launch(kernel, dim3(blocks), dim3(FW_THREADS), smem, stream, a.early != 0, a);
 }

@@ -16,6 +16,7 @@
 #include "fp4_few.cuh"
 #include "fp4_step.cuh"
 #include "packed_call.cuh"
+#include "per_device.h"
 #include "fp4_tc.cuh"
 #include <algorithm>
 
@@ -702,11 +703,13 @@ static int fl_stream(const CUtensorMap& mw, const CUtensorMap& mws, const CUtens
                      int* error_word, cudaStream_t stream) {
     constexpr size_t smem = fl_smem<BN, STAGES>();
     static_assert(smem <= 227 * 1024, "");
-    static bool configured = false;
-    if (!configured) {
+    static SsbPerDevice<bool> set;
+    bool* configured = set.here();
+    if (!configured) return SSB_ERR_UNSUPPORTED;
+    if (!*configured) {
         cudaError_t e = cudaFuncSetAttribute(fp4_stream_kernel<BN, STAGES, MODE, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
-        configured = true;
+        *configured = true;
     }
     return ssb_launch(fp4_stream_kernel<BN, STAGES, MODE, LIST>, dim3(blocks), dim3(FL_THREADS), smem, stream, early, mw, mws, mx, mxs, o, list,
                       m_tiles, n_tiles, f4_k_blocks(K), counters, pieces, error_word);
@@ -717,8 +720,10 @@ static int fl_pair(const CUtensorMap& mx, const CUtensorMap& mw, const void* xs,
                    const FlTiles& list, int m_tiles, int n_tiles, int K, int* error_word, cudaStream_t stream) {
     static_assert(FL_PAIR_SMEM <= 227 * 1024, "");
     auto kernel = fp4_pair_kernel<MODE, LIST>;
-    static int max_pairs = 0;
-    if (!max_pairs) {
+    static SsbPerDevice<int> found;
+    int* max_pairs = found.here();
+    if (!max_pairs) return SSB_ERR_UNSUPPORTED;
+    if (!*max_pairs) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FL_PAIR_SMEM);
         if (e != cudaSuccess) return (int)e;
         const int sms = ssb_sm_count();
@@ -736,9 +741,9 @@ static int fl_pair(const CUtensorMap& mx, const CUtensorMap& mw, const void* xs,
             cudaGetLastError();
             clusters = sms / 2;
         }
-        max_pairs = std::min(clusters, sms / 2);
+        *max_pairs = std::min(clusters, sms / 2);
     }
-    const int pairs = (int)std::min<long long>((long long)m_tiles * n_tiles, max_pairs);
+    const int pairs = (int)std::min<long long>((long long)m_tiles * n_tiles, *max_pairs);
     return ssb_launch(kernel, dim3(2 * pairs), dim3(32 * FL_PAIR_WARPS), FL_PAIR_SMEM, stream, true, mx, mw, (const uint8_t*)xs,
                       (const uint8_t*)ws, x_runs, o, list, m_tiles,
                       n_tiles, f4_k_blocks(K), std::min(n_tiles >= 32 ? 32 : 16, m_tiles), error_word);

@@ -10,6 +10,7 @@
 #include "fp4_few.cuh"
 #include "fp4_step.cuh"
 #include "fp4_tc.cuh"
+#include "per_device.h"
 #include <algorithm>
 
 typedef __nv_bfloat16 bf16;
@@ -205,11 +206,13 @@ static int fs_launch(const CUtensorMap& mw, const CUtensorMap& mws, const CUtens
                      int* error_word, cudaStream_t stream) {
     static_assert(fs_smem<BN>(FS_MOST_SUMS) <= 227 * 1024, "");
     auto kernel = fp4_step_kernel<BN, MODE>;
-    static bool configured = false;
-    if (!configured) {
+    static SsbPerDevice<bool> set;
+    bool* configured = set.here();
+    if (!configured) return SSB_ERR_UNSUPPORTED;
+    if (!*configured) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fs_smem<BN>(FS_MOST_SUMS));
         if (e != cudaSuccess) return (int)e;
-        configured = true;
+        *configured = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((a.N + FL_BM - 1) / FL_BM * parts);

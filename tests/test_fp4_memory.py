@@ -151,3 +151,41 @@ def declared(name):
 @pytest.mark.parametrize("name", sorted(fp4_ops._SIGNATURES))
 def test_signatures(name):
     assert [fp4_ops._FORMATS[t] for t in fp4_ops._SIGNATURES[name]] == declared(name)
+
+
+# ---- what is set once is set on every device ------------------------------------------------------------------------------------
+def test_settings_are_each_devices_own(tmp_path):
+    """csrc/per_device.h against a runtime of three devices, and one whose device has no place."""
+    import os
+    import subprocess
+    from supersonic_b200.csrc import build
+    (tmp_path / "cuda_runtime.h").write_text("""
+enum cudaError_t { cudaSuccess = 0, cudaErrorNoDevice = 100 };
+extern int device;
+inline cudaError_t cudaGetDevice(int* d) { if (device == -2) return cudaErrorNoDevice; *d = device; return cudaSuccess; }
+""")
+    (tmp_path / "check.cpp").write_text("""
+#include "per_device.h"
+int device = 0;
+template <int K> int settings() { static SsbPerDevice<int> set; int* here = set.here(); return here ? ++*here : -1; }
+int main() {
+    int wrong = 0;
+    for (device = 0; device < 3; ++device) wrong += settings<0>() != 1;
+    for (device = 0; device < 3; ++device) wrong += settings<0>() != 2;
+    wrong += (device = 1, settings<1>()) != 1;
+    wrong += (device = 64, settings<0>()) != -1;
+    wrong += (device = -2, settings<0>()) != -1;
+    return wrong;
+}
+""")
+    header = os.path.join(os.path.dirname(build.__file__))
+    subprocess.run([build.find_cxx(), "-std=c++17", "-I", str(tmp_path), "-I", header, str(tmp_path / "check.cpp"), "-o", str(tmp_path / "check")], check=True)
+    assert subprocess.run([str(tmp_path / "check")]).returncode == 0
+
+
+@pytest.mark.parametrize("source", ["fp4_few.cu", "fp4_linear.cu", "fp4_rows.cu", "fp4_step.cu"])
+def test_launches_keep_nothing_for_the_whole_process(source):
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(fp4_ops.__file__), source), encoding="utf-8") as fh:
+        assert not re.findall(r"^\s+static (?!SsbPerDevice|const)[a-z_ ]+\w+( = [^;]*)?;", fh.read(), flags=re.M)
