@@ -230,7 +230,7 @@ SSB_API int ssb_route_softmax(float* z, int ld, const float* bias, int n_tokens,
 // neighbours, a group's score is its largest c or the sum of its two largest; of the experts of the `keep` best groups the `top`
 // largest c win, in order, the lower index (expert, group) at equal scores; an expert's weight is its s times `scale`, with
 // `renormalize` divided by the sum of the chosen s (+ 1e-20).  A logit that is NaN counts as minus infinity, whose s is zero, an infinite one as the
-// largest number; a c that is NaN comes last.  Without correction the larger logit comes first, also where both have the same s.
+// largest number; a c, or a sum of two, that is NaN counts as minus infinity.  Without correction the larger logit comes first, also where both have the same s.
 //
 // What is chosen is chosen by c in 64 bits.  c in 32 bits is within rs_near of it, so a warp (a token, its experts in registers)
 // chooses in 32 bits and looks whether two neighbours of its order, the last chosen and the next among them, or a kept and a
@@ -254,7 +254,7 @@ __device__ __forceinline__ float rs_near(float c) { return 2e-6f + 1e-6f * fabsf
 __device__ __forceinline__ float rs_logit(float z) {
     return z != z || z == -INFINITY ? -INFINITY : fminf(fmaxf(z, -3.4028234663852886e38f), 3.4028234663852886e38f);
 }
-// A number's bits in an order that is the numbers'; 0 is below all of them (and NaN's).
+// A number's bits in an order that is the numbers'; 0 is below all of them, 1 (a NaN's) below minus infinity's.
 __device__ __forceinline__ uint32_t rs_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);         // (both zeros are one)
     return x != x ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -303,7 +303,8 @@ __device__ __noinline__ uint32_t rs_groups_exactly(const RsArgs& a, const float*
         second = fmax(fmin(first, f), fmax(second, s));
         first = fmax(first, f);
     }
-    const double mine = a.by_two && per > 1 ? first + second : first;
+    double mine = a.by_two && per > 1 ? first + second : first;
+    if (mine != mine) mine = -INFINITY;
     int before = 0;
     for (int o = 0; o < a.n_groups; ++o) {
         const double other = __shfl_sync(0xffffffffu, mine, o << log_share);
@@ -429,9 +430,10 @@ route_scored_kernel(const RsArgs a) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int e = j * 32 + lane;
-            const float c = e < a.n_experts ? rough(z[j]) + a.correction[e] : 0.f;
+            float c = e < a.n_experts ? rough(z[j]) + a.correction[e] : 0.f;
+            c = c != c ? -INFINITY : c;
             key[j] = e < a.n_experts ? rs_key(c) : 0u;
-            if (grouped && e < a.n_experts) member[e + 4 * group_of(e)] = c != c ? -INFINITY : c;
+            if (grouped && e < a.n_experts) member[e + 4 * group_of(e)] = c;
         }
     } else {
 #pragma unroll
@@ -457,7 +459,8 @@ route_scored_kernel(const RsArgs a) {
             second = fmaxf(fminf(first, f), fmaxf(second, s));
             first = fmaxf(first, f);
         }
-        const float mine = a.by_two && per > 1 ? first + second : first;
+        float mine = a.by_two && per > 1 ? first + second : first;
+        mine = mine != mine ? -INFINITY : mine;
         int before = 0;
         for (int o = 0; o < a.n_groups; ++o) {
             const float other = __shfl_sync(0xffffffffu, mine, o << log_share);

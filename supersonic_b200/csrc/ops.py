@@ -1755,7 +1755,7 @@ def route_scored(logits: torch.Tensor, n_experts: int, expert_of: torch.Tensor, 
     ``keep`` (all) best of ``groups`` equal groups of neighbours.  A group's score is its largest c (``group_score`` "max") or the sum
     of its two largest ("two").  pair_weight = s * scale of the chosen, with ``renormalize`` divided by the sum of their s (+ 1e-20).
     Ties go to the lower index; without a correction the larger logit comes first, also where its s is the same.  A NaN among the logits counts as minus infinity, whose s is zero, an infinite one as the largest number;
-    a c that is NaN comes last."""
+    a c, or a group's sum, that is NaN counts as minus infinity."""
     shape = logits.shape
     T, top = shape[0], expert_of.shape[-1]
     keep = groups if keep is None else keep

@@ -143,3 +143,34 @@ def test_experts_in_cut_tiles_have_the_same_bits_in_every_run(tokens, k, inter, 
     # the tokens in another order are other tiles
     order = torch.randperm(tokens, generator=g, device=DEV)
     check_experts(x[order], e[order].contiguous(), w[order].contiguous(), first, fv, down, dv, None, torch.float32)
+
+
+# ---- the scored router ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("n, top, groups, keep, by", [(32, 12, 1, 1, "max"), (64, 40, 1, 1, "max"), (64, 16, 8, 4, "two"), (256, 20, 1, 1, "max"),
+                                                      (256, 31, 8, 5, "two"), (300, 64, 3, 2, "max"), (600, 33, 4, 3, "two")])
+def test_route_of_corrections_that_are_infinite_or_no_numbers(n, top, groups, keep, by, scores):
+    """A choice score that is NaN counts as minus infinity: as one of that size, and the lower index first."""
+    g = gen(n + top)
+    inf, nan = float("inf"), float("nan")
+    logits = torch.randn((9, n), generator=g, device=DEV)
+    for share in (0.3, 0.8, 0.97, 1.0):
+        correction = torch.randn((n,), generator=g, device=DEV) * 0.1
+        pick = torch.rand((n,), generator=g, device=DEV)
+        correction[pick < share] = -inf
+        correction[pick < share / 2] = nan
+        check_route(logits, n, top, correction, scores, groups, keep, by)
+        if by == "max":                                           # (of both infinities there is no sum: below)
+            correction[pick < share / 8] = inf
+            check_route(logits, n, top, correction, scores, groups, keep, by)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_of_a_group_whose_two_best_have_no_sum(scores):
+    """Groups of (inf, -inf), (1, 1) and (2, -inf), two of which are kept: the first's sum counts as minus infinity, as the last's is."""
+    from supersonic_b200.csrc import ops
+    inf = float("inf")
+    correction = torch.tensor([inf, -inf, 1.0, 1.0, 2.0, -inf], device=DEV)
+    e, w = torch.empty((3, 3), dtype=torch.int32, device=DEV), torch.empty((3, 3), device=DEV)
+    ops.route_scored(torch.zeros((3, 6), device=DEV), 6, e, w, scores, correction, 3, 2, "two")
+    assert e.tolist() == [[0, 2, 3]] * 3 and bool(((w - 1 / 3).abs() < 1e-6).all())
