@@ -1757,7 +1757,7 @@ def route_scored(logits: torch.Tensor, n_experts: int, expert_of: torch.Tensor, 
     Ties go to the lower index; without a correction the larger logit comes first, also where its s is the same.  A NaN among the logits counts as minus infinity, whose s is zero, an infinite one as the largest number;
     a c, or a group's sum, that is NaN counts as minus infinity."""
     shape = logits.shape
-    T, top = shape[0], expert_of.shape[-1]
+    T, top = (shape[0], expert_of.shape[1]) if len(shape) == 2 and expert_of.dim() == 2 else (0, 0)
     keep = groups if keep is None else keep
     if len(shape) != 2 or logits.dtype is not torch.float32 or shape[1] < n_experts or (logits.stride(1) != 1 and shape[1] > 1) \
             or expert_of.dtype is not torch.int32 or pair_weight.dtype is not torch.float32 or expert_of.shape != (T, top) \
