@@ -191,6 +191,16 @@ def _workspace(x: Rows, needs: int, device, words: int, ahead: int = 0):
     return buffer, at + 4 * words, at
 
 
+def _over(at: int, step: int, width: int, at2: int, step2: int, width2: int, rows: int) -> bool:
+    """Whether two matrices of so many rows, ``width`` bytes every ``step``, have memory in common."""
+    if at2 >= at + (rows - 1) * step + width or at >= at2 + (rows - 1) * step2 + width2:
+        return False
+    if rows == 1 or step != step2:
+        return True
+    off = (at2 - at) % step                     # parts of the same wider rows
+    return off < width or off + width2 > step
+
+
 def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = False) -> None:
     """``out`` [rows, n] (+)= x W^T with ``x`` [rows, k] (float32 or bfloat16, quantised as it comes, or a 4-bit matrix) and ``weight``
     [n, k].  ``accumulate`` adds to a float32 ``out``.  n: a multiple of 8."""
@@ -201,8 +211,10 @@ def linear(x: Rows, weight: Fp4Matrix, out: torch.Tensor, accumulate: bool = Fal
     o_at, ldo = _rows(out, "out", rows, n)
     if accumulate and out.dtype is not torch.float32:
         raise KernelError("linear: results are added in float32 only")
-    if rows and o_at == x_at:
-        raise KernelError("linear: out must not be x")
+    step, width = (ldx * x.element_size(), k * x.element_size()) if code >= 0 else (k // 2, k // 2)
+    size = out.element_size()
+    if rows and _over(x_at, step, width, o_at, ldo * size, n * size, rows):
+        raise KernelError("linear: out must not be x, or lie over it")
     stream = _stream(index, weight.index, out.get_device())
     if rows == 0:
         return
