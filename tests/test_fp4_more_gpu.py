@@ -174,3 +174,125 @@ def test_route_of_a_group_whose_two_best_have_no_sum(scores):
     e, w = torch.empty((3, 3), dtype=torch.int32, device=DEV), torch.empty((3, 3), device=DEV)
     ops.route_scored(torch.zeros((3, 6), device=DEV), 6, e, w, scores, correction, 3, 2, "two")
     assert e.tolist() == [[0, 2, 3]] * 3 and bool(((w - 1 / 3).abs() < 1e-6).all())
+
+
+# ---- a step's rows against more tiles of channels than there are SMs --------------------------------------------------------------
+def drawn(g, *shape, gated=False):
+    """(Fp4Matrix of random codes, its float64 values with the gate rows first)"""
+    from supersonic_b200.weights import Fp4Matrix
+    codes = torch.randint(0, 256, shape[:-1] + (shape[-1] // 2,), generator=g, device=DEV).to(torch.uint8)
+    scales = torch.randint(115, 121, shape[:-1] + (shape[-1] // 32,), generator=g, device=DEV).to(torch.uint8)
+    return Fp4Matrix.from_parts(codes, scales, gated=gated), pf.values(Fp4Matrix.from_parts(codes, scales))
+
+
+@pytest.mark.parametrize("numbers", [True, False])
+@pytest.mark.parametrize("rows", [1, 8, 16, 17, 32])
+@pytest.mark.parametrize("n, k", [(19000, 1056), (28672, 4096), (40000, 288)])
+def test_wide_products_of_a_steps_rows(n, k, rows, numbers):
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(n + rows)
+    x, (w, wv) = randn(g, rows, k, dtype=torch.bfloat16), drawn(g, n, k)
+    xv, x = pf.rounded(x.double()), x if numbers else rows4(x)
+    want, slack = xv @ wv.t(), pf.sum_slack(xv, wv)
+    for dtype in TYPES.values():
+        out = torch.full((rows, n), float("nan"), dtype=dtype, device=DEV)
+        fp4_ops.linear(x, w, out)
+        check(out, want, slack)
+    was = torch.randn((rows, n), generator=g, device=DEV)
+    out = was.clone()
+    fp4_ops.linear(x, w, out, accumulate=True)
+    check(out, want + was.double(), slack)
+    fp4_ops.linear(x, w, was, accumulate=True)
+    assert torch.equal(out, was)
+
+
+@pytest.mark.parametrize("numbers", [True, False])
+@pytest.mark.parametrize("rows", [1, 8, 16, 17, 32])
+@pytest.mark.parametrize("inter, k", [(9504, 1056), (14336, 4096), (20000, 288)])
+def test_wide_units_of_a_steps_rows(inter, k, rows, numbers):
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(inter + rows)
+    x, (first, fv), (down, dv) = randn(g, rows, k, dtype=torch.bfloat16), drawn(g, 2 * inter, k, gated=True), drawn(g, 64, inter)
+    xv, x = pf.rounded(x.double()), x if numbers else rows4(x)
+    z = fp4_ops.gate_up(x, first)
+    check_inner(z, *pf.inner(xv, fv, True, None))
+    out = torch.empty((rows, 64), device=DEV)
+    fp4_ops.linear(z, down, out)
+    check(out, pf.values(z) @ dv.t(), pf.sum_slack(pf.values(z), dv))
+    wide, wv = drawn(g, 2 * inter, k)
+    z = fp4_ops.activated(x, wide, "relu_squared", scale=0.5)
+    want, slack = pf.inner(xv, wv, False, "relu_squared")
+    check_inner(z, want * 0.5, slack * 0.5)
+
+
+# ---- inner rows' scales behind the last channel ------------------------------------------------------------------------------------
+@pytest.fixture
+def poisoned(monkeypatch):
+    """Memory that the operators take is full of ones: scales that are no numbers."""
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: empty(*a, **kw).fill_(-1) if kw.get("dtype") is torch.int8 else empty(*a, **kw))
+
+
+@pytest.mark.parametrize("numbers", [True, False])
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("rows, k, inter", [(1, 512, 96), (8, 512, 1056), (12, 2048, 96), (30, 1024, 1056), (40, 512, 96), (40, 512, 1056), (120, 256, 2016),
+                                            (300, 512, 96), (300, 512, 1056), (700, 256, 288), (9, 1056, 19008), (20, 1056, 19008)])
+def test_inner_rows_end_in_scales_of_zero(poisoned, rows, k, inter, gated, numbers):
+    """Up to a whole k-block, as the product that reads them multiplies what lies there by zeros."""
+    from supersonic_b200.csrc import fp4_ops
+    g = gen(rows + inter)
+    x = randn(g, rows, k, dtype=torch.bfloat16)
+    x = x if numbers else rows4(x)
+    z = fp4_ops.gate_up(x, drawn(g, 2 * inter, k, gated=True)[0]) if gated else fp4_ops.activated(x, drawn(g, inter, k)[0], "silu")
+    runs, blocks = -(-rows // 128), -(-inter // 256) * 8
+    scales = z.scales.view(runs, blocks // 8, 2, 32, 4, 4).permute(0, 4, 3, 1, 2, 5).reshape(runs * 128, blocks)
+    assert torch.equal(scales[:rows, : inter // 32], z.plain_scales())
+    assert inter % 256 and bool((scales[:rows, inter // 32:] == 0).all())
+    down, dv = drawn(g, 72, inter)
+    out = torch.empty((rows, 72), device=DEV)
+    fp4_ops.linear(z, down, out)
+    check(out, pf.values(z) @ dv.t(), pf.sum_slack(pf.values(z), dv))
+
+
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("tokens, k, inter, experts, top", [(1, 288, 96, 8, 2), (20, 288, 96, 8, 3), (150, 288, 96, 40, 2), (90, 4128, 4128, 4, 1),
+                                                            (400, 288, 160, 4, 2)])
+def test_experts_in_memory_that_holds_anything(poisoned, tokens, k, inter, experts, top, gated):
+    g = gen(tokens + 5)
+    x = randn(g, tokens, k, dtype=torch.bfloat16)
+    (first, fv), (down, dv) = drawn(g, experts, (2 if gated else 1) * inter, k, gated=gated), drawn(g, experts, k, inter)
+    e, w = choices(g, tokens, experts, top)
+    check_experts(x, e, w, first, fv, down, dv, None if gated else "silu", torch.float32)
+
+
+# ---- a model's matrices -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["A", "D", "E"])
+def test_a_models_matrices_are_its_weights_in_4_bits(model_folders, name, dtype):
+    """Every projection and unit of a loaded model, read back, against the folder's tensors rounded by the formula."""
+    import supersonic_b200
+    from supersonic_b200.csrc import fp4_ops
+    from supersonic_b200.weights import Fp4Matrix, WeightStore
+    folder = model_folders[name][0]
+    model = supersonic_b200.load(folder, dtype=dtype, context_size=64, weight_format="mxfp4").model
+    store = WeightStore.from_dir(folder)
+
+    def read(m):
+        out = torch.empty(m.shape, device=DEV)
+        fp4_ops.values(m, out)
+        return out.double()
+
+    def stored(part, *roles):
+        kind = torch.float32 if dtype == "float32" else torch.bfloat16
+        return pf.rounded(torch.cat([store.get(part.weights[r], torch.device(DEV)).to(kind) for r in roles]).double())
+    seen = 0
+    for block, spec in zip(model.blocks, model.spec.blocks):
+        mixer, ff = block.mixer, block.feed_forward
+        if isinstance(getattr(mixer, "w_qkv", None), Fp4Matrix):
+            assert torch.equal(read(mixer.w_qkv), stored(spec.mixer, "q", "k", "v")) and torch.equal(read(mixer.w_o), stored(spec.mixer, "o"))
+            assert torch.equal(read(mixer.w_q), stored(spec.mixer, "q"))
+            seen += 1
+        if isinstance(getattr(ff, "w_gate_up", None), Fp4Matrix):
+            assert torch.equal(read(ff.w_gate_up), stored(spec.feed_forward, "gate", "up")) and torch.equal(read(ff.w_down), stored(spec.feed_forward, "down"))
+            seen += 1
+    assert seen > 0
