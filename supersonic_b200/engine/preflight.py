@@ -69,7 +69,8 @@ def _fp4_names(spec):
     for b in spec.blocks:
         names = set()
         for ps, table, what in ((b.mixer, MIXERS, "mixer"), (b.feed_forward, FEED_FORWARDS, "feed-forward")):
-            roles = getattr(lookup(table, ps.kind, what), "fp4_roles", ()) if ps is not None else ()
+            of = getattr(lookup(table, ps.kind, what), "fp4_roles", None) if ps is not None else None
+            roles = of(ps.params) if of is not None else ()
             names |= {n for r, n in (ps.weights.items() if roles else ()) if any(r == x or (x.endswith(".") and r.startswith(x)) for x in roles)}
         yield names
 
@@ -77,7 +78,7 @@ def _fp4_names(spec):
 def weight_bytes(spec, store, dtype: torch.dtype, weight_format: Optional[str] = None) -> int:
     """Matrices are kept in ``dtype``; vectors (norm weights) as stored.  A tensor two parts name
     (a tied head) is counted once.  In a 4-bit format: 17 bytes for 32 numbers of the matrices that have it, and once the largest
-    block's matrices as they are loaded (a matrix whose sizes have no such form is larger than is counted here)."""
+    block's matrices as they are loaded."""
     item = torch.empty((), dtype=dtype).element_size()
     if weight_format is not None:
         def numel(n):

@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from ..cache import PAGE_SHIFT, KvNeed
-from .fp4 import fp4_fits, fp4_of
+from .fp4 import fp4_fits, fp4_of, fp4_sizes
 from .registry import BuildContext, register_mixer
 
 
@@ -53,7 +53,10 @@ class Attention:
         self.w_q = self.w_qkv[: self.n_q * self.head_dim]     # for a stop that only reads a cache
         self.dtype = build.dtype
 
-    fp4_roles = ("q", "k", "v", "o")
+    @staticmethod
+    def fp4_roles(params):
+        fits = fp4_sizes(int(params["hidden_size"]), int(params["num_heads"]) * int(params["head_dim"]))
+        return ("q", "k", "v", "o") if fits else ()
 
     def to_fp4(self) -> bool:
         """The projections as 4-bit matrices; False (and nothing changes) where their sizes have no such form."""

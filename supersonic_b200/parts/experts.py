@@ -35,7 +35,7 @@ import torch
 
 from ..csrc.kernel_sets import as_tensor
 from ..weights.fp4 import Fp4Matrix
-from .fp4 import fp4_fits, fp4_of
+from .fp4 import fp4_fits, fp4_of, fp4_sizes
 from .registry import BuildContext, register_feed_forward
 
 ROUTERS: Dict[str, type] = {}
@@ -259,11 +259,19 @@ class Experts:
         shared = 3 * int(params["shared"]["intermediate_size"]) if params.get("shared") else 0
         return int(params["top"]) * (inner * int(params["expert_size"]) + 3 * int(params["hidden_size"])) + shared
 
-    fp4_roles = ("gate.", "up.", "down.", "shared.gate", "shared.up", "shared.down")
+    MOST_IN_FP4 = 4096                                        # experts
+
+    @staticmethod
+    def fp4_roles(params):
+        hidden, shared = int(params["hidden_size"]), params.get("shared")
+        if not fp4_sizes(hidden, int(params["expert_size"])) or int(params["n_experts"]) > Experts.MOST_IN_FP4:
+            return ()
+        takes_shared = shared and fp4_sizes(hidden, int(shared["intermediate_size"]))
+        return ("gate.", "up.", "down.") + (("shared.gate", "shared.up", "shared.down") if takes_shared else ())
 
     def to_fp4(self) -> bool:
         """The experts' matrices (and the shared one's) as 4-bit ones; False (and nothing changes) where their sizes have no such form."""
-        if not (fp4_fits(self.w_down) and fp4_fits(self.w_first) and self.inter % 32 == 0 and self.E <= 4096):
+        if not (fp4_fits(self.w_down) and fp4_fits(self.w_first) and self.inter % 32 == 0 and self.E <= self.MOST_IN_FP4):
             return False
         self.w_first, self.w_down = fp4_of(self.w_first, gated=self.gated), fp4_of(self.w_down)
         if self.shared is not None:

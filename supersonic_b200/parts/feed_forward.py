@@ -7,7 +7,7 @@ from __future__ import annotations
 import torch
 
 from ..weights.fp4 import Fp4Matrix
-from .fp4 import fp4_fits, fp4_of
+from .fp4 import fp4_fits, fp4_of, fp4_sizes
 from .registry import BuildContext, register_feed_forward
 
 
@@ -55,7 +55,9 @@ class SwiGLU:
         """Elements per token this part holds while it runs: gate and up, and their product."""
         return 3 * int(params["intermediate_size"])
 
-    fp4_roles = ("gate", "up", "down")
+    @staticmethod
+    def fp4_roles(params):
+        return ("gate", "up", "down") if fp4_sizes(int(params["hidden_size"]), int(params["intermediate_size"])) else ()
 
     def to_fp4(self) -> bool:
         """The unit's matrices as 4-bit ones; False (and nothing changes) where their sizes have no such form."""
@@ -110,7 +112,9 @@ class DenseFeedForward:
     def activation_elements(params) -> int:
         return 2 * int(params["intermediate_size"])
 
-    fp4_roles = ("up", "down")
+    @staticmethod
+    def fp4_roles(params):
+        return ("up", "down") if fp4_sizes(int(params["hidden_size"]), int(params["intermediate_size"])) else ()
 
     def to_fp4(self) -> bool:
         """The matrices as 4-bit ones; False (and nothing changes) where their sizes have no such form."""

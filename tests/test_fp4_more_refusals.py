@@ -73,3 +73,74 @@ def test_linear_refuses_results_over_rows_in_4_bits(launched):
         else:
             with pytest.raises(KernelError, match="must not be x"):
                 fp4_ops.linear(m, matrix(8, 64), out)
+
+
+def weight_bytes_of(config, weight_format):
+    from supersonic_b200.config import config_from_dict
+    from supersonic_b200.engine import preflight
+    from supersonic_b200.weights import RandomWeightStore
+    cfg = config_from_dict(config)
+    return preflight.weight_bytes(cfg.build_spec(), RandomWeightStore(cfg, 1), torch.bfloat16, weight_format)
+
+
+@pytest.mark.parametrize("hidden, inter, heads, head_dim, attention, unit", [
+    (96, 256, 3, 32, True, True), (96, 200, 3, 32, True, False), (72, 256, 3, 32, False, False), (96, 256, 3, 16, False, True),
+    (72, 200, 3, 16, False, False), (64, 72, 5, 16, False, False),
+])
+def test_memory_of_matrices_that_have_no_4_bit_form(hidden, inter, heads, head_dim, attention, unit):
+    import tiny_configs
+    config = dict(tiny_configs.B, hidden_size=hidden, intermediate_size=inter, num_attention_heads=heads, num_key_value_heads=1, head_dim=head_dim)
+    held = (2 * heads + 2) * head_dim * hidden * attention + 3 * inter * hidden * unit
+    layers = config["num_hidden_layers"]
+    assert weight_bytes_of(config, "mxfp4") == weight_bytes_of(config, None) - 2 * layers * held + layers * held * 17 // 32 + 2 * held
+
+
+@pytest.mark.parametrize("hidden, inter, shared, n", [(64, 96, None, 4), (64, 96, 32, 4), (64, 96, 40, 4), (64, 40, 32, 4), (72, 96, 32, 4), (64, 32, None, 4097)])
+def test_what_a_part_says_of_its_sizes_is_what_it_does(monkeypatch, hidden, inter, shared, n):
+    """``fp4_roles`` from the parameters, ``to_fp4`` from the matrices."""
+    from supersonic_b200.parts import attention, experts, feed_forward
+
+    def of(w, gated=False):
+        return Fp4Matrix.empty(*w.shape, device="cpu", gated=gated)
+
+    class Kernels:
+        @staticmethod
+        def pack_gate_up(gate, up):
+            return torch.cat([gate, up]), "halves"
+
+    class Weights:
+        def __init__(self, shapes):
+            self.shapes = shapes
+
+        def as_dtype(self, name, dtype):
+            return torch.zeros(1, dtype=dtype).expand(self.shapes[name.split(".")[0] if name not in self.shapes else name])
+        stored = as_dtype
+
+    class Build:
+        device, dtype, kernels = torch.device("cpu"), torch.bfloat16, Kernels
+
+        def __init__(self, shapes):
+            self.weights = Weights(shapes)
+    for module in (attention, experts, feed_forward):
+        monkeypatch.setattr(module, "fp4_of", of)
+    unit = {"gate": (inter, hidden), "up": (inter, hidden), "down": (hidden, inter)}
+    params = {"hidden_size": hidden, "intermediate_size": inter}
+    part = feed_forward.SwiGLU(params, {r: r for r in unit}, Build(unit))
+    assert part.to_fp4() == bool(part.fp4_roles(params)) == isinstance(part.w_down, Fp4Matrix)
+    part = feed_forward.DenseFeedForward(params, {r: r for r in unit}, Build(unit))
+    assert part.to_fp4() == bool(part.fp4_roles(params)) == isinstance(part.w_down, Fp4Matrix)
+    params = {"hidden_size": hidden, "num_heads": 1, "num_kv_heads": 1, "head_dim": 16 * (inter // 16), "scale": 1.0}
+    sizes = {r: (params["head_dim"], hidden) for r in "qkv"}
+    sizes["o"] = (hidden, params["head_dim"])
+    part = attention.Attention(params, {r: r for r in sizes}, Build(sizes))
+    assert part.to_fp4() == bool(part.fp4_roles(params)) == isinstance(part.w_o, Fp4Matrix)
+    params = {"hidden_size": hidden, "n_experts": n, "top": 1, "expert_size": inter, "router": {"kind": "none here"},
+              "shared": {"intermediate_size": shared} if shared else None}
+    sizes = dict(unit, **{f"shared.{r}": tuple(shared or 1 if s == inter else s for s in shape) for r, shape in unit.items()})
+    monkeypatch.setitem(experts.ROUTERS, "none here", lambda *a: None)
+    names = {f"{r}.{e}": f"{r}.{e}" for r in unit for e in range(n)}
+    names.update({f"shared.{r}": f"shared.{r}" for r in unit})
+    part = experts.Experts(params, names, Build(sizes))
+    roles = part.fp4_roles(params)
+    assert part.to_fp4() == bool(roles) == part.in_fp4
+    assert bool(shared) is False or isinstance(part.shared.w_down, Fp4Matrix) == ("shared.gate" in roles)
