@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from ..cache import SequenceCache
-from ..config import ModelSpec, load_config, spec_from_config
+from ..config import ConfigError, ModelSpec, load_config, spec_from_config
 from ..csrc.kernel_sets import kernel_set_for
 from ..parts import (BLOCKS, EMBEDDINGS, FEED_FORWARDS, HEADS, MIXERS, NORMS, POSITION_ENCODINGS, STREAM_ADAPTERS,
                      BuildContext, WeightAccess, lookup)
@@ -238,7 +238,7 @@ class Model:
             own = {"params": b.params, "weights": b.weights, "build": build} if (b.params or b.weights) else {}
             self.blocks.append(lookup(BLOCKS, b.kind, "block")(mixer, ff, n1, n2, pos, **own))
         if weight_format is not None and not any(in_fp4):
-            raise ValueError(f"weight_format {weight_format!r}: no part of this model has matrices that it can hold in that format")
+            raise ConfigError(f"weight_format {weight_format!r}: no part of this model has matrices that it can hold in that format")
         self.final_norm = part(NORMS, "norm", spec.final_norm)
         self.head = part(HEADS, "head", spec.head)
         self.adapters = [part(STREAM_ADAPTERS, "stream adapter", a) for a in spec.adapters]

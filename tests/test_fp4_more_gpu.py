@@ -296,3 +296,15 @@ def test_a_models_matrices_are_its_weights_in_4_bits(model_folders, name, dtype)
             assert torch.equal(read(ff.w_gate_up), stored(spec.feed_forward, "gate", "up")) and torch.equal(read(ff.w_down), stored(spec.feed_forward, "down"))
             seen += 1
     assert seen > 0
+
+
+def test_a_model_without_such_matrices_is_refused_with_a_line(model_folders, capsys):
+    """Sizes that are no multiples of 32: an error that the command prints."""
+    import supersonic_b200
+    from supersonic_b200.cli import main
+    from supersonic_b200.config import ConfigError
+    folder = model_folders["C"][0]
+    with pytest.raises(ConfigError, match="mxfp4"):
+        supersonic_b200.load(folder, context_size=64, weight_format="mxfp4")
+    assert main(["--model-dir", folder, "--prompt-ids", "5,17,3", "--max-new-tokens", "2", "--weight-format", "mxfp4"]) == 1
+    assert "mxfp4" in capsys.readouterr().err
