@@ -281,12 +281,12 @@ static int fw_launch(const FwArgs& a, int blocks, size_t smem, cudaStream_t stre
     return ssb_launch(kernel, dim3(blocks), dim3(FW_THREADS), smem, stream, a.early != 0, a);
 }
 
-// How a product of M rows by N x K weights runs; slots 0: not by this kernel.
+// How a product of M rows by N x K weights runs; slots 0: not by this kernel, which takes up to 16 rows, where it makes inner rows up to 8.
 struct FwPlan { int nb, k_warps, slots, blocks; size_t smem; };
 static FwPlan fw_plan(int M, int N, int K, int mode) {
     FwPlan p{};
     const int k_blocks = f4_k_blocks(K), sms = ssb_sm_count();
-    if (M > 16) return p;
+    if (M > (mode == FW_STORE ? 16 : 8)) return p;
     p.nb = M <= 8 ? 1 : 2;
     // channels a tile and warps along k: as few steps of a warp as can be, one after another on the fullest SM; a gated tile is 64
     // channels (32 inner ones, a block) at least, an ungated one of inner channels 32
@@ -317,9 +317,7 @@ int fw_product(FwArgs a, int mode, cudaStream_t stream) {
     a.k_warps = p.k_warps;
     a.slots = p.slots;
     a.k_blocks = f4_k_blocks(a.K);
-    if (p.nb == 1)
-        return mode == FW_STORE ? fw_launch<1, FW_STORE>(a, p.blocks, p.smem, stream)
-               : mode == FW_GATED ? fw_launch<1, FW_GATED>(a, p.blocks, p.smem, stream) : fw_launch<1, FW_ACT>(a, p.blocks, p.smem, stream);
-    return mode == FW_STORE ? fw_launch<2, FW_STORE>(a, p.blocks, p.smem, stream)
-           : mode == FW_GATED ? fw_launch<2, FW_GATED>(a, p.blocks, p.smem, stream) : fw_launch<2, FW_ACT>(a, p.blocks, p.smem, stream);
+    if (p.nb == 2) return fw_launch<2, FW_STORE>(a, p.blocks, p.smem, stream);
+    return mode == FW_STORE ? fw_launch<1, FW_STORE>(a, p.blocks, p.smem, stream)
+           : mode == FW_GATED ? fw_launch<1, FW_GATED>(a, p.blocks, p.smem, stream) : fw_launch<1, FW_ACT>(a, p.blocks, p.smem, stream);
 }

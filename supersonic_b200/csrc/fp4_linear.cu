@@ -686,7 +686,7 @@ struct FlScratch {
 constexpr long long FL_FEW_NUMBERS = 32768, FL_FEW_INNER = 16384;
 static bool fl_few(int M, int N, int K, int mode) {
     if ((long long)N * K > (M <= 4 ? 24 << 20 : M <= 8 ? 16 << 20 : 4 << 20)) return false;
-    if (mode == FL_STORE ? (long long)M * K > FL_FEW_NUMBERS : M > 8 || K > 4096 || (long long)M * K > FL_FEW_INNER) return false;
+    if (mode == FL_STORE ? (long long)M * K > FL_FEW_NUMBERS : K > 4096 || (long long)M * K > FL_FEW_INNER) return false;
     return fw_takes(M, N, K, mode);
 }
 

@@ -11,8 +11,6 @@ The modelled project's 4-bit lanes keep int4 codes with a float scale a group (c
 """
 from __future__ import annotations
 
-from typing import Optional
-
 import torch
 
 FP4_BLOCK = 32
