@@ -235,9 +235,11 @@ SSB_API int ssb_route_softmax(float* z, int ld, const float* bias, int n_tokens,
 // What is chosen is chosen by c in 64 bits.  c in 32 bits is within rs_near of it, so a warp (a token, its experts in registers)
 // chooses in 32 bits and looks whether two neighbours of its order, the last chosen and the next among them, or a kept and a
 // dropped group, are closer than that: only then (a token in a thousand) it computes the groups' scores, or the candidates', in 64
-// bits.  Without correction c grows with z, and the order is z's own.
+// bits.  Without correction c grows with z, and the order is z's own.  The chosen experts' weights are made in 32 bits: an exponential, a
+// sum and a quotient, some 1e-7 of them.
 // 8,192 tokens, 256 experts in 8 groups, 8 chosen by corrected sigmoids: 19 us; 1,400 instructions
-// a token and what they wait for bound it (the logits' 8.4 MB take 1.3).  Choosing round by round, a reduction over the warp for the largest and
+// a token and what they wait for bound it (the logits' 8.4 MB take 1.3); registers for eight blocks an SM leave the forms of up to 512 experts
+// stack frames of 120 to 176 bytes, spills among them (16 experts a lane: 308 bytes loaded).  Choosing round by round, a reduction over the warp for the largest and
 // one for its expert, and with all scores of a close token in 64 bits, it took 34; in that form with the latter in local memory 49.
 // ---------------------------------------------------------------------------------------
 constexpr int RS_MOST_GROUPS = 32;

@@ -4,10 +4,10 @@
 // quantised there by every block if they come as numbers.
 //
 // A block of 32 numbers is two mma.sync (m16n8k16) of float16: 16 channels x 8 rows.  Codes are exact in float16, and so are a block's
-// products and their sum in float32 (multiples of 0.25 up to 1,152); then come the two scales, and the float32 sum.  (e4m3 operands, half
-// as many instructions, are taken apart into float16 ones by the compiler: 36 million instructions for what takes half of them so.)
+// products and their sum in float32 (multiples of 0.25 up to 1,152); then come the two scales, and the float32 sum.  (With e4m3 operands,
+// half as many products, 36 million instructions were counted for what takes half of them so.)
 // tcgen05 with its own scales needs a tile's 128 channels and their rows in tensor memory before the first product and a way back after
-// the last, and rows that come as numbers a launch before it: one row x 2,048 x 2,048 takes 5.2 us so and 3.5 here.  Where each is
+// the last, and rows that come as numbers a launch before it: one row x 2,048 x 2,048 takes 5.2 us so and 3.4 here.  Where each is
 // taken: fl_few.
 #include "fp4_codes.cuh"
 #include "fp4_few.cuh"

@@ -306,7 +306,8 @@ fp4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 // in order with the products and took 0.19 us of a k-block's 0.66 (six of them; 8,192 x 14,336 x 4,096: 266 us); through shared memory
 // by TMA they stand behind the codes that were asked for before them (357 us), and by cp.async a k-block takes these warps 850 clocks.
 //
-// 8,192 x 14,336 x 4,096: 179 us, 5.4 PFLOP/s, the tensor pipe busy 73 % of the cycles.  Bound by codes on their way from L2 (two sides of
+// 8,192 x 14,336 x 4,096: 179 us (201 with rows to codes), 5.4 PFLOP/s, the tensor pipe busy 73 % of the cycles, at 1,965 MHz; where calls
+// follow one another for half a second the power cap takes the clock to some 1,500 MHz, and a call 229 us.  Bound by codes on their way from L2 (two sides of
 // 256 a tile, some 46 bytes a clock and SM) and by results on theirs (without them 35 us less).
 //
 // Results leave in runs of 128 bytes, which takes the place of a sixth stage of codes (of 64 bytes with six: 8,192 x 14,336 x 4,096 209 us
@@ -629,13 +630,15 @@ struct FlPlan {
     size_t pieces;                         // bytes
 };
 // What a product is expected to take, in microseconds, by a fit to measured times of all forms over 1 .. 1,024 rows and 4 to 117
-// million weights:
+// million weights (of the pairs' kernel with a sixth stage, which its results' runs have taken since):
 //  * a block of the streaming kernel takes 3.8 + 0.046 a row, and 0.37 a k-block of 128 weight rows whatever its rows; pieces of split
 //    tiles 2.2 and, each, 0.1 + 0.01 a row;
 //  * a pair 6.5, 0.43 a k-block of 256 x 256 and 0.03 for each tile beside it.
 // At 2,048 x 2,048: 48 rows by tiles of 64 that are whole 9.1, in 2 parts 10.7; at 4,096 x 14,336: 64 rows by 64 in 2 parts 20.4, in 4 16.7,
 // dealt out over all SMs 20.8; 128 rows by 64 in 2 parts 20.7, by 128 in 4 22.2, on pairs 30; at 14,336 x 4,096: 64 rows by 64 14.0, 128
-// by 128 17.2, on pairs 15.7; 1,024 rows by 128 70, on pairs 35.  Tiles of 16 and 32 rows are only where one holds all rows: the next one's
+// by 128 17.2, on pairs 15.7; 1,024 rows by 128 70, on pairs 35.  As they are taken now, rows to codes among them, weights from memory and
+// from L2: 14,336 x 4,096 64 rows 12.0 and 10.3, 128 17.2 and 14.2, 300 23.9 and 21.3, 1,024 39.5 and 39.3; 4,096 x 14,336 64 rows 16.1 and
+// 15.1, 128 20.1 and 19.8; 28,672 x 4,096 8 rows 16.7 and 14.1.  Tiles of 16 and 32 rows are only where one holds all rows: the next one's
 // scales would begin between the columns that a product can name (and only where there are more tiles than SMs: else fp4_step.cu).
 static FlPlan fl_plan(int M, int N, int K) {
     const int sms = ssb_sm_count(), k_blocks = f4_k_blocks(K);

@@ -132,8 +132,8 @@ def quantize(x: torch.Tensor, matrix: Fp4Matrix) -> None:
 
 
 def values(matrix: Fp4Matrix, out: torch.Tensor) -> None:
-    """``out`` (float32 or bfloat16, of its shape) gets the numbers that ``matrix`` stands for, which both types hold exactly (down to
-    2^-128); of a gated matrix the gate rows, then the up rows."""
+    """``out`` (float32 or bfloat16, of its shape) gets the numbers that ``matrix`` stands for, which both types hold exactly (from
+    2^-128; what is 2^128 or more, of scales that only parts can bring, is an infinity); of a gated matrix the gate rows, then the up rows."""
     at, ld, rows, code = _matrix_rows(out, "out", matrix)
     n, k = matrix.shape[-2:]
     _check(_fn("ssb_fp4_values")(matrix.codes_at, matrix.scales_at, at, ld, code, rows, k, n,

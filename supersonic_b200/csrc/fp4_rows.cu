@@ -30,8 +30,9 @@ struct FrStep {
 // A unit is 16 V numbers of a row: sixteen lanes of V, 32 / V lanes a block, scales in words of four.  Units run over whole
 // k-blocks; behind a row's end they write scales of zero.  TURNS units are in flight.
 //
-// Instructions bound it where there are many rows (144 for 256 numbers of bfloat16 with V = 8, places and scale bytes more than half of
-// them), so a lane takes sixteen numbers, two units in flight: 8,192 x 4,096 19.9 us (87 MB, 4.4 TB/s; eight numbers, one unit 23.7),
+// Where there are many rows, fetches and instructions bound it (59 % of issue slots, 62 % of the ALU pipe's cycles, and fetches what most warps
+// wait for; 144 instructions for 256 numbers of bfloat16 with V = 8, places and scale bytes more than half of them), so a lane takes sixteen
+// numbers, two units in flight: 8,192 x 4,096 19.9 us (87 MB, 4.4 TB/s; eight numbers, one unit 23.7),
 // 14,336 x 4,096 32 (40).  Few rows are a launch and a dependent fetch or two, on as many SMs as can be: 64 x 2,048 1.5 us (2.0 by sixteen),
 // 512 x 2,048 1.9 (2.1); they cross at about 1,024 x 2,048 (2.6, 2.5).
 template <typename T, int TURNS, int V, bool PAIRS>
@@ -179,7 +180,7 @@ static int fr_quantize(const T* x, long long ldx, uint8_t* codes, uint8_t* scale
 }
 
 // x: rows x K, rows of 16-byte pieces; ``per_expert`` rows of them are a matrix; clear: words zeroed on the way.  early: the next
-// launch may begin meanwhile, which it must not if it takes the codes for weights and reads ahead.
+// launch may begin meanwhile.
 SSB_API int ssb_fp4_quantize(const void* x, long long ldx, int dtype, void* codes, void* scales, int rows, int K, int per_expert, int inter,
                              int* clear, int n_clear, int early, cudaStream_t stream) {
     const int rc = fr_sizes(rows, K, per_expert, inter);

@@ -22,8 +22,8 @@ __device__ __forceinline__ void fl_copy_scales(uint32_t tmem, uint32_t addr) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(fl_scale_desc(addr)) : "memory");
 }
 // One lane of the warp, all of whose lanes call it together.  A warp issues its products from code that all its lanes run, under this
-// lane's predicate: descriptors and addresses are then in uniform registers as the instructions want them.  (One lane alone in a branch
-// moves each of them there, some twenty for four instructions: 875 clocks a k-block with its waits, whatever the tile.)
+// lane's predicate.  (From a branch that one lane alone runs a k-block took 875 clocks with its waits, whatever the tile: 8 x 4,096 x 14,336
+// 13.4 us for 10.9.)
 __device__ __forceinline__ bool fl_elect() {
     uint32_t one;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(one));
@@ -103,6 +103,8 @@ __device__ __forceinline__ void fl_put_inner(float (&v)[V], uint8_t* dst, uint8_
 }
 
 // Up to 16 rows' sums of a tile of 128 channels (a thread of four warps one channel) become inner rows in 4 bits; all four warps call it.
+// A gate's exponential is the fast one, good to some 1e-6 of the result, where a 4-bit step is 1/12 of it at least: a number in some hundred
+// thousand is rounded to the other side of a border.
 // Rows c0, ... of ``rows``; row m0 of the codes and row s0 of the scales are the tile's first.  A block of 32 channels is wanted in
 // neighbouring lanes: they meet in ``inner``.
 template <int MODE>
