@@ -118,6 +118,7 @@ class Fp4Matrix:
         in inference mode: until ``written`` is said.)"""
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
+        _ = self.codes, self.scales                            # (a step's rows make theirs when they are asked for)
         version = self._version()
         self._settled = ("writes", self._writes[0]) if version is None else version
         return self

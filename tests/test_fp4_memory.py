@@ -189,3 +189,9 @@ def test_launches_keep_nothing_for_the_whole_process(source):
     import re
     with open(os.path.join(os.path.dirname(fp4_ops.__file__), source), encoding="utf-8") as fh:
         assert not re.findall(r"^\s+static (?!SsbPerDevice|const)[a-z_ ]+\w+( = [^;]*)?;", fh.read(), flags=re.M)
+
+
+def test_a_steps_rows_can_be_settled_as_any_matrix(launches):
+    z = fp4_ops.gate_up(torch.zeros((40, 64)), matrix(128, 64, gated=True))
+    assert z.settle() is z and z.codes.shape == (40, 32)
+    z.written()
