@@ -36,7 +36,7 @@ class Fp4Matrix:
         if scales.dtype != torch.uint8 or tuple(scales.shape) != (runs, 1024) or not scales.is_contiguous() or scales.device != codes.device:
             raise ValueError(f"scales must be contiguous uint8 {(runs, 1024)} beside the codes, are {scales.dtype} {tuple(scales.shape)}")
         self._codes, self._scales, self.shape, self.gated, self._buffer, self._counters = codes, scales, shape, gated, None, None
-        self._writes, self._known, self._settled = [0], None, None
+        self._writes, self._known, self._settled = [0, False], None, None
         # where they are, for the kernels: the tensors stay what they are as long as the matrix lives
         self.device, self.index, self.codes_at, self.scales_at = codes.device, codes.get_device(), codes.data_ptr(), scales.data_ptr()
         if (self.codes_at | self.scales_at) % 16:
@@ -85,8 +85,11 @@ class Fp4Matrix:
     # before the launch in front of that one ended.  So the first product on a stream behind a write is launched behind everything; the
     # stream's next ones may read ahead.  Writes are counted: this package's (``written``), torch's by the tensors' versions.
     def written(self) -> None:
-        """Said by whoever writes codes or scales other than through torch (``fp4_ops.quantize`` does)."""
+        """Said by whoever writes codes or scales other than through torch (``fp4_ops.quantize`` does), or in a capture: such a write comes
+        again with every replay, so that products outside of graphs do not read ahead from then on."""
         self._writes[0] += 1
+        if self.index >= 0 and torch.cuda.is_current_stream_capturing():
+            self._writes[1] = True
 
     def _version(self):
         try:
@@ -97,6 +100,8 @@ class Fp4Matrix:
     def reads_ahead(self, stream: int) -> bool:
         """Whether a product on this stream (its handle, the current one) may read the matrix ahead of its turn; that it is launched now
         is noted."""
+        if self._writes[1] and not torch.cuda.is_current_stream_capturing():
+            return False
         version = self._version()
         if version is None:                                    # what torch writes is not seen: only what was settled, and not written by a kernel since
             return self._settled == ("writes", self._writes[0])
@@ -142,7 +147,7 @@ class Fp4Matrix:
         """A step's rows [n, k] at the start of an int8 ``buffer``: ``codes`` bytes of codes, then scales (:meth:`rows_layout`)."""
         m = cls.__new__(cls)
         m._codes = m._scales = m._counters = None          # made when somebody asks for them
-        m._writes, m._known, m._settled = [0], None, None
+        m._writes, m._known, m._settled = [0, False], None, None
         m.shape, m.gated, m._buffer, m.device, m.index = (n, k), False, buffer, buffer.device, buffer.get_device()
         m.codes_at = buffer.data_ptr()
         m.scales_at = m.codes_at + codes

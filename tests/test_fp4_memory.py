@@ -195,3 +195,21 @@ def test_a_steps_rows_can_be_settled_as_any_matrix(launches):
     z = fp4_ops.gate_up(torch.zeros((40, 64)), matrix(128, 64, gated=True))
     assert z.settle() is z and z.codes.shape == (40, 32)
     z.written()
+
+
+def test_a_captured_write_comes_again_with_every_replay(launches, monkeypatch):
+    capturing = False
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    m = matrix(64, 64)
+    m.index = 0
+    view = m.first_rows(16)
+    assert [product(launches, m) for _ in range(2)] == [0, 1]
+    capturing = True
+    m.written()
+    assert [product(launches, m) for _ in range(2)] == [0, 1]     # in the graph
+    capturing = False
+    assert [product(launches, w) for w in (m, m, view, m.first_rows(8))] == [0, 0, 0, 0]
+    m.settle()
+    assert product(launches, m) == 0
+    capturing = True
+    assert product(launches, m) == 1

@@ -94,6 +94,35 @@ def test_products_behind_writes_of_every_kind(rows, n, k, numbers):
             check(out, want, slack)
 
 
+@pytest.mark.parametrize("rows", [2, 12, 40, 300])
+def test_products_behind_replays_that_write(rows):
+    """A graph that quantises a matrix, products of it in the graph, in another and outside of both."""
+    from supersonic_b200.csrc import fp4_ops
+    from supersonic_b200.weights import Fp4Matrix
+    g = gen(rows + 40)
+    x, source, m = randn(g, rows, 1024), torch.empty((512, 1024), device=DEV), Fp4Matrix.empty(512, 1024).settle()
+    outs, xv = [torch.empty((rows, 512), device=DEV) for _ in range(3)], pf.rounded(x.double())
+    fp4_ops.linear(x, m, outs[0])
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        fp4_ops.quantize(source, m)
+        fp4_ops.linear(x, m, outs[0])
+    with torch.cuda.graph(second):
+        fp4_ops.linear(x, m, outs[1])
+    assert not m.reads_ahead(torch.cuda.current_stream().cuda_stream)
+    for turn in range(10):
+        source.normal_(generator=g)
+        torch.cuda.synchronize()
+        first.replay()
+        if turn % 2:
+            second.replay()
+        fp4_ops.linear(x, m, outs[2])
+        second.replay()
+        wv = pf.rounded(source.double())
+        for out in outs:
+            check(out, xv @ wv.t(), pf.sum_slack(xv, wv))
+
+
 # ---- scales at the ends of their range ------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("numbers", [True, False])
 @pytest.mark.parametrize("rows, n, k", [(1, 136, 512), (8, 136, 512), (12, 136, 512), (12, 136, 4096), (30, 264, 512), (40, 264, 512), (100, 136, 512),
