@@ -268,7 +268,7 @@ static size_t fw_fixed(int rows, int k_blocks, int k_warps) {
 }
 
 template <int NB, int MODE>
-static int fw_launch(const FwArgs& a, int blocks, size_t smem, cudaStream_t stream) {
+static int fw_launch(const FwArgs& a, int blocks, size_t smem, bool early, cudaStream_t stream) {
     auto kernel = fp4_few_kernel<NB, MODE>;
     static SsbPerDevice<bool> set;
     bool* configured = set.here();
@@ -278,7 +278,7 @@ static int fw_launch(const FwArgs& a, int blocks, size_t smem, cudaStream_t stre
         if (e != cudaSuccess) return (int)e;
         *configured = true;
     }
-    return ssb_launch(kernel, dim3(blocks), dim3(FW_THREADS), smem, stream, a.early != 0, a);
+    return ssb_launch(kernel, dim3(blocks), dim3(FW_THREADS), smem, stream, early, a);
 }
 
 // How a product of M rows by N x K weights runs; slots 0: not by this kernel, which takes up to 16 rows, where it makes inner rows up to 8.
@@ -311,13 +311,13 @@ static FwPlan fw_plan(int M, int N, int K, int mode) {
 }
 bool fw_takes(int M, int N, int K, int mode) { return fw_plan(M, N, K, mode).slots > 0; }
 
-int fw_product(FwArgs a, int mode, cudaStream_t stream) {
+int fw_product(FwArgs a, int mode, bool early, cudaStream_t stream) {
     const FwPlan p = fw_plan(a.M, a.N, a.K, mode);
     if (p.slots == 0) return SSB_ERR_UNSUPPORTED;
     a.k_warps = p.k_warps;
     a.slots = p.slots;
     a.k_blocks = f4_k_blocks(a.K);
-    if (p.nb == 2) return fw_launch<2, FW_STORE>(a, p.blocks, p.smem, stream);
-    return mode == FW_STORE ? fw_launch<1, FW_STORE>(a, p.blocks, p.smem, stream)
-           : mode == FW_GATED ? fw_launch<1, FW_GATED>(a, p.blocks, p.smem, stream) : fw_launch<1, FW_ACT>(a, p.blocks, p.smem, stream);
+    if (p.nb == 2) return fw_launch<2, FW_STORE>(a, p.blocks, p.smem, early, stream);
+    return mode == FW_STORE ? fw_launch<1, FW_STORE>(a, p.blocks, p.smem, early, stream)
+           : mode == FW_GATED ? fw_launch<1, FW_GATED>(a, p.blocks, p.smem, early, stream) : fw_launch<1, FW_ACT>(a, p.blocks, p.smem, early, stream);
 }

@@ -10,9 +10,9 @@ struct FwArgs {
     void* out; uint8_t* out_scales; long long ldo; int is_f32, add;   // FW_STORE: rows of ldo elements; else codes, rows of ldo bytes, and their scales
     int M, N, K;                           // rows, rows of a weight matrix, numbers a row
     int kind; float limit; const float* row_scale; int inner_blocks;  // as FlOut's (fp4_linear.cu)
-    int early;                             // the launch may begin, and read its weights, while the one in front of it still runs
     int k_warps, slots, k_blocks;          // the plan's
 };
 
 bool fw_takes(int M, int N, int K, int mode);
-int fw_product(FwArgs a, int mode, cudaStream_t stream);
+// early: the launch may begin, and read its weights, while the one in front of it still runs.
+int fw_product(FwArgs a, int mode, bool early, cudaStream_t stream);

@@ -806,8 +806,7 @@ static int fl_product(const void* x, long long ldx, int dtype, const void* xs, c
         a.out = o.out; a.out_scales = o.scales; a.ldo = o.ldo; a.is_f32 = o.is_f32; a.add = o.add;
         a.M = o.M; a.N = o.N; a.K = K;
         a.kind = o.kind; a.limit = o.limit; a.row_scale = o.row_scale; a.inner_blocks = o.inner_blocks;
-        a.early = settled || (parts && dtype >= 0);
-        return few ? fw_product(a, MODE, stream) : fs_product(a, MODE, parts, error_word, stream);
+        return few ? fw_product(a, MODE, settled, stream) : fs_product(a, MODE, parts, settled || dtype >= 0, error_word, stream);
     }
     const FlPlan p = fl_plan(o.M, o.N, K);
     if (p.blocks > FL_COUNTERS) return SSB_ERR_UNSUPPORTED;

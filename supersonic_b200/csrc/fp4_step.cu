@@ -205,7 +205,7 @@ int fs_parts(int M, int N, int K) {
 
 template <int BN, int MODE>
 static int fs_launch(const CUtensorMap& mw, const CUtensorMap& mws, const CUtensorMap& mx, const CUtensorMap& mxs, const FwArgs& a, int parts,
-                     int* error_word, cudaStream_t stream) {
+                     bool early, int* error_word, cudaStream_t stream) {
     static_assert(fs_smem<BN>(FS_MOST_SUMS) <= 227 * 1024, "");
     auto kernel = fp4_step_kernel<BN, MODE>;
     static SsbPerDevice<bool> set;
@@ -226,19 +226,19 @@ static int fs_launch(const CUtensorMap& mw, const CUtensorMap& mws, const CUtens
     attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = a.early ? 2 : 1;
+    cfg.attrs = attr; cfg.numAttrs = early ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, kernel, mw, mws, mx, mxs, a, parts, error_word);
 }
 
 template <int BN>
 static int fs_mode(const CUtensorMap& mw, const CUtensorMap& mws, const CUtensorMap& mx, const CUtensorMap& mxs, const FwArgs& a, int mode,
-                   int parts, int* error_word, cudaStream_t stream) {
-    return mode == FL_STORE ? fs_launch<BN, FL_STORE>(mw, mws, mx, mxs, a, parts, error_word, stream)
-           : mode == FL_GATED ? fs_launch<BN, FL_GATED>(mw, mws, mx, mxs, a, parts, error_word, stream)
-                              : fs_launch<BN, FL_ACT>(mw, mws, mx, mxs, a, parts, error_word, stream);
+                   int parts, bool early, int* error_word, cudaStream_t stream) {
+    return mode == FL_STORE ? fs_launch<BN, FL_STORE>(mw, mws, mx, mxs, a, parts, early, error_word, stream)
+           : mode == FL_GATED ? fs_launch<BN, FL_GATED>(mw, mws, mx, mxs, a, parts, early, error_word, stream)
+                              : fs_launch<BN, FL_ACT>(mw, mws, mx, mxs, a, parts, early, error_word, stream);
 }
 
-int fs_product(FwArgs a, int mode, int parts, int* error_word, cudaStream_t stream) {
+int fs_product(FwArgs a, int mode, int parts, bool early, int* error_word, cudaStream_t stream) {
     a.k_blocks = f4_k_blocks(a.K);
     const int bn = a.M <= 16 ? 16 : 32;
     CUtensorMap mw, mws, mx, mxs;
@@ -247,5 +247,5 @@ int fs_product(FwArgs a, int mode, int parts, int* error_word, cudaStream_t stre
     if (!rc) rc = fl_map(&mx, a.x, a.M, a.K / 2, bn);
     if (!rc) rc = fl_scale_map(&mxs, a.xs, a.k_blocks);
     if (rc) return rc;
-    return bn == 16 ? fs_mode<16>(mw, mws, mx, mxs, a, mode, parts, error_word, stream) : fs_mode<32>(mw, mws, mx, mxs, a, mode, parts, error_word, stream);
+    return bn == 16 ? fs_mode<16>(mw, mws, mx, mxs, a, mode, parts, early, error_word, stream) : fs_mode<32>(mw, mws, mx, mxs, a, mode, parts, early, error_word, stream);
 }

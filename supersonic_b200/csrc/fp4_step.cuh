@@ -4,5 +4,5 @@
 
 // Blocks that share a tile of 128 channels, or 0: the product is not for this kernel.
 int fs_parts(int M, int N, int K);
-// What the arguments say; x: codes, with the scales xs.  mode: FL_*.
-int fs_product(FwArgs a, int mode, int parts, int* error_word, cudaStream_t stream);
+// What the arguments say; x: codes, with the scales xs.  mode: FL_*.  early: as fw_product's.
+int fs_product(FwArgs a, int mode, int parts, bool early, int* error_word, cudaStream_t stream);
