@@ -637,8 +637,8 @@ struct FlPlan {
 // At 2,048 x 2,048: 48 rows by tiles of 64 that are whole 9.1, in 2 parts 10.7; at 4,096 x 14,336: 64 rows by 64 in 2 parts 20.4, in 4 16.7,
 // dealt out over all SMs 20.8; 128 rows by 64 in 2 parts 20.7, by 128 in 4 22.2, on pairs 30; at 14,336 x 4,096: 64 rows by 64 14.0, 128
 // by 128 17.2, on pairs 15.7; 1,024 rows by 128 70, on pairs 35.  As they are taken now, rows to codes among them, weights from memory and
-// from L2: 14,336 x 4,096 64 rows 12.0 and 10.3, 128 17.2 and 14.2, 300 23.9 and 21.3, 1,024 39.5 and 39.3; 4,096 x 14,336 64 rows 16.1 and
-// 15.1, 128 20.1 and 19.8; 28,672 x 4,096 8 rows 16.7 and 14.1.  Tiles of 16 and 32 rows are only where one holds all rows: the next one's
+// from L2: 14,336 x 4,096 64 rows 12.0 and 10.3, 128 17.2 and 14.2, 300 23.9 and 21.3, 1,024 39.5 and 39.3; 4,096 x 14,336 64 rows 16.2 and
+// 15.0, 128 20.2 and 19.8; 28,672 x 4,096 8 rows 16.7 and 14.1.  Tiles of 16 and 32 rows are only where one holds all rows: the next one's
 // scales would begin between the columns that a product can name (and only where there are more tiles than SMs: else fp4_step.cu).
 static FlPlan fl_plan(int M, int N, int K) {
     const int sms = ssb_sm_count(), k_blocks = f4_k_blocks(K);

@@ -1,12 +1,12 @@
 // Products of a step's rows (up to 32, in 4 bits) in microscaled 4-bit floats on tcgen05 (the format: fp4_codes.cuh).  As in the streaming
 // kernel the weights are on the M side, 128 of them a tile; here a tile's k-blocks are shared by the blocks of a cluster, which put their
 // sums into the first one's shared memory, and it adds them up in the order of k: nothing goes through memory, and nothing counts there.
-// 8 x 4,096 x 14,336 (rows in 4 bits) 8.4 us from memory, 3.7 TB/s, 7.7 where the weights are in L2; 16 x 2,048 x 8,192 6.0 and 5.4;
-// 16 x 16,384 x 2,048 5.1 and 4.3; by the streaming kernel, with pieces in memory and counters, 12.3, 9.2 and 8.5.  A launch's start, the
+// 8 x 4,096 x 14,336 (rows in 4 bits) 8.1 us from memory, 3.8 TB/s, 7.5 where the weights are in L2; 16 x 2,048 x 8,192 5.5 and 5.0;
+// 16 x 16,384 x 2,048 4.6 and 3.9; by the streaming kernel, with pieces in memory and counters, 12.3, 9.2 and 8.5.  A launch's start, the
 // first stages and the sums' meeting are some 4 us of each.
 //
-// Rows that come as numbers are quantised by a launch in front, which the first weights come beside: 11.0 us from memory and 9.2 from L2;
-// 8.2 and 7.7; 8.3 and 6.4.  By warps of every block, a k-block at a time into its stage, it took longer: 8 x 4,096 x 14,336 15.2 us for
+// Rows that come as numbers are quantised by a launch in front, which the first weights come beside: 10.7 us from memory and 8.9 from L2;
+// 7.7 and 7.2; 7.8 and 6.0.  By warps of every block, a k-block at a time into its stage, it took longer: 8 x 4,096 x 14,336 15.2 us for
 // 11.2 from memory, 16 x 2,048 x 8,192 18.3 for 8.2.
 #include "fp4_codes.cuh"
 #include "fp4_few.cuh"
@@ -203,6 +203,8 @@ int fs_parts(int M, int N, int K) {
     return best;
 }
 
+// (``early`` is no field of FwArgs: with one int more there, the kernels that store took 91 registers for 145 and 0.3 to 0.8 us longer for their
+// ends, 32 x 2,048 x 8,192 7.2 us for 6.3.)
 template <int BN, int MODE>
 static int fs_launch(const CUtensorMap& mw, const CUtensorMap& mws, const CUtensorMap& mx, const CUtensorMap& mxs, const FwArgs& a, int parts,
                      bool early, int* error_word, cudaStream_t stream) {
